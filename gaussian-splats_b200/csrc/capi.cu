@@ -28,6 +28,18 @@ int32_t launch_project_bwd(int64_t, int32_t, const float*, const float*, const f
                            const float*, const int32_t*, const gs_params&, float*, float*, float*,
                            float*, float*, cudaStream_t);
 int32_t launch_det_math(int, int64_t, const float*, float*, cudaStream_t);
+int32_t launch_window_attention(const gs_window_attention_args&, cudaStream_t);
+int32_t launch_window_attention_backward(const gs_window_attention_args&, cudaStream_t);
+int32_t launch_window_attention_step(const gs_window_attention_step_args&, cudaStream_t);
+uint64_t window_attention_workspace_size(int64_t, int64_t);
+int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
+int32_t launch_gated_scan_backward(const gs_gated_scan_args&, cudaStream_t);
+int32_t launch_gated_scan_step(int64_t, int32_t, int32_t, const void*, int64_t, const void*,
+                               int64_t, float*, void*, cudaStream_t);
+uint64_t gated_scan_workspace_size(int64_t, int64_t);
+int32_t launch_rms_norm(const gs_rms_norm_args&, cudaStream_t);
+int32_t launch_rms_norm_backward(const gs_rms_norm_args&, cudaStream_t);
+uint64_t rms_norm_workspace_size(int64_t, int64_t);
 uint64_t bin_count_workspace_size(int64_t);
 uint64_t bin_sort_workspace_size(int64_t, int64_t, const gs_params&);
 uint64_t bin_error_word_offset();
@@ -503,6 +515,60 @@ int32_t gs_l1_loss_backward(const float* image, int64_t height, int64_t width, i
   if (height < 0 || width < 0) return GS_ERR_INVALID_ARGUMENT;
   return gs::launch_l1_bwd(image, height, width, channels, target, target_height, target_width,
                            grad_loss, grad_image, as_cuda(stream));
+}
+
+uint64_t gs_window_attention_workspace_size(const gs_window_attention_args* a) {
+  return !a || a->tokens < 0 || a->heads < 1
+             ? 0
+             : gs::window_attention_workspace_size(a->tokens, a->heads);
+}
+
+int32_t gs_window_attention(const gs_window_attention_args* args, gs_stream_t stream) {
+  return args ? gs::launch_window_attention(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_window_attention_backward(const gs_window_attention_args* args, gs_stream_t stream) {
+  return args ? gs::launch_window_attention_backward(*args, as_cuda(stream))
+              : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_window_attention_step(const gs_window_attention_step_args* args, gs_stream_t stream) {
+  return args ? gs::launch_window_attention_step(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args* a) {
+  return !a || a->num_tiles < 0 || a->channels < 1
+             ? 0
+             : gs::gated_scan_workspace_size(a->num_tiles, a->channels);
+}
+
+int32_t gs_gated_scan(const gs_gated_scan_args* args, gs_stream_t stream) {
+  return args ? gs::launch_gated_scan(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_gated_scan_backward(const gs_gated_scan_args* args, gs_stream_t stream) {
+  return args ? gs::launch_gated_scan_backward(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_gated_scan_step(int64_t batch, int32_t channels, int32_t dtype, const void* x,
+                           int64_t x_stride, const void* gate, int64_t gate_stride, float* state,
+                           void* y, gs_stream_t stream) {
+  return gs::launch_gated_scan_step(batch, channels, dtype, x, x_stride, gate, gate_stride, state,
+                                    y, as_cuda(stream));
+}
+
+uint64_t gs_rms_norm_workspace_size(const gs_rms_norm_args* a) {
+  return !a || a->rows < 0 || a->channels < 1
+             ? 0
+             : gs::rms_norm_workspace_size(a->rows, a->channels);
+}
+
+int32_t gs_rms_norm(const gs_rms_norm_args* args, gs_stream_t stream) {
+  return args ? gs::launch_rms_norm(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_rms_norm_backward(const gs_rms_norm_args* args, gs_stream_t stream) {
+  return args ? gs::launch_rms_norm_backward(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
 }
 
 int32_t gs_det_exp(int64_t n, const float* x, float* y, gs_stream_t stream) {

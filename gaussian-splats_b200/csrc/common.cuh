@@ -71,19 +71,25 @@ __device__ __forceinline__ void chain_wait() {
 // also leaves its error for cudaGetLastError, which is how the launchers read
 // it (check_launch() after each launch).
 template <class... Params, class... Args>
-inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block,
-                                  cudaStream_t stream, Args&&... args) {
+inline cudaError_t launch_chained_shared(void (*kernel)(Params...), dim3 grid, dim3 block,
+                                         size_t shared_bytes, cudaStream_t stream,
+                                         Args&&... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = block;
-  config.dynamicSmemBytes = 0;
+  config.dynamicSmemBytes = shared_bytes;
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, static_cast<Args&&>(args)...);
+}
+template <class... Params, class... Args>
+inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block,
+                                  cudaStream_t stream, Args&&... args) {
+  return launch_chained_shared(kernel, grid, block, 0, stream, static_cast<Args&&>(args)...);
 }
 
 inline unsigned ceil_div(int64_t a, int64_t b) { return static_cast<unsigned>((a + b - 1) / b); }

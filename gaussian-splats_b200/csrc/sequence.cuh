@@ -1,0 +1,90 @@
+// Shared pieces of the sequence operators (attention.cu, recurrence.cu, norm.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace gs {
+
+// Element conversions: every operator computes in float and rounds once, on
+// the store.
+template <class T>
+__device__ __forceinline__ float to_float(T x) {
+  if constexpr (std::is_same_v<T, float>) return x;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(x);
+  else return __half2float(x);
+}
+template <class T>
+__device__ __forceinline__ T from_float(float x) {
+  if constexpr (std::is_same_v<T, float>) return x;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(x);
+  else return __float2half_rn(x);
+}
+
+// N consecutive elements at an address aligned to min(16, N * sizeof(T))
+// bytes, in loads and stores of that width.
+template <class T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
+};
+template <int N, class T>
+__device__ __forceinline__ void load_pack(const T* p, float (&x)[N]) {
+  const Pack<T, N> a = *reinterpret_cast<const Pack<T, N>*>(p);
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = to_float(a.v[k]);
+}
+template <int N, class T>
+__device__ __forceinline__ void store_pack(T* p, const float (&x)[N]) {
+  Pack<T, N> a;
+#pragma unroll
+  for (int k = 0; k < N; ++k) a.v[k] = from_float<T>(x[k]);
+  *reinterpret_cast<Pack<T, N>*>(p) = a;
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+inline int element_size(int32_t dtype) { return dtype == GS_FLOAT32 ? 4 : 2; }
+inline bool is_aligned(const void* p, uintptr_t a) {
+  return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
+}
+
+// Calls f with a value of the element type that `dtype` names.
+template <class F>
+inline int32_t with_dtype(int32_t dtype, F&& f) {
+  switch (dtype) {
+    case GS_FLOAT32: return f(float{});
+    case GS_BFLOAT16: return f(__nv_bfloat16{});
+    case GS_FLOAT16: return f(__half{});
+  }
+  return GS_ERR_INVALID_ARGUMENT;
+}
+
+// One tile of a packed batch: rows [start, min(start + tile, end)) of the
+// sequence that occupies rows [begin, end). A batch of one sequence needs no
+// table: its tiles follow from the row count.
+struct Tile {
+  int32_t begin, end, start, sequence;
+};
+__device__ __forceinline__ Tile tile_at(const int32_t* table, int64_t index, int32_t rows,
+                                        int32_t tile) {
+  if (table) {
+    const int4 t = __ldg(reinterpret_cast<const int4*>(table) + index);
+    return {t.x, t.y, t.z, t.w};
+  }
+  return {0, rows, static_cast<int32_t>(index * tile), 0};
+}
+
+}  // namespace gs

@@ -66,6 +66,17 @@ EXPORTED_SYMBOLS = (
     "gs_relocate",
     "gs_relocate_status",
     "gs_relocate_workspace_size",
+    "gs_window_attention",
+    "gs_window_attention_backward",
+    "gs_window_attention_step",
+    "gs_window_attention_workspace_size",
+    "gs_gated_scan",
+    "gs_gated_scan_backward",
+    "gs_gated_scan_step",
+    "gs_gated_scan_workspace_size",
+    "gs_rms_norm",
+    "gs_rms_norm_backward",
+    "gs_rms_norm_workspace_size",
     "gs_det_exp",
     "gs_det_log",
 )
@@ -171,6 +182,62 @@ def adam_params(steps, lrs, betas, eps, noise_lr=0.0, position_lr=0.0) -> AdamPa
     return h
 
 
+SEQUENCE_TILE = 128       # GS_SEQUENCE_TILE (include/gs_b200.h)
+MAX_FIRST_TOKENS = 128    # GS_MAX_FIRST_TOKENS
+MAX_NORM_CHANNELS = 16384  # GS_MAX_NORM_CHANNELS
+
+
+def _fields(kind, names):
+    return [(name, kind) for name in names.split()]
+
+
+class WindowAttentionArgs(ctypes.Structure):
+    """``gs_window_attention_args`` (include/gs_b200.h)."""
+
+    _fields_ = (_fields(ctypes.c_int64, "tokens num_tiles") + _fields(ctypes.c_void_p, "tiles") +
+                _fields(ctypes.c_int32, "heads kv_heads dim dtype left right first") +
+                _fields(ctypes.c_float, "scale") + _fields(ctypes.c_void_p, "q k v") +
+                _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "
+                                        "v_head_stride") +
+                _fields(ctypes.c_void_p, "valid out lse grad_out grad_q grad_k grad_v workspace") +
+                _fields(ctypes.c_uint64, "workspace_size"))
+
+
+class WindowAttentionStepArgs(ctypes.Structure):
+    """``gs_window_attention_step_args``."""
+
+    _fields_ = (_fields(ctypes.c_int64, "batch") +
+                _fields(ctypes.c_int32, "heads kv_heads dim dtype slots first") +
+                _fields(ctypes.c_float, "scale") + _fields(ctypes.c_void_p, "q k v") +
+                _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "
+                                        "v_head_stride") +
+                _fields(ctypes.c_void_p, "cache_k cache_v positions out"))
+
+
+class GatedScanArgs(ctypes.Structure):
+    """``gs_gated_scan_args``."""
+
+    _fields_ = (_fields(ctypes.c_int64, "tokens sequences num_tiles") +
+                _fields(ctypes.c_void_p, "tiles tile_starts") +
+                _fields(ctypes.c_int32, "channels dtype") + _fields(ctypes.c_void_p, "x gate") +
+                _fields(ctypes.c_int64, "x_stride gate_stride") +
+                _fields(ctypes.c_void_p, "initial y last entering grad_y grad_last grad_x "
+                                         "grad_gate grad_initial workspace") +
+                _fields(ctypes.c_uint64, "workspace_size"))
+
+
+class RmsNormArgs(ctypes.Structure):
+    """``gs_rms_norm_args``."""
+
+    _fields_ = (_fields(ctypes.c_int64, "rows") +
+                _fields(ctypes.c_int32, "channels dtype residual_dtype weight_dtype") +
+                _fields(ctypes.c_float, "eps") + _fields(ctypes.c_void_p, "x residual weight") +
+                _fields(ctypes.c_int64, "x_stride residual_stride sum_stride") +
+                _fields(ctypes.c_void_p, "y sum q scale grad_y grad_sum grad_x grad_residual "
+                                         "grad_weight workspace") +
+                _fields(ctypes.c_uint64, "workspace_size"))
+
+
 VIEW_RECORD_WORDS = 29  # gs_params (17 words) + camera rotation (9) + translation (3)
 
 
@@ -259,6 +326,17 @@ def lib() -> ctypes.CDLL:
                          ctypes.c_uint64, vp], i32),
         "gs_relocate_status": ([vp, vp], i32),
         "gs_relocate_workspace_size": ([i64], ctypes.c_uint64),
+        "gs_window_attention": ([ctypes.POINTER(WindowAttentionArgs), vp], i32),
+        "gs_window_attention_backward": ([ctypes.POINTER(WindowAttentionArgs), vp], i32),
+        "gs_window_attention_step": ([ctypes.POINTER(WindowAttentionStepArgs), vp], i32),
+        "gs_window_attention_workspace_size": ([ctypes.POINTER(WindowAttentionArgs)], u64),
+        "gs_gated_scan": ([ctypes.POINTER(GatedScanArgs), vp], i32),
+        "gs_gated_scan_backward": ([ctypes.POINTER(GatedScanArgs), vp], i32),
+        "gs_gated_scan_step": ([i64, i32, i32, vp, i64, vp, i64, vp, vp, vp], i32),
+        "gs_gated_scan_workspace_size": ([ctypes.POINTER(GatedScanArgs)], u64),
+        "gs_rms_norm": ([ctypes.POINTER(RmsNormArgs), vp], i32),
+        "gs_rms_norm_backward": ([ctypes.POINTER(RmsNormArgs), vp], i32),
+        "gs_rms_norm_workspace_size": ([ctypes.POINTER(RmsNormArgs)], u64),
         "gs_det_exp": ([i64, vp, vp, vp], i32),
         "gs_det_log": ([i64, vp, vp, vp], i32),
     }

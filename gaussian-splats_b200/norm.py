@@ -1,0 +1,139 @@
+"""Root-mean-square norm of a token's channels with the residual's addition.
+
+:func:`rms_norm` adds the residual stream, norms the sum and returns both
+(differentiable); :func:`rms_norm_e4m3` does the same for serving with an 8-bit
+output, one scale a token, as the next matrix product takes it.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .sequences import address, check_cuda, current_stream, element_type
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as rows with contiguous channels: a view where it has them, else a copy."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 and t.stride(0) >= 0 else t.contiguous()
+
+
+def _check(what, x, weight, residual, eps):
+    check_cuda(what, x=x, weight=weight, residual=residual)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > native.MAX_NORM_CHANNELS:
+        raise ValueError(f"{what}: x {tuple(x.shape)} must have 1 to "
+                         f"{native.MAX_NORM_CHANNELS} channels in its last axis")
+    element_type(x.dtype, what)
+    element_type(weight.dtype, f"{what} weight")
+    if weight.shape != x.shape[-1:]:
+        raise ValueError(f"{what}: weight {tuple(weight.shape)} for {x.shape[-1]} channels")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match x "
+                             f"{tuple(x.shape)}")
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{what}: the residual must be {x.dtype} or float32, got "
+                             f"{residual.dtype}")
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"{what}: eps must be >= 0 and finite, got {eps}")
+    return eps
+
+
+def _arguments(x, weight, residual, eps, **outputs):
+    """``gs_rms_norm_args`` of rows ``x`` and ``residual``, and its codes of types."""
+    dtype = element_type(x.dtype, "")
+    return native.RmsNormArgs(
+        rows=x.shape[0], channels=x.shape[1], dtype=dtype,
+        residual_dtype=dtype if residual is None else element_type(residual.dtype, ""),
+        weight_dtype=element_type(weight.dtype, ""), eps=eps, x=address(x),
+        residual=address(residual), weight=address(weight), x_stride=x.stride(0),
+        residual_stride=0 if residual is None else residual.stride(0),
+        **{name: address(t) for name, t in outputs.items()})
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        shape = x.shape
+        rows, weight = _rows(x.detach()), weight.detach().contiguous()
+        res = None if residual is None else _rows(residual.detach())
+        y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        total = None if res is None else torch.empty(shape, dtype=res.dtype, device=x.device)
+        args = _arguments(rows, weight, res, eps, y=y, sum=total)
+        with torch.cuda.device(x.device):
+            native.check(native.lib().gs_rms_norm(ctypes.byref(args), current_stream(x.device)),
+                         "gs_rms_norm")
+        ctx.save_for_backward(rows if res is None else total, weight)
+        ctx.eps, ctx.has_residual, ctx.x_dtype, ctx.shape = eps, res is not None, x.dtype, shape
+        ctx.set_materialize_grads(False)
+        return y if res is None else (y, total)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y, grad_sum=None):
+        z, weight = ctx.saved_tensors
+        rows, shape = _rows(z), ctx.shape
+        grad_y = torch.zeros(shape, dtype=ctx.x_dtype, device=z.device) if grad_y is None \
+            else grad_y.contiguous()
+        grad_sum = None if grad_sum is None else grad_sum.contiguous()
+        grad_x = torch.empty(shape, dtype=ctx.x_dtype, device=z.device)
+        grad_residual = None
+        if ctx.has_residual and z.dtype != ctx.x_dtype:
+            grad_residual = torch.empty(shape, dtype=z.dtype, device=z.device)
+        grad_weight = torch.empty_like(weight)
+        args = native.RmsNormArgs(
+            rows=rows.shape[0], channels=rows.shape[1], dtype=element_type(ctx.x_dtype, ""),
+            residual_dtype=element_type(z.dtype, ""),
+            weight_dtype=element_type(weight.dtype, ""), eps=ctx.eps, sum=address(rows),
+            sum_stride=rows.stride(0), weight=address(weight), grad_y=address(grad_y),
+            grad_sum=address(grad_sum), grad_x=address(grad_x),
+            grad_residual=address(grad_residual), grad_weight=address(grad_weight))
+        lib = native.lib()
+        size = lib.gs_rms_norm_workspace_size(ctypes.byref(args))
+        workspace = torch.empty((size,), dtype=torch.uint8, device=z.device)
+        args.workspace, args.workspace_size = address(workspace), size
+        with torch.cuda.device(z.device):
+            native.check(lib.gs_rms_norm_backward(ctypes.byref(args), current_stream(z.device)),
+                         "gs_rms_norm_backward")
+        if ctx.has_residual and grad_residual is None:
+            grad_residual = grad_x
+        return grad_x, grad_weight, grad_residual, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+             eps: float = 1e-6):
+    """``z / sqrt(mean(z**2) + eps) * weight`` over the last axis of ``z = x +
+    residual``. Without a residual returns the norm, in the type of ``x``; with
+    one (in the type of ``x``, or float32) returns the norm and ``z`` in the
+    residual's type, the residual stream for the next layer.
+
+    float32, bfloat16 or float16, at most 16,384 channels; the sum and the norm
+    are computed in float32, and the norm is that of the unrounded sum (the
+    backward reads the sum as it was stored). Differentiable in x, weight and
+    residual, through both results; deterministic in both directions."""
+    eps = _check("rms_norm", x, weight, residual, eps)
+    return _RmsNorm.apply(x, weight, residual, eps)
+
+
+@torch.no_grad()
+def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+                  eps: float = 1e-6):
+    """:func:`rms_norm` with an 8-bit result: returns ``q`` (float8_e4m3fn, the
+    shape of ``x``) and ``scale`` (float32, one a token), with ``q * scale`` the
+    norm and ``scale = max|norm| / 448`` (1 for a token of zeros); with a
+    residual, also the sum. No gradient."""
+    eps = _check("rms_norm_e4m3", x, weight, residual, eps)
+    rows, res = _rows(x), None if residual is None else _rows(residual)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    total = None if res is None else torch.empty(x.shape, dtype=res.dtype, device=x.device)
+    weight = weight.contiguous()
+    args = _arguments(rows, weight, res, eps, q=q, scale=scale, sum=total)
+    with torch.cuda.device(x.device):
+        native.check(native.lib().gs_rms_norm(ctypes.byref(args), current_stream(x.device)),
+                     "gs_rms_norm")
+    return (q, scale) if res is None else (q, scale, total)

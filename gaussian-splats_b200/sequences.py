@@ -1,0 +1,109 @@
+"""Packed batches of sequences, as the sequence operators take them.
+
+A refiner sees a scene's Gaussians as a sequence of tokens. A batch of scenes of
+different sizes is packed: the sequences' tokens follow one another along the
+first axis of every tensor, and a :class:`PackedSequences` says where each one
+begins. It is built once a batch and handed to every operator of the step.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Sequence
+
+import torch
+
+from . import native
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_FLOAT32, ...
+
+
+class PackedSequences:
+    """The layout of a packed batch: ``lengths[b]`` tokens of sequence ``b``
+    after those of the sequences before it. Lengths are host integers, zero
+    allowed. ``offsets`` (int64, one more than sequences) and the tables that
+    the kernels read live on ``device``; they are copied there once, here."""
+
+    def __init__(self, lengths: Sequence[int], device="cuda"):
+        self.lengths = tuple(int(n) for n in lengths)
+        if not self.lengths:
+            raise ValueError("PackedSequences needs at least one sequence")
+        if min(self.lengths) < 0:
+            raise ValueError(f"sequence lengths must be >= 0, got {min(self.lengths)}")
+        self.total = sum(self.lengths)
+        if self.total >= 2 ** 31:
+            raise ValueError(f"a packed batch holds less than 2**31 tokens, got {self.total}")
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        length = torch.tensor(self.lengths, dtype=torch.int64)
+        offsets = torch.zeros(len(self.lengths) + 1, dtype=torch.int64)
+        torch.cumsum(length, 0, out=offsets[1:])
+        tile = native.SEQUENCE_TILE
+        tiles = (length + tile - 1) // tile
+        starts = torch.zeros(len(self.lengths) + 1, dtype=torch.int64)
+        torch.cumsum(tiles, 0, out=starts[1:])
+        sequence = torch.repeat_interleave(torch.arange(len(self.lengths)), tiles)
+        begin, end = offsets[sequence], offsets[sequence + 1]
+        within = torch.arange(len(sequence)) - starts[sequence]
+        table = torch.stack((begin, end, begin + tile * within, sequence), 1)
+        self.offsets = offsets.to(self.device)
+        self.tiles = table.to(torch.int32).to(self.device)
+        self.tile_starts = starts.to(torch.int32).to(self.device)
+        self.num_tiles = len(sequence)
+
+    def __len__(self) -> int:
+        return len(self.lengths)
+
+
+def check_packed(packed: PackedSequences | None, tokens: int, device: torch.device,
+                 what: str) -> None:
+    """Refuses a layout that does not describe ``tokens`` rows on ``device``."""
+    if packed is None:
+        return
+    if packed.total != tokens:
+        raise ValueError(f"{what}: the packed sequences hold {packed.total} tokens, the tensors "
+                         f"{tokens}")
+    if packed.device != device:
+        raise RuntimeError(f"{what}: packed sequences on {packed.device}, tensors on {device}")
+
+
+def tile_arguments(packed: PackedSequences | None, tokens: int) -> tuple[int, int | None]:
+    """(num_tiles, tiles) of an operator's arguments: without a layout, the
+    rows are one sequence and its tiles follow from their number."""
+    if packed is None:
+        return -(-tokens // native.SEQUENCE_TILE), None
+    return packed.num_tiles, packed.tiles.data_ptr() if packed.num_tiles else None
+
+
+def element_type(dtype: torch.dtype, what: str, allowed=(torch.float32, torch.bfloat16,
+                                                         torch.float16)) -> int:
+    """The library's code of an element type."""
+    if dtype not in allowed:
+        names = ", ".join(str(d).removeprefix("torch.") for d in allowed)
+        raise ValueError(f"{what}: {dtype} is not supported (only {names})")
+    return _DTYPES[dtype]
+
+
+def current_stream(device: torch.device) -> ctypes.c_void_p:
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def check_cuda(what: str, **tensors: torch.Tensor | None) -> torch.device:
+    """The CUDA device of the tensors; raises unless all are on the same one."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} runs on CUDA devices only (there is no CPU path); {name} "
+                               f"is on {t.device}")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the others on {device}")
+    return device

@@ -477,6 +477,144 @@ int32_t gs_l1_loss_backward(const float *image, int64_t height, int64_t width, i
                             const float *target, int64_t target_height, int64_t target_width,
                             const float *grad_loss, float *grad_image, gs_stream_t stream);
 
+/* ------------------------------------------------- operators over sequences
+ *
+ * A sequence is a run of tokens (Gaussians along a space-filling order, say); a
+ * packed batch holds the sequences one after the other along the token axis,
+ * `tokens` rows in all. A batch of more than one sequence comes with a table
+ * of its tiles of GS_SEQUENCE_TILE tokens, int32 [num_tiles, 4] (16-byte
+ * aligned): the first and the end row of the tile's sequence, the tile's first
+ * row, the sequence's number; tiles in row order, none for an empty sequence.
+ * With tiles == NULL the rows are one sequence, of ceil(tokens / tile) tiles.
+ * The table is read as given: it must describe the `tokens` rows. Strides are
+ * in elements; the last axis of every array is contiguous. */
+
+enum { GS_FLOAT32 = 0, GS_BFLOAT16 = 1, GS_FLOAT16 = 2 }; /* element types */
+enum {
+  GS_SEQUENCE_TILE = 128,      /* tokens of a tile */
+  GS_MAX_FIRST_TOKENS = 128,   /* first tokens that may stay visible */
+  GS_MAX_NORM_CHANNELS = 16384 /* channels of gs_rms_norm */
+};
+
+/* Attention in a window: query i of a sequence sees key j if valid[j] (all are
+ * where `valid` is NULL; uint8 per row), j <= i + right, and j >= i - left or
+ * j < first; softmax of scale * q.k over the keys it sees, zeros where it sees
+ * none. q [tokens, heads, dim], k, v [tokens, kv_heads, dim] (query head h uses
+ * key-value head h / (heads / kv_heads)), strides per token and head multiples
+ * of 8; out, grad_* contiguous; dtype GS_BFLOAT16 or GS_FLOAT16; dim a
+ * multiple of 8 up to 128; 0 <= first <= GS_MAX_FIRST_TOKENS. All arrays
+ * 16-byte aligned. `lse` [heads, tokens] float (may be NULL in the forward)
+ * receives each row's log-sum-exp, which the backward reads together with q, k,
+ * v, out and grad_out. The backward needs a workspace of
+ * gs_window_attention_workspace_size bytes. */
+typedef struct gs_window_attention_args {
+  int64_t tokens, num_tiles;
+  const int32_t *tiles;
+  int32_t heads, kv_heads, dim, dtype;
+  int32_t left, right, first;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+  const uint8_t *valid;
+  void *out;
+  float *lse;
+  const void *grad_out;
+  void *grad_q, *grad_k, *grad_v;
+  void *workspace;
+  uint64_t workspace_size;
+} gs_window_attention_args;
+
+uint64_t gs_window_attention_workspace_size(const gs_window_attention_args *args);
+int32_t gs_window_attention(const gs_window_attention_args *args, gs_stream_t stream);
+int32_t gs_window_attention_backward(const gs_window_attention_args *args, gs_stream_t stream);
+
+/* One new token a stream: q [batch, heads, dim], k, v [batch, kv_heads, dim],
+ * positions [batch] int64 (the token's place in its sequence, -1: an idle
+ * stream, whose output is zeros and whose cache is left alone), cache_k, cache_v
+ * [batch, slots, kv_heads, dim] contiguous. Writes k and v to their slot
+ * (position < first ? position : first + (position - first) % (slots -
+ * first)), then attends over the min(position + 1, slots) tokens that the
+ * cache holds: a window of left = slots - first - 1. */
+typedef struct gs_window_attention_step_args {
+  int64_t batch;
+  int32_t heads, kv_heads, dim, dtype, slots, first;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+  void *cache_k, *cache_v;
+  const int64_t *positions;
+  void *out;
+} gs_window_attention_step_args;
+
+int32_t gs_window_attention_step(const gs_window_attention_step_args *args, gs_stream_t stream);
+
+/* Gated linear recurrence per channel: h_t = (1 - a_t) h_{t-1} + a_t x_t with
+ * a_t = sigmoid(gate_t), h_0 = initial [sequences, channels] float (NULL:
+ * zeros). x, gate [tokens, channels] with row strides; y = h (dtype of x),
+ * last [sequences, channels] float = each sequence's final state (its initial
+ * state where it is empty). `entering` [num_tiles, channels] float receives
+ * the state that enters each tile, which the backward reads; tile_starts
+ * [sequences + 1] int32 (with `tiles`) is each sequence's first tile. The
+ * backward takes grad_y [tokens, channels] contiguous and grad_last (NULL:
+ * zeros) and writes grad_x, grad_gate and, unless NULL, grad_initial. Both
+ * need a workspace of gs_gated_scan_workspace_size bytes (8-byte aligned). */
+typedef struct gs_gated_scan_args {
+  int64_t tokens, sequences, num_tiles;
+  const int32_t *tiles, *tile_starts;
+  int32_t channels, dtype;
+  const void *x, *gate;
+  int64_t x_stride, gate_stride;
+  const float *initial;
+  void *y;
+  float *last, *entering;
+  const void *grad_y;
+  const float *grad_last;
+  void *grad_x, *grad_gate;
+  float *grad_initial;
+  void *workspace;
+  uint64_t workspace_size;
+} gs_gated_scan_args;
+
+uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args *args);
+int32_t gs_gated_scan(const gs_gated_scan_args *args, gs_stream_t stream);
+int32_t gs_gated_scan_backward(const gs_gated_scan_args *args, gs_stream_t stream);
+
+/* One step of the recurrence: state [batch, channels] float is updated in
+ * place, y [batch, channels] receives it in the type of x. */
+int32_t gs_gated_scan_step(int64_t batch, int32_t channels, int32_t dtype, const void *x,
+                           int64_t x_stride, const void *gate, int64_t gate_stride, float *state,
+                           void *y, gs_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition: z = x + residual (x
+ * alone where residual is NULL), y = z / sqrt(mean(z^2) + eps) * weight. x
+ * [rows, channels] of `dtype`, residual of `residual_dtype` (dtype or
+ * GS_FLOAT32), row strides; weight [channels]. The forward writes `sum` (z, in
+ * residual_dtype; may be NULL) and y, or, when q is not NULL, instead of y the
+ * 8-bit e4m3 codes q and scale [rows] float with z's norm = q * scale. The
+ * backward reads z from `sum` with its row stride (x itself, where there was no
+ * residual; residual_dtype is then dtype), grad_y, and grad_sum (NULL: zeros),
+ * and writes grad_x, grad_residual (unless NULL) and grad_weight; it needs a
+ * workspace of gs_rms_norm_workspace_size bytes. Outputs and gradients are
+ * contiguous. */
+typedef struct gs_rms_norm_args {
+  int64_t rows;
+  int32_t channels, dtype, residual_dtype, weight_dtype;
+  float eps;
+  const void *x, *residual, *weight;
+  int64_t x_stride, residual_stride, sum_stride;
+  void *y, *sum;
+  uint8_t *q;
+  float *scale;
+  const void *grad_y, *grad_sum;
+  void *grad_x, *grad_residual, *grad_weight;
+  void *workspace;
+  uint64_t workspace_size;
+} gs_rms_norm_args;
+
+uint64_t gs_rms_norm_workspace_size(const gs_rms_norm_args *args);
+int32_t gs_rms_norm(const gs_rms_norm_args *args, gs_stream_t stream);
+int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
+
 /* The deterministic exp / log the kernels use, applied elementwise (test hook
  * for bitwise agreement with the CPU oracle). */
 int32_t gs_det_exp(int64_t n, const float *x, float *y, gs_stream_t stream);

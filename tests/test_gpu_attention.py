@@ -1,0 +1,313 @@
+"""Windowed attention against its definition in 64 bits."""
+
+import pytest
+import torch
+
+import sequence_reference as R
+
+pytestmark = pytest.mark.gpu
+
+# Half a unit in the last place, relative: an output is rounded once, and the
+# weights of a sum (probabilities, score gradients) may be rounded once to the
+# same type before the product, so |error| <= U (|result| + spread), with a
+# quarter more for float sums and exponentials. Weights under float16's normal
+# range are off by at most 2**-25 each instead.
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+def make(lengths, heads, kv_heads, dim, dtype, seed=0, dead=0.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    tokens = sum(lengths)
+    qkv = torch.randn((tokens, (heads + 2 * kv_heads) * dim), generator=g, device="cuda").to(dtype)
+    q, k, v = (t.unflatten(1, (-1, dim)) for t in
+               qkv.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+    grad = torch.randn((tokens, heads, dim), generator=g, device="cuda").to(dtype)
+    valid = torch.rand(tokens, generator=g, device="cuda") >= dead if dead else None
+    return q, k, v, grad, valid
+
+
+def call(q, k, v, grad, lengths, **window):
+    from gaussian_splats_b200.attention import window_attention
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    packed = None if len(lengths) == 1 else PackedSequences(lengths)
+    out = window_attention(*leaves, packed, **window)
+    grads = torch.autograd.grad(out, leaves, grad)
+    return dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)))
+
+
+def check(got, ref, dtype, rows, large):
+    """``rows``: how many weights a sum may have; ``large``: the largest factor
+    that a weight meets (for the weights that fall under the normal range)."""
+    for name, t in got.items():
+        bound = 1.25 * U[dtype] * (ref[name].abs() + ref[name + "_spread"]) + 1e-5
+        bound = bound + TINY[dtype] * rows * large
+        excess = ((t.double() - ref[name]).abs() - bound).max()
+        assert torch.isfinite(t).all(), name
+        assert excess <= 0, f"{name}: {excess.item():.3g} beyond its bound"
+
+
+CASES = [
+    # lengths, heads, kv_heads, dim, left, right, first, dead
+    ([1], 1, 1, 8, 0, 0, 0, 0.0),
+    ([1], 4, 2, 64, 5, 5, 3, 0.0),
+    ([2, 0, 1, 3], 2, 1, 64, 1, 0, 1, 0.0),
+    ([128], 2, 2, 64, 127, 0, 0, 0.0),
+    ([129], 2, 1, 64, 16, 16, 4, 0.0),
+    ([257], 3, 1, 72, 300, 300, 0, 0.0),           # wider than the sequence: no window
+    ([0, 5, 0, 130, 384, 0], 4, 4, 64, 40, 0, 7, 0.0),
+    ([700], 2, 1, 128, 100, 0, 128, 0.0),          # all first tokens allowed
+    ([700], 2, 1, 96, 0, 0, 0, 0.0),               # each token sees itself
+    ([640], 8, 2, 64, 200, 200, 16, 0.1),
+    ([333, 444], 4, 1, 128, 130, 64, 4, 0.5),
+    ([500], 2, 2, 32, 64, 0, 2, 0.97),             # most keys dead: rows that see nothing
+    ([1100], 2, 1, 64, 2, 700, 1, 0.0),            # wider after than before
+    ([1500, 33], 2, 2, 128, 1000, 0, 40, 0.0),
+    ([300], 1, 1, 40, 2 ** 31 - 1, 2 ** 31 - 1, 5, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_against_the_definition(case, dtype):
+    lengths, heads, kv_heads, dim, left, right, first, dead = case
+    q, k, v, grad, valid = make(lengths, heads, kv_heads, dim, dtype, dead=dead)
+    window = dict(left=left, right=right, first=first, valid=valid)
+    got = call(q, k, v, grad, lengths, **window)
+    ref = R.attention(q, k, v, lengths, grad=grad, **window)
+    check(got, ref, dtype, max(lengths) * heads // kv_heads, 6.0)
+
+
+def test_forward_alone_gives_the_same():
+    from gaussian_splats_b200.attention import window_attention
+
+    q, k, v, grad, _ = make([700], 4, 2, 64, torch.bfloat16)
+    with torch.no_grad():
+        alone = window_attention(q, k, v, left=64, right=64, first=4)
+    assert torch.equal(alone, call(q, k, v, grad, [700], left=64, right=64, first=4)["out"])
+
+
+def test_repeats_bit_for_bit():
+    q, k, v, grad, valid = make([900, 300], 8, 2, 64, torch.bfloat16, dead=0.1)
+    a = call(q, k, v, grad, [900, 300], left=128, right=30, first=8, valid=valid)
+    b = call(q, k, v, grad, [900, 300], left=128, right=30, first=8, valid=valid)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_all_keys_dead():
+    q, k, v, grad, _ = make([200, 60], 2, 1, 64, torch.bfloat16)
+    valid = torch.ones(260, dtype=torch.bool, device="cuda")
+    valid[200:] = False
+    got = call(q, k, v, grad, [200, 60], left=30, right=30, first=2, valid=valid)
+    for t in got.values():
+        assert torch.count_nonzero(t[200:]) == 0 and torch.isfinite(t).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_dead_rows_may_hold_anything(bad):
+    """Keys, values of dead tokens; the sequences beside a sequence."""
+    lengths = [190, 300, 77]
+    q, k, v, grad, valid = make(lengths, 2, 1, 64, torch.bfloat16, dead=0.2)
+    window = dict(left=50, right=20, first=3)
+    clean = call(q, k, v, grad, lengths, valid=valid, **window)
+    k, v = k.clone(), v.clone()
+    k[~valid], v[~valid] = bad, bad
+    got = call(q, k, v, grad, lengths, valid=valid, **window)
+    for n in got:
+        assert torch.equal(got[n], clean[n]), n
+    # a whole bad sequence in the middle leaves the others as they were
+    q, grad = q.clone(), grad.clone()
+    for t in (q, k, v, grad):
+        t[190:490] = bad
+    got = call(q, k, v, grad, lengths, valid=valid, **window)
+    for n in got:
+        assert torch.equal(got[n][:190], clean[n][:190]), n
+        assert torch.equal(got[n][490:], clean[n][490:]), n
+
+
+def test_a_seen_nan_shows():
+    q, k, v, grad, _ = make([100], 1, 1, 64, torch.bfloat16)
+    k = k.clone()
+    k[:] = float("nan")
+    assert torch.isnan(call(q, k, v, grad, [100], left=5)["out"]).all()
+
+
+def test_large_scores():
+    """Scores in the thousands: the running maximum carries them."""
+    q, k, v, grad, _ = make([400], 2, 2, 64, torch.bfloat16)
+    q, k = q * 30, k * 30
+    ref = R.attention(q, k, v, [400], left=150, first=2)
+    got = call(q, k, v, grad, [400], left=150, first=2)
+    # float scores of this size are exact to 2**-23 of 5e3 or so: exp is off by 1e-3 at most
+    bound = 1.25 * (U[torch.bfloat16] + 2e-3) * (ref["out"].abs() + ref["out_spread"]) + 1e-5
+    assert ((got["out"].double() - ref["out"]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("layout", ["heads first", "odd rows", "expanded", "offset"])
+def test_strides(layout):
+    q, k, v, grad, _ = make([200], 4, 2, 64, torch.float16)
+    window = dict(left=40, right=8, first=1)
+    if layout == "expanded":
+        k, v = k[:, :1].expand(-1, 2, -1), v[:1].expand(200, -1, -1)
+    expected = call(q.contiguous(), k.contiguous(), v.contiguous(), grad, [200], **window)
+    if layout == "heads first":
+        q, k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v))
+    elif layout == "odd rows":
+        q, k, v = (torch.cat((t.flatten(1), t.flatten(1)[:, :3]), 1)[:, :-3].unflatten(1, (-1, 64))
+                   for t in (q, k, v))
+    elif layout == "offset":
+        q, k, v = (torch.cat((t.flatten()[:1], t.flatten()))[1:].view(t.shape) for t in (q, k, v))
+    grad = grad.transpose(0, 1).contiguous().transpose(0, 1)
+    got = call(q, k, v, grad, [200], **window)
+    assert all(torch.equal(got[n], expected[n]) for n in got)
+
+
+def test_gradient_against_differences():
+    q, k, v, grad, _ = make([96], 2, 1, 32, torch.float16, seed=3)
+    window = dict(left=30, right=10, first=2)
+    grads = call(q, k, v, grad, [96], **window)
+    for name, at in (("dq", 0), ("dk", 1), ("dv", 2)):
+        d = grads[name].double()
+        d = 4.0 * d / d.norm()  # about 0.06 in each element
+        sides = []
+        for sign in (1, -1):
+            inputs = [q, k, v]
+            inputs[at] = (inputs[at].double() + sign * d).half()
+            out = call(*inputs, grad, [96], **window)["out"]
+            sides.append(((out.double() * grad.double()).sum(), inputs[at].double()))
+        expected = (grads[name].double() * (sides[0][1] - sides[1][1])).sum()
+        # the third order of a step of 0.1 in a score, and the outputs' rounding
+        assert abs((sides[0][0] - sides[1][0]) / expected - 1) < 0.03
+
+
+def test_on_another_stream():
+    from gaussian_splats_b200.attention import window_attention
+
+    q, k, v, grad, _ = make([3000], 4, 2, 64, torch.bfloat16)
+    expected = call(q, k, v, grad, [3000], left=100, first=4)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = window_attention(*leaves, left=100, first=4)
+        grads = torch.autograd.grad(out, leaves, grad)
+    torch.cuda.current_stream().wait_stream(stream)
+    for t, n in zip((out, *grads), ("out", "dq", "dk", "dv")):
+        assert torch.equal(t, expected[n])
+
+
+# ------------------------------------------------------------------ one new token
+
+
+STEPS = [
+    # batch, heads, kv_heads, dim, left, first
+    (1, 1, 1, 8, 0, 0),
+    (1, 8, 2, 64, 1023, 4),
+    (3, 4, 4, 128, 30, 1),
+    (5, 6, 1, 96, 200, 16),
+    (2, 16, 1, 64, 700, 0),
+    (70, 8, 8, 32, 129, 3),
+    (2, 7, 7, 120, 5000, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", STEPS, ids=str)
+def test_step_against_the_definition(case, dtype):
+    from gaussian_splats_b200.attention import window_attention_step
+
+    batch, heads, kv_heads, dim, left, first = case
+    g = torch.Generator(device="cuda").manual_seed(1)
+    slots, rand = first + left + 1, lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    q, k, v = rand(batch, heads, dim), rand(batch, kv_heads, dim), rand(batch, kv_heads, dim)
+    cache_k, cache_v = rand(batch, slots, kv_heads, dim), rand(batch, slots, kv_heads, dim)
+    positions = torch.randint(0, 3 * slots, (batch,), generator=g, device="cuda")
+    positions[0] = slots - 1
+    if batch > 1:
+        positions[1] = -1
+    if batch > 2:
+        positions[2] = 0
+    ck, cv = cache_k.clone(), cache_v.clone()
+    for b, p in enumerate(positions.tolist()):  # what no token has filled may hold anything
+        cache_k[b, p + 1:], cache_v[b, p + 1:] = float("nan"), float("nan")
+        if p < slots:
+            ck[b, p + 1:], cv[b, p + 1:] = float("nan"), float("nan")
+    out = window_attention_step(q, k, v, cache_k, cache_v, positions, first=first)
+    for b, p in enumerate(positions.tolist()):
+        if p >= 0:
+            slot = p if p < first else first + (p - first) % (left + 1)
+            ck[b, slot], cv[b, slot] = k[b], v[b]
+            n = min(p + 1, slots)
+            kk, vv = (t[b, :n].double().repeat_interleave(heads // kv_heads, 1) for t in (ck, cv))
+            w = (torch.einsum("hd,nhd->hn", q[b].double(), kk) * dim ** -0.5).softmax(1)
+            o, spread = torch.einsum("hn,nhd->hd", w, vv), torch.einsum("hn,nhd->hd", w, vv.abs())
+            bound = 1.25 * U[dtype] * (o.abs() + spread) + 1e-5 + TINY[dtype] * n * 6.0
+            assert ((out[b].double() - o).abs() <= bound).all(), b
+        else:
+            assert torch.count_nonzero(out[b]) == 0
+    for got, expected in ((cache_k, ck), (cache_v, cv)):
+        assert torch.equal(got.view(torch.int16), expected.view(torch.int16))
+
+
+def test_steps_follow_the_whole_sequence():
+    """A stream token by token gives the rows of the whole sequence's attention."""
+    from gaussian_splats_b200.attention import (window_attention, window_attention_step,
+                                                window_cache)
+
+    q, k, v, _, _ = make([150], 4, 2, 64, torch.float16, seed=5)
+    whole = window_attention(q, k, v, left=20, first=3)
+    cache = window_cache(1, 20, 3, 2, 64, torch.float16)
+    for t in range(150):
+        out = window_attention_step(q[t:t + 1], k[t:t + 1], v[t:t + 1], *cache,
+                                    torch.tensor([t], device="cuda"), first=3)
+        torch.testing.assert_close(out[0], whole[t], rtol=2 * 2.0 ** -10, atol=2e-3)
+
+
+# ------------------------------------------------------------------------ refusals
+
+
+def test_refusals():
+    from gaussian_splats_b200.attention import window_attention, window_attention_step
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    q, k, v, _, _ = make([64], 4, 2, 64, torch.bfloat16)
+    for error, match, args, window in [
+        (RuntimeError, "CUDA devices only", (q.cpu(), k.cpu(), v.cpu()), {}),
+        (ValueError, "not a multiple of 2 key-value", (q[:, :3], k, v), {}),
+        (ValueError, "does not go with", (q, k[:10], v[:10]), {}),
+        (ValueError, "does not go with", (q, k, v[:, :1]), {}),
+        (ValueError, "different types", (q, k.half(), v), {}),
+        (ValueError, "float32 is not supported", (q.float(), k.float(), v.float()), {}),
+        (ValueError, "head dim 60", (q[..., :60], k[..., :60], v[..., :60]), {}),
+        (ValueError, r"expected \[tokens", (q[0], k[0], v[0]), {}),
+        (ValueError, "left and right", (q, k, v), {"left": -1}),
+        (ValueError, "first must be", (q, k, v), {"first": 129}),
+        (ValueError, "scale must be", (q, k, v), {"scale": 0.0}),
+        (ValueError, "valid must be", (q, k, v), {"valid": torch.ones(64, device="cuda")}),
+        (ValueError, "hold 65 tokens", (q, k, v, PackedSequences([60, 5])), {}),
+        (RuntimeError, "packed sequences on cpu", (q, k, v, PackedSequences([64], "cpu")), {}),
+    ]:
+        with pytest.raises(error, match=match):
+            window_attention(*args, **{"left": 4, **window})
+    wide = torch.zeros((8, 1, 136), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="head dim 136"):
+        window_attention(wide, wide, wide, left=1)
+    cache = torch.zeros((64, 9, 2, 64), dtype=torch.bfloat16, device="cuda")
+    at = torch.zeros(64, dtype=torch.int64, device="cuda")
+    for match, args, first in [
+        ("positions must be int64", (cache, cache.clone(), at.int()), 0),
+        ("are not", (cache, cache[:, :5], at), 0),
+        ("caches of", (cache.half(), cache.half(), at), 0),
+        ("contiguous", (cache.transpose(1, 2).contiguous().transpose(1, 2), cache, at), 0),
+        ("first must be", (cache, cache.clone(), at), 9),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            window_attention_step(q, k, v, *args, first=first)
+
+
+def test_no_tokens():
+    q, k, v, grad, _ = make([0], 2, 1, 64, torch.bfloat16)
+    assert call(q, k, v, grad, [0], left=3)["out"].shape == (0, 2, 64)
+    assert call(q, k, v, grad, [0, 0], left=3)["dk"].shape == (0, 1, 64)

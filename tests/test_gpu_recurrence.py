@@ -1,0 +1,213 @@
+"""The gated recurrence against its definition in 64 bits."""
+
+import pytest
+import torch
+
+import sequence_reference as R
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def make(lengths, channels, dtype, seed=0, bias=-2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    tokens, rand = sum(lengths), lambda *s: torch.randn(s, generator=g, device="cuda")
+    both = rand(tokens, 2 * channels)
+    both[:, channels:] += bias
+    both = both.to(dtype)
+    return dict(x=both[:, :channels], gate=both[:, channels:],
+                initial=rand(len(lengths), channels), grad=rand(tokens, channels).to(dtype),
+                grad_last=rand(len(lengths), channels))
+
+
+def call(s, lengths, initial=True):
+    from gaussian_splats_b200.recurrence import gated_scan
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    leaves = [s[n].detach().requires_grad_() for n in ("x", "gate", "initial")]
+    packed = None if len(lengths) == 1 else PackedSequences(lengths)
+    y, last = gated_scan(leaves[0], leaves[1], packed, initial=leaves[2] if initial else None)
+    grads = torch.autograd.grad((y, last), leaves if initial else leaves[:2],
+                                (s["grad"], s["grad_last"]))
+    return dict(zip(("y", "last", "dx", "dgate", "dinitial"), (y.detach(), last.detach(), *grads)))
+
+
+def check(got, ref, dtype):
+    """The states and messages are averages of what went in, so their float
+    error is a few units (gates, exponentials, folds: 2e-6 in all) of the
+    largest input that they hold, 8 here; then one rounding to the type."""
+    for name, t in got.items():
+        u = U[dtype] if t.dtype == dtype else U[torch.float32]
+        bound = 1.01 * u * ref[name].abs() + 8 * 2e-6
+        if dtype == torch.float16:
+            bound = bound + 2.0 ** -25
+        error = (t.double() - ref[name]).abs()
+        assert (error <= bound).all(), f"{name}: {(error - bound).max().item():.3g} beyond"
+
+
+CASES = [
+    ([1], 1), ([1], 64), ([2, 0, 1], 3), ([127], 33), ([128], 64), ([129], 70),
+    ([0, 300, 0, 0, 5, 128, 256, 1, 0], 40), ([1000], 256), ([3, 2500, 77], 97),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16],
+                         ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lengths,channels", CASES, ids=str)
+def test_against_the_definition(lengths, channels, dtype):
+    s = make(lengths, channels, dtype)
+    ref = R.gated_scan(s["x"], s["gate"], lengths, s["initial"], s["grad"], s["grad_last"])
+    check(call(s, lengths), ref, dtype)
+
+
+@pytest.mark.parametrize("bias", [-30.0, -9.0, 0.0, 9.0, 100.0])
+def test_gates_that_are_almost_shut_or_open(bias):
+    s = make([700], 34, torch.float32, bias=bias)
+    ref = R.gated_scan(s["x"], s["gate"], [700], s["initial"], s["grad"], s["grad_last"])
+    got = call(s, [700])
+    # shut gates: the messages add up 700 gradients, so the sums' error grows with them
+    for name, t in got.items():
+        bound = 2e-6 * (8 + 40 * ref[name].abs().max()) + 1e-5 * ref[name].abs()
+        assert ((t.double() - ref[name]).abs() <= bound).all(), name
+
+
+def test_long_sequence():
+    """The tiles' scan over many tiles, against a walk in 64 bits."""
+    lengths, channels = [70001], 8
+    s = make(lengths, channels, torch.float32)
+    h, keep, push = s["initial"][0].double().cpu(), None, None
+    gate = s["gate"].double().cpu()
+    keep, push = (-gate).sigmoid(), gate.sigmoid() * s["x"].double().cpu()
+    rows = []
+    for t in range(lengths[0]):
+        h = keep[t] * h + push[t]
+        rows.append(h)
+    got = call(s, lengths)
+    assert (got["y"].double().cpu() - torch.stack(rows)).abs().max() <= 8 * 2e-6
+
+
+def test_without_initial_state_and_partial_gradients():
+    from gaussian_splats_b200.recurrence import gated_scan
+
+    s = make([300], 20, torch.float32)
+    ref = R.gated_scan(s["x"], s["gate"], [300], None, s["grad"], s["grad_last"])
+    got = call(s, [300], initial=False)
+    check(got, {n: ref[n] for n in got}, torch.float32)
+    x = s["x"].detach().requires_grad_()
+    y, last = gated_scan(x, s["gate"])
+    alone = torch.autograd.grad(last, x, s["grad_last"], retain_graph=True)[0]
+    rest = torch.autograd.grad(y, x, s["grad"])[0]
+    torch.testing.assert_close(alone + rest, got["dx"], rtol=1e-5, atol=1e-5)
+
+
+def test_repeats_bit_for_bit_and_on_another_stream():
+    s = make([5000, 300], 130, torch.bfloat16)
+    a = call(s, [5000, 300])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        b = call(s, [5000, 300])
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_strides(dtype):
+    s = make([260], 18, dtype)
+    expected = call({n: t.contiguous() for n, t in s.items()}, [260])
+    odd = torch.randn(260, 41, device="cuda").to(dtype)
+    odd[:, 1:19], odd[:, 20:38] = s["x"], s["gate"]
+    for x, gate in ((s["x"], s["gate"]), (odd[:, 1:19], odd[:, 20:38]),
+                    (s["x"].t().contiguous().t(), s["gate"].t().contiguous().t())):
+        got = call({**s, "x": x, "gate": gate,
+                    "grad": s["grad"].t().contiguous().t()}, [260])
+        for n in got:
+            torch.testing.assert_close(got[n], expected[n], rtol=0, atol=0)
+
+
+def test_a_bad_sequence_stays_alone():
+    lengths = [150, 200, 90]
+    s = make(lengths, 36, torch.float32)
+    clean = call(s, lengths)
+    s = {n: t.clone() for n, t in s.items()}
+    s["x"][150:350], s["grad"][150:350] = float("nan"), float("inf")
+    got = call(s, lengths)
+    for n in ("y", "dx", "dgate"):
+        assert torch.equal(got[n][:150], clean[n][:150])
+        assert torch.equal(got[n][350:], clean[n][350:])
+
+
+def test_gradient_against_differences():
+    s = make([200, 61], 24, torch.float32, seed=2)
+    got = call(s, [200, 61])
+
+    def value(t):
+        r = call({**s, **t}, [200, 61])
+        return (r["y"].double() * s["grad"].double()).sum() + \
+            (r["last"].double() * s["grad_last"].double()).sum()
+
+    for name, grad in (("x", "dx"), ("gate", "dgate"), ("initial", "dinitial")):
+        d = got[grad] / got[grad].norm()
+        up, down = value({name: s[name] + 0.1 * d}), value({name: s[name] - 0.1 * d})
+        # the third order of the step, and float rounding of a few thousand outputs
+        assert abs((up - down) / 0.2 / got[grad].double().norm() - 1) < 2e-3, name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16],
+                         ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("batch,channels", [(1, 1), (1, 2069), (7, 33), (130, 512)])
+def test_step(batch, channels, dtype):
+    from gaussian_splats_b200.recurrence import gated_scan_step
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    both = torch.randn((batch, 2 * channels), generator=g, device="cuda").to(dtype)
+    state = torch.randn((batch, channels), generator=g, device="cuda")
+    x, gate, a = both[:, :channels], both[:, channels:], both[:, channels:].double().sigmoid()
+    expected = (1 - a) * state.double() + a * x.double()
+    y = gated_scan_step(x, gate, state)
+    assert (state.double() - expected).abs().max() <= 1e-5
+    assert torch.equal(y, state.to(dtype))
+
+
+def test_steps_follow_the_whole_sequence():
+    from gaussian_splats_b200.recurrence import gated_scan, gated_scan_step
+
+    s = make([140], 48, torch.float32)
+    y, last = gated_scan(s["x"], s["gate"], initial=s["initial"])
+    state = s["initial"].clone()
+    for t in range(140):
+        out = gated_scan_step(s["x"][t:t + 1], s["gate"][t:t + 1], state)
+        torch.testing.assert_close(out[0], y[t], rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(state, last, rtol=1e-5, atol=1e-5)
+
+
+def test_refusals():
+    from gaussian_splats_b200.recurrence import gated_scan, gated_scan_step
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    x = torch.zeros(10, 4, device="cuda")
+    state = torch.zeros(1, 4, device="cuda")
+    for error, match, args, more in [
+        (RuntimeError, "CUDA devices only", (x.cpu(), x.cpu()), {}),
+        (ValueError, "expected x and gate", (x, x[:5]), {}),
+        (ValueError, "expected x and gate", (x[0], x[0]), {}),
+        (ValueError, "gate is", (x, x.half()), {}),
+        (ValueError, "float64 is not supported", (x.double(), x.double()), {}),
+        (ValueError, "initial must be", (x, x), {"initial": state.half()}),
+        (ValueError, "initial must be", (x, x), {"initial": x}),
+        (ValueError, "hold 9 tokens", (x, x, PackedSequences([4, 5])), {}),
+    ]:
+        with pytest.raises(error, match=match):
+            gated_scan(*args, **more)
+    with pytest.raises(ValueError, match="contiguous float32"):
+        gated_scan_step(x, x, x.half())
+    with pytest.raises(ValueError, match="contiguous float32"):
+        gated_scan_step(x, x, torch.zeros(4, 10, device="cuda").t())
+
+
+def test_no_tokens():
+    s = make([0, 0], 6, torch.bfloat16)
+    got = call(s, [0, 0])
+    assert torch.equal(got["last"], s["initial"]) and torch.equal(got["dinitial"], s["grad_last"])
+    assert got["y"].shape == (0, 6)

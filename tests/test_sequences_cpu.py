@@ -1,0 +1,139 @@
+"""Host side of the sequence operators: layouts, refusals, argument checks, and
+the oracle's own gradients. No GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+import sequence_reference as R
+from gaussian_splats_b200.sequences import PackedSequences
+
+
+def test_packed_sequences_tables():
+    p = PackedSequences([0, 128, 300, 0, 1], device="cpu")
+    assert p.total == 429 and len(p) == 5 and p.num_tiles == 5
+    assert p.offsets.tolist() == [0, 0, 128, 428, 428, 429]
+    assert p.tile_starts.tolist() == [0, 0, 1, 4, 4, 5]
+    assert p.tiles.tolist() == [[0, 128, 0, 1], [128, 428, 128, 2], [128, 428, 256, 2],
+                                [128, 428, 384, 2], [428, 429, 428, 4]]
+    assert p.tiles.dtype == torch.int32 and p.tiles.is_contiguous()
+    assert PackedSequences([0], device="cpu").tiles.shape == (0, 4)
+
+
+@pytest.mark.parametrize("lengths", [[], [3, -1], [2 ** 30, 2 ** 30]])
+def test_packed_sequences_refuses(lengths):
+    with pytest.raises(ValueError):
+        PackedSequences(lengths, device="cpu")
+
+
+def test_no_cpu_path():
+    from gaussian_splats_b200.attention import window_attention, window_attention_step
+    from gaussian_splats_b200.norm import rms_norm, rms_norm_e4m3
+    from gaussian_splats_b200.recurrence import gated_scan, gated_scan_step
+
+    t, h = torch.zeros(4, 8), torch.zeros(4, 1, 8, dtype=torch.bfloat16)
+    for call in (lambda: window_attention(h, h, h, left=1),
+                 lambda: window_attention_step(h, h, h, h[:, None], h[:, None],
+                                               torch.zeros(4, dtype=torch.int64)),
+                 lambda: gated_scan(t, t), lambda: gated_scan_step(t, t, t),
+                 lambda: rms_norm(t, t[0]), lambda: rms_norm_e4m3(t, t[0])):
+        with pytest.raises(RuntimeError, match="CUDA devices only"):
+            call()
+
+
+def test_library_checks_arguments():
+    """Bad arguments come back as statuses before anything touches a device."""
+    from gaussian_splats_b200 import native
+
+    lib, a = native.lib(), 256  # an address that passes the alignment checks, never read
+    good = dict(tokens=300, num_tiles=3, heads=4, kv_heads=2, dim=64, dtype=1, left=3, right=0,
+                first=2, scale=0.1, q=a, k=a, v=a, q_stride=64, q_head_stride=64, k_stride=64,
+                k_head_stride=64, v_stride=64, v_head_stride=64, out=a)
+    for status, bad in [(-1, dict(heads=3)), (-1, dict(dim=12)), (-4, dict(dim=136)),
+                        (-4, dict(dtype=0)), (-1, dict(left=-1)), (-1, dict(first=129)),
+                        (-1, dict(scale=float("nan"))), (-1, dict(num_tiles=2)),
+                        (-1, dict(q=None)), (-5, dict(k=a + 2)), (-5, dict(v_stride=4)),
+                        (-5, dict(tiles=a + 4)), (-1, dict(tokens=-1))]:
+        args = native.WindowAttentionArgs(**{**good, **bad})
+        assert lib.gs_window_attention(ctypes.byref(args), None) == status, bad
+    args = native.WindowAttentionArgs(**good)
+    assert lib.gs_window_attention_backward(ctypes.byref(args), None) == -1  # no gradients
+    assert lib.gs_window_attention_workspace_size(ctypes.byref(args)) >= 4 * 4 * 300
+    step = dict(batch=1, heads=4, kv_heads=2, dim=64, dtype=1, slots=9, first=2, scale=0.1, q=a,
+                k=a, v=a, q_stride=64, q_head_stride=64, k_stride=64, k_head_stride=64,
+                v_stride=64, v_head_stride=64, cache_k=a, cache_v=a, positions=a, out=a)
+    for status, bad in [(-1, dict(slots=2)), (-1, dict(positions=None)), (-5, dict(cache_v=a + 8)),
+                        (-1, dict(batch=-1)), (-4, dict(dtype=0))]:
+        args = native.WindowAttentionStepArgs(**{**step, **bad})
+        assert lib.gs_window_attention_step(ctypes.byref(args), None) == status, bad
+    scan = dict(tokens=300, sequences=1, num_tiles=3, channels=8, dtype=0, x=a, gate=a, x_stride=8,
+                gate_stride=8, y=a, last=a, entering=a, workspace=a, workspace_size=1 << 20)
+    for status, bad in [(-1, dict(channels=0)), (-1, dict(num_tiles=4)), (-1, dict(sequences=2)),
+                        (-3, dict(workspace_size=8)), (-1, dict(x=None)), (-1, dict(dtype=5)),
+                        (-1, dict(tiles=a)), (-1, dict(last=None))]:
+        args = native.GatedScanArgs(**{**scan, **bad})
+        assert lib.gs_gated_scan(ctypes.byref(args), None) == status, bad
+    assert lib.gs_gated_scan_step(-1, 8, 0, a, 8, a, 8, a, a, None) == -1
+    assert lib.gs_gated_scan_step(1, 8, 7, a, 8, a, 8, a, a, None) == -1
+    norm = dict(rows=4, channels=8, dtype=1, residual_dtype=0, weight_dtype=1, eps=1e-6, x=a,
+                weight=a, x_stride=8, y=a)
+    for status, bad in [(-1, dict(channels=0)), (-1, dict(channels=16385)), (-1, dict(y=None)),
+                        (-1, dict(weight=None)), (-4, dict(residual_dtype=2)),
+                        (-1, dict(q=a)), (-1, dict(weight_dtype=3))]:
+        args = native.RmsNormArgs(**{**norm, **bad})
+        assert lib.gs_rms_norm(ctypes.byref(args), None) == status, bad
+    args = native.RmsNormArgs(**norm, sum=a, sum_stride=8, grad_y=a, grad_x=a, grad_weight=a,
+                              workspace=a)
+    assert lib.gs_rms_norm_backward(ctypes.byref(args), None) == -3  # workspace too small
+    for entry in (lib.gs_window_attention, lib.gs_gated_scan, lib.gs_rms_norm):
+        assert entry(None, None) == -1
+
+
+def _difference(f, t, grad, step=1e-5):
+    d = torch.randn_like(t)
+    return (f(t + step * d) - f(t - step * d)) / (2 * step), (grad * d).sum()
+
+
+def test_the_oracles_gradients_against_differences():
+    torch.manual_seed(0)
+    lengths = [9, 0, 14]
+    t = dict(q=torch.randn(23, 4, 8), k=torch.randn(23, 2, 8), v=torch.randn(23, 2, 8))
+    t = {n: x.double() for n, x in t.items()}
+    grad, valid = torch.randn(23, 4, 8).double(), torch.rand(23) > 0.3
+    window = dict(left=3, right=1, first=2, valid=valid)
+    ref = R.attention(**t, lengths=lengths, grad=grad, **window)
+    for name in t:
+        f = lambda x: (R.attention(**{**t, name: x}, lengths=lengths, **window)["out"] *  # noqa
+                       grad).sum()
+        torch.testing.assert_close(*_difference(f, t[name], ref["d" + name]), rtol=1e-6, atol=1e-8)
+    s = dict(x=torch.randn(23, 5), gate=torch.randn(23, 5), initial=torch.randn(3, 5))
+    s = {n: x.double() for n, x in s.items()}
+    g, gl = torch.randn(23, 5).double(), torch.randn(3, 5).double()
+
+    def total(r):
+        return (r["y"] * g).sum() + (r["last"] * gl).sum()
+
+    ref = R.gated_scan(**s, lengths=lengths, grad=g, grad_last=gl)
+    for name in s:
+        f = lambda x: total(R.gated_scan(**{**s, name: x}, lengths=lengths))  # noqa: E731
+        torch.testing.assert_close(*_difference(f, s[name], ref["d" + name]), rtol=1e-6, atol=1e-8)
+    x, w = torch.randn(6, 9).double(), torch.randn(9).double()
+    ref = R.rms_norm(x, w, eps=1e-3, grad=(gy := torch.randn(6, 9).double()))
+    f = lambda x, w: (R.rms_norm(x, w, eps=1e-3)["y"] * gy).sum()  # noqa: E731
+    torch.testing.assert_close(*_difference(lambda u: f(u, w), x, ref["dz"]), rtol=1e-6, atol=1e-8)
+    torch.testing.assert_close(*_difference(lambda u: f(x, u), w, ref["dw"]), rtol=1e-6, atol=1e-8)
+
+
+@pytest.mark.parametrize("plant", ["window", "first", "scale", "group"])
+def test_the_oracle_tells_wrong_windows_apart(plant):
+    """A planted mistake moves the oracle's result by far more than any bound."""
+    torch.manual_seed(1)
+    q, k, v = torch.randn(40, 4, 8), torch.randn(40, 2, 8), torch.randn(40, 2, 8)
+    right = R.attention(q, k, v, [25, 15], left=4, right=2, first=2)["out"]
+    wrong = {"window": dict(left=5, right=2, first=2), "first": dict(left=4, right=2, first=1),
+             "scale": dict(left=4, right=2, first=2, scale=0.3),
+             "group": dict(left=4, right=2, first=2)}[plant]
+    if plant == "group":
+        k, v = k.flip(1), v.flip(1)
+    assert (R.attention(q, k, v, [25, 15], **wrong)["out"] - right).abs().max() > 0.05
