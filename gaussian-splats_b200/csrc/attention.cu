@@ -17,13 +17,14 @@
 // exponentials, sums and accumulators are float. Keys that no query sees are
 // never read into a sum, so what they hold (infinities, NaN) does not matter.
 
-#include "sequence.cuh"
+#include "tensorcore.cuh"
 
 namespace gs {
 
 int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t stream);
 int32_t launch_window_attention_backward(const gs_window_attention_args& a, cudaStream_t stream);
 int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cudaStream_t stream);
+int32_t window_attention_status(cudaStream_t stream);
 uint64_t window_attention_workspace_size(int64_t tokens, int64_t heads);
 
 namespace {
@@ -89,42 +90,338 @@ struct Runs {
   }
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) attention_kernel(gs_window_attention_args a) {
-  chain_wait();
-  __shared__ float s_row[kWarps][kMaxDim];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Tile tile = tile_at(a.tiles, blockIdx.x, static_cast<int32_t>(a.tokens), kTile);
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  const T* k = static_cast<const T*>(a.k) + kv_head * a.k_head_stride;
-  const T* v = static_cast<const T*>(a.v) + kv_head * a.v_head_stride;
-  const int last = min(tile.end, tile.start + kTile);
-  for (int t = tile.start + warp; t < last; t += kWarps) {
-    __syncwarp();
-    stage_row(s_row[warp], static_cast<const T*>(a.q) + t * a.q_stride + head * a.q_head_stride,
-              a.dim, lane);
-    const Runs runs(a, t - tile.begin, tile.end - tile.begin);
-    float top = -INFINITY, sum = 0.0f, acc[kWords] = {};
-    for (int base = 0; base < runs.count(); base += 32) {
-      const bool in = base + lane < runs.count();
-      const int64_t key = tile.begin + (in ? runs.key(base + lane) : 0);
-      float s = -INFINITY;
-      if (in && (!a.valid || a.valid[key]))
-        s = dot(s_row[warp], k + key * a.k_stride, a.dim) * a.scale;
-      // Nothing seen so far: any finite shift leaves exp(-inf) = 0, and a NaN score shows.
-      const float next = fmaxf(top, warp_max(s)), shift = next == -INFINITY ? 0.0f : next;
-      const float p = expf(s - shift), shrink = expf(top - shift);
-      top = next;
-      sum = fmaf(sum, shrink, warp_sum(p));
-#pragma unroll
-      for (int c = 0; c < kWords; ++c) acc[c] *= shrink;
-      add_rows(acc, p, v, a.v_stride, key, a.dim, lane);
-    }
-    store_row(static_cast<T*>(a.out) + (int64_t{t} * a.heads + head) * a.dim, acc,
-              sum == 0.0f ? 0.0f : 1.0f / sum, a.dim, lane);
-    if (a.lse && lane == 0)
-      a.lse[head * a.tokens + t] = sum == 0.0f ? -INFINITY : top + logf(sum);
+// -------------------------------------------------- whole sequences, forward
+//
+// One block: kTile queries of one head, walked over the tiles of kKeys keys
+// that they see: first the tiles of first tokens that lie before the block's
+// window, then the window. Four warps hold a query a thread; a fifth warp's
+// first thread loads the tiles and issues the products.
+//
+//   scores  S = Q K^T            tensor memory, 128 x 64 floats
+//   P = exp2(S scale log2 e - m) each thread its row; 16 bits, over S
+//   O (+)= P V                   tensor memory, 128 x dim floats
+//
+// m is the row's running maximum, but moves only when it has grown by more
+// than 2^8: until then P stays at most 2^8, which both types hold with all
+// their precision, and O need not be rescaled.
+
+constexpr int kKeys = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
+
+// A wait ran out (never in a working kernel): set for
+// gs_window_attention_status, the block's results are not valid.
+__device__ uint32_t g_timeout;
+
+// 64 bits with those under `n` set.
+__device__ __forceinline__ uint64_t below(int64_t n) {
+  return n <= 0 ? 0 : n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
+}
+
+// The keys that a tile of queries walks over, as tiles of kKeys: positions in
+// the sequence.
+struct KeyWalk {
+  int n, low, high, head, head_tiles, tiles;
+  __device__ __forceinline__ KeyWalk(const gs_window_attention_args& a, const Tile& tile) {
+    n = tile.end - tile.begin;
+    const int64_t i = tile.start - tile.begin;
+    const int64_t last = min(i + kTile, int64_t{n}) - 1;
+    low = static_cast<int>(max(int64_t{0}, i - a.left));
+    high = static_cast<int>(min(int64_t{n}, last + a.right + 1));
+    head = min(a.first, low);
+    head_tiles = (head + kKeys - 1) / kKeys;
+    tiles = head_tiles + (high - low + kKeys - 1) / kKeys;
   }
+  __device__ __forceinline__ int start(int t) const {
+    return t < head_tiles ? t * kKeys : low + (t - head_tiles) * kKeys;
+  }
+  // Keys of tile t that may be seen at all: those under this position.
+  __device__ __forceinline__ int end(int t) const { return t < head_tiles ? head : n; }
+};
+
+// Which of the keys at `start` query i sees, were all valid and in the tile.
+__device__ __forceinline__ uint64_t window_bits(const gs_window_attention_args& a, int64_t i,
+                                                int start, int end) {
+  const int64_t high = min(i + a.right + 1, int64_t{end});
+  return below(high - start) & (~below(i - a.left - start) | below(a.first - start));
+}
+
+// The valid keys among the 64 from row `row` on (bits from `rows` on are 0);
+// every lane of the warp gets them.
+__device__ __forceinline__ uint64_t valid_bits(const uint8_t* valid, int64_t row, int rows) {
+  if (!valid) return below(rows);
+  const int lane = threadIdx.x & 31;
+  const bool low = lane < rows && __ldg(valid + row + lane);
+  const bool high = lane + 32 < rows && __ldg(valid + row + lane + 32);
+  return static_cast<uint64_t>(__ballot_sync(0xffffffffu, high)) << 32 |
+         __ballot_sync(0xffffffffu, low);
+}
+
+// Zeroes the rows of a loaded tile (kDim channels, kRows = 64 rows) whose bit
+// is not set, so that what they hold (another sequence's rows, NaN of invalid
+// keys) cannot reach a sum through a weight of zero.
+template <int kDim, int kThreadCount>
+__device__ __forceinline__ void zero_rows(unsigned char* tile, uint64_t keep, int tid) {
+  constexpr int kPerRow = kThreadCount / 64;  // threads of a row
+  constexpr int kWordsEach = 8 / kPerRow;
+  const int row = tid / kPerRow;
+  if (keep >> row & 1) return;
+#pragma unroll
+  for (int box = 0; box < kDim / 64; ++box)
+#pragma unroll
+    for (int w = 0; w < kWordsEach; ++w)
+      *reinterpret_cast<uint4*>(tile + box * 8192 + row * 128 +
+                                ((tid % kPerRow) * kWordsEach + w) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+template <int kDim>
+struct ForwardShared {
+  static constexpr int kKeyStages = 2, kValueStages = 2;
+  static constexpr int kQueryBytes = kTile * kDim * 2, kTileBytes = kKeys * kDim * 2;
+  alignas(1024) unsigned char q[kQueryBytes];
+  unsigned char k[kKeyStages][kTileBytes];
+  unsigned char v[kValueStages][kTileBytes];
+  uint64_t q_full, k_full[kKeyStages], v_full[kValueStages];  // loads
+  uint64_t scores;   // S of a tile is complete
+  uint64_t weights;  // P of a tile is written (128 arrivals)
+  uint64_t summed;   // O has a tile's sum
+  uint32_t tensor;
+};
+
+template <class T, int kDim>
+__global__ void __launch_bounds__(kTile + 32, kDim == 64 ? 4 : 2)
+    attention_kernel(gs_window_attention_args a, const __grid_constant__ CUtensorMap q_map,
+                     const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map) {
+  using namespace tc;
+  using Shared = ForwardShared<kDim>;
+  constexpr int kScoreColumn = 0, kOutColumn = kKeys;
+  constexpr int kColumns = kDim == 64 ? 128 : 256;
+  constexpr int kBoxes = kDim / 64;
+  extern __shared__ __align__(1024) unsigned char shared_bytes[];
+  Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
+  chain_wait();
+  const int warp = threadIdx.x >> 5;
+  const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+  const Tile tile =
+      tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
+  const KeyWalk walk(a, tile);
+  if (threadIdx.x == 0) {
+    barrier_init(shared_address(&s.q_full), 1);
+    for (uint64_t& b : s.k_full) barrier_init(shared_address(&b), 1);
+    for (uint64_t& b : s.v_full) barrier_init(shared_address(&b), 1);
+    barrier_init(shared_address(&s.scores), 1);
+    barrier_init(shared_address(&s.weights), kTile);
+    barrier_init(shared_address(&s.summed), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == 4) tensor_alloc<kColumns>(shared_address(&s.tensor));
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tensor = s.tensor;
+  bool good = true;
+
+  if (warp == 4) {
+    if ((threadIdx.x & 31) == 0) {
+      const auto load = [&](unsigned char* dst, uint64_t* bar, const CUtensorMap* map, int h,
+                            int row, int bytes, int box_bytes) {
+        const uint32_t b = shared_address(bar), d = shared_address(dst);
+        barrier_expect(b, bytes);
+        for (int x = 0; x < kBoxes; ++x) load_box(d + x * box_bytes, map, 64 * x, h, row, b);
+      };
+      const auto load_keys = [&](int t) {
+        load(s.k[t % Shared::kKeyStages], &s.k_full[t % Shared::kKeyStages], &k_map, kv_head,
+             tile.begin + walk.start(t), Shared::kTileBytes, kKeys * 128);
+      };
+      const auto load_values = [&](int t) {
+        load(s.v[t % Shared::kValueStages], &s.v_full[t % Shared::kValueStages], &v_map, kv_head,
+             tile.begin + walk.start(t), Shared::kTileBytes, kKeys * 128);
+      };
+      load(s.q, &s.q_full, &q_map, head, tile.start, Shared::kQueryBytes, kTile * 128);
+      for (int t = 0; t < Shared::kKeyStages && t < walk.tiles; ++t) load_keys(t);
+      for (int t = 0; t < Shared::kValueStages && t < walk.tiles; ++t) load_values(t);
+
+      const int steps = (a.dim + 15) / 16;
+      const uint32_t score_kind = product_kind<T>(kKeys, false);
+      const uint32_t sum_kind = product_kind<T>((a.dim + 15) / 16 * 16, true);
+      const uint32_t q = shared_address(s.q);
+      const auto issue_scores = [&](int t) {
+        const int stage = t % Shared::kKeyStages;
+        good = good && barrier_wait(shared_address(&s.k_full[stage]),
+                                    (t / Shared::kKeyStages) & 1);
+        const uint32_t k = shared_address(s.k[stage]);
+        for (int i = 0; i < steps; ++i)
+          multiply(tensor + kScoreColumn, along_channels<kTile>(q, i), along_channels<kKeys>(k, i),
+                   score_kind, i > 0);
+        commit(shared_address(&s.scores));
+      };
+      good = barrier_wait(shared_address(&s.q_full), 0);
+      if (good) issue_scores(0);
+      int t = 0;
+      for (; t < walk.tiles && good; ++t) {
+        good = barrier_wait(shared_address(&s.weights), t & 1);
+        if (!good) break;
+        fence_after_sync();
+        // P(t) was written from S(t): the products that read K(t) are complete.
+        if (t + Shared::kKeyStages < walk.tiles) load_keys(t + Shared::kKeyStages);
+        const int stage = t % Shared::kValueStages;
+        good = barrier_wait(shared_address(&s.v_full[stage]), (t / Shared::kValueStages) & 1);
+        const uint32_t v = shared_address(s.v[stage]);
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          multiply_tensor(tensor + kOutColumn, tensor + kScoreColumn + 8 * i,
+                          along_rows<kKeys>(v, i), sum_kind, t > 0 || i > 0);
+        commit(shared_address(&s.summed));
+        // In order behind the product that reads P(t).
+        if (t + 1 < walk.tiles) issue_scores(t + 1);
+        // S(t) was complete behind the sum of t - 1: V(t - 1) is free.
+        if (t >= 1 && t - 1 + Shared::kValueStages < walk.tiles)
+          load_values(t - 1 + Shared::kValueStages);
+      }
+      if (!good) {
+        // Let what is in flight land before the shared memory is given back.
+        for (uint64_t& b : s.k_full)
+          for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+        for (uint64_t& b : s.v_full)
+          for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+        atomicExch(&g_timeout, 1u);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int row = threadIdx.x, lane = threadIdx.x & 31;
+    const uint32_t mine = tensor + (static_cast<uint32_t>(warp * 32) << 16);
+    const int64_t i = tile.start - tile.begin + row;  // the query's position
+    const float scale = a.scale * kLog2e;
+    float top = -INFINITY, sum = 0.0f;
+    // The first and the last query of the block, for what all of them see.
+    const int64_t i_first = tile.start - tile.begin, i_last = i_first + kTile - 1;
+    for (int t = 0; t < walk.tiles; ++t) {
+      const int start = walk.start(t), end = walk.end(t);
+      const uint64_t keep =
+          valid_bits(a.valid, int64_t{tile.begin} + start, min(end - start, kKeys));
+      const bool whole = keep == ~uint64_t{0} && (t < walk.head_tiles ||
+                                                  (start + kKeys <= i_first + a.right + 1 &&
+                                                   (start >= i_last - a.left ||
+                                                    start + kKeys <= a.first)));
+      if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1))) break;
+      fence_after_sync();
+      float x[2][32];
+      load_columns32(mine + kScoreColumn, x[0]);
+      load_columns32(mine + kScoreColumn + 32, x[1]);
+      wait_loads();
+      if (!whole) {
+        const uint64_t bits = keep & window_bits(a, i, start, end);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          x[0][c] = bits >> c & 1 ? x[0][c] : -INFINITY;
+          x[1][c] = bits >> (c + 32) & 1 ? x[1][c] : -INFINITY;
+        }
+      }
+      float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        high[c & 1] = fmaxf(high[c & 1], x[0][c]);
+        high[2 + (c & 1)] = fmaxf(high[2 + (c & 1)], x[1][c]);
+      }
+      const float next =
+          fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale;
+      // Sums of earlier tiles are complete: this tile's S came behind them.
+      const bool grow = next > top + kSlack || (top == -INFINITY && next > top);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float shrink = grow ? exp2_approx(top - next) : 1.0f;
+        if (grow) top = next;
+        sum *= shrink;
+        if (t > 0) {
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 16) {
+            float o[16];
+            load_columns16(mine + kOutColumn + c, o);
+            wait_loads();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] *= shrink;
+            store_columns16(mine + kOutColumn + c, o);
+          }
+        }
+      }
+      // Where nothing is seen yet any finite shift will do: exp2(-inf) is 0.
+      const float shift = top == -INFINITY ? 0.0f : -top;
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t packed[2][16];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float p0 = exp2_approx(fmaf(x[half][2 * c], scale, shift));
+          const float p1 = exp2_approx(fmaf(x[half][2 * c + 1], scale, shift));
+          part[2 * half] += p0;
+          part[2 * half + 1] += p1;
+          packed[half][c] = pack2<T>(p0, p1);
+        }
+        store_columns16(mine + kScoreColumn + 16 * half, packed[half]);
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (keep != ~uint64_t{0}) {
+        const int stage = t % Shared::kValueStages;
+        if (!(good = barrier_wait_warp(shared_address(&s.v_full[stage]),
+                                  (t / Shared::kValueStages) & 1)))
+          break;
+        zero_rows<kDim, kTile>(s.v[stage], keep, row);
+        fence_async_shared();
+      }
+      wait_stores();
+      fence_before_sync();
+      barrier_arrive(shared_address(&s.weights));
+    }
+    if (good) good = barrier_wait_warp(shared_address(&s.summed), (walk.tiles - 1) & 1);
+    fence_after_sync();
+    const bool write = tile.start + row < tile.end;
+    const float inverse = 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + (int64_t{tile.start + row} * a.heads + head) * a.dim;
+#pragma unroll
+    for (int c = 0; c < kDim; c += 32) {
+      float o[32];
+      load_columns32(mine + kOutColumn + c, o);
+      wait_loads();
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        if (write && c + e < a.dim) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            v[k] = good ? (sum == 0.0f ? 0.0f : o[e + k] * inverse) : NAN;
+          store_pack<8>(out + c + e, v);
+        }
+    }
+    if (write && a.lse)
+      a.lse[head * a.tokens + tile.start + row] =
+          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    if (!good && lane == 0) atomicExch(&g_timeout, 1u);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 4) tensor_free<kColumns>(tensor);
+}
+
+template <class T, int kDim>
+int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  CUtensorMap q, k, v;
+  GS_TRY(tc::encode_map(&q, kBf16, a.q, a.tokens, a.heads, a.dim, a.q_stride, a.q_head_stride,
+                        kTile));
+  GS_TRY(tc::encode_map(&k, kBf16, a.k, a.tokens, a.kv_heads, a.dim, a.k_stride, a.k_head_stride,
+                        kKeys));
+  GS_TRY(tc::encode_map(&v, kBf16, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride, a.v_head_stride,
+                        kKeys));
+  constexpr size_t kShared = sizeof(ForwardShared<kDim>);
+  GS_CUDA_TRY(cudaFuncSetAttribute(attention_kernel<T, kDim>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
+                        kTile + 32, kShared, stream, a, q, k, v);
+  return check_launch();
 }
 
 // dq, and D_i into `delta` for the keys' kernel.
@@ -297,7 +594,7 @@ int32_t check_heads(int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype)
 
 int32_t check_args(const gs_window_attention_args& a) {
   GS_TRY(check_heads(a.heads, a.kv_heads, a.dim, a.dtype));
-  if (a.tokens < 0 || a.tokens > INT32_MAX || a.num_tiles < 0 || a.num_tiles > INT32_MAX ||
+  if (a.tokens < 0 || a.tokens > INT32_MAX || a.num_tiles < 0 || a.num_tiles > INT32_MAX / a.heads ||
       a.left < 0 || a.right < 0 || a.first < 0 || a.first > GS_MAX_FIRST_TOKENS ||
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
@@ -329,9 +626,19 @@ int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t 
   if (a.num_tiles == 0) return GS_OK;
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
-    launch_chained(attention_kernel<T>, dim3(a.num_tiles, a.heads), kThreads, stream, a);
-    return check_launch();
+    return a.dim <= 64 ? forward<T, 64>(a, stream) : forward<T, 128>(a, stream);
   });
+}
+
+int32_t window_attention_status(cudaStream_t stream) {
+  uint32_t timeout = 0;
+  const uint32_t clear = 0;
+  GS_CUDA_TRY(cudaMemcpyFromSymbolAsync(&timeout, g_timeout, sizeof(timeout), 0,
+                                        cudaMemcpyDeviceToHost, stream));
+  GS_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &clear, sizeof(clear), 0,
+                                      cudaMemcpyHostToDevice, stream));
+  GS_CUDA_TRY(cudaStreamSynchronize(stream));
+  return timeout ? GS_ERR_TIMEOUT : GS_OK;
 }
 
 int32_t launch_window_attention_backward(const gs_window_attention_args& a, cudaStream_t stream) {

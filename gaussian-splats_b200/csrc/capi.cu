@@ -32,6 +32,7 @@ int32_t launch_window_attention(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_backward(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_step(const gs_window_attention_step_args&, cudaStream_t);
 uint64_t window_attention_workspace_size(int64_t, int64_t);
+int32_t window_attention_status(cudaStream_t);
 int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_backward(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_step(int64_t, int32_t, int32_t, const void*, int64_t, const void*,
@@ -534,6 +535,10 @@ int32_t gs_window_attention_backward(const gs_window_attention_args* args, gs_st
 
 int32_t gs_window_attention_step(const gs_window_attention_step_args* args, gs_stream_t stream) {
   return args ? gs::launch_window_attention_step(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_window_attention_status(gs_stream_t stream) {
+  return gs::window_attention_status(as_cuda(stream));
 }
 
 uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args* a) {

@@ -1,0 +1,251 @@
+// The 5th-generation tensor cores as attention.cu uses them: tiles loaded by
+// TMA into 128-byte-swizzled shared memory, products issued by one thread
+// (tcgen05.mma, 16-bit operands, float accumulators in tensor memory), results
+// read back a row a thread.
+#pragma once
+
+#include <cuda.h>
+
+#include "sequence.cuh"
+
+namespace gs {
+namespace tc {
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// ------------------------------------------------------------------ barriers
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+
+// Waits for the barrier's phase of this parity; false if it did not complete
+// within the limit (far above any wait of a working kernel, which is at most
+// a load or a few products long).
+constexpr int kWaitLimit = 1 << 20;
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// The same for all threads of a warp together.
+__device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, barrier_wait(bar, parity));
+}
+
+// Orders this thread's plain shared-memory writes before later reads of them
+// by the tensor cores or TMA.
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// ----------------------------------------------------------------------- TMA
+
+// Loads the box at (x, head, row) of a [row, head, channel] array.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int head,
+                                         int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(bar)
+      : "memory");
+}
+
+// ------------------------------------------------------------- tensor memory
+
+// Tensor memory is addressed as lane << 16 | column, 128 lanes of 512 32-bit
+// columns; a warp reaches the 32 lanes of its place in its group of four.
+template <int kColumns>
+__device__ __forceinline__ void tensor_alloc(uint32_t shared_slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   shared_slot),
+               "n"(kColumns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int kColumns>
+__device__ __forceinline__ void tensor_free(uint32_t address) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address),
+               "n"(kColumns));
+}
+__device__ __forceinline__ void fence_before_sync() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after_sync() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// 32 columns of the warp's 32 lanes, a lane a thread. Reads are complete after
+// wait_loads, writes after wait_stores.
+__device__ __forceinline__ void load_columns32(uint32_t address, float (&x)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(address)
+      : "memory");
+}
+__device__ __forceinline__ void load_columns16(uint32_t address, float (&x)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(address)
+      : "memory");
+}
+template <class V>
+__device__ __forceinline__ void store_columns16(uint32_t address, const V (&x)[16]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(x);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(address),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void wait_stores() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// ------------------------------------------------------------------ products
+
+// Tiles lie in shared memory as TMA's 128-byte swizzle writes boxes of 64
+// channels: rows of 128 bytes, eight rows to a swizzled kilobyte, one box of
+// `rows` rows after the other along the channels. The descriptor of an operand
+// whose contraction runs along the channels (a row is a row of the product)
+// names the stride between eight-row groups; that of an operand whose
+// contraction runs along the rows names it too, and the stride between boxes.
+__device__ __forceinline__ uint64_t describe(uint32_t address, uint32_t box_bytes) {
+  return static_cast<uint64_t>((address >> 4) & 0x3FFF) |
+         static_cast<uint64_t>((box_bytes >> 4) & 0x3FFF) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t{1} << 46 | uint64_t{2} << 61;
+}
+// Step `k` of 16 along the channels of a tile of kRows rows.
+template <int kRows>
+__device__ __forceinline__ uint64_t along_channels(uint32_t tile, int k) {
+  return describe(tile + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16);
+}
+// Step `k` of 16 along the rows of a tile of kRows rows.
+template <int kRows>
+__device__ __forceinline__ uint64_t along_rows(uint32_t tile, int k) {
+  return describe(tile + k * 2048, kRows * 128);
+}
+
+// What a product of 128 rows and n columns is, for both operands of type T:
+// float accumulators; `rows_b` if B's contraction runs along its rows.
+template <class T>
+__device__ __forceinline__ uint32_t product_kind(int n, bool rows_b) {
+  const uint32_t type = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+  return 1u << 4 | type << 7 | type << 10 | (rows_b ? 1u << 16 : 0u) |
+         static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+// D (+)= A B^T with A and B in shared memory.
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind,
+                                         bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+// D (+)= A B^T with A in tensor memory (two 16-bit values a column).
+__device__ __forceinline__ void multiply_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t kind,
+                                                bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+// The barrier's phase completes when the products issued so far have.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- arithmetic
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two floats rounded to the 16-bit type T, the first in the low half.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float low, float high) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  return r;
+}
+
+// ---------------------------------------------------------------------- host
+
+// The map of a [tokens, heads, dim] array of 16-bit elements for boxes of 64
+// channels and `rows` tokens of one head. Channels from `dim` up to the box's
+// end and tokens outside the array read as zeros.
+inline int32_t encode_map(CUtensorMap* map, bool bf16, const void* base, int64_t tokens,
+                          int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride,
+                          int rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    GS_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !f) return GS_ERR_UNSUPPORTED;
+    encode = reinterpret_cast<Encode>(f);
+  }
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t stride[2] = {static_cast<cuuint64_t>(head_stride) * 2,
+                                static_cast<cuuint64_t>(token_stride) * 2};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = encode(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? GS_OK : GS_ERR_INVALID_ARGUMENT;
+}
+
+}  // namespace tc
+}  // namespace gs

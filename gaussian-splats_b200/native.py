@@ -68,6 +68,7 @@ EXPORTED_SYMBOLS = (
     "gs_relocate_workspace_size",
     "gs_window_attention",
     "gs_window_attention_backward",
+    "gs_window_attention_status",
     "gs_window_attention_step",
     "gs_window_attention_workspace_size",
     "gs_gated_scan",
@@ -328,6 +329,7 @@ def lib() -> ctypes.CDLL:
         "gs_relocate_workspace_size": ([i64], ctypes.c_uint64),
         "gs_window_attention": ([ctypes.POINTER(WindowAttentionArgs), vp], i32),
         "gs_window_attention_backward": ([ctypes.POINTER(WindowAttentionArgs), vp], i32),
+        "gs_window_attention_status": ([vp], i32),
         "gs_window_attention_step": ([ctypes.POINTER(WindowAttentionStepArgs), vp], i32),
         "gs_window_attention_workspace_size": ([ctypes.POINTER(WindowAttentionArgs)], u64),
         "gs_gated_scan": ([ctypes.POINTER(GatedScanArgs), vp], i32),

@@ -528,6 +528,11 @@ uint64_t gs_window_attention_workspace_size(const gs_window_attention_args *args
 int32_t gs_window_attention(const gs_window_attention_args *args, gs_stream_t stream);
 int32_t gs_window_attention_backward(const gs_window_attention_args *args, gs_stream_t stream);
 
+/* GS_OK, or GS_ERR_TIMEOUT if a bounded wait inside an attention kernel gave
+ * up since the last call (the block's rows then hold NaN). Synchronises
+ * `stream`. */
+int32_t gs_window_attention_status(gs_stream_t stream);
+
 /* One new token a stream: q [batch, heads, dim], k, v [batch, kv_heads, dim],
  * positions [batch] int64 (the token's place in its sequence, -1: an idle
  * stream, whose output is zeros and whose cache is left alone), cache_k, cache_v
