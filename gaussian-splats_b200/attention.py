@@ -83,9 +83,8 @@ class _WindowAttention(torch.autograd.Function):
         out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
         lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if need_grad \
             else None
-        num_tiles, tiles = tile_arguments(packed, tokens)
-        args = _arguments(native.WindowAttentionArgs, q, k, v, tokens=tokens, num_tiles=num_tiles,
-                          tiles=tiles, heads=heads, kv_heads=k.shape[1], dim=dim, dtype=dtype,
+        args = _arguments(native.WindowAttentionArgs, q, k, v, tokens=tokens,
+                          **tile_arguments(packed, tokens), heads=heads, kv_heads=k.shape[1], dim=dim, dtype=dtype,
                           left=left, right=right, first=first, scale=scale, valid=address(valid),
                           out=out.data_ptr(), lse=address(lse))
         with torch.cuda.device(q.device):

@@ -17,6 +17,8 @@
 // exponentials, sums and accumulators are float. Keys that no query sees are
 // never read into a sum, so what they hold (infinities, NaN) does not matter.
 
+#include <algorithm>
+
 #include "tensorcore.cuh"
 
 namespace gs {
@@ -25,7 +27,7 @@ int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t 
 int32_t launch_window_attention_backward(const gs_window_attention_args& a, cudaStream_t stream);
 int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cudaStream_t stream);
 int32_t window_attention_status(cudaStream_t stream);
-uint64_t window_attention_workspace_size(int64_t tokens, int64_t heads);
+uint64_t window_attention_workspace_size(const gs_window_attention_args& a);
 
 namespace {
 
@@ -46,49 +48,6 @@ __device__ __forceinline__ float dot(const float* a, const T* b, int dim) {
   }
   return s;
 }
-
-template <class T>
-__device__ __forceinline__ void stage_row(float* row, const T* p, int dim, int lane) {
-  for (int c = lane; c < dim; c += 32) row[c] = to_float(p[c]);
-  __syncwarp();
-}
-
-// acc += sum over the warp's 32 (weight, row) pairs, lanes over the channels.
-template <class T>
-__device__ __forceinline__ void add_rows(float (&acc)[kWords], float weight, const T* base,
-                                         int64_t stride, int64_t row, int dim, int lane) {
-  for (int l = 0; l < 32; ++l) {
-    const float w = __shfl_sync(0xffffffffu, weight, l);
-    const int64_t r = __shfl_sync(0xffffffffu, row, l);
-    if (w == 0.0f) continue;
-#pragma unroll
-    for (int k = 0; k < kWords; ++k)
-      if (lane + 32 * k < dim) acc[k] = fmaf(w, to_float(base[r * stride + lane + 32 * k]), acc[k]);
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void store_row(T* p, const float (&acc)[kWords], float scale, int dim,
-                                          int lane) {
-#pragma unroll
-  for (int k = 0; k < kWords; ++k)
-    if (lane + 32 * k < dim) p[lane + 32 * k] = from_float<T>(acc[k] * scale);
-}
-
-// The keys a query sees, in at most two runs: first tokens before the window,
-// and the window.
-struct Runs {
-  int low, high, head;
-  __device__ __forceinline__ Runs(const gs_window_attention_args& a, int i, int n) {
-    low = static_cast<int>(max(int64_t{0}, int64_t{i} - a.left));
-    high = static_cast<int>(min(int64_t{n}, int64_t{i} + a.right + 1));
-    head = min(a.first, low);
-  }
-  __device__ __forceinline__ int count() const { return head + high - low; }
-  __device__ __forceinline__ int key(int index) const {
-    return index < head ? index : low + index - head;
-  }
-};
 
 // -------------------------------------------------- whole sequences, forward
 //
@@ -424,90 +383,578 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
   return check_launch();
 }
 
+// ------------------------------------------------- whole sequences, backward
+//
+// Two kernels of one shape: a block holds 128 rows of two operands (queries and
+// their gradients, or keys and values) and walks over tiles of 64 rows of the
+// other two, recomputing the scores,
+//
+//   S = rows0 tile0^T,  G = rows1 tile1^T      (tensor memory, floats)
+//   P = exp2(S scale log2 e - L),  E = P (G - D)  (16 bits, over S and G)
+//   queries: dQ += E tile0;   keys: dK += E tile0, dV += P tile1
+//
+// so that every sum has one owner and one order: no atomics, and the query
+// heads that share a key-value head are summed where its keys are. Eight warps
+// split the tile's columns in halves; the ninth's first thread loads and issues.
+//
+// First tokens are seen by all later queries, so the block of their keys would
+// walk the whole sequence. It walks its window like the others; the queries
+// further on are cut into chunks with a block each, and a last kernel adds the
+// chunks' sums in order.
+
+template <int kDim>
+struct BackwardShape {
+  // At 64 channels two blocks share a multiprocessor and hide each other's
+  // waits; at 128 the operands of one fill it, and it works on two tiles at once.
+  static constexpr int kBuffers = kDim == 64 ? 1 : 2;
+  static constexpr int kStages = kDim == 64 ? 3 : 4;
+  static constexpr int kBlocks = kDim == 64 ? 2 : 1;
+  static constexpr int kRowBytes = kTile * kDim * 2, kTileBytes = kKeys * kDim * 2;
+  static constexpr int kScore = 0, kGrad = kKeys;  // columns of a buffer
+  static constexpr int kBuffer = 2 * kKeys;
+  static constexpr int kSum = kBuffers * kBuffer;  // columns of the first sum
+};
+
+template <int kDim>
+struct BackwardShared {
+  using Shape = BackwardShape<kDim>;
+  alignas(1024) unsigned char rows[2][Shape::kRowBytes];
+  unsigned char tiles[Shape::kStages][2][Shape::kTileBytes];
+  float row[2][2][kKeys];  // keys' kernel: L and D of a tile's queries
+  float half[2][kTile];    // queries' kernel: halves of D
+  uint64_t rows_full, full[Shape::kStages];  // loads
+  uint64_t scores[Shape::kBuffers];          // S and G of a tile are complete
+  uint64_t weights[Shape::kBuffers];         // P and E are written (256 arrivals)
+  uint64_t summed;                           // a tile's sums are complete
+  uint64_t done;                             // all of them are
+  uint32_t tensor;
+};
+
+constexpr int kComputeThreads = 256;
+
+// Where step k of 16 of a tile's 64 weights lies: each half of the warps writes
+// over the first of the 32 columns that it read.
+__device__ __forceinline__ uint32_t weight_column(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
+
+// The ninth warp's thread. `place(t)` names the head and row of tile t.
+template <class T, int kDim, bool kKeyRows, class Place>
+__device__ __forceinline__ bool drive(BackwardShared<kDim>& s, int dim, int tiles,
+                                      const CUtensorMap* row_map0, const CUtensorMap* row_map1,
+                                      int row_head, int row, const CUtensorMap* tile_map0,
+                                      const CUtensorMap* tile_map1, const Place& place) {
+  using namespace tc;
+  using Shape = BackwardShape<kDim>;
+  constexpr int kBuffers = Shape::kBuffers, kStages = Shape::kStages;
+  const uint32_t tensor = s.tensor;
+  const auto load_tile = [&](int t) {
+    const int stage = t % kStages;
+    const uint32_t bar = shared_address(&s.full[stage]);
+    const int2 at = place(t);
+    barrier_expect(bar, 2 * Shape::kTileBytes);
+    for (int x = 0; x < kDim / 64; ++x) {
+      load_box(shared_address(s.tiles[stage][0]) + x * kKeys * 128, tile_map0, 64 * x, at.x, at.y,
+               bar);
+      load_box(shared_address(s.tiles[stage][1]) + x * kKeys * 128, tile_map1, 64 * x, at.x, at.y,
+               bar);
+    }
+  };
+  const uint32_t rows_full = shared_address(&s.rows_full);
+  barrier_expect(rows_full, 2 * Shape::kRowBytes);
+  for (int x = 0; x < kDim / 64; ++x) {
+    load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row,
+             rows_full);
+    load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row,
+             rows_full);
+  }
+  for (int t = 0; t < kStages && t < tiles; ++t) load_tile(t);
+
+  const int steps = (dim + 15) / 16;
+  const uint32_t score_kind = product_kind<T>(kKeys, false);
+  const uint32_t sum_kind = product_kind<T>((dim + 15) / 16 * 16, true);
+  const uint32_t rows0 = shared_address(s.rows[0]), rows1 = shared_address(s.rows[1]);
+  bool good = barrier_wait(rows_full, 0);
+  const auto issue_scores = [&](int t) {
+    const int stage = t % kStages;
+    good = good && barrier_wait(shared_address(&s.full[stage]), (t / kStages) & 1);
+    const uint32_t tile0 = shared_address(s.tiles[stage][0]);
+    const uint32_t tile1 = shared_address(s.tiles[stage][1]);
+    const uint32_t d = tensor + (t % kBuffers) * Shape::kBuffer;
+    for (int i = 0; i < steps; ++i)
+      multiply(d + Shape::kScore, along_channels<kTile>(rows0, i), along_channels<kKeys>(tile0, i),
+               score_kind, i > 0);
+    for (int i = 0; i < steps; ++i)
+      multiply(d + Shape::kGrad, along_channels<kTile>(rows1, i), along_channels<kKeys>(tile1, i),
+               score_kind, i > 0);
+    commit(shared_address(&s.scores[t % kBuffers]));
+  };
+  for (int t = 0; t < kBuffers && t < tiles; ++t) issue_scores(t);
+  for (int t = 0; t < tiles && good; ++t) {
+    const int buffer = t % kBuffers, stage = t % kStages;
+    good = barrier_wait(shared_address(&s.weights[buffer]), (t / kBuffers) & 1);
+    if (!good) break;
+    fence_after_sync();
+    if (t >= 1) {  // waited for before the next phase can complete
+      good = barrier_wait(shared_address(&s.summed), (t - 1) & 1);
+      if (!good) break;
+      if (t - 1 + kStages < tiles) load_tile(t - 1 + kStages);
+    }
+    const uint32_t d = tensor + buffer * Shape::kBuffer;
+    const uint32_t tile0 = shared_address(s.tiles[stage][0]);
+    const uint32_t tile1 = shared_address(s.tiles[stage][1]);
+#pragma unroll
+    for (int i = 0; i < kKeys / 16; ++i)
+      multiply_tensor(tensor + Shape::kSum, d + Shape::kGrad + weight_column(i),
+                      along_rows<kKeys>(tile0, i), sum_kind, t > 0 || i > 0);
+    if constexpr (kKeyRows) {
+#pragma unroll
+      for (int i = 0; i < kKeys / 16; ++i)
+        multiply_tensor(tensor + Shape::kSum + kDim, d + Shape::kScore + weight_column(i),
+                        along_rows<kKeys>(tile1, i), sum_kind, t > 0 || i > 0);
+    }
+    commit(shared_address(&s.summed));
+    if (t == tiles - 1) commit(shared_address(&s.done));
+    // Behind the sums that read this buffer's weights.
+    if (t + kBuffers < tiles) issue_scores(t + kBuffers);
+  }
+  if (good) return true;
+  // Let what is in flight land before the shared memory is given back.
+  for (uint64_t& b : s.full)
+    for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+  return false;
+}
+
+template <int kDim>
+__device__ __forceinline__ void backward_setup(BackwardShared<kDim>& s, int warp) {
+  using namespace tc;
+  if (threadIdx.x == 0) {
+    barrier_init(shared_address(&s.rows_full), 1);
+    for (uint64_t& b : s.full) barrier_init(shared_address(&b), 1);
+    for (uint64_t& b : s.scores) barrier_init(shared_address(&b), 1);
+    for (uint64_t& b : s.weights) barrier_init(shared_address(&b), kComputeThreads);
+    barrier_init(shared_address(&s.summed), 1);
+    barrier_init(shared_address(&s.done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == 8) tensor_alloc<kDim == 64 ? 256 : 512>(shared_address(&s.tensor));
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+}
+
+__device__ __forceinline__ void sync_compute() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kComputeThreads) : "memory");
+}
+
+// log2 of a row's sum of exponentials, and where there is none (a row that sees
+// nothing, a row past the end) what makes its weights 0.
+__device__ __forceinline__ float weight_shift(float lse) {
+  return lse == -INFINITY ? INFINITY : lse * kLog2e;
+}
+
 // dq, and D_i into `delta` for the keys' kernel.
-template <class T>
-__global__ void __launch_bounds__(kThreads) grad_query_kernel(gs_window_attention_args a,
-                                                              float* delta) {
+template <class T, int kDim>
+__global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBlocks)
+    grad_query_kernel(gs_window_attention_args a, float* delta,
+                      const __grid_constant__ CUtensorMap q_map,
+                      const __grid_constant__ CUtensorMap g_map,
+                      const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  using namespace tc;
+  using Shape = BackwardShape<kDim>;
+  extern __shared__ __align__(1024) unsigned char shared_bytes[];
+  BackwardShared<kDim>& s = *reinterpret_cast<BackwardShared<kDim>*>(shared_bytes);
   chain_wait();
-  __shared__ float s_row[kWarps][kMaxDim], s_grad[kWarps][kMaxDim];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Tile tile = tile_at(a.tiles, blockIdx.x, static_cast<int32_t>(a.tokens), kTile);
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  const T* k = static_cast<const T*>(a.k) + kv_head * a.k_head_stride;
-  const T* v = static_cast<const T*>(a.v) + kv_head * a.v_head_stride;
-  const int last = min(tile.end, tile.start + kTile);
-  for (int t = tile.start + warp; t < last; t += kWarps) {
+  const int warp = threadIdx.x >> 5;
+  const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+  const Tile tile =
+      tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
+  const KeyWalk walk(a, tile);
+  backward_setup(s, warp);
+  const uint32_t tensor = s.tensor;
+  if (warp == 8) {
+    if ((threadIdx.x & 31) == 0 &&
+        !drive<T, kDim, false>(s, a.dim, walk.tiles, &q_map, &g_map, head, tile.start, &k_map,
+                               &v_map, [&](int t) {
+                                 return make_int2(kv_head, tile.begin + walk.start(t));
+                               }))
+      atomicExch(&g_timeout, 1u);
     __syncwarp();
-    const int64_t at = (int64_t{t} * a.heads + head) * a.dim;
-    stage_row(s_row[warp], static_cast<const T*>(a.q) + t * a.q_stride + head * a.q_head_stride,
-              a.dim, lane);
-    stage_row(s_grad[warp], static_cast<const T*>(a.grad_out) + at, a.dim, lane);
-    const T* out = static_cast<const T*>(a.out) + at;
+  } else {
+    const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
+    const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int64_t i_first = tile.start - tile.begin, i = i_first + row;
+    const bool live = tile.start + row < tile.end;
+    const int64_t at = (int64_t{tile.start + row} * a.heads + head) * a.dim;
     float d = 0.0f;
-    for (int c = lane; c < a.dim; c += 32) d = fmaf(s_grad[warp][c], to_float(out[c]), d);
-    d = warp_sum(d);
-    const float lse = a.lse[head * a.tokens + t];
-    if (lane == 0) delta[head * a.tokens + t] = d;
-    const Runs runs(a, t - tile.begin, tile.end - tile.begin);
-    float acc[kWords] = {};
-    if (lse != -INFINITY)
-      for (int base = 0; base < runs.count(); base += 32) {
-        const bool in = base + lane < runs.count();
-        const int64_t key = tile.begin + (in ? runs.key(base + lane) : 0);
-        float e = 0.0f;
-        if (in && (!a.valid || a.valid[key])) {
-          const float p = expf(fmaf(dot(s_row[warp], k + key * a.k_stride, a.dim), a.scale, -lse));
-          e = p * (dot(s_grad[warp], v + key * a.v_stride, a.dim) - d);
-        }
-        add_rows(acc, e, k, a.k_stride, key, a.dim, lane);
+    if (live)
+      for (int c = 8 * half; c < a.dim; c += 16) {
+        float g[8], o[8];
+        load_pack<8>(static_cast<const T*>(a.grad_out) + at + c, g);
+        load_pack<8>(static_cast<const T*>(a.out) + at + c, o);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d = fmaf(g[k], o[k], d);
       }
-    store_row(static_cast<T*>(a.grad_q) + at, acc, a.scale, a.dim, lane);
+    s.half[half][row] = d;
+    sync_compute();
+    d = s.half[0][row] + s.half[1][row];
+    const int64_t slot = head * a.tokens + tile.start + row;
+    if (live && half == 0) delta[slot] = d;
+    const float shift = live ? weight_shift(a.lse[slot]) : INFINITY;
+    const float scale = a.scale * kLog2e;
+    bool good = true;
+    for (int t = 0; t < walk.tiles; ++t) {
+      const int start = walk.start(t), end = walk.end(t);
+      const uint64_t keep =
+          valid_bits(a.valid, int64_t{tile.begin} + start, min(end - start, kKeys));
+      const bool whole = keep == ~uint64_t{0} &&
+                         (t < walk.head_tiles ||
+                          (start + kKeys <= i_first + a.right + 1 &&
+                           (start >= i_first + kTile - 1 - a.left || start + kKeys <= a.first)));
+      const uint32_t bits = static_cast<uint32_t>(
+          (keep & window_bits(a, i, start, end)) >> (32 * half));
+      const int buffer = t % Shape::kBuffers;
+      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), (t / Shape::kBuffers) & 1)))
+        break;
+      fence_after_sync();
+      const uint32_t from = mine + buffer * Shape::kBuffer + 32 * half;
+      float x[32], g[32];
+      load_columns32(from + Shape::kScore, x);
+      load_columns32(from + Shape::kGrad, g);
+      wait_loads();
+      uint32_t packed[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float e[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float p = exp2_approx(fmaf(x[2 * c + k], scale, -shift));
+          e[k] = p * (g[2 * c + k] - d);
+          if (!whole && !(bits >> (2 * c + k) & 1)) e[k] = 0.0f;
+        }
+        packed[c] = pack2<T>(e[0], e[1]);
+      }
+      store_columns16(from + Shape::kGrad, packed);
+      if (keep != ~uint64_t{0}) {
+        const int stage = t % Shape::kStages;
+        if (!(good = barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1)))
+          break;
+        zero_rows<kDim, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
+        fence_async_shared();
+      }
+      wait_stores();
+      fence_before_sync();
+      barrier_arrive(shared_address(&s.weights[buffer]));
+    }
+    if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
+    fence_after_sync();
+    T* grad_q = static_cast<T*>(a.grad_q) + at;
+#pragma unroll
+    for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
+      float o[32];
+      load_columns32(mine + Shape::kSum + c, o);
+      wait_loads();
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        if (live && c + e < a.dim) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * a.scale : NAN;
+          store_pack<8>(grad_q + c + e, v);
+        }
+    }
+    if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+}
+
+// The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
+// dim] over their own windows, `part` [slot, ...] over the chunks of `tiles`
+// tiles of later queries. Sequence b's chunks take the slots from
+// floor(first tile of b / tiles) + b on, which no two sequences share.
+struct FirstSums {
+  float* base;
+  float* part;
+  int tiles, slots;
+  __device__ __forceinline__ int64_t slot_of(int64_t first_tile, int64_t sequence) const {
+    return first_tile / tiles + sequence;
+  }
+};
+__device__ __forceinline__ int64_t first_tile_of(const gs_window_attention_args& a, int64_t b) {
+  return a.tile_starts ? __ldg(a.tile_starts + b) : (b ? a.num_tiles : 0);
+}
+// Whether some query of a sequence of n sees first tokens before its window.
+__device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a, int n) {
+  return a.first > 0 && n > int64_t{a.left} + 1;
+}
+
+// dk and dv.
+template <class T, int kDim>
+__global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBlocks)
+    grad_key_kernel(gs_window_attention_args a, const float* delta, FirstSums sums,
+                    const __grid_constant__ CUtensorMap k_map,
+                    const __grid_constant__ CUtensorMap v_map,
+                    const __grid_constant__ CUtensorMap q_map,
+                    const __grid_constant__ CUtensorMap g_map) {
+  using namespace tc;
+  using Shape = BackwardShape<kDim>;
+  extern __shared__ __align__(1024) unsigned char shared_bytes[];
+  BackwardShared<kDim>& s = *reinterpret_cast<BackwardShared<kDim>*>(shared_bytes);
+  chain_wait();
+  const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
+  const int kv_head = blockIdx.x % a.kv_heads;
+  const int64_t item = blockIdx.x / a.kv_heads;
+  const bool chunk = item < sums.slots;  // the long items come first
+  Tile tile;
+  int64_t low, high;  // queries, as positions
+  if (chunk) {
+    int64_t b = 0, above = a.tile_starts ? a.sequences : 1;
+    while (above - b > 1) {  // the last sequence whose slots start at or before this one
+      const int64_t middle = (b + above) / 2;
+      if (sums.slot_of(first_tile_of(a, middle), middle) <= item) b = middle;
+      else above = middle;
+    }
+    const int64_t tile0 = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
+    const int64_t index = (item - sums.slot_of(tile0, b)) * sums.tiles;
+    if (index >= tiles) return;
+    tile = tile_at(a.tiles, tile0, static_cast<int32_t>(a.tokens), kTile);
+    const int64_t n = tile.end - tile.begin;
+    low = max(index * kTile, int64_t{a.left} + 1);
+    high = min((index + sums.tiles) * kTile, n);
+    if (low >= high) return;
+  } else {
+    tile = tile_at(a.tiles, item - sums.slots, static_cast<int32_t>(a.tokens), kTile);
+    const int64_t n = tile.end - tile.begin, j = tile.start - tile.begin;
+    low = max(int64_t{0}, j - a.right);
+    high = min(n, min(j + kTile, n) + a.left);
+  }
+  const int n = tile.end - tile.begin;
+  const int per_head = static_cast<int>((high - low + kKeys - 1) / kKeys);
+  const int tiles = per_head * group;
+  backward_setup(s, warp);
+  const uint32_t tensor = s.tensor;
+  if (warp == 8) {
+    if ((threadIdx.x & 31) == 0 &&
+        !drive<T, kDim, true>(s, a.dim, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
+                              [&](int t) {
+                                return make_int2(kv_head * group + t / per_head,
+                                                 tile.begin + static_cast<int>(low) +
+                                                     (t % per_head) * kKeys);
+                              }))
+      atomicExch(&g_timeout, 1u);
+    __syncwarp();
+  } else {
+    const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
+    const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int64_t j_first = tile.start - tile.begin, j = j_first + row;
+    const bool live = j < n && (!chunk || j < a.first);
+    const bool seen = live && (!a.valid || a.valid[tile.start + row]);
+    const bool any_seen = __any_sync(0xffffffffu, seen), all_seen = __all_sync(0xffffffffu, seen);
+    const float scale = a.scale * kLog2e;
+    // L and D of tile t's queries, 64 of each, a tile ahead.
+    const auto row_value = [&](int t) {
+      const int c = threadIdx.x & (kKeys - 1);
+      const int64_t i = low + (t % per_head) * kKeys + c;
+      const bool in = threadIdx.x < 2 * kKeys && t < tiles && i < n;
+      const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
+      if (threadIdx.x < kKeys) return in ? weight_shift(a.lse[at]) : INFINITY;
+      return in ? delta[at] : 0.0f;
+    };
+    if (threadIdx.x < 2 * kKeys) s.row[0][threadIdx.x / kKeys][threadIdx.x % kKeys] = row_value(0);
+    sync_compute();
+    bool good = true;
+    for (int t = 0; t < tiles; ++t) {
+      const float ahead = row_value(t + 1);
+      const int64_t start = low + (t % per_head) * kKeys;
+      uint64_t wide = seen ? below(high - start) : 0;
+      if (chunk) wide &= ~below(j + a.left + 1 - start);
+      else wide &= below(j + a.left + 1 - start) & ~below(j - a.right - start);
+      const uint32_t bits = static_cast<uint32_t>(wide >> (32 * half));
+      const bool whole = __all_sync(0xffffffffu, bits == ~0u);
+      const int buffer = t % Shape::kBuffers;
+      // After a wait that ran out the walk goes on without waiting, for the
+      // barriers that all warps meet at.
+      good = good &&
+             barrier_wait_warp(shared_address(&s.scores[buffer]), (t / Shape::kBuffers) & 1);
+      fence_after_sync();
+      const uint32_t from = mine + buffer * Shape::kBuffer + 32 * half;
+      uint32_t weight[16], packed[16];
+      if (any_seen) {
+        float x[32], g[32];
+        load_columns32(from + Shape::kScore, x);
+        load_columns32(from + Shape::kGrad, g);
+        wait_loads();
+        const float4* shifts = reinterpret_cast<const float4*>(s.row[t & 1][0] + 32 * half);
+        const float4* deltas = reinterpret_cast<const float4*>(s.row[t & 1][1] + 32 * half);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float4 l4 = shifts[c], d4 = deltas[c];
+          const float l[4] = {l4.x, l4.y, l4.z, l4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
+          float p[4], e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            p[k] = exp2_approx(fmaf(x[4 * c + k], scale, -l[k]));
+            e[k] = p[k] * (g[4 * c + k] - d[k]);
+            if (!whole && !(bits >> (4 * c + k) & 1)) p[k] = e[k] = 0.0f;
+          }
+          weight[2 * c] = pack2<T>(p[0], p[1]);
+          weight[2 * c + 1] = pack2<T>(p[2], p[3]);
+          packed[2 * c] = pack2<T>(e[0], e[1]);
+          packed[2 * c + 1] = pack2<T>(e[2], e[3]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) weight[c] = packed[c] = 0;
+      }
+      store_columns16(from + Shape::kScore, weight);
+      store_columns16(from + Shape::kGrad, packed);
+      if (start + kKeys > n) {
+        const int stage = t % Shape::kStages;
+        good =
+            good && barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1);
+        zero_rows<kDim, kComputeThreads>(s.tiles[stage][0], below(n - start), threadIdx.x);
+        zero_rows<kDim, kComputeThreads>(s.tiles[stage][1], below(n - start), threadIdx.x);
+        fence_async_shared();
+      }
+      if (threadIdx.x < 2 * kKeys)
+        s.row[(t + 1) & 1][threadIdx.x / kKeys][threadIdx.x % kKeys] = ahead;
+      wait_stores();
+      fence_before_sync();
+      barrier_arrive(shared_address(&s.weights[buffer]));
+      sync_compute();  // the next tile's L and D are there
+    }
+    if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
+    fence_after_sync();
+    // First tokens that later queries see too: floats for the sum of the chunks.
+    const bool split = j < a.first && beyond_window(a, n);
+    const int64_t where = chunk ? item : tile.sequence;
+    float* sum = (chunk ? sums.part : sums.base) +
+                 ((where * a.kv_heads + kv_head) * a.first + j) * 2 * a.dim;
+    const int64_t at = (int64_t{tile.start + row} * a.kv_heads + kv_head) * a.dim;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
+        float o[32];
+        load_columns32(mine + Shape::kSum + which * kDim + c, o);
+        wait_loads();
+        const float factor = which ? 1.0f : a.scale;
+        T* out = static_cast<T*>(which ? a.grad_v : a.grad_k) + at;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+          if (live && c + e < a.dim) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * factor : NAN;
+            if (split) store_pack<8>(sum + which * a.dim + c + e, v);
+            else store_pack<8>(out + c + e, v);
+          }
+      }
+    if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 8) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+}
+
+// dk and dv of first tokens: their window's sum and the chunks' in order, a
+// block a token and key-value head; the chunks are shared out to kParts rows of
+// threads, whose sums are added in order.
+constexpr int kParts = 4;
+template <class T>
+__global__ void __launch_bounds__(2 * kMaxDim * kParts) first_sum_kernel(
+    gs_window_attention_args a, FirstSums sums) {
+  chain_wait();
+  __shared__ float s_part[kParts][2 * kMaxDim];
+  const int j = blockIdx.x % a.first;
+  const int kv_head = blockIdx.x / a.first % a.kv_heads;
+  const int64_t b = blockIdx.x / (int64_t{a.first} * a.kv_heads);
+  const int64_t tile0 = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
+  if (tiles == 0) return;
+  const Tile tile = tile_at(a.tiles, tile0, static_cast<int32_t>(a.tokens), kTile);
+  const int64_t n = tile.end - tile.begin;
+  if (j >= n || !beyond_window(a, static_cast<int>(n))) return;
+  const int c = threadIdx.x % (2 * kMaxDim), part = threadIdx.x / (2 * kMaxDim);
+  const int64_t row = (int64_t{kv_head} * a.first + j) * 2 * a.dim + c;
+  const int64_t stride = int64_t{a.kv_heads} * a.first * 2 * a.dim;
+  const int64_t slot = sums.slot_of(tile0, b);
+  const int64_t length = int64_t{sums.tiles} * kTile;
+  const int64_t from = (int64_t{a.left} + 1) / length, to = (n + length - 1) / length;
+  float sum = 0.0f;
+  if (c < 2 * a.dim) {
+    if (part == 0) sum = sums.base[b * stride + row];
+#pragma unroll 8
+    for (int64_t k = from + part; k < to; k += kParts) sum += sums.part[(slot + k) * stride + row];
+  }
+  s_part[part][c] = sum;
+  __syncthreads();
+  if (part == 0 && c < 2 * a.dim) {
+    for (int p = 1; p < kParts; ++p) sum += s_part[p][c];
+    const int64_t at = (int64_t{tile.begin + j} * a.kv_heads + kv_head) * a.dim;
+    if (c < a.dim) static_cast<T*>(a.grad_k)[at + c] = from_float<T>(sum);
+    else static_cast<T*>(a.grad_v)[at + c - a.dim] = from_float<T>(sum);
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) grad_key_kernel(gs_window_attention_args a,
-                                                            const float* delta) {
-  chain_wait();
-  __shared__ float s_key[kWarps][kMaxDim], s_value[kWarps][kMaxDim];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Tile tile = tile_at(a.tiles, blockIdx.x, static_cast<int32_t>(a.tokens), kTile);
-  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
-  const int last = min(tile.end, tile.start + kTile), n = tile.end - tile.begin;
-  for (int t = tile.start + warp; t < last; t += kWarps) {
-    __syncwarp();
-    float dk[kWords] = {}, dv[kWords] = {};
-    if (!a.valid || a.valid[t]) {
-      stage_row(s_key[warp], static_cast<const T*>(a.k) + t * a.k_stride + kv_head * a.k_head_stride,
-                a.dim, lane);
-      stage_row(s_value[warp],
-                static_cast<const T*>(a.v) + t * a.v_stride + kv_head * a.v_head_stride, a.dim,
-                lane);
-      const int64_t j = t - tile.begin;
-      const int64_t from = max(int64_t{0}, j - a.right);
-      const int64_t to = j < a.first ? n : min(int64_t{n}, j + a.left + 1);
-      for (int h = kv_head * group; h < (kv_head + 1) * group; ++h) {
-        const T* q = static_cast<const T*>(a.q) + h * a.q_head_stride;
-        const T* g = static_cast<const T*>(a.grad_out) + int64_t{h} * a.dim;
-        const int64_t g_stride = int64_t{a.heads} * a.dim;
-        for (int64_t base = from; base < to; base += 32) {
-          const bool in = base + lane < to;
-          const int64_t row = tile.begin + (in ? base + lane : 0);
-          float p = 0.0f, e = 0.0f;
-          if (in) {
-            const float lse = a.lse[h * a.tokens + row];
-            p = expf(fmaf(dot(s_key[warp], q + row * a.q_stride, a.dim), a.scale, -lse));
-            e = p * (dot(s_value[warp], g + row * g_stride, a.dim) - delta[h * a.tokens + row]);
-          }
-          add_rows(dk, e, q, a.q_stride, row, a.dim, lane);
-          add_rows(dv, p, g, g_stride, row, a.dim, lane);
-        }
-      }
-    }
-    const int64_t at = (int64_t{t} * a.kv_heads + kv_head) * a.dim;
-    store_row(static_cast<T*>(a.grad_k) + at, dk, a.scale, a.dim, lane);
-    store_row(static_cast<T*>(a.grad_v) + at, dv, 1.0f, a.dim, lane);
+int64_t sequences_of(const gs_window_attention_args& a) { return a.tile_starts ? a.sequences : 1; }
+// D of every row, to a 256-byte boundary.
+int64_t delta_floats(const gs_window_attention_args& a) {
+  return (a.tokens * a.heads + 63) / 64 * 64;
+}
+
+// A chunk is about as long as a window's walk, so that its block takes about as
+// long as the others.
+int64_t chunk_tiles(const gs_window_attention_args& a) {
+  const int64_t window =
+      std::min(a.tokens, int64_t{a.left}) + std::min(a.tokens, int64_t{a.right});
+  return std::max<int64_t>(8, (window + kTile - 1) / kTile + 1);
+}
+int64_t chunk_slots(const gs_window_attention_args& a) {
+  return a.first > 0 ? a.num_tiles / chunk_tiles(a) + sequences_of(a) : 0;
+}
+
+template <class T, int kDim>
+int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  CUtensorMap rows[4], tiles[4];  // q, grad_out, k, v in boxes of 128 and of 64 rows
+  for (int m = 0; m < 4; ++m) {
+    const void* const base[4] = {a.q, a.grad_out, a.k, a.v};
+    const int64_t stride[4] = {a.q_stride, int64_t{a.heads} * a.dim, a.k_stride, a.v_stride};
+    const int64_t head_stride[4] = {a.q_head_stride, a.dim, a.k_head_stride, a.v_head_stride};
+    const int64_t heads = m < 2 ? a.heads : a.kv_heads;
+    GS_TRY(tc::encode_map(&rows[m], kBf16, base[m], a.tokens, heads, a.dim, stride[m],
+                          head_stride[m], kTile));
+    GS_TRY(tc::encode_map(&tiles[m], kBf16, base[m], a.tokens, heads, a.dim, stride[m],
+                          head_stride[m], kKeys));
   }
+  float* delta = static_cast<float*>(a.workspace);
+  FirstSums sums;
+  sums.tiles = static_cast<int>(chunk_tiles(a));
+  sums.slots = static_cast<int>(chunk_slots(a));
+  sums.base = delta + delta_floats(a);
+  sums.part = sums.base + sequences_of(a) * a.kv_heads * a.first * 2 * a.dim;
+  constexpr size_t kShared = sizeof(BackwardShared<kDim>);
+  GS_CUDA_TRY(cudaFuncSetAttribute(grad_query_kernel<T, kDim>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  GS_CUDA_TRY(cudaFuncSetAttribute(grad_key_kernel<T, kDim>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  const int64_t key_blocks = (a.num_tiles + sums.slots) * a.kv_heads;
+  const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
+  if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
+                        kComputeThreads + 32, kShared, stream, a, delta, rows[0], rows[1],
+                        tiles[2], tiles[3]);
+  GS_TRY(check_launch());
+  launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
+                        kComputeThreads + 32, kShared, stream, a, delta, sums, rows[2], rows[3],
+                        tiles[0], tiles[1]);
+  GS_TRY(check_launch());
+  if (first_blocks > 0)
+    launch_chained(first_sum_kernel<T>, static_cast<unsigned>(first_blocks), 2 * kMaxDim * kParts,
+                   stream, a, sums);
+  return check_launch();
 }
 
 // One new token a stream against its cache of `slots` tokens: the first
@@ -617,8 +1064,10 @@ int32_t with_sixteen_bit(int32_t dtype, F&& f) {
 
 }  // namespace
 
-uint64_t window_attention_workspace_size(int64_t tokens, int64_t heads) {
-  return sizeof(float) * static_cast<uint64_t>(tokens) * heads;
+uint64_t window_attention_workspace_size(const gs_window_attention_args& a) {
+  const int64_t first =
+      (sequences_of(a) + chunk_slots(a)) * a.kv_heads * a.first * 2 * a.dim;
+  return sizeof(float) * static_cast<uint64_t>(delta_floats(a) + first);
 }
 
 int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t stream) {
@@ -649,16 +1098,12 @@ int32_t launch_window_attention_backward(const gs_window_attention_args& a, cuda
   for (const void* p : {a.grad_out, static_cast<const void*>(a.grad_q),
                         static_cast<const void*>(a.grad_k), static_cast<const void*>(a.grad_v)})
     if (!is_aligned(p, 16)) return GS_ERR_MISALIGNED;
-  if (a.workspace_size < window_attention_workspace_size(a.tokens, a.heads))
-    return GS_ERR_CAPACITY;
-  float* delta = static_cast<float*>(a.workspace);
+  if (a.tiles && !a.tile_starts) return GS_ERR_INVALID_ARGUMENT;
+  if (!is_aligned(a.workspace, 256)) return GS_ERR_MISALIGNED;
+  if (a.workspace_size < window_attention_workspace_size(a)) return GS_ERR_CAPACITY;
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
-    launch_chained(grad_query_kernel<T>, dim3(a.num_tiles, a.heads), kThreads, stream, a, delta);
-    GS_TRY(check_launch());
-    launch_chained(grad_key_kernel<T>, dim3(a.num_tiles, a.kv_heads), kThreads, stream, a,
-                   static_cast<const float*>(delta));
-    return check_launch();
+    return a.dim <= 64 ? backward<T, 64>(a, stream) : backward<T, 128>(a, stream);
   });
 }
 

@@ -31,7 +31,7 @@ int32_t launch_det_math(int, int64_t, const float*, float*, cudaStream_t);
 int32_t launch_window_attention(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_backward(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_step(const gs_window_attention_step_args&, cudaStream_t);
-uint64_t window_attention_workspace_size(int64_t, int64_t);
+uint64_t window_attention_workspace_size(const gs_window_attention_args&);
 int32_t window_attention_status(cudaStream_t);
 int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_backward(const gs_gated_scan_args&, cudaStream_t);
@@ -519,9 +519,10 @@ int32_t gs_l1_loss_backward(const float* image, int64_t height, int64_t width, i
 }
 
 uint64_t gs_window_attention_workspace_size(const gs_window_attention_args* a) {
-  return !a || a->tokens < 0 || a->heads < 1
+  return !a || a->tokens < 0 || a->heads < 1 || a->kv_heads < 1 || a->dim < 1 || a->first < 0 ||
+                 a->left < 0 || a->right < 0
              ? 0
-             : gs::window_attention_workspace_size(a->tokens, a->heads);
+             : gs::window_attention_workspace_size(*a);
 }
 
 int32_t gs_window_attention(const gs_window_attention_args* args, gs_stream_t stream) {

@@ -239,12 +239,21 @@ inline int32_t encode_map(CUtensorMap* map, bool bf16, const void* base, int64_t
                                 static_cast<cuuint64_t>(token_stride) * 2};
   const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
   const cuuint32_t step[3] = {1, 1, 1};
-  const CUresult r = encode(
-      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-      const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? GS_OK : GS_ERR_INVALID_ARGUMENT;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    const CUresult r = encode(
+        map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+        const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return GS_OK;
+    if (r != CUDA_ERROR_INVALID_CONTEXT) break;
+    // A thread that has made no runtime call yet (an autograd worker) has no
+    // context for this driver call; selecting its device binds one.
+    int device;
+    GS_CUDA_TRY(cudaGetDevice(&device));
+    GS_CUDA_TRY(cudaSetDevice(device));
+  }
+  return GS_ERR_INVALID_ARGUMENT;
 }
 
 }  // namespace tc

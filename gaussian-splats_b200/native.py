@@ -195,7 +195,8 @@ def _fields(kind, names):
 class WindowAttentionArgs(ctypes.Structure):
     """``gs_window_attention_args`` (include/gs_b200.h)."""
 
-    _fields_ = (_fields(ctypes.c_int64, "tokens num_tiles") + _fields(ctypes.c_void_p, "tiles") +
+    _fields_ = (_fields(ctypes.c_int64, "tokens sequences num_tiles") +
+                _fields(ctypes.c_void_p, "tiles tile_starts") +
                 _fields(ctypes.c_int32, "heads kv_heads dim dtype left right first") +
                 _fields(ctypes.c_float, "scale") + _fields(ctypes.c_void_p, "q k v") +
                 _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "

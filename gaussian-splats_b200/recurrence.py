@@ -41,16 +41,14 @@ class _GatedScan(torch.autograd.Function):
         if initial is not None:
             initial = initial.detach().contiguous()
         tokens, channels = x.shape
-        device, sequences = x.device, 1 if packed is None else len(packed)
-        num_tiles, tiles = tile_arguments(packed, tokens)
+        device = x.device
+        layout = tile_arguments(packed, tokens)
         y = torch.empty((tokens, channels), dtype=x.dtype, device=device)
-        last = torch.empty((sequences, channels), dtype=torch.float32, device=device)
-        entering = torch.empty((num_tiles, channels), dtype=torch.float32, device=device)
+        last = torch.empty((layout["sequences"], channels), dtype=torch.float32, device=device)
+        entering = torch.empty((layout["num_tiles"], channels), dtype=torch.float32, device=device)
         args = native.GatedScanArgs(
-            tokens=tokens, sequences=sequences, num_tiles=num_tiles, tiles=tiles,
-            tile_starts=None if packed is None else packed.tile_starts.data_ptr(),
-            channels=channels, dtype=dtype, x=address(x), gate=address(gate),
-            x_stride=x.stride(0), gate_stride=gate.stride(0), initial=address(initial),
+            tokens=tokens, **layout, channels=channels, dtype=dtype, x=address(x),
+            gate=address(gate), x_stride=x.stride(0), gate_stride=gate.stride(0), initial=address(initial),
             y=address(y), last=address(last), entering=address(entering))
         lib = native.lib()
         size = lib.gs_gated_scan_workspace_size(ctypes.byref(args))

@@ -68,12 +68,14 @@ def check_packed(packed: PackedSequences | None, tokens: int, device: torch.devi
         raise RuntimeError(f"{what}: packed sequences on {packed.device}, tensors on {device}")
 
 
-def tile_arguments(packed: PackedSequences | None, tokens: int) -> tuple[int, int | None]:
-    """(num_tiles, tiles) of an operator's arguments: without a layout, the
-    rows are one sequence and its tiles follow from their number."""
+def tile_arguments(packed: PackedSequences | None, tokens: int) -> dict:
+    """The layout's fields of an operator's arguments: without one, the rows
+    are one sequence and its tiles follow from their number."""
     if packed is None:
-        return -(-tokens // native.SEQUENCE_TILE), None
-    return packed.num_tiles, packed.tiles.data_ptr() if packed.num_tiles else None
+        return {"sequences": 1, "num_tiles": -(-tokens // native.SEQUENCE_TILE)}
+    return {"sequences": len(packed), "num_tiles": packed.num_tiles,
+            "tiles": packed.tiles.data_ptr() if packed.num_tiles else None,
+            "tile_starts": packed.tile_starts.data_ptr()}
 
 
 def element_type(dtype: torch.dtype, what: str, allowed=(torch.float32, torch.bfloat16,

@@ -508,8 +508,8 @@ enum {
  * v, out and grad_out. The backward needs a workspace of
  * gs_window_attention_workspace_size bytes. */
 typedef struct gs_window_attention_args {
-  int64_t tokens, num_tiles;
-  const int32_t *tiles;
+  int64_t tokens, sequences, num_tiles;
+  const int32_t *tiles, *tile_starts;
   int32_t heads, kv_heads, dim, dtype;
   int32_t left, right, first;
   float scale;
