@@ -38,6 +38,12 @@ __device__ __forceinline__ float load_weight(const void* w, int32_t dtype, int64
   return __half2float(__ldg(static_cast<const __half*>(w) + c));
 }
 
+__device__ __forceinline__ void load_weights(const void* w, int32_t dtype, int c, float (&x)[8]) {
+  if (dtype == GS_FLOAT32) load_pack<8>(static_cast<const float*>(w) + c, x);
+  else if (dtype == GS_BFLOAT16) load_pack<8>(static_cast<const __nv_bfloat16*>(w) + c, x);
+  else load_pack<8>(static_cast<const __half*>(w) + c, x);
+}
+
 // The 8-bit code of z w / s' for s' = max|z w| / 448 (y / s without the m that
 // cancels), from the product in double: a float chain z m w / s is off by a few
 // units in the last place, which moves one value in some 10^5 across a rounding
@@ -69,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(gs_rms_norm_args a) {
   const float m = rsqrtf(warp_sum(square) / static_cast<float>(a.channels) + a.eps);
   double inverse = 0.0;
   const auto product = [&](int c) {
-    const double z = static_cast<double>(to_float(x[c])) + (r ? to_float(r[c]) : 0.0f);
+    const double z = to_float(x[c]) + (r ? to_float(r[c]) : 0.0f);
     return z * load_weight(a.weight, a.weight_dtype, c);
   };
   if (a.q) {
@@ -105,6 +111,98 @@ __device__ __forceinline__ float2 block_sum2(float2 v, float2* shared) {
     total.y += shared[w].y;
   }
   return total;
+}
+__device__ __forceinline__ float block_max(float v, float2* shared) {
+  v = warp_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5].x = v;
+  __syncthreads();
+  float top = shared[0].x;
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) top = fmaxf(top, shared[w].x);
+  return top;
+}
+
+// Rows of whole, aligned 16-byte words: kLanes threads (a warp or the block)
+// hold a token in registers, kIter words of 8 channels a thread, all loaded
+// before the first is used, so the row is read once and a multiprocessor has
+// tens of kilobytes in flight.
+template <class T, class R, int kLanes, int kIter>
+__global__ void __launch_bounds__(kThreads) norm_rows_kernel(gs_rms_norm_args a) {
+  chain_wait();
+  __shared__ float2 s_sum[kWarps];
+  constexpr int kRows = kThreads / kLanes;
+  const int64_t row = int64_t{blockIdx.x} * kRows + threadIdx.x / kLanes;
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x % kLanes;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const R* r = a.residual ? static_cast<const R*>(a.residual) + row * a.residual_stride : nullptr;
+  float z[kIter][8];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int c = (i * kLanes + lane) * 8;
+    if (c < a.channels) load_pack<8>(x + c, z[i]);
+  }
+  if (r)
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int c = (i * kLanes + lane) * 8;
+      float y[8];
+      if (c < a.channels) {
+        load_pack<8>(r + c, y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[i][k] += y[k];
+      }
+    }
+  float square = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int c = (i * kLanes + lane) * 8;
+    if (c < a.channels) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) square = fmaf(z[i][k], z[i][k], square);
+      if (a.sum) store_pack<8>(static_cast<R*>(a.sum) + row * a.channels + c, z[i]);
+    }
+  }
+  square = kLanes == 32 ? warp_sum(square) : block_sum2(make_float2(square, 0.0f), s_sum).x;
+  const float m = rsqrtf(square / static_cast<float>(a.channels) + a.eps);
+  double inverse = 0.0;
+  if (a.q) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int c = (i * kLanes + lane) * 8;
+      if (c < a.channels) {
+        float w[8];
+        load_weights(a.weight, a.weight_dtype, c, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(z[i][k] * w[k]));
+      }
+    }
+    top = kLanes == 32 ? warp_max(top) : block_max(top, s_sum);
+    if (top > 0.0f) inverse = kE4m3Max / static_cast<double>(top);
+    if (lane == 0) a.scale[row] = top > 0.0f ? top * m / kE4m3Max : 1.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int c = (i * kLanes + lane) * 8;
+    if (c >= a.channels) continue;
+    float w[8];
+    load_weights(a.weight, a.weight_dtype, c, w);
+    if (a.q) {
+      uint2 codes = make_uint2(0, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        codes.x |= to_e4m3(static_cast<double>(z[i][k]) * w[k], inverse) << (8 * k);
+        codes.y |= to_e4m3(static_cast<double>(z[i][k + 4]) * w[k + 4], inverse) << (8 * k);
+      }
+      *reinterpret_cast<uint2*>(a.q + row * a.channels + c) = codes;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = z[i][k] * m * w[k];
+      store_pack<8>(static_cast<T*>(a.y) + row * a.channels + c, w);
+    }
+  }
 }
 
 // Any channel count and alignment: one block a token at a time. A channel's
@@ -144,6 +242,88 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(gs_rms_norm_arg
   }
   for (int c = threadIdx.x; c < a.channels; c += kThreads)
     partials[int64_t{blockIdx.x} * a.channels + c] = s_dw[c];
+}
+
+// Rows of whole, aligned 16-byte words: kLanes threads (a warp or the block)
+// hold a token, kIter words of 8 channels a thread, and the weight gradients of
+// their channels from token to token. A block's warps add theirs up in order.
+template <class T, class R, int kLanes, int kIter>
+__global__ void __launch_bounds__(kThreads)
+    norm_rows_backward_kernel(gs_rms_norm_args a, float* partials) {
+  chain_wait();
+  extern __shared__ float s_dw[];
+  __shared__ float2 s_sum[kWarps];
+  constexpr int kRows = kThreads / kLanes;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const float inverse = 1.0f / static_cast<float>(a.channels);
+  float dw[kIter][8] = {};
+  for (int64_t row = int64_t{blockIdx.x} * kRows + group; row < a.rows;
+       row += int64_t{gridDim.x} * kRows) {
+    const R* z_row = static_cast<const R*>(a.sum) + row * a.sum_stride;
+    const int64_t at = row * a.channels;
+    Pack<R, 8> z[kIter], h[kIter];
+    Pack<T, 8> g[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int c = (i * kLanes + lane) * 8;
+      if (c < a.channels) {
+        z[i] = *reinterpret_cast<const Pack<R, 8>*>(z_row + c);
+        g[i] = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.grad_y) + at + c);
+        if (a.grad_sum)
+          h[i] = *reinterpret_cast<const Pack<R, 8>*>(static_cast<const R*>(a.grad_sum) + at + c);
+      }
+    }
+    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int c = (i * kLanes + lane) * 8;
+      if (c < a.channels) {
+        float w[8];
+        load_weights(a.weight, a.weight_dtype, c, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float zc = to_float(z[i].v[k]);
+          v.x = fmaf(zc, zc, v.x);
+          v.y = fmaf(to_float(g[i].v[k]) * w[k], zc, v.y);
+        }
+      }
+    }
+    if constexpr (kLanes == 32) v = make_float2(warp_sum(v.x), warp_sum(v.y));
+    else v = block_sum2(v, s_sum);
+    const float m = rsqrtf(v.x * inverse + a.eps);
+    const float pull = v.y * inverse * m * m;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int c = (i * kLanes + lane) * 8;
+      if (c >= a.channels) continue;
+      float w[8];
+      load_weights(a.weight, a.weight_dtype, c, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float zc = to_float(z[i].v[k]), gc = to_float(g[i].v[k]);
+        const float own = a.grad_sum ? to_float(h[i].v[k]) : 0.0f;
+        w[k] = fmaf(m, fmaf(-zc, pull, gc * w[k]), own);
+        dw[i][k] = fmaf(gc, zc * m, dw[i][k]);
+      }
+      store_pack<8>(static_cast<T*>(a.grad_x) + at + c, w);
+      if (a.grad_residual) store_pack<8>(static_cast<R*>(a.grad_residual) + at + c, w);
+    }
+  }
+  for (int turn = 0; turn < kRows; ++turn) {
+    if (group == turn)
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int c = (i * kLanes + lane) * 8;
+        if (c < a.channels)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float sum = turn ? s_dw[c + k] + dw[i][k] : dw[i][k];
+            if (turn == kRows - 1) partials[int64_t{blockIdx.x} * a.channels + c + k] = sum;
+            else s_dw[c + k] = sum;
+          }
+      }
+    __syncthreads();
+  }
 }
 
 // The weight gradient: the blocks' partial sums in block order, 32 channels a
@@ -189,8 +369,51 @@ int32_t check_args(const gs_rms_norm_args& a, bool backward) {
   return GS_OK;
 }
 
+// Calls f with (threads of a token, words of 8 channels a thread) for the
+// smallest that hold `channels`: a warp up to `warp_channels`, else the block.
+template <int N>
+using Number = std::integral_constant<int, N>;
+template <int kMaxWords, class F>
+int32_t with_shape(int channels, int warp_channels, F&& f) {
+  if (channels <= warp_channels) {
+    if (channels <= 256) return f(Number<32>{}, Number<1>{});
+    if (channels <= 512) return f(Number<32>{}, Number<2>{});
+    if constexpr (kMaxWords >= 8)
+      if (channels > 1024)
+        return f(Number<32>{}, Number<8>{});
+    return f(Number<32>{}, Number<4>{});
+  }
+  if (channels <= 2048) return f(Number<256>{}, Number<1>{});
+  if (channels <= 4096) return f(Number<256>{}, Number<2>{});
+  if constexpr (kMaxWords >= 8)
+    if (channels > 8192)
+      return f(Number<256>{}, Number<8>{});
+  return f(Number<256>{}, Number<4>{});
+}
+
+bool whole_words(const gs_rms_norm_args& a) {
+  if (a.channels % 8 || a.x_stride % 8 || a.residual_stride % 8 || a.sum_stride % 8) return false;
+  for (const void* p : {a.x, a.residual, a.weight, static_cast<const void*>(a.y),
+                        static_cast<const void*>(a.sum), static_cast<const void*>(a.q), a.grad_y,
+                        a.grad_sum, static_cast<const void*>(a.grad_x),
+                        static_cast<const void*>(a.grad_residual)})
+    if (!is_aligned(p, 16)) return false;
+  return true;
+}
+
 template <class T, class R>
 int32_t forward(const gs_rms_norm_args& a, cudaStream_t stream) {
+  if (whole_words(a)) {
+    // With fewer tokens than multiprocessors a token's latency is the call's:
+    // the whole block shares it.
+    const int warp_channels = a.rows <= kSmCount ? 256 : 2048;
+    return with_shape<8>(a.channels, warp_channels, [&](auto lanes, auto iter) {
+      constexpr int kLanes = decltype(lanes)::value, kIter = decltype(iter)::value;
+      launch_chained(norm_rows_kernel<T, R, kLanes, kIter>, ceil_div(a.rows, kThreads / kLanes),
+                     kThreads, stream, a);
+      return check_launch();
+    });
+  }
   launch_chained(norm_kernel<T, R>, ceil_div(a.rows, kWarps), kThreads, stream, a);
   return check_launch();
 }
@@ -200,11 +423,21 @@ int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
   float* partials = static_cast<float*>(a.workspace);
   const int blocks = backward_blocks(a.rows);
   const size_t shared = sizeof(float) * a.channels;
-  GS_CUDA_TRY(cudaFuncSetAttribute(norm_backward_kernel<T, R>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   sizeof(float) * GS_MAX_NORM_CHANNELS));
-  launch_chained_shared(norm_backward_kernel<T, R>, blocks, kThreads, shared, stream, a, partials);
-  GS_TRY(check_launch());
+  if (whole_words(a) && a.channels <= 8192) {
+    GS_TRY(with_shape<4>(a.channels, 1024, [&](auto lanes, auto iter) {
+      constexpr int kLanes = decltype(lanes)::value, kIter = decltype(iter)::value;
+      launch_chained_shared(norm_rows_backward_kernel<T, R, kLanes, kIter>, blocks, kThreads,
+                            kLanes == 32 ? shared : 0, stream, a, partials);
+      return check_launch();
+    }));
+  } else {
+    GS_CUDA_TRY(cudaFuncSetAttribute(norm_backward_kernel<T, R>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     sizeof(float) * GS_MAX_NORM_CHANNELS));
+    launch_chained_shared(norm_backward_kernel<T, R>, blocks, kThreads, shared, stream, a,
+                          partials);
+    GS_TRY(check_launch());
+  }
   return with_dtype(a.weight_dtype, [&](auto w) {
     using W = decltype(w);
     launch_chained(norm_weight_kernel<W>, ceil_div(a.channels, 32), kThreads, stream, partials,
