@@ -17,6 +17,8 @@
 
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "sequence.cuh"
 
 namespace gs {
@@ -29,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBackwardBlocks = 2 * kSmCount;  // rows of partial weight gradients
+constexpr int kBackwardBlocks = 4 * kSmCount;  // rows of partial weight gradients
 constexpr float kE4m3Max = 448.0f;
 
 __device__ __forceinline__ float load_weight(const void* w, int32_t dtype, int64_t c) {
@@ -244,15 +246,40 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(gs_rms_norm_arg
     partials[int64_t{blockIdx.x} * a.channels + c] = s_dw[c];
 }
 
-// Rows of whole, aligned 16-byte words: kLanes threads (a warp or the block)
-// hold a token, kIter words of 8 channels a thread, and the weight gradients of
-// their channels from token to token. A block's warps add theirs up in order.
+// Sums over a group of kLanes threads of the block; `turn` alternates between
+// two sets of slots, so that one barrier a row is enough.
+template <int kLanes>
+__device__ __forceinline__ float2 group_sum2(float2 v, float2 (*shared)[kWarps], int turn) {
+  v.x = warp_sum(v.x);
+  v.y = warp_sum(v.y);
+  if constexpr (kLanes > 32) {
+    constexpr int kGroupWarps = kLanes / 32;
+    const int warp = threadIdx.x >> 5, group = threadIdx.x / kLanes;
+    if ((threadIdx.x & 31) == 0) shared[turn][warp] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kLanes) : "memory");
+    v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kGroupWarps; ++w) {
+      v.x += shared[turn][group * kGroupWarps + w].x;
+      v.y += shared[turn][group * kGroupWarps + w].y;
+    }
+  }
+  return v;
+}
+
+// Rows of whole, aligned 16-byte words: a group of kLanes threads holds a
+// token, kIter words of 8 channels a thread, and the weight gradients of their
+// channels from token to token; a block's groups add theirs up in order. One
+// or two words a thread keep a thread at 64 registers, so that 32 warps a
+// multiprocessor cover the loads (a warp a token of 1024 channels took 160
+// registers, 8 warps, and 963 us for 262,144 tokens).
 template <class T, class R, int kLanes, int kIter>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4 / kIter)
     norm_rows_backward_kernel(gs_rms_norm_args a, float* partials) {
   chain_wait();
   extern __shared__ float s_dw[];
-  __shared__ float2 s_sum[kWarps];
+  __shared__ float2 s_sum[2][kWarps];
+  int turn = 0;
   constexpr int kRows = kThreads / kLanes;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const float inverse = 1.0f / static_cast<float>(a.channels);
@@ -288,8 +315,8 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    if constexpr (kLanes == 32) v = make_float2(warp_sum(v.x), warp_sum(v.y));
-    else v = block_sum2(v, s_sum);
+    v = group_sum2<kLanes>(v, s_sum, turn);
+    turn ^= 1;
     const float m = rsqrtf(v.x * inverse + a.eps);
     const float pull = v.y * inverse * m * m;
 #pragma unroll
@@ -309,16 +336,16 @@ __global__ void __launch_bounds__(kThreads)
       if (a.grad_residual) store_pack<8>(static_cast<R*>(a.grad_residual) + at + c, w);
     }
   }
-  for (int turn = 0; turn < kRows; ++turn) {
-    if (group == turn)
+  for (int owner = 0; owner < kRows; ++owner) {
+    if (group == owner)
 #pragma unroll
       for (int i = 0; i < kIter; ++i) {
         const int c = (i * kLanes + lane) * 8;
         if (c < a.channels)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float sum = turn ? s_dw[c + k] + dw[i][k] : dw[i][k];
-            if (turn == kRows - 1) partials[int64_t{blockIdx.x} * a.channels + c + k] = sum;
+            const float sum = owner ? s_dw[c + k] + dw[i][k] : dw[i][k];
+            if (owner == kRows - 1) partials[int64_t{blockIdx.x} * a.channels + c + k] = sum;
             else s_dw[c + k] = sum;
           }
       }
@@ -326,24 +353,25 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// The weight gradient: the blocks' partial sums in block order, 32 channels a
-// block, each warp an eighth of the rows.
+// The weight gradient: the blocks' partial sums, 32 channels a block, each warp
+// its share of the rows, the shares in order.
+constexpr int kWeightWarps = 32;
 template <class W>
-__global__ void __launch_bounds__(kThreads) norm_weight_kernel(const float* partials, int blocks,
+__global__ void __launch_bounds__(32 * kWeightWarps) norm_weight_kernel(const float* partials, int blocks,
                                                                int channels, W* grad_weight) {
   chain_wait();
-  __shared__ float s_part[kWarps][33];
+  __shared__ float s_part[kWeightWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float sum = 0.0f;
   if (c < channels)
 #pragma unroll 8
-    for (int b = warp; b < blocks; b += kWarps) sum += partials[int64_t{b} * channels + c];
+    for (int b = warp; b < blocks; b += kWeightWarps) sum += partials[int64_t{b} * channels + c];
   s_part[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < channels) {
     sum = 0.0f;
-    for (int w = 0; w < kWarps; ++w) sum += s_part[w][lane];
+    for (int w = 0; w < kWeightWarps; ++w) sum += s_part[w][lane];
     grad_weight[c] = from_float<W>(sum);
   }
 }
@@ -369,25 +397,34 @@ int32_t check_args(const gs_rms_norm_args& a, bool backward) {
   return GS_OK;
 }
 
-// Calls f with (threads of a token, words of 8 channels a thread) for the
-// smallest that hold `channels`: a warp up to `warp_channels`, else the block.
 template <int N>
 using Number = std::integral_constant<int, N>;
-template <int kMaxWords, class F>
-int32_t with_shape(int channels, int warp_channels, F&& f) {
+
+// Calls f with the forward's (threads of a token, words of 8 channels a
+// thread): a warp up to `warp_channels`, else the block.
+template <class F>
+int32_t with_forward_shape(int channels, int warp_channels, F&& f) {
   if (channels <= warp_channels) {
     if (channels <= 256) return f(Number<32>{}, Number<1>{});
     if (channels <= 512) return f(Number<32>{}, Number<2>{});
-    if constexpr (kMaxWords >= 8)
-      if (channels > 1024)
-        return f(Number<32>{}, Number<8>{});
-    return f(Number<32>{}, Number<4>{});
+    if (channels <= 1024) return f(Number<32>{}, Number<4>{});
+    return f(Number<32>{}, Number<8>{});
   }
   if (channels <= 2048) return f(Number<256>{}, Number<1>{});
   if (channels <= 4096) return f(Number<256>{}, Number<2>{});
-  if constexpr (kMaxWords >= 8)
-    if (channels > 8192)
-      return f(Number<256>{}, Number<8>{});
+  if (channels <= 8192) return f(Number<256>{}, Number<4>{});
+  return f(Number<256>{}, Number<8>{});
+}
+
+// The same for the backward, up to 8192 channels: as few words a thread as a
+// block can have.
+template <class F>
+int32_t with_backward_shape(int channels, F&& f) {
+  if (channels <= 256) return f(Number<32>{}, Number<1>{});
+  if (channels <= 512) return f(Number<64>{}, Number<1>{});
+  if (channels <= 1024) return f(Number<128>{}, Number<1>{});
+  if (channels <= 2048) return f(Number<256>{}, Number<1>{});
+  if (channels <= 4096) return f(Number<256>{}, Number<2>{});
   return f(Number<256>{}, Number<4>{});
 }
 
@@ -407,7 +444,7 @@ int32_t forward(const gs_rms_norm_args& a, cudaStream_t stream) {
     // With fewer tokens than multiprocessors a token's latency is the call's:
     // the whole block shares it.
     const int warp_channels = a.rows <= kSmCount ? 256 : 2048;
-    return with_shape<8>(a.channels, warp_channels, [&](auto lanes, auto iter) {
+    return with_forward_shape(a.channels, warp_channels, [&](auto lanes, auto iter) {
       constexpr int kLanes = decltype(lanes)::value, kIter = decltype(iter)::value;
       launch_chained(norm_rows_kernel<T, R, kLanes, kIter>, ceil_div(a.rows, kThreads / kLanes),
                      kThreads, stream, a);
@@ -421,13 +458,14 @@ int32_t forward(const gs_rms_norm_args& a, cudaStream_t stream) {
 template <class T, class R>
 int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
   float* partials = static_cast<float*>(a.workspace);
-  const int blocks = backward_blocks(a.rows);
+  int blocks = backward_blocks(a.rows);
   const size_t shared = sizeof(float) * a.channels;
   if (whole_words(a) && a.channels <= 8192) {
-    GS_TRY(with_shape<4>(a.channels, 1024, [&](auto lanes, auto iter) {
+    GS_TRY(with_backward_shape(a.channels, [&](auto lanes, auto iter) {
       constexpr int kLanes = decltype(lanes)::value, kIter = decltype(iter)::value;
+      blocks = std::min<int>(blocks, ceil_div(a.rows, kThreads / kLanes));
       launch_chained_shared(norm_rows_backward_kernel<T, R, kLanes, kIter>, blocks, kThreads,
-                            kLanes == 32 ? shared : 0, stream, a, partials);
+                            kLanes < kThreads ? shared : 0, stream, a, partials);
       return check_launch();
     }));
   } else {
@@ -440,7 +478,7 @@ int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
   }
   return with_dtype(a.weight_dtype, [&](auto w) {
     using W = decltype(w);
-    launch_chained(norm_weight_kernel<W>, ceil_div(a.channels, 32), kThreads, stream, partials,
+    launch_chained(norm_weight_kernel<W>, ceil_div(a.channels, 32), 32 * kWeightWarps, stream, partials,
                    blocks, a.channels, static_cast<W*>(a.grad_weight));
     return check_launch();
   });

@@ -13,8 +13,8 @@
 // maps s -> A s + B, which compose associatively, so the sequence is cut into
 // tiles of kTile tokens: one kernel folds each tile to its (A, B), one scans the
 // tiles of each sequence for the state that enters each tile, one walks the
-// tiles from those states. Inside a tile, each warp holds kTokens tokens of 32
-// lanes' channels in registers and the warps' folds are joined in order in
+// tiles from those states. Inside a tile, each thread holds kTokens tokens of
+// its channels in registers and the threads' folds are joined in order in
 // shared memory. Every order is fixed, so results repeat bit for bit.
 //
 // States, products and gates are float; the states that enter the tiles are
@@ -35,255 +35,284 @@ uint64_t gated_scan_workspace_size(int64_t num_tiles, int64_t channels);
 namespace {
 
 constexpr int kTile = GS_SEQUENCE_TILE;
-constexpr int kTokens = 8;               // tokens a thread holds
-constexpr int kWarps = kTile / kTokens;  // warps of a tile's block
-constexpr int kThreads = 32 * kWarps;
-constexpr int kScanWarps = 16;  // warps that share a sequence's tiles in the tile scan
+constexpr int kTokens = 8;                // tokens a thread holds
+constexpr int kGroups = kTile / kTokens;  // threads that share a channel of a tile
+constexpr int kScanThreads = 1024;
 
-// a = sigmoid(gate) and k = 1 - a, both with small relative error: the smaller
-// of the two is e / (1 + e) with e = exp(-|gate|), never a difference.
-__device__ __forceinline__ void open_gate(float gate, float& a, float& k) {
-  const float e = __expf(-fabsf(gate));
-  const float large = __fdividef(1.0f, 1.0f + e), small = e * large;
-  a = gate >= 0.0f ? large : small;
-  k = gate >= 0.0f ? small : large;
+// e = exp(-gate), a = sigmoid(gate) = 1 / (1 + e); k = 1 - a is e a, with the
+// same relative error however small it is. The exponent is cut where a is far
+// below any gate's use, so that e stays finite.
+__device__ __forceinline__ float open_gate(float gate, float& e) {
+  constexpr float kMinusLog2e = -1.4426950408889634f;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(gate * kMinusLog2e, 100.0f)));
+  return __fdividef(1.0f, 1.0f + e);
 }
 
 // A map s -> a s + b.
 struct Affine {
   float a, b;
 };
+__device__ __forceinline__ Affine then(Affine first, Affine second) {
+  return {second.a * first.a, fmaf(second.a, first.b, second.b)};
+}
 
-// What a block works on: a tile of tokens and 32 V channels, V to a lane.
+// What a block works on: a tile of tokens and kLanes V channels, V to a thread;
+// kGroups threads of kTokens tokens each share a channel.
 template <int V>
 struct Place {
+  static constexpr int kLanes = V == 1 ? 32 : 16;
+  static constexpr int kChannels = kLanes * V;
+  static constexpr int kThreads = kLanes * kGroups;
   Tile tile;
-  int64_t index;  // of the tile
-  int channel;    // the lane's first
-  int first, count;  // the warp's tokens in the tile's sequence
-  bool live;         // the lane has channels
+  int64_t index;     // of the tile
+  int channel;       // the thread's first
+  int group;
+  int first, count;  // the thread's tokens
+  bool live;         // the thread has channels
   __device__ __forceinline__ Place(const gs_gated_scan_args& a, bool reverse) {
-    const int columns = (a.channels + 32 * V - 1) / (32 * V);
+    const int columns = (a.channels + kChannels - 1) / kChannels;
     index = blockIdx.x / columns;
     if (reverse) index = a.num_tiles - 1 - index;
-    channel = (static_cast<int>(blockIdx.x % columns) * 32 + (threadIdx.x & 31)) * V;
+    channel = (static_cast<int>(blockIdx.x % columns) * kLanes + threadIdx.x % kLanes) * V;
     live = channel < a.channels;
+    group = threadIdx.x / kLanes;
     tile = tile_at(a.tiles, index, static_cast<int32_t>(a.tokens), kTile);
-    first = tile.start + static_cast<int>(threadIdx.x >> 5) * kTokens;
-    count = min(kTokens, min(tile.end, tile.start + kTile) - first);
-    if (!live) count = 0;
+    first = tile.start + group * kTokens;
+    count = live ? min(kTokens, min(tile.end, tile.start + kTile) - first) : 0;
   }
 };
 
+// The thread's tokens of one array; what it does not have reads as `missing`.
 template <class T, int V>
-__device__ __forceinline__ void load_tokens(const T* p, int64_t stride, int first, int channel,
-                                            int count, float (&x)[kTokens][V]) {
+__device__ __forceinline__ void load_tokens(const void* p, int64_t stride, const Place<V>& at,
+                                            float missing, float (&x)[kTokens][V]) {
+  const T* q = static_cast<const T*>(p) + at.first * stride + at.channel;
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t)
-    if (t < count) load_pack<V>(p + (first + t) * stride + channel, x[t]);
-}
-
-// Joins the warps' folds in order (from the last warp if `reverse`): returns
-// the map of what comes before the calling warp, and in `whole` the tile's.
-template <int V, bool reverse>
-__device__ __forceinline__ void join(const Affine (&mine)[V], Affine (&before)[V],
-                                     Affine (&whole)[V], Affine (*shared)[32 * V]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int t = 0; t < kTokens; ++t) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) shared[warp][v * 32 + lane] = mine[v];
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Affine sum = {1.0f, 0.0f};
-    before[v] = sum;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int at = reverse ? kWarps - 1 - w : w;
-      if (at == warp) before[v] = sum;
-      const Affine f = shared[at][v * 32 + lane];
-      sum = {f.a * sum.a, fmaf(f.a, sum.b, f.b)};
-    }
-    whole[v] = sum;
+    for (int v = 0; v < V; ++v) x[t][v] = missing;
+    if (t < at.count) load_pack<V>(q + t * stride, x[t]);
   }
+}
+constexpr float kShut = -INFINITY;  // a missing token's gate: the identity map
+
+// Joins the groups' maps in order (from the last group if `reverse`): one
+// thread a channel composes them, leaving in the group's place the map of all
+// before it, and returns the whole tile's (in the first kChannels threads).
+template <int V, bool reverse>
+__device__ __forceinline__ Affine join(Affine (*maps)[Place<V>::kChannels]) {
+  Affine sum = {1.0f, 0.0f};
+  __syncthreads();
+  if (threadIdx.x < Place<V>::kChannels) {
+    Affine f[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) f[g] = maps[g][threadIdx.x];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int at = reverse ? kGroups - 1 - g : g;
+      maps[at][threadIdx.x] = sum;
+      sum = then(sum, f[at]);
+    }
+  }
+  __syncthreads();
+  return sum;
 }
 
 // Folds every tile: forward the map of the state through it, backward the map
-// of the message through it (from its end to its start).
+// of the message through it (from its end to its start). h + a (x - h) and
+// A - a A save forming k.
 template <class T, int V, bool kBackward>
-__global__ void __launch_bounds__(kThreads) fold_kernel(gs_gated_scan_args a, Affine* folds) {
+__global__ void __launch_bounds__(Place<V>::kThreads) fold_kernel(gs_gated_scan_args a,
+                                                                  Affine* folds) {
   chain_wait();
-  __shared__ Affine s_fold[kWarps][32 * V];
+  __shared__ Affine s_maps[kGroups][Place<V>::kChannels];
   const Place<V> p(a, false);
   float x[kTokens][V], gate[kTokens][V];
-  load_tokens<T, V>(static_cast<const T*>(a.gate), a.gate_stride, p.first, p.channel, p.count, gate);
-  load_tokens<T, V>(static_cast<const T*>(kBackward ? a.grad_y : a.x),
-                    kBackward ? int64_t{a.channels} : a.x_stride, p.first, p.channel, p.count, x);
-  Affine mine[V], before[V], whole[V];
+  load_tokens<T>(a.gate, a.gate_stride, p, kShut, gate);
+  if constexpr (kBackward) load_tokens<T>(a.grad_y, a.channels, p, 0.0f, x);
+  else load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    mine[v] = {1.0f, 0.0f};
+    Affine f = {1.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
       const int t = kBackward ? kTokens - 1 - i : i;
-      if (t < p.count) {
-        float al, k;
-        open_gate(gate[t][v], al, k);
-        mine[v].b = kBackward ? k * (x[t][v] + mine[v].b) : fmaf(k, mine[v].b, al * x[t][v]);
-        mine[v].a *= k;
+      float e;
+      const float al = open_gate(gate[t][v], e);
+      if constexpr (kBackward) {
+        const float l = x[t][v] + f.b;
+        f.b = fmaf(-al, l, l);
+      } else {
+        f.b = fmaf(al, x[t][v] - f.b, f.b);
       }
+      f.a = fmaf(-al, f.a, f.a);
     }
+    s_maps[p.group][threadIdx.x % Place<V>::kLanes * V + v] = f;
   }
-  join<V, kBackward>(mine, before, whole, s_fold);
-  if (threadIdx.x < 32 && p.live)
-#pragma unroll
-    for (int v = 0; v < V; ++v) folds[p.index * a.channels + p.channel + v] = whole[v];
+  const Affine whole = join<V, kBackward>(s_maps);
+  const int channel = p.channel / Place<V>::kChannels * Place<V>::kChannels + threadIdx.x;
+  if (threadIdx.x < Place<V>::kChannels && channel < a.channels)
+    folds[p.index * a.channels + channel] = whole;
 }
 
-// The states (backward: messages) that enter the tiles, one block a sequence
-// and 32 channels: each warp folds its share of the sequence's tiles, the
-// shares are joined in order, each warp walks its share again.
-template <bool kBackward>
-__global__ void __launch_bounds__(32 * kScanWarps) tile_scan_kernel(gs_gated_scan_args a,
-                                                                    const Affine* folds,
-                                                                    float* entering) {
+// The states (backward: messages) that enter the tiles, a block a sequence and
+// kChannels channels: each of kScanThreads / kChannels groups of threads folds
+// its share of the sequence's tiles, the shares are joined in order, each group
+// walks its share again.
+template <bool kBackward, int kChannels>
+__global__ void __launch_bounds__(kScanThreads) tile_scan_kernel(gs_gated_scan_args a,
+                                                                 const Affine* folds,
+                                                                 float* entering) {
   chain_wait();
-  __shared__ Affine s_fold[kScanWarps][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int columns = (a.channels + 31) / 32;
+  constexpr int kShares = kScanThreads / kChannels;
+  __shared__ Affine s_fold[kShares][kChannels];
+  const int lane = threadIdx.x % kChannels, part = threadIdx.x / kChannels;
+  const int columns = (a.channels + kChannels - 1) / kChannels;
   const int64_t sequence = blockIdx.x / columns;
-  const int channel = static_cast<int>(blockIdx.x % columns) * 32 + lane;
+  const int channel = static_cast<int>(blockIdx.x % columns) * kChannels + lane;
   const bool live = channel < a.channels;
   const int64_t begin = a.tile_starts ? __ldg(a.tile_starts + sequence) : 0;
   const int64_t end = a.tile_starts ? __ldg(a.tile_starts + sequence + 1) : a.num_tiles;
-  const int64_t share = (end - begin + kScanWarps - 1) / kScanWarps;
-  const int64_t from = min(end, begin + warp * share), to = min(end, from + share);
+  const int64_t share = (end - begin + kShares - 1) / kShares;
+  const int64_t from = min(end, begin + part * share), to = min(end, from + share);
   const auto tile_of = [&](int64_t i) { return kBackward ? begin + end - 1 - i : i; };
   Affine sum = {1.0f, 0.0f};
   if (live)
-#pragma unroll 4
-    for (int64_t i = from; i < to; ++i) {
-      const Affine f = folds[tile_of(i) * a.channels + channel];
-      sum = {f.a * sum.a, fmaf(f.a, sum.b, f.b)};
+#pragma unroll 8
+    for (int64_t i = from; i < to; ++i) sum = then(sum, folds[tile_of(i) * a.channels + channel]);
+  s_fold[part][lane] = sum;
+  __syncthreads();
+  const int64_t slot = sequence * a.channels + channel;
+  if (part == 0 && live) {
+    // The state that enters each share takes the place of its map.
+    const float* start = kBackward ? a.grad_last : a.initial;
+    float state = start ? start[slot] : 0.0f;
+#pragma unroll 8
+    for (int w = 0; w < kShares; ++w) {
+      const Affine f = s_fold[w][lane];
+      s_fold[w][lane].b = state;
+      state = fmaf(f.a, state, f.b);
     }
-  s_fold[warp][lane] = sum;
+    float* final = kBackward ? a.grad_initial : a.last;
+    if (final) final[slot] = state;
+  }
   __syncthreads();
   if (!live) return;
-  const int64_t slot = sequence * a.channels + channel;
-  const float* start = kBackward ? a.grad_last : a.initial;
-  float state = start ? start[slot] : 0.0f;
-  for (int w = 0; w < warp; ++w) state = fmaf(s_fold[w][lane].a, state, s_fold[w][lane].b);
-#pragma unroll 4
+  float state = s_fold[part][lane].b;
+#pragma unroll 8
   for (int64_t i = from; i < to; ++i) {
     const int64_t at = tile_of(i) * a.channels + channel;
     const Affine f = folds[at];
     entering[at] = state;
     state = fmaf(f.a, state, f.b);
   }
-  float* final = kBackward ? a.grad_initial : a.last;
-  if (warp == kScanWarps - 1 && final) final[slot] = state;
 }
 
 // The walk from the entering states. Tiles go from the last to the first: the
 // fold just before read them from the first to the last, so the end of its
 // inputs is what L2 still holds.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) walk_kernel(gs_gated_scan_args a) {
+__global__ void __launch_bounds__(Place<V>::kThreads) walk_kernel(gs_gated_scan_args a) {
   chain_wait();
-  __shared__ Affine s_fold[kWarps][32 * V];
+  __shared__ Affine s_maps[kGroups][Place<V>::kChannels];
   const Place<V> p(a, true);
-  float x[kTokens][V], gate[kTokens][V];
-  load_tokens<T, V>(static_cast<const T*>(a.gate), a.gate_stride, p.first, p.channel, p.count, gate);
-  load_tokens<T, V>(static_cast<const T*>(a.x), a.x_stride, p.first, p.channel, p.count, x);
-  Affine mine[V], before[V], whole[V];
+  float x[kTokens][V], gate[kTokens][V], state[V];
+  load_tokens<T>(a.gate, a.gate_stride, p, kShut, gate);
+  load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
+  if (p.live) load_pack<V>(a.entering + p.index * a.channels + p.channel, state);
+  const int lane = threadIdx.x % Place<V>::kLanes * V;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    mine[v] = {1.0f, 0.0f};
+    Affine f = {1.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t)
-      if (t < p.count) {
-        float al;
-        open_gate(gate[t][v], al, gate[t][v]);
-        x[t][v] *= al;
-        mine[v] = {mine[v].a * gate[t][v], fmaf(gate[t][v], mine[v].b, x[t][v])};
-      }
+    for (int t = 0; t < kTokens; ++t) {
+      float e;
+      gate[t][v] = open_gate(gate[t][v], e);
+      f.b = fmaf(gate[t][v], x[t][v] - f.b, f.b);
+      f.a = fmaf(-gate[t][v], f.a, f.a);
+    }
+    s_maps[p.group][lane + v] = f;
   }
-  join<V, false>(mine, before, whole, s_fold);
+  join<V, false>(s_maps);
   if (!p.live) return;
-  float state[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    state[v] = fmaf(before[v].a, a.entering[p.index * a.channels + p.channel + v], before[v].b);
-  T* y = static_cast<T*>(a.y);
+  for (int v = 0; v < V; ++v) {
+    const Affine f = s_maps[p.group][lane + v];
+    state[v] = fmaf(f.a, state[v], f.b);
+  }
+  T* y = static_cast<T*>(a.y) + int64_t{p.first} * a.channels + p.channel;
 #pragma unroll
   for (int t = 0; t < kTokens; ++t)
     if (t < p.count) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) state[v] = fmaf(gate[t][v], state[v], x[t][v]);
-      store_pack<V>(y + int64_t{p.first + t} * a.channels + p.channel, state);
+      for (int v = 0; v < V; ++v) state[v] = fmaf(gate[t][v], x[t][v] - state[v], state[v]);
+      store_pack<V>(y + int64_t{t} * a.channels, state);
     }
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) walk_back_kernel(gs_gated_scan_args a,
-                                                             const float* messages) {
+__global__ void __launch_bounds__(Place<V>::kThreads) walk_back_kernel(gs_gated_scan_args a,
+                                                                       const float* messages) {
   chain_wait();
-  __shared__ Affine s_fold[2][kWarps][32 * V];
+  __shared__ Affine s_ahead[kGroups][Place<V>::kChannels], s_back[kGroups][Place<V>::kChannels];
   const Place<V> p(a, true);
-  float x[kTokens][V], gate[kTokens][V], g[kTokens][V], open[kTokens][V];
-  load_tokens<T, V>(static_cast<const T*>(a.gate), a.gate_stride, p.first, p.channel, p.count, gate);
-  load_tokens<T, V>(static_cast<const T*>(a.x), a.x_stride, p.first, p.channel, p.count, x);
-  load_tokens<T, V>(static_cast<const T*>(a.grad_y), int64_t{a.channels}, p.first, p.channel,
-                    p.count, g);
-  Affine ahead[V], back[V], before[V], after[V], whole[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    ahead[v] = back[v] = {1.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t)
-      if (t < p.count) {
-        open_gate(gate[t][v], open[t][v], gate[t][v]);
-        ahead[v].b = fmaf(gate[t][v], ahead[v].b, open[t][v] * x[t][v]);
-        ahead[v].a *= gate[t][v];
-      }
-#pragma unroll
-    for (int t = kTokens - 1; t >= 0; --t)
-      if (t < p.count) back[v].b = gate[t][v] * (g[t][v] + back[v].b);
-    back[v].a = ahead[v].a;
+  float x[kTokens][V], al[kTokens][V], g[kTokens][V], keep[kTokens][V], state[V], message[V];
+  load_tokens<T>(a.gate, a.gate_stride, p, kShut, al);
+  load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
+  load_tokens<T>(a.grad_y, a.channels, p, 0.0f, g);
+  if (p.live) {
+    load_pack<V>(a.entering + p.index * a.channels + p.channel, state);
+    load_pack<V>(messages + p.index * a.channels + p.channel, message);
   }
-  join<V, false>(ahead, before, whole, s_fold[0]);
-  join<V, true>(back, after, whole, s_fold[1]);
-  if (!p.live) return;
-  const int64_t slot = p.index * a.channels + p.channel;
+  const int lane = threadIdx.x % Place<V>::kLanes * V;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float state = fmaf(before[v].a, a.entering[slot + v], before[v].b);
-    float message = fmaf(after[v].a, messages[slot + v], after[v].b);
+    Affine ahead = {1.0f, 0.0f}, back = {1.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      float e;
+      al[t][v] = open_gate(al[t][v], e);
+      keep[t][v] = e * al[t][v];
+      ahead.b = fmaf(al[t][v], x[t][v] - ahead.b, ahead.b);
+      ahead.a *= keep[t][v];
+    }
+#pragma unroll
+    for (int t = kTokens - 1; t >= 0; --t) back.b = keep[t][v] * (g[t][v] + back.b);
+    back.a = ahead.a;
+    s_ahead[p.group][lane + v] = ahead;
+    s_back[p.group][lane + v] = back;
+  }
+  join<V, false>(s_ahead);
+  join<V, true>(s_back);
+  if (!p.live) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const Affine ahead = s_ahead[p.group][lane + v], back = s_back[p.group][lane + v];
+    float h = fmaf(ahead.a, state[v], ahead.b);
+    float u = fmaf(back.a, message[v], back.b);
     // forward: x_t becomes x_t - h_{t-1}
 #pragma unroll
-    for (int t = 0; t < kTokens; ++t)
-      if (t < p.count) {
-        const float push = open[t][v] * x[t][v];
-        x[t][v] -= state;
-        state = fmaf(gate[t][v], state, push);
-      }
+    for (int t = 0; t < kTokens; ++t) {
+      x[t][v] -= h;
+      h = fmaf(al[t][v], x[t][v], h);
+    }
     // back: x_t becomes dgate_t and g_t becomes dx_t
 #pragma unroll
-    for (int t = kTokens - 1; t >= 0; --t)
-      if (t < p.count) {
-        const float l = g[t][v] + message;
-        message = gate[t][v] * l;
-        g[t][v] = open[t][v] * l;
-        x[t][v] *= message * open[t][v];
-      }
+    for (int t = kTokens - 1; t >= 0; --t) {
+      const float l = g[t][v] + u;
+      u = keep[t][v] * l;
+      g[t][v] = al[t][v] * l;
+      x[t][v] *= u * al[t][v];
+    }
   }
-  T* grad_x = static_cast<T*>(a.grad_x);
-  T* grad_gate = static_cast<T*>(a.grad_gate);
+  const int64_t at = int64_t{p.first} * a.channels + p.channel;
+  T* grad_x = static_cast<T*>(a.grad_x) + at;
+  T* grad_gate = static_cast<T*>(a.grad_gate) + at;
 #pragma unroll
   for (int t = 0; t < kTokens; ++t)
     if (t < p.count) {
-      const int64_t at = int64_t{p.first + t} * a.channels + p.channel;
-      store_pack<V>(grad_x + at, g[t]);
-      store_pack<V>(grad_gate + at, x[t]);
+      store_pack<V>(grad_x + int64_t{t} * a.channels, g[t]);
+      store_pack<V>(grad_gate + int64_t{t} * a.channels, x[t]);
     }
 }
 
@@ -296,9 +325,9 @@ __global__ void __launch_bounds__(256) scan_step_kernel(int64_t count, int chann
   if (i >= count) return;
   const int64_t row = i / channels;
   const int c = static_cast<int>(i - row * channels);
-  float al, k;
-  open_gate(to_float(gate[row * gate_stride + c]), al, k);
-  const float h = fmaf(k, state[i], al * to_float(x[row * x_stride + c]));
+  float e;
+  const float al = open_gate(to_float(gate[row * gate_stride + c]), e);
+  const float h = fmaf(al, to_float(x[row * x_stride + c]) - state[i], state[i]);
   state[i] = h;
   y[i] = from_float<T>(h);
 }
@@ -312,7 +341,7 @@ int32_t check_args(const gs_gated_scan_args& a) {
                        a.num_tiles != (a.tokens + kTile - 1) / kTile))
     return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.tiles, 16)) return GS_ERR_MISALIGNED;
-  const int64_t columns = (int64_t{a.channels} + 31) / 32;
+  const int64_t columns = (int64_t{a.channels} + 7) / 8;
   if (columns * (a.num_tiles > a.sequences ? a.num_tiles : a.sequences) > INT32_MAX)
     return GS_ERR_CAPACITY;
   if (a.num_tiles > 0 && (!a.x || !a.gate || !a.entering || !a.workspace))
@@ -322,28 +351,45 @@ int32_t check_args(const gs_gated_scan_args& a) {
   return GS_OK;
 }
 
-// Two 16-bit channels a lane make a warp's row of a tile a full 128-byte line;
-// they need even strides and 4-byte aligned arrays. Otherwise one channel a lane.
+// Four channels a thread (8 or 16 bytes a load) need rows and arrays aligned to
+// them; otherwise one.
 template <class T>
-bool two_channels(const gs_gated_scan_args& a) {
-  if (sizeof(T) == 4 || a.channels % 2 || a.x_stride % 2 || a.gate_stride % 2) return false;
+bool four_channels(const gs_gated_scan_args& a) {
+  if (a.channels % 4 || a.x_stride % 4 || a.gate_stride % 4) return false;
   for (const void* p : {a.x, a.gate, a.grad_y, static_cast<const void*>(a.y),
                         static_cast<const void*>(a.grad_x), static_cast<const void*>(a.grad_gate)})
-    if (!is_aligned(p, 4)) return false;
-  return true;
+    if (!is_aligned(p, 4 * sizeof(T))) return false;
+  return is_aligned(a.entering, 16) && is_aligned(a.workspace, 16);
+}
+
+template <bool kBackward>
+int32_t scan_tiles(const gs_gated_scan_args& a, const Affine* folds, float* entering,
+                   cudaStream_t stream) {
+  // Long sequences: fewer channels a block, so that more threads share the
+  // tiles (7813 tiles of 64 channels: 2 blocks of 32 channels took 116 us).
+  const bool narrow = a.num_tiles / a.sequences > 256;
+  const unsigned blocks =
+      ceil_div(a.channels, narrow ? 8 : 32) * static_cast<unsigned>(a.sequences);
+  if (narrow)
+    launch_chained(tile_scan_kernel<kBackward, 8>, blocks, kScanThreads, stream, a, folds,
+                   entering);
+  else
+    launch_chained(tile_scan_kernel<kBackward, 32>, blocks, kScanThreads, stream, a, folds,
+                   entering);
+  return check_launch();
 }
 
 template <class T, int V>
 int32_t forward(const gs_gated_scan_args& a, cudaStream_t stream) {
   Affine* folds = static_cast<Affine*>(a.workspace);
-  const unsigned blocks = ceil_div(a.channels, 32 * V) * static_cast<unsigned>(a.num_tiles);
-  const unsigned chains = ceil_div(a.channels, 32) * static_cast<unsigned>(a.sequences);
+  constexpr int kThreads = Place<V>::kThreads;
+  const unsigned blocks =
+      ceil_div(a.channels, Place<V>::kChannels) * static_cast<unsigned>(a.num_tiles);
   if (blocks) {
     launch_chained(fold_kernel<T, V, false>, blocks, kThreads, stream, a, folds);
     GS_TRY(check_launch());
   }
-  launch_chained(tile_scan_kernel<false>, chains, 32 * kScanWarps, stream, a, folds, a.entering);
-  GS_TRY(check_launch());
+  GS_TRY(scan_tiles<false>(a, folds, a.entering, stream));
   if (blocks) launch_chained(walk_kernel<T, V>, blocks, kThreads, stream, a);
   return check_launch();
 }
@@ -352,14 +398,14 @@ template <class T, int V>
 int32_t backward(const gs_gated_scan_args& a, cudaStream_t stream) {
   Affine* folds = static_cast<Affine*>(a.workspace);
   float* messages = reinterpret_cast<float*>(folds + a.num_tiles * a.channels);
-  const unsigned blocks = ceil_div(a.channels, 32 * V) * static_cast<unsigned>(a.num_tiles);
-  const unsigned chains = ceil_div(a.channels, 32) * static_cast<unsigned>(a.sequences);
+  constexpr int kThreads = Place<V>::kThreads;
+  const unsigned blocks =
+      ceil_div(a.channels, Place<V>::kChannels) * static_cast<unsigned>(a.num_tiles);
   if (blocks) {
     launch_chained(fold_kernel<T, V, true>, blocks, kThreads, stream, a, folds);
     GS_TRY(check_launch());
   }
-  launch_chained(tile_scan_kernel<true>, chains, 32 * kScanWarps, stream, a, folds, messages);
-  GS_TRY(check_launch());
+  GS_TRY(scan_tiles<true>(a, folds, messages, stream));
   if (blocks) launch_chained(walk_back_kernel<T, V>, blocks, kThreads, stream, a, messages);
   return check_launch();
 }
@@ -375,9 +421,7 @@ int32_t launch_gated_scan(const gs_gated_scan_args& a, cudaStream_t stream) {
   if (!a.last || (a.num_tiles > 0 && !a.y)) return GS_ERR_INVALID_ARGUMENT;
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2)
-      if (two_channels<T>(a)) return forward<T, 2>(a, stream);
-    return forward<T, 1>(a, stream);
+    return four_channels<T>(a) ? forward<T, 4>(a, stream) : forward<T, 1>(a, stream);
   });
 }
 
@@ -386,9 +430,7 @@ int32_t launch_gated_scan_backward(const gs_gated_scan_args& a, cudaStream_t str
   if (a.num_tiles > 0 && (!a.grad_y || !a.grad_x || !a.grad_gate)) return GS_ERR_INVALID_ARGUMENT;
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2)
-      if (two_channels<T>(a)) return backward<T, 2>(a, stream);
-    return backward<T, 1>(a, stream);
+    return four_channels<T>(a) ? backward<T, 4>(a, stream) : backward<T, 1>(a, stream);
   });
 }
 
