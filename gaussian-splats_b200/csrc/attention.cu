@@ -367,13 +367,12 @@ __global__ void __launch_bounds__(kTile + 32, kDim == 64 ? 4 : 2)
 
 template <class T, int kDim>
 int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
-  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
   CUtensorMap q, k, v;
-  GS_TRY(tc::encode_map(&q, kBf16, a.q, a.tokens, a.heads, a.dim, a.q_stride, a.q_head_stride,
+  GS_TRY(tc::encode_heads(&q, a.dtype, a.q, a.tokens, a.heads, a.dim, a.q_stride, a.q_head_stride,
                         kTile));
-  GS_TRY(tc::encode_map(&k, kBf16, a.k, a.tokens, a.kv_heads, a.dim, a.k_stride, a.k_head_stride,
+  GS_TRY(tc::encode_heads(&k, a.dtype, a.k, a.tokens, a.kv_heads, a.dim, a.k_stride, a.k_head_stride,
                         kKeys));
-  GS_TRY(tc::encode_map(&v, kBf16, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride, a.v_head_stride,
+  GS_TRY(tc::encode_heads(&v, a.dtype, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride, a.v_head_stride,
                         kKeys));
   constexpr size_t kShared = sizeof(ForwardShared<kDim>);
   GS_CUDA_TRY(cudaFuncSetAttribute(attention_kernel<T, kDim>,
@@ -917,16 +916,15 @@ int64_t chunk_slots(const gs_window_attention_args& a) {
 
 template <class T, int kDim>
 int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
-  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
   CUtensorMap rows[4], tiles[4];  // q, grad_out, k, v in boxes of 128 and of 64 rows
   for (int m = 0; m < 4; ++m) {
     const void* const base[4] = {a.q, a.grad_out, a.k, a.v};
     const int64_t stride[4] = {a.q_stride, int64_t{a.heads} * a.dim, a.k_stride, a.v_stride};
     const int64_t head_stride[4] = {a.q_head_stride, a.dim, a.k_head_stride, a.v_head_stride};
     const int64_t heads = m < 2 ? a.heads : a.kv_heads;
-    GS_TRY(tc::encode_map(&rows[m], kBf16, base[m], a.tokens, heads, a.dim, stride[m],
+    GS_TRY(tc::encode_heads(&rows[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
                           head_stride[m], kTile));
-    GS_TRY(tc::encode_map(&tiles[m], kBf16, base[m], a.tokens, heads, a.dim, stride[m],
+    GS_TRY(tc::encode_heads(&tiles[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
                           head_stride[m], kKeys));
   }
   float* delta = static_cast<float*>(a.workspace);
@@ -1079,16 +1077,7 @@ int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t 
   });
 }
 
-int32_t window_attention_status(cudaStream_t stream) {
-  uint32_t timeout = 0;
-  const uint32_t clear = 0;
-  GS_CUDA_TRY(cudaMemcpyFromSymbolAsync(&timeout, g_timeout, sizeof(timeout), 0,
-                                        cudaMemcpyDeviceToHost, stream));
-  GS_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &clear, sizeof(clear), 0,
-                                      cudaMemcpyHostToDevice, stream));
-  GS_CUDA_TRY(cudaStreamSynchronize(stream));
-  return timeout ? GS_ERR_TIMEOUT : GS_OK;
-}
+int32_t window_attention_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
 
 int32_t launch_window_attention_backward(const gs_window_attention_args& a, cudaStream_t stream) {
   GS_TRY(check_args(a));

@@ -37,7 +37,8 @@ int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_backward(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_step(int64_t, int32_t, int32_t, const void*, int64_t, const void*,
                                int64_t, float*, void*, cudaStream_t);
-uint64_t gated_scan_workspace_size(int64_t, int64_t);
+uint64_t gated_scan_workspace_size(const gs_gated_scan_args&);
+int32_t gated_scan_status(cudaStream_t);
 int32_t launch_rms_norm(const gs_rms_norm_args&, cudaStream_t);
 int32_t launch_rms_norm_backward(const gs_rms_norm_args&, cudaStream_t);
 uint64_t rms_norm_workspace_size(int64_t, int64_t);
@@ -543,10 +544,12 @@ int32_t gs_window_attention_status(gs_stream_t stream) {
 }
 
 uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args* a) {
-  return !a || a->num_tiles < 0 || a->channels < 1
+  return !a || a->num_tiles < 0 || a->channels < 1 || a->sequences < 1
              ? 0
-             : gs::gated_scan_workspace_size(a->num_tiles, a->channels);
+             : gs::gated_scan_workspace_size(*a);
 }
+
+int32_t gs_gated_scan_status(gs_stream_t stream) { return gs::gated_scan_status(as_cuda(stream)); }
 
 int32_t gs_gated_scan(const gs_gated_scan_args* args, gs_stream_t stream) {
   return args ? gs::launch_gated_scan(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;

@@ -11,9 +11,9 @@
 //
 // and u_1 is the gradient of the initial state. Both directions are chains of
 // maps s -> A s + B, which compose associatively, so the sequence is cut into
-// tiles of kTile tokens: one kernel folds each tile to its (A, B), one scans the
-// tiles of each sequence for the state that enters each tile, one walks the
-// tiles from those states. Inside a tile, each thread holds kTokens tokens of
+// tiles of kTile tokens and those into spans of a few tiles: one kernel folds each span to
+// its (A, B), one scans the spans of each sequence for the state that enters
+// each, one walks the spans from those states. Inside a tile, each thread holds kTokens tokens of
 // its channels in registers and the threads' folds are joined in order in
 // shared memory. Every order is fixed, so results repeat bit for bit.
 //
@@ -21,7 +21,9 @@
 // kept in float for the backward, which recomputes h from them instead of
 // reading the rounded y.
 
-#include "sequence.cuh"
+#include <algorithm>
+
+#include "tensorcore.cuh"
 
 namespace gs {
 
@@ -30,7 +32,8 @@ int32_t launch_gated_scan_backward(const gs_gated_scan_args& a, cudaStream_t str
 int32_t launch_gated_scan_step(int64_t batch, int32_t channels, int32_t dtype, const void* x,
                                int64_t x_stride, const void* gate, int64_t gate_stride,
                                float* state, void* y, cudaStream_t stream);
-uint64_t gated_scan_workspace_size(int64_t num_tiles, int64_t channels);
+uint64_t gated_scan_workspace_size(const gs_gated_scan_args& a);
+int32_t gated_scan_status(cudaStream_t stream);
 
 namespace {
 
@@ -56,111 +59,480 @@ __device__ __forceinline__ Affine then(Affine first, Affine second) {
   return {second.a * first.a, fmaf(second.a, first.b, second.b)};
 }
 
-// What a block works on: a tile of tokens and kLanes V channels, V to a thread;
-// kGroups threads of kTokens tokens each share a channel.
-template <int V>
+// Sequences are walked in spans of `length` tiles, one block and one composed
+// map a span. Sequence b's spans take the slots from floor(first tile of b /
+// length) + b on, which no two sequences share.
+struct Spans {
+  int length, slots;
+  __device__ __forceinline__ int64_t slot_of(int64_t first_tile, int64_t sequence) const {
+    return first_tile / length + sequence;
+  }
+};
+__device__ __forceinline__ int64_t first_tile_of(const gs_gated_scan_args& a, int64_t b) {
+  return a.tile_starts ? __ldg(a.tile_starts + b) : (b ? a.num_tiles : 0);
+}
+
+// What a block works on: a span's tiles and kChannels channels, V to a thread,
+// kLanes threads side by side; kGroups threads of kTokens tokens each share a
+// channel of a tile.
+template <int V, int kLanes>
 struct Place {
-  static constexpr int kLanes = V == 1 ? 32 : 16;
   static constexpr int kChannels = kLanes * V;
-  static constexpr int kThreads = kLanes * kGroups;
-  Tile tile;
-  int64_t index;     // of the tile
-  int channel;       // the thread's first
-  int group;
-  int first, count;  // the thread's tokens
-  bool live;         // the thread has channels
-  __device__ __forceinline__ Place(const gs_gated_scan_args& a, bool reverse) {
+  int64_t slot, tile;  // the span's slot, its first tile
+  int tiles;           // 0: the slot is empty
+  int row, end;        // the first tile's first row, the sequence's end
+  int block_channel;   // the block's first channel
+  __device__ __forceinline__ Place(const gs_gated_scan_args& a, const Spans& spans, bool reverse) {
     const int columns = (a.channels + kChannels - 1) / kChannels;
-    index = blockIdx.x / columns;
-    if (reverse) index = a.num_tiles - 1 - index;
-    channel = (static_cast<int>(blockIdx.x % columns) * kLanes + threadIdx.x % kLanes) * V;
-    live = channel < a.channels;
-    group = threadIdx.x / kLanes;
-    tile = tile_at(a.tiles, index, static_cast<int32_t>(a.tokens), kTile);
-    first = tile.start + group * kTokens;
-    count = live ? min(kTokens, min(tile.end, tile.start + kTile) - first) : 0;
+    slot = blockIdx.x / columns;
+    if (reverse) slot = spans.slots - 1 - slot;
+    block_channel = static_cast<int>(blockIdx.x % columns) * kChannels;
+    int64_t b = 0, above = a.tile_starts ? a.sequences : 1;
+    while (above - b > 1) {  // the last sequence whose slots start at or before this one
+      const int64_t middle = (b + above) / 2;
+      if (spans.slot_of(first_tile_of(a, middle), middle) <= slot) b = middle;
+      else above = middle;
+    }
+    const int64_t tile0 = first_tile_of(a, b), count = first_tile_of(a, b + 1) - tile0;
+    const int64_t offset = (slot - spans.slot_of(tile0, b)) * spans.length;
+    tile = tile0 + offset;
+    tiles = static_cast<int>(max(int64_t{0}, min(int64_t{spans.length}, count - offset)));
+    if (tiles > 0) {
+      const Tile t = tile_at(a.tiles, tile, static_cast<int32_t>(a.tokens), kTile);
+      row = t.start;
+      end = t.end;
+    }
+  }
+  __device__ __forceinline__ int lane() const { return threadIdx.x % kLanes; }
+  __device__ __forceinline__ int group() const { return threadIdx.x / kLanes; }
+  __device__ __forceinline__ int channel() const { return block_channel + lane() * V; }
+  // The thread's first row of the span's tile i, and how many rows it has there.
+  __device__ __forceinline__ int first(int i) const { return row + i * kTile + group() * kTokens; }
+  __device__ __forceinline__ int count(int i) const {
+    return max(0, min(kTokens, end - first(i)));
   }
 };
 
-// The thread's tokens of one array; what it does not have reads as `missing`.
-template <class T, int V>
-__device__ __forceinline__ void load_tokens(const void* p, int64_t stride, const Place<V>& at,
-                                            float missing, float (&x)[kTokens][V]) {
-  const T* q = static_cast<const T*>(p) + at.first * stride + at.channel;
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[t][v] = missing;
-    if (t < at.count) load_pack<V>(q + t * stride, x[t]);
-  }
-}
+// Where a block's tiles come from. With whole 16-byte words a row the tensor
+// memory accelerator copies boxes of 128 bytes of channels and a tile's rows to
+// shared memory, a tile ahead of the walk; a thread then reads 8 bytes a row.
+// (Loads straight to registers left a block waiting for most of its time:
+// 2.0 TB/s.) The other arrays are loaded a channel a thread.
+constexpr int kBoxBytes = 128 * kTile;
+constexpr int kStages = 2;
 constexpr float kShut = -INFINITY;  // a missing token's gate: the identity map
 
-// Joins the groups' maps in order (from the last group if `reverse`): one
-// thread a channel composes them, leaving in the group's place the map of all
-// before it, and returns the whole tile's (in the first kChannels threads).
-template <int V, bool reverse>
-__device__ __forceinline__ Affine join(Affine (*maps)[Place<V>::kChannels]) {
-  Affine sum = {1.0f, 0.0f};
-  __syncthreads();
-  if (threadIdx.x < Place<V>::kChannels) {
-    Affine f[kGroups];
+__device__ uint32_t g_timeout;  // a wait ran out: for gs_gated_scan_status
+
+template <int kArrays>
+struct Boxes {
+  alignas(128) unsigned char data[kStages][kArrays][kBoxBytes];
+  uint64_t full[kStages];
+};
+
+template <class T, int kArrays>
+struct BoxSource {
+  static constexpr int kLanes = 16, V = 8 / sizeof(T);
+  using At = Place<V, kLanes>;
+  Boxes<kArrays>& s;
+  const CUtensorMap* const maps;
+  const At& at;
+  bool backward, good = true;
+  __device__ __forceinline__ BoxSource(unsigned char* shared, const CUtensorMap* m, const At& p,
+                                       bool back)
+      : s(*reinterpret_cast<Boxes<kArrays>*>(shared)), maps(m), at(p), backward(back) {
+    if (threadIdx.x == 0) {
+      for (uint64_t& b : s.full) tc::barrier_init(tc::shared_address(&b), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      tc::fence_async_shared();
+      for (int step = 0; step < kStages && step < at.tiles; ++step) request(step);
+    }
+    __syncthreads();
+  }
+  // Step `step` of the walk works on the span's tile:
+  __device__ __forceinline__ int tile_of(int step) const {
+    return backward ? at.tiles - 1 - step : step;
+  }
+  __device__ __forceinline__ void request(int step) {
+    const uint32_t bar = tc::shared_address(&s.full[step % kStages]);
+    tc::barrier_expect(bar, kArrays * kBoxBytes);
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) f[g] = maps[g][threadIdx.x];
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int at = reverse ? kGroups - 1 - g : g;
-      maps[at][threadIdx.x] = sum;
-      sum = then(sum, f[at]);
+    for (int k = 0; k < kArrays; ++k)
+      tc::load_box(tc::shared_address(s.data[step % kStages][k]), maps + k, at.block_channel,
+                   at.row + tile_of(step) * kTile, bar);
+  }
+  __device__ __forceinline__ void wait(int step) {
+    good = good && tc::barrier_wait_warp(tc::shared_address(&s.full[step % kStages]),
+                                         (step / kStages) & 1);
+  }
+  // Called by all once every thread has read step `step` and a barrier has passed.
+  __device__ __forceinline__ void release(int step) {
+    if (threadIdx.x == 0 && step + kStages < at.tiles && good) {
+      tc::fence_async_shared();
+      request(step + kStages);
     }
   }
-  __syncthreads();
+  template <int kArray>
+  __device__ __forceinline__ void read(int step, int t, float missing, float (&x)[V]) const {
+    const int r = at.group() * kTokens + t;
+    load_pack<V>(reinterpret_cast<const T*>(s.data[step % kStages][kArray] + r * 128) +
+                     at.lane() * V,
+                 x);
+    if (t >= at.count(tile_of(step)))
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = missing;
+  }
+  // At the end: whether all waits came back; if not, copies still in flight land first.
+  __device__ __forceinline__ void finish() {
+    if (good) return;
+    for (uint64_t& b : s.full)
+      for (int parity = 0; parity < 2; ++parity)
+        tc::barrier_wait(tc::shared_address(&b), parity);
+    if (threadIdx.x == 0) atomicExch(&g_timeout, 1u);
+  }
+};
+
+// The same from global memory, a channel a thread.
+template <class T, int kArrays>
+struct PlainSource {
+  static constexpr int kLanes = 32, V = 1;
+  using At = Place<V, kLanes>;
+  const T* base[kArrays];
+  int64_t stride[kArrays];
+  const At& at;
+  bool backward;
+  static constexpr bool good = true;
+  const bool live;
+  __device__ __forceinline__ PlainSource(const gs_gated_scan_args& a, const void* const (&p)[kArrays],
+                                         const int64_t (&strides)[kArrays], const At& place,
+                                         bool back)
+      : at(place), backward(back), live(place.channel() < a.channels) {
+#pragma unroll
+    for (int k = 0; k < kArrays; ++k) {
+      base[k] = static_cast<const T*>(p[k]);
+      stride[k] = strides[k];
+    }
+  }
+  __device__ __forceinline__ int tile_of(int step) const {
+    return backward ? at.tiles - 1 - step : step;
+  }
+  __device__ __forceinline__ void wait(int) {}
+  __device__ __forceinline__ void release(int) {}
+  __device__ __forceinline__ void finish() {}
+  template <int kArray>
+  __device__ __forceinline__ void read(int step, int t, float missing, float (&x)[V]) const {
+    const int i = tile_of(step);
+    x[0] = live && t < at.count(i)
+               ? to_float(base[kArray][(at.first(i) + t) * stride[kArray] + at.channel()])
+               : missing;
+  }
+};
+
+// The thread that joins a channel's groups: composes their maps in order.
+template <int kChannels, bool kReverse>
+__device__ __forceinline__ Affine compose(const Affine (*maps)[kChannels], Affine sum) {
+  Affine f[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) f[g] = maps[kReverse ? kGroups - 1 - g : g][threadIdx.x];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) sum = then(sum, f[g]);
   return sum;
 }
-
-// Folds every tile: forward the map of the state through it, backward the map
-// of the message through it (from its end to its start). h + a (x - h) and
-// A - a A save forming k.
-template <class T, int V, bool kBackward>
-__global__ void __launch_bounds__(Place<V>::kThreads) fold_kernel(gs_gated_scan_args a,
-                                                                  Affine* folds) {
-  chain_wait();
-  __shared__ Affine s_maps[kGroups][Place<V>::kChannels];
-  const Place<V> p(a, false);
-  float x[kTokens][V], gate[kTokens][V];
-  load_tokens<T>(a.gate, a.gate_stride, p, kShut, gate);
-  if constexpr (kBackward) load_tokens<T>(a.grad_y, a.channels, p, 0.0f, x);
-  else load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
+// The same for a value that passes through them: what enters each group.
+template <int kChannels, bool kReverse>
+__device__ __forceinline__ float pass(const Affine (*maps)[kChannels], float (*entering)[kChannels],
+                                      float value) {
+  Affine f[kGroups];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Affine f = {1.0f, 0.0f};
+  for (int g = 0; g < kGroups; ++g) f[g] = maps[kReverse ? kGroups - 1 - g : g][threadIdx.x];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    entering[kReverse ? kGroups - 1 - g : g][threadIdx.x] = value;
+    value = fmaf(f[g].a, value, f[g].b);
+  }
+  return value;
+}
+
+// Folds every span: forward the map of the state through it, backward the map
+// of the message through it (from its end to its start). h + a (x - h) and
+// A - a A save forming k. Arrays: gate, and x or grad_y.
+template <class Source, bool kBackward>
+__device__ __forceinline__ void fold(const gs_gated_scan_args& a, const typename Source::At& at,
+                                     Source& source, Affine* folds) {
+  constexpr int V = Source::V, kChannels = Source::At::kChannels;
+  __shared__ Affine s_maps[kGroups][kChannels];
+  Affine span = {1.0f, 0.0f};
+  for (int step = 0; step < at.tiles; ++step) {
+    Affine f[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = {1.0f, 0.0f};
+    source.wait(step);
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
       const int t = kBackward ? kTokens - 1 - i : i;
-      float e;
-      const float al = open_gate(gate[t][v], e);
-      if constexpr (kBackward) {
-        const float l = x[t][v] + f.b;
-        f.b = fmaf(-al, l, l);
-      } else {
-        f.b = fmaf(al, x[t][v] - f.b, f.b);
+      float gate[V], x[V];
+      source.template read<0>(step, t, kShut, gate);
+      source.template read<1>(step, t, 0.0f, x);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float e;
+        const float al = open_gate(gate[v], e);
+        if constexpr (kBackward) {
+          const float l = x[v] + f[v].b;
+          f[v].b = fmaf(-al, l, l);
+        } else {
+          f[v].b = fmaf(al, x[v] - f[v].b, f[v].b);
+        }
+        f[v].a = fmaf(-al, f[v].a, f[v].a);
       }
-      f.a = fmaf(-al, f.a, f.a);
     }
-    s_maps[p.group][threadIdx.x % Place<V>::kLanes * V + v] = f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_maps[at.group()][at.lane() * V + v] = f[v];
+    __syncthreads();
+    source.release(step);
+    if (threadIdx.x < kChannels) span = compose<kChannels, kBackward>(s_maps, span);
+    __syncthreads();
   }
-  const Affine whole = join<V, kBackward>(s_maps);
-  const int channel = p.channel / Place<V>::kChannels * Place<V>::kChannels + threadIdx.x;
-  if (threadIdx.x < Place<V>::kChannels && channel < a.channels)
-    folds[p.index * a.channels + channel] = whole;
+  const int channel = at.block_channel + threadIdx.x;
+  if (threadIdx.x < kChannels && channel < a.channels)
+    folds[at.slot * a.channels + channel] = source.good ? span : Affine{NAN, NAN};
+  source.finish();
 }
 
-// The states (backward: messages) that enter the tiles, a block a sequence and
+// The walk from the entering states. Arrays: gate, x.
+template <class T, class Source>
+__device__ __forceinline__ void walk(const gs_gated_scan_args& a, const typename Source::At& at,
+                                     Source& source, const float* states) {
+  constexpr int V = Source::V, kChannels = Source::At::kChannels;
+  __shared__ Affine s_maps[kGroups][kChannels];
+  __shared__ float s_entering[kGroups][kChannels];
+  const int joined = at.block_channel + threadIdx.x;  // the channel that the thread joins
+  const bool joins = threadIdx.x < kChannels && joined < a.channels;
+  float carry = joins ? states[at.slot * a.channels + joined] : 0.0f;
+  T* y = static_cast<T*>(a.y) + at.channel();
+  const bool live = at.channel() < a.channels;
+  for (int step = 0; step < at.tiles; ++step) {
+    float x[kTokens][V], al[kTokens][V];
+    Affine f[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = {1.0f, 0.0f};
+    source.wait(step);
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      source.template read<0>(step, t, kShut, al[t]);
+      source.template read<1>(step, t, 0.0f, x[t]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float e;
+        al[t][v] = open_gate(al[t][v], e);
+        f[v].b = fmaf(al[t][v], x[t][v] - f[v].b, f[v].b);
+        f[v].a = fmaf(-al[t][v], f[v].a, f[v].a);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_maps[at.group()][at.lane() * V + v] = f[v];
+    __syncthreads();
+    source.release(step);
+    if (threadIdx.x < kChannels) {
+      if (!source.good) carry = NAN;
+      if (joins) a.entering[(at.tile + step) * a.channels + joined] = carry;
+      carry = pass<kChannels, false>(s_maps, s_entering, carry);
+    }
+    __syncthreads();
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = s_entering[at.group()][at.lane() * V + v];
+    const int first = at.first(step), count = live ? at.count(step) : 0;
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = fmaf(al[t][v], x[t][v] - h[v], h[v]);
+      if (t < count) store_pack<V>(y + int64_t{first + t} * a.channels, h);
+    }
+  }
+  source.finish();
+}
+
+// The walk back from the entering messages. Arrays: gate, x, grad_y.
+template <class T, class Source>
+__device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
+                                          const typename Source::At& at, Source& source,
+                                          const float* messages) {
+  constexpr int V = Source::V, kChannels = Source::At::kChannels;
+  __shared__ Affine s_ahead[kGroups][kChannels], s_back[kGroups][kChannels];
+  __shared__ float s_state[kGroups][kChannels], s_message[kGroups][kChannels];
+  const int joined = at.block_channel + threadIdx.x;
+  const bool joins = threadIdx.x < kChannels && joined < a.channels;
+  float carry = joins ? messages[at.slot * a.channels + joined] : 0.0f;
+  const bool live = at.channel() < a.channels;
+  for (int step = 0; step < at.tiles; ++step) {
+    const int i = at.tiles - 1 - step;
+    const float state = joins ? a.entering[(at.tile + i) * a.channels + joined] : 0.0f;
+    float x[kTokens][V], al[kTokens][V], keep[kTokens][V];
+    Affine ahead[V], back[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) ahead[v] = back[v] = {1.0f, 0.0f};
+    source.wait(step);
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      source.template read<0>(step, t, kShut, al[t]);
+      source.template read<1>(step, t, 0.0f, x[t]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float e;
+        al[t][v] = open_gate(al[t][v], e);
+        keep[t][v] = e * al[t][v];
+        ahead[v].b = fmaf(al[t][v], x[t][v] - ahead[v].b, ahead[v].b);
+        ahead[v].a *= keep[t][v];
+      }
+    }
+#pragma unroll
+    for (int t = kTokens - 1; t >= 0; --t) {
+      float g[V];
+      source.template read<2>(step, t, 0.0f, g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) back[v].b = keep[t][v] * (g[v] + back[v].b);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      back[v].a = ahead[v].a;
+      s_ahead[at.group()][at.lane() * V + v] = ahead[v];
+      s_back[at.group()][at.lane() * V + v] = back[v];
+    }
+    __syncthreads();
+    // The last step's gradients have been read for the second time by now.
+    if (step > 0) source.release(step - 1);
+    if (threadIdx.x < kChannels) {
+      if (!source.good) carry = NAN;
+      pass<kChannels, false>(s_ahead, s_state, state);
+      carry = pass<kChannels, true>(s_back, s_message, carry);
+    }
+    __syncthreads();
+    float h[V], u[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      h[v] = s_state[at.group()][at.lane() * V + v];
+      u[v] = s_message[at.group()][at.lane() * V + v];
+    }
+    const int count = live ? at.count(i) : 0;
+    const int64_t offset = int64_t{at.first(i)} * a.channels + at.channel();
+    T* grad_x = static_cast<T*>(a.grad_x) + offset;
+    T* grad_gate = static_cast<T*>(a.grad_gate) + offset;
+    // forward: x_t becomes x_t - h_{t-1}
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[t][v] -= h[v];
+        h[v] = fmaf(al[t][v], x[t][v], h[v]);
+      }
+    // back: g becomes dx_t and x_t becomes dgate_t
+#pragma unroll
+    for (int t = kTokens - 1; t >= 0; --t) {
+      float g[V];
+      source.template read<2>(step, t, 0.0f, g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float l = g[v] + u[v];
+        u[v] = keep[t][v] * l;
+        g[v] = al[t][v] * l;
+        x[t][v] *= u[v] * al[t][v];
+      }
+      if (t < count) {
+        store_pack<V>(grad_x + int64_t{t} * a.channels, g);
+        store_pack<V>(grad_gate + int64_t{t} * a.channels, x[t]);
+      }
+    }
+  }
+  source.finish();
+}
+
+struct Maps {
+  CUtensorMap gate, x, grad;
+};
+
+constexpr int kBoxThreads = 16 * kGroups, kPlainThreads = 32 * kGroups;
+
+template <class T, bool kBackward>
+__global__ void __launch_bounds__(kBoxThreads, 3)
+    fold_boxes_kernel(gs_gated_scan_args a, Spans spans, Affine* folds,
+                      const __grid_constant__ Maps maps) {
+  chain_wait();
+  extern __shared__ __align__(128) unsigned char s_boxes[];
+  using Source = BoxSource<T, 2>;
+  const typename Source::At at(a, spans, false);
+  if (at.tiles == 0) return;
+  Source source(s_boxes, &maps.gate, at, kBackward);
+  fold<Source, kBackward>(a, at, source, folds);
+}
+template <class T, bool kBackward>
+__global__ void __launch_bounds__(kPlainThreads)
+    fold_kernel(gs_gated_scan_args a, Spans spans, Affine* folds) {
+  chain_wait();
+  using Source = PlainSource<T, 2>;
+  const typename Source::At at(a, spans, false);
+  if (at.tiles == 0) return;
+  Source source(a, {a.gate, kBackward ? a.grad_y : a.x},
+                {a.gate_stride, kBackward ? int64_t{a.channels} : a.x_stride}, at, kBackward);
+  fold<Source, kBackward>(a, at, source, folds);
+}
+
+// Walks go over the spans from the last to the first: the fold just before
+// read them from the first to the last, so the end of its inputs is what L2
+// still holds.
+template <class T>
+__global__ void __launch_bounds__(kBoxThreads, 2)
+    walk_boxes_kernel(gs_gated_scan_args a, Spans spans, const float* states,
+                      const __grid_constant__ Maps maps) {
+  chain_wait();
+  extern __shared__ __align__(128) unsigned char s_boxes[];
+  using Source = BoxSource<T, 2>;
+  const typename Source::At at(a, spans, true);
+  if (at.tiles == 0) return;
+  Source source(s_boxes, &maps.gate, at, false);
+  walk<T>(a, at, source, states);
+}
+template <class T>
+__global__ void __launch_bounds__(kPlainThreads)
+    walk_kernel(gs_gated_scan_args a, Spans spans, const float* states) {
+  chain_wait();
+  using Source = PlainSource<T, 2>;
+  const typename Source::At at(a, spans, true);
+  if (at.tiles == 0) return;
+  Source source(a, {a.gate, a.x}, {a.gate_stride, a.x_stride}, at, false);
+  walk<T>(a, at, source, states);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kBoxThreads, 2)
+    walk_back_boxes_kernel(gs_gated_scan_args a, Spans spans, const float* messages,
+                           const __grid_constant__ Maps maps) {
+  chain_wait();
+  extern __shared__ __align__(128) unsigned char s_boxes[];
+  using Source = BoxSource<T, 3>;
+  const typename Source::At at(a, spans, true);
+  if (at.tiles == 0) return;
+  Source source(s_boxes, &maps.gate, at, true);
+  walk_back<T>(a, at, source, messages);
+}
+template <class T>
+__global__ void __launch_bounds__(kPlainThreads)
+    walk_back_kernel(gs_gated_scan_args a, Spans spans, const float* messages) {
+  chain_wait();
+  using Source = PlainSource<T, 3>;
+  const typename Source::At at(a, spans, true);
+  if (at.tiles == 0) return;
+  Source source(a, {a.gate, a.x, a.grad_y}, {a.gate_stride, a.x_stride, int64_t{a.channels}}, at,
+                true);
+  walk_back<T>(a, at, source, messages);
+}
+
+// The states (backward: messages) that enter the spans, a block a sequence and
 // kChannels channels: each of kScanThreads / kChannels groups of threads folds
-// its share of the sequence's tiles, the shares are joined in order, each group
+// its share of the sequence's spans, the shares are joined in order, each group
 // walks its share again.
 template <bool kBackward, int kChannels>
-__global__ void __launch_bounds__(kScanThreads) tile_scan_kernel(gs_gated_scan_args a,
+__global__ void __launch_bounds__(kScanThreads) span_scan_kernel(gs_gated_scan_args a, Spans spans,
                                                                  const Affine* folds,
                                                                  float* entering) {
   chain_wait();
@@ -171,15 +543,17 @@ __global__ void __launch_bounds__(kScanThreads) tile_scan_kernel(gs_gated_scan_a
   const int64_t sequence = blockIdx.x / columns;
   const int channel = static_cast<int>(blockIdx.x % columns) * kChannels + lane;
   const bool live = channel < a.channels;
-  const int64_t begin = a.tile_starts ? __ldg(a.tile_starts + sequence) : 0;
-  const int64_t end = a.tile_starts ? __ldg(a.tile_starts + sequence + 1) : a.num_tiles;
+  const int64_t tile0 = first_tile_of(a, sequence);
+  const int64_t tiles = first_tile_of(a, sequence + 1) - tile0;
+  const int64_t begin = spans.slot_of(tile0, sequence);
+  const int64_t end = begin + (tiles + spans.length - 1) / spans.length;
   const int64_t share = (end - begin + kShares - 1) / kShares;
   const int64_t from = min(end, begin + part * share), to = min(end, from + share);
-  const auto tile_of = [&](int64_t i) { return kBackward ? begin + end - 1 - i : i; };
+  const auto slot_of = [&](int64_t i) { return kBackward ? begin + end - 1 - i : i; };
   Affine sum = {1.0f, 0.0f};
   if (live)
 #pragma unroll 8
-    for (int64_t i = from; i < to; ++i) sum = then(sum, folds[tile_of(i) * a.channels + channel]);
+    for (int64_t i = from; i < to; ++i) sum = then(sum, folds[slot_of(i) * a.channels + channel]);
   s_fold[part][lane] = sum;
   __syncthreads();
   const int64_t slot = sequence * a.channels + channel;
@@ -201,119 +575,11 @@ __global__ void __launch_bounds__(kScanThreads) tile_scan_kernel(gs_gated_scan_a
   float state = s_fold[part][lane].b;
 #pragma unroll 8
   for (int64_t i = from; i < to; ++i) {
-    const int64_t at = tile_of(i) * a.channels + channel;
+    const int64_t at = slot_of(i) * a.channels + channel;
     const Affine f = folds[at];
     entering[at] = state;
     state = fmaf(f.a, state, f.b);
   }
-}
-
-// The walk from the entering states. Tiles go from the last to the first: the
-// fold just before read them from the first to the last, so the end of its
-// inputs is what L2 still holds.
-template <class T, int V>
-__global__ void __launch_bounds__(Place<V>::kThreads) walk_kernel(gs_gated_scan_args a) {
-  chain_wait();
-  __shared__ Affine s_maps[kGroups][Place<V>::kChannels];
-  const Place<V> p(a, true);
-  float x[kTokens][V], gate[kTokens][V], state[V];
-  load_tokens<T>(a.gate, a.gate_stride, p, kShut, gate);
-  load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
-  if (p.live) load_pack<V>(a.entering + p.index * a.channels + p.channel, state);
-  const int lane = threadIdx.x % Place<V>::kLanes * V;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Affine f = {1.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      float e;
-      gate[t][v] = open_gate(gate[t][v], e);
-      f.b = fmaf(gate[t][v], x[t][v] - f.b, f.b);
-      f.a = fmaf(-gate[t][v], f.a, f.a);
-    }
-    s_maps[p.group][lane + v] = f;
-  }
-  join<V, false>(s_maps);
-  if (!p.live) return;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const Affine f = s_maps[p.group][lane + v];
-    state[v] = fmaf(f.a, state[v], f.b);
-  }
-  T* y = static_cast<T*>(a.y) + int64_t{p.first} * a.channels + p.channel;
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t)
-    if (t < p.count) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) state[v] = fmaf(gate[t][v], x[t][v] - state[v], state[v]);
-      store_pack<V>(y + int64_t{t} * a.channels, state);
-    }
-}
-
-template <class T, int V>
-__global__ void __launch_bounds__(Place<V>::kThreads) walk_back_kernel(gs_gated_scan_args a,
-                                                                       const float* messages) {
-  chain_wait();
-  __shared__ Affine s_ahead[kGroups][Place<V>::kChannels], s_back[kGroups][Place<V>::kChannels];
-  const Place<V> p(a, true);
-  float x[kTokens][V], al[kTokens][V], g[kTokens][V], keep[kTokens][V], state[V], message[V];
-  load_tokens<T>(a.gate, a.gate_stride, p, kShut, al);
-  load_tokens<T>(a.x, a.x_stride, p, 0.0f, x);
-  load_tokens<T>(a.grad_y, a.channels, p, 0.0f, g);
-  if (p.live) {
-    load_pack<V>(a.entering + p.index * a.channels + p.channel, state);
-    load_pack<V>(messages + p.index * a.channels + p.channel, message);
-  }
-  const int lane = threadIdx.x % Place<V>::kLanes * V;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Affine ahead = {1.0f, 0.0f}, back = {1.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      float e;
-      al[t][v] = open_gate(al[t][v], e);
-      keep[t][v] = e * al[t][v];
-      ahead.b = fmaf(al[t][v], x[t][v] - ahead.b, ahead.b);
-      ahead.a *= keep[t][v];
-    }
-#pragma unroll
-    for (int t = kTokens - 1; t >= 0; --t) back.b = keep[t][v] * (g[t][v] + back.b);
-    back.a = ahead.a;
-    s_ahead[p.group][lane + v] = ahead;
-    s_back[p.group][lane + v] = back;
-  }
-  join<V, false>(s_ahead);
-  join<V, true>(s_back);
-  if (!p.live) return;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const Affine ahead = s_ahead[p.group][lane + v], back = s_back[p.group][lane + v];
-    float h = fmaf(ahead.a, state[v], ahead.b);
-    float u = fmaf(back.a, message[v], back.b);
-    // forward: x_t becomes x_t - h_{t-1}
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      x[t][v] -= h;
-      h = fmaf(al[t][v], x[t][v], h);
-    }
-    // back: x_t becomes dgate_t and g_t becomes dx_t
-#pragma unroll
-    for (int t = kTokens - 1; t >= 0; --t) {
-      const float l = g[t][v] + u;
-      u = keep[t][v] * l;
-      g[t][v] = al[t][v] * l;
-      x[t][v] *= u * al[t][v];
-    }
-  }
-  const int64_t at = int64_t{p.first} * a.channels + p.channel;
-  T* grad_x = static_cast<T*>(a.grad_x) + at;
-  T* grad_gate = static_cast<T*>(a.grad_gate) + at;
-#pragma unroll
-  for (int t = 0; t < kTokens; ++t)
-    if (t < p.count) {
-      store_pack<V>(grad_x + int64_t{t} * a.channels, g[t]);
-      store_pack<V>(grad_gate + int64_t{t} * a.channels, x[t]);
-    }
 }
 
 template <class T>
@@ -342,86 +608,155 @@ int32_t check_args(const gs_gated_scan_args& a) {
     return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.tiles, 16)) return GS_ERR_MISALIGNED;
   const int64_t columns = (int64_t{a.channels} + 7) / 8;
-  if (columns * (a.num_tiles > a.sequences ? a.num_tiles : a.sequences) > INT32_MAX)
-    return GS_ERR_CAPACITY;
+  if (columns * (a.num_tiles + a.sequences) > INT32_MAX) return GS_ERR_CAPACITY;
   if (a.num_tiles > 0 && (!a.x || !a.gate || !a.entering || !a.workspace))
     return GS_ERR_INVALID_ARGUMENT;
-  if (a.workspace_size < gated_scan_workspace_size(a.num_tiles, a.channels))
+  if (a.workspace_size < gated_scan_workspace_size(a))
     return GS_ERR_CAPACITY;
   return GS_OK;
 }
 
-// Four channels a thread (8 or 16 bytes a load) need rows and arrays aligned to
-// them; otherwise one.
+// Boxes need whole 16-byte words: arrays, rows and strides.
 template <class T>
-bool four_channels(const gs_gated_scan_args& a) {
-  if (a.channels % 4 || a.x_stride % 4 || a.gate_stride % 4) return false;
+bool whole_words(const gs_gated_scan_args& a) {
+  constexpr int kWord = 16 / sizeof(T);
+  if (a.channels % kWord || a.x_stride % kWord || a.gate_stride % kWord || a.x_stride <= 0 ||
+      a.gate_stride <= 0)
+    return false;
   for (const void* p : {a.x, a.gate, a.grad_y, static_cast<const void*>(a.y),
                         static_cast<const void*>(a.grad_x), static_cast<const void*>(a.grad_gate)})
-    if (!is_aligned(p, 4 * sizeof(T))) return false;
-  return is_aligned(a.entering, 16) && is_aligned(a.workspace, 16);
+    if (!is_aligned(p, 16)) return false;
+  return true;
+}
+
+int64_t slots_of(const gs_gated_scan_args& a, int64_t length) {
+  return a.num_tiles / length + (a.tile_starts ? a.sequences : 1);
+}
+
+// Long spans give a block a walk to load ahead in and leave few maps to scan;
+// but first every multiprocessor gets its blocks, several times over. At most
+// 8 tiles: longer ones gain nothing more.
+template <class T>
+Spans spans_of(const gs_gated_scan_args& a, bool boxes) {
+  const int64_t items = a.num_tiles * ceil_div(a.channels, boxes ? 128 / sizeof(T) : 32);
+  const int64_t length = std::clamp<int64_t>(items / (8 * kSmCount), 1, 8);
+  return {static_cast<int>(length), static_cast<int>(slots_of(a, length))};
 }
 
 template <bool kBackward>
-int32_t scan_tiles(const gs_gated_scan_args& a, const Affine* folds, float* entering,
-                   cudaStream_t stream) {
+int32_t scan_spans(const gs_gated_scan_args& a, const Spans& spans, const Affine* folds,
+                   float* entering, cudaStream_t stream) {
   // Long sequences: fewer channels a block, so that more threads share the
-  // tiles (7813 tiles of 64 channels: 2 blocks of 32 channels took 116 us).
-  const bool narrow = a.num_tiles / a.sequences > 256;
-  const unsigned blocks =
-      ceil_div(a.channels, narrow ? 8 : 32) * static_cast<unsigned>(a.sequences);
+  // spans.
+  const int64_t sequences = a.tile_starts ? a.sequences : 1;
+  const bool narrow = spans.slots / sequences > 128;
+  const unsigned blocks = ceil_div(a.channels, narrow ? 8 : 32) * static_cast<unsigned>(sequences);
   if (narrow)
-    launch_chained(tile_scan_kernel<kBackward, 8>, blocks, kScanThreads, stream, a, folds,
+    launch_chained(span_scan_kernel<kBackward, 8>, blocks, kScanThreads, stream, a, spans, folds,
                    entering);
   else
-    launch_chained(tile_scan_kernel<kBackward, 32>, blocks, kScanThreads, stream, a, folds,
+    launch_chained(span_scan_kernel<kBackward, 32>, blocks, kScanThreads, stream, a, spans, folds,
                    entering);
   return check_launch();
 }
 
-template <class T, int V>
+// The maps of the arrays that a pass loads: gate, then x and grad_y in the order
+// given (backward's fold: gate, grad_y).
+template <class T>
+int32_t encode_maps(const gs_gated_scan_args& a, bool grad_first, Maps* maps) {
+  GS_TRY(tc::encode_rows(&maps->gate, a.dtype, a.gate, a.tokens, a.channels, a.gate_stride, kTile));
+  GS_TRY(tc::encode_rows(grad_first ? &maps->grad : &maps->x, a.dtype, a.x, a.tokens, a.channels,
+                         a.x_stride, kTile));
+  if (a.grad_y)
+    GS_TRY(tc::encode_rows(grad_first ? &maps->x : &maps->grad, a.dtype, a.grad_y, a.tokens,
+                           a.channels, a.channels, kTile));
+  return GS_OK;
+}
+
+template <class Kernel>
+int32_t allow_shared(Kernel* kernel, size_t bytes) {
+  GS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(bytes)));
+  return GS_OK;
+}
+
+template <class T>
 int32_t forward(const gs_gated_scan_args& a, cudaStream_t stream) {
+  const bool boxes = whole_words<T>(a);
+  const Spans spans = spans_of<T>(a, boxes);
   Affine* folds = static_cast<Affine*>(a.workspace);
-  constexpr int kThreads = Place<V>::kThreads;
-  const unsigned blocks =
-      ceil_div(a.channels, Place<V>::kChannels) * static_cast<unsigned>(a.num_tiles);
-  if (blocks) {
-    launch_chained(fold_kernel<T, V, false>, blocks, kThreads, stream, a, folds);
-    GS_TRY(check_launch());
+  float* states = reinterpret_cast<float*>(folds + int64_t{spans.slots} * a.channels);
+  const unsigned blocks = a.num_tiles == 0 ? 0
+                                           : ceil_div(a.channels, boxes ? 128 / sizeof(T) : 32) *
+                                                 static_cast<unsigned>(spans.slots);
+  constexpr size_t kShared = sizeof(Boxes<2>);
+  Maps maps = {};
+  if (blocks && boxes) {
+    GS_TRY(encode_maps<T>(a, false, &maps));
+    GS_TRY(allow_shared(fold_boxes_kernel<T, false>, kShared));
+    GS_TRY(allow_shared(walk_boxes_kernel<T>, kShared));
+    launch_chained_shared(fold_boxes_kernel<T, false>, blocks, kBoxThreads, kShared, stream, a,
+                          spans, folds, maps);
+  } else if (blocks) {
+    launch_chained(fold_kernel<T, false>, blocks, kPlainThreads, stream, a, spans, folds);
   }
-  GS_TRY(scan_tiles<false>(a, folds, a.entering, stream));
-  if (blocks) launch_chained(walk_kernel<T, V>, blocks, kThreads, stream, a);
+  GS_TRY(check_launch());
+  GS_TRY(scan_spans<false>(a, spans, folds, states, stream));
+  if (blocks && boxes)
+    launch_chained_shared(walk_boxes_kernel<T>, blocks, kBoxThreads, kShared, stream, a, spans,
+                          states, maps);
+  else if (blocks)
+    launch_chained(walk_kernel<T>, blocks, kPlainThreads, stream, a, spans, states);
   return check_launch();
 }
 
-template <class T, int V>
+template <class T>
 int32_t backward(const gs_gated_scan_args& a, cudaStream_t stream) {
+  const bool boxes = whole_words<T>(a);
+  const Spans spans = spans_of<T>(a, boxes);
   Affine* folds = static_cast<Affine*>(a.workspace);
-  float* messages = reinterpret_cast<float*>(folds + a.num_tiles * a.channels);
-  constexpr int kThreads = Place<V>::kThreads;
-  const unsigned blocks =
-      ceil_div(a.channels, Place<V>::kChannels) * static_cast<unsigned>(a.num_tiles);
-  if (blocks) {
-    launch_chained(fold_kernel<T, V, true>, blocks, kThreads, stream, a, folds);
-    GS_TRY(check_launch());
+  float* messages = reinterpret_cast<float*>(folds + int64_t{spans.slots} * a.channels);
+  const unsigned blocks = a.num_tiles == 0 ? 0
+                                           : ceil_div(a.channels, boxes ? 128 / sizeof(T) : 32) *
+                                                 static_cast<unsigned>(spans.slots);
+  if (blocks && boxes) {
+    Maps maps = {};
+    GS_TRY(encode_maps<T>(a, true, &maps));
+    GS_TRY(allow_shared(fold_boxes_kernel<T, true>, sizeof(Boxes<2>)));
+    launch_chained_shared(fold_boxes_kernel<T, true>, blocks, kBoxThreads, sizeof(Boxes<2>),
+                          stream, a, spans, folds, maps);
+  } else if (blocks) {
+    launch_chained(fold_kernel<T, true>, blocks, kPlainThreads, stream, a, spans, folds);
   }
-  GS_TRY(scan_tiles<true>(a, folds, messages, stream));
-  if (blocks) launch_chained(walk_back_kernel<T, V>, blocks, kThreads, stream, a, messages);
+  GS_TRY(check_launch());
+  GS_TRY(scan_spans<true>(a, spans, folds, messages, stream));
+  if (blocks && boxes) {
+    Maps maps = {};
+    GS_TRY(encode_maps<T>(a, false, &maps));
+    GS_TRY(allow_shared(walk_back_boxes_kernel<T>, sizeof(Boxes<3>)));
+    launch_chained_shared(walk_back_boxes_kernel<T>, blocks, kBoxThreads, sizeof(Boxes<3>),
+                          stream, a, spans, messages, maps);
+  } else if (blocks) {
+    launch_chained(walk_back_kernel<T>, blocks, kPlainThreads, stream, a, spans, messages);
+  }
   return check_launch();
 }
 
 }  // namespace
 
-uint64_t gated_scan_workspace_size(int64_t num_tiles, int64_t channels) {
-  return (sizeof(Affine) + sizeof(float)) * static_cast<uint64_t>(num_tiles) * channels;
+// Maps and states of the spans, which are never more than with one tile each.
+uint64_t gated_scan_workspace_size(const gs_gated_scan_args& a) {
+  return (sizeof(Affine) + sizeof(float)) * static_cast<uint64_t>(slots_of(a, 1)) * a.channels;
 }
+
+int32_t gated_scan_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
 
 int32_t launch_gated_scan(const gs_gated_scan_args& a, cudaStream_t stream) {
   GS_TRY(check_args(a));
   if (!a.last || (a.num_tiles > 0 && !a.y)) return GS_ERR_INVALID_ARGUMENT;
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return four_channels<T>(a) ? forward<T, 4>(a, stream) : forward<T, 1>(a, stream);
+    return forward<T>(a, stream);
   });
 }
 
@@ -430,7 +765,7 @@ int32_t launch_gated_scan_backward(const gs_gated_scan_args& a, cudaStream_t str
   if (a.num_tiles > 0 && (!a.grad_y || !a.grad_x || !a.grad_gate)) return GS_ERR_INVALID_ARGUMENT;
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return four_channels<T>(a) ? backward<T, 4>(a, stream) : backward<T, 1>(a, stream);
+    return backward<T>(a, stream);
   });
 }
 

@@ -72,6 +72,18 @@ inline int32_t with_dtype(int32_t dtype, F&& f) {
   return GS_ERR_INVALID_ARGUMENT;
 }
 
+// Reads and clears the flag that a kernel sets when a bounded wait ran out.
+inline int32_t take_timeout(const uint32_t& flag, cudaStream_t stream) {
+  uint32_t value = 0;
+  const uint32_t clear = 0;
+  GS_CUDA_TRY(cudaMemcpyFromSymbolAsync(&value, flag, sizeof(value), 0, cudaMemcpyDeviceToHost,
+                                        stream));
+  GS_CUDA_TRY(cudaMemcpyToSymbolAsync(flag, &clear, sizeof(clear), 0, cudaMemcpyHostToDevice,
+                                      stream));
+  GS_CUDA_TRY(cudaStreamSynchronize(stream));
+  return value ? GS_ERR_TIMEOUT : GS_OK;
+}
+
 // One tile of a packed batch: rows [start, min(start + tile, end)) of the
 // sequence that occupies rows [begin, end). A batch of one sequence needs no
 // table: its tiles follow from the row count.

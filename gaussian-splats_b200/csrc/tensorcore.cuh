@@ -69,6 +69,16 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// Loads the box at (x, row) of a [row, channel] array.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int row,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+      : "memory");
+}
+
 // ------------------------------------------------------------- tensor memory
 
 // Tensor memory is addressed as lane << 16 | column, 128 lanes of 512 32-bit
@@ -215,36 +225,32 @@ __device__ __forceinline__ uint32_t pack2(float low, float high) {
 
 // ---------------------------------------------------------------------- host
 
-// The map of a [tokens, heads, dim] array of 16-bit elements for boxes of 64
-// channels and `rows` tokens of one head. Channels from `dim` up to the box's
-// end and tokens outside the array read as zeros.
-inline int32_t encode_map(CUtensorMap* map, bool bf16, const void* base, int64_t tokens,
-                          int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride,
-                          int rows) {
+// Encodes the map of an array of `axes` axes (innermost first, contiguous;
+// strides in bytes from the second axis on) for boxes of `box`; what lies
+// outside the array reads as zeros.
+inline int32_t encode(CUtensorMap* map, int32_t dtype, const void* base, int axes,
+                      const cuuint64_t* size, const cuuint64_t* stride, const cuuint32_t* box,
+                      CUtensorMapSwizzle swizzle) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                               const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = nullptr;
-  if (!encode) {
+  static Encode call = nullptr;
+  if (!call) {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
     GS_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
     if (found != cudaDriverEntryPointSuccess || !f) return GS_ERR_UNSUPPORTED;
-    encode = reinterpret_cast<Encode>(f);
+    call = reinterpret_cast<Encode>(f);
   }
-  const cuuint64_t size[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
-                              static_cast<cuuint64_t>(tokens)};
-  const cuuint64_t stride[2] = {static_cast<cuuint64_t>(head_stride) * 2,
-                                static_cast<cuuint64_t>(token_stride) * 2};
-  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  const CUtensorMapDataType type = dtype == GS_FLOAT32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == GS_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t step[3] = {1, 1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
-    const CUresult r = encode(
-        map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-        const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = call(map, type, axes, const_cast<void*>(base), size, stride, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r == CUDA_SUCCESS) return GS_OK;
     if (r != CUDA_ERROR_INVALID_CONTEXT) break;
     // A thread that has made no runtime call yet (an autograd worker) has no
@@ -254,6 +260,30 @@ inline int32_t encode_map(CUtensorMap* map, bool bf16, const void* base, int64_t
     GS_CUDA_TRY(cudaSetDevice(device));
   }
   return GS_ERR_INVALID_ARGUMENT;
+}
+
+// A [tokens, heads, dim] array of 16-bit elements in boxes of 64 channels and
+// `rows` tokens of one head, swizzled as the products read them.
+inline int32_t encode_heads(CUtensorMap* map, int32_t dtype, const void* base, int64_t tokens,
+                            int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride,
+                            int rows) {
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t stride[2] = {static_cast<cuuint64_t>(head_stride) * 2,
+                                static_cast<cuuint64_t>(token_stride) * 2};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  return encode(map, dtype, base, 3, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// A [rows, channels] array in boxes of 128 bytes of channels and `box_rows` rows.
+inline int32_t encode_rows(CUtensorMap* map, int32_t dtype, const void* base, int64_t rows,
+                           int64_t channels, int64_t row_stride, int box_rows) {
+  const int64_t element = element_size(dtype);
+  const cuuint64_t size[2] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t stride[1] = {static_cast<cuuint64_t>(row_stride * element)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / element),
+                             static_cast<cuuint32_t>(box_rows)};
+  return encode(map, dtype, base, 2, size, stride, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace tc

@@ -73,6 +73,7 @@ EXPORTED_SYMBOLS = (
     "gs_window_attention_workspace_size",
     "gs_gated_scan",
     "gs_gated_scan_backward",
+    "gs_gated_scan_status",
     "gs_gated_scan_step",
     "gs_gated_scan_workspace_size",
     "gs_rms_norm",
@@ -335,6 +336,7 @@ def lib() -> ctypes.CDLL:
         "gs_window_attention_workspace_size": ([ctypes.POINTER(WindowAttentionArgs)], u64),
         "gs_gated_scan": ([ctypes.POINTER(GatedScanArgs), vp], i32),
         "gs_gated_scan_backward": ([ctypes.POINTER(GatedScanArgs), vp], i32),
+        "gs_gated_scan_status": ([vp], i32),
         "gs_gated_scan_step": ([i64, i32, i32, vp, i64, vp, i64, vp, vp, vp], i32),
         "gs_gated_scan_workspace_size": ([ctypes.POINTER(GatedScanArgs)], u64),
         "gs_rms_norm": ([ctypes.POINTER(RmsNormArgs), vp], i32),

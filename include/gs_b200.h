@@ -583,6 +583,8 @@ typedef struct gs_gated_scan_args {
 uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args *args);
 int32_t gs_gated_scan(const gs_gated_scan_args *args, gs_stream_t stream);
 int32_t gs_gated_scan_backward(const gs_gated_scan_args *args, gs_stream_t stream);
+/* As gs_window_attention_status, for the recurrence (NaN from the span on). */
+int32_t gs_gated_scan_status(gs_stream_t stream);
 
 /* One step of the recurrence: state [batch, channels] float is updated in
  * place, y [batch, channels] receives it in the type of x. */
