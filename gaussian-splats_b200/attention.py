@@ -25,8 +25,8 @@ import math
 import torch
 
 from . import native
-from .sequences import (PackedSequences, address, check_cuda, check_packed, current_stream,
-                        element_type, tile_arguments)
+from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
+                        tile_arguments)
 
 MAX_HEAD_DIM = 128
 _TYPES = (torch.bfloat16, torch.float16)
@@ -87,10 +87,7 @@ class _WindowAttention(torch.autograd.Function):
                           **tile_arguments(packed, tokens), heads=heads, kv_heads=k.shape[1], dim=dim, dtype=dtype,
                           left=left, right=right, first=first, scale=scale, valid=address(valid),
                           out=out.data_ptr(), lse=address(lse))
-        with torch.cuda.device(q.device):
-            native.check(native.lib().gs_window_attention(ctypes.byref(args),
-                                                          current_stream(q.device)),
-                         "gs_window_attention")
+        call("gs_window_attention", q.device, ctypes.byref(args))
         if need_grad:
             ctx.save_for_backward(q, k, v, out, lse, valid)
             ctx.packed, ctx.args = packed, args  # sizes, strides, the layout's table
@@ -113,10 +110,7 @@ class _WindowAttention(torch.autograd.Function):
         args.grad_out, args.grad_q = grad_out.data_ptr(), grad_q.data_ptr()
         args.grad_k, args.grad_v = grad_k.data_ptr(), grad_v.data_ptr()
         args.workspace, args.workspace_size = workspace.data_ptr(), size
-        with torch.cuda.device(q.device):
-            native.check(lib.gs_window_attention_backward(ctypes.byref(args),
-                                                          current_stream(q.device)),
-                         "gs_window_attention_backward")
+        call("gs_window_attention_backward", q.device, ctypes.byref(args))
         return (grad_q, grad_k, grad_v) + (None,) * 8
 
 
@@ -179,7 +173,6 @@ def window_cache(batch: int, left: int, first: int, kv_heads: int, dim: int,
             torch.zeros(shape, dtype=dtype, device=device))
 
 
-@torch.no_grad()
 def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           cache_k: torch.Tensor, cache_v: torch.Tensor, positions: torch.Tensor,
                           *, first: int = 0, scale: float | None = None) -> torch.Tensor:
@@ -226,8 +219,5 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       scale=_scale(what, scale, dim), cache_k=cache_k.data_ptr(),
                       cache_v=cache_v.data_ptr(), positions=positions.data_ptr(),
                       out=out.data_ptr())
-    with torch.cuda.device(device):
-        native.check(native.lib().gs_window_attention_step(ctypes.byref(args),
-                                                           current_stream(device)),
-                     "gs_window_attention_step")
+    call("gs_window_attention_step", device, ctypes.byref(args))
     return out

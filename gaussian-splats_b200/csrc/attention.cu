@@ -32,22 +32,7 @@ uint64_t window_attention_workspace_size(const gs_window_attention_args& a);
 namespace {
 
 constexpr int kTile = GS_SEQUENCE_TILE;  // queries (or keys) of a block
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 128;
-constexpr int kWords = kMaxDim / 32;  // channels of a row that a lane sums
-
-template <class T>
-__device__ __forceinline__ float dot(const float* a, const T* b, int dim) {
-  float s = 0.0f;
-  for (int c = 0; c < dim; c += 8) {
-    float x[8];
-    load_pack<8>(b + c, x);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s = fmaf(a[c + k], x[k], s);
-  }
-  return s;
-}
 
 // -------------------------------------------------- whole sequences, forward
 //
@@ -955,74 +940,299 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   return check_launch();
 }
 
-// One new token a stream against its cache of `slots` tokens: the first
-// `first` tokens keep their slots, later ones take the others in turn. The new
-// token's key and value come from the arguments; the block of a key-value
-// head's first query head also writes them to their slot, which no block reads.
+// ------------------------------------------------- one new token a stream
+//
+// The cache is read once: that is the bound. A cluster of blocks shares the
+// slots of a stream and key-value head, a warp takes 16 slots at a time for up
+// to 16 query heads (more: more clusters), and everything that it reads comes
+// straight to registers in the shape of the warp's matrix products:
+//
+//   scores [heads x slots] = q K^T: a lane's 16 bytes of a key row are its
+//     parts of two products, with q's channels permuted alike;
+//   out [heads x dim] += P V: a lane's 16 bytes of two value rows, interleaved,
+//     are its parts of eight products, one channel of eight to each; the scores'
+//     places in the registers are the ones that P needs.
+//
+// The warps' maxima, sums and outputs are joined in order, in the block and then
+// across the cluster through distributed shared memory: one launch, no
+// workspace, no atomics.
+
+constexpr int kStepWarps = 4;
+constexpr int kStepThreads = 32 * kStepWarps;
+constexpr int kStepSlots = 16;  // a warp's slots at a time
+constexpr int kStepHeads = 16;  // query heads of a cluster
+
 template <class T>
-__global__ void __launch_bounds__(kThreads) attention_step_kernel(gs_window_attention_step_args a) {
+__device__ __forceinline__ void warp_product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// A float at the same place of another block's shared memory.
+__device__ __forceinline__ float read_block(const float* p, uint32_t rank) {
+  uint32_t there;
+  float x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(there)
+               : "r"(tc::shared_address(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(there) : "memory");
+  return x;
+}
+
+template <class T, int kDim>
+__global__ void __launch_bounds__(kStepThreads, 3)
+    attention_step_kernel(gs_window_attention_step_args a) {
   chain_wait();
-  __shared__ float s_row[kMaxDim], s_acc[kWarps][kMaxDim], s_top[kWarps], s_sum[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t b = blockIdx.x;
-  const int head = blockIdx.y, group = a.heads / a.kv_heads, kv_head = head / group;
+  constexpr int kChunks = kDim / 32;  // of a key row, two products each
+  constexpr int kParts = kDim / 64;   // of a value row, eight products each
+  __shared__ float s_out[kStepWarps][kStepHeads][kDim];
+  __shared__ float s_top[kStepWarps][kStepHeads], s_sum[kStepWarps][kStepHeads];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  const uint32_t rank = cluster_rank(), blocks = cluster_size();
+  const int group = a.heads / a.kv_heads, pieces = (group + kStepHeads - 1) / kStepHeads;
+  const int64_t item = blockIdx.x / blocks;
+  const int piece = static_cast<int>(item % pieces);
+  const int kv_head = static_cast<int>(item / pieces % a.kv_heads);
+  const int64_t b = item / pieces / a.kv_heads;
+  const int head0 = kv_head * group + piece * kStepHeads;
+  const int heads = min(kStepHeads, group - piece * kStepHeads);
   const int64_t position = a.positions[b];
-  T* out = static_cast<T*>(a.out) + (b * a.heads + head) * a.dim;
-  if (position < 0) {
-    for (int c = threadIdx.x; c < a.dim; c += kThreads) out[c] = from_float<T>(0.0f);
-    return;
-  }
-  const int64_t slot = position < a.first
-                           ? position
-                           : a.first + (position - a.first) % (a.slots - a.first);
-  const int count = static_cast<int>(min(position + 1, int64_t{a.slots}));
+  const bool idle = position < 0;
+  const int64_t slot = idle                 ? -1
+                       : position < a.first ? position
+                                            : a.first + (position - a.first) % (a.slots - a.first);
+  const int count = idle ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
   const int64_t row = int64_t{a.kv_heads} * a.dim;
   T* cache_k = static_cast<T*>(a.cache_k) + b * a.slots * row + kv_head * a.dim;
   T* cache_v = static_cast<T*>(a.cache_v) + b * a.slots * row + kv_head * a.dim;
   const T* k = static_cast<const T*>(a.k) + b * a.k_stride + kv_head * a.k_head_stride;
   const T* v = static_cast<const T*>(a.v) + b * a.v_stride + kv_head * a.v_head_stride;
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride + head * a.q_head_stride;
-  if (head % group == 0)
-    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+  // The new token's slot is read by nobody: its rows come from the arguments.
+  if (!idle && rank == 0 && piece == 0)
+    for (int c = threadIdx.x; c < a.dim; c += kStepThreads) {
       cache_k[slot * row + c] = k[c];
       cache_v[slot * row + c] = v[c];
     }
-  for (int c = threadIdx.x; c < a.dim; c += kThreads) s_row[c] = to_float(q[c]);
-  __syncthreads();
-  float top = -INFINITY, sum = 0.0f, acc[kWords] = {};
-  for (int base = 32 * warp; base < count; base += kThreads) {
-    const bool in = base + lane < count;
-    float s = -INFINITY;
-    if (in) s = dot(s_row, base + lane == slot ? k : cache_k + (base + lane) * row, a.dim) * a.scale;
-    const float next = fmaxf(top, warp_max(s));
-    const float p = in ? expf(s - next) : 0.0f, shrink = expf(top - next);
-    top = next;
-    sum = fmaf(sum, shrink, warp_sum(p));
+
+  // q's rows g and g + 8, in the order of the key rows' products.
+  uint32_t q[kChunks][2][4];
 #pragma unroll
-    for (int c = 0; c < kWords; ++c) acc[c] *= shrink;
-    for (int l = 0; l < min(32, count - base); ++l) {
-      const float w = __shfl_sync(0xffffffffu, p, l);
-      const T* value = base + l == slot ? v : cache_v + (base + l) * row;
+  for (int c = 0; c < kChunks; ++c) {
+    uint4 word[2] = {};
 #pragma unroll
-      for (int c = 0; c < kWords; ++c)
-        if (lane + 32 * c < a.dim) acc[c] = fmaf(w, to_float(value[lane + 32 * c]), acc[c]);
+    for (int r = 0; r < 2; ++r)
+      if (g + 8 * r < heads && 32 * c + 8 * j < a.dim)
+        word[r] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride +
+                                                  (head0 + g + 8 * r) * a.q_head_stride + 32 * c +
+                                                  8 * j);
+    q[c][0][0] = word[0].x; q[c][0][1] = word[1].x; q[c][0][2] = word[0].y; q[c][0][3] = word[1].y;
+    q[c][1][0] = word[0].z; q[c][1][1] = word[1].z; q[c][1][2] = word[0].w; q[c][1][3] = word[1].w;
+  }
+  const float scale = a.scale * kLog2e;
+  float out[kParts][8][4] = {};
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  for (int base = (static_cast<int>(rank) * kStepWarps + warp) * kStepSlots; base < count;
+       base += static_cast<int>(blocks) * kStepWarps * kStepSlots) {
+    // Keys base + g and base + 8 + g; values of the slots 2j, 2j+1, 2j+8, 2j+9.
+    uint4 key[2][kChunks], value[kParts][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int s = base + 8 * n + g;
+      const T* p = s == slot ? k : cache_k + s * row;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        key[n][c] = make_uint4(0, 0, 0, 0);
+        if (s < count && 32 * c + 8 * j < a.dim)
+          key[n][c] = *reinterpret_cast<const uint4*>(p + 32 * c + 8 * j);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int s = base + 2 * j + (n & 1) + 8 * (n >> 1);
+      const T* p = s == slot ? v : cache_v + s * row;
+#pragma unroll
+      for (int h = 0; h < kParts; ++h) {
+        value[h][n] = make_uint4(0, 0, 0, 0);
+        if (s < count && 64 * h + 8 * g < a.dim)
+          value[h][n] = *reinterpret_cast<const uint4*>(p + 64 * h + 8 * g);
+      }
+    }
+    float x[2][4] = {};  // scores of the slots 8n + 2j, 8n + 2j + 1 for rows g, g + 8
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        warp_product<T>(x[n], q[c][0], key[n][c].x, key[n][c].y);
+        warp_product<T>(x[n], q[c][1], key[n][c].z, key[n][c].w);
+      }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (base + 8 * n + 2 * j + (e & 1) >= count) x[n][e] = -INFINITY;
+    uint32_t p[4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float next = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
+      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 1));
+      next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 2)) * scale;
+      const bool grow = next > top[r] + kSlack || (top[r] == -INFINITY && next > top[r]);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float shrink = grow ? tc::exp2_approx(top[r] - next) : 1.0f;
+        if (grow) top[r] = next;
+        sum[r] *= shrink;
+#pragma unroll
+        for (int h = 0; h < kParts; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            out[h][i][2 * r] *= shrink;
+            out[h][i][2 * r + 1] *= shrink;
+          }
+      }
+      const float shift = top[r] == -INFINITY ? 0.0f : -top[r];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float p0 = tc::exp2_approx(fmaf(x[n][2 * r], scale, shift));
+        const float p1 = tc::exp2_approx(fmaf(x[n][2 * r + 1], scale, shift));
+        sum[r] += p0 + p1;
+        p[2 * n + r] = tc::pack2<T>(p0, p1);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) {
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&value[h][0]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&value[h][1]);
+      const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&value[h][2]);
+      const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&value[h][3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        warp_product<T>(out[h][2 * i], p, __byte_perm(v0[i], v1[i], 0x5410),
+                        __byte_perm(v8[i], v9[i], 0x5410));
+        warp_product<T>(out[h][2 * i + 1], p, __byte_perm(v0[i], v1[i], 0x7632),
+                        __byte_perm(v8[i], v9[i], 0x7632));
+      }
     }
   }
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_sum[warp] = sum;
-  }
+
+  // The warp's rows to shared memory: product i's column n is channel 8n + i of
+  // its part.
 #pragma unroll
-  for (int c = 0; c < kWords; ++c) s_acc[warp][lane + 32 * c] = acc[c];
-  __syncthreads();
-  float whole = -INFINITY, total = 0.0f;
-  for (int w = 0; w < kWarps; ++w) whole = fmaxf(whole, s_top[w]);
-  for (int w = 0; w < kWarps; ++w) total = fmaf(s_sum[w], expf(s_top[w] - whole), total);
-  for (int c = threadIdx.x; c < a.dim; c += kThreads) {
-    float o = 0.0f;
-    for (int w = 0; w < kWarps; ++w) o = fmaf(s_acc[w][c], expf(s_top[w] - whole), o);
-    out[c] = from_float<T>(o / total);
+  for (int r = 0; r < 2; ++r) {
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    if (j == 0) {
+      s_top[warp][g + 8 * r] = top[r];
+      s_sum[warp][g + 8 * r] = sum[r];
+    }
+#pragma unroll
+    for (int h = 0; h < kParts; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          s_out[warp][g + 8 * r][64 * h + 8 * (2 * j + e) + i] = out[h][i][2 * r + e];
   }
+  __syncthreads();
+  // The warps joined into the first one's place.
+  for (int c = threadIdx.x; c < heads * kDim; c += kStepThreads) {
+    const int h = c / kDim, d = c % kDim;
+    float whole = -INFINITY, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s_top[w][h]);
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w)
+      o = fmaf(s_out[w][h][d], tc::exp2_approx(s_top[w][h] - shift), o);
+    s_out[0][h][d] = o;
+  }
+  __syncthreads();
+  if (threadIdx.x < heads) {
+    const int h = threadIdx.x;
+    float whole = -INFINITY, total = 0.0f;
+    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s_top[w][h]);
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+    for (int w = 0; w < kStepWarps; ++w)
+      total = fmaf(s_sum[w][h], tc::exp2_approx(s_top[w][h] - shift), total);
+    s_top[0][h] = whole;
+    s_sum[0][h] = total;
+  }
+  cluster_sync();
+  // The blocks joined, each block a part of the outputs.
+  for (int c = static_cast<int>(rank) * kStepThreads + threadIdx.x; c < heads * kDim;
+       c += static_cast<int>(blocks) * kStepThreads) {
+    const int h = c / kDim, d = c % kDim;
+    float whole = -INFINITY, total = 0.0f, o = 0.0f;
+    for (uint32_t r = 0; r < blocks; ++r) whole = fmaxf(whole, read_block(&s_top[0][h], r));
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+    for (uint32_t r = 0; r < blocks; ++r) {
+      const float w = tc::exp2_approx(read_block(&s_top[0][h], r) - shift);
+      total = fmaf(read_block(&s_sum[0][h], r), w, total);
+      o = fmaf(read_block(&s_out[0][h][d], r), w, o);
+    }
+    if (d < a.dim)
+      static_cast<T*>(a.out)[(b * a.heads + head0 + h) * a.dim + d] =
+          from_float<T>(total == 0.0f ? 0.0f : o / total);
+  }
+  cluster_sync();  // the others have read this block's shared memory
+}
+
+// Blocks of a cluster: enough that every multiprocessor has several blocks, as
+// far as each warp still gets slots.
+int step_blocks(const gs_window_attention_step_args& a) {
+  const int64_t items =
+      a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, kStepHeads);
+  int blocks = 1;
+  while (blocks < 16 && items * blocks < 8 * kSmCount &&
+         2 * blocks * kStepWarps * kStepSlots <= a.slots)
+    blocks *= 2;
+  return blocks;
+}
+
+template <class T, int kDim>
+int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
+  const int blocks = step_blocks(a);
+  const int64_t grid = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, kStepHeads) * blocks;
+  if (grid > INT32_MAX) return GS_ERR_CAPACITY;
+  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim>,
+                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = static_cast<unsigned>(grid);
+  config.blockDim = kStepThreads;
+  config.stream = stream;
+  config.attrs = attr;
+  config.numAttrs = 2;
+  cudaLaunchKernelEx(&config, attention_step_kernel<T, kDim>, a);
+  return check_launch();
 }
 
 bool sixteen_bit(int32_t dtype) { return dtype == GS_BFLOAT16 || dtype == GS_FLOAT16; }
@@ -1111,8 +1321,7 @@ int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cud
     return GS_ERR_MISALIGNED;
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
-    launch_chained(attention_step_kernel<T>, dim3(a.batch, a.heads), kThreads, stream, a);
-    return check_launch();
+    return a.dim <= 64 ? step<T, 64>(a, stream) : step<T, 128>(a, stream);
   });
 }
 

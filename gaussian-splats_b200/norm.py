@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import native
-from .sequences import address, check_cuda, current_stream, element_type
+from .sequences import address, call, check_cuda, element_type
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -64,9 +64,7 @@ class _RmsNorm(torch.autograd.Function):
         y = torch.empty(shape, dtype=x.dtype, device=x.device)
         total = None if res is None else torch.empty(shape, dtype=res.dtype, device=x.device)
         args = _arguments(rows, weight, res, eps, y=y, sum=total)
-        with torch.cuda.device(x.device):
-            native.check(native.lib().gs_rms_norm(ctypes.byref(args), current_stream(x.device)),
-                         "gs_rms_norm")
+        call("gs_rms_norm", x.device, ctypes.byref(args))
         ctx.save_for_backward(rows if res is None else total, weight)
         ctx.eps, ctx.has_residual, ctx.x_dtype, ctx.shape = eps, res is not None, x.dtype, shape
         ctx.set_materialize_grads(False)
@@ -96,9 +94,7 @@ class _RmsNorm(torch.autograd.Function):
         size = lib.gs_rms_norm_workspace_size(ctypes.byref(args))
         workspace = torch.empty((size,), dtype=torch.uint8, device=z.device)
         args.workspace, args.workspace_size = address(workspace), size
-        with torch.cuda.device(z.device):
-            native.check(lib.gs_rms_norm_backward(ctypes.byref(args), current_stream(z.device)),
-                         "gs_rms_norm_backward")
+        call("gs_rms_norm_backward", z.device, ctypes.byref(args))
         if ctx.has_residual and grad_residual is None:
             grad_residual = grad_x
         return grad_x, grad_weight, grad_residual, None
@@ -119,7 +115,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     return _RmsNorm.apply(x, weight, residual, eps)
 
 
-@torch.no_grad()
 def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
                   eps: float = 1e-6):
     """:func:`rms_norm` with an 8-bit result: returns ``q`` (float8_e4m3fn, the
@@ -133,7 +128,5 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     total = None if res is None else torch.empty(x.shape, dtype=res.dtype, device=x.device)
     weight = weight.contiguous()
     args = _arguments(rows, weight, res, eps, q=q, scale=scale, sum=total)
-    with torch.cuda.device(x.device):
-        native.check(native.lib().gs_rms_norm(ctypes.byref(args), current_stream(x.device)),
-                     "gs_rms_norm")
+    call("gs_rms_norm", x.device, ctypes.byref(args))
     return (q, scale) if res is None else (q, scale, total)

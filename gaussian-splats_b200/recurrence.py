@@ -16,8 +16,8 @@ import ctypes
 import torch
 
 from . import native
-from .sequences import (PackedSequences, address, check_cuda, check_packed, current_stream,
-                        element_type, tile_arguments)
+from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
+                        tile_arguments)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -54,9 +54,7 @@ class _GatedScan(torch.autograd.Function):
         size = lib.gs_gated_scan_workspace_size(ctypes.byref(args))
         workspace = torch.empty((size,), dtype=torch.uint8, device=device)
         args.workspace, args.workspace_size = address(workspace), size
-        with torch.cuda.device(device):
-            native.check(lib.gs_gated_scan(ctypes.byref(args), current_stream(device)),
-                         "gs_gated_scan")
+        call("gs_gated_scan", device, ctypes.byref(args))
         ctx.save_for_backward(x, gate, entering)
         ctx.packed, ctx.args, ctx.size = packed, args, size
         ctx.has_initial = initial is not None
@@ -83,10 +81,7 @@ class _GatedScan(torch.autograd.Function):
         args.grad_y, args.grad_last = address(grad_y), address(grad_last)
         args.grad_x, args.grad_gate = address(grad_x), address(grad_gate)
         args.grad_initial, args.workspace = address(grad_initial), address(workspace)
-        with torch.cuda.device(device):
-            native.check(native.lib().gs_gated_scan_backward(ctypes.byref(args),
-                                                             current_stream(device)),
-                         "gs_gated_scan_backward")
+        call("gs_gated_scan_backward", device, ctypes.byref(args))
         return grad_x, grad_gate, grad_initial, None, None
 
 
@@ -117,7 +112,6 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, packed: PackedSequences | No
     return _GatedScan.apply(x, gate, initial, packed, dtype)
 
 
-@torch.no_grad()
 def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     """One step of each stream: updates ``state`` [batch, channels] float32 in
     place from ``x`` and ``gate`` [batch, channels] and returns it in the type of
@@ -131,8 +125,6 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
                          f"{'' if state.is_contiguous() else ' (not contiguous)'}")
     x, gate = _rows(x), _rows(gate)
     y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    with torch.cuda.device(device):
-        native.check(native.lib().gs_gated_scan_step(
-            x.shape[0], x.shape[1], dtype, address(x), x.stride(0), address(gate), gate.stride(0),
-            address(state), address(y), current_stream(device)), "gs_gated_scan_step")
+    call("gs_gated_scan_step", device, x.shape[0], x.shape[1], dtype, address(x), x.stride(0),
+         address(gate), gate.stride(0), address(state), address(y))
     return y

@@ -87,8 +87,18 @@ def element_type(dtype: torch.dtype, what: str, allowed=(torch.float32, torch.bf
     return _DTYPES[dtype]
 
 
-def current_stream(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def call(name: str, device: torch.device, *arguments) -> None:
+    """Calls a library function on the device's current stream; raises for a
+    status other than success."""
+    stream = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+    function = getattr(native.lib(), name)
+    if device.index == torch.cuda.current_device():
+        status = function(*arguments, stream)
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, stream)
+    if status:
+        native.check(status, name)
 
 
 def address(t: torch.Tensor | None) -> int | None:
