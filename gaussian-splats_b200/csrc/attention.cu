@@ -943,9 +943,11 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
 // ------------------------------------------------- one new token a stream
 //
 // The cache is read once: that is the bound. A cluster of blocks shares the
-// slots of a stream and key-value head, a warp takes 16 slots at a time for up
-// to 16 query heads (more: more clusters), and everything that it reads comes
-// straight to registers in the shape of the warp's matrix products:
+// slots of a stream and key-value head, up to 16 query heads (more: more
+// clusters). TMA brings tiles of 64 slots to shared memory some tiles ahead,
+// which keeps over 100 KB in flight a multiprocessor (loads straight to
+// registers, 12 warps: 4.3 TB/s); a warp takes 16 slots of each and reads
+// them in the shape of its matrix products:
 //
 //   scores [heads x slots] = q K^T: a lane's 16 bytes of a key row are its
 //     parts of two products, with q's channels permuted alike;
@@ -959,24 +961,60 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
 
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
-constexpr int kStepSlots = 16;  // a warp's slots at a time
-constexpr int kStepHeads = 16;  // query heads of a cluster
+constexpr int kStepSlots = 16;  // a warp's slots of a tile
+constexpr int kStepTile = kStepWarps * kStepSlots;
+constexpr int kStepStages = 3;
 
-template <class T>
-__device__ __forceinline__ void warp_product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+template <int kDim, int kHalves>
+struct StepShared {
+  static constexpr int kTileBytes = kStepTile * kDim * 2;
+  union {
+    struct {
+      alignas(1024) unsigned char k[kStepStages][kTileBytes];
+      unsigned char v[kStepStages][kTileBytes];
+    };
+    float out[kStepWarps][8 * kHalves][kDim];  // once the tiles are done
+  };
+  float top[kStepWarps][8 * kHalves], sum[kStepWarps][8 * kHalves];
+  uint64_t full[kStepStages], empty[kStepStages];
+};
+
+// Sixteen bytes, number `word`, of a row of a loaded tile.
+__device__ __forceinline__ uint4 tile_word(const unsigned char* tile, int row, int word) {
+  return *reinterpret_cast<const uint4*>(tile + (word >> 3) * (kStepTile * 128) + row * 128 +
+                                         (((word & 7) ^ (row & 7)) << 4));
+}
+
+// c += a b for kHalves halves of 8 rows; with one, the rows of the second are
+// zeros that need no registers.
+template <class T, int kHalves>
+__device__ __forceinline__ void warp_product(float (&half)[kHalves][2],
+                                             const uint32_t (&rows)[kHalves][2], uint32_t b0,
                                              uint32_t b1) {
+  float c[4] = {half[0][0], half[0][1], 0.0f, 0.0f};
+  uint32_t a[4] = {rows[0][0], 0, rows[0][1], 0};
+  if constexpr (kHalves == 2) {
+    c[2] = half[1][0]; c[3] = half[1][1];
+    a[1] = rows[1][0]; a[3] = rows[1][1];
+  }
   if constexpr (std::is_same_v<T, __nv_bfloat16>)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  half[0][0] = c[0];
+  half[0][1] = c[1];
+  if constexpr (kHalves == 2) {
+    half[1][0] = c[2];
+    half[1][1] = c[3];
+  }
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -1003,14 +1041,17 @@ __device__ __forceinline__ float read_block(const float* p, uint32_t rank) {
   return x;
 }
 
-template <class T, int kDim>
-__global__ void __launch_bounds__(kStepThreads, 3)
-    attention_step_kernel(gs_window_attention_step_args a) {
+template <class T, int kDim, int kHalves>
+__global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
+    attention_step_kernel(gs_window_attention_step_args a, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map) {
+  using Shared = StepShared<kDim, kHalves>;
+  extern __shared__ __align__(1024) unsigned char shared_bytes[];
+  Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   chain_wait();
   constexpr int kChunks = kDim / 32;  // of a key row, two products each
   constexpr int kParts = kDim / 64;   // of a value row, eight products each
-  __shared__ float s_out[kStepWarps][kStepHeads][kDim];
-  __shared__ float s_top[kStepWarps][kStepHeads], s_sum[kStepWarps][kStepHeads];
+  constexpr int kStepHeads = 8 * kHalves;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   const uint32_t rank = cluster_rank(), blocks = cluster_size();
   const int group = a.heads / a.kv_heads, pieces = (group + kStepHeads - 1) / kStepHeads;
@@ -1038,66 +1079,101 @@ __global__ void __launch_bounds__(kStepThreads, 3)
       cache_v[slot * row + c] = v[c];
     }
 
-  // q's rows g and g + 8, in the order of the key rows' products.
-  uint32_t q[kChunks][2][4];
+  // q's rows g (and g + 8), in the order of the key rows' products.
+  uint32_t q[kChunks][2][kHalves][2];
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    uint4 word[2] = {};
+  for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < kHalves; ++r) {
+      uint4 word = make_uint4(0, 0, 0, 0);
       if (g + 8 * r < heads && 32 * c + 8 * j < a.dim)
-        word[r] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride +
-                                                  (head0 + g + 8 * r) * a.q_head_stride + 32 * c +
-                                                  8 * j);
-    q[c][0][0] = word[0].x; q[c][0][1] = word[1].x; q[c][0][2] = word[0].y; q[c][0][3] = word[1].y;
-    q[c][1][0] = word[0].z; q[c][1][1] = word[1].z; q[c][1][2] = word[0].w; q[c][1][3] = word[1].w;
-  }
+        word = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride +
+                                               (head0 + g + 8 * r) * a.q_head_stride + 32 * c +
+                                               8 * j);
+      q[c][0][r][0] = word.x;
+      q[c][0][r][1] = word.y;
+      q[c][1][r][0] = word.z;
+      q[c][1][r][1] = word.w;
+    }
   const float scale = a.scale * kLog2e;
-  float out[kParts][8][4] = {};
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-  for (int base = (static_cast<int>(rank) * kStepWarps + warp) * kStepSlots; base < count;
-       base += static_cast<int>(blocks) * kStepWarps * kStepSlots) {
+  float out[kParts][8][kHalves][2] = {};
+  float top[kHalves], sum[kHalves] = {};
+#pragma unroll
+  for (int r = 0; r < kHalves; ++r) top[r] = -INFINITY;
+
+  // This block's tiles of the stream's slots: rank, rank + blocks, ...
+  const int tiles = max(0, ((count + kStepTile - 1) / kStepTile - static_cast<int>(rank) +
+                            static_cast<int>(blocks) - 1) /
+                               static_cast<int>(blocks));
+  const auto base_of = [&](int t) {
+    return (static_cast<int>(rank) + t * static_cast<int>(blocks)) * kStepTile;
+  };
+  const auto load_tile = [&](int t) {
+    const int stage = t % kStepStages;
+    const uint32_t bar = tc::shared_address(&s.full[stage]);
+    const int first = static_cast<int>(b * a.slots) + base_of(t);
+    tc::barrier_expect(bar, 2 * Shared::kTileBytes);
+    for (int x = 0; x < kDim / 64; ++x) {
+      tc::load_box(tc::shared_address(s.k[stage]) + x * kStepTile * 128, &k_map, 64 * x, kv_head,
+                   first, bar);
+      tc::load_box(tc::shared_address(s.v[stage]) + x * kStepTile * 128, &v_map, 64 * x, kv_head,
+                   first, bar);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStepStages; ++i) {
+      tc::barrier_init(tc::shared_address(&s.full[i]), 1);
+      tc::barrier_init(tc::shared_address(&s.empty[i]), kStepWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_async_shared();
+    for (int t = 0; t < kStepStages && t < tiles; ++t) load_tile(t);
+  }
+  __syncthreads();
+  bool good = true;
+  for (int t = 0; t < tiles; ++t) {
+    const int stage = t % kStepStages;
+    // The tile before last's stage gets its next tile once all warps are done
+    // with it, which by now they mostly are.
+    if (threadIdx.x == 0 && t >= 1 && t - 1 + kStepStages < tiles) {
+      good = good && tc::barrier_wait(tc::shared_address(&s.empty[(t - 1) % kStepStages]),
+                                      ((t - 1) / kStepStages) & 1);
+      if (good) load_tile(t - 1 + kStepStages);
+    }
+    good = tc::barrier_wait_warp(tc::shared_address(&s.full[stage]), (t / kStepStages) & 1) && good;
+    const int row0 = warp * kStepSlots, base = base_of(t) + row0;
     // Keys base + g and base + 8 + g; values of the slots 2j, 2j+1, 2j+8, 2j+9.
-    uint4 key[2][kChunks], value[kParts][4];
+    uint4 key[2][kChunks];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int s = base + 8 * n + g;
-      const T* p = s == slot ? k : cache_k + s * row;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        key[n][c] = make_uint4(0, 0, 0, 0);
-        if (s < count && 32 * c + 8 * j < a.dim)
-          key[n][c] = *reinterpret_cast<const uint4*>(p + 32 * c + 8 * j);
-      }
+      for (int c = 0; c < kChunks; ++c) key[n][c] = tile_word(s.k[stage], row0 + 8 * n + g, 4 * c + j);
+      if (base + 8 * n + g == slot)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          key[n][c] = 32 * c + 8 * j < a.dim
+                          ? *reinterpret_cast<const uint4*>(k + 32 * c + 8 * j)
+                          : make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int s = base + 2 * j + (n & 1) + 8 * (n >> 1);
-      const T* p = s == slot ? v : cache_v + s * row;
-#pragma unroll
-      for (int h = 0; h < kParts; ++h) {
-        value[h][n] = make_uint4(0, 0, 0, 0);
-        if (s < count && 64 * h + 8 * g < a.dim)
-          value[h][n] = *reinterpret_cast<const uint4*>(p + 64 * h + 8 * g);
-      }
-    }
-    float x[2][4] = {};  // scores of the slots 8n + 2j, 8n + 2j + 1 for rows g, g + 8
+    float x[2][kHalves][2] = {};  // scores of the slots 8n + 2j, 8n + 2j + 1
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        warp_product<T>(x[n], q[c][0], key[n][c].x, key[n][c].y);
-        warp_product<T>(x[n], q[c][1], key[n][c].z, key[n][c].w);
+        warp_product<T, kHalves>(x[n], q[c][0], key[n][c].x, key[n][c].y);
+        warp_product<T, kHalves>(x[n], q[c][1], key[n][c].z, key[n][c].w);
       }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (base + 8 * n + 2 * j + (e & 1) >= count) x[n][e] = -INFINITY;
-    uint32_t p[4];
+      for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float next = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
+        for (int e = 0; e < 2; ++e)
+          if (base + 8 * n + 2 * j + e >= count) x[n][r][e] = -INFINITY;
+    uint32_t p[kHalves][2];
+#pragma unroll
+    for (int r = 0; r < kHalves; ++r) {
+      float next = fmaxf(fmaxf(x[0][r][0], x[0][r][1]), fmaxf(x[1][r][0], x[1][r][1]));
       next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 1));
       next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 2)) * scale;
       const bool grow = next > top[r] + kSlack || (top[r] == -INFINITY && next > top[r]);
@@ -1109,44 +1185,64 @@ __global__ void __launch_bounds__(kStepThreads, 3)
         for (int h = 0; h < kParts; ++h)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            out[h][i][2 * r] *= shrink;
-            out[h][i][2 * r + 1] *= shrink;
+            out[h][i][r][0] *= shrink;
+            out[h][i][r][1] *= shrink;
           }
       }
       const float shift = top[r] == -INFINITY ? 0.0f : -top[r];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const float p0 = tc::exp2_approx(fmaf(x[n][2 * r], scale, shift));
-        const float p1 = tc::exp2_approx(fmaf(x[n][2 * r + 1], scale, shift));
+        const float p0 = tc::exp2_approx(fmaf(x[n][r][0], scale, shift));
+        const float p1 = tc::exp2_approx(fmaf(x[n][r][1], scale, shift));
         sum[r] += p0 + p1;
-        p[2 * n + r] = tc::pack2<T>(p0, p1);
+        p[r][n] = tc::pack2<T>(p0, p1);
       }
     }
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&value[h][0]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&value[h][1]);
-      const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&value[h][2]);
-      const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&value[h][3]);
+      uint4 value[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int r = 2 * j + (n & 1) + 8 * (n >> 1);
+        value[n] = tile_word(s.v[stage], row0 + r, 8 * h + g);
+        // What an empty slot holds must not meet its weight of zero.
+        if (base + r == slot && 64 * h + 8 * g < a.dim)
+          value[n] = *reinterpret_cast<const uint4*>(v + 64 * h + 8 * g);
+        if (base + r >= count) value[n] = make_uint4(0, 0, 0, 0);
+      }
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&value[0]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&value[1]);
+      const uint32_t* v8 = reinterpret_cast<const uint32_t*>(&value[2]);
+      const uint32_t* v9 = reinterpret_cast<const uint32_t*>(&value[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        warp_product<T>(out[h][2 * i], p, __byte_perm(v0[i], v1[i], 0x5410),
-                        __byte_perm(v8[i], v9[i], 0x5410));
-        warp_product<T>(out[h][2 * i + 1], p, __byte_perm(v0[i], v1[i], 0x7632),
-                        __byte_perm(v8[i], v9[i], 0x7632));
+        warp_product<T, kHalves>(out[h][2 * i], p, __byte_perm(v0[i], v1[i], 0x5410),
+                                 __byte_perm(v8[i], v9[i], 0x5410));
+        warp_product<T, kHalves>(out[h][2 * i + 1], p, __byte_perm(v0[i], v1[i], 0x7632),
+                                 __byte_perm(v8[i], v9[i], 0x7632));
       }
     }
+    __syncwarp();
+    if (lane == 0) tc::barrier_arrive(tc::shared_address(&s.empty[stage]));
   }
+  if (!good) {  // let what is in flight land, and show that the result is not valid
+    for (uint64_t& bar : s.full)
+      for (int parity = 0; parity < 2; ++parity)
+        tc::barrier_wait(tc::shared_address(&bar), parity);
+    for (float& x : sum) x = NAN;
+    if (lane == 0) atomicExch(&g_timeout, 1u);
+  }
+  __syncthreads();  // the tiles' place is free for the outputs
 
   // The warp's rows to shared memory: product i's column n is channel 8n + i of
   // its part.
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
+  for (int r = 0; r < kHalves; ++r) {
     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
     if (j == 0) {
-      s_top[warp][g + 8 * r] = top[r];
-      s_sum[warp][g + 8 * r] = sum[r];
+      s.top[warp][g + 8 * r] = top[r];
+      s.sum[warp][g + 8 * r] = sum[r];
     }
 #pragma unroll
     for (int h = 0; h < kParts; ++h)
@@ -1154,7 +1250,7 @@ __global__ void __launch_bounds__(kStepThreads, 3)
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          s_out[warp][g + 8 * r][64 * h + 8 * (2 * j + e) + i] = out[h][i][2 * r + e];
+          s.out[warp][g + 8 * r][64 * h + 8 * (2 * j + e) + i] = out[h][i][r][e];
   }
   __syncthreads();
   // The warps joined into the first one's place.
@@ -1162,23 +1258,23 @@ __global__ void __launch_bounds__(kStepThreads, 3)
     const int h = c / kDim, d = c % kDim;
     float whole = -INFINITY, o = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s_top[w][h]);
+    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
     const float shift = whole == -INFINITY ? 0.0f : whole;
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w)
-      o = fmaf(s_out[w][h][d], tc::exp2_approx(s_top[w][h] - shift), o);
-    s_out[0][h][d] = o;
+      o = fmaf(s.out[w][h][d], tc::exp2_approx(s.top[w][h] - shift), o);
+    s.out[0][h][d] = o;
   }
   __syncthreads();
   if (threadIdx.x < heads) {
     const int h = threadIdx.x;
     float whole = -INFINITY, total = 0.0f;
-    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s_top[w][h]);
+    for (int w = 0; w < kStepWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
     const float shift = whole == -INFINITY ? 0.0f : whole;
     for (int w = 0; w < kStepWarps; ++w)
-      total = fmaf(s_sum[w][h], tc::exp2_approx(s_top[w][h] - shift), total);
-    s_top[0][h] = whole;
-    s_sum[0][h] = total;
+      total = fmaf(s.sum[w][h], tc::exp2_approx(s.top[w][h] - shift), total);
+    s.top[0][h] = whole;
+    s.sum[0][h] = total;
   }
   cluster_sync();
   // The blocks joined, each block a part of the outputs.
@@ -1186,12 +1282,12 @@ __global__ void __launch_bounds__(kStepThreads, 3)
        c += static_cast<int>(blocks) * kStepThreads) {
     const int h = c / kDim, d = c % kDim;
     float whole = -INFINITY, total = 0.0f, o = 0.0f;
-    for (uint32_t r = 0; r < blocks; ++r) whole = fmaxf(whole, read_block(&s_top[0][h], r));
+    for (uint32_t r = 0; r < blocks; ++r) whole = fmaxf(whole, read_block(&s.top[0][h], r));
     const float shift = whole == -INFINITY ? 0.0f : whole;
     for (uint32_t r = 0; r < blocks; ++r) {
-      const float w = tc::exp2_approx(read_block(&s_top[0][h], r) - shift);
-      total = fmaf(read_block(&s_sum[0][h], r), w, total);
-      o = fmaf(read_block(&s_out[0][h][d], r), w, o);
+      const float w = tc::exp2_approx(read_block(&s.top[0][h], r) - shift);
+      total = fmaf(read_block(&s.sum[0][h], r), w, total);
+      o = fmaf(read_block(&s.out[0][h][d], r), w, o);
     }
     if (d < a.dim)
       static_cast<T*>(a.out)[(b * a.heads + head0 + h) * a.dim + d] =
@@ -1202,23 +1298,30 @@ __global__ void __launch_bounds__(kStepThreads, 3)
 
 // Blocks of a cluster: enough that every multiprocessor has several blocks, as
 // far as each warp still gets slots.
-int step_blocks(const gs_window_attention_step_args& a) {
-  const int64_t items =
-      a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, kStepHeads);
+int step_blocks(const gs_window_attention_step_args& a, int64_t items) {
   int blocks = 1;
   while (blocks < 16 && items * blocks < 8 * kSmCount &&
-         2 * blocks * kStepWarps * kStepSlots <= a.slots)
+         2 * blocks * kStepTile <= a.slots)
     blocks *= 2;
   return blocks;
 }
 
-template <class T, int kDim>
+template <class T, int kDim, int kHalves>
 int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
-  const int blocks = step_blocks(a);
-  const int64_t grid = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, kStepHeads) * blocks;
-  if (grid > INT32_MAX) return GS_ERR_CAPACITY;
-  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim>,
+  const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kHalves);
+  const int blocks = step_blocks(a, items);
+  if (items * blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  CUtensorMap k, v;
+  const int64_t row = int64_t{a.kv_heads} * a.dim;
+  GS_TRY(tc::encode_heads(&k, a.dtype, a.cache_k, a.batch * a.slots, a.kv_heads, a.dim, row, a.dim,
+                          kStepTile));
+  GS_TRY(tc::encode_heads(&v, a.dtype, a.cache_v, a.batch * a.slots, a.kv_heads, a.dim, row, a.dim,
+                          kStepTile));
+  constexpr size_t kShared = sizeof(StepShared<kDim, kHalves>);
+  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim, kHalves>,
                                    cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim, kHalves>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1226,12 +1329,13 @@ int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   attr[1].val.clusterDim.x = blocks;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = static_cast<unsigned>(grid);
+  config.gridDim = static_cast<unsigned>(items * blocks);
   config.blockDim = kStepThreads;
+  config.dynamicSmemBytes = kShared;
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, attention_step_kernel<T, kDim>, a);
+  cudaLaunchKernelEx(&config, attention_step_kernel<T, kDim, kHalves>, a, k, v);
   return check_launch();
 }
 
@@ -1308,7 +1412,7 @@ int32_t launch_window_attention_backward(const gs_window_attention_args& a, cuda
 
 int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   GS_TRY(check_heads(a.heads, a.kv_heads, a.dim, a.dtype));
-  if (a.batch < 0 || a.batch > INT32_MAX || a.first < 0 || a.slots <= a.first ||
+  if (a.batch < 0 || a.first < 0 || a.slots <= a.first || a.batch > INT32_MAX / a.slots ||
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return GS_OK;
@@ -1321,7 +1425,9 @@ int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cud
     return GS_ERR_MISALIGNED;
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return a.dim <= 64 ? step<T, 64>(a, stream) : step<T, 128>(a, stream);
+    if (a.heads / a.kv_heads <= 8)
+      return a.dim <= 64 ? step<T, 64, 1>(a, stream) : step<T, 128, 1>(a, stream);
+    return a.dim <= 64 ? step<T, 64, 2>(a, stream) : step<T, 128, 2>(a, stream);
   });
 }
 
