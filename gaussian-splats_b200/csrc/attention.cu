@@ -1297,10 +1297,11 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
 }
 
 // Blocks of a cluster: enough that every multiprocessor has several blocks, as
-// far as each warp still gets slots.
+// far as each warp still gets slots (96 streams of 4100 slots: 138 us with
+// clusters of 2, 148 us with 4).
 int step_blocks(const gs_window_attention_step_args& a, int64_t items) {
   int blocks = 1;
-  while (blocks < 16 && items * blocks < 8 * kSmCount &&
+  while (blocks < 16 && items * blocks < 4 * kSmCount &&
          2 * blocks * kStepTile <= a.slots)
     blocks *= 2;
   return blocks;
