@@ -36,20 +36,23 @@ constexpr int kMaxDim = 128;
 
 // -------------------------------------------------- whole sequences, forward
 //
-// One block: kTile queries of one head, walked over the tiles of kKeys keys
-// that they see: first the tiles of first tokens that lie before the block's
-// window, then the window. Four warps hold a query a thread; a fifth warp's
-// first thread loads the tiles and issues the products.
+// One block: two tiles of 128 queries of one head, walked over the tiles of
+// kKeys keys that they see: first the tiles of first tokens that lie before the
+// block's window, then the window. A group of four warps holds a tile of
+// queries, one a thread; a ninth warp loads, a tenth issues the products.
 //
-//   scores  S = Q K^T            tensor memory, 128 x 64 floats
+//   scores  S = Q K^T            tensor memory, 128 x kKeys floats a group
 //   P = exp2(S scale log2 e - m) each thread its row; 16 bits, over S
-//   O (+)= P V                   tensor memory, 128 x dim floats
+//   O (+)= P V                   tensor memory, 128 x dim floats a group
 //
-// m is the row's running maximum, but moves only when it has grown by more
-// than 2^8: until then P stays at most 2^8, which both types hold with all
-// their precision, and O need not be rescaled.
+// While one group takes its exponentials, the tensor cores work for the other,
+// and both read the same keys and values. m is the row's running maximum, but
+// moves only when it has grown by more than 2^8: until then P stays at most
+// 2^8, which both types hold with all their precision, and O need not be
+// rescaled. What bounds it: 16 exponentials a clock and multiprocessor at 64
+// channels (a 128 x 128 tile takes 1024 clocks of them, 512 of products), both
+// at 128.
 
-constexpr int kKeys = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
@@ -58,312 +61,452 @@ constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
 // gs_window_attention_status, the block's results are not valid.
 __device__ uint32_t g_timeout;
 
-// 64 bits with those under `n` set.
+// 32 or 64 bits with those under `n` set.
+__device__ __forceinline__ uint32_t below32(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+}
 __device__ __forceinline__ uint64_t below(int64_t n) {
   return n <= 0 ? 0 : n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
 }
+// `x` as a position that comparisons within a sequence cannot tell from it.
+__device__ __forceinline__ int position(int64_t x) {
+  return static_cast<int>(max(int64_t{-1}, min(x, int64_t{INT32_MAX})));
+}
 
-// The keys that a tile of queries walks over, as tiles of kKeys: positions in
-// the sequence.
+// First tile of sequence b.
+__device__ __forceinline__ int64_t first_tile_of(const gs_window_attention_args& a, int64_t b) {
+  return a.tile_starts ? __ldg(a.tile_starts + b) : (b ? a.num_tiles : 0);
+}
+// Runs of `length` tiles: sequence b's take the numbers from floor(first tile of
+// b / length) + b on, which no two sequences share (some stay empty).
+__device__ __forceinline__ int64_t run_of(int64_t first_tile, int64_t sequence, int length) {
+  return first_tile / length + sequence;
+}
+// The sequence whose runs include number `run`.
+__device__ __forceinline__ int64_t sequence_of_run(const gs_window_attention_args& a, int64_t run,
+                                                   int length) {
+  int64_t b = 0, above = a.tile_starts ? a.sequences : 1;
+  while (above - b > 1) {  // the last one whose runs start at or before it
+    const int64_t middle = (b + above) / 2;
+    if (run_of(first_tile_of(a, middle), middle, length) <= run) b = middle;
+    else above = middle;
+  }
+  return b;
+}
+
+// Which of 32 keys from position `start` on query i sees, if those under `end`
+// are valid.
+__device__ __forceinline__ uint32_t window_bits(const gs_window_attention_args& a, int i,
+                                                int start, int end) {
+  const int high = min(position(int64_t{i} + a.right + 1), end);
+  const int low = position(int64_t{i} - a.left);
+  return below32(high - start) & (~below32(low - start) | below32(a.first - start));
+}
+
+// The valid keys among the 32 from row `row` on (bits from `rows` on are 0);
+// every lane of the warp gets them.
+__device__ __forceinline__ uint32_t valid_bits(const uint8_t* valid, int64_t row, int rows) {
+  if (!valid) return below32(rows);
+  const int lane = threadIdx.x & 31;
+  return __ballot_sync(0xffffffffu, lane < rows && __ldg(valid + row + lane));
+}
+
+// Zeroes the rows of a loaded tile (kRows rows, kDim channels) whose bit is not
+// set, so that what they hold (another sequence's rows, NaN of invalid keys)
+// cannot reach a sum through a weight of zero.
+template <int kDim, int kRows, int kThreadCount>
+__device__ __forceinline__ void zero_rows(unsigned char* tile, const uint32_t (&keep)[kRows / 32],
+                                          int tid) {
+  constexpr int kPerRow = kThreadCount / kRows;  // threads of a row
+  constexpr int kWordsEach = 8 / kPerRow;
+  const int row = tid / kPerRow;
+  uint32_t bits = keep[0];
+#pragma unroll
+  for (int c = 1; c < kRows / 32; ++c)
+    if (row >= 32 * c) bits = keep[c];
+  if (bits >> (row & 31) & 1) return;
+#pragma unroll
+  for (int box = 0; box < kDim / 64; ++box)
+#pragma unroll
+    for (int w = 0; w < kWordsEach; ++w)
+      *reinterpret_cast<uint4*>(tile + box * (kRows * 128) + row * 128 +
+                                ((tid % kPerRow) * kWordsEach + w) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// The tiles of keys that a run of kGroups tiles of queries walks over, as
+// positions in the sequence, and each group's part of them.
+template <int kKeys, int kGroups>
 struct KeyWalk {
-  int n, low, high, head, head_tiles, tiles;
+  int n, i, low, head, head_tiles, tiles;
+  int from[kGroups], to[kGroups], high[kGroups];  // of the window's tiles; past its last key
   __device__ __forceinline__ KeyWalk(const gs_window_attention_args& a, const Tile& tile) {
     n = tile.end - tile.begin;
-    const int64_t i = tile.start - tile.begin;
-    const int64_t last = min(i + kTile, int64_t{n}) - 1;
-    low = static_cast<int>(max(int64_t{0}, i - a.left));
-    high = static_cast<int>(min(int64_t{n}, last + a.right + 1));
+    i = tile.start - tile.begin;
+    low = max(0, position(int64_t{i} - a.left));
     head = min(a.first, low);
     head_tiles = (head + kKeys - 1) / kKeys;
-    tiles = head_tiles + (high - low + kKeys - 1) / kKeys;
+    tiles = head_tiles;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int first = i + g * kTile, last = min(first + kTile, n) - 1;
+      high[g] = min(position(int64_t{last} + a.right + 1), n);
+      // First tokens that reach into the window's tiles are seen by every group.
+      from[g] = a.first > low ? 0 : (max(low, position(int64_t{first} - a.left)) - low) / kKeys;
+      to[g] = first < n ? (high[g] - low + kKeys - 1) / kKeys : 0;
+      if (first < n) tiles = head_tiles + to[g];
+    }
   }
   __device__ __forceinline__ int start(int t) const {
     return t < head_tiles ? t * kKeys : low + (t - head_tiles) * kKeys;
   }
   // Keys of tile t that may be seen at all: those under this position.
   __device__ __forceinline__ int end(int t) const { return t < head_tiles ? head : n; }
+  // How many tiles a group walks over, and the number of its step s.
+  __device__ __forceinline__ int steps(int g) const {
+    return i + g * kTile < n ? head_tiles + to[g] - from[g] : 0;
+  }
+  __device__ __forceinline__ int tile_of(int g, int s) const {
+    return s < head_tiles ? s : s + from[g];
+  }
+  // Whether group g walks over tile t.
+  __device__ __forceinline__ bool walks(int g, int t) const {
+    return i + g * kTile < n &&
+           (t < head_tiles || (t - head_tiles >= from[g] && t - head_tiles < to[g]));
+  }
+  // Whether group g is the last to read tile t: at the same step the second of
+  // two groups is, else the first, which is behind in the window.
+  __device__ __forceinline__ bool last_reader(int g, int t) const {
+    const int other = 1 - g;
+    return !walks(other, t) || (t < head_tiles || from[1] == 0 ? g == 1 : g == 0);
+  }
+  // How many sets of 32 keys of tile t group g needs.
+  __device__ __forceinline__ int sets(int g, int t) const {
+    const int keys = min(kKeys, (t < head_tiles ? head : high[g]) - start(t));
+    return (keys + 31) / 32;
+  }
 };
 
-// Which of the keys at `start` query i sees, were all valid and in the tile.
-__device__ __forceinline__ uint64_t window_bits(const gs_window_attention_args& a, int64_t i,
-                                                int start, int end) {
-  const int64_t high = min(i + a.right + 1, int64_t{end});
-  return below(high - start) & (~below(i - a.left - start) | below(a.first - start));
-}
-
-// The valid keys among the 64 from row `row` on (bits from `rows` on are 0);
-// every lane of the warp gets them.
-__device__ __forceinline__ uint64_t valid_bits(const uint8_t* valid, int64_t row, int rows) {
-  if (!valid) return below(rows);
-  const int lane = threadIdx.x & 31;
-  const bool low = lane < rows && __ldg(valid + row + lane);
-  const bool high = lane + 32 < rows && __ldg(valid + row + lane + 32);
-  return static_cast<uint64_t>(__ballot_sync(0xffffffffu, high)) << 32 |
-         __ballot_sync(0xffffffffu, low);
-}
-
-// Zeroes the rows of a loaded tile (kDim channels, kRows = 64 rows) whose bit
-// is not set, so that what they hold (another sequence's rows, NaN of invalid
-// keys) cannot reach a sum through a weight of zero.
-template <int kDim, int kThreadCount>
-__device__ __forceinline__ void zero_rows(unsigned char* tile, uint64_t keep, int tid) {
-  constexpr int kPerRow = kThreadCount / 64;  // threads of a row
-  constexpr int kWordsEach = 8 / kPerRow;
-  const int row = tid / kPerRow;
-  if (keep >> row & 1) return;
-#pragma unroll
-  for (int box = 0; box < kDim / 64; ++box)
-#pragma unroll
-    for (int w = 0; w < kWordsEach; ++w)
-      *reinterpret_cast<uint4*>(tile + box * 8192 + row * 128 +
-                                ((tid % kPerRow) * kWordsEach + w) * 16) = make_uint4(0, 0, 0, 0);
-}
+template <int kDim>
+struct ForwardShape {
+  // At 64 channels two blocks share a multiprocessor, 16 warps for the
+  // exponentials; at 128 one block fills it.
+  static constexpr int kKeys = kDim == 64 ? 64 : 128;
+  static constexpr int kBlocks = kDim == 64 ? 2 : 1;
+  static constexpr int kColumns = kDim == 64 ? 256 : 512;
+  static constexpr int kGroupColumns = kKeys + kDim;  // S, then O
+};
+constexpr int kForwardThreads = 2 * kTile + 64;
 
 template <int kDim>
 struct ForwardShared {
-  static constexpr int kKeyStages = 2, kValueStages = 2;
+  // The second group is kTile / kKeys tiles ahead of the first.
+  static constexpr int kStages = kDim == 64 ? 4 : 2;
+  static constexpr int kKeys = ForwardShape<kDim>::kKeys;
   static constexpr int kQueryBytes = kTile * kDim * 2, kTileBytes = kKeys * kDim * 2;
-  alignas(1024) unsigned char q[kQueryBytes];
-  unsigned char k[kKeyStages][kTileBytes];
-  unsigned char v[kValueStages][kTileBytes];
-  uint64_t q_full, k_full[kKeyStages], v_full[kValueStages];  // loads
-  uint64_t scores;   // S of a tile is complete
-  uint64_t weights;  // P of a tile is written (128 arrivals)
-  uint64_t summed;   // O has a tile's sum
+  alignas(1024) unsigned char q[2][kQueryBytes];
+  unsigned char k[kStages][kTileBytes];
+  unsigned char v[kStages][kTileBytes];
+  uint64_t q_full[2], k_full[kStages], v_full[kStages];  // loads
+  uint64_t k_empty[kStages], v_empty[kStages];  // both groups' products with a tile are complete
+  uint64_t scores[2];                           // S of a group's step is complete
+  uint64_t weights[2];                          // P is written (128 arrivals)
+  uint64_t summed[2];                           // all of a group's sums are complete
   uint32_t tensor;
 };
 
 template <class T, int kDim>
-__global__ void __launch_bounds__(kTile + 32, kDim == 64 ? 4 : 2)
+__global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
     attention_kernel(gs_window_attention_args a, const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map) {
   using namespace tc;
+  using Shape = ForwardShape<kDim>;
   using Shared = ForwardShared<kDim>;
-  constexpr int kScoreColumn = 0, kOutColumn = kKeys;
-  constexpr int kColumns = kDim == 64 ? 128 : 256;
-  constexpr int kBoxes = kDim / 64;
+  constexpr int kKeys = Shape::kKeys, kStages = Shared::kStages, kSets = kKeys / 32;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   chain_wait();
   const int warp = threadIdx.x >> 5;
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
-  const Tile tile =
-      tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
-  const KeyWalk walk(a, tile);
+  const int64_t run = blockIdx.x / a.heads;
+  const int64_t sequence = sequence_of_run(a, run, 2);
+  const int64_t tile0 = first_tile_of(a, sequence);
+  const int64_t index = tile0 + 2 * (run - run_of(tile0, sequence, 2));
+  if (index >= first_tile_of(a, sequence + 1)) return;
+  const Tile tile = tile_at(a.tiles, index, static_cast<int32_t>(a.tokens), kTile);
+  const KeyWalk<kKeys, 2> walk(a, tile);
   if (threadIdx.x == 0) {
-    barrier_init(shared_address(&s.q_full), 1);
-    for (uint64_t& b : s.k_full) barrier_init(shared_address(&b), 1);
-    for (uint64_t& b : s.v_full) barrier_init(shared_address(&b), 1);
-    barrier_init(shared_address(&s.scores), 1);
-    barrier_init(shared_address(&s.weights), kTile);
-    barrier_init(shared_address(&s.summed), 1);
+    for (int g = 0; g < 2; ++g) {
+      barrier_init(shared_address(&s.q_full[g]), 1);
+      barrier_init(shared_address(&s.scores[g]), 1);
+      barrier_init(shared_address(&s.weights[g]), kTile);
+      barrier_init(shared_address(&s.summed[g]), 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      barrier_init(shared_address(&s.k_full[i]), 1);
+      barrier_init(shared_address(&s.v_full[i]), 1);
+      barrier_init(shared_address(&s.k_empty[i]), 1);
+      barrier_init(shared_address(&s.v_empty[i]), 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
-  if (warp == 4) tensor_alloc<kColumns>(shared_address(&s.tensor));
+  if (warp == 9) tensor_alloc<Shape::kColumns>(shared_address(&s.tensor));
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tensor = s.tensor;
   bool good = true;
 
-  if (warp == 4) {
+  if (warp == 8) {  // loads
     if ((threadIdx.x & 31) == 0) {
       const auto load = [&](unsigned char* dst, uint64_t* bar, const CUtensorMap* map, int h,
-                            int row, int bytes, int box_bytes) {
+                            int row, int rows) {
         const uint32_t b = shared_address(bar), d = shared_address(dst);
-        barrier_expect(b, bytes);
-        for (int x = 0; x < kBoxes; ++x) load_box(d + x * box_bytes, map, 64 * x, h, row, b);
+        barrier_expect(b, rows * kDim * 2);
+        for (int x = 0; x < kDim / 64; ++x) load_box(d + x * rows * 128, map, 64 * x, h, row, b);
       };
-      const auto load_keys = [&](int t) {
-        load(s.k[t % Shared::kKeyStages], &s.k_full[t % Shared::kKeyStages], &k_map, kv_head,
-             tile.begin + walk.start(t), Shared::kTileBytes, kKeys * 128);
-      };
-      const auto load_values = [&](int t) {
-        load(s.v[t % Shared::kValueStages], &s.v_full[t % Shared::kValueStages], &v_map, kv_head,
-             tile.begin + walk.start(t), Shared::kTileBytes, kKeys * 128);
-      };
-      load(s.q, &s.q_full, &q_map, head, tile.start, Shared::kQueryBytes, kTile * 128);
-      for (int t = 0; t < Shared::kKeyStages && t < walk.tiles; ++t) load_keys(t);
-      for (int t = 0; t < Shared::kValueStages && t < walk.tiles; ++t) load_values(t);
-
-      const int steps = (a.dim + 15) / 16;
-      const uint32_t score_kind = product_kind<T>(kKeys, false);
-      const uint32_t sum_kind = product_kind<T>((a.dim + 15) / 16 * 16, true);
-      const uint32_t q = shared_address(s.q);
-      const auto issue_scores = [&](int t) {
-        const int stage = t % Shared::kKeyStages;
-        good = good && barrier_wait(shared_address(&s.k_full[stage]),
-                                    (t / Shared::kKeyStages) & 1);
-        const uint32_t k = shared_address(s.k[stage]);
-        for (int i = 0; i < steps; ++i)
-          multiply(tensor + kScoreColumn, along_channels<kTile>(q, i), along_channels<kKeys>(k, i),
-                   score_kind, i > 0);
-        commit(shared_address(&s.scores));
-      };
-      good = barrier_wait(shared_address(&s.q_full), 0);
-      if (good) issue_scores(0);
-      int t = 0;
-      for (; t < walk.tiles && good; ++t) {
-        good = barrier_wait(shared_address(&s.weights), t & 1);
+      load(s.q[0], &s.q_full[0], &q_map, head, tile.start, kTile);
+      for (int t = 0; t < walk.tiles && good; ++t) {
+        const int stage = t % kStages, turn = t / kStages;
+        if (turn > 0) good = barrier_wait(shared_address(&s.k_empty[stage]), (turn - 1) & 1);
         if (!good) break;
-        fence_after_sync();
-        // P(t) was written from S(t): the products that read K(t) are complete.
-        if (t + Shared::kKeyStages < walk.tiles) load_keys(t + Shared::kKeyStages);
-        const int stage = t % Shared::kValueStages;
-        good = barrier_wait(shared_address(&s.v_full[stage]), (t / Shared::kValueStages) & 1);
-        const uint32_t v = shared_address(s.v[stage]);
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          multiply_tensor(tensor + kOutColumn, tensor + kScoreColumn + 8 * i,
-                          along_rows<kKeys>(v, i), sum_kind, t > 0 || i > 0);
-        commit(shared_address(&s.summed));
-        // In order behind the product that reads P(t).
-        if (t + 1 < walk.tiles) issue_scores(t + 1);
-        // S(t) was complete behind the sum of t - 1: V(t - 1) is free.
-        if (t >= 1 && t - 1 + Shared::kValueStages < walk.tiles)
-          load_values(t - 1 + Shared::kValueStages);
+        load(s.k[stage], &s.k_full[stage], &k_map, kv_head, tile.begin + walk.start(t), kKeys);
+        if (t == 0 && walk.steps(1) > 0)
+          load(s.q[1], &s.q_full[1], &q_map, head, tile.start + kTile, kTile);
+        if (turn > 0) good = barrier_wait(shared_address(&s.v_empty[stage]), (turn - 1) & 1);
+        if (!good) break;
+        load(s.v[stage], &s.v_full[stage], &v_map, kv_head, tile.begin + walk.start(t), kKeys);
       }
-      if (!good) {
-        // Let what is in flight land before the shared memory is given back.
-        for (uint64_t& b : s.k_full)
-          for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
-        for (uint64_t& b : s.v_full)
-          for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+      if (!good) {  // let what is in flight land before the shared memory is given back
+        for (int i = 0; i < kStages; ++i)
+          for (int p = 0; p < 2; ++p) {
+            barrier_wait(shared_address(&s.k_full[i]), p);
+            barrier_wait(shared_address(&s.v_full[i]), p);
+          }
         atomicExch(&g_timeout, 1u);
       }
     }
     __syncwarp();
+  } else if (warp == 9) {  // products
+    if ((threadIdx.x & 31) == 0) {
+      const int dim_steps = (a.dim + 15) / 16;
+      const uint32_t sum_kind = product_kind<T>(dim_steps * 16, true);
+      const uint32_t score_kind = product_kind<T>(0, false);
+      const uint32_t q = channels_word<kTile>(shared_address(s.q[0]));
+      const uint32_t k = channels_word<kKeys>(shared_address(s.k[0]));
+      const uint32_t v = rows_word<kKeys>(shared_address(s.v[0]));
+      const int steps[2] = {walk.steps(0), walk.steps(1)};
+      int keys_here = 0, values_here = 0;  // tiles whose loads have been waited for
+      const auto issue_scores = [&](auto number, int step) {
+        constexpr int g = decltype(number)::value;
+        const int t = walk.tile_of(g, step), stage = t % kStages;
+        const uint32_t kind = score_kind | static_cast<uint32_t>(4 * walk.sets(g, t)) << 17;
+        const bool last = walk.last_reader(g, t);
+        if (step == 0) good = good && barrier_wait(shared_address(&s.q_full[g]), 0);
+        if (t >= keys_here) {
+          good = good && barrier_wait(shared_address(&s.k_full[stage]), (t / kStages) & 1);
+          keys_here = t + 1;
+        }
+        const uint32_t a0 = q + g * (Shared::kQueryBytes >> 4);
+        const uint32_t b0 = k + stage * (Shared::kTileBytes >> 4);
+#pragma unroll
+        for (int i = 0; i < kDim / 16; ++i)
+          if (i < dim_steps)
+            multiply(tensor + g * Shape::kGroupColumns, a0 + channels_step<kTile>(i),
+                     b0 + channels_step<kKeys>(i), kind, i > 0);
+        commit(shared_address(&s.scores[g]));
+        if (last) commit(shared_address(&s.k_empty[stage]));
+      };
+      const auto issue_sums = [&](auto number, int step) {
+        constexpr int g = decltype(number)::value;
+        if (step >= steps[g] || !good) return;
+        const int t = walk.tile_of(g, step), stage = t % kStages, sets = walk.sets(g, t);
+        const bool last = walk.last_reader(g, t);
+        if (t >= values_here) {
+          good = barrier_wait(shared_address(&s.v_full[stage]), (t / kStages) & 1);
+          values_here = t + 1;
+        }
+        good = good && barrier_wait(shared_address(&s.weights[g]), step & 1);
+        if (!good) return;
+        fence_after_sync();
+        const uint32_t b0 = v + stage * (Shared::kTileBytes >> 4);
+        constexpr uint32_t column = g * Shape::kGroupColumns;
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          if (i < 2 * sets)
+            multiply_tensor(tensor + column + kKeys, tensor + column + 8 * i, b0 + rows_step(i),
+                            sum_kind, step > 0 || i > 0);
+        if (last) commit(shared_address(&s.v_empty[stage]));
+        if (step == steps[g] - 1) commit(shared_address(&s.summed[g]));
+        else issue_scores(number, step + 1);  // in order behind the product that reads P
+      };
+      using First = std::integral_constant<int, 0>;
+      using Second = std::integral_constant<int, 1>;
+      issue_scores(First{}, 0);
+      if (steps[1] > 0) issue_scores(Second{}, 0);
+      for (int step = 0; step < max(steps[0], steps[1]) && good; ++step) {
+        issue_sums(First{}, step);
+        issue_sums(Second{}, step);
+      }
+      if (!good) atomicExch(&g_timeout, 1u);
+    }
+    __syncwarp();
   } else {
-    const int row = threadIdx.x, lane = threadIdx.x & 31;
-    const uint32_t mine = tensor + (static_cast<uint32_t>(warp * 32) << 16);
-    const int64_t i = tile.start - tile.begin + row;  // the query's position
+    const int group = warp >> 2, row = threadIdx.x & (kTile - 1);
+    const uint32_t scores = tensor + group * Shape::kGroupColumns +
+                            (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t sums = scores + kKeys;
+    const int i_first = walk.i + group * kTile, i = i_first + row;
     const float scale = a.scale * kLog2e;
     float top = -INFINITY, sum = 0.0f;
-    // The first and the last query of the block, for what all of them see.
-    const int64_t i_first = tile.start - tile.begin, i_last = i_first + kTile - 1;
-    for (int t = 0; t < walk.tiles; ++t) {
-      const int start = walk.start(t), end = walk.end(t);
-      const uint64_t keep =
-          valid_bits(a.valid, int64_t{tile.begin} + start, min(end - start, kKeys));
-      const bool whole = keep == ~uint64_t{0} && (t < walk.head_tiles ||
-                                                  (start + kKeys <= i_first + a.right + 1 &&
-                                                   (start >= i_last - a.left ||
-                                                    start + kKeys <= a.first)));
-      if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1))) break;
+    const int steps = walk.steps(group);
+    for (int step = 0; step < steps; ++step) {
+      const int t = walk.tile_of(group, step), start = walk.start(t), end = walk.end(t);
+      const int sets = walk.sets(group, t);
+      uint32_t keep[kSets];
+      bool all = true;
+#pragma unroll
+      for (int c = 0; c < kSets; ++c) {
+        keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
+                             max(0, min(end - start - 32 * c, 32)));
+        all = all && keep[c] == ~0u;
+      }
+      // Whether every query of the group sees every key of the tile.
+      const bool whole =
+          all && (t < walk.head_tiles ||
+                  (start + kKeys <= position(int64_t{i_first} + a.right + 1) &&
+                   (start >= position(int64_t{i_first} + kTile - 1 - a.left) ||
+                    start + kKeys <= a.first)));
+      good = good && barrier_wait_warp(shared_address(&s.scores[group]), step & 1);
+      if (!good) break;
       fence_after_sync();
-      float x[2][32];
-      load_columns32(mine + kScoreColumn, x[0]);
-      load_columns32(mine + kScoreColumn + 32, x[1]);
+      float x[kSets][32];
+#pragma unroll
+      for (int c = 0; c < kSets; ++c)
+        if (c < sets) load_columns32(scores + 32 * c, x[c]);
       wait_loads();
       if (!whole) {
-        const uint64_t bits = keep & window_bits(a, i, start, end);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          x[0][c] = bits >> c & 1 ? x[0][c] : -INFINITY;
-          x[1][c] = bits >> (c + 32) & 1 ? x[1][c] : -INFINITY;
+        for (int c = 0; c < kSets; ++c)
+          if (c < sets) {
+            const uint32_t bits = keep[c] & window_bits(a, i, start + 32 * c, end);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[c][e] = bits >> e & 1 ? x[c][e] : -INFINITY;
+          }
+      }
+      float next = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kSets; ++c)
+        if (c < sets) {
+          float high[4] = {x[c][0], x[c][1], x[c][2], x[c][3]};
+#pragma unroll
+          for (int e = 4; e < 32; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              high[k] = e + 4 < 32 ? max3(high[k], x[c][e + k], x[c][e + 4 + k])
+                                   : fmaxf(high[k], x[c][e + k]);
+          next = max3(next, max3(high[0], high[1], high[2]), high[3]);
         }
-      }
-      float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        high[c & 1] = fmaxf(high[c & 1], x[0][c]);
-        high[2 + (c & 1)] = fmaxf(high[2 + (c & 1)], x[1][c]);
-      }
-      const float next =
-          fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale;
+      next *= scale;
       // Sums of earlier tiles are complete: this tile's S came behind them.
       const bool grow = next > top + kSlack || (top == -INFINITY && next > top);
       if (__any_sync(0xffffffffu, grow)) {
         const float shrink = grow ? exp2_approx(top - next) : 1.0f;
         if (grow) top = next;
         sum *= shrink;
-        if (t > 0) {
+        if (step > 0) {
 #pragma unroll 1
           for (int c = 0; c < kDim; c += 16) {
             float o[16];
-            load_columns16(mine + kOutColumn + c, o);
+            load_columns16(sums + c, o);
             wait_loads();
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] *= shrink;
-            store_columns16(mine + kOutColumn + c, o);
+            store_columns16(sums + c, o);
           }
         }
       }
       // Where nothing is seen yet any finite shift will do: exp2(-inf) is 0.
-      const float shift = top == -INFINITY ? 0.0f : -top;
-      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint32_t packed[2][16];
+      const float2 shift = make_float2(top == -INFINITY ? 0.0f : -top, top == -INFINITY ? 0.0f : -top);
+      const float2 factor = make_float2(scale, scale);
+      float2 part[2] = {};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int c = 0; c < kSets; ++c)
+        if (c < sets) {
+          uint32_t packed[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float p0 = exp2_approx(fmaf(x[half][2 * c], scale, shift));
-          const float p1 = exp2_approx(fmaf(x[half][2 * c + 1], scale, shift));
-          part[2 * half] += p0;
-          part[2 * half + 1] += p1;
-          packed[half][c] = pack2<T>(p0, p1);
+          for (int e = 0; e < 16; ++e) {
+            const float2 y =
+                fma2(make_float2(x[c][2 * e], x[c][2 * e + 1]), factor, shift);
+            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            part[e & 1] = add2(part[e & 1], p);
+            packed[e] = pack2<T>(p.x, p.y);
+          }
+          store_columns16(scores + 16 * c, packed);
         }
-        store_columns16(mine + kScoreColumn + 16 * half, packed[half]);
-      }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-      if (keep != ~uint64_t{0}) {
-        const int stage = t % Shared::kValueStages;
-        if (!(good = barrier_wait_warp(shared_address(&s.v_full[stage]),
-                                  (t / Shared::kValueStages) & 1)))
-          break;
-        zero_rows<kDim, kTile>(s.v[stage], keep, row);
+      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+      if (!all) {
+        const int stage = t % kStages;
+        good = barrier_wait_warp(shared_address(&s.v_full[stage]), (t / kStages) & 1);
+        if (!good) break;
+        zero_rows<kDim, kKeys, kTile>(s.v[stage], keep, row);
         fence_async_shared();
       }
       wait_stores();
       fence_before_sync();
-      barrier_arrive(shared_address(&s.weights));
+      barrier_arrive(shared_address(&s.weights[group]));
     }
-    if (good) good = barrier_wait_warp(shared_address(&s.summed), (walk.tiles - 1) & 1);
-    fence_after_sync();
-    const bool write = tile.start + row < tile.end;
-    const float inverse = 1.0f / sum;
-    T* out = static_cast<T*>(a.out) + (int64_t{tile.start + row} * a.heads + head) * a.dim;
+    if (steps > 0) {
+      if (good) good = barrier_wait_warp(shared_address(&s.summed[group]), 0);
+      fence_after_sync();
+      const int64_t token = int64_t{tile.start} + group * kTile + row;
+      const bool write = token < tile.end;
+      const float inverse = good ? 1.0f / sum : NAN;  // a wait that ran out shows
+      T* out = static_cast<T*>(a.out) + (token * a.heads + head) * a.dim;
 #pragma unroll
-    for (int c = 0; c < kDim; c += 32) {
-      float o[32];
-      load_columns32(mine + kOutColumn + c, o);
-      wait_loads();
+      for (int c = 0; c < kDim; c += 32) {
+        float o[32];
+        load_columns32(sums + c, o);
+        wait_loads();
 #pragma unroll
-      for (int e = 0; e < 32; e += 8)
-        if (write && c + e < a.dim) {
-          float v[8];
+        for (int e = 0; e < 32; e += 8)
+          if (write && c + e < a.dim) {
+            float v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            v[k] = good ? (sum == 0.0f ? 0.0f : o[e + k] * inverse) : NAN;
-          store_pack<8>(out + c + e, v);
-        }
+            for (int k = 0; k < 8; ++k) v[k] = sum == 0.0f ? 0.0f : o[e + k] * inverse;
+            store_pack<8>(out + c + e, v);
+          }
+      }
+      if (write && a.lse)
+        a.lse[head * a.tokens + token] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
     }
-    if (write && a.lse)
-      a.lse[head * a.tokens + tile.start + row] =
-          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-    if (!good && lane == 0) atomicExch(&g_timeout, 1u);
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 4) tensor_free<kColumns>(tensor);
+  if (warp == 9) tensor_free<Shape::kColumns>(tensor);
 }
+
+int64_t sequences_of(const gs_window_attention_args& a) { return a.tile_starts ? a.sequences : 1; }
 
 template <class T, int kDim>
 int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
+  constexpr int kKeys = ForwardShape<kDim>::kKeys;
   CUtensorMap q, k, v;
   GS_TRY(tc::encode_heads(&q, a.dtype, a.q, a.tokens, a.heads, a.dim, a.q_stride, a.q_head_stride,
-                        kTile));
-  GS_TRY(tc::encode_heads(&k, a.dtype, a.k, a.tokens, a.kv_heads, a.dim, a.k_stride, a.k_head_stride,
-                        kKeys));
-  GS_TRY(tc::encode_heads(&v, a.dtype, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride, a.v_head_stride,
-                        kKeys));
+                          kTile));
+  GS_TRY(tc::encode_heads(&k, a.dtype, a.k, a.tokens, a.kv_heads, a.dim, a.k_stride,
+                          a.k_head_stride, kKeys));
+  GS_TRY(tc::encode_heads(&v, a.dtype, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride,
+                          a.v_head_stride, kKeys));
   constexpr size_t kShared = sizeof(ForwardShared<kDim>);
   GS_CUDA_TRY(cudaFuncSetAttribute(attention_kernel<T, kDim>,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
-  launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kTile + 32, kShared, stream, a, q, k, v);
+  const int64_t blocks = (a.num_tiles / 2 + sequences_of(a)) * a.heads;
+  if (blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(blocks), kForwardThreads,
+                        kShared, stream, a, q, k, v);
   return check_launch();
 }
 
@@ -385,6 +528,8 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // walk the whole sequence. It walks its window like the others; the queries
 // further on are cut into chunks with a block each, and a last kernel adds the
 // chunks' sums in order.
+
+constexpr int kKeys = 64;  // rows of the backward's tiles
 
 template <int kDim>
 struct BackwardShape {
@@ -455,20 +600,26 @@ __device__ __forceinline__ bool drive(BackwardShared<kDim>& s, int dim, int tile
   const int steps = (dim + 15) / 16;
   const uint32_t score_kind = product_kind<T>(kKeys, false);
   const uint32_t sum_kind = product_kind<T>((dim + 15) / 16 * 16, true);
-  const uint32_t rows0 = shared_address(s.rows[0]), rows1 = shared_address(s.rows[1]);
+  const uint32_t rows0 = channels_word<kTile>(shared_address(s.rows[0]));
+  const uint32_t rows1 = channels_word<kTile>(shared_address(s.rows[1]));
+  const uint32_t tiles0 = shared_address(s.tiles[0][0]);
+  constexpr uint32_t kStageWords = 2 * Shape::kTileBytes >> 4, kHalfWords = Shape::kTileBytes >> 4;
   bool good = barrier_wait(rows_full, 0);
   const auto issue_scores = [&](int t) {
     const int stage = t % kStages;
     good = good && barrier_wait(shared_address(&s.full[stage]), (t / kStages) & 1);
-    const uint32_t tile0 = shared_address(s.tiles[stage][0]);
-    const uint32_t tile1 = shared_address(s.tiles[stage][1]);
+    const uint32_t tile = channels_word<kKeys>(tiles0) + stage * kStageWords;
     const uint32_t d = tensor + (t % kBuffers) * Shape::kBuffer;
-    for (int i = 0; i < steps; ++i)
-      multiply(d + Shape::kScore, along_channels<kTile>(rows0, i), along_channels<kKeys>(tile0, i),
-               score_kind, i > 0);
-    for (int i = 0; i < steps; ++i)
-      multiply(d + Shape::kGrad, along_channels<kTile>(rows1, i), along_channels<kKeys>(tile1, i),
-               score_kind, i > 0);
+#pragma unroll
+    for (int i = 0; i < kDim / 16; ++i)
+      if (i < steps)
+        multiply(d + Shape::kScore, rows0 + channels_step<kTile>(i),
+                 tile + channels_step<kKeys>(i), score_kind, i > 0);
+#pragma unroll
+    for (int i = 0; i < kDim / 16; ++i)
+      if (i < steps)
+        multiply(d + Shape::kGrad, rows1 + channels_step<kTile>(i),
+                 tile + kHalfWords + channels_step<kKeys>(i), score_kind, i > 0);
     commit(shared_address(&s.scores[t % kBuffers]));
   };
   for (int t = 0; t < kBuffers && t < tiles; ++t) issue_scores(t);
@@ -483,17 +634,16 @@ __device__ __forceinline__ bool drive(BackwardShared<kDim>& s, int dim, int tile
       if (t - 1 + kStages < tiles) load_tile(t - 1 + kStages);
     }
     const uint32_t d = tensor + buffer * Shape::kBuffer;
-    const uint32_t tile0 = shared_address(s.tiles[stage][0]);
-    const uint32_t tile1 = shared_address(s.tiles[stage][1]);
+    const uint32_t tile = rows_word<kKeys>(tiles0) + stage * kStageWords;
 #pragma unroll
     for (int i = 0; i < kKeys / 16; ++i)
       multiply_tensor(tensor + Shape::kSum, d + Shape::kGrad + weight_column(i),
-                      along_rows<kKeys>(tile0, i), sum_kind, t > 0 || i > 0);
+                      tile + rows_step(i), sum_kind, t > 0 || i > 0);
     if constexpr (kKeyRows) {
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i)
         multiply_tensor(tensor + Shape::kSum + kDim, d + Shape::kScore + weight_column(i),
-                        along_rows<kKeys>(tile1, i), sum_kind, t > 0 || i > 0);
+                        tile + kHalfWords + rows_step(i), sum_kind, t > 0 || i > 0);
     }
     commit(shared_address(&s.summed));
     if (t == tiles - 1) commit(shared_address(&s.done));
@@ -553,7 +703,7 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const Tile tile =
       tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
-  const KeyWalk walk(a, tile);
+  const KeyWalk<kKeys, 1> walk(a, tile);
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
   if (warp == 8) {
@@ -567,7 +717,7 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int64_t i_first = tile.start - tile.begin, i = i_first + row;
+    const int i_first = walk.i, i = i_first + row;
     const bool live = tile.start + row < tile.end;
     const int64_t at = (int64_t{tile.start + row} * a.heads + head) * a.dim;
     float d = 0.0f;
@@ -589,14 +739,18 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
     bool good = true;
     for (int t = 0; t < walk.tiles; ++t) {
       const int start = walk.start(t), end = walk.end(t);
-      const uint64_t keep =
-          valid_bits(a.valid, int64_t{tile.begin} + start, min(end - start, kKeys));
-      const bool whole = keep == ~uint64_t{0} &&
-                         (t < walk.head_tiles ||
-                          (start + kKeys <= i_first + a.right + 1 &&
-                           (start >= i_first + kTile - 1 - a.left || start + kKeys <= a.first)));
-      const uint32_t bits = static_cast<uint32_t>(
-          (keep & window_bits(a, i, start, end)) >> (32 * half));
+      uint32_t keep[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
+                             max(0, min(end - start - 32 * c, 32)));
+      const bool all = (keep[0] & keep[1]) == ~0u;
+      const bool whole =
+          all && (t < walk.head_tiles ||
+                  (start + kKeys <= position(int64_t{i_first} + a.right + 1) &&
+                   (start >= position(int64_t{i_first} + kTile - 1 - a.left) ||
+                    start + kKeys <= a.first)));
+      const uint32_t bits = keep[half] & window_bits(a, i, start + 32 * half, end);
       const int buffer = t % Shape::kBuffers;
       if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), (t / Shape::kBuffers) & 1)))
         break;
@@ -619,11 +773,11 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
         packed[c] = pack2<T>(e[0], e[1]);
       }
       store_columns16(from + Shape::kGrad, packed);
-      if (keep != ~uint64_t{0}) {
+      if (!all) {
         const int stage = t % Shape::kStages;
         if (!(good = barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1)))
           break;
-        zero_rows<kDim, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
+        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
         fence_async_shared();
       }
       wait_stores();
@@ -656,19 +810,12 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
 
 // The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
 // dim] over their own windows, `part` [slot, ...] over the chunks of `tiles`
-// tiles of later queries. Sequence b's chunks take the slots from
-// floor(first tile of b / tiles) + b on, which no two sequences share.
+// tiles of later queries, numbered as runs of tiles are.
 struct FirstSums {
   float* base;
   float* part;
   int tiles, slots;
-  __device__ __forceinline__ int64_t slot_of(int64_t first_tile, int64_t sequence) const {
-    return first_tile / tiles + sequence;
-  }
 };
-__device__ __forceinline__ int64_t first_tile_of(const gs_window_attention_args& a, int64_t b) {
-  return a.tile_starts ? __ldg(a.tile_starts + b) : (b ? a.num_tiles : 0);
-}
 // Whether some query of a sequence of n sees first tokens before its window.
 __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a, int n) {
   return a.first > 0 && n > int64_t{a.left} + 1;
@@ -694,14 +841,9 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   Tile tile;
   int64_t low, high;  // queries, as positions
   if (chunk) {
-    int64_t b = 0, above = a.tile_starts ? a.sequences : 1;
-    while (above - b > 1) {  // the last sequence whose slots start at or before this one
-      const int64_t middle = (b + above) / 2;
-      if (sums.slot_of(first_tile_of(a, middle), middle) <= item) b = middle;
-      else above = middle;
-    }
+    const int64_t b = sequence_of_run(a, item, sums.tiles);
     const int64_t tile0 = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
-    const int64_t index = (item - sums.slot_of(tile0, b)) * sums.tiles;
+    const int64_t index = (item - run_of(tile0, b, sums.tiles)) * sums.tiles;
     if (index >= tiles) return;
     tile = tile_at(a.tiles, tile0, static_cast<int32_t>(a.tokens), kTile);
     const int64_t n = tile.end - tile.begin;
@@ -798,8 +940,10 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
         const int stage = t % Shape::kStages;
         good =
             good && barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1);
-        zero_rows<kDim, kComputeThreads>(s.tiles[stage][0], below(n - start), threadIdx.x);
-        zero_rows<kDim, kComputeThreads>(s.tiles[stage][1], below(n - start), threadIdx.x);
+        const int rest = n - static_cast<int>(start);
+        const uint32_t keep[2] = {below32(rest), below32(rest - 32)};
+        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
+        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][1], keep, threadIdx.x);
         fence_async_shared();
       }
       if (threadIdx.x < 2 * kKeys)
@@ -863,7 +1007,7 @@ __global__ void __launch_bounds__(2 * kMaxDim * kParts) first_sum_kernel(
   const int c = threadIdx.x % (2 * kMaxDim), part = threadIdx.x / (2 * kMaxDim);
   const int64_t row = (int64_t{kv_head} * a.first + j) * 2 * a.dim + c;
   const int64_t stride = int64_t{a.kv_heads} * a.first * 2 * a.dim;
-  const int64_t slot = sums.slot_of(tile0, b);
+  const int64_t slot = run_of(tile0, b, sums.tiles);
   const int64_t length = int64_t{sums.tiles} * kTile;
   const int64_t from = (int64_t{a.left} + 1) / length, to = (n + length - 1) / length;
   float sum = 0.0f;
@@ -882,7 +1026,6 @@ __global__ void __launch_bounds__(2 * kMaxDim * kParts) first_sum_kernel(
   }
 }
 
-int64_t sequences_of(const gs_window_attention_args& a) { return a.tile_starts ? a.sequences : 1; }
 // D of every row, to a 256-byte boundary.
 int64_t delta_floats(const gs_window_attention_args& a) {
   return (a.tokens * a.heads + 63) / 64 * 64;
@@ -1361,6 +1504,7 @@ int32_t check_args(const gs_window_attention_args& a) {
   if (!a.tiles && a.num_tiles != (a.tokens + kTile - 1) / kTile) return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.tiles, 16)) return GS_ERR_MISALIGNED;
   if (a.num_tiles == 0) return GS_OK;
+  if (a.tiles && !a.tile_starts) return GS_ERR_INVALID_ARGUMENT;
   if (!a.q || !a.k || !a.v || !a.out) return GS_ERR_INVALID_ARGUMENT;
   if (!strided16(a.q, a.q_stride, a.q_head_stride) ||
       !strided16(a.k, a.k_stride, a.k_head_stride) ||
@@ -1402,7 +1546,6 @@ int32_t launch_window_attention_backward(const gs_window_attention_args& a, cuda
   for (const void* p : {a.grad_out, static_cast<const void*>(a.grad_q),
                         static_cast<const void*>(a.grad_k), static_cast<const void*>(a.grad_v)})
     if (!is_aligned(p, 16)) return GS_ERR_MISALIGNED;
-  if (a.tiles && !a.tile_starts) return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.workspace, 256)) return GS_ERR_MISALIGNED;
   if (a.workspace_size < window_attention_workspace_size(a)) return GS_ERR_CAPACITY;
   return with_sixteen_bit(a.dtype, [&](auto t) {

@@ -151,24 +151,33 @@ __device__ __forceinline__ void wait_stores() {
 
 // Tiles lie in shared memory as TMA's 128-byte swizzle writes boxes of 64
 // channels: rows of 128 bytes, eight rows to a swizzled kilobyte, one box of
-// `rows` rows after the other along the channels. The descriptor of an operand
-// whose contraction runs along the channels (a row is a row of the product)
-// names the stride between eight-row groups; that of an operand whose
-// contraction runs along the rows names it too, and the stride between boxes.
-__device__ __forceinline__ uint64_t describe(uint32_t address, uint32_t box_bytes) {
-  return static_cast<uint64_t>((address >> 4) & 0x3FFF) |
-         static_cast<uint64_t>((box_bytes >> 4) & 0x3FFF) << 16 |
-         static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t{1} << 46 | uint64_t{2} << 61;
-}
-// Step `k` of 16 along the channels of a tile of kRows rows.
+// kRows rows after the other along the channels. An operand's descriptor names
+// where it starts, the stride between eight-row groups and, if the contraction
+// runs along the rows, the stride between boxes. The one thread that issues the
+// products is their bottleneck if it has to assemble descriptors (130 clocks a
+// product, where a product takes 32 to 64), so it only adds to their low words:
+// `channels_word` / `rows_word` of a tile, plus a constant for step k of 16 along
+// the channels or along the rows.
 template <int kRows>
-__device__ __forceinline__ uint64_t along_channels(uint32_t tile, int k) {
-  return describe(tile + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16);
+__device__ __forceinline__ uint32_t channels_word(uint32_t tile) {
+  return (tile >> 4) | 1u << 16;
 }
-// Step `k` of 16 along the rows of a tile of kRows rows.
 template <int kRows>
-__device__ __forceinline__ uint64_t along_rows(uint32_t tile, int k) {
-  return describe(tile + k * 2048, kRows * 128);
+__device__ __forceinline__ constexpr uint32_t channels_step(int k) {
+  return static_cast<uint32_t>((k >> 2) * (kRows * 8) + (k & 3) * 2);
+}
+template <int kRows>
+__device__ __forceinline__ uint32_t rows_word(uint32_t tile) {
+  return (tile >> 4) | static_cast<uint32_t>(kRows * 8) << 16;
+}
+__device__ __forceinline__ constexpr uint32_t rows_step(int k) {
+  return static_cast<uint32_t>(k * 128);
+}
+__device__ __forceinline__ uint64_t descriptor(uint32_t word) {
+  constexpr uint32_t kHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(word), "r"(kHigh));
+  return d;
 }
 
 // What a product of 128 rows and n columns is, for both operands of type T:
@@ -180,22 +189,22 @@ __device__ __forceinline__ uint32_t product_kind(int n, bool rows_b) {
          static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
-// D (+)= A B^T with A and B in shared memory.
-__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind,
+// D (+)= A B^T with A and B in shared memory (low words of descriptors).
+__device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint32_t b, uint32_t kind,
                                          bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+      "l"(descriptor(a)), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add))
       : "memory");
 }
 // D (+)= A B^T with A in tensor memory (two 16-bit values a column).
-__device__ __forceinline__ void multiply_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t kind,
+__device__ __forceinline__ void multiply_tensor(uint32_t d, uint32_t a, uint32_t b, uint32_t kind,
                                                 bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(kind), "r"(static_cast<uint32_t>(add))
+      "r"(a), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add))
       : "memory");
 }
 // The barrier's phase completes when the products issued so far have.
@@ -210,6 +219,27 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two floats at a time in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(y))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(y))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return y;
 }
 // Two floats rounded to the 16-bit type T, the first in the low half.
