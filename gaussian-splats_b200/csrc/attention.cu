@@ -288,69 +288,104 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {  // products
-    if ((threadIdx.x & 31) == 0) {
-      const int dim_steps = (a.dim + 15) / 16;
-      const uint32_t sum_kind = product_kind<T>(dim_steps * 16, true);
-      const uint32_t score_kind = product_kind<T>(0, false);
-      const uint32_t q = channels_word<kTile>(shared_address(s.q[0]));
-      const uint32_t k = channels_word<kKeys>(shared_address(s.k[0]));
-      const uint32_t v = rows_word<kKeys>(shared_address(s.v[0]));
-      const int steps[2] = {walk.steps(0), walk.steps(1)};
-      int keys_here = 0, values_here = 0;  // tiles whose loads have been waited for
-      const auto issue_scores = [&](auto number, int step) {
-        constexpr int g = decltype(number)::value;
-        const int t = walk.tile_of(g, step), stage = t % kStages;
-        const uint32_t kind = score_kind | static_cast<uint32_t>(4 * walk.sets(g, t)) << 17;
-        const bool last = walk.last_reader(g, t);
-        if (step == 0) good = good && barrier_wait(shared_address(&s.q_full[g]), 0);
-        if (t >= keys_here) {
-          good = good && barrier_wait(shared_address(&s.k_full[stage]), (t / kStages) & 1);
-          keys_here = t + 1;
-        }
-        const uint32_t a0 = q + g * (Shared::kQueryBytes >> 4);
-        const uint32_t b0 = k + stage * (Shared::kTileBytes >> 4);
+  } else if (warp == 9) {  // products, issued by the first lane
+    const int lane = threadIdx.x & 31;
+    const int dim_steps = (a.dim + 15) / 16;
+    const uint32_t sum_kind = product_kind<T>(dim_steps * 16, true);
+    const uint32_t score_kind = product_kind<T>(0, false);
+    const uint32_t q = channels_word<kTile>(shared_address(s.q[0]));
+    const uint32_t k = channels_word<kKeys>(shared_address(s.k[0]));
+    const uint32_t v = rows_word<kKeys>(shared_address(s.v[0]));
+    const int steps[2] = {walk.steps(0), walk.steps(1)};
+    // One thread's arithmetic on what a step needs would take longer than the
+    // step's products, so the lanes do it for 32 steps at a time. Eight bits of a
+    // plan are for the values of a step, eight for the keys of the next one:
+    // stage, parity of its load, whether to wait for the load (the tile's first
+    // reader) and to release it (its last reader); then the sets of both.
+    const auto tile_plan = [&](int g, int t) {
+      const bool last = walk.last_reader(g, t), first = !last || !walk.walks(1 - g, t);
+      return static_cast<uint32_t>(t % kStages | ((t / kStages) & 1) << 4 | first << 5 | last << 6);
+    };
+    const auto plan_of = [&](int g, int step) {
+      uint32_t plan = 0;
+      if (step >= 0 && step < steps[g]) {
+        const int t = walk.tile_of(g, step);
+        plan = tile_plan(g, t) | static_cast<uint32_t>(walk.sets(g, t)) << 16;
+      }
+      if (step + 1 < steps[g]) {
+        const int t = walk.tile_of(g, step + 1);
+        plan |= tile_plan(g, t) << 8 | static_cast<uint32_t>(walk.sets(g, t)) << 20;
+      }
+      return plan;
+    };
+    const auto wait_for = [&](uint64_t* bars, uint32_t plan) {
+      if (plan & 32)
+        good = good && barrier_wait_warp(shared_address(&bars[plan & 15]), plan >> 4 & 1);
+    };
+    const auto release = [&](uint64_t* bars, uint32_t plan) {
+      if (plan & 64) commit(shared_address(&bars[plan & 15]));
+    };
+    const auto issue_scores = [&](auto number, uint32_t plan) {
+      constexpr int g = decltype(number)::value;
+      const uint32_t keys = k + (plan >> 8 & 15) * (Shared::kTileBytes >> 4);
+      const uint32_t kind = score_kind | (plan >> 20 & 15) << 19;  // 32 columns a set
 #pragma unroll
-        for (int i = 0; i < kDim / 16; ++i)
-          if (i < dim_steps)
-            multiply(tensor + g * Shape::kGroupColumns, a0 + channels_step<kTile>(i),
-                     b0 + channels_step<kKeys>(i), kind, i > 0);
-        commit(shared_address(&s.scores[g]));
-        if (last) commit(shared_address(&s.k_empty[stage]));
-      };
-      const auto issue_sums = [&](auto number, int step) {
-        constexpr int g = decltype(number)::value;
-        if (step >= steps[g] || !good) return;
-        const int t = walk.tile_of(g, step), stage = t % kStages, sets = walk.sets(g, t);
-        const bool last = walk.last_reader(g, t);
-        if (t >= values_here) {
-          good = barrier_wait(shared_address(&s.v_full[stage]), (t / kStages) & 1);
-          values_here = t + 1;
-        }
-        good = good && barrier_wait(shared_address(&s.weights[g]), step & 1);
-        if (!good) return;
+      for (int i = 0; i < kDim / 16; ++i)
+        if (i < dim_steps)
+          multiply(tensor + g * Shape::kGroupColumns,
+                   q + g * (Shared::kQueryBytes >> 4) + channels_step<kTile>(i),
+                   keys + channels_step<kKeys>(i), kind, i > 0);
+      commit(shared_address(&s.scores[g]));
+    };
+    const auto run_step = [&](auto number, int step, uint32_t plan) {
+      constexpr int g = decltype(number)::value;
+      if (step >= steps[g]) return;
+      const bool more = step + 1 < steps[g];
+      wait_for(s.v_full, plan);
+      if (more) wait_for(s.k_full, plan >> 8);
+      good = good && barrier_wait_warp(shared_address(&s.weights[g]), step & 1);
+      if (good && lane == 0) {
         fence_after_sync();
-        const uint32_t b0 = v + stage * (Shared::kTileBytes >> 4);
         constexpr uint32_t column = g * Shape::kGroupColumns;
+        const uint32_t values = v + (plan & 15) * (Shared::kTileBytes >> 4);
+        const uint32_t count = plan >> 15 & 30;  // two steps of 16 keys a set
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i)
-          if (i < 2 * sets)
-            multiply_tensor(tensor + column + kKeys, tensor + column + 8 * i, b0 + rows_step(i),
-                            sum_kind, step > 0 || i > 0);
-        if (last) commit(shared_address(&s.v_empty[stage]));
-        if (step == steps[g] - 1) commit(shared_address(&s.summed[g]));
-        else issue_scores(number, step + 1);  // in order behind the product that reads P
-      };
-      using First = std::integral_constant<int, 0>;
-      using Second = std::integral_constant<int, 1>;
-      issue_scores(First{}, 0);
-      if (steps[1] > 0) issue_scores(Second{}, 0);
-      for (int step = 0; step < max(steps[0], steps[1]) && good; ++step) {
-        issue_sums(First{}, step);
-        issue_sums(Second{}, step);
+          if (i < count)
+            multiply_tensor(tensor + column + kKeys, tensor + column + 8 * i,
+                            values + rows_step(i), sum_kind, step > 0 || i > 0);
+        if (more) issue_scores(number, plan);  // in order behind the product that reads P
+        else commit(shared_address(&s.summed[g]));
+        release(s.v_empty, plan);
+        if (more) release(s.k_empty, plan >> 8);
       }
-      if (!good) atomicExch(&g_timeout, 1u);
+      __syncwarp();
+    };
+    const auto start = [&](auto number) {
+      constexpr int g = decltype(number)::value;
+      if (steps[g] == 0) return;
+      const uint32_t plan = plan_of(g, -1);
+      wait_for(s.k_full, plan >> 8);
+      good = good && barrier_wait_warp(shared_address(&s.q_full[g]), 0);
+      if (good && lane == 0) {
+        issue_scores(number, plan);
+        release(s.k_empty, plan >> 8);
+      }
+      __syncwarp();
+    };
+    using First = std::integral_constant<int, 0>;
+    using Second = std::integral_constant<int, 1>;
+    start(First{});
+    start(Second{});
+    const int most = max(steps[0], steps[1]);
+    for (int base = 0; base < most && good; base += 32) {
+      const uint32_t first = plan_of(0, base + lane), second = plan_of(1, base + lane);
+      for (int step = base; step < min(base + 32, most) && good; ++step) {
+        run_step(First{}, step, __shfl_sync(0xffffffffu, first, step - base));
+        run_step(Second{}, step, __shfl_sync(0xffffffffu, second, step - base));
+      }
     }
+    if (!good && lane == 0) atomicExch(&g_timeout, 1u);
     __syncwarp();
   } else {
     const int group = warp >> 2, row = threadIdx.x & (kTile - 1);
