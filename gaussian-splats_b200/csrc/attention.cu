@@ -396,54 +396,57 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
     const float scale = a.scale * kLog2e;
     float top = -INFINITY, sum = 0.0f;
     const int steps = walk.steps(group);
+    // Every query of the group sees every valid key of a tile that lies from
+    // `from` (or under `first`) to `to`.
+    const int from = position(int64_t{i_first} + kTile - 1 - a.left);
+    const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
     for (int step = 0; step < steps; ++step) {
       const int t = walk.tile_of(group, step), start = walk.start(t), end = walk.end(t);
-      const int sets = walk.sets(group, t);
+      bool whole = t < walk.head_tiles
+                       ? start + kKeys <= end
+                       : start + kKeys <= to && (start >= from || start + kKeys <= a.first);
+      bool all = whole;  // the keys are all valid
       uint32_t keep[kSets];
-      bool all = true;
+      if (a.valid || !whole) {
+        all = true;
 #pragma unroll
-      for (int c = 0; c < kSets; ++c) {
-        keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
-                             max(0, min(end - start - 32 * c, 32)));
-        all = all && keep[c] == ~0u;
+        for (int c = 0; c < kSets; ++c) {
+          keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
+                               max(0, min(end - start - 32 * c, 32)));
+          all = all && keep[c] == ~0u;
+        }
+        whole = whole && all;
       }
-      // Whether every query of the group sees every key of the tile.
-      const bool whole =
-          all && (t < walk.head_tiles ||
-                  (start + kKeys <= position(int64_t{i_first} + a.right + 1) &&
-                   (start >= position(int64_t{i_first} + kTile - 1 - a.left) ||
-                    start + kKeys <= a.first)));
       good = good && barrier_wait_warp(shared_address(&s.scores[group]), step & 1);
       if (!good) break;
       fence_after_sync();
+      // All columns, also where the products made fewer: what is not seen is
+      // masked, and straight code is worth more than a few exponentials.
       float x[kSets][32];
 #pragma unroll
-      for (int c = 0; c < kSets; ++c)
-        if (c < sets) load_columns32(scores + 32 * c, x[c]);
+      for (int c = 0; c < kSets; ++c) load_columns32(scores + 32 * c, x[c]);
       wait_loads();
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < kSets; ++c)
-          if (c < sets) {
-            const uint32_t bits = keep[c] & window_bits(a, i, start + 32 * c, end);
+        for (int c = 0; c < kSets; ++c) {
+          const uint32_t bits = keep[c] & window_bits(a, i, start + 32 * c, end);
+          if (!__all_sync(0xffffffffu, bits == ~0u)) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[c][e] = bits >> e & 1 ? x[c][e] : -INFINITY;
           }
+        }
       }
-      float next = -INFINITY;
+      float high[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) high[k] = fmaxf(x[0][k], x[0][k + 8]);
 #pragma unroll
       for (int c = 0; c < kSets; ++c)
-        if (c < sets) {
-          float high[4] = {x[c][0], x[c][1], x[c][2], x[c][3]};
 #pragma unroll
-          for (int e = 4; e < 32; e += 8)
+        for (int e = c == 0 ? 16 : 0; e < 32; e += 16)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              high[k] = e + 4 < 32 ? max3(high[k], x[c][e + k], x[c][e + 4 + k])
-                                   : fmaxf(high[k], x[c][e + k]);
-          next = max3(next, max3(high[0], high[1], high[2]), high[3]);
-        }
-      next *= scale;
+          for (int k = 0; k < 8; ++k) high[k] = max3(high[k], x[c][e + k], x[c][e + k + 8]);
+      const float next = max3(max3(high[0], high[1], high[2]), max3(high[3], high[4], high[5]),
+                              fmaxf(high[6], high[7])) * scale;
       // Sums of earlier tiles are complete: this tile's S came behind them.
       const bool grow = next > top + kSlack || (top == -INFINITY && next > top);
       if (__any_sync(0xffffffffu, grow)) {
@@ -463,23 +466,21 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
         }
       }
       // Where nothing is seen yet any finite shift will do: exp2(-inf) is 0.
-      const float2 shift = make_float2(top == -INFINITY ? 0.0f : -top, top == -INFINITY ? 0.0f : -top);
-      const float2 factor = make_float2(scale, scale);
+      const float down = top == -INFINITY ? 0.0f : -top;
+      const float2 shift = make_float2(down, down), factor = make_float2(scale, scale);
       float2 part[2] = {};
 #pragma unroll
-      for (int c = 0; c < kSets; ++c)
-        if (c < sets) {
-          uint32_t packed[16];
+      for (int c = 0; c < kSets; ++c) {
+        uint32_t packed[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 y =
-                fma2(make_float2(x[c][2 * e], x[c][2 * e + 1]), factor, shift);
-            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-            part[e & 1] = add2(part[e & 1], p);
-            packed[e] = pack2<T>(p.x, p.y);
-          }
-          store_columns16(scores + 16 * c, packed);
+        for (int e = 0; e < 16; ++e) {
+          const float2 y = fma2(make_float2(x[c][2 * e], x[c][2 * e + 1]), factor, shift);
+          const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          part[e & 1] = add2(part[e & 1], p);
+          packed[e] = pack2<T>(p.x, p.y);
         }
+        store_columns16(scores + 16 * c, packed);
+      }
       sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
       if (!all) {
         const int stage = t % kStages;
