@@ -558,7 +558,7 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 //
 // so that every sum has one owner and one order: no atomics, and the query
 // heads that share a key-value head are summed where its keys are. Eight warps
-// split the tile's columns in halves; the ninth's first thread loads and issues.
+// split the tile's columns in halves; a ninth loads, a tenth issues the products.
 //
 // First tokens are seen by all later queries, so the block of their keys would
 // walk the whole sequence. It walks its window like the others; the queries
@@ -585,67 +585,99 @@ struct BackwardShared {
   using Shape = BackwardShape<kDim>;
   alignas(1024) unsigned char rows[2][Shape::kRowBytes];
   unsigned char tiles[Shape::kStages][2][Shape::kTileBytes];
-  float row[2][2][kKeys];  // keys' kernel: L and D of a tile's queries
-  float half[2][kTile];    // queries' kernel: halves of D
+  float row[Shape::kStages][2][kKeys];  // keys' kernel: -L and -D of a tile's queries
+  float half[2][kTile];                 // queries' kernel: halves of D
   uint64_t rows_full, full[Shape::kStages];  // loads
+  uint64_t empty[Shape::kStages];            // a tile's sums are complete
   uint64_t scores[Shape::kBuffers];          // S and G of a tile are complete
   uint64_t weights[Shape::kBuffers];         // P and E are written (256 arrivals)
-  uint64_t summed;                           // a tile's sums are complete
-  uint64_t done;                             // all of them are
+  uint64_t done;                             // all sums are complete
   uint32_t tensor;
 };
 
 constexpr int kComputeThreads = 256;
+constexpr int kBackwardThreads = kComputeThreads + 64;
 
 // Where step k of 16 of a tile's 64 weights lies: each half of the warps writes
 // over the first of the 32 columns that it read.
-__device__ __forceinline__ uint32_t weight_column(int k) { return (k >> 1) * 32 + (k & 1) * 8; }
+__device__ __forceinline__ constexpr uint32_t weight_column(int k) {
+  return (k >> 1) * 32 + (k & 1) * 8;
+}
 
-// The ninth warp's thread. `place(t)` names the head and row of tile t.
-template <class T, int kDim, bool kKeyRows, class Place>
-__device__ __forceinline__ bool drive(BackwardShared<kDim>& s, int dim, int tiles,
-                                      const CUtensorMap* row_map0, const CUtensorMap* row_map1,
-                                      int row_head, int row, const CUtensorMap* tile_map0,
-                                      const CUtensorMap* tile_map1, const Place& place) {
+// The ninth warp: loads. `place(t)` names the head and row of tile t; `rows(t,
+// lane)` loads what else a tile needs and `keep(stage, ...)` puts it to shared
+// memory, all lanes taking part.
+template <int kDim, class Place, class Rows, class Keep>
+__device__ __forceinline__ void load_tiles(BackwardShared<kDim>& s, int tiles,
+                                           const CUtensorMap* row_map0,
+                                           const CUtensorMap* row_map1, int row_head, int row,
+                                           const CUtensorMap* tile_map0,
+                                           const CUtensorMap* tile_map1, const Place& place,
+                                           const Rows& rows, const Keep& keep) {
+  using namespace tc;
+  using Shape = BackwardShape<kDim>;
+  constexpr int kStages = Shape::kStages;
+  const int lane = threadIdx.x & 31;
+  bool good = true;
+  if (lane == 0) {
+    const uint32_t bar = shared_address(&s.rows_full);
+    barrier_expect(bar, 2 * Shape::kRowBytes);
+    for (int x = 0; x < kDim / 64; ++x) {
+      load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row, bar);
+      load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row, bar);
+    }
+  }
+  auto ahead = rows(0, lane);
+  for (int t = 0; t < tiles; ++t) {
+    const int stage = t % kStages;
+    const auto values = ahead;
+    if (t + 1 < tiles) ahead = rows(t + 1, lane);
+    if (t >= kStages)
+      good = good && barrier_wait_warp(shared_address(&s.empty[stage]), (t / kStages - 1) & 1);
+    if (!good) break;
+    const uint32_t bar = shared_address(&s.full[stage]);
+    keep(stage, lane, values);
+    if (lane == 0) {
+      const int2 at = place(t);
+      barrier_expect(bar, 2 * Shape::kTileBytes);
+      for (int x = 0; x < kDim / 64; ++x) {
+        load_box(shared_address(s.tiles[stage][0]) + x * kKeys * 128, tile_map0, 64 * x, at.x,
+                 at.y, bar);
+        load_box(shared_address(s.tiles[stage][1]) + x * kKeys * 128, tile_map1, 64 * x, at.x,
+                 at.y, bar);
+      }
+    } else {
+      barrier_arrive(bar);
+    }
+  }
+  if (!good) {  // let what is in flight land before the shared memory is given back
+    for (uint64_t& b : s.full)
+      for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+    if (lane == 0) atomicExch(&g_timeout, 1u);
+  }
+  __syncwarp();
+}
+
+// The tenth warp: products, issued by its first lane.
+template <class T, int kDim, bool kKeyRows>
+__device__ __forceinline__ void issue_products(BackwardShared<kDim>& s, int dim, int tiles) {
   using namespace tc;
   using Shape = BackwardShape<kDim>;
   constexpr int kBuffers = Shape::kBuffers, kStages = Shape::kStages;
+  constexpr uint32_t kStageWords = 2 * Shape::kTileBytes >> 4, kHalfWords = Shape::kTileBytes >> 4;
   const uint32_t tensor = s.tensor;
-  const auto load_tile = [&](int t) {
-    const int stage = t % kStages;
-    const uint32_t bar = shared_address(&s.full[stage]);
-    const int2 at = place(t);
-    barrier_expect(bar, 2 * Shape::kTileBytes);
-    for (int x = 0; x < kDim / 64; ++x) {
-      load_box(shared_address(s.tiles[stage][0]) + x * kKeys * 128, tile_map0, 64 * x, at.x, at.y,
-               bar);
-      load_box(shared_address(s.tiles[stage][1]) + x * kKeys * 128, tile_map1, 64 * x, at.x, at.y,
-               bar);
-    }
-  };
-  const uint32_t rows_full = shared_address(&s.rows_full);
-  barrier_expect(rows_full, 2 * Shape::kRowBytes);
-  for (int x = 0; x < kDim / 64; ++x) {
-    load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row,
-             rows_full);
-    load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row,
-             rows_full);
-  }
-  for (int t = 0; t < kStages && t < tiles; ++t) load_tile(t);
-
+  const bool issues = (threadIdx.x & 31) == 0;
   const int steps = (dim + 15) / 16;
   const uint32_t score_kind = product_kind<T>(kKeys, false);
   const uint32_t sum_kind = product_kind<T>((dim + 15) / 16 * 16, true);
   const uint32_t rows0 = channels_word<kTile>(shared_address(s.rows[0]));
   const uint32_t rows1 = channels_word<kTile>(shared_address(s.rows[1]));
-  const uint32_t tiles0 = shared_address(s.tiles[0][0]);
-  constexpr uint32_t kStageWords = 2 * Shape::kTileBytes >> 4, kHalfWords = Shape::kTileBytes >> 4;
-  bool good = barrier_wait(rows_full, 0);
-  const auto issue_scores = [&](int t) {
-    const int stage = t % kStages;
-    good = good && barrier_wait(shared_address(&s.full[stage]), (t / kStages) & 1);
-    const uint32_t tile = channels_word<kKeys>(tiles0) + stage * kStageWords;
-    const uint32_t d = tensor + (t % kBuffers) * Shape::kBuffer;
+  const uint32_t by_channels = channels_word<kKeys>(shared_address(s.tiles[0][0]));
+  const uint32_t by_rows = rows_word<kKeys>(shared_address(s.tiles[0][0]));
+  // S and G of the tile in a stage, to a buffer.
+  const auto issue_scores = [&](int stage, int buffer) {
+    const uint32_t tile = by_channels + stage * kStageWords;
+    const uint32_t d = tensor + buffer * Shape::kBuffer;
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
       if (i < steps)
@@ -656,41 +688,58 @@ __device__ __forceinline__ bool drive(BackwardShared<kDim>& s, int dim, int tile
       if (i < steps)
         multiply(d + Shape::kGrad, rows1 + channels_step<kTile>(i),
                  tile + kHalfWords + channels_step<kKeys>(i), score_kind, i > 0);
-    commit(shared_address(&s.scores[t % kBuffers]));
+    commit(shared_address(&s.scores[buffer]));
   };
-  for (int t = 0; t < kBuffers && t < tiles; ++t) issue_scores(t);
-  for (int t = 0; t < tiles && good; ++t) {
-    const int buffer = t % kBuffers, stage = t % kStages;
-    good = barrier_wait(shared_address(&s.weights[buffer]), (t / kBuffers) & 1);
-    if (!good) break;
-    fence_after_sync();
-    if (t >= 1) {  // waited for before the next phase can complete
-      good = barrier_wait(shared_address(&s.summed), (t - 1) & 1);
-      if (!good) break;
-      if (t - 1 + kStages < tiles) load_tile(t - 1 + kStages);
+  bool good = barrier_wait_warp(shared_address(&s.rows_full), 0);
+  int ahead = 0, ahead_parity = 0;  // stage and parity of the tile whose S is next
+  const auto wait_ahead = [&] {
+    good = good && barrier_wait_warp(shared_address(&s.full[ahead]), ahead_parity);
+  };
+  const auto step_ahead = [&] {
+    if (++ahead == kStages) {
+      ahead = 0;
+      ahead_parity ^= 1;
     }
-    const uint32_t d = tensor + buffer * Shape::kBuffer;
-    const uint32_t tile = rows_word<kKeys>(tiles0) + stage * kStageWords;
-#pragma unroll
-    for (int i = 0; i < kKeys / 16; ++i)
-      multiply_tensor(tensor + Shape::kSum, d + Shape::kGrad + weight_column(i),
-                      tile + rows_step(i), sum_kind, t > 0 || i > 0);
-    if constexpr (kKeyRows) {
+  };
+  for (int t = 0; t < kBuffers && t < tiles; ++t) {
+    wait_ahead();
+    if (good && issues) issue_scores(ahead, t);
+    __syncwarp();
+    step_ahead();
+  }
+  int stage = 0, buffer = 0, parity = 0;
+  for (int t = 0; t < tiles && good; ++t) {
+    const bool more = t + kBuffers < tiles;
+    if (more) wait_ahead();
+    good = good && barrier_wait_warp(shared_address(&s.weights[buffer]), parity);
+    if (good && issues) {
+      fence_after_sync();
+      const uint32_t d = tensor + buffer * Shape::kBuffer;
+      const uint32_t tile = by_rows + stage * kStageWords;
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i)
-        multiply_tensor(tensor + Shape::kSum + kDim, d + Shape::kScore + weight_column(i),
-                        tile + kHalfWords + rows_step(i), sum_kind, t > 0 || i > 0);
+        multiply_tensor(tensor + Shape::kSum, d + Shape::kGrad + weight_column(i),
+                        tile + rows_step(i), sum_kind, t > 0 || i > 0);
+      if constexpr (kKeyRows) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          multiply_tensor(tensor + Shape::kSum + kDim, d + Shape::kScore + weight_column(i),
+                          tile + kHalfWords + rows_step(i), sum_kind, t > 0 || i > 0);
+      }
+      // In order behind the sums that read this buffer's weights.
+      if (more) issue_scores(ahead, buffer);
+      commit(shared_address(t == tiles - 1 ? &s.done : &s.empty[stage]));
     }
-    commit(shared_address(&s.summed));
-    if (t == tiles - 1) commit(shared_address(&s.done));
-    // Behind the sums that read this buffer's weights.
-    if (t + kBuffers < tiles) issue_scores(t + kBuffers);
+    __syncwarp();
+    step_ahead();
+    if (++stage == kStages) stage = 0;
+    if (++buffer == kBuffers) {
+      buffer = 0;
+      parity ^= 1;
+    }
   }
-  if (good) return true;
-  // Let what is in flight land before the shared memory is given back.
-  for (uint64_t& b : s.full)
-    for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
-  return false;
+  if (!good && issues) atomicExch(&g_timeout, 1u);
+  __syncwarp();
 }
 
 template <int kDim>
@@ -698,15 +747,15 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim>& s, int warp
   using namespace tc;
   if (threadIdx.x == 0) {
     barrier_init(shared_address(&s.rows_full), 1);
-    for (uint64_t& b : s.full) barrier_init(shared_address(&b), 1);
+    for (uint64_t& b : s.full) barrier_init(shared_address(&b), 32);
+    for (uint64_t& b : s.empty) barrier_init(shared_address(&b), 1);
     for (uint64_t& b : s.scores) barrier_init(shared_address(&b), 1);
     for (uint64_t& b : s.weights) barrier_init(shared_address(&b), kComputeThreads);
-    barrier_init(shared_address(&s.summed), 1);
     barrier_init(shared_address(&s.done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
-  if (warp == 8) tensor_alloc<kDim == 64 ? 256 : 512>(shared_address(&s.tensor));
+  if (warp == 9) tensor_alloc<kDim == 64 ? 256 : 512>(shared_address(&s.tensor));
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -724,7 +773,7 @@ __device__ __forceinline__ float weight_shift(float lse) {
 
 // dq, and D_i into `delta` for the keys' kernel.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBlocks)
+__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks)
     grad_query_kernel(gs_window_attention_args a, float* delta,
                       const __grid_constant__ CUtensorMap q_map,
                       const __grid_constant__ CUtensorMap g_map,
@@ -743,13 +792,12 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
   if (warp == 8) {
-    if ((threadIdx.x & 31) == 0 &&
-        !drive<T, kDim, false>(s, a.dim, walk.tiles, &q_map, &g_map, head, tile.start, &k_map,
-                               &v_map, [&](int t) {
-                                 return make_int2(kv_head, tile.begin + walk.start(t));
-                               }))
-      atomicExch(&g_timeout, 1u);
-    __syncwarp();
+    load_tiles<kDim>(
+        s, walk.tiles, &q_map, &g_map, head, tile.start, &k_map, &v_map,
+        [&](int t) { return make_int2(kv_head, tile.begin + walk.start(t)); },
+        [](int, int) { return 0; }, [](int, int, int) {});
+  } else if (warp == 9) {
+    issue_products<T, kDim, false>(s, a.dim, walk.tiles);
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -772,45 +820,54 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
     if (live && half == 0) delta[slot] = d;
     const float shift = live ? weight_shift(a.lse[slot]) : INFINITY;
     const float scale = a.scale * kLog2e;
+    // Every query sees every valid key of a tile that lies from `from` (or under
+    // `first`) to `to`.
+    const int from = position(int64_t{i_first} + kTile - 1 - a.left);
+    const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
+    const float2 factor = make_float2(scale, scale), down = make_float2(-shift, -shift);
+    const float2 less = make_float2(-d, -d);
     bool good = true;
+    int stage = 0, buffer = 0, parity = 0;
     for (int t = 0; t < walk.tiles; ++t) {
       const int start = walk.start(t), end = walk.end(t);
-      uint32_t keep[2];
+      bool whole = t < walk.head_tiles
+                       ? start + kKeys <= end
+                       : start + kKeys <= to && (start >= from || start + kKeys <= a.first);
+      bool all = whole;
+      uint32_t keep[2], bits = ~0u;
+      if (a.valid || !whole) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
-                             max(0, min(end - start - 32 * c, 32)));
-      const bool all = (keep[0] & keep[1]) == ~0u;
-      const bool whole =
-          all && (t < walk.head_tiles ||
-                  (start + kKeys <= position(int64_t{i_first} + a.right + 1) &&
-                   (start >= position(int64_t{i_first} + kTile - 1 - a.left) ||
-                    start + kKeys <= a.first)));
-      const uint32_t bits = keep[half] & window_bits(a, i, start + 32 * half, end);
-      const int buffer = t % Shape::kBuffers;
-      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), (t / Shape::kBuffers) & 1)))
-        break;
+        for (int c = 0; c < 2; ++c)
+          keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
+                               max(0, min(end - start - 32 * c, 32)));
+        all = (keep[0] & keep[1]) == ~0u;
+        whole = whole && all;
+        bits = keep[half] & window_bits(a, i, start + 32 * half, end);
+      }
+      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), parity))) break;
       fence_after_sync();
-      const uint32_t from = mine + buffer * Shape::kBuffer + 32 * half;
+      const uint32_t columns = mine + buffer * Shape::kBuffer + 32 * half;
       float x[32], g[32];
-      load_columns32(from + Shape::kScore, x);
-      load_columns32(from + Shape::kGrad, g);
+      load_columns32(columns + Shape::kScore, x);
+      load_columns32(columns + Shape::kGrad, g);
       wait_loads();
-      uint32_t packed[16];
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        float e[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float p = exp2_approx(fmaf(x[2 * c + k], scale, -shift));
-          e[k] = p * (g[2 * c + k] - d);
-          if (!whole && !(bits >> (2 * c + k) & 1)) e[k] = 0.0f;
-        }
-        packed[c] = pack2<T>(e[0], e[1]);
+        const float2 y = fma2(make_float2(x[2 * c], x[2 * c + 1]), factor, down);
+        const float2 e = mul2(make_float2(exp2_approx(y.x), exp2_approx(y.y)),
+                              add2(make_float2(g[2 * c], g[2 * c + 1]), less));
+        x[2 * c] = e.x;
+        x[2 * c + 1] = e.y;
       }
-      store_columns16(from + Shape::kGrad, packed);
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = bits >> c & 1 ? x[c] : 0.0f;
+      }
+      uint32_t packed[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
+      store_columns16(columns + Shape::kGrad, packed);
       if (!all) {
-        const int stage = t % Shape::kStages;
         if (!(good = barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1)))
           break;
         zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
@@ -819,6 +876,11 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
       wait_stores();
       fence_before_sync();
       barrier_arrive(shared_address(&s.weights[buffer]));
+      if (++stage == Shape::kStages) stage = 0;
+      if (++buffer == Shape::kBuffers) {
+        buffer = 0;
+        parity ^= 1;
+      }
     }
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
@@ -841,7 +903,7 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 8) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+  if (warp == 9) tensor_free<kDim == 64 ? 256 : 512>(tensor);
 }
 
 // The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
@@ -859,7 +921,7 @@ __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a,
 
 // dk and dv.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBlocks)
+__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks)
     grad_key_kernel(gs_window_attention_args a, const float* delta, FirstSums sums,
                     const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map,
@@ -898,15 +960,35 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
   if (warp == 8) {
-    if ((threadIdx.x & 31) == 0 &&
-        !drive<T, kDim, true>(s, a.dim, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
-                              [&](int t) {
-                                return make_int2(kv_head * group + t / per_head,
-                                                 tile.begin + static_cast<int>(low) +
-                                                     (t % per_head) * kKeys);
-                              }))
-      atomicExch(&g_timeout, 1u);
-    __syncwarp();
+    // L and D of a tile's queries come along, negated, two of each a lane.
+    load_tiles<kDim>(
+        s, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
+        [&](int t) {
+          return make_int2(kv_head * group + t / per_head,
+                           tile.begin + static_cast<int>(low) + (t % per_head) * kKeys);
+        },
+        [&](int t, int lane) {
+          float4 v = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+          const int64_t i = low + (t % per_head) * kKeys + lane;
+          const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
+          if (i < n) {
+            v.x = -weight_shift(a.lse[at]);
+            v.z = -delta[at];
+          }
+          if (i + 32 < n) {
+            v.y = -weight_shift(a.lse[at + 32]);
+            v.w = -delta[at + 32];
+          }
+          return v;
+        },
+        [&](int stage, int lane, const float4& v) {
+          s.row[stage][0][lane] = v.x;
+          s.row[stage][0][lane + 32] = v.y;
+          s.row[stage][1][lane] = v.z;
+          s.row[stage][1][lane + 32] = v.w;
+        });
+  } else if (warp == 9) {
+    issue_products<T, kDim, true>(s, a.dim, tiles);
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -915,79 +997,83 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
     const bool seen = live && (!a.valid || a.valid[tile.start + row]);
     const bool any_seen = __any_sync(0xffffffffu, seen), all_seen = __all_sync(0xffffffffu, seen);
     const float scale = a.scale * kLog2e;
-    // L and D of tile t's queries, 64 of each, a tile ahead.
-    const auto row_value = [&](int t) {
-      const int c = threadIdx.x & (kKeys - 1);
-      const int64_t i = low + (t % per_head) * kKeys + c;
-      const bool in = threadIdx.x < 2 * kKeys && t < tiles && i < n;
-      const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
-      if (threadIdx.x < kKeys) return in ? weight_shift(a.lse[at]) : INFINITY;
-      return in ? delta[at] : 0.0f;
-    };
-    if (threadIdx.x < 2 * kKeys) s.row[0][threadIdx.x / kKeys][threadIdx.x % kKeys] = row_value(0);
-    sync_compute();
+    const float2 factor = make_float2(scale, scale);
     bool good = true;
+    int stage = 0, full_parity = 0, buffer = 0, parity = 0, index = 0;
     for (int t = 0; t < tiles; ++t) {
-      const float ahead = row_value(t + 1);
-      const int64_t start = low + (t % per_head) * kKeys;
+      const int64_t start = low + index * kKeys;
       uint64_t wide = seen ? below(high - start) : 0;
       if (chunk) wide &= ~below(j + a.left + 1 - start);
       else wide &= below(j + a.left + 1 - start) & ~below(j - a.right - start);
       const uint32_t bits = static_cast<uint32_t>(wide >> (32 * half));
       const bool whole = __all_sync(0xffffffffu, bits == ~0u);
-      const int buffer = t % Shape::kBuffers;
-      // After a wait that ran out the walk goes on without waiting, for the
-      // barriers that all warps meet at.
-      good = good &&
-             barrier_wait_warp(shared_address(&s.scores[buffer]), (t / Shape::kBuffers) & 1);
+      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), parity) &&
+                   barrier_wait_warp(shared_address(&s.full[stage]), full_parity)))
+        break;
       fence_after_sync();
-      const uint32_t from = mine + buffer * Shape::kBuffer + 32 * half;
+      const uint32_t columns = mine + buffer * Shape::kBuffer + 32 * half;
       uint32_t weight[16], packed[16];
       if (any_seen) {
         float x[32], g[32];
-        load_columns32(from + Shape::kScore, x);
-        load_columns32(from + Shape::kGrad, g);
+        load_columns32(columns + Shape::kScore, x);
+        load_columns32(columns + Shape::kGrad, g);
         wait_loads();
-        const float4* shifts = reinterpret_cast<const float4*>(s.row[t & 1][0] + 32 * half);
-        const float4* deltas = reinterpret_cast<const float4*>(s.row[t & 1][1] + 32 * half);
+        const float4* shifts = reinterpret_cast<const float4*>(s.row[stage][0] + 32 * half);
+        const float4* deltas = reinterpret_cast<const float4*>(s.row[stage][1] + 32 * half);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const float4 l4 = shifts[c], d4 = deltas[c];
-          const float l[4] = {l4.x, l4.y, l4.z, l4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
-          float p[4], e[4];
+          const float4 l = shifts[c], d = deltas[c];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            p[k] = exp2_approx(fmaf(x[4 * c + k], scale, -l[k]));
-            e[k] = p[k] * (g[4 * c + k] - d[k]);
-            if (!whole && !(bits >> (4 * c + k) & 1)) p[k] = e[k] = 0.0f;
+          for (int k = 0; k < 2; ++k) {
+            const int at = 4 * c + 2 * k;
+            const float2 y = fma2(make_float2(x[at], x[at + 1]), factor,
+                                  k ? make_float2(l.z, l.w) : make_float2(l.x, l.y));
+            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+            const float2 e = mul2(p, add2(make_float2(g[at], g[at + 1]),
+                                          k ? make_float2(d.z, d.w) : make_float2(d.x, d.y)));
+            x[at] = p.x;
+            x[at + 1] = p.y;
+            g[at] = e.x;
+            g[at + 1] = e.y;
           }
-          weight[2 * c] = pack2<T>(p[0], p[1]);
-          weight[2 * c + 1] = pack2<T>(p[2], p[3]);
-          packed[2 * c] = pack2<T>(e[0], e[1]);
-          packed[2 * c + 1] = pack2<T>(e[2], e[3]);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            x[c] = bits >> c & 1 ? x[c] : 0.0f;
+            g[c] = bits >> c & 1 ? g[c] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          weight[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
+          packed[c] = pack2<T>(g[2 * c], g[2 * c + 1]);
         }
       } else {
 #pragma unroll
         for (int c = 0; c < 16; ++c) weight[c] = packed[c] = 0;
       }
-      store_columns16(from + Shape::kScore, weight);
-      store_columns16(from + Shape::kGrad, packed);
+      store_columns16(columns + Shape::kScore, weight);
+      store_columns16(columns + Shape::kGrad, packed);
       if (start + kKeys > n) {
-        const int stage = t % Shape::kStages;
-        good =
-            good && barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1);
         const int rest = n - static_cast<int>(start);
         const uint32_t keep[2] = {below32(rest), below32(rest - 32)};
         zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
         zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][1], keep, threadIdx.x);
         fence_async_shared();
       }
-      if (threadIdx.x < 2 * kKeys)
-        s.row[(t + 1) & 1][threadIdx.x / kKeys][threadIdx.x % kKeys] = ahead;
       wait_stores();
       fence_before_sync();
       barrier_arrive(shared_address(&s.weights[buffer]));
-      sync_compute();  // the next tile's L and D are there
+      if (++index == per_head) index = 0;
+      if (++stage == Shape::kStages) {
+        stage = 0;
+        full_parity ^= 1;
+      }
+      if (++buffer == Shape::kBuffers) {
+        buffer = 0;
+        parity ^= 1;
+      }
     }
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
@@ -1020,7 +1106,7 @@ __global__ void __launch_bounds__(kComputeThreads + 32, BackwardShape<kDim>::kBl
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 8) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+  if (warp == 9) tensor_free<kDim == 64 ? 256 : 512>(tensor);
 }
 
 // dk and dv of first tokens: their window's sum and the chunks' in order, a
@@ -1106,11 +1192,11 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
   launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kComputeThreads + 32, kShared, stream, a, delta, rows[0], rows[1],
+                        kBackwardThreads, kShared, stream, a, delta, rows[0], rows[1],
                         tiles[2], tiles[3]);
   GS_TRY(check_launch());
   launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
-                        kComputeThreads + 32, kShared, stream, a, delta, sums, rows[2], rows[3],
+                        kBackwardThreads, kShared, stream, a, delta, sums, rows[2], rows[3],
                         tiles[0], tiles[1]);
   GS_TRY(check_launch());
   if (first_blocks > 0)

@@ -242,6 +242,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return y;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 y;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(y))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return y;
+}
 // Two floats rounded to the 16-bit type T, the first in the low half.
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float low, float high) {
