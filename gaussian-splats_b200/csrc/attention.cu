@@ -549,213 +549,250 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // ------------------------------------------------- whole sequences, backward
 //
 // Two kernels of one shape: a block holds 128 rows of two operands (queries and
-// their gradients, or keys and values) and walks over tiles of 64 rows of the
+// their gradients, or keys and values) and walks over tiles of 128 rows of the
 // other two, recomputing the scores,
 //
-//   S = rows0 tile0^T,  G = rows1 tile1^T      (tensor memory, floats)
-//   P = exp2(S scale log2 e - L),  E = P (G - D)  (16 bits, over S and G)
+//   S = rows0 tile0^T,  G = rows1 tile1^T          (tensor memory, floats)
+//   P = exp2(S scale log2 e - L),  E = P (G - D)   (16 bits)
 //   queries: dQ += E tile0;   keys: dK += E tile0, dV += P tile1
 //
 // so that every sum has one owner and one order: no atomics, and the query
-// heads that share a key-value head are summed where its keys are. Eight warps
-// split the tile's columns in halves; a ninth loads, a tenth issues the products.
+// heads that share a key-value head are summed where its keys are. Seven products
+// instead of the five of a kernel that adds to dQ from many blocks.
 //
+// Eight warps hold half a row a thread, a ninth loads, a tenth issues the
+// products, which are what bounds the kernels: a 128 x 128 x 16 product takes 64
+// clocks, as does one of 64 columns, because shared memory delivers the 128 rows
+// no faster (with tiles of 64 rows: 1577 and 1670 us where this takes the times
+// below). To keep the tensor cores busy, S of the next tile follows as soon as
+// this one's has been read (queries) or used (keys), while the warps work on G,
+// and G of the next while they work on S.
+
 // First tokens are seen by all later queries, so the block of their keys would
 // walk the whole sequence. It walks its window like the others; the queries
 // further on are cut into chunks with a block each, and a last kernel adds the
 // chunks' sums in order.
 
-constexpr int kKeys = 64;  // rows of the backward's tiles
-
-template <int kDim>
+template <int kDim, bool kKeyRows>
 struct BackwardShape {
-  // At 64 channels two blocks share a multiprocessor and hide each other's
-  // waits; at 128 the operands of one fill it, and it works on two tiles at once.
-  static constexpr int kBuffers = kDim == 64 ? 1 : 2;
-  static constexpr int kStages = kDim == 64 ? 3 : 4;
-  static constexpr int kBlocks = kDim == 64 ? 2 : 1;
-  static constexpr int kRowBytes = kTile * kDim * 2, kTileBytes = kKeys * kDim * 2;
-  static constexpr int kScore = 0, kGrad = kKeys;  // columns of a buffer
-  static constexpr int kBuffer = 2 * kKeys;
-  static constexpr int kSum = kBuffers * kBuffer;  // columns of the first sum
+  // Tiles of operand 0 wait for the sums, those of operand 1 no longer than for
+  // G: at 128 channels there is room for three of the one and two of the other.
+  static constexpr int kStages0 = kDim == 64 ? 4 : 3, kStages1 = kDim == 64 ? 3 : 2;
+  static constexpr int kBytes = kTile * kDim * 2;  // of an operand's rows
+  // Columns of tensor memory. E lies over G, and the keys' P over S; the queries
+  // have room for G twice.
+  static constexpr int kGrad = kTile, kGrads = kKeyRows ? 1 : 2;
+  static constexpr int kSum = kGrad + kGrads * kTile;
 };
 
-template <int kDim>
+template <int kDim, bool kKeyRows>
 struct BackwardShared {
-  using Shape = BackwardShape<kDim>;
-  alignas(1024) unsigned char rows[2][Shape::kRowBytes];
-  unsigned char tiles[Shape::kStages][2][Shape::kTileBytes];
-  float row[Shape::kStages][2][kKeys];  // keys' kernel: -L and -D of a tile's queries
-  float half[2][kTile];                 // queries' kernel: halves of D
-  uint64_t rows_full, full[Shape::kStages];  // loads
-  uint64_t empty[Shape::kStages];            // a tile's sums are complete
-  uint64_t scores[Shape::kBuffers];          // S and G of a tile are complete
-  uint64_t weights[Shape::kBuffers];         // P and E are written (256 arrivals)
-  uint64_t done;                             // all sums are complete
+  using Shape = BackwardShape<kDim, kKeyRows>;
+  static constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
+  alignas(1024) unsigned char rows[2][Shape::kBytes];
+  unsigned char tiles0[kStages0][Shape::kBytes];
+  unsigned char tiles1[kStages1][Shape::kBytes];
+  union {
+    float row[kStages1][2][kTile];  // keys: -L and -D of a tile's queries
+    float part[2][kTile];           // queries: halves of D
+  };
+  uint64_t rows_full, full0[kStages0], full1[kStages1];  // loads
+  uint64_t empty[kStages0];                              // a tile's sums are complete
+  uint64_t scores, grads[2];  // S, G of a tile are complete
+  uint64_t read;     // S is read (queries), P is written (keys): 256 arrivals
+  // E is written (256 arrivals). The queries' next S and G do not wait for it, so
+  // a warp may be a tile ahead of another: even and odd tiles have one each.
+  uint64_t weights[2];
+  uint64_t done;     // all sums are complete
   uint32_t tensor;
 };
 
 constexpr int kComputeThreads = 256;
+constexpr int kLoadWarp = kComputeThreads / 32, kProductWarp = kLoadWarp + 1;
 constexpr int kBackwardThreads = kComputeThreads + 64;
 
-// Where step k of 16 of a tile's 64 weights lies: each half of the warps writes
-// over the first of the 32 columns that it read.
+// Where step k of 16 of a tile's 128 weights lies: 32 columns' weights are
+// written over the first of them.
 __device__ __forceinline__ constexpr uint32_t weight_column(int k) {
   return (k >> 1) * 32 + (k & 1) * 8;
 }
 
-// The ninth warp: loads. `place(t)` names the head and row of tile t; `rows(t,
+// The warp that loads. `place(t)` names the head and row of tile t; `rows(t,
 // lane)` loads what else a tile needs and `keep(stage, ...)` puts it to shared
-// memory, all lanes taking part.
-template <int kDim, class Place, class Rows, class Keep>
-__device__ __forceinline__ void load_tiles(BackwardShared<kDim>& s, int tiles,
+// memory, all lanes taking part; it goes with operand 1.
+template <int kDim, bool kKeyRows, class Place, class Rows, class Keep>
+__device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, int tiles,
                                            const CUtensorMap* row_map0,
                                            const CUtensorMap* row_map1, int row_head, int row,
                                            const CUtensorMap* tile_map0,
                                            const CUtensorMap* tile_map1, const Place& place,
                                            const Rows& rows, const Keep& keep) {
   using namespace tc;
-  using Shape = BackwardShape<kDim>;
-  constexpr int kStages = Shape::kStages;
+  using Shape = BackwardShape<kDim, kKeyRows>;
+  constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
   const int lane = threadIdx.x & 31;
   bool good = true;
   if (lane == 0) {
     const uint32_t bar = shared_address(&s.rows_full);
-    barrier_expect(bar, 2 * Shape::kRowBytes);
+    barrier_expect(bar, 2 * Shape::kBytes);
     for (int x = 0; x < kDim / 64; ++x) {
       load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row, bar);
       load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row, bar);
     }
   }
+  const auto load = [&](unsigned char* dst, uint64_t* full, const CUtensorMap* map, int2 at) {
+    const uint32_t bar = shared_address(full);
+    barrier_expect(bar, Shape::kBytes);
+    for (int x = 0; x < kDim / 64; ++x)
+      load_box(shared_address(dst) + x * kTile * 128, map, 64 * x, at.x, at.y, bar);
+  };
+  // The tile that had the place before has been summed up.
+  const auto wait_for = [&](int t) {
+    if (t >= 0)
+      good = good && barrier_wait_warp(shared_address(&s.empty[t % kStages0]), (t / kStages0) & 1);
+  };
   auto ahead = rows(0, lane);
   for (int t = 0; t < tiles; ++t) {
-    const int stage = t % kStages;
     const auto values = ahead;
     if (t + 1 < tiles) ahead = rows(t + 1, lane);
-    if (t >= kStages)
-      good = good && barrier_wait_warp(shared_address(&s.empty[stage]), (t / kStages - 1) & 1);
+    const int stage0 = t % kStages0, stage1 = t % kStages1;
+    wait_for(t - kStages0);
     if (!good) break;
-    const uint32_t bar = shared_address(&s.full[stage]);
-    keep(stage, lane, values);
-    if (lane == 0) {
-      const int2 at = place(t);
-      barrier_expect(bar, 2 * Shape::kTileBytes);
-      for (int x = 0; x < kDim / 64; ++x) {
-        load_box(shared_address(s.tiles[stage][0]) + x * kKeys * 128, tile_map0, 64 * x, at.x,
-                 at.y, bar);
-        load_box(shared_address(s.tiles[stage][1]) + x * kKeys * 128, tile_map1, 64 * x, at.x,
-                 at.y, bar);
-      }
-    } else {
-      barrier_arrive(bar);
-    }
+    const int2 at = place(t);
+    if (lane == 0) load(s.tiles0[stage0], &s.full0[stage0], tile_map0, at);
+    __syncwarp();
+    wait_for(t - kStages1);
+    if (!good) break;
+    keep(stage1, lane, values);
+    if (lane == 0) load(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
+    else barrier_arrive(shared_address(&s.full1[stage1]));
+    __syncwarp();
   }
   if (!good) {  // let what is in flight land before the shared memory is given back
-    for (uint64_t& b : s.full)
-      for (int p = 0; p < 2; ++p) barrier_wait(shared_address(&b), p);
+    for (int p = 0; p < 2; ++p) {
+      for (uint64_t& b : s.full0) barrier_wait(shared_address(&b), p);
+      for (uint64_t& b : s.full1) barrier_wait(shared_address(&b), p);
+    }
     if (lane == 0) atomicExch(&g_timeout, 1u);
   }
   __syncwarp();
 }
 
-// The tenth warp: products, issued by its first lane.
-template <class T, int kDim, bool kKeyRows>
-__device__ __forceinline__ void issue_products(BackwardShared<kDim>& s, int dim, int tiles) {
+// The warp whose first lane issues the products. `sets(t)` says how many
+// sets of 32 rows tile t needs.
+template <class T, int kDim, bool kKeyRows, class Sets>
+__device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s, int dim,
+                                               int tiles, const Sets& sets) {
   using namespace tc;
-  using Shape = BackwardShape<kDim>;
-  constexpr int kBuffers = Shape::kBuffers, kStages = Shape::kStages;
-  constexpr uint32_t kStageWords = 2 * Shape::kTileBytes >> 4, kHalfWords = Shape::kTileBytes >> 4;
+  using Shape = BackwardShape<kDim, kKeyRows>;
+  constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
+  constexpr uint32_t kWords = Shape::kBytes >> 4;
   const uint32_t tensor = s.tensor;
   const bool issues = (threadIdx.x & 31) == 0;
   const int steps = (dim + 15) / 16;
-  const uint32_t score_kind = product_kind<T>(kKeys, false);
+  const uint32_t score_kind = product_kind<T>(0, false);
   const uint32_t sum_kind = product_kind<T>((dim + 15) / 16 * 16, true);
-  const uint32_t rows0 = channels_word<kTile>(shared_address(s.rows[0]));
-  const uint32_t rows1 = channels_word<kTile>(shared_address(s.rows[1]));
-  const uint32_t by_channels = channels_word<kKeys>(shared_address(s.tiles[0][0]));
-  const uint32_t by_rows = rows_word<kKeys>(shared_address(s.tiles[0][0]));
-  // S and G of the tile in a stage, to a buffer.
-  const auto issue_scores = [&](int stage, int buffer) {
-    const uint32_t tile = by_channels + stage * kStageWords;
-    const uint32_t d = tensor + buffer * Shape::kBuffer;
+  const uint32_t rows = channels_word<kTile>(shared_address(s.rows[0]));
+  const uint32_t tiles0 = shared_address(s.tiles0[0]), tiles1 = shared_address(s.tiles1[0]);
+  // S (operand 0) or G (operand 1) of the tile in a stage.
+  const auto issue_scores = [&](int operand, int stage, int count, uint32_t column,
+                                uint64_t* ready) {
+    const uint32_t a = rows + operand * kWords;
+    const uint32_t b = channels_word<kTile>(operand ? tiles1 : tiles0) + stage * kWords;
+    const uint32_t kind = score_kind | static_cast<uint32_t>(count) << 19;  // 32 columns a set
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
       if (i < steps)
-        multiply(d + Shape::kScore, rows0 + channels_step<kTile>(i),
-                 tile + channels_step<kKeys>(i), score_kind, i > 0);
+        multiply(tensor + column, a + channels_step<kTile>(i), b + channels_step<kTile>(i), kind,
+                 i > 0);
+    commit(shared_address(ready));
+  };
+  // A sum from the weights at `column` and operand `operand` of a stage.
+  const auto issue_sum = [&](int operand, int stage, int count, uint32_t column, uint32_t sum,
+                             bool add) {
+    const uint32_t b = rows_word<kTile>(operand ? tiles1 : tiles0) + stage * kWords;
 #pragma unroll
-    for (int i = 0; i < kDim / 16; ++i)
-      if (i < steps)
-        multiply(d + Shape::kGrad, rows1 + channels_step<kTile>(i),
-                 tile + kHalfWords + channels_step<kKeys>(i), score_kind, i > 0);
-    commit(shared_address(&s.scores[buffer]));
+    for (int i = 0; i < kTile / 16; ++i)
+      if (i < 2 * count)
+        multiply_tensor(tensor + sum, tensor + column + weight_column(i), b + rows_step(i),
+                        sum_kind, add || i > 0);
   };
-  bool good = barrier_wait_warp(shared_address(&s.rows_full), 0);
-  int ahead = 0, ahead_parity = 0;  // stage and parity of the tile whose S is next
-  const auto wait_ahead = [&] {
-    good = good && barrier_wait_warp(shared_address(&s.full[ahead]), ahead_parity);
-  };
-  const auto step_ahead = [&] {
-    if (++ahead == kStages) {
-      ahead = 0;
-      ahead_parity ^= 1;
-    }
-  };
-  for (int t = 0; t < kBuffers && t < tiles; ++t) {
-    wait_ahead();
-    if (good && issues) issue_scores(ahead, t);
-    __syncwarp();
-    step_ahead();
+  bool good = barrier_wait_warp(shared_address(&s.rows_full), 0) &&
+              barrier_wait_warp(shared_address(&s.full0[0]), 0) &&
+              barrier_wait_warp(shared_address(&s.full1[0]), 0);
+  int count = sets(0);
+  if (good && issues) {
+    issue_scores(0, 0, count, 0, &s.scores);
+    issue_scores(1, 0, count, Shape::kGrad, &s.grads[0]);
   }
-  int stage = 0, buffer = 0, parity = 0;
+  __syncwarp();
+  int stage0 = 0, stage1 = 0;  // of tile t
+  int next0 = 0, parity0 = 0, next1 = 0, parity1 = 0;  // of tile t + 1
   for (int t = 0; t < tiles && good; ++t) {
-    const bool more = t + kBuffers < tiles;
-    if (more) wait_ahead();
-    good = good && barrier_wait_warp(shared_address(&s.weights[buffer]), parity);
+    const bool more = t + 1 < tiles;
+    if (++next0 == kStages0) {
+      next0 = 0;
+      parity0 ^= 1;
+    }
+    if (++next1 == kStages1) {
+      next1 = 0;
+      parity1 ^= 1;
+    }
+    const int next_count = more ? sets(t + 1) : 0;
+    const uint32_t grad = Shape::kGrad + (kKeyRows ? 0 : (t & 1) * kTile);
+    const uint32_t next_grad = Shape::kGrad + (kKeyRows ? 0 : ((t + 1) & 1) * kTile);
+    uint64_t* next_ready = &s.grads[kKeyRows ? 0 : (t + 1) & 1];
+    if (more) good = barrier_wait_warp(shared_address(&s.full0[next0]), parity0);
+    if (more && !kKeyRows)
+      good = good && barrier_wait_warp(shared_address(&s.full1[next1]), parity1);
+    good = good && barrier_wait_warp(shared_address(&s.read), t & 1);
     if (good && issues) {
       fence_after_sync();
-      const uint32_t d = tensor + buffer * Shape::kBuffer;
-      const uint32_t tile = by_rows + stage * kStageWords;
-#pragma unroll
-      for (int i = 0; i < kKeys / 16; ++i)
-        multiply_tensor(tensor + Shape::kSum, d + Shape::kGrad + weight_column(i),
-                        tile + rows_step(i), sum_kind, t > 0 || i > 0);
-      if constexpr (kKeyRows) {
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          multiply_tensor(tensor + Shape::kSum + kDim, d + Shape::kScore + weight_column(i),
-                          tile + kHalfWords + rows_step(i), sum_kind, t > 0 || i > 0);
+      if constexpr (kKeyRows) issue_sum(1, stage1, count, 0, Shape::kSum + kDim, t > 0);
+      // In order behind the sum that reads P (keys), with S read (queries).
+      if (more) {
+        issue_scores(0, next0, next_count, 0, &s.scores);
+        // The other half of G was last read by the sum of the tile before.
+        if constexpr (!kKeyRows) issue_scores(1, next1, next_count, next_grad, next_ready);
       }
-      // In order behind the sums that read this buffer's weights.
-      if (more) issue_scores(ahead, buffer);
-      commit(shared_address(t == tiles - 1 ? &s.done : &s.empty[stage]));
     }
     __syncwarp();
-    step_ahead();
-    if (++stage == kStages) stage = 0;
-    if (++buffer == kBuffers) {
-      buffer = 0;
-      parity ^= 1;
+    if (more && kKeyRows)
+      good = good && barrier_wait_warp(shared_address(&s.full1[next1]), parity1);
+    good = good && barrier_wait_warp(shared_address(&s.weights[t & 1]), (t >> 1) & 1);
+    if (good && issues) {
+      fence_after_sync();
+      issue_sum(0, stage0, count, grad, Shape::kSum, t > 0);
+      commit(shared_address(more ? &s.empty[stage0] : &s.done));
+      if constexpr (kKeyRows)
+        if (more) issue_scores(1, next1, next_count, next_grad, next_ready);
     }
+    __syncwarp();
+    stage0 = next0;
+    stage1 = next1;
+    count = next_count;
   }
   if (!good && issues) atomicExch(&g_timeout, 1u);
   __syncwarp();
 }
 
-template <int kDim>
-__device__ __forceinline__ void backward_setup(BackwardShared<kDim>& s, int warp) {
+template <int kDim, bool kKeyRows>
+__device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s, int warp) {
   using namespace tc;
   if (threadIdx.x == 0) {
     barrier_init(shared_address(&s.rows_full), 1);
-    for (uint64_t& b : s.full) barrier_init(shared_address(&b), 32);
+    for (uint64_t& b : s.full0) barrier_init(shared_address(&b), 1);
+    for (uint64_t& b : s.full1) barrier_init(shared_address(&b), 32);
     for (uint64_t& b : s.empty) barrier_init(shared_address(&b), 1);
-    for (uint64_t& b : s.scores) barrier_init(shared_address(&b), 1);
+    barrier_init(shared_address(&s.scores), 1);
+    for (uint64_t& b : s.grads) barrier_init(shared_address(&b), 1);
+    barrier_init(shared_address(&s.read), kComputeThreads);
     for (uint64_t& b : s.weights) barrier_init(shared_address(&b), kComputeThreads);
     barrier_init(shared_address(&s.done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
-  if (warp == 9) tensor_alloc<kDim == 64 ? 256 : 512>(shared_address(&s.tensor));
+  if (warp == kProductWarp) tensor_alloc<512>(shared_address(&s.tensor));
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -773,31 +810,34 @@ __device__ __forceinline__ float weight_shift(float lse) {
 
 // dq, and D_i into `delta` for the keys' kernel.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks)
+__global__ void __launch_bounds__(kBackwardThreads, 1)
     grad_query_kernel(gs_window_attention_args a, float* delta,
                       const __grid_constant__ CUtensorMap q_map,
                       const __grid_constant__ CUtensorMap g_map,
                       const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
   using namespace tc;
-  using Shape = BackwardShape<kDim>;
+  using Shape = BackwardShape<kDim, false>;
+  using Shared = BackwardShared<kDim, false>;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
-  BackwardShared<kDim>& s = *reinterpret_cast<BackwardShared<kDim>*>(shared_bytes);
+  Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   chain_wait();
   const int warp = threadIdx.x >> 5;
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const Tile tile =
       tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
+  constexpr int kKeys = kTile, kSets = kKeys / 32;
   const KeyWalk<kKeys, 1> walk(a, tile);
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
-  if (warp == 8) {
-    load_tiles<kDim>(
+  if (warp == kLoadWarp) {
+    load_tiles<kDim, false>(
         s, walk.tiles, &q_map, &g_map, head, tile.start, &k_map, &v_map,
         [&](int t) { return make_int2(kv_head, tile.begin + walk.start(t)); },
         [](int, int) { return 0; }, [](int, int, int) {});
-  } else if (warp == 9) {
-    issue_products<T, kDim, false>(s, a.dim, walk.tiles);
+  } else if (warp == kProductWarp) {
+    issue_products<T, kDim, false>(s, a.dim, walk.tiles,
+                                   [&](int t) { return walk.sets(0, t); });
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -813,9 +853,9 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
 #pragma unroll
         for (int k = 0; k < 8; ++k) d = fmaf(g[k], o[k], d);
       }
-    s.half[half][row] = d;
+    s.part[half][row] = d;
     sync_compute();
-    d = s.half[0][row] + s.half[1][row];
+    d = s.part[0][row] + s.part[1][row];
     const int64_t slot = head * a.tokens + tile.start + row;
     if (live && half == 0) delta[slot] = d;
     const float shift = live ? weight_shift(a.lse[slot]) : INFINITY;
@@ -826,72 +866,104 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
     const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
     const float2 factor = make_float2(scale, scale), down = make_float2(-shift, -shift);
     const float2 less = make_float2(-d, -d);
+    const uint32_t scores = mine + 64 * half;
     bool good = true;
-    int stage = 0, buffer = 0, parity = 0;
+    // Whether the lane's keys of tile t are valid, a tile ahead.
+    bool valid[kSets];
+    const auto load_valid = [&](int t) {
+      if (!a.valid || t >= walk.tiles) return;
+      const int start = walk.start(t) + (threadIdx.x & 31), end = walk.end(t);
+#pragma unroll
+      for (int c = 0; c < kSets; ++c)
+        valid[c] = start + 32 * c < end && __ldg(a.valid + tile.begin + start + 32 * c);
+    };
+    load_valid(0);
     for (int t = 0; t < walk.tiles; ++t) {
       const int start = walk.start(t), end = walk.end(t);
+      // What no query sees has no products either.
+      const int sets = walk.sets(0, t) - 2 * half;
       bool whole = t < walk.head_tiles
                        ? start + kKeys <= end
                        : start + kKeys <= to && (start >= from || start + kKeys <= a.first);
       bool all = whole;
-      uint32_t keep[2], bits = ~0u;
+      uint32_t keep[kSets], bits[2] = {~0u, ~0u};
       if (a.valid || !whole) {
+        all = true;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
-                               max(0, min(end - start - 32 * c, 32)));
-        all = (keep[0] & keep[1]) == ~0u;
+        for (int c = 0; c < kSets; ++c) {
+          keep[c] = a.valid ? __ballot_sync(0xffffffffu, valid[c]) : below32(end - start - 32 * c);
+          all = all && keep[c] == ~0u;
+        }
         whole = whole && all;
-        bits = keep[half] & window_bits(a, i, start + 32 * half, end);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          bits[h] = (half ? keep[2 + h] : keep[h]) &
+                    window_bits(a, i, start + 64 * half + 32 * h, end);
       }
-      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), parity))) break;
+      load_valid(t + 1);
+      if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1))) break;
       fence_after_sync();
-      const uint32_t columns = mine + buffer * Shape::kBuffer + 32 * half;
-      float x[32], g[32];
-      load_columns32(columns + Shape::kScore, x);
-      load_columns32(columns + Shape::kGrad, g);
+      float x[2][32];
+      if (sets > 0) load_columns32(scores, x[0]);
+      if (sets > 1) load_columns32(scores + 32, x[1]);
       wait_loads();
+      fence_before_sync();
+      barrier_arrive(shared_address(&s.read));
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float2 y = fma2(make_float2(x[2 * c], x[2 * c + 1]), factor, down);
-        const float2 e = mul2(make_float2(exp2_approx(y.x), exp2_approx(y.y)),
-                              add2(make_float2(g[2 * c], g[2 * c + 1]), less));
-        x[2 * c] = e.x;
-        x[2 * c + 1] = e.y;
-      }
-      if (!whole) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = bits >> c & 1 ? x[c] : 0.0f;
-      }
-      uint32_t packed[16];
+        for (int c = 0; c < 32; c += 2) {
+          const float2 y = fma2(make_float2(x[h][c], x[h][c + 1]), factor, down);
+          x[h][c] = exp2_approx(y.x);
+          x[h][c + 1] = exp2_approx(y.y);
+        }
+      if (!(good = barrier_wait_warp(shared_address(&s.grads[t & 1]), (t >> 1) & 1))) break;
+      fence_after_sync();
+      const uint32_t grads = scores + Shape::kGrad + (t & 1) * kTile;
 #pragma unroll
-      for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
-      store_columns16(columns + Shape::kGrad, packed);
+      for (int h = 0; h < 2; ++h)
+        if (h < sets) {
+          float g[32];
+          load_columns32(grads + 32 * h, g);
+          wait_loads();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float2 e = mul2(make_float2(x[h][c], x[h][c + 1]),
+                                  add2(make_float2(g[c], g[c + 1]), less));
+            g[c] = e.x;
+            g[c + 1] = e.y;
+          }
+          if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) g[c] = bits[h] >> c & 1 ? g[c] : 0.0f;
+          }
+          uint32_t packed[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(g[2 * c], g[2 * c + 1]);
+          store_columns16(grads + 32 * h, packed);
+        }
       if (!all) {
-        if (!(good = barrier_wait_warp(shared_address(&s.full[stage]), (t / Shape::kStages) & 1)))
+        const int stage = t % Shape::kStages0;
+        if (!(good =
+                  barrier_wait_warp(shared_address(&s.full0[stage]), (t / Shape::kStages0) & 1)))
           break;
-        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
+        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles0[stage], keep, threadIdx.x);
         fence_async_shared();
       }
       wait_stores();
       fence_before_sync();
-      barrier_arrive(shared_address(&s.weights[buffer]));
-      if (++stage == Shape::kStages) stage = 0;
-      if (++buffer == Shape::kBuffers) {
-        buffer = 0;
-        parity ^= 1;
-      }
+      barrier_arrive(shared_address(&s.weights[t & 1]));
     }
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
     T* grad_q = static_cast<T*>(a.grad_q) + at;
 #pragma unroll
-    for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
-      float o[32];
-      load_columns32(mine + Shape::kSum + c, o);
+    for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 16) {
+      float o[16];
+      load_columns16(mine + Shape::kSum + c, o);
       wait_loads();
 #pragma unroll
-      for (int e = 0; e < 32; e += 8)
+      for (int e = 0; e < 16; e += 8)
         if (live && c + e < a.dim) {
           float v[8];
 #pragma unroll
@@ -903,7 +975,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 9) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+  if (warp == kProductWarp) tensor_free<512>(tensor);
 }
 
 // The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
@@ -921,16 +993,17 @@ __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a,
 
 // dk and dv.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks)
+__global__ void __launch_bounds__(kBackwardThreads, 1)
     grad_key_kernel(gs_window_attention_args a, const float* delta, FirstSums sums,
                     const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map,
                     const __grid_constant__ CUtensorMap q_map,
                     const __grid_constant__ CUtensorMap g_map) {
   using namespace tc;
-  using Shape = BackwardShape<kDim>;
+  using Shape = BackwardShape<kDim, true>;
+  using Shared = BackwardShared<kDim, true>;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
-  BackwardShared<kDim>& s = *reinterpret_cast<BackwardShared<kDim>*>(shared_bytes);
+  Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   chain_wait();
   const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
   const int kv_head = blockIdx.x % a.kv_heads;
@@ -955,124 +1028,160 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
     high = min(n, min(j + kTile, n) + a.left);
   }
   const int n = tile.end - tile.begin;
-  const int per_head = static_cast<int>((high - low + kKeys - 1) / kKeys);
+  const int per_head = static_cast<int>((high - low + kTile - 1) / kTile);
   const int tiles = per_head * group;
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
-  if (warp == 8) {
-    // L and D of a tile's queries come along, negated, two of each a lane.
-    load_tiles<kDim>(
+  if (warp == kLoadWarp) {
+    // L and D of a tile's queries come along, negated, four of each a lane.
+    struct RowValues {
+      float shift[4], delta[4];
+    };
+    load_tiles<kDim, true>(
         s, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
         [&](int t) {
           return make_int2(kv_head * group + t / per_head,
-                           tile.begin + static_cast<int>(low) + (t % per_head) * kKeys);
+                           tile.begin + static_cast<int>(low) + (t % per_head) * kTile);
         },
         [&](int t, int lane) {
-          float4 v = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
-          const int64_t i = low + (t % per_head) * kKeys + lane;
+          RowValues v;
+          const int64_t i = low + (t % per_head) * kTile + lane;
           const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
-          if (i < n) {
-            v.x = -weight_shift(a.lse[at]);
-            v.z = -delta[at];
-          }
-          if (i + 32 < n) {
-            v.y = -weight_shift(a.lse[at + 32]);
-            v.w = -delta[at + 32];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bool in = i + 32 * k < n;
+            v.shift[k] = in ? -weight_shift(a.lse[at + 32 * k]) : -INFINITY;
+            v.delta[k] = in ? -delta[at + 32 * k] : 0.0f;
           }
           return v;
         },
-        [&](int stage, int lane, const float4& v) {
-          s.row[stage][0][lane] = v.x;
-          s.row[stage][0][lane + 32] = v.y;
-          s.row[stage][1][lane] = v.z;
-          s.row[stage][1][lane + 32] = v.w;
+        [&](int stage, int lane, const RowValues& v) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s.row[stage][0][lane + 32 * k] = v.shift[k];
+            s.row[stage][1][lane + 32 * k] = v.delta[k];
+          }
         });
-  } else if (warp == 9) {
-    issue_products<T, kDim, true>(s, a.dim, tiles);
+  } else if (warp == kProductWarp) {
+    issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
+      return static_cast<int>(min(int64_t{4}, (high - low - (t % per_head) * kTile + 31) / 32));
+    });
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int64_t j_first = tile.start - tile.begin, j = j_first + row;
     const bool live = j < n && (!chunk || j < a.first);
     const bool seen = live && (!a.valid || a.valid[tile.start + row]);
-    const bool any_seen = __any_sync(0xffffffffu, seen), all_seen = __all_sync(0xffffffffu, seen);
+    const bool any_seen = __any_sync(0xffffffffu, seen);
     const float scale = a.scale * kLog2e;
     const float2 factor = make_float2(scale, scale);
+    const uint32_t scores = mine + 64 * half, grads = scores + Shape::kGrad;
     bool good = true;
-    int stage = 0, full_parity = 0, buffer = 0, parity = 0, index = 0;
+    int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
     for (int t = 0; t < tiles; ++t) {
-      const int64_t start = low + index * kKeys;
-      uint64_t wide = seen ? below(high - start) : 0;
-      if (chunk) wide &= ~below(j + a.left + 1 - start);
-      else wide &= below(j + a.left + 1 - start) & ~below(j - a.right - start);
-      const uint32_t bits = static_cast<uint32_t>(wide >> (32 * half));
-      const bool whole = __all_sync(0xffffffffu, bits == ~0u);
-      if (!(good = barrier_wait_warp(shared_address(&s.scores[buffer]), parity) &&
-                   barrier_wait_warp(shared_address(&s.full[stage]), full_parity)))
+      const int64_t start = low + index * kTile, first = start + 64 * half;
+      // Sets of 32 queries of this half; what lies past the last has no products.
+      const int sets = static_cast<int>(min(int64_t{2}, (high - first + 31) >> 5));
+      uint64_t wide = seen ? below(high - first) : 0;
+      if (chunk) wide &= ~below(j + a.left + 1 - first);
+      else wide &= below(j + a.left + 1 - first) & ~below(j - a.right - first);
+      const bool whole = __all_sync(0xffffffffu, wide == ~uint64_t{0});
+      const uint32_t bits[2] = {static_cast<uint32_t>(wide), static_cast<uint32_t>(wide >> 32)};
+      if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1) &&
+                   barrier_wait_warp(shared_address(&s.full1[stage1]), parity1)))
         break;
       fence_after_sync();
-      const uint32_t columns = mine + buffer * Shape::kBuffer + 32 * half;
-      uint32_t weight[16], packed[16];
+      float x[2][32];
       if (any_seen) {
-        float x[32], g[32];
-        load_columns32(columns + Shape::kScore, x);
-        load_columns32(columns + Shape::kGrad, g);
+        if (sets > 0) load_columns32(scores, x[0]);
+        if (sets > 1) load_columns32(scores + 32, x[1]);
         wait_loads();
-        const float4* shifts = reinterpret_cast<const float4*>(s.row[stage][0] + 32 * half);
-        const float4* deltas = reinterpret_cast<const float4*>(s.row[stage][1] + 32 * half);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float4 l = shifts[c], d = deltas[c];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int at = 4 * c + 2 * k;
-            const float2 y = fma2(make_float2(x[at], x[at + 1]), factor,
-                                  k ? make_float2(l.z, l.w) : make_float2(l.x, l.y));
-            const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-            const float2 e = mul2(p, add2(make_float2(g[at], g[at + 1]),
-                                          k ? make_float2(d.z, d.w) : make_float2(d.x, d.y)));
-            x[at] = p.x;
-            x[at + 1] = p.y;
-            g[at] = e.x;
-            g[at + 1] = e.y;
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            x[c] = bits >> c & 1 ? x[c] : 0.0f;
-            g[c] = bits >> c & 1 ? g[c] : 0.0f;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          weight[c] = pack2<T>(x[2 * c], x[2 * c + 1]);
-          packed[c] = pack2<T>(g[2 * c], g[2 * c + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) weight[c] = packed[c] = 0;
       }
-      store_columns16(columns + Shape::kScore, weight);
-      store_columns16(columns + Shape::kGrad, packed);
-      if (start + kKeys > n) {
+      const float4* shifts = reinterpret_cast<const float4*>(s.row[stage1][0] + 64 * half);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (h < sets) {
+          uint32_t packed[16];
+          if (any_seen) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float4 l = shifts[8 * h + c];
+              float* p = &x[h][4 * c];
+              const float2 y0 = fma2(make_float2(p[0], p[1]), factor, make_float2(l.x, l.y));
+              const float2 y1 = fma2(make_float2(p[2], p[3]), factor, make_float2(l.z, l.w));
+              p[0] = exp2_approx(y0.x);
+              p[1] = exp2_approx(y0.y);
+              p[2] = exp2_approx(y1.x);
+              p[3] = exp2_approx(y1.y);
+            }
+            if (!whole) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[h][c] = bits[h] >> c & 1 ? x[h][c] : 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(x[h][2 * c], x[h][2 * c + 1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) packed[c] = 0;
+          }
+          store_columns16(scores + 32 * h, packed);
+        }
+      if (start + kTile > n) {
         const int rest = n - static_cast<int>(start);
-        const uint32_t keep[2] = {below32(rest), below32(rest - 32)};
-        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][0], keep, threadIdx.x);
-        zero_rows<kDim, kKeys, kComputeThreads>(s.tiles[stage][1], keep, threadIdx.x);
+        const uint32_t keep[4] = {below32(rest), below32(rest - 32), below32(rest - 64),
+                                  below32(rest - 96)};
+        zero_rows<kDim, kTile, kComputeThreads>(s.tiles0[stage0], keep, threadIdx.x);
+        zero_rows<kDim, kTile, kComputeThreads>(s.tiles1[stage1], keep, threadIdx.x);
         fence_async_shared();
       }
       wait_stores();
       fence_before_sync();
-      barrier_arrive(shared_address(&s.weights[buffer]));
+      barrier_arrive(shared_address(&s.read));
+      if (!(good = barrier_wait_warp(shared_address(&s.grads[0]), t & 1))) break;
+      fence_after_sync();
+      const float4* deltas = reinterpret_cast<const float4*>(s.row[stage1][1] + 64 * half);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (h < sets) {
+          uint32_t packed[16];
+          if (any_seen) {
+            float g[32];
+            load_columns32(grads + 32 * h, g);
+            wait_loads();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float4 d = deltas[8 * h + c];
+              float* e = &g[4 * c];
+              const float* p = &x[h][4 * c];
+              const float2 e0 = mul2(make_float2(p[0], p[1]),
+                                     add2(make_float2(e[0], e[1]), make_float2(d.x, d.y)));
+              const float2 e1 = mul2(make_float2(p[2], p[3]),
+                                     add2(make_float2(e[2], e[3]), make_float2(d.z, d.w)));
+              e[0] = e0.x;
+              e[1] = e0.y;
+              e[2] = e1.x;
+              e[3] = e1.y;
+            }
+            if (!whole) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) g[c] = bits[h] >> c & 1 ? g[c] : 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 16; ++c) packed[c] = pack2<T>(g[2 * c], g[2 * c + 1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) packed[c] = 0;
+          }
+          store_columns16(grads + 32 * h, packed);
+        }
+      wait_stores();
+      fence_before_sync();
+      barrier_arrive(shared_address(&s.weights[t & 1]));
       if (++index == per_head) index = 0;
-      if (++stage == Shape::kStages) {
-        stage = 0;
-        full_parity ^= 1;
-      }
-      if (++buffer == Shape::kBuffers) {
-        buffer = 0;
-        parity ^= 1;
+      if (++stage0 == Shape::kStages0) stage0 = 0;
+      if (++stage1 == Shape::kStages1) {
+        stage1 = 0;
+        parity1 ^= 1;
       }
     }
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
@@ -1086,14 +1195,14 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
-      for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 32) {
-        float o[32];
-        load_columns32(mine + Shape::kSum + which * kDim + c, o);
+      for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 16) {
+        float o[16];
+        load_columns16(mine + Shape::kSum + which * kDim + c, o);
         wait_loads();
         const float factor = which ? 1.0f : a.scale;
         T* out = static_cast<T*>(which ? a.grad_v : a.grad_k) + at;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
+        for (int e = 0; e < 16; e += 8)
           if (live && c + e < a.dim) {
             float v[8];
 #pragma unroll
@@ -1106,7 +1215,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim>::kBlocks
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 9) tensor_free<kDim == 64 ? 256 : 512>(tensor);
+  if (warp == kProductWarp) tensor_free<512>(tensor);
 }
 
 // dk and dv of first tokens: their window's sum and the chunks' in order, a
@@ -1166,38 +1275,35 @@ int64_t chunk_slots(const gs_window_attention_args& a) {
 
 template <class T, int kDim>
 int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
-  CUtensorMap rows[4], tiles[4];  // q, grad_out, k, v in boxes of 128 and of 64 rows
-  for (int m = 0; m < 4; ++m) {
-    const void* const base[4] = {a.q, a.grad_out, a.k, a.v};
-    const int64_t stride[4] = {a.q_stride, int64_t{a.heads} * a.dim, a.k_stride, a.v_stride};
-    const int64_t head_stride[4] = {a.q_head_stride, a.dim, a.k_head_stride, a.v_head_stride};
-    const int64_t heads = m < 2 ? a.heads : a.kv_heads;
-    GS_TRY(tc::encode_heads(&rows[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
-                          head_stride[m], kTile));
-    GS_TRY(tc::encode_heads(&tiles[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
-                          head_stride[m], kKeys));
-  }
+  CUtensorMap maps[4];  // q, grad_out, k, v
+  const void* const base[4] = {a.q, a.grad_out, a.k, a.v};
+  const int64_t stride[4] = {a.q_stride, int64_t{a.heads} * a.dim, a.k_stride, a.v_stride};
+  const int64_t head_stride[4] = {a.q_head_stride, a.dim, a.k_head_stride, a.v_head_stride};
+  for (int m = 0; m < 4; ++m)
+    GS_TRY(tc::encode_heads(&maps[m], a.dtype, base[m], a.tokens, m < 2 ? a.heads : a.kv_heads,
+                            a.dim, stride[m], head_stride[m], kTile));
   float* delta = static_cast<float*>(a.workspace);
   FirstSums sums;
   sums.tiles = static_cast<int>(chunk_tiles(a));
   sums.slots = static_cast<int>(chunk_slots(a));
   sums.base = delta + delta_floats(a);
   sums.part = sums.base + sequences_of(a) * a.kv_heads * a.first * 2 * a.dim;
-  constexpr size_t kShared = sizeof(BackwardShared<kDim>);
+  constexpr size_t kQueryShared = sizeof(BackwardShared<kDim, false>);
+  constexpr size_t kKeyShared = sizeof(BackwardShared<kDim, true>);
   GS_CUDA_TRY(cudaFuncSetAttribute(grad_query_kernel<T, kDim>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kQueryShared));
   GS_CUDA_TRY(cudaFuncSetAttribute(grad_key_kernel<T, kDim>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyShared));
   const int64_t key_blocks = (a.num_tiles + sums.slots) * a.kv_heads;
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
   launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kBackwardThreads, kShared, stream, a, delta, rows[0], rows[1],
-                        tiles[2], tiles[3]);
+                        kBackwardThreads, kQueryShared, stream, a, delta, maps[0], maps[1],
+                        maps[2], maps[3]);
   GS_TRY(check_launch());
   launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
-                        kBackwardThreads, kShared, stream, a, delta, sums, rows[2], rows[3],
-                        tiles[0], tiles[1]);
+                        kBackwardThreads, kKeyShared, stream, a, delta, sums, maps[2], maps[3],
+                        maps[0], maps[1]);
   GS_TRY(check_launch());
   if (first_blocks > 0)
     launch_chained(first_sum_kernel<T>, static_cast<unsigned>(first_blocks), 2 * kMaxDim * kParts,
