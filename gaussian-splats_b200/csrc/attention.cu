@@ -549,8 +549,8 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // ------------------------------------------------- whole sequences, backward
 //
 // Two kernels of one shape: a block holds 128 rows of two operands (queries and
-// their gradients, or keys and values) and walks over tiles of 128 rows of the
-// other two, recomputing the scores,
+// their gradients, or keys and values) and walks over tiles of the other two,
+// recomputing the scores,
 //
 //   S = rows0 tile0^T,  G = rows1 tile1^T          (tensor memory, floats)
 //   P = exp2(S scale log2 e - L),  E = P (G - D)   (16 bits)
@@ -578,11 +578,16 @@ struct BackwardShape {
   // Tiles of operand 0 wait for the sums, those of operand 1 no longer than for
   // G: at 128 channels there is room for three of the one and two of the other.
   static constexpr int kStages0 = kDim == 64 ? 4 : 3, kStages1 = kDim == 64 ? 3 : 2;
-  static constexpr int kBytes = kTile * kDim * 2;  // of an operand's rows
+  // Rows of a tile. At 64 channels exponentials bound the kernels before products
+  // do: two blocks a multiprocessor with smaller tiles take turns (one block with
+  // tiles of 128 rows was 9% slower).
+  static constexpr int kRows = kDim == 64 ? 64 : 128, kSets = kRows / 32;
+  static constexpr int kBlocks = kDim == 64 ? 2 : 1, kColumns = kDim == 64 ? 256 : 512;
+  static constexpr int kBytes = kTile * kDim * 2, kTileBytes = kRows * kDim * 2;
   // Columns of tensor memory. E lies over G, and the keys' P over S; the queries
   // have room for G twice.
-  static constexpr int kGrad = kTile, kGrads = kKeyRows ? 1 : 2;
-  static constexpr int kSum = kGrad + kGrads * kTile;
+  static constexpr int kGrad = kRows, kGrads = kKeyRows ? 1 : 2;
+  static constexpr int kSum = kGrad + kGrads * kRows;
 };
 
 template <int kDim, bool kKeyRows>
@@ -590,11 +595,11 @@ struct BackwardShared {
   using Shape = BackwardShape<kDim, kKeyRows>;
   static constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
   alignas(1024) unsigned char rows[2][Shape::kBytes];
-  unsigned char tiles0[kStages0][Shape::kBytes];
-  unsigned char tiles1[kStages1][Shape::kBytes];
+  unsigned char tiles0[kStages0][Shape::kTileBytes];
+  unsigned char tiles1[kStages1][Shape::kTileBytes];
   union {
-    float row[kStages1][2][kTile];  // keys: -L and -D of a tile's queries
-    float part[2][kTile];           // queries: halves of D
+    float row[kStages1][2][Shape::kRows];  // keys: -L and -D of a tile's queries
+    float part[2][kTile];                  // queries: halves of D
   };
   uint64_t rows_full, full0[kStages0], full1[kStages1];  // loads
   uint64_t empty[kStages0];                              // a tile's sums are complete
@@ -611,7 +616,7 @@ constexpr int kComputeThreads = 256;
 constexpr int kLoadWarp = kComputeThreads / 32, kProductWarp = kLoadWarp + 1;
 constexpr int kBackwardThreads = kComputeThreads + 64;
 
-// Where step k of 16 of a tile's 128 weights lies: 32 columns' weights are
+// Where step k of 16 of a tile's weights lies: 32 columns' weights are
 // written over the first of them.
 __device__ __forceinline__ constexpr uint32_t weight_column(int k) {
   return (k >> 1) * 32 + (k & 1) * 8;
@@ -642,9 +647,9 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
   }
   const auto load = [&](unsigned char* dst, uint64_t* full, const CUtensorMap* map, int2 at) {
     const uint32_t bar = shared_address(full);
-    barrier_expect(bar, Shape::kBytes);
+    barrier_expect(bar, Shape::kTileBytes);
     for (int x = 0; x < kDim / 64; ++x)
-      load_box(shared_address(dst) + x * kTile * 128, map, 64 * x, at.x, at.y, bar);
+      load_box(shared_address(dst) + x * Shape::kRows * 128, map, 64 * x, at.x, at.y, bar);
   };
   // The tile that had the place before has been summed up.
   const auto wait_for = [&](int t) {
@@ -686,7 +691,8 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
   using namespace tc;
   using Shape = BackwardShape<kDim, kKeyRows>;
   constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
-  constexpr uint32_t kWords = Shape::kBytes >> 4;
+  constexpr int kRows = Shape::kRows;
+  constexpr uint32_t kWords = Shape::kBytes >> 4, kTileWords = Shape::kTileBytes >> 4;
   const uint32_t tensor = s.tensor;
   const bool issues = (threadIdx.x & 31) == 0;
   const int steps = (dim + 15) / 16;
@@ -698,21 +704,21 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
   const auto issue_scores = [&](int operand, int stage, int count, uint32_t column,
                                 uint64_t* ready) {
     const uint32_t a = rows + operand * kWords;
-    const uint32_t b = channels_word<kTile>(operand ? tiles1 : tiles0) + stage * kWords;
+    const uint32_t b = channels_word<kRows>(operand ? tiles1 : tiles0) + stage * kTileWords;
     const uint32_t kind = score_kind | static_cast<uint32_t>(count) << 19;  // 32 columns a set
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
       if (i < steps)
-        multiply(tensor + column, a + channels_step<kTile>(i), b + channels_step<kTile>(i), kind,
+        multiply(tensor + column, a + channels_step<kTile>(i), b + channels_step<kRows>(i), kind,
                  i > 0);
     commit(shared_address(ready));
   };
   // A sum from the weights at `column` and operand `operand` of a stage.
   const auto issue_sum = [&](int operand, int stage, int count, uint32_t column, uint32_t sum,
                              bool add) {
-    const uint32_t b = rows_word<kTile>(operand ? tiles1 : tiles0) + stage * kWords;
+    const uint32_t b = rows_word<kRows>(operand ? tiles1 : tiles0) + stage * kTileWords;
 #pragma unroll
-    for (int i = 0; i < kTile / 16; ++i)
+    for (int i = 0; i < kRows / 16; ++i)
       if (i < 2 * count)
         multiply_tensor(tensor + sum, tensor + column + weight_column(i), b + rows_step(i),
                         sum_kind, add || i > 0);
@@ -739,8 +745,8 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
       parity1 ^= 1;
     }
     const int next_count = more ? sets(t + 1) : 0;
-    const uint32_t grad = Shape::kGrad + (kKeyRows ? 0 : (t & 1) * kTile);
-    const uint32_t next_grad = Shape::kGrad + (kKeyRows ? 0 : ((t + 1) & 1) * kTile);
+    const uint32_t grad = Shape::kGrad + (kKeyRows ? 0 : (t & 1) * kRows);
+    const uint32_t next_grad = Shape::kGrad + (kKeyRows ? 0 : ((t + 1) & 1) * kRows);
     uint64_t* next_ready = &s.grads[kKeyRows ? 0 : (t + 1) & 1];
     if (more) good = barrier_wait_warp(shared_address(&s.full0[next0]), parity0);
     if (more && !kKeyRows)
@@ -779,6 +785,7 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
 template <int kDim, bool kKeyRows>
 __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s, int warp) {
   using namespace tc;
+  using Shape = BackwardShape<kDim, kKeyRows>;
   if (threadIdx.x == 0) {
     barrier_init(shared_address(&s.rows_full), 1);
     for (uint64_t& b : s.full0) barrier_init(shared_address(&b), 1);
@@ -792,7 +799,7 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
-  if (warp == kProductWarp) tensor_alloc<512>(shared_address(&s.tensor));
+  if (warp == kProductWarp) tensor_alloc<Shape::kColumns>(shared_address(&s.tensor));
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -810,7 +817,7 @@ __device__ __forceinline__ float weight_shift(float lse) {
 
 // dq, and D_i into `delta` for the keys' kernel.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kBackwardThreads, 1)
+__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::kBlocks)
     grad_query_kernel(gs_window_attention_args a, float* delta,
                       const __grid_constant__ CUtensorMap q_map,
                       const __grid_constant__ CUtensorMap g_map,
@@ -826,7 +833,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const Tile tile =
       tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
-  constexpr int kKeys = kTile, kSets = kKeys / 32;
+  constexpr int kKeys = Shape::kRows, kSets = Shape::kSets, kHalfSets = kSets / 2;
   const KeyWalk<kKeys, 1> walk(a, tile);
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
@@ -866,7 +873,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
     const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
     const float2 factor = make_float2(scale, scale), down = make_float2(-shift, -shift);
     const float2 less = make_float2(-d, -d);
-    const uint32_t scores = mine + 64 * half;
+    const uint32_t scores = mine + 32 * kHalfSets * half;
     bool good = true;
     // Whether the lane's keys of tile t are valid, a tile ahead.
     bool valid[kSets];
@@ -881,12 +888,12 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
     for (int t = 0; t < walk.tiles; ++t) {
       const int start = walk.start(t), end = walk.end(t);
       // What no query sees has no products either.
-      const int sets = walk.sets(0, t) - 2 * half;
+      const int sets = walk.sets(0, t) - kHalfSets * half;
       bool whole = t < walk.head_tiles
                        ? start + kKeys <= end
                        : start + kKeys <= to && (start >= from || start + kKeys <= a.first);
       bool all = whole;
-      uint32_t keep[kSets], bits[2] = {~0u, ~0u};
+      uint32_t keep[kSets], bits[kHalfSets];
       if (a.valid || !whole) {
         all = true;
 #pragma unroll
@@ -896,21 +903,22 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
         }
         whole = whole && all;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          bits[h] = (half ? keep[2 + h] : keep[h]) &
-                    window_bits(a, i, start + 64 * half + 32 * h, end);
+        for (int h = 0; h < kHalfSets; ++h)
+          bits[h] = (half ? keep[kHalfSets + h] : keep[h]) &
+                    window_bits(a, i, start + 32 * (kHalfSets * half + h), end);
       }
       load_valid(t + 1);
       if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1))) break;
       fence_after_sync();
-      float x[2][32];
-      if (sets > 0) load_columns32(scores, x[0]);
-      if (sets > 1) load_columns32(scores + 32, x[1]);
+      float x[kHalfSets][32];
+#pragma unroll
+      for (int h = 0; h < kHalfSets; ++h)
+        if (h < sets) load_columns32(scores + 32 * h, x[h]);
       wait_loads();
       fence_before_sync();
       barrier_arrive(shared_address(&s.read));
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalfSets; ++h)
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           const float2 y = fma2(make_float2(x[h][c], x[h][c + 1]), factor, down);
@@ -919,9 +927,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
         }
       if (!(good = barrier_wait_warp(shared_address(&s.grads[t & 1]), (t >> 1) & 1))) break;
       fence_after_sync();
-      const uint32_t grads = scores + Shape::kGrad + (t & 1) * kTile;
+      const uint32_t grads = scores + Shape::kGrad + (t & 1) * kKeys;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalfSets; ++h)
         if (h < sets) {
           float g[32];
           load_columns32(grads + 32 * h, g);
@@ -975,7 +983,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == kProductWarp) tensor_free<512>(tensor);
+  if (warp == kProductWarp) tensor_free<Shape::kColumns>(tensor);
 }
 
 // The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
@@ -993,7 +1001,7 @@ __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a,
 
 // dk and dv.
 template <class T, int kDim>
-__global__ void __launch_bounds__(kBackwardThreads, 1)
+__global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::kBlocks)
     grad_key_kernel(gs_window_attention_args a, const float* delta, FirstSums sums,
                     const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map,
@@ -1002,6 +1010,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
   using namespace tc;
   using Shape = BackwardShape<kDim, true>;
   using Shared = BackwardShared<kDim, true>;
+  constexpr int kRows = Shape::kRows, kSets = Shape::kSets, kHalfSets = kSets / 2;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   chain_wait();
@@ -1028,27 +1037,27 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
     high = min(n, min(j + kTile, n) + a.left);
   }
   const int n = tile.end - tile.begin;
-  const int per_head = static_cast<int>((high - low + kTile - 1) / kTile);
+  const int per_head = static_cast<int>((high - low + kRows - 1) / kRows);
   const int tiles = per_head * group;
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
   if (warp == kLoadWarp) {
-    // L and D of a tile's queries come along, negated, four of each a lane.
+    // L and D of a tile's queries come along, negated.
     struct RowValues {
-      float shift[4], delta[4];
+      float shift[kSets], delta[kSets];
     };
     load_tiles<kDim, true>(
         s, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
         [&](int t) {
           return make_int2(kv_head * group + t / per_head,
-                           tile.begin + static_cast<int>(low) + (t % per_head) * kTile);
+                           tile.begin + static_cast<int>(low) + (t % per_head) * kRows);
         },
         [&](int t, int lane) {
           RowValues v;
-          const int64_t i = low + (t % per_head) * kTile + lane;
+          const int64_t i = low + (t % per_head) * kRows + lane;
           const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < kSets; ++k) {
             const bool in = i + 32 * k < n;
             v.shift[k] = in ? -weight_shift(a.lse[at + 32 * k]) : -INFINITY;
             v.delta[k] = in ? -delta[at + 32 * k] : 0.0f;
@@ -1057,14 +1066,15 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
         },
         [&](int stage, int lane, const RowValues& v) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < kSets; ++k) {
             s.row[stage][0][lane + 32 * k] = v.shift[k];
             s.row[stage][1][lane + 32 * k] = v.delta[k];
           }
         });
   } else if (warp == kProductWarp) {
     issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
-      return static_cast<int>(min(int64_t{4}, (high - low - (t % per_head) * kTile + 31) / 32));
+      return static_cast<int>(
+          min(int64_t{kSets}, (high - low - (t % per_head) * kRows + 31) / 32));
     });
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
@@ -1075,31 +1085,38 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
     const bool any_seen = __any_sync(0xffffffffu, seen);
     const float scale = a.scale * kLog2e;
     const float2 factor = make_float2(scale, scale);
-    const uint32_t scores = mine + 64 * half, grads = scores + Shape::kGrad;
+    const uint32_t scores = mine + 32 * kHalfSets * half, grads = scores + Shape::kGrad;
     bool good = true;
     int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
     for (int t = 0; t < tiles; ++t) {
-      const int64_t start = low + index * kTile, first = start + 64 * half;
+      const int64_t start = low + index * kRows, first = start + 32 * kHalfSets * half;
       // Sets of 32 queries of this half; what lies past the last has no products.
-      const int sets = static_cast<int>(min(int64_t{2}, (high - first + 31) >> 5));
+      const int sets = static_cast<int>(min(int64_t{kHalfSets}, (high - first + 31) >> 5));
       uint64_t wide = seen ? below(high - first) : 0;
       if (chunk) wide &= ~below(j + a.left + 1 - first);
       else wide &= below(j + a.left + 1 - first) & ~below(j - a.right - first);
-      const bool whole = __all_sync(0xffffffffu, wide == ~uint64_t{0});
-      const uint32_t bits[2] = {static_cast<uint32_t>(wide), static_cast<uint32_t>(wide >> 32)};
+      uint32_t bits[kHalfSets];
+      bool mine_whole = true;
+#pragma unroll
+      for (int h = 0; h < kHalfSets; ++h) {
+        bits[h] = static_cast<uint32_t>(wide >> (32 * h));
+        mine_whole = mine_whole && bits[h] == ~0u;
+      }
+      const bool whole = __all_sync(0xffffffffu, mine_whole);
       if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1) &&
                    barrier_wait_warp(shared_address(&s.full1[stage1]), parity1)))
         break;
       fence_after_sync();
-      float x[2][32];
+      float x[kHalfSets][32];
       if (any_seen) {
-        if (sets > 0) load_columns32(scores, x[0]);
-        if (sets > 1) load_columns32(scores + 32, x[1]);
+#pragma unroll
+        for (int h = 0; h < kHalfSets; ++h)
+          if (h < sets) load_columns32(scores + 32 * h, x[h]);
         wait_loads();
       }
-      const float4* shifts = reinterpret_cast<const float4*>(s.row[stage1][0] + 64 * half);
+      const float4* shifts = reinterpret_cast<const float4*>(s.row[stage1][0] + 32 * kHalfSets * half);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalfSets; ++h)
         if (h < sets) {
           uint32_t packed[16];
           if (any_seen) {
@@ -1126,12 +1143,13 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
           }
           store_columns16(scores + 32 * h, packed);
         }
-      if (start + kTile > n) {
+      if (start + kRows > n) {
         const int rest = n - static_cast<int>(start);
-        const uint32_t keep[4] = {below32(rest), below32(rest - 32), below32(rest - 64),
-                                  below32(rest - 96)};
-        zero_rows<kDim, kTile, kComputeThreads>(s.tiles0[stage0], keep, threadIdx.x);
-        zero_rows<kDim, kTile, kComputeThreads>(s.tiles1[stage1], keep, threadIdx.x);
+        uint32_t keep[kSets];
+#pragma unroll
+        for (int c = 0; c < kSets; ++c) keep[c] = below32(rest - 32 * c);
+        zero_rows<kDim, kRows, kComputeThreads>(s.tiles0[stage0], keep, threadIdx.x);
+        zero_rows<kDim, kRows, kComputeThreads>(s.tiles1[stage1], keep, threadIdx.x);
         fence_async_shared();
       }
       wait_stores();
@@ -1139,9 +1157,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
       barrier_arrive(shared_address(&s.read));
       if (!(good = barrier_wait_warp(shared_address(&s.grads[0]), t & 1))) break;
       fence_after_sync();
-      const float4* deltas = reinterpret_cast<const float4*>(s.row[stage1][1] + 64 * half);
+      const float4* deltas = reinterpret_cast<const float4*>(s.row[stage1][1] + 32 * kHalfSets * half);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalfSets; ++h)
         if (h < sets) {
           uint32_t packed[16];
           if (any_seen) {
@@ -1215,7 +1233,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == kProductWarp) tensor_free<512>(tensor);
+  if (warp == kProductWarp) tensor_free<Shape::kColumns>(tensor);
 }
 
 // dk and dv of first tokens: their window's sum and the chunks' in order, a
@@ -1275,13 +1293,20 @@ int64_t chunk_slots(const gs_window_attention_args& a) {
 
 template <class T, int kDim>
 int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
-  CUtensorMap maps[4];  // q, grad_out, k, v
+  CUtensorMap rows[4], tiles[4];  // q, grad_out, k, v
   const void* const base[4] = {a.q, a.grad_out, a.k, a.v};
   const int64_t stride[4] = {a.q_stride, int64_t{a.heads} * a.dim, a.k_stride, a.v_stride};
   const int64_t head_stride[4] = {a.q_head_stride, a.dim, a.k_head_stride, a.v_head_stride};
-  for (int m = 0; m < 4; ++m)
-    GS_TRY(tc::encode_heads(&maps[m], a.dtype, base[m], a.tokens, m < 2 ? a.heads : a.kv_heads,
-                            a.dim, stride[m], head_stride[m], kTile));
+  for (int m = 0; m < 4; ++m) {
+    const int64_t heads = m < 2 ? a.heads : a.kv_heads;
+    constexpr int kRows = BackwardShape<kDim, true>::kRows;
+    GS_TRY(tc::encode_heads(&rows[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
+                            head_stride[m], kTile));
+    if constexpr (kRows == kTile) tiles[m] = rows[m];
+    else
+      GS_TRY(tc::encode_heads(&tiles[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
+                              head_stride[m], kRows));
+  }
   float* delta = static_cast<float*>(a.workspace);
   FirstSums sums;
   sums.tiles = static_cast<int>(chunk_tiles(a));
@@ -1298,12 +1323,12 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
   launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kBackwardThreads, kQueryShared, stream, a, delta, maps[0], maps[1],
-                        maps[2], maps[3]);
+                        kBackwardThreads, kQueryShared, stream, a, delta, rows[0], rows[1],
+                        tiles[2], tiles[3]);
   GS_TRY(check_launch());
   launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
-                        kBackwardThreads, kKeyShared, stream, a, delta, sums, maps[2], maps[3],
-                        maps[0], maps[1]);
+                        kBackwardThreads, kKeyShared, stream, a, delta, sums, rows[2], rows[3],
+                        tiles[0], tiles[1]);
   GS_TRY(check_launch());
   if (first_blocks > 0)
     launch_chained(first_sum_kernel<T>, static_cast<unsigned>(first_blocks), 2 * kMaxDim * kParts,
