@@ -18,6 +18,7 @@
 // never read into a sum, so what they hold (infinities, NaN) does not matter.
 
 #include <algorithm>
+#include <cmath>
 
 #include "tensorcore.cuh"
 
@@ -805,6 +806,27 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
   fence_after_sync();
 }
 
+// float16 loses bits below 2^-14, where a wide window's weights are: P is stored
+// times 2^p (about the window's width; P is at most 1) and E times 2^e (at most
+// 16, so that it overflows at 4094 at the earliest), and the sums are scaled
+// back. bfloat16 needs neither: p = e = 0.
+struct WeightScale {
+  float p;         // log2 of P's factor
+  float e, e_p;    // E's factor, and that over P's
+  float dk, dv;    // what scales the sums back (dk: dq too)
+};
+WeightScale weight_scale(const gs_window_attention_args& a) {
+  int p = 0, e = 0;
+  if (a.dtype == GS_FLOAT16) {
+    const int64_t seen =
+        std::min(a.tokens, int64_t{a.left} + int64_t{a.right} + 1 + int64_t{a.first});
+    while (p < 15 && int64_t{2} << p <= seen) ++p;
+    e = std::min(4, p / 2);
+  }
+  return {static_cast<float>(p), std::ldexp(1.0f, e), std::ldexp(1.0f, e - p),
+          std::ldexp(a.scale, -e), std::ldexp(1.0f, -p)};
+}
+
 __device__ __forceinline__ void sync_compute() {
   asm volatile("bar.sync 1, %0;" ::"n"(kComputeThreads) : "memory");
 }
@@ -818,7 +840,7 @@ __device__ __forceinline__ float weight_shift(float lse) {
 // dq, and D_i into `delta` for the keys' kernel.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::kBlocks)
-    grad_query_kernel(gs_window_attention_args a, float* delta,
+    grad_query_kernel(gs_window_attention_args a, WeightScale weights, float* delta,
                       const __grid_constant__ CUtensorMap q_map,
                       const __grid_constant__ CUtensorMap g_map,
                       const __grid_constant__ CUtensorMap k_map,
@@ -872,7 +894,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     const int from = position(int64_t{i_first} + kTile - 1 - a.left);
     const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
     const float2 factor = make_float2(scale, scale), down = make_float2(-shift, -shift);
-    const float2 less = make_float2(-d, -d);
+    const float2 grow = make_float2(weights.e, weights.e);
+    const float2 less = make_float2(-d * weights.e, -d * weights.e);
     const uint32_t scores = mine + 32 * kHalfSets * half;
     bool good = true;
     // Whether the lane's keys of tile t are valid, a tile ahead.
@@ -937,7 +960,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             const float2 e = mul2(make_float2(x[h][c], x[h][c + 1]),
-                                  add2(make_float2(g[c], g[c + 1]), less));
+                                  fma2(make_float2(g[c], g[c + 1]), grow, less));
             g[c] = e.x;
             g[c + 1] = e.y;
           }
@@ -975,7 +998,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
         if (live && c + e < a.dim) {
           float v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * a.scale : NAN;
+          for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * weights.dk : NAN;
           store_pack<8>(grad_q + c + e, v);
         }
     }
@@ -1002,7 +1025,8 @@ __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a,
 // dk and dv.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::kBlocks)
-    grad_key_kernel(gs_window_attention_args a, const float* delta, FirstSums sums,
+    grad_key_kernel(gs_window_attention_args a, WeightScale weights, const float* delta,
+                    FirstSums sums,
                     const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map,
                     const __grid_constant__ CUtensorMap q_map,
@@ -1059,8 +1083,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
             const bool in = i + 32 * k < n;
-            v.shift[k] = in ? -weight_shift(a.lse[at + 32 * k]) : -INFINITY;
-            v.delta[k] = in ? -delta[at + 32 * k] : 0.0f;
+            v.shift[k] = in ? weights.p - weight_shift(a.lse[at + 32 * k]) : -INFINITY;
+            v.delta[k] = in ? -delta[at + 32 * k] * weights.e_p : 0.0f;
           }
           return v;
         },
@@ -1084,7 +1108,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     const bool seen = live && (!a.valid || a.valid[tile.start + row]);
     const bool any_seen = __any_sync(0xffffffffu, seen);
     const float scale = a.scale * kLog2e;
-    const float2 factor = make_float2(scale, scale);
+    const float2 factor = make_float2(scale, scale), grow = make_float2(weights.e_p, weights.e_p);
     const uint32_t scores = mine + 32 * kHalfSets * half, grads = scores + Shape::kGrad;
     bool good = true;
     int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
@@ -1172,9 +1196,9 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
               float* e = &g[4 * c];
               const float* p = &x[h][4 * c];
               const float2 e0 = mul2(make_float2(p[0], p[1]),
-                                     add2(make_float2(e[0], e[1]), make_float2(d.x, d.y)));
+                                     fma2(make_float2(e[0], e[1]), grow, make_float2(d.x, d.y)));
               const float2 e1 = mul2(make_float2(p[2], p[3]),
-                                     add2(make_float2(e[2], e[3]), make_float2(d.z, d.w)));
+                                     fma2(make_float2(e[2], e[3]), grow, make_float2(d.z, d.w)));
               e[0] = e0.x;
               e[1] = e0.y;
               e[2] = e1.x;
@@ -1217,7 +1241,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         float o[16];
         load_columns16(mine + Shape::kSum + which * kDim + c, o);
         wait_loads();
-        const float factor = which ? 1.0f : a.scale;
+        const float factor = which ? weights.dv : weights.dk;
         T* out = static_cast<T*>(which ? a.grad_v : a.grad_k) + at;
 #pragma unroll
         for (int e = 0; e < 16; e += 8)
@@ -1307,6 +1331,7 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
       GS_TRY(tc::encode_heads(&tiles[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
                               head_stride[m], kRows));
   }
+  const WeightScale weights = weight_scale(a);
   float* delta = static_cast<float*>(a.workspace);
   FirstSums sums;
   sums.tiles = static_cast<int>(chunk_tiles(a));
@@ -1323,11 +1348,11 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
   launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kBackwardThreads, kQueryShared, stream, a, delta, rows[0], rows[1],
+                        kBackwardThreads, kQueryShared, stream, a, weights, delta, rows[0], rows[1],
                         tiles[2], tiles[3]);
   GS_TRY(check_launch());
   launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
-                        kBackwardThreads, kKeyShared, stream, a, delta, sums, rows[2], rows[3],
+                        kBackwardThreads, kKeyShared, stream, a, weights, delta, sums, rows[2], rows[3],
                         tiles[0], tiles[1]);
   GS_TRY(check_launch());
   if (first_blocks > 0)
