@@ -137,3 +137,20 @@ def test_the_oracle_tells_wrong_windows_apart(plant):
     if plant == "group":
         k, v = k.flip(1), v.flip(1)
     assert (R.attention(q, k, v, [25, 15], **wrong)["out"] - right).abs().max() > 0.05
+
+
+def test_morton_order():
+    from gaussian_splats_b200.refine import morton_order
+
+    corners = torch.tensor([[x, y, z] for z in (0.0, 1.0) for y in (0.0, 1.0) for x in (0.0, 1.0)])
+    shuffled = torch.randperm(8, generator=torch.Generator().manual_seed(0))
+    assert torch.equal(shuffled[morton_order(corners[shuffled])], torch.arange(8))
+    points = torch.rand(4000, 3, generator=torch.Generator().manual_seed(1))
+    order = morton_order(points)
+    assert torch.equal(order.sort().values, torch.arange(4000))
+    # neighbours along the order are near: far nearer than random pairs (0.66 apart)
+    assert (points[order][1:] - points[order][:-1]).norm(dim=1).mean() < 0.12
+    assert torch.equal(morton_order(torch.ones(5, 3)), torch.arange(5))  # ties by index
+    assert morton_order(torch.empty(0, 3)).shape == (0,)
+    with pytest.raises(ValueError):
+        morton_order(torch.zeros(3, 2))
