@@ -238,16 +238,16 @@ __device__ __forceinline__ Affine compose(const Affine (*maps)[kChannels], Affin
   for (int g = 0; g < kGroups; ++g) sum = then(sum, f[g]);
   return sum;
 }
-// The same for a value that passes through them: what enters each group.
+// The same for a value that passes through them: what enters each group takes
+// the place of its map (in `b`).
 template <int kChannels, bool kReverse>
-__device__ __forceinline__ float pass(const Affine (*maps)[kChannels], float (*entering)[kChannels],
-                                      float value) {
+__device__ __forceinline__ float pass(Affine (*maps)[kChannels], int channel, float value) {
   Affine f[kGroups];
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) f[g] = maps[kReverse ? kGroups - 1 - g : g][threadIdx.x];
+  for (int g = 0; g < kGroups; ++g) f[g] = maps[kReverse ? kGroups - 1 - g : g][channel];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    entering[kReverse ? kGroups - 1 - g : g][threadIdx.x] = value;
+    maps[kReverse ? kGroups - 1 - g : g][channel].b = value;
     value = fmaf(f[g].a, value, f[g].b);
   }
   return value;
@@ -305,7 +305,6 @@ __device__ __forceinline__ void walk(const gs_gated_scan_args& a, const typename
                                      Source& source, const float* states) {
   constexpr int V = Source::V, kChannels = Source::At::kChannels;
   __shared__ Affine s_maps[kGroups][kChannels];
-  __shared__ float s_entering[kGroups][kChannels];
   const int joined = at.block_channel + threadIdx.x;  // the channel that the thread joins
   const bool joins = threadIdx.x < kChannels && joined < a.channels;
   float carry = joins ? states[at.slot * a.channels + joined] : 0.0f;
@@ -336,12 +335,12 @@ __device__ __forceinline__ void walk(const gs_gated_scan_args& a, const typename
     if (threadIdx.x < kChannels) {
       if (!source.good) carry = NAN;
       if (joins) a.entering[(at.tile + step) * a.channels + joined] = carry;
-      carry = pass<kChannels, false>(s_maps, s_entering, carry);
+      carry = pass<kChannels, false>(s_maps, threadIdx.x, carry);
     }
     __syncthreads();
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = s_entering[at.group()][at.lane() * V + v];
+    for (int v = 0; v < V; ++v) h[v] = s_maps[at.group()][at.lane() * V + v].b;
     const int first = at.first(step), count = live ? at.count(step) : 0;
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
@@ -360,14 +359,15 @@ __device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
                                           const float* messages) {
   constexpr int V = Source::V, kChannels = Source::At::kChannels;
   __shared__ Affine s_ahead[kGroups][kChannels], s_back[kGroups][kChannels];
-  __shared__ float s_state[kGroups][kChannels], s_message[kGroups][kChannels];
-  const int joined = at.block_channel + threadIdx.x;
-  const bool joins = threadIdx.x < kChannels && joined < a.channels;
-  float carry = joins ? messages[at.slot * a.channels + joined] : 0.0f;
+  // One thread a channel passes the state on, another one the message.
+  const int joined = at.block_channel + threadIdx.x % kChannels;
+  const bool forward = threadIdx.x < kChannels;
+  const bool joins = threadIdx.x < 2 * kChannels && joined < a.channels;
+  float carry = joins && !forward ? messages[at.slot * a.channels + joined] : 0.0f;
   const bool live = at.channel() < a.channels;
   for (int step = 0; step < at.tiles; ++step) {
     const int i = at.tiles - 1 - step;
-    const float state = joins ? a.entering[(at.tile + i) * a.channels + joined] : 0.0f;
+    if (joins && forward) carry = a.entering[(at.tile + i) * a.channels + joined];
     float x[kTokens][V], al[kTokens][V], keep[kTokens][V];
     Affine ahead[V], back[V];
 #pragma unroll
@@ -402,17 +402,16 @@ __device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
     __syncthreads();
     // The last step's gradients have been read for the second time by now.
     if (step > 0) source.release(step - 1);
-    if (threadIdx.x < kChannels) {
-      if (!source.good) carry = NAN;
-      pass<kChannels, false>(s_ahead, s_state, state);
-      carry = pass<kChannels, true>(s_back, s_message, carry);
-    }
+    if (!source.good) carry = NAN;
+    if (forward) pass<kChannels, false>(s_ahead, threadIdx.x, carry);
+    else if (threadIdx.x < 2 * kChannels)
+      carry = pass<kChannels, true>(s_back, threadIdx.x - kChannels, carry);
     __syncthreads();
     float h[V], u[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      h[v] = s_state[at.group()][at.lane() * V + v];
-      u[v] = s_message[at.group()][at.lane() * V + v];
+      h[v] = s_ahead[at.group()][at.lane() * V + v].b;
+      u[v] = s_back[at.group()][at.lane() * V + v].b;
     }
     const int count = live ? at.count(i) : 0;
     const int64_t offset = int64_t{at.first(i)} * a.channels + at.channel();
