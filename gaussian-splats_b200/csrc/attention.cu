@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {  // products, issued by the first lane
+  } else if (warp == 9) {  // products
     const int lane = threadIdx.x & 31;
+    const uint32_t elected = elect_lane();
     const int dim_steps = (a.dim + 15) / 16;
     const uint32_t sum_kind = product_kind<T>(dim_steps * 16, true);
     const uint32_t score_kind = product_kind<T>(0, false);
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
         good = good && barrier_wait_warp(shared_address(&bars[plan & 15]), plan >> 4 & 1);
     };
     const auto release = [&](uint64_t* bars, uint32_t plan) {
-      if (plan & 64) commit(shared_address(&bars[plan & 15]));
+      if (plan & 64) commit(elected, shared_address(&bars[plan & 15]));
     };
     const auto issue_scores = [&](auto number, uint32_t plan) {
       constexpr int g = decltype(number)::value;
@@ -333,10 +334,10 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
 #pragma unroll
       for (int i = 0; i < kDim / 16; ++i)
         if (i < dim_steps)
-          multiply(tensor + g * Shape::kGroupColumns,
+          multiply(elected, tensor + g * Shape::kGroupColumns,
                    q + g * (Shared::kQueryBytes >> 4) + channels_step<kTile>(i),
                    keys + channels_step<kKeys>(i), kind, i > 0);
-      commit(shared_address(&s.scores[g]));
+      commit(elected, shared_address(&s.scores[g]));
     };
     const auto run_step = [&](auto number, int step, uint32_t plan) {
       constexpr int g = decltype(number)::value;
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
       wait_for(s.v_full, plan);
       if (more) wait_for(s.k_full, plan >> 8);
       good = good && barrier_wait_warp(shared_address(&s.weights[g]), step & 1);
-      if (good && lane == 0) {
+      if (good) {
         fence_after_sync();
         constexpr uint32_t column = g * Shape::kGroupColumns;
         const uint32_t values = v + (plan & 15) * (Shared::kTileBytes >> 4);
@@ -353,14 +354,13 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i)
           if (i < count)
-            multiply_tensor(tensor + column + kKeys, tensor + column + 8 * i,
+            multiply_tensor(elected, tensor + column + kKeys, tensor + column + 8 * i,
                             values + rows_step(i), sum_kind, step > 0 || i > 0);
         if (more) issue_scores(number, plan);  // in order behind the product that reads P
-        else commit(shared_address(&s.summed[g]));
+        else commit(elected, shared_address(&s.summed[g]));
         release(s.v_empty, plan);
         if (more) release(s.k_empty, plan >> 8);
       }
-      __syncwarp();
     };
     const auto start = [&](auto number) {
       constexpr int g = decltype(number)::value;
@@ -368,11 +368,10 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
       const uint32_t plan = plan_of(g, -1);
       wait_for(s.k_full, plan >> 8);
       good = good && barrier_wait_warp(shared_address(&s.q_full[g]), 0);
-      if (good && lane == 0) {
+      if (good) {
         issue_scores(number, plan);
         release(s.k_empty, plan >> 8);
       }
-      __syncwarp();
     };
     using First = std::integral_constant<int, 0>;
     using Second = std::integral_constant<int, 1>;
@@ -695,7 +694,7 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
   constexpr int kRows = Shape::kRows;
   constexpr uint32_t kWords = Shape::kBytes >> 4, kTileWords = Shape::kTileBytes >> 4;
   const uint32_t tensor = s.tensor;
-  const bool issues = (threadIdx.x & 31) == 0;
+  const uint32_t elected = elect_lane();
   const int steps = (dim + 15) / 16;
   const uint32_t score_kind = product_kind<T>(0, false);
   const uint32_t sum_kind = product_kind<T>((dim + 15) / 16 * 16, true);
@@ -710,9 +709,9 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
       if (i < steps)
-        multiply(tensor + column, a + channels_step<kTile>(i), b + channels_step<kRows>(i), kind,
+        multiply(elected, tensor + column, a + channels_step<kTile>(i), b + channels_step<kRows>(i), kind,
                  i > 0);
-    commit(shared_address(ready));
+    commit(elected, shared_address(ready));
   };
   // A sum from the weights at `column` and operand `operand` of a stage.
   const auto issue_sum = [&](int operand, int stage, int count, uint32_t column, uint32_t sum,
@@ -721,18 +720,17 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
 #pragma unroll
     for (int i = 0; i < kRows / 16; ++i)
       if (i < 2 * count)
-        multiply_tensor(tensor + sum, tensor + column + weight_column(i), b + rows_step(i),
+        multiply_tensor(elected, tensor + sum, tensor + column + weight_column(i), b + rows_step(i),
                         sum_kind, add || i > 0);
   };
   bool good = barrier_wait_warp(shared_address(&s.rows_full), 0) &&
               barrier_wait_warp(shared_address(&s.full0[0]), 0) &&
               barrier_wait_warp(shared_address(&s.full1[0]), 0);
   int count = sets(0);
-  if (good && issues) {
+  if (good) {
     issue_scores(0, 0, count, 0, &s.scores);
     issue_scores(1, 0, count, Shape::kGrad, &s.grads[0]);
   }
-  __syncwarp();
   int stage0 = 0, stage1 = 0;  // of tile t
   int next0 = 0, parity0 = 0, next1 = 0, parity1 = 0;  // of tile t + 1
   for (int t = 0; t < tiles && good; ++t) {
@@ -753,7 +751,7 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
     if (more && !kKeyRows)
       good = good && barrier_wait_warp(shared_address(&s.full1[next1]), parity1);
     good = good && barrier_wait_warp(shared_address(&s.read), t & 1);
-    if (good && issues) {
+    if (good) {
       fence_after_sync();
       if constexpr (kKeyRows) issue_sum(1, stage1, count, 0, Shape::kSum + kDim, t > 0);
       // In order behind the sum that reads P (keys), with S read (queries).
@@ -763,23 +761,21 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
         if constexpr (!kKeyRows) issue_scores(1, next1, next_count, next_grad, next_ready);
       }
     }
-    __syncwarp();
     if (more && kKeyRows)
       good = good && barrier_wait_warp(shared_address(&s.full1[next1]), parity1);
     good = good && barrier_wait_warp(shared_address(&s.weights[t & 1]), (t >> 1) & 1);
-    if (good && issues) {
+    if (good) {
       fence_after_sync();
       issue_sum(0, stage0, count, grad, Shape::kSum, t > 0);
-      commit(shared_address(more ? &s.empty[stage0] : &s.done));
+      commit(elected, shared_address(more ? &s.empty[stage0] : &s.done));
       if constexpr (kKeyRows)
         if (more) issue_scores(1, next1, next_count, next_grad, next_ready);
     }
-    __syncwarp();
     stage0 = next0;
     stage1 = next1;
     count = next_count;
   }
-  if (!good && issues) atomicExch(&g_timeout, 1u);
+  if (!good && elected) atomicExch(&g_timeout, 1u);
   __syncwarp();
 }
 

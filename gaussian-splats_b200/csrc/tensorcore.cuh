@@ -189,28 +189,43 @@ __device__ __forceinline__ uint32_t product_kind(int n, bool rows_b) {
          static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
-// D (+)= A B^T with A and B in shared memory (low words of descriptors).
-__device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint32_t b, uint32_t kind,
-                                         bool add) {
+// One lane of a warp that is converged here: 1 for it, 0 for the others. The
+// whole warp goes through the code that issues products, with the instruction
+// itself predicated to that lane: its operands are then the warp's and stay in
+// uniform registers.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t elected;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(descriptor(a)), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add))
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(elected));
+  return elected;
+}
+// D (+)= A B^T with A and B in shared memory (low words of descriptors).
+__device__ __forceinline__ void multiply(uint32_t elected, uint32_t d, uint32_t a, uint32_t b,
+                                         uint32_t kind, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(descriptor(a)), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add)),
+      "r"(elected)
       : "memory");
 }
 // D (+)= A B^T with A in tensor memory (two 16-bit values a column).
-__device__ __forceinline__ void multiply_tensor(uint32_t d, uint32_t a, uint32_t b, uint32_t kind,
-                                                bool add) {
+__device__ __forceinline__ void multiply_tensor(uint32_t elected, uint32_t d, uint32_t a,
+                                                uint32_t b, uint32_t kind, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add))
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add)), "r"(elected)
       : "memory");
 }
 // The barrier's phase completes when the products issued so far have.
-__device__ __forceinline__ void commit(uint32_t bar) {
+__device__ __forceinline__ void commit(uint32_t elected, uint32_t bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(elected)
       : "memory");
 }
 
