@@ -666,7 +666,12 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
     const int2 at = place(t);
     if (lane == 0) load(s.tiles0[stage0], &s.full0[stage0], tile_map0, at);
     __syncwarp();
-    wait_for(t - kStages1);
+    if constexpr (kKeyRows) {
+      wait_for(t - kStages1);
+    } else if (t >= kStages1) {  // only G read the tile that had the place before
+      const int u = t - kStages1;
+      good = good && barrier_wait_warp(shared_address(&s.grads[u & 1]), (u >> 1) & 1);
+    }
     if (!good) break;
     keep(stage1, lane, values);
     if (lane == 0) load(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
@@ -1039,7 +1044,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
   const int64_t item = blockIdx.x / a.kv_heads;
   const bool chunk = item < sums.slots;  // the long items come first
   Tile tile;
-  int64_t low, high;  // queries, as positions
+  int low, high;  // queries, as positions
   if (chunk) {
     const int64_t b = sequence_of_run(a, item, sums.tiles);
     const int64_t tile0 = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
@@ -1047,17 +1052,17 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     if (index >= tiles) return;
     tile = tile_at(a.tiles, tile0, static_cast<int32_t>(a.tokens), kTile);
     const int64_t n = tile.end - tile.begin;
-    low = max(index * kTile, int64_t{a.left} + 1);
-    high = min((index + sums.tiles) * kTile, n);
+    low = position(max(index * kTile, int64_t{a.left} + 1));
+    high = static_cast<int>(min((index + sums.tiles) * kTile, n));
     if (low >= high) return;
   } else {
     tile = tile_at(a.tiles, item - sums.slots, static_cast<int32_t>(a.tokens), kTile);
     const int64_t n = tile.end - tile.begin, j = tile.start - tile.begin;
-    low = max(int64_t{0}, j - a.right);
-    high = min(n, min(j + kTile, n) + a.left);
+    low = max(0, position(j - a.right));
+    high = static_cast<int>(min(n, min(j + kTile, n) + a.left));
   }
   const int n = tile.end - tile.begin;
-  const int per_head = static_cast<int>((high - low + kRows - 1) / kRows);
+  const int per_head = (high - low + kRows - 1) / kRows;
   const int tiles = per_head * group;
   backward_setup(s, warp);
   const uint32_t tensor = s.tensor;
@@ -1070,11 +1075,11 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         s, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
         [&](int t) {
           return make_int2(kv_head * group + t / per_head,
-                           tile.begin + static_cast<int>(low) + (t % per_head) * kRows);
+                           tile.begin + low + (t % per_head) * kRows);
         },
         [&](int t, int lane) {
           RowValues v;
-          const int64_t i = low + (t % per_head) * kRows + lane;
+          const int i = low + (t % per_head) * kRows + lane;
           const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
@@ -1093,36 +1098,37 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         });
   } else if (warp == kProductWarp) {
     issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
-      return static_cast<int>(
-          min(int64_t{kSets}, (high - low - (t % per_head) * kRows + 31) / 32));
+      return min(kSets, (high - low - (t % per_head) * kRows + 31) / 32);
     });
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int64_t j_first = tile.start - tile.begin, j = j_first + row;
+    const int j_first = tile.start - tile.begin, j = j_first + row;
     const bool live = j < n && (!chunk || j < a.first);
     const bool seen = live && (!a.valid || a.valid[tile.start + row]);
-    const bool any_seen = __any_sync(0xffffffffu, seen);
+    const bool any_seen = __any_sync(0xffffffffu, seen), all_seen = __all_sync(0xffffffffu, seen);
+    // The queries that see key j: those from `from` to `to`. All of the block's keys
+    // are seen by the queries from `all_from` to `all_to`.
+    const int from = chunk ? position(int64_t{j} + a.left + 1) : position(int64_t{j} - a.right);
+    const int to = chunk ? high : min(high, position(int64_t{j} + a.left + 1));
+    const int all_from = position(int64_t{j_first} + kTile - 1 - a.right);
+    const int all_to = chunk ? 0 : min(high, position(int64_t{j_first} + a.left + 1));
     const float scale = a.scale * kLog2e;
     const float2 factor = make_float2(scale, scale), grow = make_float2(weights.e_p, weights.e_p);
     const uint32_t scores = mine + 32 * kHalfSets * half, grads = scores + Shape::kGrad;
     bool good = true;
     int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
     for (int t = 0; t < tiles; ++t) {
-      const int64_t start = low + index * kRows, first = start + 32 * kHalfSets * half;
+      const int start = low + index * kRows, first = start + 32 * kHalfSets * half;
       // Sets of 32 queries of this half; what lies past the last has no products.
-      const int sets = static_cast<int>(min(int64_t{kHalfSets}, (high - first + 31) >> 5));
-      uint64_t wide = seen ? below(high - first) : 0;
-      if (chunk) wide &= ~below(j + a.left + 1 - first);
-      else wide &= below(j + a.left + 1 - first) & ~below(j - a.right - first);
+      const int sets = min(kHalfSets, (high - first + 31) >> 5);
+      const bool whole = all_seen && start >= all_from && start + kRows <= all_to;
       uint32_t bits[kHalfSets];
-      bool mine_whole = true;
+      if (!whole) {
 #pragma unroll
-      for (int h = 0; h < kHalfSets; ++h) {
-        bits[h] = static_cast<uint32_t>(wide >> (32 * h));
-        mine_whole = mine_whole && bits[h] == ~0u;
+        for (int h = 0; h < kHalfSets; ++h)
+          bits[h] = seen ? below32(to - first - 32 * h) & ~below32(from - first - 32 * h) : 0;
       }
-      const bool whole = __all_sync(0xffffffffu, mine_whole);
       if (!(good = barrier_wait_warp(shared_address(&s.scores), t & 1) &&
                    barrier_wait_warp(shared_address(&s.full1[stage1]), parity1)))
         break;
@@ -1164,7 +1170,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
           store_columns16(scores + 32 * h, packed);
         }
       if (start + kRows > n) {
-        const int rest = n - static_cast<int>(start);
+        const int rest = n - start;
         uint32_t keep[kSets];
 #pragma unroll
         for (int c = 0; c < kSets; ++c) keep[c] = below32(rest - 32 * c);
