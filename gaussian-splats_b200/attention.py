@@ -80,9 +80,8 @@ class _WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, packed, left, right, first, valid, scale, dtype, need_grad):
         q, k, v = _strided(q.detach()), _strided(k.detach()), _strided(v.detach())
         tokens, heads, dim = q.shape
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-        lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if need_grad \
-            else None
+        out = q.new_empty((tokens, heads, dim))
+        lse = q.new_empty((heads, tokens), dtype=torch.float32) if need_grad else None
         args = _arguments(native.WindowAttentionArgs, q, k, v, tokens=tokens,
                           **tile_arguments(packed, tokens), heads=heads, kv_heads=k.shape[1], dim=dim, dtype=dtype,
                           left=left, right=right, first=first, scale=scale, valid=address(valid),
@@ -100,13 +99,12 @@ class _WindowAttention(torch.autograd.Function):
         grad_out = grad_out.contiguous()
         if grad_out.data_ptr() % 16:
             grad_out = grad_out.clone()
-        grad_q, grad_k, grad_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                                  for t in (q, k, v))
+        grad_q, grad_k, grad_v = (t.new_empty(t.shape) for t in (q, k, v))
         lib, args = native.lib(), native.WindowAttentionArgs.from_buffer_copy(ctx.args)
         args.q, args.k, args.v, args.out = (t.data_ptr() for t in (q, k, v, out))
         args.lse, args.valid = lse.data_ptr(), address(valid)
         size = lib.gs_window_attention_workspace_size(ctypes.byref(args))
-        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty((size,), dtype=torch.uint8)
         args.grad_out, args.grad_q = grad_out.data_ptr(), grad_q.data_ptr()
         args.grad_k, args.grad_v = grad_k.data_ptr(), grad_v.data_ptr()
         args.workspace, args.workspace_size = workspace.data_ptr(), size
@@ -213,7 +211,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          f"{tuple(positions.shape)}")
     positions = positions.contiguous()
     q, k, v = _strided(q), _strided(k), _strided(v)
-    out = torch.empty((batch, heads, dim), dtype=q.dtype, device=device)
+    out = q.new_empty((batch, heads, dim))
     args = _arguments(native.WindowAttentionStepArgs, q, k, v, batch=batch, heads=heads,
                       kv_heads=k.shape[1], dim=dim, dtype=dtype, slots=shape[1], first=first,
                       scale=_scale(what, scale, dim), cache_k=cache_k.data_ptr(),

@@ -537,8 +537,7 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
   GS_TRY(tc::encode_heads(&v, a.dtype, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride,
                           a.v_head_stride, kKeys));
   constexpr size_t kShared = sizeof(ForwardShared<kDim>);
-  GS_CUDA_TRY(cudaFuncSetAttribute(attention_kernel<T, kDim>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  GS_TRY((allow_shared<attention_kernel<T, kDim>>(kShared)));
   const int64_t blocks = (a.num_tiles / 2 + sequences_of(a)) * a.heads;
   if (blocks > INT32_MAX) return GS_ERR_CAPACITY;
   launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(blocks), kForwardThreads,
@@ -1342,10 +1341,8 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   sums.part = sums.base + sequences_of(a) * a.kv_heads * a.first * 2 * a.dim;
   constexpr size_t kQueryShared = sizeof(BackwardShared<kDim, false>);
   constexpr size_t kKeyShared = sizeof(BackwardShared<kDim, true>);
-  GS_CUDA_TRY(cudaFuncSetAttribute(grad_query_kernel<T, kDim>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kQueryShared));
-  GS_CUDA_TRY(cudaFuncSetAttribute(grad_key_kernel<T, kDim>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyShared));
+  GS_TRY((allow_shared<grad_query_kernel<T, kDim>>(kQueryShared)));
+  GS_TRY((allow_shared<grad_key_kernel<T, kDim>>(kKeyShared)));
   const int64_t key_blocks = (a.num_tiles + sums.slots) * a.kv_heads;
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
@@ -1742,10 +1739,7 @@ int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   GS_TRY(tc::encode_heads(&v, a.dtype, a.cache_v, a.batch * a.slots, a.kv_heads, a.dim, row, a.dim,
                           kStepTile));
   constexpr size_t kShared = sizeof(StepShared<kDim, kHalves>);
-  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim, kHalves>,
-                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  GS_CUDA_TRY(cudaFuncSetAttribute(attention_step_kernel<T, kDim, kHalves>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  GS_TRY((allow_shared<attention_step_kernel<T, kDim, kHalves>>(kShared, true)));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

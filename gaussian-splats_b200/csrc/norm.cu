@@ -469,9 +469,7 @@ int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
       return check_launch();
     }));
   } else {
-    GS_CUDA_TRY(cudaFuncSetAttribute(norm_backward_kernel<T, R>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     sizeof(float) * GS_MAX_NORM_CHANNELS));
+    GS_TRY((allow_shared<norm_backward_kernel<T, R>>(sizeof(float) * GS_MAX_NORM_CHANNELS)));
     launch_chained_shared(norm_backward_kernel<T, R>, blocks, kThreads, shared, stream, a,
                           partials);
     GS_TRY(check_launch());

@@ -672,13 +672,6 @@ int32_t encode_maps(const gs_gated_scan_args& a, bool grad_first, Maps* maps) {
   return GS_OK;
 }
 
-template <class Kernel>
-int32_t allow_shared(Kernel* kernel, size_t bytes) {
-  GS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(bytes)));
-  return GS_OK;
-}
-
 template <class T>
 int32_t forward(const gs_gated_scan_args& a, cudaStream_t stream) {
   const bool boxes = whole_words<T>(a);
@@ -692,8 +685,8 @@ int32_t forward(const gs_gated_scan_args& a, cudaStream_t stream) {
   Maps maps = {};
   if (blocks && boxes) {
     GS_TRY(encode_maps<T>(a, false, &maps));
-    GS_TRY(allow_shared(fold_boxes_kernel<T, false>, kShared));
-    GS_TRY(allow_shared(walk_boxes_kernel<T>, kShared));
+    GS_TRY((allow_shared<fold_boxes_kernel<T, false>>(kShared)));
+    GS_TRY((allow_shared<walk_boxes_kernel<T>>(kShared)));
     launch_chained_shared(fold_boxes_kernel<T, false>, blocks, kBoxThreads, kShared, stream, a,
                           spans, folds, maps);
   } else if (blocks) {
@@ -721,7 +714,7 @@ int32_t backward(const gs_gated_scan_args& a, cudaStream_t stream) {
   if (blocks && boxes) {
     Maps maps = {};
     GS_TRY(encode_maps<T>(a, true, &maps));
-    GS_TRY(allow_shared(fold_boxes_kernel<T, true>, sizeof(Boxes<2>)));
+    GS_TRY((allow_shared<fold_boxes_kernel<T, true>>(sizeof(Boxes<2>))));
     launch_chained_shared(fold_boxes_kernel<T, true>, blocks, kBoxThreads, sizeof(Boxes<2>),
                           stream, a, spans, folds, maps);
   } else if (blocks) {
@@ -732,7 +725,7 @@ int32_t backward(const gs_gated_scan_args& a, cudaStream_t stream) {
   if (blocks && boxes) {
     Maps maps = {};
     GS_TRY(encode_maps<T>(a, false, &maps));
-    GS_TRY(allow_shared(walk_back_boxes_kernel<T>, sizeof(Boxes<3>)));
+    GS_TRY((allow_shared<walk_back_boxes_kernel<T>>(sizeof(Boxes<3>))));
     launch_chained_shared(walk_back_boxes_kernel<T>, blocks, kBoxThreads, sizeof(Boxes<3>),
                           stream, a, spans, messages, maps);
   } else if (blocks) {

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -70,6 +71,23 @@ inline int32_t with_dtype(int32_t dtype, F&& f) {
     case GS_FLOAT16: return f(__half{});
   }
   return GS_ERR_INVALID_ARGUMENT;
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory (and clusters of 16 blocks),
+// once a device: the attribute calls cost as much as a launch's other host work.
+template <auto kKernel>
+inline int32_t allow_shared(size_t bytes, bool wide_clusters = false) {
+  static std::atomic<uint64_t> done{0};
+  int device;
+  GS_CUDA_TRY(cudaGetDevice(&device));
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return GS_OK;
+  GS_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(bytes)));
+  if (wide_clusters)
+    GS_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return GS_OK;
 }
 
 // Reads and clears the flag that a kernel sets when a bounded wait ran out.

@@ -61,8 +61,8 @@ class _RmsNorm(torch.autograd.Function):
         shape = x.shape
         rows, weight = _rows(x.detach()), weight.detach().contiguous()
         res = None if residual is None else _rows(residual.detach())
-        y = torch.empty(shape, dtype=x.dtype, device=x.device)
-        total = None if res is None else torch.empty(shape, dtype=res.dtype, device=x.device)
+        y = x.new_empty(shape)
+        total = None if res is None else res.new_empty(shape)
         args = _arguments(rows, weight, res, eps, y=y, sum=total)
         call("gs_rms_norm", x.device, ctypes.byref(args))
         ctx.save_for_backward(rows if res is None else total, weight)
@@ -75,13 +75,13 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, grad_y, grad_sum=None):
         z, weight = ctx.saved_tensors
         rows, shape = _rows(z), ctx.shape
-        grad_y = torch.zeros(shape, dtype=ctx.x_dtype, device=z.device) if grad_y is None \
+        grad_y = z.new_zeros(shape, dtype=ctx.x_dtype) if grad_y is None \
             else grad_y.contiguous()
         grad_sum = None if grad_sum is None else grad_sum.contiguous()
-        grad_x = torch.empty(shape, dtype=ctx.x_dtype, device=z.device)
+        grad_x = z.new_empty(shape, dtype=ctx.x_dtype)
         grad_residual = None
         if ctx.has_residual and z.dtype != ctx.x_dtype:
-            grad_residual = torch.empty(shape, dtype=z.dtype, device=z.device)
+            grad_residual = z.new_empty(shape)
         grad_weight = torch.empty_like(weight)
         args = native.RmsNormArgs(
             rows=rows.shape[0], channels=rows.shape[1], dtype=element_type(ctx.x_dtype, ""),
@@ -92,7 +92,7 @@ class _RmsNorm(torch.autograd.Function):
             grad_residual=address(grad_residual), grad_weight=address(grad_weight))
         lib = native.lib()
         size = lib.gs_rms_norm_workspace_size(ctypes.byref(args))
-        workspace = torch.empty((size,), dtype=torch.uint8, device=z.device)
+        workspace = z.new_empty((size,), dtype=torch.uint8)
         args.workspace, args.workspace_size = address(workspace), size
         call("gs_rms_norm_backward", z.device, ctypes.byref(args))
         if ctx.has_residual and grad_residual is None:
@@ -123,9 +123,9 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     residual, also the sum. No gradient."""
     eps = _check("rms_norm_e4m3", x, weight, residual, eps)
     rows, res = _rows(x), None if residual is None else _rows(residual)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    total = None if res is None else torch.empty(x.shape, dtype=res.dtype, device=x.device)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    total = None if res is None else res.new_empty(x.shape)
     weight = weight.contiguous()
     args = _arguments(rows, weight, res, eps, q=q, scale=scale, sum=total)
     call("gs_rms_norm", x.device, ctypes.byref(args))

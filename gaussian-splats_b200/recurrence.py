@@ -43,16 +43,16 @@ class _GatedScan(torch.autograd.Function):
         tokens, channels = x.shape
         device = x.device
         layout = tile_arguments(packed, tokens)
-        y = torch.empty((tokens, channels), dtype=x.dtype, device=device)
-        last = torch.empty((layout["sequences"], channels), dtype=torch.float32, device=device)
-        entering = torch.empty((layout["num_tiles"], channels), dtype=torch.float32, device=device)
+        y = x.new_empty((tokens, channels))
+        last = x.new_empty((layout["sequences"], channels), dtype=torch.float32)
+        entering = x.new_empty((layout["num_tiles"], channels), dtype=torch.float32)
         args = native.GatedScanArgs(
             tokens=tokens, **layout, channels=channels, dtype=dtype, x=address(x),
             gate=address(gate), x_stride=x.stride(0), gate_stride=gate.stride(0), initial=address(initial),
             y=address(y), last=address(last), entering=address(entering))
         lib = native.lib()
         size = lib.gs_gated_scan_workspace_size(ctypes.byref(args))
-        workspace = torch.empty((size,), dtype=torch.uint8, device=device)
+        workspace = x.new_empty((size,), dtype=torch.uint8)
         args.workspace, args.workspace_size = address(workspace), size
         call("gs_gated_scan", device, ctypes.byref(args))
         ctx.save_for_backward(x, gate, entering)
@@ -66,18 +66,17 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, grad_y, grad_last):
         x, gate, entering = ctx.saved_tensors
         device = x.device
-        grad_y = torch.zeros(x.shape, dtype=x.dtype, device=device) if grad_y is None \
+        grad_y = x.new_zeros(x.shape) if grad_y is None \
             else grad_y.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
-        grad_x, grad_gate = (torch.empty(x.shape, dtype=x.dtype, device=device) for _ in range(2))
+        grad_x, grad_gate = x.new_empty(x.shape), x.new_empty(x.shape)
         args = native.GatedScanArgs.from_buffer_copy(ctx.args)
         args.x, args.gate, args.entering = address(x), address(gate), address(entering)
         args.initial = args.y = args.last = None
         grad_initial = None
         if ctx.has_initial and ctx.needs_input_grad[2]:
-            grad_initial = torch.empty((args.sequences, args.channels), dtype=torch.float32,
-                                       device=device)
-        workspace = torch.empty((ctx.size,), dtype=torch.uint8, device=device)
+            grad_initial = x.new_empty((args.sequences, args.channels), dtype=torch.float32)
+        workspace = x.new_empty((ctx.size,), dtype=torch.uint8)
         args.grad_y, args.grad_last = address(grad_y), address(grad_last)
         args.grad_x, args.grad_gate = address(grad_x), address(grad_gate)
         args.grad_initial, args.workspace = address(grad_initial), address(workspace)
@@ -124,7 +123,7 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
                          f"{tuple(x.shape)}, got {state.dtype} {tuple(state.shape)}"
                          f"{'' if state.is_contiguous() else ' (not contiguous)'}")
     x, gate = _rows(x), _rows(gate)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = x.new_empty(x.shape)
     call("gs_gated_scan_step", device, x.shape[0], x.shape[1], dtype, address(x), x.stride(0),
          address(gate), gate.stride(0), address(state), address(y))
     return y
