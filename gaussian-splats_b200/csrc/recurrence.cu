@@ -42,19 +42,84 @@ constexpr int kTokens = 8;                // tokens a thread holds
 constexpr int kGroups = kTile / kTokens;  // threads that share a channel of a tile
 constexpr int kScanThreads = 1024;
 
-// e = exp(-gate), a = sigmoid(gate) = 1 / (1 + e); k = 1 - a is e a, with the
-// same relative error however small it is. The exponent is cut where a is far
-// below any gate's use, so that e stays finite.
-__device__ __forceinline__ float open_gate(float gate, float& e) {
-  constexpr float kMinusLog2e = -1.4426950408889634f;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(gate * kMinusLog2e, 100.0f)));
-  return __fdividef(1.0f, 1.0f + e);
+constexpr float kMinusLog2e = -1.4426950408889634f;
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 both(float x) { return {x, x}; }
+__device__ __forceinline__ float2 minus(float2 a, float2 b) {
+  return tc::fma2(b, both(-1.0f), a);
+}
+
+// Two gates at a time, as is all arithmetic here: the instructions that a pass
+// issued took longer than its memory did. -a = -sigmoid(gate) = 1 / (-1 - e),
+// e = exp(-gate); e may be infinite, a NaN stays one.
+__device__ __forceinline__ float2 minus_gate(float2 gate) {
+  const float2 t = tc::mul2(gate, both(kMinusLog2e));
+  const float2 d =
+      tc::fma2({tc::exp2_approx(t.x), tc::exp2_approx(t.y)}, both(-1.0f), both(-1.0f));
+  return {reciprocal(d.x), reciprocal(d.y)};
+}
+// a, and k = 1 - a as e a, with the same relative error however small it is. e is
+// cut at 2^100 so that it stays finite; 2^-100 less, a shut gate's a is nothing.
+__device__ __forceinline__ float2 open_gate(float2 gate, float2& keep) {
+  const float2 t = tc::mul2(gate, both(kMinusLog2e));
+  const auto cut = [](float x) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(100.0f));
+    return tc::exp2_approx(y);
+  };
+  const float2 e = {cut(t.x), cut(t.y)}, d = tc::add2(e, both(1.0f));
+  const float2 a = {reciprocal(d.x), reciprocal(d.y)};
+  keep = tc::mul2(e, a);
+  return tc::add2(a, both(-0x1p-100f));
+}
+
+// N channels of a thread, in pairs. (A last one alone has a pair of its own.)
+template <int N>
+constexpr int kPairs = (N + 1) / 2;
+template <int N, class T>
+__device__ __forceinline__ void store_pairs(T* p, const float2 (&x)[kPairs<N>]) {
+  Pack<T, N> a;
+#pragma unroll
+  for (int v = 0; v < N; ++v) a.v[v] = from_float<T>(v % 2 ? x[v / 2].y : x[v / 2].x);
+  *reinterpret_cast<Pack<T, N>*>(p) = a;
+}
+// A word of shared memory: two values of 16 bits, or one.
+template <class T>
+__device__ __forceinline__ float2 from_word(uint32_t w) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+  else
+    return __half22float2(reinterpret_cast<const __half2&>(w));
 }
 
 // A map s -> a s + b.
 struct Affine {
   float a, b;
 };
+template <int N>
+struct Affines {  // those of N channels
+  float2 a[kPairs<N>], b[kPairs<N>];
+  __device__ __forceinline__ Affines() {
+#pragma unroll
+    for (int v = 0; v < kPairs<N>; ++v) a[v] = both(1.0f), b[v] = both(0.0f);
+  }
+  __device__ __forceinline__ void put(Affine* maps) const {
+#pragma unroll
+    for (int v = 0; v < N; ++v)
+      maps[v] = v % 2 ? Affine{a[v / 2].y, b[v / 2].y} : Affine{a[v / 2].x, b[v / 2].x};
+  }
+};
+// The values that `pass` left in the maps.
+template <int N>
+__device__ __forceinline__ void take(const Affine* maps, float2 (&x)[kPairs<N>]) {
+#pragma unroll
+  for (int v = 0; v < N; ++v) (v % 2 ? x[v / 2].y : x[v / 2].x) = maps[v].b;
+  if constexpr (N % 2) x[N / 2].y = 0.0f;
+}
 __device__ __forceinline__ Affine then(Affine first, Affine second) {
   return {second.a * first.a, fmaf(second.a, first.b, second.b)};
 }
@@ -172,15 +237,23 @@ struct BoxSource {
       request(step + kStages);
     }
   }
+  // Array 0 is the gate.
   template <int kArray>
-  __device__ __forceinline__ void read(int step, int t, float missing, float (&x)[V]) const {
+  __device__ __forceinline__ void read(int step, int t, float2 (&x)[kPairs<V>]) const {
     const int r = at.group() * kTokens + t;
-    load_pack<V>(reinterpret_cast<const T*>(s.data[step % kStages][kArray] + r * 128) +
-                     at.lane() * V,
-                 x);
-    if (t >= at.count(tile_of(step)))
-#pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = missing;
+    uint2 w = *reinterpret_cast<const uint2*>(s.data[step % kStages][kArray] + r * 128 +
+                                              at.lane() * 8);
+    constexpr uint32_t kMissing = kArray                              ? 0u
+                                  : std::is_same_v<T, float>          ? 0xff800000u
+                                  : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u
+                                                                      : 0xfc00fc00u;
+    if (t >= at.count(tile_of(step))) w = {kMissing, kMissing};
+    if constexpr (std::is_same_v<T, float>) {
+      x[0] = {__uint_as_float(w.x), __uint_as_float(w.y)};
+    } else {
+      x[0] = from_word<T>(w.x);
+      x[1] = from_word<T>(w.y);
+    }
   }
   // At the end: whether all waits came back; if not, copies still in flight land first.
   __device__ __forceinline__ void finish() {
@@ -220,11 +293,12 @@ struct PlainSource {
   __device__ __forceinline__ void release(int) {}
   __device__ __forceinline__ void finish() {}
   template <int kArray>
-  __device__ __forceinline__ void read(int step, int t, float missing, float (&x)[V]) const {
+  __device__ __forceinline__ void read(int step, int t, float2 (&x)[1]) const {
     const int i = tile_of(step);
-    x[0] = live && t < at.count(i)
-               ? to_float(base[kArray][(at.first(i) + t) * stride[kArray] + at.channel()])
-               : missing;
+    x[0].x = live && t < at.count(i)
+                 ? to_float(base[kArray][(at.first(i) + t) * stride[kArray] + at.channel()])
+                 : (kArray ? 0.0f : kShut);
+    x[0].y = 0.0f;
   }
 };
 
@@ -254,8 +328,8 @@ __device__ __forceinline__ float pass(Affine (*maps)[kChannels], int channel, fl
 }
 
 // Folds every span: forward the map of the state through it, backward the map
-// of the message through it (from its end to its start). h + a (x - h) and
-// A - a A save forming k. Arrays: gate, and x or grad_y.
+// of the message through it (from its end to its start). h - (-a) (x - h) and
+// A + (-a) A save forming k. Arrays: gate, and x or grad_y.
 template <class Source, bool kBackward>
 __device__ __forceinline__ void fold(const gs_gated_scan_args& a, const typename Source::At& at,
                                      Source& source, Affine* folds) {
@@ -263,31 +337,27 @@ __device__ __forceinline__ void fold(const gs_gated_scan_args& a, const typename
   __shared__ Affine s_maps[kGroups][kChannels];
   Affine span = {1.0f, 0.0f};
   for (int step = 0; step < at.tiles; ++step) {
-    Affine f[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = {1.0f, 0.0f};
+    Affines<V> f;
     source.wait(step);
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
       const int t = kBackward ? kTokens - 1 - i : i;
-      float gate[V], x[V];
-      source.template read<0>(step, t, kShut, gate);
-      source.template read<1>(step, t, 0.0f, x);
+      float2 gate[kPairs<V>], x[kPairs<V>];
+      source.template read<0>(step, t, gate);
+      source.template read<1>(step, t, x);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float e;
-        const float al = open_gate(gate[v], e);
+      for (int v = 0; v < kPairs<V>; ++v) {
+        const float2 al = minus_gate(gate[v]);
         if constexpr (kBackward) {
-          const float l = x[v] + f[v].b;
-          f[v].b = fmaf(-al, l, l);
+          const float2 l = tc::add2(x[v], f.b[v]);
+          f.b[v] = tc::fma2(al, l, l);
         } else {
-          f[v].b = fmaf(al, x[v] - f[v].b, f[v].b);
+          f.b[v] = tc::fma2(al, minus(f.b[v], x[v]), f.b[v]);
         }
-        f[v].a = fmaf(-al, f[v].a, f[v].a);
+        f.a[v] = tc::fma2(al, f.a[v], f.a[v]);
       }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) s_maps[at.group()][at.lane() * V + v] = f[v];
+    f.put(&s_maps[at.group()][at.lane() * V]);
     __syncthreads();
     source.release(step);
     if (threadIdx.x < kChannels) span = compose<kChannels, kBackward>(s_maps, span);
@@ -311,25 +381,21 @@ __device__ __forceinline__ void walk(const gs_gated_scan_args& a, const typename
   T* y = static_cast<T*>(a.y) + at.channel();
   const bool live = at.channel() < a.channels;
   for (int step = 0; step < at.tiles; ++step) {
-    float x[kTokens][V], al[kTokens][V];
-    Affine f[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = {1.0f, 0.0f};
+    float2 x[kTokens][kPairs<V>], al[kTokens][kPairs<V>];  // al: -a
+    Affines<V> f;
     source.wait(step);
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
-      source.template read<0>(step, t, kShut, al[t]);
-      source.template read<1>(step, t, 0.0f, x[t]);
+      source.template read<0>(step, t, al[t]);
+      source.template read<1>(step, t, x[t]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float e;
-        al[t][v] = open_gate(al[t][v], e);
-        f[v].b = fmaf(al[t][v], x[t][v] - f[v].b, f[v].b);
-        f[v].a = fmaf(-al[t][v], f[v].a, f[v].a);
+      for (int v = 0; v < kPairs<V>; ++v) {
+        al[t][v] = minus_gate(al[t][v]);
+        f.b[v] = tc::fma2(al[t][v], minus(f.b[v], x[t][v]), f.b[v]);
+        f.a[v] = tc::fma2(al[t][v], f.a[v], f.a[v]);
       }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) s_maps[at.group()][at.lane() * V + v] = f[v];
+    f.put(&s_maps[at.group()][at.lane() * V]);
     __syncthreads();
     source.release(step);
     if (threadIdx.x < kChannels) {
@@ -338,15 +404,14 @@ __device__ __forceinline__ void walk(const gs_gated_scan_args& a, const typename
       carry = pass<kChannels, false>(s_maps, threadIdx.x, carry);
     }
     __syncthreads();
-    float h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = s_maps[at.group()][at.lane() * V + v].b;
+    float2 h[kPairs<V>];
+    take<V>(&s_maps[at.group()][at.lane() * V], h);
     const int first = at.first(step), count = live ? at.count(step) : 0;
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = fmaf(al[t][v], x[t][v] - h[v], h[v]);
-      if (t < count) store_pack<V>(y + int64_t{first + t} * a.channels, h);
+      for (int v = 0; v < kPairs<V>; ++v) h[v] = tc::fma2(al[t][v], minus(h[v], x[t][v]), h[v]);
+      if (t < count) store_pairs<V>(y + int64_t{first + t} * a.channels, h);
     }
   }
   source.finish();
@@ -368,37 +433,32 @@ __device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
   for (int step = 0; step < at.tiles; ++step) {
     const int i = at.tiles - 1 - step;
     if (joins && forward) carry = a.entering[(at.tile + i) * a.channels + joined];
-    float x[kTokens][V], al[kTokens][V], keep[kTokens][V];
-    Affine ahead[V], back[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) ahead[v] = back[v] = {1.0f, 0.0f};
+    float2 x[kTokens][kPairs<V>], al[kTokens][kPairs<V>], keep[kTokens][kPairs<V>];
+    Affines<V> ahead, back;
     source.wait(step);
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
-      source.template read<0>(step, t, kShut, al[t]);
-      source.template read<1>(step, t, 0.0f, x[t]);
+      source.template read<0>(step, t, al[t]);
+      source.template read<1>(step, t, x[t]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float e;
-        al[t][v] = open_gate(al[t][v], e);
-        keep[t][v] = e * al[t][v];
-        ahead[v].b = fmaf(al[t][v], x[t][v] - ahead[v].b, ahead[v].b);
-        ahead[v].a *= keep[t][v];
+      for (int v = 0; v < kPairs<V>; ++v) {
+        al[t][v] = open_gate(al[t][v], keep[t][v]);
+        ahead.b[v] = tc::fma2(al[t][v], minus(x[t][v], ahead.b[v]), ahead.b[v]);
+        ahead.a[v] = tc::mul2(ahead.a[v], keep[t][v]);
       }
     }
 #pragma unroll
     for (int t = kTokens - 1; t >= 0; --t) {
-      float g[V];
-      source.template read<2>(step, t, 0.0f, g);
+      float2 g[kPairs<V>];
+      source.template read<2>(step, t, g);
 #pragma unroll
-      for (int v = 0; v < V; ++v) back[v].b = keep[t][v] * (g[v] + back[v].b);
+      for (int v = 0; v < kPairs<V>; ++v)
+        back.b[v] = tc::mul2(keep[t][v], tc::add2(g[v], back.b[v]));
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      back[v].a = ahead[v].a;
-      s_ahead[at.group()][at.lane() * V + v] = ahead[v];
-      s_back[at.group()][at.lane() * V + v] = back[v];
-    }
+    for (int v = 0; v < kPairs<V>; ++v) back.a[v] = ahead.a[v];
+    ahead.put(&s_ahead[at.group()][at.lane() * V]);
+    back.put(&s_back[at.group()][at.lane() * V]);
     __syncthreads();
     // The last step's gradients have been read for the second time by now.
     if (step > 0) source.release(step - 1);
@@ -407,12 +467,9 @@ __device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
     else if (threadIdx.x < 2 * kChannels)
       carry = pass<kChannels, true>(s_back, threadIdx.x - kChannels, carry);
     __syncthreads();
-    float h[V], u[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = s_ahead[at.group()][at.lane() * V + v].b;
-      u[v] = s_back[at.group()][at.lane() * V + v].b;
-    }
+    float2 h[kPairs<V>], u[kPairs<V>];
+    take<V>(&s_ahead[at.group()][at.lane() * V], h);
+    take<V>(&s_back[at.group()][at.lane() * V], u);
     const int count = live ? at.count(i) : 0;
     const int64_t offset = int64_t{at.first(i)} * a.channels + at.channel();
     T* grad_x = static_cast<T*>(a.grad_x) + offset;
@@ -421,25 +478,25 @@ __device__ __forceinline__ void walk_back(const gs_gated_scan_args& a,
 #pragma unroll
     for (int t = 0; t < kTokens; ++t)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        x[t][v] -= h[v];
-        h[v] = fmaf(al[t][v], x[t][v], h[v]);
+      for (int v = 0; v < kPairs<V>; ++v) {
+        x[t][v] = minus(x[t][v], h[v]);
+        h[v] = tc::fma2(al[t][v], x[t][v], h[v]);
       }
     // back: g becomes dx_t and x_t becomes dgate_t
 #pragma unroll
     for (int t = kTokens - 1; t >= 0; --t) {
-      float g[V];
-      source.template read<2>(step, t, 0.0f, g);
+      float2 g[kPairs<V>];
+      source.template read<2>(step, t, g);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float l = g[v] + u[v];
-        u[v] = keep[t][v] * l;
-        g[v] = al[t][v] * l;
-        x[t][v] *= u[v] * al[t][v];
+      for (int v = 0; v < kPairs<V>; ++v) {
+        const float2 l = tc::add2(g[v], u[v]);
+        u[v] = tc::mul2(keep[t][v], l);
+        g[v] = tc::mul2(al[t][v], l);
+        x[t][v] = tc::mul2(x[t][v], tc::mul2(u[v], al[t][v]));
       }
       if (t < count) {
-        store_pack<V>(grad_x + int64_t{t} * a.channels, g);
-        store_pack<V>(grad_gate + int64_t{t} * a.channels, x[t]);
+        store_pairs<V>(grad_x + int64_t{t} * a.channels, g);
+        store_pairs<V>(grad_gate + int64_t{t} * a.channels, x[t]);
       }
     }
   }
@@ -590,9 +647,8 @@ __global__ void __launch_bounds__(256) scan_step_kernel(int64_t count, int chann
   if (i >= count) return;
   const int64_t row = i / channels;
   const int c = static_cast<int>(i - row * channels);
-  float e;
-  const float al = open_gate(to_float(gate[row * gate_stride + c]), e);
-  const float h = fmaf(al, to_float(x[row * x_stride + c]) - state[i], state[i]);
+  const float al = minus_gate(both(to_float(gate[row * gate_stride + c]))).x;
+  const float h = fmaf(al, state[i] - to_float(x[row * x_stride + c]), state[i]);
   state[i] = h;
   y[i] = from_float<T>(h);
 }

@@ -138,6 +138,35 @@ def test_a_bad_sequence_stays_alone():
         assert torch.equal(got[n][350:], clean[n][350:])
 
 
+@pytest.mark.parametrize("channels", [64, 33], ids=["boxes", "plain"])
+def test_infinite_gates_and_nan(channels):
+    """A gate of minus infinity keeps the state, one of plus infinity takes the
+    input; a NaN is in its own channel's states from there on and in the
+    gradients up to there."""
+    s = make([300], channels, torch.float32, bias=0.0)
+    s["gate"][100, 1], s["gate"][150, 2], s["gate"][200, 3] = -torch.inf, torch.inf, torch.nan
+    got = call(s, [300])
+    y, x = got["y"], s["x"]
+    assert y[100, 1] == y[99, 1] and got["dx"][100, 1] == 0 and got["dgate"][100, 1] == 0
+    torch.testing.assert_close(y[150, 2], x[150, 2], rtol=1e-6, atol=1e-6)
+    assert got["dgate"][150, 2] == 0
+    assert y[200:, 3].isnan().all() and got["last"][0, 3].isnan()
+    assert got["dx"][:201, 3].isnan().all() and got["dinitial"][0, 3].isnan()
+    y[200:, 3] = 0
+    assert y.isfinite().all() and got["dx"][201:].isfinite().all()
+    other = [c for c in range(channels) if c != 3]
+    assert all(t[..., other].isfinite().all() for t in got.values())
+
+
+def test_step_with_infinite_gates_and_nan():
+    from gaussian_splats_b200.recurrence import gated_scan_step
+
+    x, state = torch.tensor([[1.0, 2.0, 3.0]], device="cuda"), torch.full((1, 3), 5.0, device="cuda")
+    gate = torch.tensor([[-torch.inf, torch.inf, torch.nan]], device="cuda")
+    y = gated_scan_step(x, gate, state)
+    assert y[0, 0] == 5 and y[0, 1] == 2 and y[0, 2].isnan() and state[0, 2].isnan()
+
+
 def test_gradient_against_differences():
     s = make([200, 61], 24, torch.float32, seed=2)
     got = call(s, [200, 61])
