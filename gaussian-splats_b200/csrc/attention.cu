@@ -50,9 +50,15 @@ constexpr int kMaxDim = 128;
 // and both read the same keys and values. m is the row's running maximum, but
 // moves only when it has grown by more than 2^8: until then P stays at most
 // 2^8, which both types hold with all their precision, and O need not be
-// rescaled. What bounds it: 16 exponentials a clock and multiprocessor at 64
-// channels (a 128 x 128 tile takes 1024 clocks of them, 512 of products), both
-// at 128.
+// rescaled.
+//
+// What bounds it: 16 exponentials a clock and multiprocessor at 64 channels (a
+// 128 x 128 tile takes 1024 clocks of them, 512 of products), both at 128
+// (1024 each); then the chain product, exponentials, product of a step, which
+// two groups cover only in part. Two blocks a multiprocessor at 64 channels.
+// Measured: 500,000 tokens, 4 heads of 64, 1025 keys seen: 990 us, 540 TFLOP/s,
+// the exponentials' pipe 58% and the tensor cores 45% of the time busy; 131,072
+// tokens, 8 heads of 128, 1025 keys: 862 us, 620 TFLOP/s.
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -62,13 +68,11 @@ constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
 // gs_window_attention_status, the block's results are not valid.
 __device__ uint32_t g_timeout;
 
-// 32 or 64 bits with those under `n` set.
+// 32 bits with those under `n` set.
 __device__ __forceinline__ uint32_t below32(int n) {
   return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
 }
-__device__ __forceinline__ uint64_t below(int64_t n) {
-  return n <= 0 ? 0 : n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
-}
+
 // `x` as a position that comparisons within a sequence cannot tell from it.
 __device__ __forceinline__ int position(int64_t x) {
   return static_cast<int>(max(int64_t{-1}, min(x, int64_t{INT32_MAX})));
@@ -560,17 +564,22 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // instead of the five of a kernel that adds to dQ from many blocks.
 //
 // Eight warps hold half a row a thread, a ninth loads, a tenth issues the
-// products, which are what bounds the kernels: a 128 x 128 x 16 product takes 64
-// clocks, as does one of 64 columns, because shared memory delivers the 128 rows
-// no faster (with tiles of 64 rows: 1577 and 1670 us where this takes the times
-// below). To keep the tensor cores busy, S of the next tile follows as soon as
-// this one's has been read (queries) or used (keys), while the warps work on G,
-// and G of the next while they work on S.
+// products. One of 128 x 128 x 16 takes 64 clocks, and one of 64 columns no fewer,
+// because shared memory delivers the 128 rows no faster: hence tiles of 128 rows
+// at 128 channels (with 64: 1577 and 1670 us where this takes 1240 and 1250). To
+// keep the tensor cores busy, S of the next tile follows as soon as this one's
+// has been read (queries) or used (keys), while the warps work on G, and G of the
+// next while they work on S. Sixteen warps were no faster.
+//
+// What bounds them is a tile's chain S, P, G, E, sum, of which one block's tiles
+// overlap in part. Measured: 131,072 tokens, 8 heads (4 of keys) of 128, 1025 keys
+// seen: queries 1240 us (650 TFLOP/s of products, the tensor cores busy for 36%
+// of the time), keys 1250 us (860 TFLOP/s, 52%).
 
 // First tokens are seen by all later queries, so the block of their keys would
 // walk the whole sequence. It walks its window like the others; the queries
 // further on are cut into chunks with a block each, and a last kernel adds the
-// chunks' sums in order.
+// chunks' sums in order (131,072 tokens in 8 sequences: 8 us).
 
 template <int kDim, bool kKeyRows>
 struct BackwardShape {
@@ -687,7 +696,7 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
   __syncwarp();
 }
 
-// The warp whose first lane issues the products. `sets(t)` says how many
+// The warp that issues the products (one elected lane of it). `sets(t)` says how many
 // sets of 32 rows tile t needs.
 template <class T, int kDim, bool kKeyRows, class Sets>
 __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s, int dim,
@@ -1362,7 +1371,9 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
 
 // ------------------------------------------------- one new token a stream
 //
-// The cache is read once: that is the bound. A cluster of blocks shares the
+// The cache is read once: that is the bound (96 streams of 4100 slots, 4
+// key-value heads of 128: 806 MB in 139 us, 5.8 TB/s; one stream takes 9 us, the
+// latency of a launch, a load and the join). A cluster of blocks shares the
 // slots of a stream and key-value head, up to 16 query heads (more: more
 // clusters). TMA brings tiles of 64 slots to shared memory some tiles ahead,
 // which keeps over 100 KB in flight a multiprocessor (loads straight to

@@ -17,6 +17,13 @@
 // its channels in registers and the threads' folds are joined in order in
 // shared memory. Every order is fixed, so results repeat bit for bit.
 //
+// What bounds it: memory; the fold's second reading of gate and x (of gate and
+// grad_y on the way back) is the price of a sequence split without blocks that
+// wait for one another. Walks go the other way round from folds, so that part of
+// it comes from L2. Measured at 1,000,000 tokens of 64 16-bit channels (128 MB an
+// array): fold 45 us (5.7 TB/s), walk 69 us (5.6 TB/s), back 46 and 109 us (5.9
+// TB/s), the scans of the spans' maps 10 us each.
+//
 // States, products and gates are float; the states that enter the tiles are
 // kept in float for the backward, which recomputes h from them instead of
 // reading the rounded y.
@@ -638,6 +645,8 @@ __global__ void __launch_bounds__(kScanThreads) span_scan_kernel(gs_gated_scan_a
   }
 }
 
+// One token: a state's 14 bytes (16-bit types) once. 512 x 2048 states: 6.5 us, of which
+// 2.2 us of memory; the rest is a launch's latency.
 template <class T>
 __global__ void __launch_bounds__(256) scan_step_kernel(int64_t count, int channels, const T* x,
                                                         int64_t x_stride, const T* gate,
