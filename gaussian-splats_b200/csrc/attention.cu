@@ -58,7 +58,7 @@ constexpr int kMaxDim = 128;
 // two groups cover only in part. Two blocks a multiprocessor at 64 channels.
 // Measured: 500,000 tokens, 4 heads of 64, 1025 keys seen: 990 us, 540 TFLOP/s,
 // the exponentials' pipe 58% and the tensor cores 45% of the time busy; 131,072
-// tokens, 8 heads of 128, 1025 keys: 862 us, 620 TFLOP/s.
+// tokens, 8 heads of 128, 1025 keys: 840 us, 640 TFLOP/s.
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -199,8 +199,12 @@ struct ForwardShape {
   static constexpr int kBlocks = kDim == 64 ? 2 : 1;
   static constexpr int kColumns = kDim == 64 ? 256 : 512;
   static constexpr int kGroupColumns = kKeys + kDim;  // S, then O
+  // At 128 a row of S does not fit a thread's 168 registers: the groups take 56 of
+  // each thread of a third group of warps (two of them idle), 2% faster.
+  static constexpr int kThreads = 2 * kTile + (kDim == 64 ? 64 : 128);
+  static constexpr int kLaunched = 168, kWide = 224, kNarrow = 56;
+  static_assert(2 * kWide + kNarrow <= 3 * kLaunched, "more would be waited for without end");
 };
-constexpr int kForwardThreads = 2 * kTile + 64;
 
 template <int kDim>
 struct ForwardShared {
@@ -220,7 +224,7 @@ struct ForwardShared {
 };
 
 template <class T, int kDim>
-__global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
+__global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDim>::kBlocks)
     attention_kernel(gs_window_attention_args a, const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map) {
@@ -263,6 +267,8 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
   const uint32_t tensor = s.tensor;
   bool good = true;
 
+  if constexpr (kDim == 128)
+    if (warp >= 8) registers_down<Shape::kNarrow>();
   if (warp == 8) {  // loads
     if ((threadIdx.x & 31) == 0) {
       const auto load = [&](unsigned char* dst, uint64_t* bar, const CUtensorMap* map, int h,
@@ -391,7 +397,8 @@ __global__ void __launch_bounds__(kForwardThreads, ForwardShape<kDim>::kBlocks)
     }
     if (!good && lane == 0) atomicExch(&g_timeout, 1u);
     __syncwarp();
-  } else {
+  } else if (warp < 8) {
+    if constexpr (kDim == 128) registers_up<Shape::kWide>();
     const int group = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t scores = tensor + group * Shape::kGroupColumns +
                             (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -532,7 +539,8 @@ int64_t sequences_of(const gs_window_attention_args& a) { return a.tile_starts ?
 
 template <class T, int kDim>
 int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
-  constexpr int kKeys = ForwardShape<kDim>::kKeys;
+  using Shape = ForwardShape<kDim>;
+  constexpr int kKeys = Shape::kKeys;
   CUtensorMap q, k, v;
   GS_TRY(tc::encode_heads(&q, a.dtype, a.q, a.tokens, a.heads, a.dim, a.q_stride, a.q_head_stride,
                           kTile));
@@ -541,11 +549,12 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
   GS_TRY(tc::encode_heads(&v, a.dtype, a.v, a.tokens, a.kv_heads, a.dim, a.v_stride,
                           a.v_head_stride, kKeys));
   constexpr size_t kShared = sizeof(ForwardShared<kDim>);
-  GS_TRY((allow_shared<attention_kernel<T, kDim>>(kShared)));
+  GS_TRY((allow_shared<attention_kernel<T, kDim>>(kShared, false,
+                                                  kDim == 64 ? 0 : Shape::kLaunched)));
   const int64_t blocks = (a.num_tiles / 2 + sequences_of(a)) * a.heads;
   if (blocks > INT32_MAX) return GS_ERR_CAPACITY;
-  launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(blocks), kForwardThreads,
-                        kShared, stream, a, q, k, v);
+  launch_chained_shared(attention_kernel<T, kDim>, static_cast<unsigned>(blocks),
+                        Shape::kThreads, kShared, stream, a, q, k, v);
   return check_launch();
 }
 

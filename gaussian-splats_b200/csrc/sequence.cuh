@@ -75,8 +75,10 @@ inline int32_t with_dtype(int32_t dtype, F&& f) {
 
 // Lets a kernel have `bytes` of dynamic shared memory (and clusters of 16 blocks),
 // once a device: the attribute calls cost as much as a launch's other host work.
+// `registers`: refuses a build that launches with fewer a thread, for a kernel whose
+// warps share them out.
 template <auto kKernel>
-inline int32_t allow_shared(size_t bytes, bool wide_clusters = false) {
+inline int32_t allow_shared(size_t bytes, bool wide_clusters = false, int registers = 0) {
   static std::atomic<uint64_t> done{0};
   int device;
   GS_CUDA_TRY(cudaGetDevice(&device));
@@ -84,6 +86,11 @@ inline int32_t allow_shared(size_t bytes, bool wide_clusters = false) {
   if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return GS_OK;
   GS_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(bytes)));
+  if (registers) {
+    cudaFuncAttributes attributes;
+    GS_CUDA_TRY(cudaFuncGetAttributes(&attributes, reinterpret_cast<const void*>(kKernel)));
+    if (attributes.numRegs < registers) return GS_ERR_UNSUPPORTED;
+  }
   if (wide_clusters)
     GS_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   done.fetch_or(bit, std::memory_order_relaxed);

@@ -231,6 +231,16 @@ __device__ __forceinline__ void commit(uint32_t elected, uint32_t bar) {
 
 // ---------------------------------------------------------------- arithmetic
 
+// A group of four warps gives registers back or takes them, to kCount a thread; who
+// takes waits for those that the block was launched with to become free.
+template <int kCount>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCount));
+}
+template <int kCount>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kCount));
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
