@@ -108,14 +108,6 @@ __device__ __forceinline__ uint32_t window_bits(const gs_window_attention_args& 
   return below32(high - start) & (~below32(low - start) | below32(a.first - start));
 }
 
-// The valid keys among the 32 from row `row` on (bits from `rows` on are 0);
-// every lane of the warp gets them.
-__device__ __forceinline__ uint32_t valid_bits(const uint8_t* valid, int64_t row, int rows) {
-  if (!valid) return below32(rows);
-  const int lane = threadIdx.x & 31;
-  return __ballot_sync(0xffffffffu, lane < rows && __ldg(valid + row + lane));
-}
-
 // Zeroes the rows of a loaded tile (kRows rows, kDim channels) whose bit is not
 // set, so that what they hold (another sequence's rows, NaN of invalid keys)
 // cannot reach a sum through a weight of zero.
@@ -136,6 +128,29 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const uint32_t (&
     for (int w = 0; w < kWordsEach; ++w)
       *reinterpret_cast<uint4*>(tile + box * (kRows * 128) + row * 128 +
                                 ((tid % kPerRow) * kWordsEach + w) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// A block's results go through shared memory, where a thread puts its row's words
+// and from where rows are written side by side: sixteen bytes a row and
+// instruction, half a sector each, kept the memory system busy for 8000 clocks of
+// the next block's time.
+template <class T, int kDim>
+__device__ __forceinline__ void put_word(unsigned char* rows, int row, int word,
+                                         const float (&v)[8]) {
+  store_pack<8>(reinterpret_cast<T*>(rows + row * (2 * kDim) + (word ^ (row & 7)) * 16), v);
+}
+// Rows `from` to `to` of the tile; row 0 of the array is at `out`.
+template <class T, int kDim, int kThreadCount>
+__device__ __forceinline__ void write_rows(const unsigned char* rows, T* out, int64_t stride,
+                                           int from, int to, int dim, int thread) {
+  constexpr int kLanes = kDim / 8;
+  const int word = thread % kLanes;
+  if (8 * word >= dim) return;
+#pragma unroll
+  for (int row = thread / kLanes; row < kTile; row += kThreadCount / kLanes)
+    if (row >= from && row < to)
+      *reinterpret_cast<uint4*>(out + row * stride + 8 * word) =
+          *reinterpret_cast<const uint4*>(rows + row * (2 * kDim) + (word ^ (row & 7)) * 16);
 }
 
 // The tiles of keys that a run of kGroups tiles of queries walks over, as
@@ -421,11 +436,18 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
       if (a.valid || !whole) {
         all = true;
 #pragma unroll
-        for (int c = 0; c < kSets; ++c) {
-          keep[c] = valid_bits(a.valid, int64_t{tile.begin} + start + 32 * c,
-                               max(0, min(end - start - 32 * c, 32)));
-          all = all && keep[c] == ~0u;
+        for (int c = 0; c < kSets; ++c) keep[c] = below32(end - start - 32 * c);
+        if (a.valid) {
+          const uint8_t* at = a.valid + tile.begin;
+          uint8_t valid[kSets];  // all on their way at once
+#pragma unroll
+          for (int c = 0; c < kSets; ++c)
+            valid[c] = __ldg(at + min(start + static_cast<int>(threadIdx.x & 31) + 32 * c, end - 1));
+#pragma unroll
+          for (int c = 0; c < kSets; ++c) keep[c] &= __ballot_sync(0xffffffffu, valid[c] != 0);
         }
+#pragma unroll
+        for (int c = 0; c < kSets; ++c) all = all && keep[c] == ~0u;
         whole = whole && all;
       }
       good = good && barrier_wait_warp(shared_address(&s.scores[group]), step & 1);
@@ -510,7 +532,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
       const int64_t token = int64_t{tile.start} + group * kTile + row;
       const bool write = token < tile.end;
       const float inverse = good ? 1.0f / sum : NAN;  // a wait that ran out shows
-      T* out = static_cast<T*>(a.out) + (token * a.heads + head) * a.dim;
+      unsigned char* rows = s.q[group];  // the products with the queries are complete
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
         float o[32];
@@ -518,13 +540,17 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         wait_loads();
 #pragma unroll
         for (int e = 0; e < 32; e += 8)
-          if (write && c + e < a.dim) {
+          if (c + e < a.dim) {
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = sum == 0.0f ? 0.0f : o[e + k] * inverse;
-            store_pack<8>(out + c + e, v);
+            put_word<T, kDim>(rows, row, (c + e) / 8, v);
           }
       }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kTile) : "memory");
+      write_rows<T, kDim, kTile>(
+          rows, static_cast<T*>(a.out) + ((token - row) * a.heads + head) * a.dim,
+          int64_t{a.heads} * a.dim, 0, static_cast<int>(tile.end - (token - row)), a.dim, row);
       if (write && a.lse)
         a.lse[head * a.tokens + token] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
       if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
@@ -616,7 +642,7 @@ struct BackwardShared {
   unsigned char tiles1[kStages1][Shape::kTileBytes];
   union {
     float row[kStages1][2][Shape::kRows];  // keys: -L and -D of a tile's queries
-    float part[2][kTile];                  // queries: halves of D
+    float part[kTile];                     // queries: D
   };
   uint64_t rows_full, full0[kStages0], full1[kStages1];  // loads
   uint64_t empty[kStages0];                              // a tile's sums are complete
@@ -640,7 +666,7 @@ __device__ __forceinline__ constexpr uint32_t weight_column(int k) {
 }
 
 // The warp that loads. `place(t)` names the head and row of tile t; `rows(t,
-// lane)` loads what else a tile needs and `keep(stage, ...)` puts it to shared
+// lane)` loads what else a tile needs and `keep(t, stage, ...)` puts it to shared
 // memory, all lanes taking part; it goes with operand 1.
 template <int kDim, bool kKeyRows, class Place, class Rows, class Keep>
 __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, int tiles,
@@ -675,6 +701,10 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
   };
   auto ahead = rows(0, lane);
   for (int t = 0; t < tiles; ++t) {
+    // What the first tile needs comes first: the others' boxes would hold it up.
+    if (t == 1)
+      good = barrier_wait_warp(shared_address(&s.rows_full), 0) &&
+             barrier_wait_warp(shared_address(&s.full1[0]), 0);
     const auto values = ahead;
     if (t + 1 < tiles) ahead = rows(t + 1, lane);
     const int stage0 = t % kStages0, stage1 = t % kStages1;
@@ -690,7 +720,7 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
       good = good && barrier_wait_warp(shared_address(&s.grads[u & 1]), (u >> 1) & 1);
     }
     if (!good) break;
-    keep(stage1, lane, values);
+    keep(t, stage1, lane, values);
     if (lane == 0) load(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
     else barrier_arrive(shared_address(&s.full1[stage1]));
     __syncwarp();
@@ -849,6 +879,45 @@ __device__ __forceinline__ void sync_compute() {
   asm volatile("bar.sync 1, %0;" ::"n"(kComputeThreads) : "memory");
 }
 
+// D, the sums of gradient times output, of the tile's queries, by the compute warps:
+// kDim / 8 lanes read a row of the outputs side by side; the gradients are in shared
+// memory. False: they did not come.
+template <class T, int kDim>
+__device__ __forceinline__ bool row_products(const gs_window_attention_args& a, const Tile& tile,
+                                             int head, BackwardShared<kDim, false>& s) {
+  constexpr int kLanes = kDim / 8, kRows = 32 / kLanes;  // of a warp's step
+  constexpr int kSteps = kTile / (kComputeThreads / 32) / kRows;
+  const int lane = threadIdx.x & 31, word = lane % kLanes;
+  const int first = (threadIdx.x >> 5) * kSteps * kRows + lane / kLanes;
+  // Every lane loads, from a row and word that exist: loads that are branched around
+  // came one after the other (22,000 clocks).
+  const bool used = 8 * word < a.dim;
+  const T* out = static_cast<const T*>(a.out) + (used ? 8 * word : 0);
+  uint4 o[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int64_t token = min(tile.start + first + k * kRows, tile.end - 1);
+    o[k] = *reinterpret_cast<const uint4*>(out + (token * a.heads + head) * a.dim);
+  }
+  if (!tc::barrier_wait_warp(tc::shared_address(&s.rows_full), 0)) return false;
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int row = first + k * kRows;
+    float g[8], d = 0.0f;
+    load_pack<8>(reinterpret_cast<const T*>(s.rows[1] + word / 8 * (kTile * 128) + row * 128 +
+                                            ((word ^ row) & 7) * 16),
+                 g);
+    const Pack<T, 8>& values = reinterpret_cast<const Pack<T, 8>&>(o[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d = fmaf(g[e], to_float(values.v[e]), d);
+    if (!used) d = 0.0f;
+#pragma unroll
+    for (int x = kLanes / 2; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+    if (word == 0) s.part[row] = d;
+  }
+  return true;
+}
+
 // log2 of a row's sum of exponentials, and where there is none (a row that sees
 // nothing, a row past the end) what makes its weights 0.
 __device__ __forceinline__ float weight_shift(float lse) {
@@ -881,7 +950,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     load_tiles<kDim, false>(
         s, walk.tiles, &q_map, &g_map, head, tile.start, &k_map, &v_map,
         [&](int t) { return make_int2(kv_head, tile.begin + walk.start(t)); },
-        [](int, int) { return 0; }, [](int, int, int) {});
+        [](int, int) { return 0; }, [](int, int, int, int) {});
   } else if (warp == kProductWarp) {
     issue_products<T, kDim, false>(s, a.dim, walk.tiles,
                                    [&](int t) { return walk.sets(0, t); });
@@ -890,22 +959,12 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int i_first = walk.i, i = i_first + row;
     const bool live = tile.start + row < tile.end;
-    const int64_t at = (int64_t{tile.start + row} * a.heads + head) * a.dim;
-    float d = 0.0f;
-    if (live)
-      for (int c = 8 * half; c < a.dim; c += 16) {
-        float g[8], o[8];
-        load_pack<8>(static_cast<const T*>(a.grad_out) + at + c, g);
-        load_pack<8>(static_cast<const T*>(a.out) + at + c, o);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) d = fmaf(g[k], o[k], d);
-      }
-    s.part[half][row] = d;
-    sync_compute();
-    d = s.part[0][row] + s.part[1][row];
     const int64_t slot = head * a.tokens + tile.start + row;
-    if (live && half == 0) delta[slot] = d;
     const float shift = live ? weight_shift(a.lse[slot]) : INFINITY;
+    bool good = row_products<T, kDim>(a, tile, head, s);
+    sync_compute();
+    const float d = live ? s.part[row] : 0.0f;
+    if (live && half == 0) delta[slot] = d;
     const float scale = a.scale * kLog2e;
     // Every query sees every valid key of a tile that lies from `from` (or under
     // `first`) to `to`.
@@ -915,7 +974,6 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     const float2 grow = make_float2(weights.e, weights.e);
     const float2 less = make_float2(-d * weights.e, -d * weights.e);
     const uint32_t scores = mine + 32 * kHalfSets * half;
-    bool good = true;
     // Whether the lane's keys of tile t are valid, a tile ahead.
     bool valid[kSets];
     const auto load_valid = [&](int t) {
@@ -923,10 +981,11 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
       const int start = walk.start(t) + (threadIdx.x & 31), end = walk.end(t);
 #pragma unroll
       for (int c = 0; c < kSets; ++c)
-        valid[c] = start + 32 * c < end && __ldg(a.valid + tile.begin + start + 32 * c);
+        valid[c] = __ldg(a.valid + tile.begin + min(start + 32 * c, end - 1)) &&
+                   start + 32 * c < end;
     };
     load_valid(0);
-    for (int t = 0; t < walk.tiles; ++t) {
+    for (int t = 0; t < walk.tiles && good; ++t) {
       const int start = walk.start(t), end = walk.end(t);
       // What no query sees has no products either.
       const int sets = walk.sets(0, t) - kHalfSets * half;
@@ -1005,7 +1064,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     }
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
-    T* grad_q = static_cast<T*>(a.grad_q) + at;
+    unsigned char* rows = s.rows[0];  // the products with the queries are complete
 #pragma unroll
     for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 16) {
       float o[16];
@@ -1013,13 +1072,17 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
       wait_loads();
 #pragma unroll
       for (int e = 0; e < 16; e += 8)
-        if (live && c + e < a.dim) {
+        if (c + e < a.dim) {
           float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * weights.dk : NAN;
-          store_pack<8>(grad_q + c + e, v);
+          put_word<T, kDim>(rows, row, (c + e) / 8, v);
         }
     }
+    sync_compute();
+    write_rows<T, kDim, kComputeThreads>(
+        rows, static_cast<T*>(a.grad_q) + (int64_t{tile.start} * a.heads + head) * a.dim,
+        int64_t{a.heads} * a.dim, 0, tile.end - tile.start, a.dim, threadIdx.x);
     if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
   }
   fence_before_sync();
@@ -1097,20 +1160,24 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         [&](int t, int lane) {
           RowValues v;
           const int i = low + (t % per_head) * kRows + lane;
-          const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin + i;
+          const int64_t at = (kv_head * group + t / per_head) * a.tokens + tile.begin;
+          // Loads from rows that exist, all on their way at once.
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
-            const bool in = i + 32 * k < n;
-            v.shift[k] = in ? weights.p - weight_shift(a.lse[at + 32 * k]) : -INFINITY;
-            v.delta[k] = in ? -delta[at + 32 * k] * weights.e_p : 0.0f;
+            const int64_t where = at + min(i + 32 * k, n - 1);
+            v.shift[k] = a.lse[where];
+            v.delta[k] = delta[where];
           }
           return v;
         },
-        [&](int stage, int lane, const RowValues& v) {
+        [&](int t, int stage, int lane, const RowValues& v) {
+          const int i = low + (t % per_head) * kRows + lane;
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
-            s.row[stage][0][lane + 32 * k] = v.shift[k];
-            s.row[stage][1][lane + 32 * k] = v.delta[k];
+            const bool in = i + 32 * k < n;
+            s.row[stage][0][lane + 32 * k] =
+                in ? weights.p - weight_shift(v.shift[k]) : -INFINITY;
+            s.row[stage][1][lane + 32 * k] = in ? -v.delta[k] * weights.e_p : 0.0f;
           }
         });
   } else if (warp == kProductWarp) {
@@ -1248,11 +1315,10 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
     // First tokens that later queries see too: floats for the sum of the chunks.
-    const bool split = j < a.first && beyond_window(a, n);
+    const int summed = beyond_window(a, n) ? a.first : 0;
     const int64_t where = chunk ? item : tile.sequence;
     float* sum = (chunk ? sums.part : sums.base) +
                  ((where * a.kv_heads + kv_head) * a.first + j) * 2 * a.dim;
-    const int64_t at = (int64_t{tile.start + row} * a.kv_heads + kv_head) * a.dim;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -1261,17 +1327,25 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         load_columns16(mine + Shape::kSum + which * kDim + c, o);
         wait_loads();
         const float factor = which ? weights.dv : weights.dk;
-        T* out = static_cast<T*>(which ? a.grad_v : a.grad_k) + at;
 #pragma unroll
         for (int e = 0; e < 16; e += 8)
           if (live && c + e < a.dim) {
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * factor : NAN;
-            if (split) store_pack<8>(sum + which * a.dim + c + e, v);
-            else store_pack<8>(out + c + e, v);
+            if (j < summed) store_pack<8>(sum + which * a.dim + c + e, v);
+            else put_word<T, kDim>(s.rows[which], row, (c + e) / 8, v);
           }
       }
+    if (!chunk) {
+      sync_compute();
+      for (int which = 0; which < 2; ++which)
+        write_rows<T, kDim, kComputeThreads>(
+            s.rows[which],
+            static_cast<T*>(which ? a.grad_v : a.grad_k) +
+                (int64_t{tile.start} * a.kv_heads + kv_head) * a.dim,
+            int64_t{a.kv_heads} * a.dim, summed - j_first, n - j_first, a.dim, threadIdx.x);
+    }
     if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
   }
   fence_before_sync();
