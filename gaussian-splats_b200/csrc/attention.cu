@@ -146,11 +146,21 @@ __device__ __forceinline__ void write_rows(const unsigned char* rows, T* out, in
   constexpr int kLanes = kDim / 8;
   const int word = thread % kLanes;
   if (8 * word >= dim) return;
+  constexpr int kStep = kThreadCount / kLanes, kAtOnce = kTile / kStep < 8 ? kTile / kStep : 8;
 #pragma unroll
-  for (int row = thread / kLanes; row < kTile; row += kThreadCount / kLanes)
-    if (row >= from && row < to)
-      *reinterpret_cast<uint4*>(out + row * stride + 8 * word) =
-          *reinterpret_cast<const uint4*>(rows + row * (2 * kDim) + (word ^ (row & 7)) * 16);
+  for (int base = 0; base < kTile; base += kAtOnce * kStep) {
+    uint4 x[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int row = base + k * kStep + thread / kLanes;
+      x[k] = *reinterpret_cast<const uint4*>(rows + row * (2 * kDim) + (word ^ (row & 7)) * 16);
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int row = base + k * kStep + thread / kLanes;
+      if (row >= from && row < to) *reinterpret_cast<uint4*>(out + row * stride + 8 * word) = x[k];
+    }
+  }
 }
 
 // The tiles of keys that a run of kGroups tiles of queries walks over, as
@@ -259,7 +269,13 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
   if (index >= first_tile_of(a, sequence + 1)) return;
   const Tile tile = tile_at(a.tiles, index, static_cast<int32_t>(a.tokens), kTile);
   const KeyWalk<kKeys, 2> walk(a, tile);
-  if (threadIdx.x == 0) {
+  const auto load = [&](unsigned char* dst, uint64_t* bar, const CUtensorMap* map, int h, int row,
+                        int rows) {
+    const uint32_t b = shared_address(bar), d = shared_address(dst);
+    barrier_expect(b, rows * kDim * 2);
+    for (int x = 0; x < kDim / 64; ++x) load_box(d + x * rows * 128, map, 64 * x, h, row, b);
+  };
+  if (threadIdx.x == 8 * 32) {
     for (int g = 0; g < 2; ++g) {
       barrier_init(shared_address(&s.q_full[g]), 1);
       barrier_init(shared_address(&s.scores[g]), 1);
@@ -274,6 +290,12 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
+    // The first loads do not wait for the others to be ready.
+    load(s.q[0], &s.q_full[0], &q_map, head, tile.start, kTile);
+    load(s.k[0], &s.k_full[0], &k_map, kv_head, tile.begin + walk.start(0), kKeys);
+    if (walk.steps(1) > 0)
+      load(s.q[1], &s.q_full[1], &q_map, head, tile.start + kTile, kTile);
+    load(s.v[0], &s.v_full[0], &v_map, kv_head, tile.begin + walk.start(0), kKeys);
   }
   if (warp == 9) tensor_alloc<Shape::kColumns>(shared_address(&s.tensor));
   fence_before_sync();
@@ -286,20 +308,11 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
     if (warp >= 8) registers_down<Shape::kNarrow>();
   if (warp == 8) {  // loads
     if ((threadIdx.x & 31) == 0) {
-      const auto load = [&](unsigned char* dst, uint64_t* bar, const CUtensorMap* map, int h,
-                            int row, int rows) {
-        const uint32_t b = shared_address(bar), d = shared_address(dst);
-        barrier_expect(b, rows * kDim * 2);
-        for (int x = 0; x < kDim / 64; ++x) load_box(d + x * rows * 128, map, 64 * x, h, row, b);
-      };
-      load(s.q[0], &s.q_full[0], &q_map, head, tile.start, kTile);
-      for (int t = 0; t < walk.tiles && good; ++t) {
+      for (int t = 1; t < walk.tiles && good; ++t) {
         const int stage = t % kStages, turn = t / kStages;
         if (turn > 0) good = barrier_wait(shared_address(&s.k_empty[stage]), (turn - 1) & 1);
         if (!good) break;
         load(s.k[stage], &s.k_full[stage], &k_map, kv_head, tile.begin + walk.start(t), kKeys);
-        if (t == 0 && walk.steps(1) > 0)
-          load(s.q[1], &s.q_full[1], &q_map, head, tile.start + kTile, kTile);
         if (turn > 0) good = barrier_wait(shared_address(&s.v_empty[stage]), (turn - 1) & 1);
         if (!good) break;
         load(s.v[stage], &s.v_full[stage], &v_map, kv_head, tile.begin + walk.start(t), kKeys);
@@ -539,13 +552,12 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         load_columns32(sums + c, o);
         wait_loads();
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-          if (c + e < a.dim) {
-            float v[8];
+        for (int e = 0; e < 32; e += 8) {
+          float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = sum == 0.0f ? 0.0f : o[e + k] * inverse;
-            put_word<T, kDim>(rows, row, (c + e) / 8, v);
-          }
+          for (int k = 0; k < 8; ++k) v[k] = sum == 0.0f ? 0.0f : o[e + k] * inverse;
+          put_word<T, kDim>(rows, row, (c + e) / 8, v);
+        }
       }
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kTile) : "memory");
       write_rows<T, kDim, kTile>(
@@ -665,13 +677,22 @@ __device__ __forceinline__ constexpr uint32_t weight_column(int k) {
   return (k >> 1) * 32 + (k & 1) * 8;
 }
 
-// The warp that loads. `place(t)` names the head and row of tile t; `rows(t,
-// lane)` loads what else a tile needs and `keep(t, stage, ...)` puts it to shared
-// memory, all lanes taking part; it goes with operand 1.
+// A tile of an operand, by one thread.
+template <int kDim, bool kKeyRows>
+__device__ __forceinline__ void load_tile(unsigned char* dst, uint64_t* full,
+                                          const CUtensorMap* map, int2 at) {
+  using Shape = BackwardShape<kDim, kKeyRows>;
+  const uint32_t bar = tc::shared_address(full);
+  tc::barrier_expect(bar, Shape::kTileBytes);
+  for (int x = 0; x < kDim / 64; ++x)
+    tc::load_box(tc::shared_address(dst) + x * Shape::kRows * 128, map, 64 * x, at.x, at.y, bar);
+}
+
+// The warp that loads what backward_setup has not. `place(t)` names the head and row of tile
+// t; `rows(t, lane)` loads what else a tile needs and `keep(t, stage, ...)` puts it
+// to shared memory, all lanes taking part; it goes with operand 1.
 template <int kDim, bool kKeyRows, class Place, class Rows, class Keep>
 __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, int tiles,
-                                           const CUtensorMap* row_map0,
-                                           const CUtensorMap* row_map1, int row_head, int row,
                                            const CUtensorMap* tile_map0,
                                            const CUtensorMap* tile_map1, const Place& place,
                                            const Rows& rows, const Keep& keep) {
@@ -680,20 +701,6 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
   constexpr int kStages0 = Shape::kStages0, kStages1 = Shape::kStages1;
   const int lane = threadIdx.x & 31;
   bool good = true;
-  if (lane == 0) {
-    const uint32_t bar = shared_address(&s.rows_full);
-    barrier_expect(bar, 2 * Shape::kBytes);
-    for (int x = 0; x < kDim / 64; ++x) {
-      load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row, bar);
-      load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row, bar);
-    }
-  }
-  const auto load = [&](unsigned char* dst, uint64_t* full, const CUtensorMap* map, int2 at) {
-    const uint32_t bar = shared_address(full);
-    barrier_expect(bar, Shape::kTileBytes);
-    for (int x = 0; x < kDim / 64; ++x)
-      load_box(shared_address(dst) + x * Shape::kRows * 128, map, 64 * x, at.x, at.y, bar);
-  };
   // The tile that had the place before has been summed up.
   const auto wait_for = [&](int t) {
     if (t >= 0)
@@ -711,7 +718,8 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
     wait_for(t - kStages0);
     if (!good) break;
     const int2 at = place(t);
-    if (lane == 0) load(s.tiles0[stage0], &s.full0[stage0], tile_map0, at);
+    if (lane == 0 && t > 0)
+      load_tile<kDim, kKeyRows>(s.tiles0[stage0], &s.full0[stage0], tile_map0, at);
     __syncwarp();
     if constexpr (kKeyRows) {
       wait_for(t - kStages1);
@@ -721,8 +729,11 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
     }
     if (!good) break;
     keep(t, stage1, lane, values);
-    if (lane == 0) load(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
-    else barrier_arrive(shared_address(&s.full1[stage1]));
+    __syncwarp();  // lane 0 has arrived at the first tile's barrier already
+    if (lane > 0)
+      barrier_arrive(shared_address(&s.full1[stage1]));
+    else if (t > 0)
+      load_tile<kDim, kKeyRows>(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
     __syncwarp();
   }
   if (!good) {  // let what is in flight land before the shared memory is given back
@@ -831,11 +842,17 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
   __syncwarp();
 }
 
+// Barriers and tensor memory; the block's rows and the first tile are on their way
+// before the other warps are ready.
 template <int kDim, bool kKeyRows>
-__device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s, int warp) {
+__device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s, int warp,
+                                               const CUtensorMap* row_map0,
+                                               const CUtensorMap* row_map1, int row_head, int row,
+                                               const CUtensorMap* tile_map0,
+                                               const CUtensorMap* tile_map1, int2 first) {
   using namespace tc;
   using Shape = BackwardShape<kDim, kKeyRows>;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 32 * kLoadWarp) {
     barrier_init(shared_address(&s.rows_full), 1);
     for (uint64_t& b : s.full0) barrier_init(shared_address(&b), 1);
     for (uint64_t& b : s.full1) barrier_init(shared_address(&b), 32);
@@ -847,6 +864,14 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
     barrier_init(shared_address(&s.done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
+    const uint32_t bar = shared_address(&s.rows_full);
+    barrier_expect(bar, 2 * Shape::kBytes);
+    for (int x = 0; x < kDim / 64; ++x)
+      load_box(shared_address(s.rows[0]) + x * kTile * 128, row_map0, 64 * x, row_head, row, bar);
+    load_tile<kDim, kKeyRows>(s.tiles0[0], &s.full0[0], tile_map0, first);
+    for (int x = 0; x < kDim / 64; ++x)
+      load_box(shared_address(s.rows[1]) + x * kTile * 128, row_map1, 64 * x, row_head, row, bar);
+    load_tile<kDim, kKeyRows>(s.tiles1[0], &s.full1[0], tile_map1, first);
   }
   if (warp == kProductWarp) tensor_alloc<Shape::kColumns>(shared_address(&s.tensor));
   fence_before_sync();
@@ -944,11 +969,12 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
       tile_at(a.tiles, blockIdx.x / a.heads, static_cast<int32_t>(a.tokens), kTile);
   constexpr int kKeys = Shape::kRows, kSets = Shape::kSets, kHalfSets = kSets / 2;
   const KeyWalk<kKeys, 1> walk(a, tile);
-  backward_setup(s, warp);
+  backward_setup(s, warp, &q_map, &g_map, head, tile.start, &k_map, &v_map,
+                 make_int2(kv_head, tile.begin + walk.start(0)));
   const uint32_t tensor = s.tensor;
   if (warp == kLoadWarp) {
     load_tiles<kDim, false>(
-        s, walk.tiles, &q_map, &g_map, head, tile.start, &k_map, &v_map,
+        s, walk.tiles, &k_map, &v_map,
         [&](int t) { return make_int2(kv_head, tile.begin + walk.start(t)); },
         [](int, int) { return 0; }, [](int, int, int, int) {});
   } else if (warp == kProductWarp) {
@@ -1065,19 +1091,18 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     if (good) good = barrier_wait_warp(shared_address(&s.done), 0);
     fence_after_sync();
     unsigned char* rows = s.rows[0];  // the products with the queries are complete
+    float o[kDim / 2];
 #pragma unroll
-    for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 16) {
-      float o[16];
-      load_columns16(mine + Shape::kSum + c, o);
-      wait_loads();
+    for (int c = 0; c < kDim / 2; c += 32)
+      load_columns32(mine + Shape::kSum + half * (kDim / 2) + c,
+                     reinterpret_cast<float(&)[32]>(o[c]));
+    wait_loads();
 #pragma unroll
-      for (int e = 0; e < 16; e += 8)
-        if (c + e < a.dim) {
-          float v[8];
+    for (int e = 0; e < kDim / 2; e += 8) {
+      float v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * weights.dk : NAN;
-          put_word<T, kDim>(rows, row, (c + e) / 8, v);
-        }
+      for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * weights.dk : NAN;
+      put_word<T, kDim>(rows, row, (half * (kDim / 2) + e) / 8, v);
     }
     sync_compute();
     write_rows<T, kDim, kComputeThreads>(
@@ -1144,7 +1169,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
   const int n = tile.end - tile.begin;
   const int per_head = (high - low + kRows - 1) / kRows;
   const int tiles = per_head * group;
-  backward_setup(s, warp);
+  backward_setup(s, warp, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
+                 make_int2(kv_head * group, tile.begin + low));
   const uint32_t tensor = s.tensor;
   if (warp == kLoadWarp) {
     // L and D of a tile's queries come along, negated.
@@ -1152,7 +1178,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
       float shift[kSets], delta[kSets];
     };
     load_tiles<kDim, true>(
-        s, tiles, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
+        s, tiles, &q_map, &g_map,
         [&](int t) {
           return make_int2(kv_head * group + t / per_head,
                            tile.begin + low + (t % per_head) * kRows);
@@ -1320,23 +1346,24 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     float* sum = (chunk ? sums.part : sums.base) +
                  ((where * a.kv_heads + kv_head) * a.first + j) * 2 * a.dim;
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
+    for (int which = 0; which < 2; ++which) {
+      float o[kDim / 2];
 #pragma unroll
-      for (int c = half * (kDim / 2); c < (half + 1) * (kDim / 2); c += 16) {
-        float o[16];
-        load_columns16(mine + Shape::kSum + which * kDim + c, o);
-        wait_loads();
-        const float factor = which ? weights.dv : weights.dk;
+      for (int c = 0; c < kDim / 2; c += 32)
+        load_columns32(mine + Shape::kSum + which * kDim + half * (kDim / 2) + c,
+                       reinterpret_cast<float(&)[32]>(o[c]));
+      wait_loads();
+      const float factor = which ? weights.dv : weights.dk;
 #pragma unroll
-        for (int e = 0; e < 16; e += 8)
-          if (live && c + e < a.dim) {
-            float v[8];
+      for (int e = 0; e < kDim / 2; e += 8) {
+        const int c = half * (kDim / 2) + e;
+        float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * factor : NAN;
-            if (j < summed) store_pack<8>(sum + which * a.dim + c + e, v);
-            else put_word<T, kDim>(s.rows[which], row, (c + e) / 8, v);
-          }
+        for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * factor : NAN;
+        put_word<T, kDim>(s.rows[which], row, c / 8, v);
+        if (live && j < summed && c < a.dim) store_pack<8>(sum + which * a.dim + c, v);
       }
+    }
     if (!chunk) {
       sync_compute();
       for (int which = 0; which < 2; ++which)
