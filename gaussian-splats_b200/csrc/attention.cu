@@ -58,7 +58,8 @@ constexpr int kMaxDim = 128;
 // two groups cover only in part. Two blocks a multiprocessor at 64 channels.
 // Measured: 500,000 tokens, 4 heads of 64, 1025 keys seen: 990 us, 540 TFLOP/s,
 // the exponentials' pipe 58% and the tensor cores 45% of the time busy; 131,072
-// tokens, 8 heads of 128, 1025 keys: 840 us, 640 TFLOP/s.
+// tokens, 8 heads of 128, 1025 keys: 812 us, 660 TFLOP/s. A block of nine tiles
+// spends a sixth of its time before the first exponential and after the last.
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -131,9 +132,8 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const uint32_t (&
 }
 
 // A block's results go through shared memory, where a thread puts its row's words
-// and from where rows are written side by side: sixteen bytes a row and
-// instruction, half a sector each, kept the memory system busy for 8000 clocks of
-// the next block's time.
+// and from where rows are written side by side (2 to 4% of the kernels' time, next
+// to sixteen bytes, half a sector, a row and instruction).
 template <class T, int kDim>
 __device__ __forceinline__ void put_word(unsigned char* rows, int row, int word,
                                          const float (&v)[8]) {
@@ -613,15 +613,14 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // Eight warps hold half a row a thread, a ninth loads, a tenth issues the
 // products. One of 128 x 128 x 16 takes 64 clocks, and one of 64 columns no fewer,
 // because shared memory delivers the 128 rows no faster: hence tiles of 128 rows
-// at 128 channels (with 64: 1577 and 1670 us where this takes 1240 and 1250). To
-// keep the tensor cores busy, S of the next tile follows as soon as this one's
+// at 128 channels (64 took 8% longer). To keep the tensor cores busy, S of the next tile follows as soon as this one's
 // has been read (queries) or used (keys), while the warps work on G, and G of the
 // next while they work on S. Sixteen warps were no faster.
 //
 // What bounds them is a tile's chain S, P, G, E, sum, of which one block's tiles
 // overlap in part. Measured: 131,072 tokens, 8 heads (4 of keys) of 128, 1025 keys
-// seen: queries 1240 us (650 TFLOP/s of products, the tensor cores busy for 36%
-// of the time), keys 1250 us (860 TFLOP/s, 52%).
+// seen: queries 1066 us (760 TFLOP/s of products, the tensor cores busy for 43%
+// of the time), keys 1205 us (890 TFLOP/s, 55%).
 
 // First tokens are seen by all later queries, so the block of their keys would
 // walk the whole sequence. It walks its window like the others; the queries
@@ -915,7 +914,7 @@ __device__ __forceinline__ bool row_products(const gs_window_attention_args& a, 
   const int lane = threadIdx.x & 31, word = lane % kLanes;
   const int first = (threadIdx.x >> 5) * kSteps * kRows + lane / kLanes;
   // Every lane loads, from a row and word that exist: loads that are branched around
-  // came one after the other (22,000 clocks).
+  // came one after the other (22,000 clocks until D was known, 8000 now).
   const bool used = 8 * word < a.dim;
   const T* out = static_cast<const T*>(a.out) + (used ? 8 * word : 0);
   uint4 o[kSteps];
