@@ -613,9 +613,10 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // Eight warps hold half a row a thread, a ninth loads, a tenth issues the
 // products. One of 128 x 128 x 16 takes 64 clocks, and one of 64 columns no fewer,
 // because shared memory delivers the 128 rows no faster: hence tiles of 128 rows
-// at 128 channels (64 took 8% longer). To keep the tensor cores busy, S of the next tile follows as soon as this one's
-// has been read (queries) or used (keys), while the warps work on G, and G of the
-// next while they work on S. Sixteen warps were no faster.
+// at 128 channels (64 took 8% longer). To keep the tensor cores busy, S of the next
+// tile follows as soon as this one's has been read (queries) or used (keys), while
+// the warps work on G, and G of the next while they work on S. Sixteen warps were
+// no faster.
 //
 // What bounds them is a tile's chain S, P, G, E, sum, of which one block's tiles
 // overlap in part. Measured: 131,072 tokens, 8 heads (4 of keys) of 128, 1025 keys

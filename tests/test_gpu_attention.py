@@ -311,3 +311,44 @@ def test_no_tokens():
     q, k, v, grad, _ = make([0], 2, 1, 64, torch.bfloat16)
     assert call(q, k, v, grad, [0], left=3)["out"].shape == (0, 2, 64)
     assert call(q, k, v, grad, [0, 0], left=3)["dk"].shape == (0, 1, 64)
+
+
+def test_no_wait_ran_out():
+    """The status call: every bounded wait of the kernels came back."""
+    from gaussian_splats_b200 import native
+
+    q, k, v, grad, valid = make([700, 0, 129], 4, 2, 128, torch.float16, dead=0.3)
+    call(q, k, v, grad, [700, 0, 129], valid=valid, left=200, right=9, first=5)
+    assert native.lib().gs_window_attention_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+def test_outputs_end_where_the_sequence_ends():
+    """Rows are written side by side: none of a neighbour's, none past the end."""
+    import ctypes
+
+    from gaussian_splats_b200 import native
+    from gaussian_splats_b200.attention import _arguments
+    from gaussian_splats_b200.sequences import (PackedSequences, call as run, element_type,
+                                                tile_arguments)
+
+    lengths, heads, kv_heads, dim = [130, 1, 255, 66], 3, 3, 72
+    q, k, v, grad, _ = make(lengths, heads, kv_heads, dim, torch.bfloat16)
+    tokens, packed = sum(lengths), PackedSequences(lengths)
+    spare = {n: torch.full((tokens + 300, heads, dim), 7.0, dtype=q.dtype, device="cuda")
+             for n in ("out", "grad_q", "grad_k", "grad_v")}
+    lse = torch.empty((heads, tokens), device="cuda")
+    q, k, v, grad = (t.contiguous() for t in (q, k, v, grad))
+    args = _arguments(native.WindowAttentionArgs, q, k, v, tokens=tokens,
+                      **tile_arguments(packed, tokens), heads=heads, kv_heads=kv_heads, dim=dim,
+                      dtype=element_type(q.dtype, "q"), left=40, right=3, first=2,
+                      scale=0.1, lse=lse.data_ptr(), grad_out=grad.data_ptr(),
+                      **{n: t.data_ptr() for n, t in spare.items()})
+    size = native.lib().gs_window_attention_workspace_size(ctypes.byref(args))
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    args.workspace, args.workspace_size = workspace.data_ptr(), size
+    run("gs_window_attention", q.device, ctypes.byref(args))
+    run("gs_window_attention_backward", q.device, ctypes.byref(args))
+    want = call(q, k, v, grad, lengths, left=40, right=3, first=2, scale=0.1)
+    for name, other in (("out", "out"), ("grad_q", "dq"), ("grad_k", "dk"), ("grad_v", "dv")):
+        assert torch.equal(spare[name][:tokens], want[other]), name
+        assert (spare[name][tokens:] == 7).all(), name

@@ -240,3 +240,11 @@ def test_no_tokens():
     got = call(s, [0, 0])
     assert torch.equal(got["last"], s["initial"]) and torch.equal(got["dinitial"], s["grad_last"])
     assert got["y"].shape == (0, 6)
+
+
+def test_no_wait_ran_out():
+    from gaussian_splats_b200 import native
+
+    s = make([3000, 5], 64, torch.bfloat16)
+    call(s, [3000, 5])
+    assert native.lib().gs_gated_scan_status(torch.cuda.current_stream().cuda_stream) == 0
