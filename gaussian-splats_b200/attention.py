@@ -78,7 +78,7 @@ def _arguments(kind, q, k, v, **values):
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, packed, left, right, first, valid, scale, dtype, need_grad):
-        q, k, v = _strided(q.detach()), _strided(k.detach()), _strided(v.detach())
+        q, k, v = _strided(q), _strided(k), _strided(v)
         tokens, heads, dim = q.shape
         out = q.new_empty((tokens, heads, dim))
         lse = q.new_empty((heads, tokens), dtype=torch.float32) if need_grad else None

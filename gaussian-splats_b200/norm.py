@@ -59,14 +59,15 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         shape = x.shape
-        rows, weight = _rows(x.detach()), weight.detach().contiguous()
-        res = None if residual is None else _rows(residual.detach())
+        rows, weight = _rows(x), weight.contiguous()
+        res = None if residual is None else _rows(residual)
         y = x.new_empty(shape)
         total = None if res is None else res.new_empty(shape)
         args = _arguments(rows, weight, res, eps, y=y, sum=total)
         call("gs_rms_norm", x.device, ctypes.byref(args))
         ctx.save_for_backward(rows if res is None else total, weight)
-        ctx.eps, ctx.has_residual, ctx.x_dtype, ctx.shape = eps, res is not None, x.dtype, shape
+        args.sum_stride = rows.stride(0) if res is None else rows.shape[1]
+        ctx.args, ctx.has_residual, ctx.x_dtype, ctx.shape = args, res is not None, x.dtype, shape
         ctx.set_materialize_grads(False)
         return y if res is None else (y, total)
 
@@ -74,7 +75,7 @@ class _RmsNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_sum=None):
         z, weight = ctx.saved_tensors
-        rows, shape = _rows(z), ctx.shape
+        shape = ctx.shape
         grad_y = z.new_zeros(shape, dtype=ctx.x_dtype) if grad_y is None \
             else grad_y.contiguous()
         grad_sum = None if grad_sum is None else grad_sum.contiguous()
@@ -83,13 +84,13 @@ class _RmsNorm(torch.autograd.Function):
         if ctx.has_residual and z.dtype != ctx.x_dtype:
             grad_residual = z.new_empty(shape)
         grad_weight = torch.empty_like(weight)
-        args = native.RmsNormArgs(
-            rows=rows.shape[0], channels=rows.shape[1], dtype=element_type(ctx.x_dtype, ""),
-            residual_dtype=element_type(z.dtype, ""),
-            weight_dtype=element_type(weight.dtype, ""), eps=ctx.eps, sum=address(rows),
-            sum_stride=rows.stride(0), weight=address(weight), grad_y=address(grad_y),
-            grad_sum=address(grad_sum), grad_x=address(grad_x),
-            grad_residual=address(grad_residual), grad_weight=address(grad_weight))
+        args = native.RmsNormArgs.from_buffer_copy(ctx.args)  # sizes, types, the sum's stride
+        args.x = args.residual = args.y = None
+        args.x_stride = args.residual_stride = 0
+        args.sum, args.weight = address(z), address(weight)
+        args.grad_y, args.grad_sum = address(grad_y), address(grad_sum)
+        args.grad_x, args.grad_residual = address(grad_x), address(grad_residual)
+        args.grad_weight = address(grad_weight)
         lib = native.lib()
         size = lib.gs_rms_norm_workspace_size(ctypes.byref(args))
         workspace = z.new_empty((size,), dtype=torch.uint8)

@@ -37,9 +37,9 @@ def _check_pair(what, x, gate, rows_name):
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, packed, dtype):
-        x, gate = _rows(x.detach()), _rows(gate.detach())
+        x, gate = _rows(x), _rows(gate)
         if initial is not None:
-            initial = initial.detach().contiguous()
+            initial = initial.contiguous()
         tokens, channels = x.shape
         device = x.device
         layout = tile_arguments(packed, tokens)

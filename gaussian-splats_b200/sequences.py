@@ -92,7 +92,7 @@ def call(name: str, device: torch.device, *arguments) -> None:
     status other than success."""
     stream = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
     function = getattr(native.lib(), name)
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         status = function(*arguments, stream)
     else:
         with torch.cuda.device(device):
