@@ -69,10 +69,21 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
         memory_format=torch.contiguous_format)
 
 
-def _arguments(kind, q, k, v, **values):
-    return kind(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q.stride(0),
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _place(q, k, v):
+    """The fields of an operator's arguments that say where q, k and v lie."""
+    return dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q.stride(0),
                 q_head_stride=q.stride(1), k_stride=k.stride(0), k_head_stride=k.stride(1),
-                v_stride=v.stride(0), v_head_stride=v.stride(1), **values)
+                v_stride=v.stride(0), v_head_stride=v.stride(1))
+
+
+def _arguments(kind, q, k, v, **values):
+    return kind(**_place(q, k, v), **values)
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -89,20 +100,22 @@ class _WindowAttention(torch.autograd.Function):
         call("gs_window_attention", q.device, ctypes.byref(args))
         if need_grad:
             ctx.save_for_backward(q, k, v, out, lse, valid)
-            ctx.packed, ctx.args = packed, args  # sizes, strides, the layout's table
+            ctx.packed, ctx.args = packed, args  # sizes, the layout's table
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, v, out, lse, valid = ctx.saved_tensors
-        grad_out = grad_out.contiguous()
-        if grad_out.data_ptr() % 16:
-            grad_out = grad_out.clone()
+        # A saved-tensor hook (offloading to the host, say) may have brought back
+        # tensors that lie differently than the forward's did.
+        q, k, v, out, grad_out = _strided(q), _strided(k), _strided(v), _whole(out), _whole(grad_out)
+        lse, valid = lse.contiguous(), None if valid is None else valid.contiguous()
         grad_q, grad_k, grad_v = (t.new_empty(t.shape) for t in (q, k, v))
         lib, args = native.lib(), native.WindowAttentionArgs.from_buffer_copy(ctx.args)
-        args.q, args.k, args.v, args.out = (t.data_ptr() for t in (q, k, v, out))
-        args.lse, args.valid = lse.data_ptr(), address(valid)
+        for name, value in _place(q, k, v).items():
+            setattr(args, name, value)
+        args.out, args.lse, args.valid = out.data_ptr(), lse.data_ptr(), address(valid)
         size = lib.gs_window_attention_workspace_size(ctypes.byref(args))
         workspace = q.new_empty((size,), dtype=torch.uint8)
         args.grad_out, args.grad_q = grad_out.data_ptr(), grad_q.data_ptr()

@@ -66,7 +66,6 @@ class _RmsNorm(torch.autograd.Function):
         args = _arguments(rows, weight, res, eps, y=y, sum=total)
         call("gs_rms_norm", x.device, ctypes.byref(args))
         ctx.save_for_backward(rows if res is None else total, weight)
-        args.sum_stride = rows.stride(0) if res is None else rows.shape[1]
         ctx.args, ctx.has_residual, ctx.x_dtype, ctx.shape = args, res is not None, x.dtype, shape
         ctx.set_materialize_grads(False)
         return y if res is None else (y, total)
@@ -75,6 +74,8 @@ class _RmsNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_sum=None):
         z, weight = ctx.saved_tensors
+        # A saved-tensor hook may have brought back tensors that lie differently.
+        z, weight = _rows(z), weight.contiguous()
         shape = ctx.shape
         grad_y = z.new_zeros(shape, dtype=ctx.x_dtype) if grad_y is None \
             else grad_y.contiguous()
@@ -84,10 +85,10 @@ class _RmsNorm(torch.autograd.Function):
         if ctx.has_residual and z.dtype != ctx.x_dtype:
             grad_residual = z.new_empty(shape)
         grad_weight = torch.empty_like(weight)
-        args = native.RmsNormArgs.from_buffer_copy(ctx.args)  # sizes, types, the sum's stride
+        args = native.RmsNormArgs.from_buffer_copy(ctx.args)  # sizes and types
         args.x = args.residual = args.y = None
         args.x_stride = args.residual_stride = 0
-        args.sum, args.weight = address(z), address(weight)
+        args.sum, args.weight, args.sum_stride = address(z), address(weight), z.stride(0)
         args.grad_y, args.grad_sum = address(grad_y), address(grad_sum)
         args.grad_x, args.grad_residual = address(grad_x), address(grad_residual)
         args.grad_weight = address(grad_weight)

@@ -65,6 +65,8 @@ class _GatedScan(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_last):
         x, gate, entering = ctx.saved_tensors
+        # A saved-tensor hook may have brought back tensors that lie differently.
+        x, gate, entering = _rows(x), _rows(gate), entering.contiguous()
         device = x.device
         grad_y = x.new_zeros(x.shape) if grad_y is None \
             else grad_y.contiguous()
@@ -72,6 +74,7 @@ class _GatedScan(torch.autograd.Function):
         grad_x, grad_gate = x.new_empty(x.shape), x.new_empty(x.shape)
         args = native.GatedScanArgs.from_buffer_copy(ctx.args)
         args.x, args.gate, args.entering = address(x), address(gate), address(entering)
+        args.x_stride, args.gate_stride = x.stride(0), gate.stride(0)
         args.initial = args.y = args.last = None
         grad_initial = None
         if ctx.has_initial and ctx.needs_input_grad[2]:

@@ -1,0 +1,65 @@
+"""What the sequence operators share: saved tensors, layouts, graphs, streams."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def operators(tokens=300):
+    """For each operator a call on slices of one projection and its gradients:
+    name -> (function, leaves, gradients of its outputs)."""
+    from gaussian_splats_b200.attention import window_attention
+    from gaussian_splats_b200.norm import rms_norm
+    from gaussian_splats_b200.recurrence import gated_scan
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    half = rand(tokens, 512).to(torch.bfloat16)
+    packed = PackedSequences([tokens - 100, 0, 100])
+    valid = rand(tokens) > -1.0
+
+    def leaves(*parts):
+        return [t.detach().requires_grad_() for t in parts]
+
+    def slices(*widths):
+        return half[:, :sum(widths)].split(widths, 1)
+
+    q, k, v = (t.unflatten(1, (-1, 64)) for t in slices(256, 128, 128))
+    x, gate = slices(128, 128)
+    odd_x, odd_gate = half[:, 1:98], half[:, 101:198]
+    weight, initial = rand(128).to(torch.bfloat16), rand(3, 128)
+    return {
+        "attention": (lambda q, k, v: [window_attention(q, k, v, packed, left=40, right=9, first=3,
+                                                        valid=valid)],
+                      leaves(q, k, v), [rand(tokens, 4, 64).to(torch.bfloat16)]),
+        "scan": (lambda x, gate, initial: gated_scan(x, gate, packed, initial=initial),
+                 leaves(x, gate, initial), [rand(tokens, 128).to(torch.bfloat16), rand(3, 128)]),
+        "scan, odd": (lambda x, gate: gated_scan(x, gate, packed), leaves(odd_x, odd_gate),
+                      [rand(tokens, 97).to(torch.bfloat16), rand(3, 97)]),
+        "norm": (lambda x, w: [rms_norm(x, w)], leaves(x, weight),
+                 [rand(tokens, 128).to(torch.bfloat16)]),
+        "norm, residual": (lambda x, w, r: rms_norm(x, w, r), leaves(x, weight, gate.float()),
+                           [rand(tokens, 128).to(torch.bfloat16), rand(tokens, 128)]),
+    }
+
+
+NAMES = ["attention", "scan", "scan, odd", "norm", "norm, residual"]
+
+
+def run(function, inputs, grads):
+    outputs = function(*inputs)
+    return [*outputs, *torch.autograd.grad(outputs, inputs, grads)]
+
+
+@pytest.mark.parametrize("pinned", [False, True], ids=["pageable", "pinned"])
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_kept_on_the_host(name, pinned):
+    """Offloading brings strided inputs back contiguous."""
+    function, inputs, grads = operators()[name]
+    expected = run(function, inputs, grads)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
+        outputs = function(*inputs)
+    got = [*outputs, *torch.autograd.grad(outputs, inputs, grads)]
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))

@@ -154,3 +154,66 @@ def test_morton_order():
     assert morton_order(torch.empty(0, 3)).shape == (0,)
     with pytest.raises(ValueError):
         morton_order(torch.zeros(3, 2))
+
+
+def _backward_calls(monkeypatch, build, hooks):
+    """The arguments that a backward passes to the library, and the tensors that the
+    hooks gave it; the library itself is not called."""
+    from gaussian_splats_b200 import attention, norm, recurrence
+
+    seen, unpacked = {}, []
+
+    def record(name, device, args):
+        if name.endswith("backward"):
+            seen["args"] = type(args._obj).from_buffer_copy(args._obj)
+
+    for module in (attention, norm, recurrence):
+        monkeypatch.setattr(module, "call", record)
+
+    def unpack(t):
+        unpacked.append(hooks[1](t))
+        return unpacked[-1]
+
+    with torch.autograd.graph.saved_tensors_hooks(hooks[0], unpack):
+        outputs, inputs = build()
+    torch.autograd.grad(outputs, inputs, [torch.ones_like(t) for t in outputs])
+    return seen["args"], {t.data_ptr(): t for t in unpacked}
+
+
+@pytest.mark.parametrize("packed", ["as it is", "contiguous", "wider"])
+@pytest.mark.parametrize("operator", ["attention", "scan", "norm"])
+def test_backward_goes_by_the_tensors_it_gets(monkeypatch, operator, packed):
+    """Saved-tensor hooks may hand back other strides than the forward's."""
+    wide = torch.randn(40, 4 * 64)
+    half = wide.to(torch.bfloat16)
+
+    def build():
+        from gaussian_splats_b200 import attention, norm, recurrence
+
+        if operator == "attention":
+            leaves = [half[:, s].unflatten(1, (-1, 64)).detach().requires_grad_()
+                      for s in (slice(0, 128), slice(128, 192), slice(192, 256))]
+            return [attention._WindowAttention.apply(*leaves, None, 3, 0, 0, None, 0.1, 1, True)], leaves
+        leaves = [wide[:, s].detach().requires_grad_() for s in (slice(0, 128), slice(128, 256))]
+        if operator == "scan":
+            return [recurrence._GatedScan.apply(*leaves, None, None, 0)[0]], leaves
+        weight = torch.ones(128, requires_grad=True)
+        return [norm._RmsNorm.apply(leaves[0], weight, None, 1e-6)], [leaves[0], weight]
+
+    def wider(t):
+        if t.dim() != 2 and t.dim() != 3:
+            return t.detach().clone()
+        return torch.cat((t, t, t), -1)[..., :t.shape[-1]].detach()
+
+    pack = {"as it is": lambda t: t.detach(), "contiguous": lambda t: t.detach().clone(
+        memory_format=torch.contiguous_format), "wider": wider}[packed]
+    args, tensors = _backward_calls(monkeypatch, build, (pack, lambda t: t))
+    fields = {"attention": ("q", "k", "v"), "scan": ("x", "gate"), "norm": ("sum",)}[operator]
+    for name in fields:
+        t = tensors[getattr(args, name)]
+        assert getattr(args, name + "_stride") == t.stride(0), name
+        if operator == "attention":
+            assert getattr(args, name + "_head_stride") == t.stride(1), name
+    for name in {"attention": ("out", "lse"), "scan": ("entering",), "norm": ("weight",)}[operator]:
+        t = tensors.get(getattr(args, name))  # or a contiguous copy of it
+        assert t is None or t.is_contiguous(), name
