@@ -654,8 +654,11 @@ struct BackwardShared {
   unsigned char tiles1[kStages1][Shape::kTileBytes];
   union {
     float row[kStages1][2][Shape::kRows];  // keys: -L and -D of a tile's queries
-    float part[kTile];                     // queries: D
+    struct {                               // queries: D, the squared norm of the gradient
+      float part[kTile], norm[kTile];
+    };
   };
+  float grow, back;  // keys: E's factor over P's, and what scales dK back
   uint64_t rows_full, full0[kStages0], full1[kStages1];  // loads
   uint64_t empty[kStages0];                              // a tile's sums are complete
   uint64_t scores, grads[2];  // S, G of a tile are complete
@@ -879,27 +882,94 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
   fence_after_sync();
 }
 
-// float16 loses bits below 2^-14, where a wide window's weights are: P is stored
-// times 2^p (about the window's width; P is at most 1) and E times 2^e (at most
-// 16, so that it overflows at 4094 at the earliest), and the sums are scaled
-// back. bfloat16 needs neither: p = e = 0.
-struct WeightScale {
-  float p;         // log2 of P's factor
-  float e, e_p;    // E's factor, and that over P's
-  float dk, dv;    // what scales the sums back (dk: dq too)
-};
-WeightScale weight_scale(const gs_window_attention_args& a) {
-  int p = 0, e = 0;
+// float16 loses bits below 2^-14, where a wide window's weights are, and ends at
+// 65504, which E passes under a loss scale. So P, at most 1, is stored times 2^p (about
+// the window's width), and E times 2^e, with e from what bounds it:
+//
+//   |E_ij| <= |G_ij - D_i| <= |g_i| |v_j| + |D_i|,  |D_i| <= |g_i| max_j |v_j|
+//
+// over the keys that query i sees. The exponent brings the bound to between 2^13 and
+// 2^15: a query's from its gradient's norm and the largest norm of a value in its block's
+// tiles, a block of keys' from its values and the largest norm and D of its queries. The
+// sums are scaled back by the same power of two. Rows that are not finite are left out
+// of the maxima: what they reach is not finite whatever the scale. bfloat16 needs
+// neither factor: it has the floats' range.
+constexpr int kScaleLimit = 40;
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+// e for a bound of at most `bound`.
+__device__ __forceinline__ int weight_exponent(float bound) {
+  const int log = (__float_as_int(bound) >> 23) - 127;  // bound < 2^(log + 1)
+  return max(-kScaleLimit, min(14 - log, kScaleLimit));
+}
+__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.0f; }
+
+template <class T>
+constexpr bool kScaled = std::is_same_v<T, __half>;
+
+// p, for the keys' kernel.
+int weight_power(const gs_window_attention_args& a) {
+  int p = 0;
   if (a.dtype == GS_FLOAT16) {
     const int64_t seen =
         std::min(a.tokens, int64_t{a.left} + int64_t{a.right} + 1 + int64_t{a.first});
     while (p < 15 && int64_t{2} << p <= seen) ++p;
-    e = std::min(4, p / 2);
   }
-  return {static_cast<float>(p), std::ldexp(1.0f, e), std::ldexp(1.0f, e - p),
-          std::ldexp(a.scale, -e), std::ldexp(1.0f, -p)};
+  return p;
 }
 
+// float16's maxima: of the squared norms of a tile's values [tile, kv head], and of the
+// squared norm of the gradient and |D| of 32 queries [set of 32, head].
+struct Peaks {
+  float* values;
+  float2* queries;
+};
+constexpr int kTileSets = kTile / 32;
+
+// The squared norms of values: a block a tile and key-value head. Bound by memory and a
+// launch; with the exponents' work a pass of 16,384 tokens, 8 heads of 64, takes 245 us
+// instead of 229, one of 65,536 tokens, 8 heads (4) of 128, 1700 instead of 1650.
+constexpr int kPeakThreads = 256;
+template <class T, int kDim>
+__global__ void __launch_bounds__(kPeakThreads) value_peak_kernel(gs_window_attention_args a,
+                                                                  float* peaks) {
+  chain_wait();
+  __shared__ float s_peak[kPeakThreads / 32];
+  constexpr int kLanes = kDim / 8, kStep = kPeakThreads / kLanes, kSteps = kTile / kStep;
+  const int kv_head = blockIdx.x % a.kv_heads;
+  const Tile tile =
+      tile_at(a.tiles, blockIdx.x / a.kv_heads, static_cast<int32_t>(a.tokens), kTile);
+  const int word = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  const bool used = 8 * word < a.dim;
+  const T* v = static_cast<const T*>(a.v) + kv_head * a.v_head_stride + (used ? 8 * word : 0);
+  Pack<T, 8> x[kSteps];
+  uint8_t valid[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int64_t token = min(int64_t{tile.start} + row + k * kStep, int64_t{tile.end} - 1);
+    x[k] = *reinterpret_cast<const Pack<T, 8>*>(v + token * a.v_stride);
+    valid[k] = a.valid ? __ldg(a.valid + token) : 1;
+  }
+  float peak = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    float square = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) square = fmaf(to_float(x[k].v[e]), to_float(x[k].v[e]), square);
+    if (!used) square = 0.0f;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+    if (valid[k]) peak = fmaxf(peak, finite_or_zero(square));
+  }
+  peak = warp_max(peak);
+  if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPeakThreads / 32; ++w) peak = fmaxf(peak, s_peak[w]);
+    peaks[blockIdx.x] = peak;
+  }
+}
+
+__device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 __device__ __forceinline__ void sync_compute() {
   asm volatile("bar.sync 1, %0;" ::"n"(kComputeThreads) : "memory");
 }
@@ -928,7 +998,7 @@ __device__ __forceinline__ bool row_products(const gs_window_attention_args& a, 
 #pragma unroll
   for (int k = 0; k < kSteps; ++k) {
     const int row = first + k * kRows;
-    float g[8], d = 0.0f;
+    float g[8], d = 0.0f, square = 0.0f;
     load_pack<8>(reinterpret_cast<const T*>(s.rows[1] + word / 8 * (kTile * 128) + row * 128 +
                                             ((word ^ row) & 7) * 16),
                  g);
@@ -939,6 +1009,14 @@ __device__ __forceinline__ bool row_products(const gs_window_attention_args& a, 
 #pragma unroll
     for (int x = kLanes / 2; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
     if (word == 0) s.part[row] = d;
+    if constexpr (kScaled<T>) {  // channels past the last are zeros
+#pragma unroll
+      for (int e = 0; e < 8; ++e) square = fmaf(g[e], g[e], square);
+#pragma unroll
+      for (int x = kLanes / 2; x > 0; x >>= 1)
+        square += __shfl_xor_sync(0xffffffffu, square, x);
+      if (word == 0) s.norm[row] = square;
+    }
   }
   return true;
 }
@@ -952,7 +1030,7 @@ __device__ __forceinline__ float weight_shift(float lse) {
 // dq, and D_i into `delta` for the keys' kernel.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::kBlocks)
-    grad_query_kernel(gs_window_attention_args a, WeightScale weights, float* delta,
+    grad_query_kernel(gs_window_attention_args a, float* delta, Peaks peaks,
                       const __grid_constant__ CUtensorMap q_map,
                       const __grid_constant__ CUtensorMap g_map,
                       const __grid_constant__ CUtensorMap k_map,
@@ -987,18 +1065,39 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     const bool live = tile.start + row < tile.end;
     const int64_t slot = head * a.tokens + tile.start + row;
     const float shift = live ? weight_shift(a.lse[slot]) : INFINITY;
+    const int64_t index = blockIdx.x / a.heads;  // the tile's number
+    float value_peak = 0.0f;
+    if constexpr (kScaled<T>) {  // of the tiles that hold the walk's keys
+      const int low = walk.low / kTile, count = (walk.high[0] - 1) / kTile - low + 1;
+      const float* of = peaks.values + (index - i_first / kTile) * a.kv_heads + kv_head;
+      for (int k = threadIdx.x & 31; k < count + (walk.head_tiles > 0); k += 32)
+        value_peak = fmaxf(value_peak, of[int64_t{k < count ? low + k : 0} * a.kv_heads]);
+    }
     bool good = row_products<T, kDim>(a, tile, head, s);
     sync_compute();
     const float d = live ? s.part[row] : 0.0f;
     if (live && half == 0) delta[slot] = d;
+    float up = 1.0f, back = a.scale;
+    if constexpr (kScaled<T>) {
+      const float norm = live ? s.norm[row] : 0.0f;
+      const int e = weight_exponent(2.0f * sqrtf(norm * warp_max(value_peak)));
+      up = power_of_two(e);
+      back *= power_of_two(-e);
+      if (half == 0) {
+        const bool counts = shift != INFINITY;
+        const float2 peak = make_float2(warp_max(counts ? finite_or_zero(norm) : 0.0f),
+                                        warp_max(counts ? finite_or_zero(fabsf(d)) : 0.0f));
+        if ((threadIdx.x & 31) == 0)
+          peaks.queries[(index * kTileSets + warp) * a.heads + head] = peak;
+      }
+    }
     const float scale = a.scale * kLog2e;
     // Every query sees every valid key of a tile that lies from `from` (or under
     // `first`) to `to`.
     const int from = position(int64_t{i_first} + kTile - 1 - a.left);
     const int to = min(position(int64_t{i_first} + a.right + 1), walk.n);
     const float2 factor = make_float2(scale, scale), down = make_float2(-shift, -shift);
-    const float2 grow = make_float2(weights.e, weights.e);
-    const float2 less = make_float2(-d * weights.e, -d * weights.e);
+    const float2 grow = make_float2(up, up), less = make_float2(-d * up, -d * up);
     const uint32_t scores = mine + 32 * kHalfSets * half;
     // Whether the lane's keys of tile t are valid, a tile ahead.
     bool valid[kSets];
@@ -1101,7 +1200,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     for (int e = 0; e < kDim / 2; e += 8) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * weights.dk : NAN;
+      for (int k = 0; k < 8; ++k) v[k] = good ? o[e + k] * back : NAN;
       put_word<T, kDim>(rows, row, (half * (kDim / 2) + e) / 8, v);
     }
     sync_compute();
@@ -1131,7 +1230,7 @@ __device__ __forceinline__ bool beyond_window(const gs_window_attention_args& a,
 // dk and dv.
 template <class T, int kDim>
 __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::kBlocks)
-    grad_key_kernel(gs_window_attention_args a, WeightScale weights, const float* delta,
+    grad_key_kernel(gs_window_attention_args a, int power, const float* delta, Peaks peaks,
                     FirstSums sums,
                     const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map,
@@ -1149,10 +1248,11 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
   const int64_t item = blockIdx.x / a.kv_heads;
   const bool chunk = item < sums.slots;  // the long items come first
   Tile tile;
-  int low, high;  // queries, as positions
+  int low, high;   // queries, as positions
+  int64_t number;  // of the block's tile of keys
   if (chunk) {
     const int64_t b = sequence_of_run(a, item, sums.tiles);
-    const int64_t tile0 = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
+    const int64_t tile0 = number = first_tile_of(a, b), tiles = first_tile_of(a, b + 1) - tile0;
     const int64_t index = (item - run_of(tile0, b, sums.tiles)) * sums.tiles;
     if (index >= tiles) return;
     tile = tile_at(a.tiles, tile0, static_cast<int32_t>(a.tokens), kTile);
@@ -1161,7 +1261,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     high = static_cast<int>(min((index + sums.tiles) * kTile, n));
     if (low >= high) return;
   } else {
-    tile = tile_at(a.tiles, item - sums.slots, static_cast<int32_t>(a.tokens), kTile);
+    number = item - sums.slots;
+    tile = tile_at(a.tiles, number, static_cast<int32_t>(a.tokens), kTile);
     const int64_t n = tile.end - tile.begin, j = tile.start - tile.begin;
     low = max(0, position(j - a.right));
     high = static_cast<int>(min(n, min(j + kTile, n) + a.left));
@@ -1173,6 +1274,25 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
                  make_int2(kv_head * group, tile.begin + low));
   const uint32_t tensor = s.tensor;
   if (warp == kLoadWarp) {
+    float grow = 1.0f, value_peak = 0.0f;
+    float2 peak[4] = {};  // of the lane's sets of 32 queries
+    if constexpr (kScaled<T>) {
+      const int set = low / 32, count = ((high - 1) / 32 - set + 1) * group;
+      const float2* of = peaks.queries +
+                         ((number - (tile.start - tile.begin) / kTile) * kTileSets + set) * a.heads +
+                         kv_head * group;
+      const auto at = [&](int k) {  // a number past the last names the last again
+        k = min(k, count - 1);
+        return of[int64_t{k / group} * a.heads + k % group];
+      };
+      value_peak = peaks.values[number * a.kv_heads + kv_head];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) peak[k] = at(lane_id() + 32 * k);
+      for (int k = lane_id() + 128; k < count; k += 32) {
+        const float2 x = at(k);
+        peak[0] = make_float2(fmaxf(peak[0].x, x.x), fmaxf(peak[0].y, x.y));
+      }
+    }
     // L and D of a tile's queries come along, negated.
     struct RowValues {
       float shift[kSets], delta[kSets];
@@ -1197,13 +1317,25 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
           return v;
         },
         [&](int t, int stage, int lane, const RowValues& v) {
+          if (kScaled<T> && t == 0) {  // the tile's values and the peaks were loaded side by side
+            const float norm = warp_max(fmaxf(fmaxf(peak[0].x, peak[1].x),
+                                              fmaxf(peak[2].x, peak[3].x)));
+            const float d = warp_max(fmaxf(fmaxf(peak[0].y, peak[1].y),
+                                           fmaxf(peak[2].y, peak[3].y)));
+            const int e = weight_exponent(fmaf(1.001f, sqrtf(norm * value_peak), d));
+            grow = power_of_two(e - power);
+            if (lane == 0) {
+              s.grow = grow;
+              s.back = a.scale * power_of_two(-e);
+            }
+          }
           const int i = low + (t % per_head) * kRows + lane;
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
             const bool in = i + 32 * k < n;
             s.row[stage][0][lane + 32 * k] =
-                in ? weights.p - weight_shift(v.shift[k]) : -INFINITY;
-            s.row[stage][1][lane + 32 * k] = in ? -v.delta[k] * weights.e_p : 0.0f;
+                in ? power - weight_shift(v.shift[k]) : -INFINITY;
+            s.row[stage][1][lane + 32 * k] = in ? -v.delta[k] * grow : 0.0f;
           }
         });
   } else if (warp == kProductWarp) {
@@ -1224,7 +1356,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     const int all_from = position(int64_t{j_first} + kTile - 1 - a.right);
     const int all_to = chunk ? 0 : min(high, position(int64_t{j_first} + a.left + 1));
     const float scale = a.scale * kLog2e;
-    const float2 factor = make_float2(scale, scale), grow = make_float2(weights.e_p, weights.e_p);
+    const float2 factor = make_float2(scale, scale);
     const uint32_t scores = mine + 32 * kHalfSets * half, grads = scores + Shape::kGrad;
     bool good = true;
     int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
@@ -1293,6 +1425,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
       barrier_arrive(shared_address(&s.read));
       if (!(good = barrier_wait_warp(shared_address(&s.grads[0]), t & 1))) break;
       fence_after_sync();
+      const float up = kScaled<T> ? s.grow : 1.0f;
+      const float2 grow = make_float2(up, up);
       const float4* deltas = reinterpret_cast<const float4*>(s.row[stage1][1] + 32 * kHalfSets * half);
 #pragma unroll
       for (int h = 0; h < kHalfSets; ++h)
@@ -1353,7 +1487,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
         load_columns32(mine + Shape::kSum + which * kDim + half * (kDim / 2) + c,
                        reinterpret_cast<float(&)[32]>(o[c]));
       wait_loads();
-      const float factor = which ? weights.dv : weights.dk;
+      const float factor = which ? power_of_two(-power) : kScaled<T> ? s.back : a.scale;
 #pragma unroll
       for (int e = 0; e < kDim / 2; e += 8) {
         const int c = half * (kDim / 2) + e;
@@ -1424,6 +1558,16 @@ int64_t delta_floats(const gs_window_attention_args& a) {
   return (a.tokens * a.heads + 63) / 64 * 64;
 }
 
+// float16's maxima: floats of those of the queries, and of all of them to a 256-byte
+// boundary.
+int64_t query_peak_floats(const gs_window_attention_args& a) {
+  return a.num_tiles * kTileSets * a.heads * 2;
+}
+int64_t peak_floats(const gs_window_attention_args& a) {
+  if (a.dtype != GS_FLOAT16) return 0;
+  return (query_peak_floats(a) + a.num_tiles * a.kv_heads + 63) / 64 * 64;
+}
+
 // A chunk is about as long as a window's walk, so that its block takes about as
 // long as the others.
 int64_t chunk_tiles(const gs_window_attention_args& a) {
@@ -1451,12 +1595,13 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
       GS_TRY(tc::encode_heads(&tiles[m], a.dtype, base[m], a.tokens, heads, a.dim, stride[m],
                               head_stride[m], kRows));
   }
-  const WeightScale weights = weight_scale(a);
   float* delta = static_cast<float*>(a.workspace);
+  float* maxima = delta + delta_floats(a);
+  const Peaks peaks = {maxima + query_peak_floats(a), reinterpret_cast<float2*>(maxima)};
   FirstSums sums;
   sums.tiles = static_cast<int>(chunk_tiles(a));
   sums.slots = static_cast<int>(chunk_slots(a));
-  sums.base = delta + delta_floats(a);
+  sums.base = maxima + peak_floats(a);
   sums.part = sums.base + sequences_of(a) * a.kv_heads * a.first * 2 * a.dim;
   constexpr size_t kQueryShared = sizeof(BackwardShared<kDim, false>);
   constexpr size_t kKeyShared = sizeof(BackwardShared<kDim, true>);
@@ -1465,12 +1610,18 @@ int32_t backward(const gs_window_attention_args& a, cudaStream_t stream) {
   const int64_t key_blocks = (a.num_tiles + sums.slots) * a.kv_heads;
   const int64_t first_blocks = sequences_of(a) * a.kv_heads * a.first;
   if (key_blocks > INT32_MAX || first_blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  if constexpr (kScaled<T>) {
+    launch_chained(value_peak_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.kv_heads),
+                   kPeakThreads, stream, a, peaks.values);
+    GS_TRY(check_launch());
+  }
   launch_chained_shared(grad_query_kernel<T, kDim>, static_cast<unsigned>(a.num_tiles * a.heads),
-                        kBackwardThreads, kQueryShared, stream, a, weights, delta, rows[0], rows[1],
+                        kBackwardThreads, kQueryShared, stream, a, delta, peaks, rows[0], rows[1],
                         tiles[2], tiles[3]);
   GS_TRY(check_launch());
   launch_chained_shared(grad_key_kernel<T, kDim>, static_cast<unsigned>(key_blocks),
-                        kBackwardThreads, kKeyShared, stream, a, weights, delta, sums, rows[2], rows[3],
+                        kBackwardThreads, kKeyShared, stream, a, weight_power(a), delta, peaks, sums, rows[2],
+                        rows[3],
                         tiles[0], tiles[1]);
   GS_TRY(check_launch());
   if (first_blocks > 0)
@@ -1919,7 +2070,7 @@ int32_t with_sixteen_bit(int32_t dtype, F&& f) {
 uint64_t window_attention_workspace_size(const gs_window_attention_args& a) {
   const int64_t first =
       (sequences_of(a) + chunk_slots(a)) * a.kv_heads * a.first * 2 * a.dim;
-  return sizeof(float) * static_cast<uint64_t>(delta_floats(a) + first);
+  return sizeof(float) * static_cast<uint64_t>(delta_floats(a) + peak_floats(a) + first);
 }
 
 int32_t launch_window_attention(const gs_window_attention_args& a, cudaStream_t stream) {

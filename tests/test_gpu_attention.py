@@ -352,3 +352,42 @@ def test_outputs_end_where_the_sequence_ends():
     for name, other in (("out", "out"), ("grad_q", "dq"), ("grad_k", "dk"), ("grad_v", "dv")):
         assert torch.equal(spare[name][:tokens], want[other]), name
         assert (spare[name][tokens:] == 7).all(), name
+
+
+@pytest.mark.parametrize("size", [2.0 ** -9, 2.0 ** 10], ids=["small", "large"])
+@pytest.mark.parametrize("dim,left,right,first", [(64, 300, 200, 5), (128, 700, 0, 0),
+                                                  (64, 1, 1, 2)], ids=str)
+def test_float16_gradients_of_any_size(dim, left, right, first, size):
+    """Gradients under a loss scale, or far below one: powers of two times the unit
+    ones, so the bounds are those of the unit ones times the size, and half a unit of
+    the subnormal results. Peaked weights (scores of deviation 3) make score
+    gradients of several thousand at the larger size, where the results fit."""
+    lengths = [900, 0, 270]
+    q, k, v, grad, valid = make(lengths, 4, 2, dim, torch.float16, seed=7, dead=0.1)
+    q, grad = 3 * q, size * grad
+    window = dict(left=left, right=right, first=first, valid=valid)
+    ref = R.attention(q, k, v, lengths, grad=grad, **window)
+    got = call(q, k, v, grad, lengths, **window)
+    for name in ("dq", "dk", "dv"):
+        assert ref[name].abs().max() < torch.finfo(torch.float16).max
+        bound = 1.25 * U[torch.float16] * (ref[name].abs() + ref[name + "_spread"])
+        bound = bound + size * (1e-5 + TINY[torch.float16] * 900 * 2 * 18.0) + 2.0 ** -25
+        assert torch.isfinite(got[name]).all(), name
+        excess = ((got[name].double() - ref[name]).abs() - bound).max()
+        assert excess <= 0, f"{name}: {excess.item():.3g} beyond its bound"
+
+
+def test_float16_gradients_of_one_query_leave_the_others_theirs():
+    """One query's gradient of 2**15 times the others' size, in another sequence and in
+    the same one out of reach: those that it does not meet keep their bits."""
+    lengths = [400, 900]
+    q, k, v, grad, _ = make(lengths, 2, 1, 64, torch.float16, seed=8)
+    grad = grad * 2.0 ** -6
+    window = dict(left=20, right=20)
+    clean = call(q, k, v, grad, lengths, **window)
+    grad[450] *= 2.0 ** 15
+    got = call(q, k, v, grad, lengths, **window)
+    for name in ("dq", "dk", "dv"):
+        assert torch.isfinite(got[name]).all()
+        assert torch.equal(got[name][:400], clean[name][:400]), name
+        assert torch.equal(got[name][900:], clean[name][900:]), name
