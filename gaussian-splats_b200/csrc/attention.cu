@@ -2047,10 +2047,10 @@ int32_t check_args(const gs_window_attention_args& a) {
       a.left < 0 || a.right < 0 || a.first < 0 || a.first > GS_MAX_FIRST_TOKENS ||
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
-  if (!a.tiles && a.num_tiles != (a.tokens + kTile - 1) / kTile) return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.tiles, 16)) return GS_ERR_MISALIGNED;
+  if (!layout_holds(a.tokens, a.sequences, a.num_tiles, a.tiles, a.tile_starts))
+    return GS_ERR_INVALID_ARGUMENT;
   if (a.num_tiles == 0) return GS_OK;
-  if (a.tiles && !a.tile_starts) return GS_ERR_INVALID_ARGUMENT;
   if (!a.q || !a.k || !a.v || !a.out) return GS_ERR_INVALID_ARGUMENT;
   if (!strided16(a.q, a.q_stride, a.q_head_stride) ||
       !strided16(a.k, a.k_stride, a.k_head_stride) ||

@@ -521,7 +521,8 @@ int32_t gs_l1_loss_backward(const float* image, int64_t height, int64_t width, i
 
 uint64_t gs_window_attention_workspace_size(const gs_window_attention_args* a) {
   return !a || a->tokens < 0 || a->heads < 1 || a->kv_heads < 1 || a->dim < 1 || a->first < 0 ||
-                 a->left < 0 || a->right < 0
+                 a->left < 0 || a->right < 0 || a->num_tiles < 0 ||
+                 (a->tile_starts && a->sequences < 1)
              ? 0
              : gs::window_attention_workspace_size(*a);
 }

@@ -684,9 +684,8 @@ int32_t check_args(const gs_gated_scan_args& a) {
   if (a.tokens < 0 || a.tokens > INT32_MAX || a.channels < 1 || a.sequences < 1 ||
       a.num_tiles < 0 || a.dtype < GS_FLOAT32 || a.dtype > GS_FLOAT16)
     return GS_ERR_INVALID_ARGUMENT;
-  if (a.tile_starts ? (a.num_tiles > 0 && !a.tiles)
-                    : (a.tiles || a.sequences != 1 ||
-                       a.num_tiles != (a.tokens + kTile - 1) / kTile))
+  if (!layout_holds(a.tokens, a.sequences, a.num_tiles, a.tiles, a.tile_starts) ||
+      (!a.tile_starts && a.sequences != 1))
     return GS_ERR_INVALID_ARGUMENT;
   if (!is_aligned(a.tiles, 16) || !is_aligned(a.workspace, 8)) return GS_ERR_MISALIGNED;
   const int64_t columns = (int64_t{a.channels} + 7) / 8;

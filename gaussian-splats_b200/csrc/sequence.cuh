@@ -62,6 +62,16 @@ inline bool is_aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
 }
 
+// Whether a batch's layout may be walked: a table with its sequences' first tiles,
+// or neither and the tiles of one sequence.
+inline bool layout_holds(int64_t tokens, int64_t sequences, int64_t num_tiles,
+                         const int32_t* tiles, const int32_t* tile_starts) {
+  if (tile_starts)
+    return sequences >= 1 && sequences <= INT32_MAX / 2 && num_tiles <= INT32_MAX &&
+           (num_tiles == 0 || tiles);
+  return !tiles && num_tiles == (tokens + GS_SEQUENCE_TILE - 1) / GS_SEQUENCE_TILE;
+}
+
 // Calls f with a value of the element type that `dtype` names.
 template <class F>
 inline int32_t with_dtype(int32_t dtype, F&& f) {

@@ -485,7 +485,8 @@ int32_t gs_l1_loss_backward(const float *image, int64_t height, int64_t width, i
  * of its tiles of GS_SEQUENCE_TILE tokens, int32 [num_tiles, 4] (16-byte
  * aligned): the first and the end row of the tile's sequence, the tile's first
  * row, the sequence's number; tiles in row order, none for an empty sequence.
- * With tiles == NULL the rows are one sequence, of ceil(tokens / tile) tiles.
+ * tile_starts [sequences + 1] int32 is each sequence's first tile. With both NULL the
+ * rows are one sequence, of ceil(tokens / tile) tiles; one without the other is refused.
  * The table is read as given: it must describe the `tokens` rows. Strides are
  * in elements; the last axis of every array is contiguous. */
 
@@ -558,10 +559,9 @@ int32_t gs_window_attention_step(const gs_window_attention_step_args *args, gs_s
  * zeros). x, gate [tokens, channels] with row strides; y = h (dtype of x),
  * last [sequences, channels] float = each sequence's final state (its initial
  * state where it is empty). `entering` [num_tiles, channels] float receives
- * the state that enters each tile, which the backward reads; tile_starts
- * [sequences + 1] int32 (with `tiles`) is each sequence's first tile. The
- * backward takes grad_y [tokens, channels] contiguous and grad_last (NULL:
- * zeros) and writes grad_x, grad_gate and, unless NULL, grad_initial. Both
+ * the state that enters each tile, which the backward reads. The backward takes
+ * grad_y [tokens, channels] contiguous and grad_last (NULL: zeros) and writes
+ * grad_x, grad_gate and, unless NULL, grad_initial. Both
  * need a workspace of gs_gated_scan_workspace_size bytes (8-byte aligned). */
 typedef struct gs_gated_scan_args {
   int64_t tokens, sequences, num_tiles;

@@ -217,3 +217,31 @@ def test_backward_goes_by_the_tensors_it_gets(monkeypatch, operator, packed):
     for name in {"attention": ("out", "lse"), "scan": ("entering",), "norm": ("weight",)}[operator]:
         t = tensors.get(getattr(args, name))  # or a contiguous copy of it
         assert t is None or t.is_contiguous(), name
+
+
+def test_library_refuses_half_a_layout():
+    """A table of tiles without the sequences' first tiles, first tiles without a
+    table, or no sequences: never walked."""
+    from gaussian_splats_b200 import native
+
+    lib, a = native.lib(), 256
+    attention = dict(tokens=300, num_tiles=3, heads=4, kv_heads=2, dim=64, dtype=1, left=3, first=2,
+                     scale=0.1, q=a, k=a, v=a, q_stride=64, q_head_stride=64, k_stride=64,
+                     k_head_stride=64, v_stride=64, v_head_stride=64, out=a, lse=a, grad_out=a,
+                     grad_q=a, grad_k=a, grad_v=a, workspace=a, workspace_size=1 << 40)
+    scan = dict(tokens=300, num_tiles=3, channels=8, x=a, gate=a, x_stride=8, gate_stride=8, y=a,
+                last=a, entering=a, grad_y=a, grad_x=a, grad_gate=a, workspace=a,
+                workspace_size=1 << 40)
+    for layout in (dict(tile_starts=a, sequences=2), dict(tiles=a, sequences=2),
+                   dict(tiles=a, tile_starts=a, sequences=0),
+                   dict(tiles=a, tile_starts=a, sequences=-3),
+                   dict(tiles=a, tile_starts=a, sequences=2 ** 62),
+                   dict(tiles=a, tile_starts=a, sequences=2, num_tiles=2 ** 61)):
+        args = native.WindowAttentionArgs(**{**attention, **layout})
+        assert lib.gs_window_attention(ctypes.byref(args), None) == -1, layout
+        assert lib.gs_window_attention_backward(ctypes.byref(args), None) == -1, layout
+        args = native.GatedScanArgs(**{**scan, **layout})
+        assert lib.gs_gated_scan(ctypes.byref(args), None) == -1, layout
+        assert lib.gs_gated_scan_backward(ctypes.byref(args), None) == -1, layout
+    args = native.WindowAttentionArgs(**{**attention, "tiles": a, "tile_starts": a})
+    assert lib.gs_window_attention_workspace_size(ctypes.byref(args)) == 0
