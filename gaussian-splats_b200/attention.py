@@ -26,11 +26,11 @@ import torch
 
 from . import native
 from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
-                        tile_arguments)
+                        check_tokens, tile_arguments)
 
 MAX_HEAD_DIM = 128
 _TYPES = (torch.bfloat16, torch.float16)
-_LONGEST = 2 ** 31 - 1
+_WIDEST = 2 ** 31 - 1  # of a window's sides: no window
 
 
 def _heads(what, q, k, v, rows_name):
@@ -152,8 +152,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     device = check_cuda(what, q=q, k=k, v=v, valid=valid)
     dtype = _heads(what, q, k, v, "tokens")
     tokens = q.shape[0]
-    if tokens > _LONGEST:
-        raise ValueError(f"{what}: {tokens} tokens, at most {_LONGEST} are supported")
+    check_tokens(tokens, what)
     check_packed(packed, tokens, device, what)
     left, right, first = int(left), int(right), int(first)
     if left < 0 or right < 0:
@@ -167,7 +166,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         valid = valid.contiguous()
     need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
                                              v.requires_grad)
-    return _WindowAttention.apply(q, k, v, packed, min(left, _LONGEST), min(right, _LONGEST),
+    return _WindowAttention.apply(q, k, v, packed, min(left, _WIDEST), min(right, _WIDEST),
                                   first, valid, _scale(what, scale, q.shape[2]), dtype, need_grad)
 
 
@@ -215,6 +214,9 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             cache_v.data_ptr() % 16:
         raise ValueError(f"{what}: the caches must be contiguous and 16-byte aligned (they are "
                          "updated in place)")
+    if batch * shape[1] > native.MAX_SEQUENCE_TOKENS:
+        raise ValueError(f"{what}: caches of {batch} x {shape[1]} slots, at most "
+                         f"{native.MAX_SEQUENCE_TOKENS} in all are supported")
     first = int(first)
     if not 0 <= first < shape[1]:
         raise ValueError(f"{what}: first must be in [0, {shape[1]}) for {shape[1]} slots, got "

@@ -2043,7 +2043,7 @@ int32_t check_heads(int32_t heads, int32_t kv_heads, int32_t dim, int32_t dtype)
 
 int32_t check_args(const gs_window_attention_args& a) {
   GS_TRY(check_heads(a.heads, a.kv_heads, a.dim, a.dtype));
-  if (a.tokens < 0 || a.tokens > INT32_MAX || a.num_tiles < 0 || a.num_tiles > INT32_MAX / a.heads ||
+  if (a.tokens < 0 || a.tokens > GS_MAX_SEQUENCE_TOKENS || a.num_tiles < 0 || a.num_tiles > INT32_MAX / a.heads ||
       a.left < 0 || a.right < 0 || a.first < 0 || a.first > GS_MAX_FIRST_TOKENS ||
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
@@ -2102,7 +2102,7 @@ int32_t launch_window_attention_backward(const gs_window_attention_args& a, cuda
 
 int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   GS_TRY(check_heads(a.heads, a.kv_heads, a.dim, a.dtype));
-  if (a.batch < 0 || a.first < 0 || a.slots <= a.first || a.batch > INT32_MAX / a.slots ||
+  if (a.batch < 0 || a.first < 0 || a.slots <= a.first || a.batch > GS_MAX_SEQUENCE_TOKENS / a.slots ||
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return GS_OK;

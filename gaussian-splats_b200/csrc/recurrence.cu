@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(int64_t count, int chann
 }
 
 int32_t check_args(const gs_gated_scan_args& a) {
-  if (a.tokens < 0 || a.tokens > INT32_MAX || a.channels < 1 || a.sequences < 1 ||
+  if (a.tokens < 0 || a.tokens > GS_MAX_SEQUENCE_TOKENS || a.channels < 1 || a.sequences < 1 ||
       a.num_tiles < 0 || a.dtype < GS_FLOAT32 || a.dtype > GS_FLOAT16)
     return GS_ERR_INVALID_ARGUMENT;
   if (!layout_holds(a.tokens, a.sequences, a.num_tiles, a.tiles, a.tile_starts) ||

@@ -187,6 +187,7 @@ def adam_params(steps, lrs, betas, eps, noise_lr=0.0, position_lr=0.0) -> AdamPa
 SEQUENCE_TILE = 128       # GS_SEQUENCE_TILE (include/gs_b200.h)
 MAX_FIRST_TOKENS = 128    # GS_MAX_FIRST_TOKENS
 MAX_NORM_CHANNELS = 16384  # GS_MAX_NORM_CHANNELS
+MAX_SEQUENCE_TOKENS = 2 ** 31 - 512  # GS_MAX_SEQUENCE_TOKENS
 
 
 def _fields(kind, names):

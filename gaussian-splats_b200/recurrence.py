@@ -17,7 +17,7 @@ import torch
 
 from . import native
 from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
-                        tile_arguments)
+                        check_tokens, tile_arguments)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -103,8 +103,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, packed: PackedSequences | No
     device = check_cuda(what, x=x, gate=gate, initial=initial)
     dtype = _check_pair(what, x, gate, "tokens")
     tokens, channels = x.shape
-    if tokens >= 2 ** 31:
-        raise ValueError(f"{what}: {tokens} tokens, less than 2**31 are supported")
+    check_tokens(tokens, what)
     check_packed(packed, tokens, device, what)
     if initial is not None:
         expected = (1 if packed is None else len(packed), channels)

@@ -31,8 +31,7 @@ class PackedSequences:
         if min(self.lengths) < 0:
             raise ValueError(f"sequence lengths must be >= 0, got {min(self.lengths)}")
         self.total = sum(self.lengths)
-        if self.total >= 2 ** 31:
-            raise ValueError(f"a packed batch holds less than 2**31 tokens, got {self.total}")
+        check_tokens(self.total, "PackedSequences")
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -54,6 +53,13 @@ class PackedSequences:
 
     def __len__(self) -> int:
         return len(self.lengths)
+
+
+def check_tokens(tokens: int, what: str) -> None:
+    """Refuses more tokens than the kernels' 32-bit positions count."""
+    if tokens > native.MAX_SEQUENCE_TOKENS:
+        raise ValueError(f"{what}: {tokens} tokens, at most {native.MAX_SEQUENCE_TOKENS} are "
+                         "supported")
 
 
 def check_packed(packed: PackedSequences | None, tokens: int, device: torch.device,

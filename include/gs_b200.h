@@ -494,7 +494,10 @@ enum { GS_FLOAT32 = 0, GS_BFLOAT16 = 1, GS_FLOAT16 = 2 }; /* element types */
 enum {
   GS_SEQUENCE_TILE = 128,      /* tokens of a tile */
   GS_MAX_FIRST_TOKENS = 128,   /* first tokens that may stay visible */
-  GS_MAX_NORM_CHANNELS = 16384 /* channels of gs_rms_norm */
+  GS_MAX_NORM_CHANNELS = 16384, /* channels of gs_rms_norm */
+  /* tokens of a packed batch (slots of all streams' caches): positions are 32-bit, and the
+   * last tile of a walk reaches past the last token */
+  GS_MAX_SEQUENCE_TOKENS = 0x7fffffff - 511
 };
 
 /* Attention in a window: query i of a sequence sees key j if valid[j] (all are

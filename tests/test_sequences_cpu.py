@@ -245,3 +245,30 @@ def test_library_refuses_half_a_layout():
         assert lib.gs_gated_scan_backward(ctypes.byref(args), None) == -1, layout
     args = native.WindowAttentionArgs(**{**attention, "tiles": a, "tile_starts": a})
     assert lib.gs_window_attention_workspace_size(ctypes.byref(args)) == 0
+
+
+def test_positions_end_before_32_bits_do():
+    """The last tile of a walk reaches up to 256 tokens past the last one: lengths for
+    which that position has no 32-bit number are refused."""
+    from gaussian_splats_b200 import native
+
+    lib, a, longest = native.lib(), 256, native.MAX_SEQUENCE_TOKENS
+    assert longest + 511 <= 2 ** 31 - 1
+    for tokens in (longest + 1, 2 ** 31 - 1):
+        with pytest.raises(ValueError, match="at most"):
+            PackedSequences([tokens], device="cpu")
+        args = native.WindowAttentionArgs(
+            tokens=tokens, num_tiles=-(-tokens // 128), heads=1, kv_heads=1, dim=8, dtype=1,
+            scale=0.1, q=a, k=a, v=a, q_stride=8, q_head_stride=8, k_stride=8, k_head_stride=8,
+            v_stride=8, v_head_stride=8, out=a)
+        assert lib.gs_window_attention(ctypes.byref(args), None) == -1
+        args = native.GatedScanArgs(
+            tokens=tokens, sequences=1, num_tiles=-(-tokens // 128), channels=8, dtype=1, x=a,
+            gate=a, x_stride=8, gate_stride=8, y=a, last=a, entering=a, workspace=a,
+            workspace_size=1 << 50)
+        assert lib.gs_gated_scan(ctypes.byref(args), None) == -1
+        args = native.WindowAttentionStepArgs(
+            batch=1, heads=1, kv_heads=1, dim=8, dtype=1, slots=tokens, scale=0.1, q=a, k=a, v=a,
+            q_stride=8, q_head_stride=8, k_stride=8, k_head_stride=8, v_stride=8, v_head_stride=8,
+            cache_k=a, cache_v=a, positions=a, out=a)
+        assert lib.gs_window_attention_step(ctypes.byref(args), None) == -1
