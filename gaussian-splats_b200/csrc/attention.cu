@@ -724,12 +724,12 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
     if (lane == 0 && t > 0)
       load_tile<kDim, kKeyRows>(s.tiles0[stage0], &s.full0[stage0], tile_map0, at);
     __syncwarp();
-    if constexpr (kKeyRows) {
-      wait_for(t - kStages1);
-    } else if (t >= kStages1) {  // only G read the tile that had the place before
-      const int u = t - kStages1;
-      good = good && barrier_wait_warp(shared_address(&s.grads[u & 1]), (u >> 1) & 1);
-    }
+    // Queries: only G read the tile that had operand 1's place before, and G of a tile
+    // is complete with the sum of the tile before it. (Waiting for G itself would be
+    // wrong if this warp fell two of its phases behind: their parity is the same.)
+    static_assert(kKeyRows || kStages0 == kStages1 + 1, "wait_for(t - kStages0) covers it");
+    if constexpr (kKeyRows) wait_for(t - kStages1);
+    else if (t == kStages1) wait_for(0);
     if (!good) break;
     keep(t, stage1, lane, values);
     __syncwarp();  // lane 0 has arrived at the first tile's barrier already
