@@ -69,6 +69,24 @@ constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
 // gs_window_attention_status, the block's results are not valid.
 __device__ uint32_t g_timeout;
 
+// A row's result: NaN where a wait ran out, whatever the row has seen until then, and
+// `empty` where there was nothing to see.
+constexpr float row_value(bool good, bool none, float value, float empty) {
+  return !good ? NAN : none ? empty : value;
+}
+static_assert(row_value(false, true, 0.0f, 0.0f) != row_value(false, true, 0.0f, 0.0f) &&
+                  row_value(false, false, 1.0f, 0.0f) != row_value(false, false, 1.0f, 0.0f) &&
+                  row_value(true, true, NAN, 0.0f) == 0.0f && row_value(true, false, 1.0f, 0.0f) == 1.0f,
+              "a wait that ran out shows");
+
+// After a wait that ran out, by the warp that issues products: those that it has issued
+// read shared and write tensor memory until they are complete.
+__device__ __forceinline__ void drain(uint64_t* bar) {
+  tc::commit(tc::elect_lane(), tc::shared_address(bar));
+  tc::barrier_settle(tc::shared_address(bar));
+  __syncwarp();
+}
+
 // 32 bits with those under `n` set.
 __device__ __forceinline__ uint32_t below32(int n) {
   return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
@@ -245,6 +263,7 @@ struct ForwardShared {
   uint64_t scores[2];                           // S of a group's step is complete
   uint64_t weights[2];                          // P is written (128 arrivals)
   uint64_t summed[2];                           // all of a group's sums are complete
+  uint64_t drained;                             // a wait ran out: the products that were issued
   uint32_t tensor;
 };
 
@@ -282,6 +301,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
       barrier_init(shared_address(&s.weights[g]), kTile);
       barrier_init(shared_address(&s.summed[g]), 1);
     }
+    barrier_init(shared_address(&s.drained), 1);
     for (int i = 0; i < kStages; ++i) {
       barrier_init(shared_address(&s.k_full[i]), 1);
       barrier_init(shared_address(&s.v_full[i]), 1);
@@ -316,14 +336,6 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         if (turn > 0) good = barrier_wait(shared_address(&s.v_empty[stage]), (turn - 1) & 1);
         if (!good) break;
         load(s.v[stage], &s.v_full[stage], &v_map, kv_head, tile.begin + walk.start(t), kKeys);
-      }
-      if (!good) {  // let what is in flight land before the shared memory is given back
-        for (int i = 0; i < kStages; ++i)
-          for (int p = 0; p < 2; ++p) {
-            barrier_wait(shared_address(&s.k_full[i]), p);
-            barrier_wait(shared_address(&s.v_full[i]), p);
-          }
-        atomicExch(&g_timeout, 1u);
       }
     }
     __syncwarp();
@@ -423,7 +435,6 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         run_step(Second{}, step, __shfl_sync(0xffffffffu, second, step - base));
       }
     }
-    if (!good && lane == 0) atomicExch(&g_timeout, 1u);
     __syncwarp();
   } else if (warp < 8) {
     if constexpr (kDim == 128) registers_up<Shape::kWide>();
@@ -544,7 +555,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
       fence_after_sync();
       const int64_t token = int64_t{tile.start} + group * kTile + row;
       const bool write = token < tile.end;
-      const float inverse = good ? 1.0f / sum : NAN;  // a wait that ran out shows
+      const float inverse = 1.0f / sum;
       unsigned char* rows = s.q[group];  // the products with the queries are complete
 #pragma unroll
       for (int c = 0; c < kDim; c += 32) {
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         for (int e = 0; e < 32; e += 8) {
           float v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = sum == 0.0f ? 0.0f : o[e + k] * inverse;
+          for (int k = 0; k < 8; ++k) v[k] = row_value(good, sum == 0.0f, o[e + k] * inverse, 0.0f);
           put_word<T, kDim>(rows, row, (c + e) / 8, v);
         }
       }
@@ -564,12 +575,20 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
           rows, static_cast<T*>(a.out) + ((token - row) * a.heads + head) * a.dim,
           int64_t{a.heads} * a.dim, 0, static_cast<int>(tile.end - (token - row)), a.dim, row);
       if (write && a.lse)
-        a.lse[head * a.tokens + token] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-      if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
+        a.lse[head * a.tokens + token] =
+            row_value(good, sum == 0.0f, (top + log2f(sum)) * kLn2, -INFINITY);
     }
   }
   fence_before_sync();
-  __syncthreads();
+  if (__syncthreads_or(!good)) {
+    if (warp == 8 && (threadIdx.x & 31) == 0) {
+      atomicExch(&g_timeout, 1u);
+      for (uint64_t& b : s.q_full) barrier_settle(shared_address(&b));
+      for (uint64_t& b : s.k_full) barrier_settle(shared_address(&b));
+      for (uint64_t& b : s.v_full) barrier_settle(shared_address(&b));
+    }
+    if (warp == 9) drain(&s.drained);
+  }
   if (warp == 9) tensor_free<Shape::kColumns>(tensor);
 }
 
@@ -667,6 +686,7 @@ struct BackwardShared {
   // a warp may be a tile ahead of another: even and odd tiles have one each.
   uint64_t weights[2];
   uint64_t done;     // all sums are complete
+  uint64_t drained;  // a wait ran out: the products that were issued are complete
   uint32_t tensor;
 };
 
@@ -693,9 +713,9 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, uint64_t* full,
 
 // The warp that loads what backward_setup has not. `place(t)` names the head and row of tile
 // t; `rows(t, lane)` loads what else a tile needs and `keep(t, stage, ...)` puts it
-// to shared memory, all lanes taking part; it goes with operand 1.
+// to shared memory, all lanes taking part; it goes with operand 1. False: a wait ran out.
 template <int kDim, bool kKeyRows, class Place, class Rows, class Keep>
-__device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, int tiles,
+__device__ __forceinline__ bool load_tiles(BackwardShared<kDim, kKeyRows>& s, int tiles,
                                            const CUtensorMap* tile_map0,
                                            const CUtensorMap* tile_map1, const Place& place,
                                            const Rows& rows, const Keep& keep) {
@@ -739,20 +759,14 @@ __device__ __forceinline__ void load_tiles(BackwardShared<kDim, kKeyRows>& s, in
       load_tile<kDim, kKeyRows>(s.tiles1[stage1], &s.full1[stage1], tile_map1, at);
     __syncwarp();
   }
-  if (!good) {  // let what is in flight land before the shared memory is given back
-    for (int p = 0; p < 2; ++p) {
-      for (uint64_t& b : s.full0) barrier_wait(shared_address(&b), p);
-      for (uint64_t& b : s.full1) barrier_wait(shared_address(&b), p);
-    }
-    if (lane == 0) atomicExch(&g_timeout, 1u);
-  }
   __syncwarp();
+  return good;
 }
 
 // The warp that issues the products (one elected lane of it). `sets(t)` says how many
-// sets of 32 rows tile t needs.
+// sets of 32 rows tile t needs. False: a wait ran out.
 template <class T, int kDim, bool kKeyRows, class Sets>
-__device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s, int dim,
+__device__ __forceinline__ bool issue_products(BackwardShared<kDim, kKeyRows>& s, int dim,
                                                int tiles, const Sets& sets) {
   using namespace tc;
   using Shape = BackwardShape<kDim, kKeyRows>;
@@ -841,8 +855,28 @@ __device__ __forceinline__ void issue_products(BackwardShared<kDim, kKeyRows>& s
     stage1 = next1;
     count = next_count;
   }
-  if (!good && elected) atomicExch(&g_timeout, 1u);
   __syncwarp();
+  return good;
+}
+
+// The end of a block, all threads: tensor memory is given back, after a wait that ran
+// out behind what is still in flight.
+template <int kDim, bool kKeyRows>
+__device__ __forceinline__ void backward_end(BackwardShared<kDim, kKeyRows>& s, int warp,
+                                             uint32_t tensor, bool good) {
+  using namespace tc;
+  fence_before_sync();
+  if (__syncthreads_or(!good)) {
+    if (threadIdx.x == 32 * kLoadWarp) {
+      atomicExch(&g_timeout, 1u);
+      barrier_settle(shared_address(&s.rows_full));
+      for (uint64_t& b : s.full0) barrier_settle(shared_address(&b));
+      for (uint64_t& b : s.full1) barrier_settle(shared_address(&b));
+    }
+    if (warp == kProductWarp) drain(&s.drained);
+  }
+  if (warp == kProductWarp)
+    tensor_free<BackwardShape<kDim, kKeyRows>::kColumns>(tensor);
 }
 
 // Barriers and tensor memory; the block's rows and the first tile are on their way
@@ -865,6 +899,7 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
     barrier_init(shared_address(&s.read), kComputeThreads);
     for (uint64_t& b : s.weights) barrier_init(shared_address(&b), kComputeThreads);
     barrier_init(shared_address(&s.done), 1);
+    barrier_init(shared_address(&s.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
     const uint32_t bar = shared_address(&s.rows_full);
@@ -1050,14 +1085,15 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
   backward_setup(s, warp, &q_map, &g_map, head, tile.start, &k_map, &v_map,
                  make_int2(kv_head, tile.begin + walk.start(0)));
   const uint32_t tensor = s.tensor;
+  bool good = true;
   if (warp == kLoadWarp) {
-    load_tiles<kDim, false>(
+    good = load_tiles<kDim, false>(
         s, walk.tiles, &k_map, &v_map,
         [&](int t) { return make_int2(kv_head, tile.begin + walk.start(t)); },
         [](int, int) { return 0; }, [](int, int, int, int) {});
   } else if (warp == kProductWarp) {
-    issue_products<T, kDim, false>(s, a.dim, walk.tiles,
-                                   [&](int t) { return walk.sets(0, t); });
+    good = issue_products<T, kDim, false>(s, a.dim, walk.tiles,
+                                          [&](int t) { return walk.sets(0, t); });
   } else {
     const int half = warp >> 2, row = threadIdx.x & (kTile - 1);
     const uint32_t mine = tensor + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -1073,7 +1109,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
       for (int k = threadIdx.x & 31; k < count + (walk.head_tiles > 0); k += 32)
         value_peak = fmaxf(value_peak, of[int64_t{k < count ? low + k : 0} * a.kv_heads]);
     }
-    bool good = row_products<T, kDim>(a, tile, head, s);
+    good = row_products<T, kDim>(a, tile, head, s);
     sync_compute();
     const float d = live ? s.part[row] : 0.0f;
     if (live && half == 0) delta[slot] = d;
@@ -1207,11 +1243,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, false>::
     write_rows<T, kDim, kComputeThreads>(
         rows, static_cast<T*>(a.grad_q) + (int64_t{tile.start} * a.heads + head) * a.dim,
         int64_t{a.heads} * a.dim, 0, tile.end - tile.start, a.dim, threadIdx.x);
-    if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
   }
-  fence_before_sync();
-  __syncthreads();
-  if (warp == kProductWarp) tensor_free<Shape::kColumns>(tensor);
+  backward_end(s, warp, tensor, good);
 }
 
 // The sums of first tokens' keys: `base` [sequence, kv head, first, 2 (dK, dV),
@@ -1273,6 +1306,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
   backward_setup(s, warp, &k_map, &v_map, kv_head, tile.start, &q_map, &g_map,
                  make_int2(kv_head * group, tile.begin + low));
   const uint32_t tensor = s.tensor;
+  bool good = true;
   if (warp == kLoadWarp) {
     float grow = 1.0f, value_peak = 0.0f;
     float2 peak[4] = {};  // of the lane's sets of 32 queries
@@ -1297,7 +1331,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     struct RowValues {
       float shift[kSets], delta[kSets];
     };
-    load_tiles<kDim, true>(
+    good = load_tiles<kDim, true>(
         s, tiles, &q_map, &g_map,
         [&](int t) {
           return make_int2(kv_head * group + t / per_head,
@@ -1339,7 +1373,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
           }
         });
   } else if (warp == kProductWarp) {
-    issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
+    good = issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
       return min(kSets, (high - low - (t % per_head) * kRows + 31) / 32);
     });
   } else {
@@ -1358,7 +1392,6 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
     const float scale = a.scale * kLog2e;
     const float2 factor = make_float2(scale, scale);
     const uint32_t scores = mine + 32 * kHalfSets * half, grads = scores + Shape::kGrad;
-    bool good = true;
     int stage0 = 0, stage1 = 0, parity1 = 0, index = 0;
     for (int t = 0; t < tiles; ++t) {
       const int start = low + index * kRows, first = start + 32 * kHalfSets * half;
@@ -1507,11 +1540,8 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
                 (int64_t{tile.start} * a.kv_heads + kv_head) * a.dim,
             int64_t{a.kv_heads} * a.dim, summed - j_first, n - j_first, a.dim, threadIdx.x);
     }
-    if (!good && (threadIdx.x & 31) == 0) atomicExch(&g_timeout, 1u);
   }
-  fence_before_sync();
-  __syncthreads();
-  if (warp == kProductWarp) tensor_free<Shape::kColumns>(tensor);
+  backward_end(s, warp, tensor, good);
 }
 
 // dk and dv of first tokens: their window's sum and the chunks' in order, a
@@ -1832,7 +1862,9 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
                                       ((t - 1) / kStepStages) & 1);
       if (good) load_tile(t - 1 + kStepStages);
     }
-    good = tc::barrier_wait_warp(tc::shared_address(&s.full[stage]), (t / kStepStages) & 1) && good;
+    good = __all_sync(0xffffffffu, good) &&
+           tc::barrier_wait_warp(tc::shared_address(&s.full[stage]), (t / kStepStages) & 1);
+    if (!good) break;
     const int row0 = warp * kStepSlots, base = base_of(t) + row0;
     // Keys base + g and base + 8 + g; values of the slots 2j, 2j+1, 2j+8, 2j+9.
     uint4 key[2][kChunks];
@@ -1918,9 +1950,7 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
     if (lane == 0) tc::barrier_arrive(tc::shared_address(&s.empty[stage]));
   }
   if (!good) {  // let what is in flight land, and show that the result is not valid
-    for (uint64_t& bar : s.full)
-      for (int parity = 0; parity < 2; ++parity)
-        tc::barrier_wait(tc::shared_address(&bar), parity);
+    for (uint64_t& bar : s.full) tc::barrier_settle(tc::shared_address(&bar));
     for (float& x : sum) x = NAN;
     if (lane == 0) atomicExch(&g_timeout, 1u);
   }

@@ -265,9 +265,7 @@ struct BoxSource {
   // At the end: whether all waits came back; if not, copies still in flight land first.
   __device__ __forceinline__ void finish() {
     if (good) return;
-    for (uint64_t& b : s.full)
-      for (int parity = 0; parity < 2; ++parity)
-        tc::barrier_wait(tc::shared_address(&b), parity);
+    for (uint64_t& b : s.full) tc::barrier_settle(tc::shared_address(&b));
     if (threadIdx.x == 0) atomicExch(&g_timeout, 1u);
   }
 };

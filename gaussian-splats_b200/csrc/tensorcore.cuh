@@ -29,11 +29,13 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
 }
 
 // Waits for the barrier's phase of this parity; false if it did not complete
-// within the limit (far above any wait of a working kernel, which is at most
-// a load or a few products long).
+// within the limit of tries, 1.5 us each: 1.6 s, far above any wait of a working
+// kernel, which is at most a load or a few products long. A warp whose wait ran out
+// waits no more, and the block's others run out behind it.
 constexpr int kWaitLimit = 1 << 20;
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kWaitLimit; ++i) {
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity,
+                                             int limit = kWaitLimit) {
+  for (int i = 0; i < limit; ++i) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -45,6 +47,11 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     if (done) return true;
   }
   return false;
+}
+// After a wait that ran out: time (25 ms) for what is still on its way to the
+// barrier, whichever phase that is, before the shared memory is given back.
+__device__ __forceinline__ void barrier_settle(uint32_t bar) {
+  for (uint32_t parity = 0; parity < 2; ++parity) barrier_wait(bar, parity, 1 << 14);
 }
 // The same for all threads of a warp together.
 __device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity) {
