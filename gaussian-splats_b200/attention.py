@@ -138,9 +138,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     ``packed`` says which rows form which sequence (None: all rows are one).
     ``valid`` [tokens] bool leaves keys out, e.g. of dead splats; what invalid
-    rows hold does not matter, nor does their gradient, which is zero. A non-finite
-    value of a valid key or value reaches every query that sees it, and may
-    reach others of the same sequence less than a window and 128 tokens away.
+    rows of k and v hold does not matter, and their gradient is zero. An invalid
+    token still asks: its row of q counts like any other. What a query that sees
+    nothing holds does not matter either. A non-finite value of a valid key or
+    value reaches every query that sees it, one of a query or of its output's
+    gradient the gradients of every key that it sees; both may reach others of
+    the same sequence less than a window and 128 tokens away.
     ``scale`` multiplies the scores (default ``dim ** -0.5``).
 
     bfloat16 or float16, dim a multiple of 8 up to 128; scores, softmax and

@@ -678,6 +678,7 @@ struct BackwardShared {
     };
   };
   float grow, back;  // keys: E's factor over P's, and what scales dK back
+  bool none[kStages1];  // keys: some of the tile's rows see nothing, or are not the sequence's
   uint64_t rows_full, full0[kStages0], full1[kStages1];  // loads
   uint64_t empty[kStages0];                              // a tile's sums are complete
   uint64_t scores, grads[2];  // S, G of a tile are complete
@@ -1364,13 +1365,17 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
             }
           }
           const int i = low + (t % per_head) * kRows + lane;
+          bool none = false;
 #pragma unroll
           for (int k = 0; k < kSets; ++k) {
             const bool in = i + 32 * k < n;
+            none = none || !in || v.shift[k] == -INFINITY;
             s.row[stage][0][lane + 32 * k] =
                 in ? power - weight_shift(v.shift[k]) : -INFINITY;
             s.row[stage][1][lane + 32 * k] = in ? -v.delta[k] * grow : 0.0f;
           }
+          none = __any_sync(0xffffffffu, none);
+          if (lane == 0) s.none[stage] = none;
         });
   } else if (warp == kProductWarp) {
     good = issue_products<T, kDim, true>(s, a.dim, tiles, [&](int t) {
@@ -1408,6 +1413,7 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
                    barrier_wait_warp(shared_address(&s.full1[stage1]), parity1)))
         break;
       fence_after_sync();
+      const bool none = !whole && s.none[stage1];
       float x[kHalfSets][32];
       if (any_seen) {
 #pragma unroll
@@ -1444,11 +1450,13 @@ __global__ void __launch_bounds__(kBackwardThreads, BackwardShape<kDim, true>::k
           }
           store_columns16(scores + 32 * h, packed);
         }
-      if (start + kRows > n) {
-        const int rest = n - start;
+      // No gradient flows through a query that sees nothing: what it and its gradient
+      // hold must not meet its weights of zero, nor what the next sequence's rows do.
+      if (none) {
         uint32_t keep[kSets];
 #pragma unroll
-        for (int c = 0; c < kSets; ++c) keep[c] = below32(rest - 32 * c);
+        for (int c = 0; c < kSets; ++c)
+          keep[c] = __ballot_sync(0xffffffffu, s.row[stage1][0][lane_id() + 32 * c] != -INFINITY);
         zero_rows<kDim, kRows, kComputeThreads>(s.tiles0[stage0], keep, threadIdx.x);
         zero_rows<kDim, kRows, kComputeThreads>(s.tiles1[stage1], keep, threadIdx.x);
         fence_async_shared();

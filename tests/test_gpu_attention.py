@@ -391,3 +391,21 @@ def test_float16_gradients_of_one_query_leave_the_others_theirs():
         assert torch.isfinite(got[name]).all()
         assert torch.equal(got[name][:400], clean[name][:400]), name
         assert torch.equal(got[name][900:], clean[name][900:]), name
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_that_see_nothing_may_hold_anything(dim, bad):
+    """A run of dead tokens longer than the window: those inside it see nothing, and no
+    gradient flows through them, whatever they and their output's gradient hold."""
+    q, k, v, grad, _ = make([500], 4, 2, dim, torch.bfloat16)
+    valid = torch.ones(500, dtype=torch.bool, device="cuda")
+    valid[200:240] = False
+    window = dict(left=6, right=3, valid=valid)
+    clean = call(q, k, v, grad, [500], **window)
+    q, grad = q.clone(), grad.clone()
+    q[206:237], grad[206:237] = bad, bad
+    got = call(q, k, v, grad, [500], **window)
+    for name in got:
+        assert torch.equal(got[name], clean[name]), name
+    assert torch.count_nonzero(got["dq"][206:237]) == 0
