@@ -188,7 +188,9 @@ def window_cache(batch: int, left: int, first: int, kv_heads: int, dim: int,
 
 def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           cache_k: torch.Tensor, cache_v: torch.Tensor, positions: torch.Tensor,
-                          *, first: int = 0, scale: float | None = None) -> torch.Tensor:
+                          *, first: int = 0, scale: float | None = None,
+                          valid: torch.Tensor | None = None,
+                          cache_valid: torch.Tensor | None = None) -> torch.Tensor:
     """One new token of each stream: writes ``k`` and ``v`` [batch, kv_heads,
     dim] to the caches [batch, slots, kv_heads, dim] in place and returns the
     attention of ``q`` [batch, heads, dim] over what the caches then hold, the
@@ -199,10 +201,15 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     from zero; -1 marks an idle stream (zeros come back, its cache is left
     alone). Token ``p`` goes to slot ``p`` while ``p < first`` and then to
     ``first + (p - first) % (slots - first)``, so a stream's tokens must come in
-    order. No gradient."""
+    order.
+
+    ``cache_valid`` [batch, slots] bool leaves slots out as
+    :func:`window_attention`'s ``valid`` leaves keys out (None: none are); it goes
+    with the caches and is updated in place from ``valid`` [batch] bool, which says
+    whether the new tokens may be seen (None: all may). No gradient."""
     what = "window_attention_step"
     device = check_cuda(what, q=q, k=k, v=v, cache_k=cache_k, cache_v=cache_v,
-                        positions=positions)
+                        positions=positions, valid=valid, cache_valid=cache_valid)
     dtype = _heads(what, q, k, v, "batch")
     batch, heads, dim = q.shape
     shape = tuple(cache_k.shape)
@@ -227,6 +234,18 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if positions.dtype != torch.int64 or positions.shape != (batch,):
         raise ValueError(f"{what}: positions must be int64 [{batch}], got {positions.dtype} "
                          f"{tuple(positions.shape)}")
+    if cache_valid is None and valid is not None:
+        raise ValueError(f"{what}: valid without cache_valid, which keeps it for the later tokens")
+    if cache_valid is not None and (cache_valid.dtype != torch.bool or
+                                    tuple(cache_valid.shape) != shape[:2] or
+                                    not cache_valid.is_contiguous()):
+        raise ValueError(f"{what}: cache_valid must be a contiguous bool tensor {shape[:2]}, got "
+                         f"{cache_valid.dtype} {tuple(cache_valid.shape)}")
+    if valid is not None:
+        if valid.dtype != torch.bool or valid.shape != (batch,):
+            raise ValueError(f"{what}: valid must be bool [{batch}], got {valid.dtype} "
+                             f"{tuple(valid.shape)}")
+        valid = valid.contiguous()
     positions = positions.contiguous()
     q, k, v = _strided(q), _strided(k), _strided(v)
     out = q.new_empty((batch, heads, dim))
@@ -234,6 +253,6 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       kv_heads=k.shape[1], dim=dim, dtype=dtype, slots=shape[1], first=first,
                       scale=_scale(what, scale, dim), cache_k=cache_k.data_ptr(),
                       cache_v=cache_v.data_ptr(), positions=positions.data_ptr(),
-                      out=out.data_ptr())
+                      out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid))
     call("gs_window_attention_step", device, ctypes.byref(args))
     return out

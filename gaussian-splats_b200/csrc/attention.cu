@@ -1771,7 +1771,8 @@ __device__ __forceinline__ float read_block(const float* p, uint32_t rank) {
   return x;
 }
 
-template <class T, int kDim, int kHalves>
+// kMasked: with validity of the slots (3% more time).
+template <class T, int kDim, int kHalves, bool kMasked>
 __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
     attention_step_kernel(gs_window_attention_step_args a, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map) {
@@ -1802,7 +1803,12 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
   T* cache_v = static_cast<T*>(a.cache_v) + b * a.slots * row + kv_head * a.dim;
   const T* k = static_cast<const T*>(a.k) + b * a.k_stride + kv_head * a.k_head_stride;
   const T* v = static_cast<const T*>(a.v) + b * a.v_stride + kv_head * a.v_head_stride;
-  // The new token's slot is read by nobody: its rows come from the arguments.
+  // The new token's slot is read by nobody: its rows and its validity come from the
+  // arguments.
+  uint8_t* const slots_valid = kMasked ? a.cache_valid + b * a.slots : nullptr;
+  const bool token_valid = !kMasked || !a.valid || a.valid[b];
+  if (kMasked && !idle && rank == 0 && piece == 0 && kv_head == 0 && threadIdx.x == 0)
+    slots_valid[slot] = token_valid;
   if (!idle && rank == 0 && piece == 0)
     for (int c = threadIdx.x; c < a.dim; c += kStepThreads) {
       cache_k[slot * row + c] = k[c];
@@ -1870,10 +1876,18 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
                                       ((t - 1) / kStepStages) & 1);
       if (good) load_tile(t - 1 + kStepStages);
     }
+    const int row0 = warp * kStepSlots, base = base_of(t) + row0;
+    // Which of the lane's slots, 2j, 2j+1, 2j+8 and 2j+9, may be seen.
+    bool seen[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int at = base + 2 * j + (m & 1) + 8 * (m >> 1);
+      seen[m] = at < count;
+      if (kMasked && seen[m]) seen[m] = at == slot ? token_valid : slots_valid[at] != 0;
+    }
     good = __all_sync(0xffffffffu, good) &&
            tc::barrier_wait_warp(tc::shared_address(&s.full[stage]), (t / kStepStages) & 1);
     if (!good) break;
-    const int row0 = warp * kStepSlots, base = base_of(t) + row0;
     // Keys base + g and base + 8 + g; values of the slots 2j, 2j+1, 2j+8, 2j+9.
     uint4 key[2][kChunks];
 #pragma unroll
@@ -1901,7 +1915,7 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
       for (int r = 0; r < kHalves; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (base + 8 * n + 2 * j + e >= count) x[n][r][e] = -INFINITY;
+          if (!seen[2 * n + e]) x[n][r][e] = -INFINITY;
     uint32_t p[kHalves][2];
 #pragma unroll
     for (int r = 0; r < kHalves; ++r) {
@@ -1937,10 +1951,10 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
       for (int n = 0; n < 4; ++n) {
         const int r = 2 * j + (n & 1) + 8 * (n >> 1);
         value[n] = tile_word(s.v[stage], row0 + r, 8 * h + g);
-        // What an empty slot holds must not meet its weight of zero.
+        // What an empty slot, or one left out, holds must not meet its weight of zero.
         if (base + r == slot && 64 * h + 8 * g < a.dim)
           value[n] = *reinterpret_cast<const uint4*>(v + 64 * h + 8 * g);
-        if (base + r >= count) value[n] = make_uint4(0, 0, 0, 0);
+        if (!seen[n]) value[n] = make_uint4(0, 0, 0, 0);
       }
       const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&value[0]);
       const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&value[1]);
@@ -2037,7 +2051,7 @@ int step_blocks(const gs_window_attention_step_args& a, int64_t items) {
   return blocks;
 }
 
-template <class T, int kDim, int kHalves>
+template <class T, int kDim, int kHalves, bool kMasked>
 int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kHalves);
   const int blocks = step_blocks(a, items);
@@ -2049,7 +2063,7 @@ int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   GS_TRY(tc::encode_heads(&v, a.dtype, a.cache_v, a.batch * a.slots, a.kv_heads, a.dim, row, a.dim,
                           kStepTile));
   constexpr size_t kShared = sizeof(StepShared<kDim, kHalves>);
-  GS_TRY((allow_shared<attention_step_kernel<T, kDim, kHalves>>(kShared, true)));
+  GS_TRY((allow_shared<attention_step_kernel<T, kDim, kHalves, kMasked>>(kShared, true)));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -2063,7 +2077,7 @@ int32_t step(const gs_window_attention_step_args& a, cudaStream_t stream) {
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, attention_step_kernel<T, kDim, kHalves>, a, k, v);
+  cudaLaunchKernelEx(&config, attention_step_kernel<T, kDim, kHalves, kMasked>, a, k, v);
   return check_launch();
 }
 
@@ -2144,7 +2158,8 @@ int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cud
       !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
   if (a.batch == 0) return GS_OK;
-  if (!a.q || !a.k || !a.v || !a.cache_k || !a.cache_v || !a.positions || !a.out)
+  if (!a.q || !a.k || !a.v || !a.cache_k || !a.cache_v || !a.positions || !a.out ||
+      (a.valid && !a.cache_valid))
     return GS_ERR_INVALID_ARGUMENT;
   if (!strided16(a.q, a.q_stride, a.q_head_stride) ||
       !strided16(a.k, a.k_stride, a.k_head_stride) ||
@@ -2153,9 +2168,15 @@ int32_t launch_window_attention_step(const gs_window_attention_step_args& a, cud
     return GS_ERR_MISALIGNED;
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.heads / a.kv_heads <= 8)
-      return a.dim <= 64 ? step<T, 64, 1>(a, stream) : step<T, 128, 1>(a, stream);
-    return a.dim <= 64 ? step<T, 64, 2>(a, stream) : step<T, 128, 2>(a, stream);
+    const auto shaped = [&](auto masked) {
+      constexpr bool kMasked = decltype(masked)::value;
+      if (a.heads / a.kv_heads <= 8)
+        return a.dim <= 64 ? step<T, 64, 1, kMasked>(a, stream)
+                           : step<T, 128, 1, kMasked>(a, stream);
+      return a.dim <= 64 ? step<T, 64, 2, kMasked>(a, stream)
+                         : step<T, 128, 2, kMasked>(a, stream);
+    };
+    return a.cache_valid ? shaped(std::true_type{}) : shaped(std::false_type{});
   });
 }
 

@@ -215,7 +215,7 @@ class WindowAttentionStepArgs(ctypes.Structure):
                 _fields(ctypes.c_float, "scale") + _fields(ctypes.c_void_p, "q k v") +
                 _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "
                                         "v_head_stride") +
-                _fields(ctypes.c_void_p, "cache_k cache_v positions out"))
+                _fields(ctypes.c_void_p, "cache_k cache_v positions out valid cache_valid"))
 
 
 class GatedScanArgs(ctypes.Structure):

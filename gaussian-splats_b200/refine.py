@@ -54,6 +54,11 @@ def morton_order(points: torch.Tensor, bits: int = 16) -> torch.Tensor:
     return torch.argsort(code, stable=True)
 
 
+def _alive(splats: GaussianSplat) -> torch.Tensor:
+    """Which splats the others' attention may see."""
+    return splats.opacity.detach()[:, 0].sigmoid() >= _DEAD_OPACITY
+
+
 class _Product(nn.Linear):
     """A bfloat16 linear layer that can be switched to 8-bit products."""
 
@@ -124,9 +129,10 @@ class _Block(nn.Module):
         x, _ = gated_scan(*mix.chunk(2, -1), packed)
         return self.mix_out(x), residual
 
-    def step(self, x, residual, positions, cache, state):
+    def step(self, x, residual, positions, cache, state, valid, cache_valid):
         qkv, residual = self._normed(x, residual, self.norm_attend, self.qkv)
-        x = window_attention_step(*self._heads(qkv), *cache, positions, first=self.shape.first)
+        x = window_attention_step(*self._heads(qkv), *cache, positions, first=self.shape.first,
+                                  valid=valid, cache_valid=cache_valid)
         x = self.attend_out(x.flatten(1))
         mix, residual = self._normed(x, residual, self.norm_mix, self.mix)
         x = gated_scan_step(*mix.chunk(2, -1), state)
@@ -180,9 +186,8 @@ class SplatRefiner(nn.Module):
             order = morton_order(splats.mean)
             orders.append((features, order))
             tokens += [self.scene, self.embed(features[order])]
-            opacity = splats.opacity.detach()[order, 0].sigmoid()
-            alive += [torch.ones(first, dtype=torch.bool, device=opacity.device),
-                      opacity >= _DEAD_OPACITY]
+            alive += [torch.ones(first, dtype=torch.bool, device=order.device),
+                      _alive(splats)[order]]
         packed = PackedSequences([first + len(order) for _, order in orders],
                                  device=self.scene.device)
         residual, valid = torch.cat(tokens), torch.cat(alive)
@@ -211,19 +216,20 @@ class SplatRefiner(nn.Module):
         if self.shape.right:
             raise ValueError("only a causal refiner (right=0) takes splats one by one")
         s, device = self.shape, self.scene.device
-        state = {"length": 0, "blocks": [
+        alive = torch.zeros(batch, s.first + s.left + 1, dtype=torch.bool, device=device)
+        state = {"length": 0, "alive": alive, "blocks": [
             (window_cache(batch, s.left, s.first, s.kv_heads, block.dim, device=device),
              torch.zeros(batch, s.width, device=device)) for block in self.blocks]}
         for token in self.scene:
-            self._advance(token.expand(batch, -1).contiguous(), state)
+            self._advance(token.expand(batch, -1).contiguous(), None, state)
         return state
 
-    def _advance(self, residual, state):
+    def _advance(self, residual, alive, state):
         positions = torch.full((len(residual),), state["length"], dtype=torch.int64,
                                device=residual.device)
         x = torch.zeros(residual.shape, dtype=torch.bfloat16, device=residual.device)
         for block, (cache, scan) in zip(self.blocks, state["blocks"]):
-            x, residual = block.step(x, residual, positions, cache, scan)
+            x, residual = block.step(x, residual, positions, cache, scan, alive, state["alive"])
         state["length"] += 1
         return x, residual
 
@@ -232,5 +238,5 @@ class SplatRefiner(nn.Module):
         """The refined parameters of one new splat of each stream (``splats`` holds
         one a stream), given those that came before it; advances ``state``."""
         features = self._features(splats)
-        x, residual = self._advance(self.embed(features), state)
+        x, residual = self._advance(self.embed(features), _alive(splats), state)
         return self._unpack(features + self._update(x, residual))

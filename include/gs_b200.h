@@ -543,7 +543,10 @@ int32_t gs_window_attention_status(gs_stream_t stream);
  * [batch, slots, kv_heads, dim] contiguous. Writes k and v to their slot
  * (position < first ? position : first + (position - first) % (slots -
  * first)), then attends over the min(position + 1, slots) tokens that the
- * cache holds: a window of left = slots - first - 1. */
+ * cache holds: a window of left = slots - first - 1. cache_valid [batch, slots]
+ * uint8 (may be NULL: all are) says which slots' keys may be seen, as `valid` does
+ * above: the token's byte, valid[batch] (NULL: 1), goes to its slot with it, and
+ * slots of 0 are left out, whatever they hold. */
 typedef struct gs_window_attention_step_args {
   int64_t batch;
   int32_t heads, kv_heads, dim, dtype, slots, first;
@@ -553,6 +556,8 @@ typedef struct gs_window_attention_step_args {
   void *cache_k, *cache_v;
   const int64_t *positions;
   void *out;
+  const uint8_t *valid;
+  uint8_t *cache_valid;
 } gs_window_attention_step_args;
 
 int32_t gs_window_attention_step(const gs_window_attention_step_args *args, gs_stream_t stream);

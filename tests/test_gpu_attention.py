@@ -409,3 +409,74 @@ def test_queries_that_see_nothing_may_hold_anything(dim, bad):
     for name in got:
         assert torch.equal(got[name], clean[name]), name
     assert torch.count_nonzero(got["dq"][206:237]) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("case", STEPS, ids=str)
+def test_step_leaves_slots_out(case, dtype):
+    """Slots that are not valid, the new token's own among them, whatever they hold."""
+    from gaussian_splats_b200.attention import window_attention_step
+
+    batch, heads, kv_heads, dim, left, first = case
+    g = torch.Generator(device="cuda").manual_seed(2)
+    slots, rand = first + left + 1, lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    q, k, v = rand(batch, heads, dim), rand(batch, kv_heads, dim), rand(batch, kv_heads, dim)
+    cache_k, cache_v = rand(batch, slots, kv_heads, dim), rand(batch, slots, kv_heads, dim)
+    positions = torch.randint(0, 3 * slots, (batch,), generator=g, device="cuda")
+    if batch > 4:
+        positions[1], positions[2] = -1, 0
+    seen = torch.rand(batch, slots, generator=g, device="cuda") > 0.4
+    valid = torch.rand(batch, generator=g, device="cuda") > 0.5
+    seen[-1] = False  # nothing but the token itself, or not even that
+    at, expected = positions.tolist(), seen.clone()
+    for b, p in enumerate(at):
+        if p >= 0:
+            expected[b, p if p < first else first + (p - first) % (left + 1)] = valid[b]
+    for t in (cache_k, cache_v):
+        t[~seen] = float("nan")
+    bad = ~valid[:, None, None]
+    k, v = torch.where(bad, float("inf"), k), torch.where(bad, float("nan"), v)
+    cache_valid = seen.clone()
+    out = window_attention_step(q, k, v, cache_k, cache_v, positions, first=first, valid=valid,
+                                cache_valid=cache_valid)
+    assert torch.equal(cache_valid, expected)
+    for b, p in enumerate(at):
+        keys = expected[b].clone()
+        keys[max(p + 1, 0):] = False
+        if p < 0 or not keys.any():
+            assert torch.count_nonzero(out[b]) == 0, b
+            continue
+        kk, vv = (t[b, keys].double().repeat_interleave(heads // kv_heads, 1)
+                  for t in (cache_k, cache_v))
+        w = (torch.einsum("hd,nhd->hn", q[b].double(), kk) * dim ** -0.5).softmax(1)
+        o, spread = torch.einsum("hn,nhd->hd", w, vv), torch.einsum("hn,nhd->hd", w, vv.abs())
+        bound = 1.25 * U[dtype] * (o.abs() + spread) + 1e-5 + TINY[dtype] * len(kk) * 6.0
+        assert ((out[b].double() - o).abs() <= bound).all(), b
+
+
+def test_step_without_valid_fills_cache_valid():
+    from gaussian_splats_b200.attention import window_attention_step, window_cache
+
+    q, k, v, _, _ = make([3], 2, 2, 64, torch.bfloat16)
+    cache, positions = window_cache(3, 4, 1, 2, 64), torch.tensor([0, -1, 7], device="cuda")
+    seen = torch.zeros(3, 6, dtype=torch.bool, device="cuda")
+    out = window_attention_step(q, k, v, *cache, positions, first=1, cache_valid=seen)
+    assert seen.nonzero().tolist() == [[0, 0], [2, 2]]
+    assert torch.equal(out[0], v[0]) and torch.equal(out[2], v[2])
+
+
+def test_step_refuses_validity_that_does_not_fit():
+    from gaussian_splats_b200.attention import window_attention_step, window_cache
+
+    q, k, v, _, _ = make([3], 2, 2, 64, torch.bfloat16)
+    cache, at = window_cache(3, 4, 1, 2, 64), torch.zeros(3, dtype=torch.int64, device="cuda")
+    seen = torch.ones(3, 6, dtype=torch.bool, device="cuda")
+    for match, valid, cache_valid in [
+        ("without cache_valid", seen[:, 0], None), ("valid must be bool", seen[:2, 0], seen),
+        ("valid must be bool", at, seen), ("cache_valid must be", seen[:, 0], seen[:, :5]),
+        ("cache_valid must be", None, seen.int()),
+        ("cache_valid must be", None, seen.t().contiguous().t()),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            window_attention_step(q, k, v, *cache, at, first=1, valid=valid,
+                                  cache_valid=cache_valid)

@@ -138,3 +138,24 @@ def test_refusals():
         SplatRefiner(sh_degree=1)([scene(10, 0)])
     with pytest.raises(ValueError, match="causal"):
         SplatRefiner().stream(1)
+
+
+def test_stream_follows_a_scene_with_dead_splats():
+    """A causal refiner is one model: dead splats are no keys in either form."""
+    from gaussian_splats_b200.refine import morton_order
+
+    torch.manual_seed(0)
+    shape = RefinerShape(width=128, heads=2, kv_heads=1, left=16, right=0, first=3)
+    refiner = shaken(SplatRefiner(shape=shape))
+    splats = scene(90, 5, dead=40)
+    with torch.no_grad():
+        splats.mean[:40] *= 30  # far out: keys that would be seen, were they seen
+        whole = refiner([splats])[0]
+        state = refiner.stream(2)
+        for at in morton_order(splats.mean).tolist():
+            one = GaussianSplat.from_tensors(*(getattr(splats, n)[at:at + 1].detach().expand(
+                2, *getattr(splats, n).shape[1:]).contiguous()
+                for n in ("mean", "rotation", "scale", "opacity", "color")))
+            out = refiner.step(one, state)
+            for name in whole:
+                torch.testing.assert_close(out[name][0], whole[name][at], rtol=0, atol=3e-2)

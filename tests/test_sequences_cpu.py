@@ -272,3 +272,14 @@ def test_positions_end_before_32_bits_do():
             q_stride=8, q_head_stride=8, k_stride=8, k_head_stride=8, v_stride=8, v_head_stride=8,
             cache_k=a, cache_v=a, positions=a, out=a)
         assert lib.gs_window_attention_step(ctypes.byref(args), None) == -1
+
+
+def test_library_refuses_validity_without_a_place_for_it():
+    from gaussian_splats_b200 import native
+
+    a = 256
+    args = native.WindowAttentionStepArgs(
+        batch=1, heads=1, kv_heads=1, dim=8, dtype=1, slots=4, scale=0.1, q=a, k=a, v=a, q_stride=8,
+        q_head_stride=8, k_stride=8, k_head_stride=8, v_stride=8, v_head_stride=8, cache_k=a,
+        cache_v=a, positions=a, out=a, valid=a)
+    assert native.lib().gs_window_attention_step(ctypes.byref(args), None) == -1
