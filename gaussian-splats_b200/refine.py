@@ -64,15 +64,25 @@ class _Product(nn.Linear):
 
     def __init__(self, inputs: int, outputs: int, device=None):
         super().__init__(inputs, outputs, bias=False, device=device, dtype=torch.bfloat16)
-        self.codes = self.scales = None
+        # Made from the weight: they move with the module, but are not saved.
+        self.register_buffer("codes", None, persistent=False)
+        self.register_buffer("scales", None, persistent=False)
+        self.rounded = None
+
+    def _changes(self) -> int | None:
+        """The count of the weight's changes in place (inference tensors have none)."""
+        return None if self.weight.is_inference() else self.weight._version
 
     def quantize(self) -> None:
-        """e4m3 weights with one scale an output."""
+        """e4m3 weights with one scale an output, of the weight as it is now."""
+        self.rounded = self._changes()
         w = self.weight.detach().float()
         self.scales = (w.abs().amax(1) / 448.0).clamp(min=1e-12)
         self.codes = (w / self.scales[:, None]).to(torch.float8_e4m3fn)
 
     def eight_bit(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        if self.rounded != self._changes():  # an optimizer's step, a loaded checkpoint
+            self.quantize()
         return torch._scaled_mm(codes, self.codes.t(), scale[:, None], self.scales[None],
                                 out_dtype=torch.bfloat16)
 
@@ -159,7 +169,9 @@ class SplatRefiner(nn.Module):
 
     def quantize(self) -> None:
         """Switches the products behind a norm to 8 bits for calls without
-        gradients (their weights are rounded here; training goes on in bfloat16)."""
+        gradients. Their weights are rounded here, and again by the first such call
+        after they have changed in place; training goes on in bfloat16, and what
+        ``state_dict`` saves is the bfloat16 weights."""
         for block in self.blocks:
             block.qkv.quantize()
             block.mix.quantize()

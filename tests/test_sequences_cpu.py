@@ -283,3 +283,35 @@ def test_library_refuses_validity_without_a_place_for_it():
         q_head_stride=8, k_stride=8, k_head_stride=8, v_stride=8, v_head_stride=8, cache_k=a,
         cache_v=a, positions=a, out=a, valid=a)
     assert native.lib().gs_window_attention_step(ctypes.byref(args), None) == -1
+
+
+def test_eight_bit_weights_follow_the_weights(monkeypatch):
+    """After further training or a loaded checkpoint the codes are those of the new
+    weights; they move with the module and are not saved."""
+    from gaussian_splats_b200.refine import _Product
+
+    used = []
+    monkeypatch.setattr(torch, "_scaled_mm", lambda a, b, sa, sb, out_dtype: used.append(
+        b.float() * sb))
+    x, scale = torch.zeros(4, 32).to(torch.float8_e4m3fn), torch.ones(4)
+    p = _Product(32, 48)
+    names = set(p.state_dict())
+    p.quantize()
+    codes = p.codes
+    p.eight_bit(x, scale)
+    assert p.codes is codes  # not rounded again without need
+    optimizer = torch.optim.SGD(p.parameters(), lr=1.0)
+    p.weight.grad = torch.randn_like(p.weight)
+    optimizer.step()
+    p.eight_bit(x, scale)
+    other = _Product(32, 48)
+    p.load_state_dict(other.state_dict())
+    p.eight_bit(x, scale)
+    for got, weight in ((used[1], None), (used[2], other.weight)):
+        if weight is not None:  # half a step of e4m3 (2**-4), or half its smallest (2**-10)
+            w = weight.detach().float().t()
+            assert ((got - w).abs() <= 1.01 * torch.maximum(
+                w.abs() * 2.0 ** -4, w.abs().amax(0) / 448 * 2.0 ** -10)).all()
+        assert not torch.equal(got, used[0])
+    assert set(p.state_dict()) == names
+    assert p.to("meta").codes.is_meta and p.scales.is_meta
