@@ -25,8 +25,8 @@ import math
 import torch
 
 from . import native
-from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
-                        check_tokens, tile_arguments)
+from .sequences import (PackedSequences, address, call, changed_in_place, check_cuda,
+                        check_packed, check_tokens, element_type, tile_arguments)
 
 MAX_HEAD_DIM = 128
 _TYPES = (torch.bfloat16, torch.float16)
@@ -255,4 +255,5 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       cache_v=cache_v.data_ptr(), positions=positions.data_ptr(),
                       out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid))
     call("gs_window_attention_step", device, ctypes.byref(args))
+    changed_in_place(cache_k, cache_v, cache_valid)
     return out

@@ -16,8 +16,8 @@ import ctypes
 import torch
 
 from . import native
-from .sequences import (PackedSequences, address, call, check_cuda, check_packed, element_type,
-                        check_tokens, tile_arguments)
+from .sequences import (PackedSequences, address, call, changed_in_place, check_cuda,
+                        check_packed, check_tokens, element_type, tile_arguments)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -128,4 +128,5 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor) ->
     y = x.new_empty(x.shape)
     call("gs_gated_scan_step", device, x.shape[0], x.shape[1], dtype, address(x), x.stride(0),
          address(gate), gate.stride(0), address(state), address(y))
+    changed_in_place(state)
     return y

@@ -107,6 +107,12 @@ def call(name: str, device: torch.device, *arguments) -> None:
         native.check(status, name)
 
 
+def changed_in_place(*tensors: torch.Tensor | None) -> None:
+    """Tells autograd that a library call wrote to tensors of its caller: a graph
+    that saved one before then refuses its backward instead of using what is there now."""
+    torch.autograd.graph.increment_version(tuple(t for t in tensors if t is not None))
+
+
 def address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -315,3 +315,28 @@ def test_eight_bit_weights_follow_the_weights(monkeypatch):
         assert not torch.equal(got, used[0])
     assert set(p.state_dict()) == names
     assert p.to("meta").codes.is_meta and p.scales.is_meta
+
+
+def test_steps_tell_autograd_what_they_write(monkeypatch):
+    """A graph that saved a cache or a state must not go on with what a step wrote."""
+    from gaussian_splats_b200 import attention, recurrence
+
+    for module in (attention, recurrence):
+        monkeypatch.setattr(module, "call", lambda *arguments: None)
+        monkeypatch.setattr(module, "check_cuda", lambda what, **tensors: torch.device("cpu"))
+    h = torch.zeros(4, 1, 8, dtype=torch.bfloat16)
+    k, v = torch.zeros(4, 5, 1, 8, dtype=torch.bfloat16), torch.zeros(4, 5, 1, 8, dtype=torch.bfloat16)
+    seen, state, x = torch.zeros(4, 5, dtype=torch.bool), torch.zeros(4, 8), torch.zeros(4, 8)
+    at = torch.zeros(4, dtype=torch.int64)
+    for written, step in (
+            ([k, v, seen], lambda: attention.window_attention_step(h, h, h, k, v, at,
+                                                                   cache_valid=seen)),
+            ([k, v], lambda: attention.window_attention_step(h, h, h, k, v, at)),
+            ([state], lambda: recurrence.gated_scan_step(x, x, state))):
+        for t in written:
+            factor = torch.ones_like(t, dtype=torch.float32, requires_grad=True)
+            product = factor * t  # saves t
+            with torch.no_grad():
+                step()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                product.sum().backward()
