@@ -50,9 +50,14 @@ class PackedSequences:
         self.tiles = table.to(torch.int32).to(self.device)
         self.tile_starts = starts.to(torch.int32).to(self.device)
         self.num_tiles = len(sequence)
+        self._stream = _raw_stream(self.device)
 
     def __len__(self) -> int:
         return len(self.lengths)
+
+
+def _raw_stream(device: torch.device) -> int | None:
+    return torch._C._cuda_getCurrentRawStream(device.index) if device.type == "cuda" else None
 
 
 def check_tokens(tokens: int, what: str) -> None:
@@ -79,6 +84,11 @@ def tile_arguments(packed: PackedSequences | None, tokens: int) -> dict:
     are one sequence and its tiles follow from their number."""
     if packed is None:
         return {"sequences": 1, "num_tiles": -(-tokens // native.SEQUENCE_TILE)}
+    if packed._stream != _raw_stream(packed.device):
+        # A caller cannot know of these tables: their memory is kept until this
+        # stream's work is done, also if the layout is dropped before.
+        for table in (packed.tiles, packed.tile_starts):
+            table.record_stream(torch.cuda.current_stream(packed.device))
     return {"sequences": len(packed), "num_tiles": packed.num_tiles,
             "tiles": packed.tiles.data_ptr() if packed.num_tiles else None,
             "tile_starts": packed.tile_starts.data_ptr()}

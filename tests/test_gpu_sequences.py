@@ -63,3 +63,25 @@ def test_saved_tensors_kept_on_the_host(name, pinned):
         outputs = function(*inputs)
     got = [*outputs, *torch.autograd.grad(outputs, inputs, grads)]
     assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+def test_a_layout_dropped_while_another_stream_reads_it():
+    """The tables' memory is not given out again before that stream is done."""
+    from gaussian_splats_b200.recurrence import gated_scan
+    from gaussian_splats_b200.sequences import PackedSequences
+
+    x = torch.randn(700, 64, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    packed = PackedSequences([300, 400])
+    sizes = [(t.data_ptr(), t.numel()) for t in (packed.tiles, packed.tile_starts)]
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)  # 0.1 s
+        y, _ = gated_scan(x, x, packed)
+    del packed
+    for pointer, numel in sizes:
+        others = [torch.empty(numel, dtype=torch.int32, device="cuda") for _ in range(50)]
+        assert all(t.data_ptr() != pointer for t in others)
+    assert not stream.query(), "the stream was done before the test was"
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(y, gated_scan(x, x, PackedSequences([300, 400]))[0])
