@@ -85,3 +85,64 @@ def test_a_layout_dropped_while_another_stream_reads_it():
     assert not stream.query(), "the stream was done before the test was"
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(y, gated_scan(x, x, PackedSequences([300, 400]))[0])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_captured_in_a_graph(name):
+    """A pass, forward and backward, is captured and gives the same again."""
+    function, inputs, grads = operators()[name]
+    expected = [t.detach().clone() for t in run(function, inputs, grads)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(function, inputs, grads)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outputs = run(function, inputs, grads)
+    for _ in range(2):
+        with torch.no_grad():
+            for t in outputs:
+                t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outputs, expected))
+
+
+def test_steps_captured_in_a_graph():
+    """Single-token forms: replays advance the cache and the state in place."""
+    from gaussian_splats_b200.attention import window_attention_step, window_cache
+    from gaussian_splats_b200.norm import rms_norm_e4m3
+    from gaussian_splats_b200.recurrence import gated_scan_step
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    tokens = rand(12, 3, 4, 64).to(torch.bfloat16)
+    weight = torch.ones(64, device="cuda")
+
+    def fresh():
+        return (*window_cache(3, 6, 1, 2, 64), torch.zeros(3, 256, device="cuda"),
+                torch.zeros(3, dtype=torch.int64, device="cuda"), tokens[0].clone())
+
+    def step(cache_k, cache_v, state, positions, token):
+        out = window_attention_step(token, token[:, :2], token[:, 2:], cache_k, cache_v, positions,
+                                    first=1)
+        y = gated_scan_step(token.flatten(1), out.flatten(1), state)
+        positions += 1
+        return out, y, *rms_norm_e4m3(out, weight)
+
+    eager, called = fresh(), []
+    for t in tokens:
+        eager[4].copy_(t)
+        called.append([x.clone() for x in step(*eager)])
+    held = fresh()
+    step(*held)  # warm
+    for a, b in zip(held, fresh()):
+        a.copy_(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step(*held)
+    for t, expected in zip(tokens, called):
+        held[4].copy_(t)
+        graph.replay()
+        for a, b in zip(results, expected):
+            assert torch.equal(a.float(), b.float())
