@@ -304,13 +304,15 @@ inline int32_t encode(CUtensorMap* map, int32_t dtype, const void* base, int axe
                               const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode call = nullptr;
+  static std::atomic<Encode> found_before{nullptr};  // threads may come here side by side
+  Encode call = found_before.load(std::memory_order_acquire);
   if (!call) {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult found;
     GS_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
     if (found != cudaDriverEntryPointSuccess || !f) return GS_ERR_UNSUPPORTED;
     call = reinterpret_cast<Encode>(f);
+    found_before.store(call, std::memory_order_release);
   }
   const CUtensorMapDataType type = dtype == GS_FLOAT32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == GS_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16

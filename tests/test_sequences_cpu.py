@@ -340,3 +340,22 @@ def test_steps_tell_autograd_what_they_write(monkeypatch):
                 step()
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 product.sum().backward()
+
+
+def test_threads_share_the_entry_points():
+    """The library's first calls from many threads at once (autograd has its own):
+    without a GPU all come back with the same status, and none crashes."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from gaussian_splats_b200 import native
+
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not to be read")
+    lib, a = native.lib(), 256
+    args = native.WindowAttentionArgs(
+        tokens=300, num_tiles=3, heads=4, kv_heads=2, dim=64, dtype=1, left=3, scale=0.1, q=a, k=a,
+        v=a, q_stride=64, q_head_stride=64, k_stride=64, k_head_stride=64, v_stride=64,
+        v_head_stride=64, out=a)
+    with ThreadPoolExecutor(16) as pool:
+        got = set(pool.map(lambda _: lib.gs_window_attention(ctypes.byref(args), None), range(200)))
+    assert len(got) == 1 and got.pop() < 0
