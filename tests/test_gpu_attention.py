@@ -480,3 +480,24 @@ def test_step_refuses_validity_that_does_not_fit():
         with pytest.raises(ValueError, match=match):
             window_attention_step(q, k, v, *cache, at, first=1, valid=valid,
                                   cache_valid=cache_valid)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("tokens,dim,left,right,first", [
+    (2600, 64, 2300, 0, 0),    # more than 32 tiles of 64 keys: the plan's second batch
+    (2700, 64, 1200, 1400, 70),
+    (4700, 128, 4500, 0, 3),   # more than 32 tiles of 128 keys
+    (6000, 64, 50, 0, 9),      # six chunks of first tokens' later queries
+    (6200, 128, 30, 40, 128),
+], ids=str)
+def test_long_walks(tokens, dim, left, right, first, dtype):
+    if max(left, right) > 1000:
+        seen = min(left, tokens) + right + 1
+        assert seen > 32 * (64 if dim == 64 else 128)
+    else:
+        assert tokens > 5 * 8 * 128 and left + right < 7 * 128  # chunks of 8 tiles
+    q, k, v, grad, _ = make([tokens], 2, 1, dim, dtype, seed=12)
+    window = dict(left=left, right=right, first=first)
+    got = call(q, k, v, grad, [tokens], **window)
+    ref = R.attention(q, k, v, [tokens], grad=grad, **window)
+    check(got, ref, dtype, tokens * 2, 6.0)

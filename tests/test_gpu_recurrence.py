@@ -248,3 +248,82 @@ def test_no_wait_ran_out():
     s = make([3000, 5], 64, torch.bfloat16)
     call(s, [3000, 5])
     assert native.lib().gs_gated_scan_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+def tiles_of_a_span(lengths, channels, dtype):
+    """How many tiles a block walks: what spans_of in recurrence.cu makes of these sizes."""
+    tiles = sum(-(-n // 128) for n in lengths)
+    boxes = channels % (16 // dtype.itemsize) == 0
+    columns = -(-channels // (128 // dtype.itemsize if boxes else 32))
+    return min(max(tiles * columns // (8 * 148), 1), 8)
+
+
+SPANS = [
+    # lengths, channels, type, tiles of a span; sequences end inside spans and inside tiles
+    ([5000, 0, 1, 1029, 3500], 1024, torch.float32, 2),
+    ([5000, 0, 1, 1029, 3500], 4096, torch.bfloat16, 4),
+    ([9000, 127, 0, 10400], 4096, torch.float16, 8),
+    ([5000, 0, 1, 1029, 3500], 1001, torch.bfloat16, 2),
+    ([4700, 300, 0, 4600], 4001, torch.float32, 8),
+]
+
+
+@pytest.mark.parametrize("lengths,channels,dtype,span", SPANS, ids=str)
+def test_spans_of_several_tiles(lengths, channels, dtype, span):
+    """Loads into places that were used before, the carry from tile to tile, and the
+    walk back through a span, for copied boxes and for plain loads."""
+    assert tiles_of_a_span(lengths, channels, dtype) == span
+    s = make(lengths, channels, dtype, seed=9)
+    ref = R.gated_scan(s["x"], s["gate"], lengths, s["initial"], s["grad"], s["grad_last"])
+    check(call(s, lengths), ref, dtype)
+
+
+def one_sequence(s):
+    """The definition for one long sequence: pieces of its length's root walked side by
+    side in 64 bits, then joined in order."""
+    x, gate = s["x"].double(), s["gate"].double()
+    a, keep = gate.sigmoid(), (-gate).sigmoid()
+    n, channels = x.shape
+
+    def walk(chain, push, start):
+        size = int(n ** 0.5)
+        pieces = -(-n // size)
+        fill = torch.zeros(pieces * size - n, channels, dtype=x.dtype, device=x.device)
+        chain = torch.cat((chain, fill)).view(pieces, size, channels)
+        push = torch.cat((push, fill)).view(pieces, size, channels)
+        h, through = torch.zeros_like(push), torch.zeros_like(push)
+        now, factor = torch.zeros_like(push[:, 0]), torch.ones_like(push[:, 0])
+        for t in range(size):
+            now, factor = chain[:, t] * now + push[:, t], chain[:, t] * factor
+            h[:, t], through[:, t] = now, factor
+        for piece in range(pieces):
+            h[piece] += through[piece] * start
+            start = h[piece, -1]
+        return h.view(-1, channels)[:n]
+
+    h = walk(keep, a * x, s["initial"][0].double())
+    before = torch.cat((s["initial"].double(), h[:-1]))
+    # u_t = keep_t (g_t + u_{t+1}), from the end
+    u = walk(keep.flip(0), (keep * s["grad"].double()).flip(0), s["grad_last"][0].double()).flip(0)
+    back = s["grad"].double() + torch.cat((u[1:], s["grad_last"].double()))
+    return {"y": h, "last": h[-1:], "dx": a * back, "dgate": back * (x - before) * a * keep,
+            "dinitial": u[:1]}
+
+
+def test_the_pieces_give_the_definition():
+    s = make([157], 5, torch.float32, seed=10)
+    ref = R.gated_scan(s["x"], s["gate"], [157], s["initial"], s["grad"], s["grad_last"])
+    for name, t in one_sequence(s).items():
+        torch.testing.assert_close(t, ref[name], rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("tokens,channels,span", [(70001, 8, 1), (70001, 7, 1), (310001, 8, 2),
+                                                  (310001, 7, 2), (1310001, 16, 8)])
+def test_long_narrow_sequences(tokens, channels, span, dtype):
+    """More than 128 spans of a sequence: the scan that shares them out to 1024 threads,
+    in both directions."""
+    assert tiles_of_a_span([tokens], channels, dtype) == span
+    assert -(-tokens // 128) // span > 128
+    s = make([tokens], channels, dtype, seed=11)
+    check(call(s, [tokens]), one_sequence(s), dtype)

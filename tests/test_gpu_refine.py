@@ -159,3 +159,34 @@ def test_stream_follows_a_scene_with_dead_splats():
             out = refiner.step(one, state)
             for name in whole:
                 torch.testing.assert_close(out[name][0], whole[name][at], rtol=0, atol=3e-2)
+
+
+def test_dead_splats_are_no_keys(monkeypatch):
+    """With a recurrence that passes nothing on, what dead splats hold is seen by
+    themselves alone; what live ones hold is seen by others."""
+    from gaussian_splats_b200 import refine
+
+    monkeypatch.setattr(refine, "gated_scan", lambda x, gate, packed: (torch.zeros_like(x), None))
+    torch.manual_seed(0)
+    refiner = shaken(SplatRefiner(shape=RefinerShape(width=128, heads=2, kv_heads=1, left=40,
+                                                     right=20)))
+    splats, changes = scene(400, 4, dead=50), scene(400, 7)
+
+    def refined(rows):
+        """The live splats' results with the rows' parameters replaced, order and
+        opacity kept."""
+        with torch.no_grad():
+            tensors = {n: getattr(splats, n).detach().clone()
+                       for n in ("mean", "rotation", "scale", "opacity", "color")}
+            for n in ("rotation", "scale", "color"):
+                tensors[n][rows] = 5 * getattr(changes, n)[rows]
+            out = refiner([GaussianSplat.from_tensors(*tensors.values())])[0]
+        return torch.cat([out[n][100:].flatten(1) for n in out], 1)
+
+    plain = refined(slice(0, 0))
+    assert torch.equal(refined(slice(0, 50)), plain)          # dead ones
+    assert not torch.equal(refined(slice(50, 100)), plain)    # live ones
+    attention = refine.window_attention
+    monkeypatch.setattr(refine, "window_attention",
+                        lambda *a, valid, **k: attention(*a, valid=None, **k))
+    assert not torch.equal(refined(slice(0, 50)), refined(slice(0, 0)))  # were they keys
