@@ -49,8 +49,7 @@ constexpr int kMaxDim = 128;
 // While one group takes its exponentials, the tensor cores work for the other,
 // and both read the same keys and values. m is the row's running maximum, but
 // moves only when it has grown by more than 2^8: until then P stays at most
-// 2^8, which both types hold with all their precision, and O need not be
-// rescaled.
+// 2^8 and O need not be rescaled.
 //
 // What bounds it: 16 exponentials a clock and multiprocessor at 64 channels (a
 // 128 x 128 tile takes 1024 clocks of them, 512 of products), both at 128
@@ -64,6 +63,10 @@ constexpr int kMaxDim = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // log2 of the growth that m lets pass
+// log2 of what P is stored times. float16 cuts off what is below 2^-25, which a wide
+// window may have many of: it gets what its range has left above 2^kSlack.
+template <class T>
+constexpr float kLift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
 // A wait ran out (never in a working kernel): set for
 // gs_window_attention_status, the block's results are not valid.
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
         }
       }
       // Where nothing is seen yet any finite shift will do: exp2(-inf) is 0.
-      const float down = top == -INFINITY ? 0.0f : -top;
+      const float down = top == -INFINITY ? 0.0f : kLift<T> - top;
       const float2 shift = make_float2(down, down), factor = make_float2(scale, scale);
       float2 part[2] = {};
 #pragma unroll
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(ForwardShape<kDim>::kThreads, ForwardShape<kDi
           int64_t{a.heads} * a.dim, 0, static_cast<int>(tile.end - (token - row)), a.dim, row);
       if (write && a.lse)
         a.lse[head * a.tokens + token] =
-            row_value(good, sum == 0.0f, (top + log2f(sum)) * kLn2, -INFINITY);
+            row_value(good, sum == 0.0f, (top - kLift<T> + log2f(sum)) * kLn2, -INFINITY);
     }
   }
   fence_before_sync();
@@ -1935,7 +1938,7 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
             out[h][i][r][1] *= shrink;
           }
       }
-      const float shift = top[r] == -INFINITY ? 0.0f : -top[r];
+      const float shift = top[r] == -INFINITY ? 0.0f : kLift<T> - top[r];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float p0 = tc::exp2_approx(fmaf(x[n][r][0], scale, shift));

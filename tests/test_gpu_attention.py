@@ -501,3 +501,26 @@ def test_long_walks(tokens, dim, left, right, first, dtype):
     got = call(q, k, v, grad, [tokens], **window)
     ref = R.attention(q, k, v, [tokens], grad=grad, **window)
     check(got, ref, dtype, tokens * 2, 6.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("depth", [20.5, 25.2], ids=str)
+def test_float16_keeps_many_small_weights(dim, depth):
+    """One key holds nearly all of the weight, thousands have 2**-depth of it each: the
+    sum of these is kept, not cut off under float16's smallest number. Stored times
+    2**7 they are off by at most 2**-32, 4096 of them by 2**-20 of a value."""
+    from gaussian_splats_b200.attention import window_attention, window_attention_step
+
+    n = 4096
+    q = torch.zeros(n, 1, dim, dtype=torch.float16, device="cuda")
+    k, v = q.clone(), torch.ones_like(q)
+    q[..., 0], k[0, 0, 0], v[0] = 1.0, 32.0, 0.0
+    scale = depth * 0.6931471805599453 / 32.0
+    small = torch.arange(n, device="cuda").double() * 2.0 ** -depth
+    expected = small / (1.0 + small)
+    bound = 1.25 * 2 * U[torch.float16] * expected + 2.0 ** -20 + 2.0 ** -25
+    out = window_attention(q, k, v, left=n, scale=scale)
+    assert ((out[:, 0].double() - expected[:, None]).abs() <= bound[:, None]).all()
+    step = window_attention_step(q[:1], k[-1:], v[-1:], k[None].clone(), v[None].clone(),
+                                 torch.tensor([n - 1], device="cuda"), scale=scale)
+    assert ((step[0, 0].double() - expected[-1]).abs() <= bound[-1]).all()
