@@ -10,8 +10,10 @@
 //   dz = m (g w - z m^2 mean(g w z)) + h,   dw = sum over tokens of g z m
 //
 // dz is the gradient of x and of r. Everything is computed in float. The
-// forward norms the unrounded z; the backward reads z as it was stored (in
-// the residual's type), which is what the next layer saw too.
+// forward norms the unrounded z, and so does the backward: it reads z as it was
+// stored where that is a float (or x itself), and adds x and r again where a 16-bit
+// sum would bring its rounding into every term (dw's error against the definition
+// is then half as large again; the price is one more 16-bit array to read).
 //
 // Bound by memory: a token's row is read and written once. 262,144 tokens of 1024
 // 16-bit channels on a 32-bit residual: forward 467 us (6.9 TB/s), backward 650 us
@@ -212,7 +214,8 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(gs_rms_norm_args a)
 // Any channel count and alignment: one block a token at a time. A channel's
 // weight gradient is summed by the one thread that owns the channel, token
 // after token, in shared memory; the block's sums go to its row of partials.
-template <class T, class R>
+// kAgain: z is x + r again, else the stored sum.
+template <class T, class R, bool kAgain>
 __global__ void __launch_bounds__(kThreads) norm_backward_kernel(gs_rms_norm_args a,
                                                                  float* partials) {
   chain_wait();
@@ -221,12 +224,18 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(gs_rms_norm_arg
   for (int c = threadIdx.x; c < a.channels; c += kThreads) s_dw[c] = 0.0f;
   const float inverse = 1.0f / static_cast<float>(a.channels);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const R* z = static_cast<const R*>(a.sum) + row * a.sum_stride;
+    const R* sum = kAgain ? nullptr : static_cast<const R*>(a.sum) + row * a.sum_stride;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const R* r = static_cast<const R*>(a.residual) + row * a.residual_stride;
+    const auto z = [&](int c) {
+      if constexpr (kAgain) return to_float(x[c]) + to_float(r[c]);
+      else return to_float(sum[c]);
+    };
     const T* g = static_cast<const T*>(a.grad_y) + row * a.channels;
     const R* h = a.grad_sum ? static_cast<const R*>(a.grad_sum) + row * a.channels : nullptr;
     float2 v = make_float2(0.0f, 0.0f);
     for (int c = threadIdx.x; c < a.channels; c += kThreads) {
-      const float zc = to_float(z[c]);
+      const float zc = z(c);
       const float gw = to_float(g[c]) * load_weight(a.weight, a.weight_dtype, c);
       v.x = fmaf(zc, zc, v.x);
       v.y = fmaf(gw, zc, v.y);
@@ -235,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(gs_rms_norm_arg
     const float m = rsqrtf(v.x * inverse + a.eps);
     const float pull = v.y * inverse * m * m;
     for (int c = threadIdx.x; c < a.channels; c += kThreads) {
-      const float zc = to_float(z[c]), gc = to_float(g[c]);
+      const float zc = z(c), gc = to_float(g[c]);
       const float gw = gc * load_weight(a.weight, a.weight_dtype, c);
       const float d = fmaf(m, fmaf(-zc, pull, gw), h ? to_float(h[c]) : 0.0f);
       static_cast<T*>(a.grad_x)[row * a.channels + c] = from_float<T>(d);
@@ -274,8 +283,10 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2 (*shared)[kWarps],
 // channels from token to token; a block's groups add theirs up in order. One
 // or two words a thread keep a thread at 64 registers, so that 32 warps a
 // multiprocessor cover the loads (a warp a token of 1024 channels took 160
-// registers, 8 warps, and 963 us for 262,144 tokens).
-template <class T, class R, int kLanes, int kIter>
+// registers, 8 warps, and 963 us for 262,144 tokens). kAgain spills a few words at 64
+// registers; three blocks instead of four without spills took 967 us for a pass of
+// 262,144 x 1024 bf16 on a bf16 residual, four 801 (712 with the stored sum).
+template <class T, class R, bool kAgain, int kLanes, int kIter>
 __global__ void __launch_bounds__(kThreads, 4 / kIter)
     norm_rows_backward_kernel(gs_rms_norm_args a, float* partials) {
   chain_wait();
@@ -288,15 +299,22 @@ __global__ void __launch_bounds__(kThreads, 4 / kIter)
   float dw[kIter][8] = {};
   for (int64_t row = int64_t{blockIdx.x} * kRows + group; row < a.rows;
        row += int64_t{gridDim.x} * kRows) {
-    const R* z_row = static_cast<const R*>(a.sum) + row * a.sum_stride;
+    const R* z_row = kAgain ? static_cast<const R*>(a.residual) + row * a.residual_stride
+                            : static_cast<const R*>(a.sum) + row * a.sum_stride;
+    const T* x_row = static_cast<const T*>(a.x) + row * a.x_stride;
     const int64_t at = row * a.channels;
-    Pack<R, 8> z[kIter], h[kIter];
-    Pack<T, 8> g[kIter];
+    Pack<R, 8> z[kIter], h[kIter];  // kAgain: r in z's place
+    Pack<T, 8> g[kIter], x[kIter];
+    const auto value = [&](int i, int k) {
+      if constexpr (kAgain) return to_float(x[i].v[k]) + to_float(z[i].v[k]);
+      else return to_float(z[i].v[k]);
+    };
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
       const int c = (i * kLanes + lane) * 8;
       if (c < a.channels) {
         z[i] = *reinterpret_cast<const Pack<R, 8>*>(z_row + c);
+        if constexpr (kAgain) x[i] = *reinterpret_cast<const Pack<T, 8>*>(x_row + c);
         g[i] = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.grad_y) + at + c);
         if (a.grad_sum)
           h[i] = *reinterpret_cast<const Pack<R, 8>*>(static_cast<const R*>(a.grad_sum) + at + c);
@@ -311,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 4 / kIter)
         load_weights(a.weight, a.weight_dtype, c, w);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float zc = to_float(z[i].v[k]);
+          const float zc = value(i, k);
           v.x = fmaf(zc, zc, v.x);
           v.y = fmaf(to_float(g[i].v[k]) * w[k], zc, v.y);
         }
@@ -329,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 4 / kIter)
       load_weights(a.weight, a.weight_dtype, c, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float zc = to_float(z[i].v[k]), gc = to_float(g[i].v[k]);
+        const float zc = value(i, k), gc = to_float(g[i].v[k]);
         const float own = a.grad_sum ? to_float(h[i].v[k]) : 0.0f;
         w[k] = fmaf(m, fmaf(-zc, pull, gc * w[k]), own);
         dw[i][k] = fmaf(gc, zc * m, dw[i][k]);
@@ -382,6 +400,11 @@ int backward_blocks(int64_t rows) {
   return static_cast<int>(rows < kBackwardBlocks ? rows : kBackwardBlocks);
 }
 
+// Whether the backward makes a 16-bit sum again from its parts.
+bool adds_again(const gs_rms_norm_args& a) {
+  return !a.sum && a.x && a.residual && a.dtype != GS_FLOAT32 && a.residual_dtype == a.dtype;
+}
+
 int32_t check_args(const gs_rms_norm_args& a, bool backward) {
   const auto valid = [](int32_t t) { return t >= GS_FLOAT32 && t <= GS_FLOAT16; };
   if (a.rows < 0 || a.channels < 1 || a.channels > GS_MAX_NORM_CHANNELS || !valid(a.dtype) ||
@@ -390,7 +413,7 @@ int32_t check_args(const gs_rms_norm_args& a, bool backward) {
   if (a.residual_dtype != a.dtype && a.residual_dtype != GS_FLOAT32) return GS_ERR_UNSUPPORTED;
   if (a.rows == 0) return GS_OK;
   if (backward) {
-    if (!a.sum || !a.grad_y || !a.grad_x || !a.grad_weight || !a.workspace)
+    if ((!a.sum && !adds_again(a)) || !a.grad_y || !a.grad_x || !a.grad_weight || !a.workspace)
       return GS_ERR_INVALID_ARGUMENT;
     if (a.workspace_size < rms_norm_workspace_size(a.rows, a.channels)) return GS_ERR_CAPACITY;
   } else if (!a.x || (a.q ? !a.scale : !a.y)) {
@@ -457,7 +480,7 @@ int32_t forward(const gs_rms_norm_args& a, cudaStream_t stream) {
   return check_launch();
 }
 
-template <class T, class R>
+template <class T, class R, bool kAgain>
 int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
   float* partials = static_cast<float*>(a.workspace);
   int blocks = backward_blocks(a.rows);
@@ -466,13 +489,14 @@ int32_t backward(const gs_rms_norm_args& a, cudaStream_t stream) {
     GS_TRY(with_backward_shape(a.channels, [&](auto lanes, auto iter) {
       constexpr int kLanes = decltype(lanes)::value, kIter = decltype(iter)::value;
       blocks = std::min<int>(blocks, ceil_div(a.rows, kThreads / kLanes));
-      launch_chained_shared(norm_rows_backward_kernel<T, R, kLanes, kIter>, blocks, kThreads,
+      launch_chained_shared(norm_rows_backward_kernel<T, R, kAgain, kLanes, kIter>, blocks, kThreads,
                             kLanes < kThreads ? shared : 0, stream, a, partials);
       return check_launch();
     }));
   } else {
-    GS_TRY((allow_shared<norm_backward_kernel<T, R>>(sizeof(float) * GS_MAX_NORM_CHANNELS)));
-    launch_chained_shared(norm_backward_kernel<T, R>, blocks, kThreads, shared, stream, a,
+    GS_TRY((allow_shared<norm_backward_kernel<T, R, kAgain>>(sizeof(float) *
+                                                             GS_MAX_NORM_CHANNELS)));
+    launch_chained_shared(norm_backward_kernel<T, R, kAgain>, blocks, kThreads, shared, stream, a,
                           partials);
     GS_TRY(check_launch());
   }
@@ -510,7 +534,10 @@ int32_t launch_rms_norm_backward(const gs_rms_norm_args& a, cudaStream_t stream)
   }
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return a.residual_dtype == a.dtype ? backward<T, T>(a, stream) : backward<T, float>(a, stream);
+    if constexpr (!std::is_same_v<T, float>)
+      if (adds_again(a)) return backward<T, T, true>(a, stream);
+    return a.residual_dtype == a.dtype ? backward<T, T, false>(a, stream)
+                                       : backward<T, float, false>(a, stream);
   });
 }
 

@@ -65,7 +65,9 @@ class _RmsNorm(torch.autograd.Function):
         total = None if res is None else res.new_empty(shape)
         args = _arguments(rows, weight, res, eps, y=y, sum=total)
         call("gs_rms_norm", x.device, ctypes.byref(args))
-        ctx.save_for_backward(rows if res is None else total, weight)
+        # The sum itself where it lost nothing, else what it was made of.
+        again = res is not None and res.dtype != torch.float32
+        ctx.save_for_backward(rows if res is None or again else total, weight, res if again else None)
         ctx.args, ctx.has_residual, ctx.x_dtype, ctx.shape = args, res is not None, x.dtype, shape
         ctx.set_materialize_grads(False)
         return y if res is None else (y, total)
@@ -73,7 +75,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y, grad_sum=None):
-        z, weight = ctx.saved_tensors
+        z, weight, residual = ctx.saved_tensors
         # A saved-tensor hook may have brought back tensors that lie differently.
         z, weight = _rows(z), weight.contiguous()
         shape = ctx.shape
@@ -82,13 +84,19 @@ class _RmsNorm(torch.autograd.Function):
         grad_sum = None if grad_sum is None else grad_sum.contiguous()
         grad_x = z.new_empty(shape, dtype=ctx.x_dtype)
         grad_residual = None
-        if ctx.has_residual and z.dtype != ctx.x_dtype:
+        if ctx.has_residual and residual is None and z.dtype != ctx.x_dtype:
             grad_residual = z.new_empty(shape)
         grad_weight = torch.empty_like(weight)
         args = native.RmsNormArgs.from_buffer_copy(ctx.args)  # sizes and types
-        args.x = args.residual = args.y = None
-        args.x_stride = args.residual_stride = 0
-        args.sum, args.weight, args.sum_stride = address(z), address(weight), z.stride(0)
+        args.x = args.residual = args.y = args.sum = None
+        args.x_stride = args.residual_stride = args.sum_stride = 0
+        if residual is None:
+            args.sum, args.sum_stride = address(z), z.stride(0)
+        else:
+            residual = _rows(residual)
+            args.x, args.x_stride = address(z), z.stride(0)
+            args.residual, args.residual_stride = address(residual), residual.stride(0)
+        args.weight = address(weight)
         args.grad_y, args.grad_sum = address(grad_y), address(grad_sum)
         args.grad_x, args.grad_residual = address(grad_x), address(grad_residual)
         args.grad_weight = address(grad_weight)
@@ -110,9 +118,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     residual's type, the residual stream for the next layer.
 
     float32, bfloat16 or float16, at most 16,384 channels; the sum and the norm
-    are computed in float32, and the norm is that of the unrounded sum (the
-    backward reads the sum as it was stored). Differentiable in x, weight and
-    residual, through both results; deterministic in both directions."""
+    are computed in float32, and the norm and its gradients are those of the
+    unrounded sum. Differentiable in x, weight and residual, through both results;
+    deterministic in both directions."""
     eps = _check("rms_norm", x, weight, residual, eps)
     return _RmsNorm.apply(x, weight, residual, eps)
 

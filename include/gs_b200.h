@@ -607,7 +607,9 @@ int32_t gs_gated_scan_step(int64_t batch, int32_t channels, int32_t dtype, const
  * residual_dtype; may be NULL) and y, or, when q is not NULL, instead of y the
  * 8-bit e4m3 codes q and scale [rows] float with z's norm = q * scale. The
  * backward reads z from `sum` with its row stride (x itself, where there was no
- * residual; residual_dtype is then dtype), grad_y, and grad_sum (NULL: zeros),
+ * residual; residual_dtype is then dtype), or, where sum is NULL and dtype and
+ * residual_dtype are one 16-bit type, adds x and residual again, which spares its
+ * terms the rounding of the sum; it reads grad_y, and grad_sum (NULL: zeros),
  * and writes grad_x, grad_residual (unless NULL) and grad_weight; it needs a
  * workspace of gs_rms_norm_workspace_size bytes. Outputs and gradients are
  * contiguous. */

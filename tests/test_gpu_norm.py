@@ -194,3 +194,30 @@ def test_no_rows():
     s = make(0, 64, torch.bfloat16, torch.float32)
     got = call(s)
     assert got["y"].shape == (0, 64) and torch.count_nonzero(got["dw"]) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows,channels", SHAPES + [(5003, 320)])
+def test_gradients_are_those_of_the_unrounded_sum(rows, channels, dtype):
+    """With a 16-bit residual the sum is returned rounded, but its rounding is in no
+    gradient: one rounding of the result, and float sums."""
+    s = make(rows, channels, dtype, dtype, seed=5)
+    got, ref = call(s), R.rms_norm(s["x"], s["w"], s["r"], 1e-6, s["g"], s["h"])
+    z, gw = ref["sum"], (s["g"].double() * s["w"].double()).abs()
+    root = (z.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    pull = (gw * z.abs()).mean(-1, keepdim=True) * z.abs() / root ** 3
+    dz = 4e-6 * (gw / root + pull) + 1e-6 * s["h"].double().abs()
+    dw = 4e-6 * (s["g"].double() * z / root).abs().sum(0) + 1e-6
+    for name, expected, inner in (("dx", "dz", dz), ("dr", "dz", dz), ("dw", "dw", dw)):
+        bound = 1.01 * U[dtype] * ref[expected].abs() + inner + 2.0 ** -25
+        error = (got[name].double() - ref[expected]).abs()
+        assert (error <= bound).all(), f"{name}: {(error - bound).max().item():.3g} beyond"
+
+
+def test_a_16_bit_sum_with_rows_of_their_own_strides():
+    s = make(60, 96, torch.bfloat16, torch.bfloat16)
+    expected = call(s)
+    wide = torch.cat((s["x"], s["r"], s["r"]), 1)
+    for x, r in ((wide[:, :96], wide[:, 96:192]), (s["x"].t().contiguous().t(), wide[:, 192:])):
+        got = call({**s, "x": x, "r": r})
+        assert all(torch.equal(got[n], expected[n]) for n in got)

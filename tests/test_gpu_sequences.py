@@ -42,10 +42,13 @@ def operators(tokens=300):
                  [rand(tokens, 128).to(torch.bfloat16)]),
         "norm, residual": (lambda x, w, r: rms_norm(x, w, r), leaves(x, weight, gate.float()),
                            [rand(tokens, 128).to(torch.bfloat16), rand(tokens, 128)]),
+        "norm, 16-bit residual": (lambda x, w, r: rms_norm(x, w, r), leaves(x, weight, gate),
+                                  [rand(tokens, 128).to(torch.bfloat16) for _ in range(2)]),
     }
 
 
-NAMES = ["attention", "scan", "scan, odd", "norm", "norm, residual"]
+NAMES = ["attention", "scan", "scan, odd", "norm", "norm, residual",
+         "norm, 16-bit residual"]
 
 
 def run(function, inputs, grads):
