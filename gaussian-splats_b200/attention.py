@@ -146,8 +146,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     the same sequence less than a window and 128 tokens away.
     ``scale`` multiplies the scores (default ``dim ** -0.5``).
 
-    bfloat16 or float16, dim a multiple of 8 up to 128; scores, softmax and
-    sums in float32. q, k and v may be slices of one projection: they are read
+    bfloat16 or float16, dim a multiple of 8 up to 128; scores, maxima and sums
+    in float32. The probabilities, and in the backward the score gradients, are
+    rounded to the inputs' type for their products (float16's are scaled into its
+    range, whatever the gradients' size). q, k and v may be slices of one projection: they are read
     in place if rows and heads start on 16-byte boundaries, and copied
     otherwise. Returns [tokens, heads, dim]; differentiable in q, k and v, and
     deterministic in both directions."""

@@ -14,8 +14,10 @@
 //   dq_i = scale sum_j e_ij k_j,  dk_j = scale sum_i e_ij q_i,  dv_j = sum_i p_ij g_i
 //
 // where a key's sums also run over the query heads that share it. Scores,
-// exponentials, sums and accumulators are float. Keys that no query sees are
-// never read into a sum, so what they hold (infinities, NaN) does not matter.
+// exponentials, sums and accumulators are float; p and e are rounded to the inputs'
+// type for their products, as the tensor cores take them, and D comes from the rounded
+// outputs. Keys that no query sees, and queries that see none, never reach a sum, so
+// what they hold (infinities, NaN) does not matter.
 
 #include <algorithm>
 #include <cmath>
@@ -55,9 +57,9 @@ constexpr int kMaxDim = 128;
 // 128 x 128 tile takes 1024 clocks of them, 512 of products), both at 128
 // (1024 each); then the chain product, exponentials, product of a step, which
 // two groups cover only in part. Two blocks a multiprocessor at 64 channels.
-// Measured: 500,000 tokens, 4 heads of 64, 1025 keys seen: 990 us, 540 TFLOP/s,
+// Measured: 500,000 tokens, 4 heads of 64, 1041 keys seen: 990 us, 540 TFLOP/s,
 // the exponentials' pipe 58% and the tensor cores 45% of the time busy; 131,072
-// tokens, 8 heads of 128, 1025 keys: 812 us, 660 TFLOP/s. A block of nine tiles
+// tokens, 8 heads of 128, 1029 keys: 822 us, 650 TFLOP/s. A block of nine tiles
 // spends a sixth of its time before the first exponential and after the last.
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -641,9 +643,9 @@ int32_t forward(const gs_window_attention_args& a, cudaStream_t stream) {
 // no faster.
 //
 // What bounds them is a tile's chain S, P, G, E, sum, of which one block's tiles
-// overlap in part. Measured: 131,072 tokens, 8 heads (4 of keys) of 128, 1025 keys
-// seen: queries 1066 us (760 TFLOP/s of products, the tensor cores busy for 43%
-// of the time), keys 1205 us (890 TFLOP/s, 55%).
+// overlap in part. Measured: 131,072 tokens, 8 heads (4 of keys) of 128, 1029 keys
+// seen: queries 1078 us (750 TFLOP/s of products, the tensor cores busy for 43%
+// of the time), keys 1250 us (860 TFLOP/s, 55%).
 
 // First tokens are seen by all later queries, so the block of their keys would
 // walk the whole sequence. It walks its window like the others; the queries

@@ -16,8 +16,8 @@
 // is then half as large again; the price is one more 16-bit array to read).
 //
 // Bound by memory: a token's row is read and written once. 262,144 tokens of 1024
-// 16-bit channels on a 32-bit residual: forward 467 us (6.9 TB/s), backward 650 us
-// (6.6 TB/s) and 6 us for the weight's sums; 16 tokens to 8 bits 4.5 us.
+// 16-bit channels on a 32-bit residual: forward 467 us (6.9 TB/s), backward 665 us
+// (6.5 TB/s) and 6 us for the weight's sums; 16 tokens to 8 bits 4.5 us.
 
 #include <cuda_fp8.h>
 

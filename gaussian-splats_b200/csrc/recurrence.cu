@@ -21,7 +21,7 @@
 // grad_y on the way back) is the price of a sequence split without blocks that
 // wait for one another. Walks go the other way round from folds, so that part of
 // it comes from L2. Measured at 1,000,000 tokens of 64 16-bit channels (128 MB an
-// array): fold 45 us (5.7 TB/s), walk 69 us (5.6 TB/s), back 46 and 109 us (5.9
+// array): fold 46 us (5.6 TB/s), walk 69 us (5.6 TB/s), back 47 and 110 us (5.8
 // TB/s), the scans of the spans' maps 10 us each.
 //
 // States, products and gates are float; the states that enter the tiles are
