@@ -54,11 +54,16 @@ __device__ __forceinline__ void load_weights(const void* w, int32_t dtype, int c
 // cancels), from the product in double: a float chain z m w / s is off by a few
 // units in the last place, which moves one value in some 10^5 across a rounding
 // boundary of e4m3. The last conversion rounds a float that keeps, in its lowest
-// bit, whether bits were cut off, so that the one rounding is to e4m3.
+// bit, whether anything was cut off, so that the one rounding is to e4m3. Quotients
+// of 16-bit inputs often lie halfway between two codes, where the rounding of
+// `inverse` must not decide: it is 2^-50 too large, so that such a product is not below
+// the halfway point, and what is less than 2^-40 above it (448 * 1.5 * 2^-50 at most)
+// counts as nothing. The nearest other quotient of 16-bit inputs is 2^-37 away.
+constexpr double kAbove = 1.0 + 0x1p-50;
 __device__ __forceinline__ uint8_t to_e4m3(double zw, double inverse) {
   const double v = zw * inverse;
   float f = __double2float_rz(v);
-  if (static_cast<double>(f) != v && v == v) f = __int_as_float(__float_as_int(f) | 1);
+  if (fabs(v - static_cast<double>(f)) > 0x1p-40) f = __int_as_float(__float_as_int(f) | 1);
   return __nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
 }
 
@@ -89,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(gs_rms_norm_args a) {
     for (int c = lane; c < a.channels; c += 32)
       top = fmaxf(top, fabsf(static_cast<float>(product(c))));
     top = warp_max(top);
-    if (top > 0.0f) inverse = kE4m3Max / static_cast<double>(top);
+    if (top > 0.0f) inverse = kE4m3Max / static_cast<double>(top) * kAbove;
     if (lane == 0) a.scale[row] = top > 0.0f ? top * m / kE4m3Max : 1.0f;
   }
   for (int c = lane; c < a.channels; c += 32) {
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(gs_rms_norm_args a)
       }
     }
     top = kLanes == 32 ? warp_max(top) : block_max(top, s_sum);
-    if (top > 0.0f) inverse = kE4m3Max / static_cast<double>(top);
+    if (top > 0.0f) inverse = kE4m3Max / static_cast<double>(top) * kAbove;
     if (lane == 0) a.scale[row] = top > 0.0f ? top * m / kE4m3Max : 1.0f;
   }
 #pragma unroll

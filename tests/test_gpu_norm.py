@@ -221,3 +221,26 @@ def test_a_16_bit_sum_with_rows_of_their_own_strides():
     for x, r in ((wide[:, :96], wide[:, 96:192]), (s["x"].t().contiguous().t(), wide[:, 192:])):
         got = call({**s, "x": x, "r": r})
         assert all(torch.equal(got[n], expected[n]) for n in got)
+
+
+@pytest.mark.parametrize("channels", [30, 32], ids=["any", "words"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32],
+                         ids=["bf16", "f16", "f32"])
+def test_eight_bits_halfway_between_two_codes(dtype, channels):
+    """Values whose quotient by the scale is a halfway point go to the even code. The
+    largest value is 448 n, so value h n is h in units of the scale; n is odd, and for
+    all but the first a product with the rounded 1 / n misses some of the points."""
+    from gaussian_splats_b200.norm import rms_norm_e4m3
+
+    halves = [17, 19, 21, 23, 25, 27, 29, 31, 8.5, 9.5, 1.0625, 1.1875, 104, 120, 2.0 ** -10,
+              3 * 2.0 ** -10, 5 * 2.0 ** -10, 7 * 2.0 ** -10]
+    even = [16, 20, 20, 24, 24, 28, 28, 32, 8, 10, 1, 1.25, 104, 120, 0, 2 * 2.0 ** -9,
+            2 * 2.0 ** -9, 4 * 2.0 ** -9]  # 104 and 120 are codes
+    x = torch.tensor([448.0] + halves + [0.0] * (channels - 1 - len(halves)), device="cuda")
+    expected = torch.tensor([448.0] + even, device="cuda")
+    assert torch.equal(x.to(dtype).float(), x)
+    for n in (1, 49, 75, 77, 91, 93):
+        weight = torch.full((channels,), float(n), dtype=dtype, device="cuda")
+        for sign in (1, -1):
+            q, _ = rms_norm_e4m3((sign * x[None]).to(dtype), weight)
+            assert torch.equal(q.float()[0, :len(expected)], sign * expected), (n, sign)
