@@ -119,7 +119,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
 
     float32, bfloat16 or float16, at most 16,384 channels; the sum and the norm
     are computed in float32, and the norm and its gradients are those of the
-    unrounded sum. Differentiable in x, weight and residual, through both results;
+    unrounded sum, for which a 16-bit residual's call keeps x and the residual for
+    the backward. Differentiable in x, weight and residual, through both results;
     deterministic in both directions."""
     eps = _check("rms_norm", x, weight, residual, eps)
     return _RmsNorm.apply(x, weight, residual, eps)

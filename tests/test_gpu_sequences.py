@@ -74,12 +74,13 @@ def test_a_layout_dropped_while_another_stream_reads_it():
     from gaussian_splats_b200.sequences import PackedSequences
 
     x = torch.randn(700, 64, device="cuda")
+    expected, _ = gated_scan(x, x, PackedSequences([300, 400]))  # and the kernels are loaded
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     packed = PackedSequences([300, 400])
     sizes = [(t.data_ptr(), t.numel()) for t in (packed.tiles, packed.tile_starts)]
     with torch.cuda.stream(stream):
-        torch.cuda._sleep(200_000_000)  # 0.1 s
+        torch.cuda._sleep(1_000_000_000)  # 0.5 s
         y, _ = gated_scan(x, x, packed)
     del packed
     for pointer, numel in sizes:
@@ -87,7 +88,7 @@ def test_a_layout_dropped_while_another_stream_reads_it():
         assert all(t.data_ptr() != pointer for t in others)
     assert not stream.query(), "the stream was done before the test was"
     torch.cuda.current_stream().wait_stream(stream)
-    assert torch.equal(y, gated_scan(x, x, PackedSequences([300, 400]))[0])
+    assert torch.equal(y, expected)
 
 
 @pytest.mark.parametrize("name", NAMES)
