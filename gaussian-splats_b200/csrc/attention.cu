@@ -929,7 +929,7 @@ __device__ __forceinline__ void backward_setup(BackwardShared<kDim, kKeyRows>& s
 //
 //   |E_ij| <= |G_ij - D_i| <= |g_i| |v_j| + |D_i|,  |D_i| <= |g_i| max_j |v_j|
 //
-// over the keys that query i sees. The exponent brings the bound to between 2^13 and
+// over the keys that query i sees. The exponent brings the bound to between 2^14 and
 // 2^15: a query's from its gradient's norm and the largest norm of a value in its block's
 // tiles, a block of keys' from its values and the largest norm and D of its queries. The
 // sums are scaled back by the same power of two. Rows that are not finite are left out
