@@ -11,6 +11,9 @@ few first tokens that stand for the scene or the camera. Two entry points:
     one new token of each of a batch of streams against a cache of fixed size
     (:func:`window_cache`): the first tokens keep their slots, later tokens
     take the others in turn.
+:func:`window_attention_step_4bit`
+    the same against a cache that holds keys and values in 4 bits
+    (:func:`window_cache_4bit`): a quarter of the memory, and of the reading.
 
 Query ``i`` of a sequence sees key ``j`` if the key is valid, ``j <= i + right``,
 and ``j >= i - left`` or ``j < first``. A query that sees nothing gets zeros, and
@@ -21,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -188,6 +192,30 @@ def window_cache(batch: int, left: int, first: int, kv_heads: int, dim: int,
             torch.zeros(shape, dtype=dtype, device=device))
 
 
+def _step_checks(what, batch, slots, positions, first, valid, cache_valid):
+    """``first`` and ``valid`` of a step, as the kernels take them."""
+    first = int(first)
+    if not 0 <= first < slots:
+        raise ValueError(f"{what}: first must be in [0, {slots}) for {slots} slots, got "
+                         f"{first}")
+    if positions.dtype != torch.int64 or positions.shape != (batch,):
+        raise ValueError(f"{what}: positions must be int64 [{batch}], got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if cache_valid is None and valid is not None:
+        raise ValueError(f"{what}: valid without cache_valid, which keeps it for the later tokens")
+    if cache_valid is not None and (cache_valid.dtype != torch.bool or
+                                    tuple(cache_valid.shape) != (batch, slots) or
+                                    not cache_valid.is_contiguous()):
+        raise ValueError(f"{what}: cache_valid must be a contiguous bool tensor {(batch, slots)}, got "
+                         f"{cache_valid.dtype} {tuple(cache_valid.shape)}")
+    if valid is not None:
+        if valid.dtype != torch.bool or valid.shape != (batch,):
+            raise ValueError(f"{what}: valid must be bool [{batch}], got {valid.dtype} "
+                             f"{tuple(valid.shape)}")
+        valid = valid.contiguous()
+    return first, valid
+
+
 def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           cache_k: torch.Tensor, cache_v: torch.Tensor, positions: torch.Tensor,
                           *, first: int = 0, scale: float | None = None,
@@ -229,25 +257,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if batch * shape[1] > native.MAX_SEQUENCE_TOKENS:
         raise ValueError(f"{what}: caches of {batch} x {shape[1]} slots, at most "
                          f"{native.MAX_SEQUENCE_TOKENS} in all are supported")
-    first = int(first)
-    if not 0 <= first < shape[1]:
-        raise ValueError(f"{what}: first must be in [0, {shape[1]}) for {shape[1]} slots, got "
-                         f"{first}")
-    if positions.dtype != torch.int64 or positions.shape != (batch,):
-        raise ValueError(f"{what}: positions must be int64 [{batch}], got {positions.dtype} "
-                         f"{tuple(positions.shape)}")
-    if cache_valid is None and valid is not None:
-        raise ValueError(f"{what}: valid without cache_valid, which keeps it for the later tokens")
-    if cache_valid is not None and (cache_valid.dtype != torch.bool or
-                                    tuple(cache_valid.shape) != shape[:2] or
-                                    not cache_valid.is_contiguous()):
-        raise ValueError(f"{what}: cache_valid must be a contiguous bool tensor {shape[:2]}, got "
-                         f"{cache_valid.dtype} {tuple(cache_valid.shape)}")
-    if valid is not None:
-        if valid.dtype != torch.bool or valid.shape != (batch,):
-            raise ValueError(f"{what}: valid must be bool [{batch}], got {valid.dtype} "
-                             f"{tuple(valid.shape)}")
-        valid = valid.contiguous()
+    first, valid = _step_checks(what, batch, shape[1], positions, first, valid, cache_valid)
     positions = positions.contiguous()
     q, k, v = _strided(q), _strided(k), _strided(v)
     out = q.new_empty((batch, heads, dim))
@@ -258,4 +268,82 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid))
     call("gs_window_attention_step", device, ctypes.byref(args))
     changed_in_place(cache_k, cache_v, cache_valid)
+    return out
+
+
+class FourBitCache(NamedTuple):
+    """Keys and values of a batch of streams in 4 bits. Codes are uint8 [batch,
+    kv_heads, slots, dim / 2], channel ``2i`` in the low half of byte ``i`` and
+    ``2i + 1`` in the high one; ranges are [batch, kv_heads, slots, 2] in the
+    tokens' type: code ``c`` of a row stands for ``(c - 7.5) * range[0] + range[1]``."""
+
+    k_codes: torch.Tensor
+    k_range: torch.Tensor
+    v_codes: torch.Tensor
+    v_range: torch.Tensor
+
+
+def window_cache_4bit(batch: int, left: int, first: int, kv_heads: int, dim: int,
+                      dtype: torch.dtype = torch.bfloat16, device="cuda") -> FourBitCache:
+    """:func:`window_cache` in 4 bits: an empty cache for ``batch`` streams with a
+    window of ``left`` tokens before the new one and ``first`` first tokens."""
+    if left < 0 or first < 0:
+        raise ValueError(f"window_cache_4bit: left and first must be >= 0, got {left} and {first}")
+    if dim < 8 or dim % 8:
+        raise ValueError(f"window_cache_4bit: dim must be a multiple of 8, got {dim}")
+    shape = (batch, kv_heads, first + left + 1)
+    codes = [torch.zeros((*shape, dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+    ranges = [torch.zeros((*shape, 2), dtype=dtype, device=device) for _ in range(2)]
+    return FourBitCache(codes[0], ranges[0], codes[1], ranges[1])
+
+
+def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                               cache: FourBitCache, positions: torch.Tensor, *, first: int = 0,
+                               scale: float | None = None, valid: torch.Tensor | None = None,
+                               cache_valid: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`window_attention_step` against a :class:`FourBitCache`, which is
+    updated in place: the new token's row ``x`` of each key-value head is held as
+    16 even steps between its least and its greatest channel, ``range = ((max x - min
+    x) / 15, (max x + min x) / 2)`` rounded to the tokens' type and codes ``(x -
+    range[1]) / range[0] + 7.5`` rounded to the nearest, ties to even. The output is
+    the attention over what the cache then holds, the new token as it is held
+    included; scores and sums in float32. A row with a channel that is not finite is
+    held as one that is not finite.
+
+    q, k and v [batch, heads, dim], bfloat16 or float16, dim a multiple of 8 up to
+    128; ``positions``, ``first``, ``scale``, ``valid`` and ``cache_valid`` as
+    :func:`window_attention_step` takes them. No gradient."""
+    what = "window_attention_step_4bit"
+    cache = FourBitCache(*cache)
+    device = check_cuda(what, q=q, k=k, v=v, **cache._asdict(), positions=positions, valid=valid,
+                        cache_valid=cache_valid)
+    dtype = _heads(what, q, k, v, "batch")
+    batch, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    slots = cache.k_codes.shape[2] if cache.k_codes.dim() == 4 else 0
+    for name, t in cache._asdict().items():
+        codes = name.endswith("codes")
+        shape, kind = (batch, kv_heads, slots, dim // 2 if codes else 2), \
+            torch.uint8 if codes else q.dtype
+        if slots < 1 or tuple(t.shape) != shape or t.dtype != kind:
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} is not [batch, kv_heads, "
+                             f"slots, {'dim / 2' if codes else '2'}] of {kind} for k "
+                             f"{tuple(k.shape)}")
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{what}: the cache must be contiguous and 16-byte aligned (it is "
+                             "updated in place)")
+    if batch * slots > native.MAX_SEQUENCE_TOKENS:
+        raise ValueError(f"{what}: caches of {batch} x {slots} slots, at most "
+                         f"{native.MAX_SEQUENCE_TOKENS} in all are supported")
+    first, valid = _step_checks(what, batch, slots, positions, first, valid, cache_valid)
+    positions = positions.contiguous()
+    q, k, v = _strided(q), _strided(k), _strided(v)
+    out = q.new_empty((batch, heads, dim))
+    args = _arguments(native.WindowAttentionStep4BitArgs, q, k, v, batch=batch, heads=heads,
+                      kv_heads=kv_heads, dim=dim, dtype=dtype, slots=slots, first=first,
+                      scale=_scale(what, scale, dim), positions=positions.data_ptr(),
+                      out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid),
+                      **{name: t.data_ptr() for name, t in cache._asdict().items()})
+    call("gs_window_attention_step_4bit", device, ctypes.byref(args))
+    changed_in_place(*cache, cache_valid)
     return out

@@ -31,6 +31,7 @@ int32_t launch_det_math(int, int64_t, const float*, float*, cudaStream_t);
 int32_t launch_window_attention(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_backward(const gs_window_attention_args&, cudaStream_t);
 int32_t launch_window_attention_step(const gs_window_attention_step_args&, cudaStream_t);
+int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_args&, cudaStream_t);
 uint64_t window_attention_workspace_size(const gs_window_attention_args&);
 int32_t window_attention_status(cudaStream_t);
 int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
@@ -42,6 +43,10 @@ int32_t gated_scan_status(cudaStream_t);
 int32_t launch_rms_norm(const gs_rms_norm_args&, cudaStream_t);
 int32_t launch_rms_norm_backward(const gs_rms_norm_args&, cudaStream_t);
 uint64_t rms_norm_workspace_size(int64_t, int64_t);
+int32_t launch_linear(const gs_linear_args&, cudaStream_t);
+int32_t launch_linear_backward(const gs_linear_args&, cudaStream_t);
+uint64_t linear_workspace_size(const gs_linear_args&);
+int32_t linear_status(cudaStream_t);
 uint64_t bin_count_workspace_size(int64_t);
 uint64_t bin_sort_workspace_size(int64_t, int64_t, const gs_params&);
 uint64_t bin_error_word_offset();
@@ -66,7 +71,10 @@ int32_t launch_composite_bwd_deterministic(int64_t, int64_t, const float*, const
                                            const int32_t*, cudaStream_t);
 int32_t launch_adam_step(int64_t, int32_t, const gs_splat_arrays&, const gs_splat_arrays&,
                          const gs_splat_arrays&, const gs_splat_arrays&, const gs_adam_params&,
-                         const float*, cudaStream_t);
+                         const float*, const float*, cudaStream_t);
+uint64_t clip_grad_norm_workspace_size(int64_t);
+int32_t launch_clip_grad_norm(int64_t, const gs_gradient*, double, bool, float*, void*, uint64_t,
+                              cudaStream_t);
 int32_t launch_project_bwd_peers(int64_t, int32_t, int32_t, const float*, const float*,
                                  const float*, const float*, const float*, const void*,
                                  const float* const*, const int32_t* const*, float*, float*,
@@ -332,10 +340,10 @@ int32_t gs_project_bwd(int64_t n, int32_t num_sh, const float* mean, const float
                                 grad_scale, grad_opacity, grad_color, as_cuda(stream));
 }
 
-int32_t gs_adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays* params,
-                     const gs_splat_arrays* grads, const gs_splat_arrays* exp_avg,
-                     const gs_splat_arrays* exp_avg_sq, const gs_adam_params* hyper,
-                     const float* randn, gs_stream_t stream) {
+static int32_t adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays* params,
+                         const gs_splat_arrays* grads, const gs_splat_arrays* exp_avg,
+                         const gs_splat_arrays* exp_avg_sq, const gs_adam_params* hyper,
+                         const float* randn, const float* factor, gs_stream_t stream) {
   if (!params || !grads || !exp_avg || !exp_avg_sq || !hyper) return GS_ERR_INVALID_ARGUMENT;
   if (n < 0 || n >= gs::kMaxGaussians) return GS_ERR_INVALID_ARGUMENT;
   if (num_sh < 1 || num_sh > 25) return GS_ERR_INVALID_ARGUMENT;
@@ -347,7 +355,34 @@ int32_t gs_adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays* params,
   }
   if (grads->color && !gs::aligned(grads->color, 16)) return GS_ERR_MISALIGNED;
   return gs::launch_adam_step(n, num_sh, *params, *grads, *exp_avg, *exp_avg_sq, *hyper, randn,
-                              as_cuda(stream));
+                              factor, as_cuda(stream));
+}
+
+int32_t gs_adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays* params,
+                     const gs_splat_arrays* grads, const gs_splat_arrays* exp_avg,
+                     const gs_splat_arrays* exp_avg_sq, const gs_adam_params* hyper,
+                     const float* randn, gs_stream_t stream) {
+  return adam_step(n, num_sh, params, grads, exp_avg, exp_avg_sq, hyper, randn, nullptr, stream);
+}
+
+int32_t gs_adam_step_clipped(int64_t n, int32_t num_sh, const gs_splat_arrays* params,
+                             const gs_splat_arrays* grads, const gs_splat_arrays* exp_avg,
+                             const gs_splat_arrays* exp_avg_sq, const gs_adam_params* hyper,
+                             const float* randn, const float* factor, gs_stream_t stream) {
+  if (!factor) return GS_ERR_INVALID_ARGUMENT;
+  if (!gs::aligned(factor, 4)) return GS_ERR_MISALIGNED;
+  return adam_step(n, num_sh, params, grads, exp_avg, exp_avg_sq, hyper, randn, factor, stream);
+}
+
+uint64_t gs_clip_grad_norm_workspace_size(int64_t tensors) {
+  return tensors < 1 ? 0 : gs::clip_grad_norm_workspace_size(tensors);
+}
+
+int32_t gs_clip_grad_norm(int64_t tensors, const gs_gradient* list, double max_norm,
+                          int32_t scale, float* result, void* workspace,
+                          uint64_t workspace_size, gs_stream_t stream) {
+  return gs::launch_clip_grad_norm(tensors, list, max_norm, scale != 0, result, workspace,
+                                   workspace_size, as_cuda(stream));
 }
 
 int32_t gs_project_bwd_views(int64_t n, int32_t num_sh, int32_t num_views, const float* mean,
@@ -544,6 +579,12 @@ int32_t gs_window_attention_status(gs_stream_t stream) {
   return gs::window_attention_status(as_cuda(stream));
 }
 
+int32_t gs_window_attention_step_4bit(const gs_window_attention_step_4bit_args* args,
+                                      gs_stream_t stream) {
+  return args ? gs::launch_window_attention_step_4bit(*args, as_cuda(stream))
+              : GS_ERR_INVALID_ARGUMENT;
+}
+
 uint64_t gs_gated_scan_workspace_size(const gs_gated_scan_args* a) {
   return !a || a->num_tiles < 0 || a->channels < 1 || a->sequences < 1
              ? 0
@@ -580,6 +621,20 @@ int32_t gs_rms_norm(const gs_rms_norm_args* args, gs_stream_t stream) {
 int32_t gs_rms_norm_backward(const gs_rms_norm_args* args, gs_stream_t stream) {
   return args ? gs::launch_rms_norm_backward(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
 }
+
+uint64_t gs_linear_workspace_size(const gs_linear_args* a) {
+  return a ? gs::linear_workspace_size(*a) : 0;
+}
+
+int32_t gs_linear(const gs_linear_args* args, gs_stream_t stream) {
+  return args ? gs::launch_linear(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_linear_backward(const gs_linear_args* args, gs_stream_t stream) {
+  return args ? gs::launch_linear_backward(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_linear_status(gs_stream_t stream) { return gs::linear_status(as_cuda(stream)); }
 
 int32_t gs_det_exp(int64_t n, const float* x, float* y, gs_stream_t stream) {
   if (n < 0) return GS_ERR_INVALID_ARGUMENT;

@@ -1,0 +1,575 @@
+// A linear layer with its epilogue, and its gradients.
+//
+//   z = x W^T + b,  y = act(z) + residual
+//   dz = grad_y act'(z),  dx = dz W,  dW = dz^T x,  db = sum of dz over the rows
+//
+// One product kernel makes all three products D = A B^T on the tensor cores: tiles of
+// 128 x kN, operands by TMA, sums in tensor memory. x W^T contracts along the channels
+// of both operands, dz W along W's rows, dz^T x along the rows of both (an operand's
+// descriptor says which, nothing is transposed).
+#include "tensorcore.cuh"
+
+namespace gs {
+namespace {
+
+using namespace tc;
+
+// ---------------------------------------------------------------- activations
+
+// act'(z) is kept in 16 bits, as (slope + 1/6) 49152: slopes lie in [-0.13, 1.13], so
+// the error is 1.02e-5 at most, where float16's would be 2.4e-4 next to 1 and add
+// to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact. (A
+// float32 bias's gradient is a sum of unrounded dz: there slopes are kept as floats.)
+constexpr float kSlopeScale = 49152.0f, kSlopeZero = 8192.0f, kTwo23 = 8388608.0f;
+__device__ __forceinline__ uint32_t slope_code(float slope) {
+  // The sum's low bits are the nearest whole number.
+  return __float_as_uint(fmaf(slope, kSlopeScale, kTwo23 + kSlopeZero)) & 0xffffu;
+}
+__device__ __forceinline__ float slope_value(uint32_t code) {
+  return (__uint_as_float(0x4b000000u | code) - (kTwo23 + kSlopeZero)) * (1.0f / kSlopeScale);
+}
+
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(z) in z, act'(z) in slope.
+//
+// gelu: with t = |z|, the normal distribution's upper tail is e^(-t^2/2) R(t), R smooth
+// (Mills' ratio over sqrt(2 pi)); R = u P(u) with u = 1 / (1 + 0.3 t) and P the polynomial
+// of degree 7 with the least relative error for t up to 14, 1.5e-7. The density that
+// the slope needs is the same exponential.
+template <int kCount>
+__device__ __forceinline__ void activate(int kind, float (&z)[kCount], float (&slope)[kCount]) {
+  if (kind == GS_RELU) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      slope[i] = z[i] > 0.0f ? 1.0f : 0.0f;
+      z[i] = z[i] < 0.0f ? 0.0f : z[i];  // NaN stays
+    }
+  } else if (kind == GS_GELU) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const float t = fabsf(z[i]);
+      const float u = reciprocal_approx(fmaf(t, 0.3f, 1.0f));
+      const float e = exp2_approx(z[i] * z[i] * -0.72134752f);
+      float p = fmaf(0.0356748066842556f, u, -0.15720321238040924f);
+      p = fmaf(p, u, 0.20635370910167694f);
+      p = fmaf(p, u, -0.053683821111917496f);
+      p = fmaf(p, u, 0.12856172025203705f);
+      p = fmaf(p, u, 0.09991347044706345f);
+      p = fmaf(p, u, 0.12075395882129669f);
+      p = fmaf(p, u, 0.11962930113077164f);
+      const float tail = p * u * e;
+      const float below = z[i] < 0.0f ? tail : 1.0f - tail;
+      slope[i] = fmaf(z[i] * 0.39894228f, e, below);
+      z[i] = z[i] * below;
+    }
+  } else if (kind == GS_SILU) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const float gate = reciprocal_approx(1.0f + exp2_approx(z[i] * -1.44269504f));
+      const float y = z[i] * gate;
+      slope[i] = fmaf(y, 1.0f - gate, gate);
+      z[i] = y;
+    }
+  }
+}
+
+__device__ __forceinline__ float read_as(const void* p, int dtype, int64_t i) {
+  return dtype == GS_FLOAT32    ? static_cast<const float*>(p)[i]
+         : dtype == GS_BFLOAT16 ? to_float(static_cast<const __nv_bfloat16*>(p)[i])
+                                : to_float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void write_as(void* p, int dtype, int64_t i, float x) {
+  if (dtype == GS_FLOAT32) static_cast<float*>(p)[i] = x;
+  else if (dtype == GS_BFLOAT16) static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(x);
+  else static_cast<__half*>(p)[i] = from_float<__half>(x);
+}
+
+// ------------------------------------------------------------- product kernel
+
+// Set when a bounded wait ran out (linear_status).
+__device__ uint32_t g_timeout;
+
+constexpr int kRows = 128;   // of a tile
+constexpr int kDepth = 64;   // of a stage: 128 bytes of channels, or 64 rows
+constexpr int kEpilogueWarps = 8;
+constexpr int kProductThreads = 32 * (kEpilogueWarps + 2);
+
+// What becomes of the sums D(m, n).
+struct Epilogue {
+  int64_t rows;  // D's extents
+  int32_t columns;
+  void* out;
+  int64_t out_stride;
+  int32_t out_dtype;
+  // the forward's
+  int32_t activation, bias_dtype;
+  const void *bias, *residual;
+  int64_t residual_stride;
+  void* slope;
+  int64_t slope_stride;
+  bool slope_float;
+};
+
+// Items are (split, row tile, column tile), the last one fastest.
+struct Plan {
+  int32_t row_tiles, column_tiles, splits;
+  int32_t steps;            // of kDepth, in the whole contraction
+  int32_t steps_per_split;
+  int64_t split_rows;       // rows of `out` from one split's sums to the next one's
+};
+
+template <int kN>
+struct ProductShared {
+  static constexpr int kStages = kN == 256 ? 3 : 4;
+  static constexpr int kABytes = kRows * kDepth * 2, kBBytes = kN * kDepth * 2;
+  alignas(1024) unsigned char a[kStages][kABytes];
+  alignas(1024) unsigned char b[kStages][kBBytes];
+  alignas(1024) float out[kEpilogueWarps][32 * 32];
+  uint64_t full[kStages], empty[kStages], ready[2], drained[2];
+  uint32_t tensor;
+};
+
+// kRowsA, kRowsB: the operand's contraction runs along its rows.
+template <class T, int kN, bool kRowsA, bool kRowsB>
+__global__ void __launch_bounds__(kProductThreads, 1)
+    product_kernel(Plan plan, Epilogue e, const __grid_constant__ CUtensorMap a_map,
+                   const __grid_constant__ CUtensorMap b_map) {
+  using Shared = ProductShared<kN>;
+  constexpr int kStages = Shared::kStages;
+  extern __shared__ __align__(1024) unsigned char shared_bytes[];
+  Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
+  chain_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 32 * kEpilogueWarps) {
+    for (int i = 0; i < kStages; ++i) {
+      barrier_init(shared_address(&s.full[i]), 1);
+      barrier_init(shared_address(&s.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(shared_address(&s.ready[i]), 1);
+      barrier_init(shared_address(&s.drained[i]), kEpilogueWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == kEpilogueWarps + 1) tensor_alloc<2 * kN>(shared_address(&s.tensor));
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tensor = s.tensor;
+  const int64_t tiles = int64_t{plan.row_tiles} * plan.column_tiles, items = tiles * plan.splits;
+  bool good = true;
+  const auto steps_of = [&](int64_t item) {
+    const int first = static_cast<int>(item / tiles) * plan.steps_per_split;
+    return min(plan.steps_per_split, plan.steps - first);
+  };
+
+  if (warp == kEpilogueWarps) {  // loads
+    if (lane == 0) {
+      uint32_t turn = 0;  // stages used so far
+      for (int64_t item = blockIdx.x; item < items && good; item += gridDim.x) {
+        const int tile = static_cast<int>(item % tiles);
+        const int m0 = tile / plan.column_tiles * kRows, n0 = tile % plan.column_tiles * kN;
+        const int first = static_cast<int>(item / tiles) * plan.steps_per_split;
+        const int steps = steps_of(item);
+        for (int k = 0; k < steps; ++k, ++turn) {
+          const uint32_t stage = turn % kStages, round = turn / kStages;
+          if (round > 0) good = barrier_wait(shared_address(&s.empty[stage]), (round - 1) & 1);
+          if (!good) break;
+          const uint32_t bar = shared_address(&s.full[stage]);
+          const uint32_t a = shared_address(s.a[stage]), b = shared_address(s.b[stage]);
+          const int k0 = (first + k) * kDepth;
+          barrier_expect(bar, Shared::kABytes + Shared::kBBytes);
+          if constexpr (kRowsA)
+            for (int i = 0; i < kRows / 64; ++i)
+              load_box(a + i * kDepth * 128, &a_map, m0 + 64 * i, k0, bar);
+          else
+            load_box(a, &a_map, k0, m0, bar);
+          if constexpr (kRowsB)
+            for (int i = 0; i < kN / 64; ++i)
+              load_box(b + i * kDepth * 128, &b_map, n0 + 64 * i, k0, bar);
+          else
+            load_box(b, &b_map, k0, n0, bar);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kEpilogueWarps + 1) {  // products
+    const uint32_t elected = elect_lane();
+    const uint32_t kind = product_kind<T>(kN, kRowsB) | (kRowsA ? 1u << 15 : 0u);
+    const uint32_t a_word = kRowsA ? rows_word<kDepth>(shared_address(s.a[0]))
+                                   : channels_word<kRows>(shared_address(s.a[0]));
+    const uint32_t b_word = kRowsB ? rows_word<kDepth>(shared_address(s.b[0]))
+                                   : channels_word<kN>(shared_address(s.b[0]));
+    uint32_t turn = 0, count = 0;
+    for (int64_t item = blockIdx.x; item < items && good; item += gridDim.x, ++count) {
+      const uint32_t buffer = count & 1, round = count >> 1;
+      const int steps = steps_of(item);
+      if (round > 0)
+        good = barrier_wait_warp(shared_address(&s.drained[buffer]), (round - 1) & 1);
+      fence_after_sync();
+      for (int k = 0; k < steps && good; ++k, ++turn) {
+        const uint32_t stage = turn % kStages;
+        good = barrier_wait_warp(shared_address(&s.full[stage]), turn / kStages & 1);
+        if (!good) break;
+        fence_after_sync();
+        const uint32_t a = a_word + stage * (Shared::kABytes >> 4);
+        const uint32_t b = b_word + stage * (Shared::kBBytes >> 4);
+#pragma unroll
+        for (int i = 0; i < kDepth / 16; ++i)
+          multiply(elected, tensor + buffer * kN,
+                   a + (kRowsA ? rows_step(i) : channels_step<kRows>(i)),
+                   b + (kRowsB ? rows_step(i) : channels_step<kN>(i)), kind, k > 0 || i > 0);
+        commit(elected, shared_address(&s.empty[stage]));
+      }
+      if (good) commit(elected, shared_address(&s.ready[buffer]));
+    }
+  } else {  // epilogue: a row a thread, 32 columns at a time
+    float* const staged = s.out[warp];
+    uint32_t count = 0;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
+      const int tile = static_cast<int>(item % tiles);
+      const int64_t split = item / tiles;
+      const int64_t m0 = int64_t{tile / plan.column_tiles} * kRows + 32 * (warp & 3);
+      const int n0 = tile % plan.column_tiles * kN;
+      const uint32_t buffer = count & 1;
+      good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
+      fence_after_sync();
+      for (int c = warp >> 2; c < kN / 32; c += 2) {
+        float z[32], slope[32];
+        load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * c,
+                       z);
+        wait_loads();
+        if (!good)
+          for (float& x : z) x = NAN;
+        const int n = n0 + 32 * c;
+        if (n >= e.columns) continue;
+        if (e.bias)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            z[i] += n + i < e.columns ? read_as(e.bias, e.bias_dtype, n + i) : 0.0f;
+        activate(e.activation, z, slope);
+        // Through shared memory, so that a warp writes 32 columns of one row at a time.
+        const auto store = [&](const float(&x)[32], auto&& put) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) staged[32 * lane + (i ^ lane)] = x[i];
+          __syncwarp();
+          if (n + lane < e.columns)
+            for (int r = 0; r < 32 && m0 + r < e.rows; ++r)
+              put(m0 + r, n + lane, staged[32 * r + (lane ^ r)]);
+        };
+        store(z, [&](int64_t m, int64_t column, float y) {
+          if (e.residual) y += read_as(e.residual, e.out_dtype, m * e.residual_stride + column);
+          write_as(e.out, e.out_dtype, (split * plan.split_rows + m) * e.out_stride + column, y);
+        });
+        if (e.slope)
+          store(slope, [&](int64_t m, int64_t column, float x) {
+            if (e.slope_float) static_cast<float*>(e.slope)[m * e.slope_stride + column] = x;
+            else
+              static_cast<uint16_t*>(e.slope)[m * e.slope_stride + column] =
+                  static_cast<uint16_t>(slope_code(x));
+          });
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_address(&s.drained[buffer]));
+    }
+  }
+  if (!good) {  // let what is in flight land
+    for (uint64_t& bar : s.full) barrier_settle(shared_address(&bar));
+    for (uint64_t& bar : s.empty) barrier_settle(shared_address(&bar));
+    for (uint64_t& bar : s.ready) barrier_settle(shared_address(&bar));
+    if (lane == 0) atomicExch(&g_timeout, 1u);
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (warp == kEpilogueWarps + 1) tensor_free<2 * kN>(tensor);
+}
+
+// An operand: a [rows, channels] array of 16-bit elements, and whether the
+// contraction runs along its rows.
+struct Operand {
+  const void* data;
+  int64_t rows, channels, stride;
+};
+
+int32_t encode_operand(CUtensorMap* map, int32_t dtype, const Operand& o, int box_rows) {
+  const cuuint64_t size[2] = {static_cast<cuuint64_t>(o.channels), static_cast<cuuint64_t>(o.rows)};
+  const cuuint64_t stride[1] = {static_cast<cuuint64_t>(o.stride) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  return encode(map, dtype, o.data, 2, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <class T, int kN, bool kRowsA, bool kRowsB>
+int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan,
+                       const Epilogue& e, cudaStream_t stream) {
+  CUtensorMap a_map, b_map;
+  GS_TRY(encode_operand(&a_map, dtype, a, kRowsA ? kDepth : kRows));
+  GS_TRY(encode_operand(&b_map, dtype, b, kRowsB ? kDepth : kN));
+  constexpr size_t kShared = sizeof(ProductShared<kN>);
+  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB>>(kShared)));
+  const int64_t items = int64_t{plan.row_tiles} * plan.column_tiles * plan.splits;
+  launch_chained_shared(product_kernel<T, kN, kRowsA, kRowsB>,
+                        dim3(static_cast<unsigned>(items < kSmCount ? items : kSmCount)),
+                        dim3(kProductThreads), kShared, stream, plan, e, a_map, b_map);
+  return check_launch();
+}
+
+int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+Plan plan_of(int64_t rows, int64_t columns, int64_t depth, int n, int splits) {
+  Plan p = {};
+  p.row_tiles = static_cast<int32_t>(ceil_div(rows, kRows));
+  p.column_tiles = static_cast<int32_t>(ceil_div(columns, n));
+  p.steps = static_cast<int32_t>(ceil_div(depth, kDepth));
+  p.steps_per_split = static_cast<int32_t>(ceil_div(p.steps, splits));
+  p.splits = static_cast<int32_t>(ceil_div(p.steps, p.steps_per_split));
+  p.split_rows = int64_t{p.row_tiles} * kRows;
+  return p;
+}
+
+// The tile's columns: the widest of which there are enough tiles for every
+// multiprocessor, or the narrowest.
+int columns_of(int64_t rows, int64_t columns, int splits, int least) {
+  int n = 256;
+  while (n > least && (n / 2 >= columns || int64_t{ceil_div(rows, kRows)} * ceil_div(columns, n) *
+                                                   splits < kSmCount))
+    n /= 2;
+  return n;
+}
+
+// D = A B^T by `e`, with tiles of n columns.
+template <class T, bool kRowsA, bool kRowsB>
+int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan, int n,
+                    const Epilogue& e, cudaStream_t stream) {
+  switch (n) {
+    case 256: return launch_product<T, 256, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+    case 128: return launch_product<T, 128, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+    case 64: return launch_product<T, 64, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+    case 32:
+      if constexpr (!kRowsB)
+        return launch_product<T, 32, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+  }
+  return GS_ERR_UNSUPPORTED;
+}
+
+// ------------------------------------------------- the gradient of the sums
+
+constexpr int kSlopeThreads = 256;
+constexpr int kSlopeRows = 512;  // of a strip
+
+// dz = grad_y act'(z) rounded to the operands' type, and each strip's sums of its columns
+// (of what was not rounded).
+template <class T, class G>
+__global__ void __launch_bounds__(kSlopeThreads)
+    slope_kernel(gs_linear_args a, int64_t stride, bool slope_float, T* dz, float* sums) {
+  chain_wait();
+  const int64_t column = blockIdx.y * int64_t{kSlopeThreads} + threadIdx.x;
+  const int64_t row0 = blockIdx.x * int64_t{kSlopeRows};
+  if (column >= a.outputs) return;
+  float sum = 0.0f;
+  for (int64_t m = row0; m < row0 + kSlopeRows && m < a.rows; ++m) {
+    float g = to_float(static_cast<const G*>(a.grad_y)[m * a.outputs + column]);
+    if (a.slope)
+      g *= slope_float ? static_cast<const float*>(a.slope)[m * stride + column]
+                       : slope_value(static_cast<const uint16_t*>(a.slope)[m * stride + column]);
+    sum += g;
+    if (dz) dz[m * stride + column] = from_float<T>(g);
+  }
+  if (sums) sums[blockIdx.x * int64_t{a.outputs} + column] = sum;
+}
+
+// The sums of the splits, or of the strips, in order, rounded to the result's type.
+__global__ void __launch_bounds__(256)
+    join_kernel(const float* parts, int count, int64_t part_size, int64_t rows, int columns,
+                int64_t stride, void* out, int dtype) {
+  chain_wait();
+  const int64_t at = blockIdx.x * int64_t{256} + threadIdx.x;
+  if (at >= rows * columns) return;
+  const int64_t from = at / columns * stride + at % columns;
+  float sum = 0.0f;
+  for (int i = 0; i < count; ++i) sum += parts[i * part_size + from];
+  write_as(out, dtype, at, sum);
+}
+
+// --------------------------------------------------------------------- host
+
+int32_t check_args(const gs_linear_args& a) {
+  if (a.rows < 0 || a.rows > GS_MAX_SEQUENCE_TOKENS || a.inputs < 1 ||
+      a.inputs > GS_MAX_LINEAR_FEATURES || a.outputs < 1 || a.outputs > GS_MAX_LINEAR_FEATURES ||
+      a.activation < GS_IDENTITY || a.activation > GS_SILU)
+    return GS_ERR_INVALID_ARGUMENT;
+  if (a.dtype != GS_BFLOAT16 && a.dtype != GS_FLOAT16) return GS_ERR_UNSUPPORTED;
+  for (int32_t t : {a.bias_dtype, a.residual_dtype})
+    if (t != a.dtype && t != GS_FLOAT32) return GS_ERR_INVALID_ARGUMENT;
+  if (!a.weight || (a.rows > 0 && !a.x)) return GS_ERR_INVALID_ARGUMENT;
+  if (a.x_stride < a.inputs || a.weight_stride < a.inputs) return GS_ERR_INVALID_ARGUMENT;
+  if (!is_aligned(a.x, 16) || !is_aligned(a.weight, 16) || a.x_stride % 8 || a.weight_stride % 8)
+    return GS_ERR_MISALIGNED;
+  return GS_OK;
+}
+
+template <class F>
+int32_t with_sixteen_bit(int32_t dtype, F&& f) {
+  return dtype == GS_BFLOAT16 ? f(__nv_bfloat16{}) : f(__half{});
+}
+
+int64_t slope_stride(const gs_linear_args& a) { return round_up(a.outputs, 8); }
+
+// The backward's workspace: dz (where grad_y cannot be read in its place), the strips'
+// sums of dz, the splits' sums of dz^T x.
+struct BackwardPlan {
+  bool own_dz;
+  int64_t strips;
+  int columns, x_columns;
+  Plan weight, x;
+  uint64_t dz, sums, parts, size;  // byte offsets, and the whole
+};
+
+BackwardPlan backward_plan(const gs_linear_args& a) {
+  BackwardPlan p = {};
+  if (a.rows == 0) return p;
+  p.own_dz = a.activation != GS_IDENTITY || a.residual_dtype != a.dtype || a.outputs % 8 != 0;
+  p.strips = ceil_div(a.rows, kSlopeRows);
+  // The weight's gradient has few tiles and a long contraction: split so that the items
+  // are about one a multiprocessor.
+  p.columns = columns_of(a.outputs, a.inputs, 1 << 20, 64);
+  const int64_t tiles = int64_t{ceil_div(a.outputs, kRows)} * ceil_div(a.inputs, p.columns);
+  const int64_t splits = kSmCount / tiles;
+  p.weight = plan_of(a.outputs, a.inputs, a.rows, p.columns,
+                     static_cast<int>(splits < 1 ? 1 : splits));
+  p.x_columns = columns_of(a.rows, a.inputs, 1, 64);
+  p.x = plan_of(a.rows, a.inputs, a.outputs, p.x_columns, 1);
+  uint64_t at = 0;
+  const auto take = [&](uint64_t bytes) {
+    const uint64_t from = at;
+    at += (bytes + 255) / 256 * 256;
+    return from;
+  };
+  p.dz = take(p.own_dz ? static_cast<uint64_t>(a.rows) * slope_stride(a) * 2 : 0);
+  p.sums = take(static_cast<uint64_t>(p.strips) * a.outputs * 4);
+  p.parts = take(static_cast<uint64_t>(p.weight.splits) * p.weight.split_rows *
+                 round_up(a.inputs, 4) * 4);
+  p.size = at;
+  return p;
+}
+
+}  // namespace
+
+uint64_t linear_workspace_size(const gs_linear_args& a) {
+  return check_args(a) == GS_OK ? backward_plan(a).size : 0;
+}
+
+int32_t linear_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
+
+int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
+  GS_TRY(check_args(a));
+  if (a.rows == 0) return GS_OK;
+  if (!a.y) return GS_ERR_INVALID_ARGUMENT;
+  Epilogue e = {};
+  e.rows = a.rows;
+  e.columns = a.outputs;
+  e.out = a.y;
+  e.out_stride = a.outputs;
+  e.out_dtype = a.residual_dtype;
+  e.activation = a.activation;
+  e.bias = a.bias;
+  e.bias_dtype = a.bias_dtype;
+  e.residual = a.residual;
+  e.residual_stride = a.residual_stride;
+  e.slope = a.activation == GS_IDENTITY ? nullptr : a.slope;
+  e.slope_stride = slope_stride(a);
+  e.slope_float = a.bias && a.bias_dtype == GS_FLOAT32;
+  const int n = columns_of(a.rows, a.outputs, 1, 32);
+  return with_sixteen_bit(a.dtype, [&](auto t) {
+    return run_product<decltype(t), false, false>(
+        a.dtype, {a.x, a.rows, a.inputs, a.x_stride},
+        {a.weight, a.outputs, a.inputs, a.weight_stride},
+        plan_of(a.rows, a.outputs, a.inputs, n, 1), n, e, stream);
+  });
+}
+
+int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
+  GS_TRY(check_args(a));
+  if (a.rows > 0 && (!a.grad_y || !a.workspace || (a.activation != GS_IDENTITY && !a.slope)))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (!is_aligned(a.grad_y, 16) || !is_aligned(a.slope, 16) || !is_aligned(a.workspace, 256))
+    return GS_ERR_MISALIGNED;
+  const BackwardPlan p = backward_plan(a);
+  if (a.workspace_size < p.size) return GS_ERR_CAPACITY;
+  if (a.rows == 0) {
+    if (a.grad_weight)
+      GS_CUDA_TRY(cudaMemsetAsync(a.grad_weight, 0, int64_t{a.inputs} * a.outputs * 2, stream));
+    if (a.grad_bias)
+      GS_CUDA_TRY(cudaMemsetAsync(a.grad_bias, 0, int64_t{a.outputs} * element_size(a.bias_dtype),
+                                  stream));
+    return GS_OK;
+  }
+  unsigned char* const work = static_cast<unsigned char*>(a.workspace);
+  float* const sums = a.grad_bias ? reinterpret_cast<float*>(work + p.sums) : nullptr;
+  float* const parts = reinterpret_cast<float*>(work + p.parts);
+  void* const dz = p.own_dz ? work + p.dz : const_cast<void*>(a.grad_y);
+  const bool products = a.grad_x || a.grad_weight;
+  const Operand dz_operand = {dz, a.rows, a.outputs, p.own_dz ? slope_stride(a) : a.outputs};
+  return with_sixteen_bit(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    if ((p.own_dz && products) || sums) {
+      const dim3 grid(static_cast<unsigned>(p.strips), ceil_div(a.outputs, kSlopeThreads));
+      const bool slope_float = a.bias && a.bias_dtype == GS_FLOAT32;
+      gs_linear_args b = a;
+      if (a.activation == GS_IDENTITY) b.slope = nullptr;
+      T* const to = p.own_dz && products ? static_cast<T*>(dz) : nullptr;
+      if (a.residual_dtype == GS_FLOAT32)
+        launch_chained(slope_kernel<T, float>, grid, kSlopeThreads, stream, b, slope_stride(a),
+                       slope_float, to, sums);
+      else
+        launch_chained(slope_kernel<T, T>, grid, kSlopeThreads, stream, b, slope_stride(a),
+                       slope_float, to, sums);
+      GS_TRY(check_launch());
+    }
+    if (a.grad_bias) {
+      launch_chained(join_kernel, ceil_div(a.outputs, 256), 256, stream,
+                     static_cast<const float*>(sums), static_cast<int>(p.strips),
+                     int64_t{a.outputs}, int64_t{1}, a.outputs, int64_t{a.outputs}, a.grad_bias,
+                     a.bias_dtype);
+      GS_TRY(check_launch());
+    }
+    if (a.grad_x) {
+      Epilogue e = {};
+      e.rows = a.rows;
+      e.columns = a.inputs;
+      e.out = a.grad_x;
+      e.out_stride = a.inputs;
+      e.out_dtype = a.dtype;
+      GS_TRY((run_product<T, false, true>(a.dtype, dz_operand,
+                                          {a.weight, a.outputs, a.inputs, a.weight_stride}, p.x,
+                                          p.x_columns, e, stream)));
+    }
+    if (a.grad_weight) {
+      Epilogue e = {};
+      e.rows = a.outputs;
+      e.columns = a.inputs;
+      e.out = parts;
+      e.out_stride = round_up(a.inputs, 4);
+      e.out_dtype = GS_FLOAT32;
+      GS_TRY((run_product<T, true, true>(a.dtype, dz_operand,
+                                         {a.x, a.rows, a.inputs, a.x_stride}, p.weight, p.columns,
+                                         e, stream)));
+      launch_chained(join_kernel, ceil_div(int64_t{a.outputs} * a.inputs, 256), 256, stream,
+                     static_cast<const float*>(parts), p.weight.splits,
+                     p.weight.split_rows * round_up(a.inputs, 4), int64_t{a.outputs}, a.inputs,
+                     round_up(a.inputs, 4), a.grad_weight, a.dtype);
+      GS_TRY(check_launch());
+    }
+    return static_cast<int32_t>(GS_OK);
+  });
+}
+
+}  // namespace gs

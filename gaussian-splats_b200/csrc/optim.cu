@@ -47,7 +47,10 @@ __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + det_ex
 template <bool kNoise>
 __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
     int64_t n, int64_t color_per, gs_splat_arrays p, gs_splat_arrays g, gs_splat_arrays m,
-    gs_splat_arrays v, gs_adam_params hp, const float* __restrict__ randn) {
+    gs_splat_arrays v, gs_adam_params hp, const float* __restrict__ randn,
+    const float* __restrict__ factor) {
+  // What clips the gradients; 1 leaves each of them as it is.
+  const float f = factor ? *factor : 1.0f;
   const Moments c{hp.lerp_weight, hp.beta2, hp.sq_weight, hp.eps};
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kOptThreads + threadIdx.x;
   if (i < n) {
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
         float mk = m.mean[3 * i + k], vk = v.mean[3 * i + k];
-        mean[k] = adam_one(mean[k], g.mean[3 * i + k], mk, vk, hp.neg_step_size[0], hp.bias2_sqrt[0], c);
+        mean[k] = adam_one(mean[k], f * g.mean[3 * i + k], mk, vk, hp.neg_step_size[0], hp.bias2_sqrt[0], c);
         m.mean[3 * i + k] = mk;
         v.mean[3 * i + k] = vk;
       }
@@ -72,7 +75,7 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float mk = m.rotation[4 * i + k], vk = v.rotation[4 * i + k];
-        rot[k] = adam_one(rot[k], g.rotation[4 * i + k], mk, vk, hp.neg_step_size[1], hp.bias2_sqrt[1], c);
+        rot[k] = adam_one(rot[k], f * g.rotation[4 * i + k], mk, vk, hp.neg_step_size[1], hp.bias2_sqrt[1], c);
         m.rotation[4 * i + k] = mk;
         v.rotation[4 * i + k] = vk;
         p.rotation[4 * i + k] = rot[k];
@@ -82,7 +85,7 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
         float mk = m.scale[3 * i + k], vk = v.scale[3 * i + k];
-        scale[k] = adam_one(scale[k], g.scale[3 * i + k], mk, vk, hp.neg_step_size[2], hp.bias2_sqrt[2], c);
+        scale[k] = adam_one(scale[k], f * g.scale[3 * i + k], mk, vk, hp.neg_step_size[2], hp.bias2_sqrt[2], c);
         m.scale[3 * i + k] = mk;
         v.scale[3 * i + k] = vk;
         p.scale[3 * i + k] = scale[k];
@@ -90,7 +93,7 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
     }
     if (g.opacity) {
       float mk = m.opacity[i], vk = v.opacity[i];
-      opacity = adam_one(opacity, g.opacity[i], mk, vk, hp.neg_step_size[3], hp.bias2_sqrt[3], c);
+      opacity = adam_one(opacity, f * g.opacity[i], mk, vk, hp.neg_step_size[3], hp.bias2_sqrt[3], c);
       m.opacity[i] = mk;
       v.opacity[i] = vk;
       p.opacity[i] = opacity;
@@ -144,17 +147,17 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
     const float4 gg = *reinterpret_cast<const float4*>(g.color + e);
     float4 mm = *reinterpret_cast<const float4*>(m.color + e);
     float4 vv = *reinterpret_cast<const float4*>(v.color + e);
-    pp.x = adam_one(pp.x, gg.x, mm.x, vv.x, ns, bs, c);
-    pp.y = adam_one(pp.y, gg.y, mm.y, vv.y, ns, bs, c);
-    pp.z = adam_one(pp.z, gg.z, mm.z, vv.z, ns, bs, c);
-    pp.w = adam_one(pp.w, gg.w, mm.w, vv.w, ns, bs, c);
+    pp.x = adam_one(pp.x, f * gg.x, mm.x, vv.x, ns, bs, c);
+    pp.y = adam_one(pp.y, f * gg.y, mm.y, vv.y, ns, bs, c);
+    pp.z = adam_one(pp.z, f * gg.z, mm.z, vv.z, ns, bs, c);
+    pp.w = adam_one(pp.w, f * gg.w, mm.w, vv.w, ns, bs, c);
     *reinterpret_cast<float4*>(p.color + e) = pp;
     *reinterpret_cast<float4*>(m.color + e) = mm;
     *reinterpret_cast<float4*>(v.color + e) = vv;
   }
   for (; e < c1; ++e) {  // the ragged end of the last CTA's run
     float mk = m.color[e], vk = v.color[e];
-    p.color[e] = adam_one(p.color[e], g.color[e], mk, vk, ns, bs, c);
+    p.color[e] = adam_one(p.color[e], f * g.color[e], mk, vk, ns, bs, c);
     m.color[e] = mk;
     v.color[e] = vk;
   }
@@ -165,16 +168,16 @@ __global__ void __launch_bounds__(kOptThreads) adam_step_kernel(
 int32_t launch_adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays& p,
                          const gs_splat_arrays& g, const gs_splat_arrays& m,
                          const gs_splat_arrays& v, const gs_adam_params& hp, const float* randn,
-                         cudaStream_t stream) {
+                         const float* factor, cudaStream_t stream) {
   if (n == 0) return GS_OK;
   const unsigned blocks = ceil_div(n, kOptThreads);
   const int64_t color_per = 3 * static_cast<int64_t>(num_sh);
   if (randn)
     adam_step_kernel<true><<<blocks, kOptThreads, 0, stream>>>(n, color_per, p, g, m, v, hp,
-                                                               randn);
+                                                               randn, factor);
   else
     adam_step_kernel<false><<<blocks, kOptThreads, 0, stream>>>(n, color_per, p, g, m, v, hp,
-                                                                nullptr);
+                                                                nullptr, factor);
   return check_launch();
 }
 

@@ -1,0 +1,137 @@
+"""A linear layer with what usually follows it in its epilogue.
+
+:func:`linear` computes ``act(x @ weight.T + bias) + residual`` in one kernel: the
+product's sums are biased, activated and added to the residual stream before they
+are rounded and written. Differentiable; the forward of a training pass also
+keeps the activation's slope, so that the backward needs neither the sums nor
+another product to make them again.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import native
+from .attention import _whole
+from .norm import _rows
+from .sequences import address, call, check_cuda, check_tokens, element_type
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}  # GS_IDENTITY, ...
+_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, channels] as the kernels read a product's operand: rows of contiguous
+    channels that start on 16-byte borders. ``t`` itself if it lies so, else a copy."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and \
+            t.data_ptr() % 16 == 0:
+        return t
+    rows, channels = t.shape
+    copy = t.new_empty((rows, -(-channels // 8) * 8))[:, :channels]
+    return copy.copy_(t)
+
+
+def _arguments(x, weight, bias, **values):
+    """``gs_linear_args`` of operands ``x`` and ``weight``."""
+    dtype = element_type(x.dtype, "")
+    return native.LinearArgs(
+        rows=x.shape[0], inputs=x.shape[1], outputs=weight.shape[0], dtype=dtype,
+        bias_dtype=dtype if bias is None else element_type(bias.dtype, ""),
+        x=address(x), weight=address(weight), bias=address(bias), x_stride=x.stride(0),
+        weight_stride=weight.stride(0), **values)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, train):
+        shape = x.shape[:-1] + weight.shape[:1]
+        rows, w = _operand(x.reshape(-1, x.shape[-1])), _operand(weight)
+        b = None if bias is None else bias.contiguous()
+        res = None if residual is None else _rows(residual)
+        y = (x if res is None else res).new_empty(shape)
+        slope = None
+        if train and activation:
+            exact = b is not None and b.dtype == torch.float32
+            slope = x.new_empty((rows.shape[0], -(-w.shape[0] // 8) * 8),
+                                dtype=torch.float32 if exact else torch.int16)
+        args = _arguments(rows, w, b, activation=activation,
+                          residual_dtype=element_type(y.dtype, ""), residual=address(res),
+                          residual_stride=0 if res is None else res.stride(0), y=address(y),
+                          slope=address(slope))
+        call("gs_linear", x.device, ctypes.byref(args))
+        if train:
+            ctx.save_for_backward(rows, w, b, slope)
+            ctx.activation, ctx.shape = activation, x.shape
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, bias, slope = ctx.saved_tensors
+        # A saved-tensor hook may have brought back tensors that lie differently.
+        x, weight = _operand(x), _operand(weight)
+        slope = None if slope is None else _whole(slope)
+        want_x, want_weight, want_bias, want_residual = ctx.needs_input_grad[:4]
+        grads = [x.new_empty(ctx.shape) if want_x else None,
+                 weight.new_empty(weight.shape) if want_weight else None,
+                 torch.empty_like(bias) if want_bias else None]
+        if want_x or want_weight or want_bias:
+            rows = _whole(grad_y.reshape(x.shape[0], weight.shape[0]))
+            args = _arguments(x, weight, bias, activation=ctx.activation,
+                              residual_dtype=element_type(rows.dtype, ""), slope=address(slope),
+                              grad_y=address(rows), grad_x=address(grads[0]),
+                              grad_weight=address(grads[1]), grad_bias=address(grads[2]))
+            size = native.lib().gs_linear_workspace_size(ctypes.byref(args))
+            workspace = x.new_empty((size,), dtype=torch.uint8)
+            args.workspace, args.workspace_size = address(workspace), size
+            call("gs_linear_backward", x.device, ctypes.byref(args))
+        return (*grads, grad_y if want_residual else None, None, None)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+           residual: torch.Tensor | None = None, *, activation: str | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` for ``x`` [..., inputs] and ``weight``
+    [outputs, inputs], any number of rows. ``activation`` is None, ``"relu"``,
+    ``"gelu"`` (``z`` times the normal distribution function of ``z``) or ``"silu"``.
+
+    x and weight are bfloat16 or float16 (one type), the bias [outputs] in their type
+    or float32, the residual [..., outputs] too; the result has the residual's type, or
+    x's where there is none: a float32 residual stream stays one. Sums, bias, activation
+    and the residual's addition are in float32, rounded once.
+
+    Differentiable in x, weight, bias and residual, and deterministic in both
+    directions. The backward rounds the gradient of the sums, ``grad * act'``, to the
+    inputs' type, as its products need; float16 gradients below 6e-8 vanish there, as in
+    any float16 tensor (scale the loss). Operands are read in place if their rows are
+    contiguous and start on 16-byte borders (any slice of a projection does whose
+    channels are multiples of 8) and copied otherwise."""
+    what = "linear"
+    device = check_cuda(what, x=x, weight=weight, bias=bias, residual=residual)
+    element_type(x.dtype, what, _TYPES)
+    if weight.dtype != x.dtype:
+        raise ValueError(f"{what}: weight of {weight.dtype} for x of {x.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: weight {tuple(weight.shape)} does not go with x "
+                         f"{tuple(x.shape)}")
+    outputs, inputs = weight.shape
+    if not (1 <= inputs <= native.MAX_LINEAR_FEATURES and
+            1 <= outputs <= native.MAX_LINEAR_FEATURES):
+        raise ValueError(f"{what}: 1 to {native.MAX_LINEAR_FEATURES} inputs and outputs are "
+                         f"supported, got {inputs} and {outputs}")
+    check_tokens(x.numel() // inputs, what)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be one of {tuple(ACTIVATIONS)}, got "
+                         f"{activation!r}")
+    for name, t, shape in (("bias", bias, (outputs,)),
+                           ("residual", residual, (*x.shape[:-1], outputs))):
+        if t is None:
+            continue
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} is not {shape}")
+        if t.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{what}: the {name} must be {x.dtype} or float32, got {t.dtype}")
+    train = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation], train)

@@ -48,6 +48,9 @@ EXPORTED_SYMBOLS = (
     "gs_project_bwd",
     "gs_project_bwd_views",
     "gs_adam_step",
+    "gs_adam_step_clipped",
+    "gs_clip_grad_norm",
+    "gs_clip_grad_norm_workspace_size",
     "gs_exchange_layout_for",
     "gs_exchange_begin",
     "gs_exchange_publish",
@@ -70,6 +73,7 @@ EXPORTED_SYMBOLS = (
     "gs_window_attention_backward",
     "gs_window_attention_status",
     "gs_window_attention_step",
+    "gs_window_attention_step_4bit",
     "gs_window_attention_workspace_size",
     "gs_gated_scan",
     "gs_gated_scan_backward",
@@ -79,6 +83,10 @@ EXPORTED_SYMBOLS = (
     "gs_rms_norm",
     "gs_rms_norm_backward",
     "gs_rms_norm_workspace_size",
+    "gs_linear",
+    "gs_linear_backward",
+    "gs_linear_status",
+    "gs_linear_workspace_size",
     "gs_det_exp",
     "gs_det_log",
 )
@@ -167,6 +175,12 @@ class AdamParams(ctypes.Structure):
         ("noise_lr", ctypes.c_float), ("position_lr", ctypes.c_float)]
 
 
+class Gradient(ctypes.Structure):
+    """``gs_gradient``: one tensor for ``gs_clip_grad_norm``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("count", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
 def adam_params(steps, lrs, betas, eps, noise_lr=0.0, position_lr=0.0) -> AdamParams:
     """Fold one Adam step for the five groups (mean, rotation, scale, opacity,
     color) with step numbers ``steps`` (1-based) and learning rates ``lrs`` the
@@ -187,6 +201,7 @@ def adam_params(steps, lrs, betas, eps, noise_lr=0.0, position_lr=0.0) -> AdamPa
 SEQUENCE_TILE = 128       # GS_SEQUENCE_TILE (include/gs_b200.h)
 MAX_FIRST_TOKENS = 128    # GS_MAX_FIRST_TOKENS
 MAX_NORM_CHANNELS = 16384  # GS_MAX_NORM_CHANNELS
+MAX_LINEAR_FEATURES = 65536  # GS_MAX_LINEAR_FEATURES
 MAX_SEQUENCE_TOKENS = 2 ** 31 - 512  # GS_MAX_SEQUENCE_TOKENS
 
 
@@ -218,6 +233,18 @@ class WindowAttentionStepArgs(ctypes.Structure):
                 _fields(ctypes.c_void_p, "cache_k cache_v positions out valid cache_valid"))
 
 
+class WindowAttentionStep4BitArgs(ctypes.Structure):
+    """``gs_window_attention_step_4bit_args``."""
+
+    _fields_ = (_fields(ctypes.c_int64, "batch") +
+                _fields(ctypes.c_int32, "heads kv_heads dim dtype slots first") +
+                _fields(ctypes.c_float, "scale") + _fields(ctypes.c_void_p, "q k v") +
+                _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "
+                                        "v_head_stride") +
+                _fields(ctypes.c_void_p, "k_codes v_codes k_range v_range positions out valid "
+                                         "cache_valid"))
+
+
 class GatedScanArgs(ctypes.Structure):
     """``gs_gated_scan_args``."""
 
@@ -239,6 +266,19 @@ class RmsNormArgs(ctypes.Structure):
                 _fields(ctypes.c_int64, "x_stride residual_stride sum_stride") +
                 _fields(ctypes.c_void_p, "y sum q scale grad_y grad_sum grad_x grad_residual "
                                          "grad_weight workspace") +
+                _fields(ctypes.c_uint64, "workspace_size"))
+
+
+class LinearArgs(ctypes.Structure):
+    """``gs_linear_args``."""
+
+    _fields_ = (_fields(ctypes.c_int64, "rows") +
+                _fields(ctypes.c_int32, "inputs outputs dtype bias_dtype residual_dtype "
+                                        "activation") +
+                _fields(ctypes.c_void_p, "x weight bias residual") +
+                _fields(ctypes.c_int64, "x_stride weight_stride residual_stride") +
+                _fields(ctypes.c_void_p, "y slope grad_y grad_x grad_weight grad_bias "
+                                         "workspace") +
                 _fields(ctypes.c_uint64, "workspace_size"))
 
 
@@ -309,6 +349,10 @@ def lib() -> ctypes.CDLL:
         "gs_project_bwd_views": ([i64, i32, i32] + [vp] * 13 + [vp], i32),
         "gs_adam_step": ([i64, i32] + [ctypes.POINTER(SplatArrays)] * 4 +
                          [ctypes.POINTER(AdamParams), vp, vp], i32),
+        "gs_adam_step_clipped": ([i64, i32] + [ctypes.POINTER(SplatArrays)] * 4 +
+                                 [ctypes.POINTER(AdamParams), vp, vp, vp], i32),
+        "gs_clip_grad_norm": ([i64, vp, ctypes.c_double, i32, vp, vp, u64, vp], i32),
+        "gs_clip_grad_norm_workspace_size": ([i64], u64),
         "gs_exchange_layout_for": ([i64, i32, ctypes.POINTER(ExchangeLayout)], i32),
         "gs_exchange_begin": ([ctypes.POINTER(PeerGroup), vp], i32),
         "gs_exchange_publish": ([ctypes.POINTER(PeerGroup), i64, vp], i32),
@@ -334,6 +378,7 @@ def lib() -> ctypes.CDLL:
         "gs_window_attention_backward": ([ctypes.POINTER(WindowAttentionArgs), vp], i32),
         "gs_window_attention_status": ([vp], i32),
         "gs_window_attention_step": ([ctypes.POINTER(WindowAttentionStepArgs), vp], i32),
+        "gs_window_attention_step_4bit": ([ctypes.POINTER(WindowAttentionStep4BitArgs), vp], i32),
         "gs_window_attention_workspace_size": ([ctypes.POINTER(WindowAttentionArgs)], u64),
         "gs_gated_scan": ([ctypes.POINTER(GatedScanArgs), vp], i32),
         "gs_gated_scan_backward": ([ctypes.POINTER(GatedScanArgs), vp], i32),
@@ -343,6 +388,10 @@ def lib() -> ctypes.CDLL:
         "gs_rms_norm": ([ctypes.POINTER(RmsNormArgs), vp], i32),
         "gs_rms_norm_backward": ([ctypes.POINTER(RmsNormArgs), vp], i32),
         "gs_rms_norm_workspace_size": ([ctypes.POINTER(RmsNormArgs)], u64),
+        "gs_linear": ([ctypes.POINTER(LinearArgs), vp], i32),
+        "gs_linear_backward": ([ctypes.POINTER(LinearArgs), vp], i32),
+        "gs_linear_status": ([vp], i32),
+        "gs_linear_workspace_size": ([ctypes.POINTER(LinearArgs)], u64),
         "gs_det_exp": ([i64, vp, vp, vp], i32),
         "gs_det_log": ([i64, vp, vp, vp], i32),
     }

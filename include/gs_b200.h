@@ -423,6 +423,36 @@ int32_t gs_adam_step(int64_t n, int32_t num_sh, const gs_splat_arrays *params,
                      const gs_splat_arrays *exp_avg_sq, const gs_adam_params *hyper,
                      const float *randn, gs_stream_t stream);
 
+/* The same step with every gradient multiplied by the device scalar `*factor` on
+ * the way (what gs_clip_grad_norm leaves in result[1]); the gradient arrays stay
+ * as they are. */
+int32_t gs_adam_step_clipped(int64_t n, int32_t num_sh, const gs_splat_arrays *params,
+                             const gs_splat_arrays *grads, const gs_splat_arrays *exp_avg,
+                             const gs_splat_arrays *exp_avg_sq, const gs_adam_params *hyper,
+                             const float *randn, const float *factor, gs_stream_t stream);
+
+/* A gradient for gs_clip_grad_norm: `count` contiguous elements at `data`, of an
+ * element type GS_FLOAT32, GS_BFLOAT16 or GS_FLOAT16 (below), any alignment that
+ * their type allows. */
+typedef struct gs_gradient {
+  void *data;
+  int64_t count;
+  int32_t dtype;
+} gs_gradient;
+
+/* The norm of all elements of `tensors` (1 to 2^20) gradients together, `list` a host
+ * array that is read before the call returns: result[0] = norm, result[1] = factor =
+ * min(1, max_norm / (norm + 1e-6)) (device floats; squares summed in double beyond 128
+ * bytes of elements, so that no norm over- or underflows on the way). `scale` != 0
+ * multiplies every element by the factor (the gradients must not overlap; a factor of
+ * 1 writes nothing); a NaN in a gradient makes norm and factor NaN, an infinity the
+ * factor 0. max_norm >= 0, infinity for the norm alone. The workspace is 8-byte
+ * aligned. Results repeat bit for bit. */
+uint64_t gs_clip_grad_norm_workspace_size(int64_t tensors);
+int32_t gs_clip_grad_norm(int64_t tensors, const gs_gradient *list, double max_norm,
+                          int32_t scale, float *result, void *workspace,
+                          uint64_t workspace_size, gs_stream_t stream);
+
 /* Workspace bytes gs_relocate needs for `n_src` counts (16-byte aligned). */
 uint64_t gs_relocate_workspace_size(int64_t n_src);
 
@@ -562,6 +592,31 @@ typedef struct gs_window_attention_step_args {
 
 int32_t gs_window_attention_step(const gs_window_attention_step_args *args, gs_stream_t stream);
 
+/* The same step against a cache held in 4 bits: k_codes, v_codes [batch, kv_heads, slots,
+ * dim / 2] (channel 2i in the low half of byte i, 2i + 1 in the high one) and k_range,
+ * v_range [batch, kv_heads, slots, 2] of `dtype`, all contiguous: a row's code c stands
+ * for (c - 7.5) * range[0] + range[1]. The new token's rows x are rounded into their slot:
+ * range = ((max x - min x) / 15, (max x + min x) / 2), each rounded to `dtype`, and c =
+ * (x - range[1]) / range[0] + 7.5, computed in double, rounded to the nearest, ties to
+ * even, and clamped to 0..15; 8 where range[0] is not positive and finite. The output is that of
+ * what the cache then holds. */
+typedef struct gs_window_attention_step_4bit_args {
+  int64_t batch;
+  int32_t heads, kv_heads, dim, dtype, slots, first;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+  uint8_t *k_codes, *v_codes;
+  void *k_range, *v_range;
+  const int64_t *positions;
+  void *out;
+  const uint8_t *valid;
+  uint8_t *cache_valid;
+} gs_window_attention_step_4bit_args;
+
+int32_t gs_window_attention_step_4bit(const gs_window_attention_step_4bit_args *args,
+                                      gs_stream_t stream);
+
 /* Gated linear recurrence per channel: h_t = (1 - a_t) h_{t-1} + a_t x_t with
  * a_t = sigmoid(gate_t), h_0 = initial [sequences, channels] float (NULL:
  * zeros). x, gate [tokens, channels] with row strides; y = h (dtype of x),
@@ -631,6 +686,41 @@ typedef struct gs_rms_norm_args {
 uint64_t gs_rms_norm_workspace_size(const gs_rms_norm_args *args);
 int32_t gs_rms_norm(const gs_rms_norm_args *args, gs_stream_t stream);
 int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
+
+/* A linear layer with its epilogue: z = x W^T + bias, y = act(z) + residual. x [rows,
+ * inputs] and weight [outputs, inputs] of `dtype` (GS_BFLOAT16 or GS_FLOAT16), 16-byte
+ * aligned, row strides multiples of 8; bias [outputs] of bias_dtype (may be NULL);
+ * residual [rows, outputs] of residual_dtype with a row stride (may be NULL); both
+ * types are dtype or GS_FLOAT32. y [rows, outputs] of residual_dtype, contiguous.
+ * `slope` [rows, outputs rounded up to 8], 16-byte aligned, receives act'(z) for the
+ * backward (NULL: not kept): floats where there is a bias of GS_FLOAT32, else 16 bits,
+ * (act' + 1/6) * 49152 rounded. Sums and epilogue in float.
+ *
+ * The backward reads x, weight, grad_y (contiguous, residual_dtype) and, unless the
+ * activation is GS_IDENTITY, slope, and writes those of grad_x [rows, inputs],
+ * grad_weight [outputs, inputs] (both of dtype, contiguous) and grad_bias [outputs]
+ * (bias_dtype) that are not NULL; what reaches the products is dz = grad_y act'(z)
+ * rounded to dtype. It needs a workspace of gs_linear_workspace_size bytes, 256-byte
+ * aligned. Outputs are 16-byte aligned. No atomics: results repeat bit for bit. */
+enum { GS_IDENTITY = 0, GS_RELU = 1, GS_GELU = 2, GS_SILU = 3 }; /* activations */
+enum { GS_MAX_LINEAR_FEATURES = 65536 };                         /* inputs, outputs */
+typedef struct gs_linear_args {
+  int64_t rows;
+  int32_t inputs, outputs, dtype, bias_dtype, residual_dtype, activation;
+  const void *x, *weight, *bias, *residual;
+  int64_t x_stride, weight_stride, residual_stride;
+  void *y, *slope;
+  const void *grad_y;
+  void *grad_x, *grad_weight, *grad_bias;
+  void *workspace;
+  uint64_t workspace_size;
+} gs_linear_args;
+
+uint64_t gs_linear_workspace_size(const gs_linear_args *args);
+int32_t gs_linear(const gs_linear_args *args, gs_stream_t stream);
+int32_t gs_linear_backward(const gs_linear_args *args, gs_stream_t stream);
+/* As gs_window_attention_status, for these products (the block's tiles hold NaN). */
+int32_t gs_linear_status(gs_stream_t stream);
 
 /* The deterministic exp / log the kernels use, applied elementwise (test hook
  * for bitwise agreement with the CPU oracle). */

@@ -1,0 +1,238 @@
+"""The step against a 4-bit cache, from its definition in 64 bits."""
+
+import pytest
+import torch
+
+import operator_reference as R
+
+pytestmark = pytest.mark.gpu
+
+U = R.U
+BF, HF = torch.bfloat16, torch.float16
+
+
+def rand(g, *shape, dtype, size=1.0):
+    return (size * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+
+def bound(dtype, dim, out, spread, size, scores):
+    """The result's rounding; the weights times the steps rounded to the inputs' type
+    (a weight's rounding error meets a value's distance from its middle) and, for their
+    sum with the middles, float sums; a score's error shifts its weight by as much:
+    (dim + 8) units 2^-23 of its parts' sizes, twice for the ratio of two weights."""
+    shift = 2.0 * (dim + 8) * 2.0 ** -23 * scores[..., None] + 2.0 ** -20
+    return 1.01 * (U[dtype] * out.abs() + U[dtype] * spread + shift * 2.0 * size +
+                   2.0 ** -18 * (spread + size) + 2.0 ** -25)
+
+
+def compare(got, ref, dtype, dim):
+    out = ref[0]
+    error = (got.double() - out).abs()
+    limit = bound(dtype, dim, *ref)
+    # Rows at float16's limit: the step, 131008 / 15 rounded to 8736, holds 65504 as 7.5
+    # steps, 65520, which is where rounding to float16 gives infinity.
+    if dtype == HF:
+        error[(got == out.sign() * float("inf")) & (out.abs() + limit >= 65520.0)] = 0.0
+    assert (error <= limit).all(), f"{(error - limit).max().item():.3g} beyond"
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (2, 1, 64), (8, 2, 64), (6, 2, 40),
+                                                (4, 4, 96), (16, 4, 128), (24, 2, 128),
+                                                (9, 1, 32), (40, 2, 16), (3, 3, 120)])
+def test_streams(heads, kv_heads, dim, dtype):
+    """From empty caches past their wrap, streams at different positions, one idle now
+    and then, dead tokens."""
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(heads * 1000 + dim)
+    for left, first, masked in ((0, 0, False), (6, 0, True), (20, 3, False), (20, 3, True)):
+        batch, slots = 4, first + left + 1
+        cache = window_cache_4bit(batch, left, first, kv_heads, dim, dtype)
+        ref = R.Streams(batch, slots, first, kv_heads, dim, dtype, "cuda")
+        cache_valid = torch.zeros(batch, slots, dtype=torch.bool, device="cuda") if masked else None
+        at = torch.zeros(batch, dtype=torch.int64)
+        for turn in range(2 * slots + 3):
+            busy = torch.tensor([True, turn % 2 == 0, turn % 3 > 0, turn > slots])
+            positions = torch.where(busy, at, -1).cuda()
+            at = at + busy
+            q = rand(g, batch, heads, dim, dtype=dtype)
+            k = rand(g, batch, kv_heads, dim, dtype=dtype)
+            v = rand(g, batch, kv_heads, dim, dtype=dtype, size=3.0) + 1.0
+            valid = torch.rand(batch, generator=g, device="cuda") < 0.6 if masked else None
+            out = window_attention_step_4bit(q, k, v, cache, positions, first=first, valid=valid,
+                                             cache_valid=cache_valid)
+            want = ref.step(q, k, v, positions, dim ** -0.5, valid)
+            compare(out, want, dtype, dim)
+            for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
+                assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
+            if masked:
+                assert torch.equal(cache_valid, ref.seen)
+
+
+def fill(ref, g, dtype, batch, kv_heads, slots, dim, full=True):
+    """Caches as earlier tokens left them."""
+    for i, kept in enumerate((ref.k, ref.v)):
+        code, step, middle = R.held(rand(g, batch, kv_heads, slots, dim, dtype=dtype, size=1 + i))
+        ref.codes[i][:], ref.ranges[i][:] = R.packed(code), torch.stack((step, middle), -1)
+        kept[:] = (code.double() - 7.5) * step.double()[..., None] + middle.double()[..., None]
+    ref.seen[:] = full
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,left,first,dtype", [
+    (1, 8, 2, 64, 1023, 4, BF), (3, 4, 1, 128, 5000, 0, HF), (2, 6, 2, 96, 2047, 16, BF),
+    (1, 16, 1, 128, 20000, 1, HF), (5, 3, 3, 32, 700, 2, BF), (2, 20, 1, 72, 3001, 0, HF),
+    (64, 4, 4, 64, 130, 0, BF)])
+def test_long_caches(batch, heads, kv_heads, dim, left, first, dtype):
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(left)
+    slots = first + left + 1
+    for masked in (False, True):
+        ref = R.Streams(batch, slots, first, kv_heads, dim, dtype, "cuda")
+        positions = torch.randint(slots, 5 * slots, (batch,), generator=g, device="cuda")
+        fill(ref, g, dtype, batch, kv_heads, slots, dim)
+        if masked:  # stream 0 sees its own token at most
+            ref.seen[:] = torch.rand(batch, slots, generator=g, device="cuda") < 0.5
+            ref.seen[0] = False
+        cache = FourBitCache(ref.codes[0].clone(), ref.ranges[0].clone(), ref.codes[1].clone(),
+                             ref.ranges[1].clone())
+        q = rand(g, batch, heads, dim, dtype=dtype)
+        k, v = (rand(g, batch, kv_heads, dim, dtype=dtype) for _ in range(2))
+        cache_valid = ref.seen.clone() if masked else None
+        valid = torch.arange(batch, device="cuda") % 3 != 0 if masked else None
+        out = window_attention_step_4bit(q, k, v, cache, positions, first=first, valid=valid,
+                                         cache_valid=cache_valid)
+        want = ref.step(q, k, v, positions, dim ** -0.5, valid)
+        compare(out, want, dtype, dim)
+        if masked:
+            assert (out[0] == 0).all() and torch.equal(cache_valid, ref.seen)
+        assert torch.equal(cache.k_codes, ref.codes[0]) and torch.equal(cache.v_codes, ref.codes[1])
+        # partly filled: what lies past the token's position is not looked at
+        few = torch.full((batch,), slots // 3, device="cuda")
+        nan = [t.clone() for t in cache]
+        nan[1][:, :, slots // 3 + 1:] = float("nan")
+        nan[3][:, :, slots // 3 + 1:] = float("nan")
+        ref.seen[:, slots // 3 + 1:] = False
+        if masked:  # nor what is left out
+            cache_valid = ref.seen.clone()
+            out_of = ~ref.seen[:, None, :, None].expand_as(nan[1])
+            nan[1][out_of] = nan[3][out_of] = float("nan")
+            out_of = out_of[..., :1].expand_as(nan[0])
+            nan[0][out_of] = nan[2][out_of] = 255
+        else:
+            ref.seen[:, :slots // 3] = True
+        out = window_attention_step_4bit(q, k, v, FourBitCache(*nan), few, first=first,
+                                         valid=valid, cache_valid=cache_valid)
+        compare(out, ref.step(q, k, v, few, dim ** -0.5, valid), dtype, dim)
+
+
+def test_rows_that_are_special():
+    """Rows of one value, of zeros, of subnormals, of the type's limits, and not finite."""
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    for dtype in (BF, HF):
+        top = torch.finfo(dtype).max if dtype == HF else 1e30
+        rows = [torch.zeros(32), torch.full((32,), 3.5), torch.full((32,), -2.0 ** -20),
+                torch.linspace(-1, 1, 32) * 2.0 ** -22, torch.linspace(-1, 1, 32) * top,
+                torch.tensor([0.0] * 31 + [1.0]), torch.arange(32) / 31.0 * 15.0]
+        batch = len(rows)
+        k = torch.stack(rows).to(dtype).cuda()[:, None]
+        v = k.clone()
+        cache = window_cache_4bit(batch, 4, 0, 1, 32, dtype)
+        ref = R.Streams(batch, 5, 0, 1, 32, dtype, "cuda")
+        q = torch.full((batch, 1, 32), 2.0 ** -10, device="cuda", dtype=dtype)
+        positions = torch.zeros(batch, dtype=torch.int64, device="cuda")
+        out = window_attention_step_4bit(q, k, v, cache, positions)
+        want = ref.step(q, k, v, positions, 32 ** -0.5)
+        for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
+            assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
+        compare(out, want, dtype, 32)
+        for bad in (float("nan"), float("inf")):
+            v2 = v.clone()
+            v2[:, :, 5] = bad
+            out = window_attention_step_4bit(q, k, v2, cache, positions + 1)
+            assert not out.isfinite().any()
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 bytes of codes: its last slots are where they belong."""
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    kv_heads, dim, slots = 8, 128, 9_000_001
+    codes = [torch.full((1, kv_heads, slots, dim // 2), 0x88, dtype=torch.uint8, device="cuda")
+             for _ in range(2)]
+    ranges = [torch.zeros(1, kv_heads, slots, 2, dtype=BF, device="cuda") for _ in range(2)]
+    ranges[0][..., 0] = 0.125  # keys (8 - 7.5) / 8
+    codes[0][:, :, -3] = 0xff
+    ranges[0][:, :, -3, 0] = 64.0  # one key that outweighs all others
+    ranges[1][:, :, -3, 1] = torch.arange(1, kv_heads + 1, device="cuda").to(BF)
+    q = torch.ones(1, kv_heads, dim, device="cuda", dtype=BF)
+    token = torch.zeros(1, kv_heads, dim, device="cuda", dtype=BF)
+    out = window_attention_step_4bit(q, token, token, FourBitCache(codes[0], ranges[0], codes[1],
+                                                                   ranges[1]),
+                                     torch.tensor([slots * 3 + 5], device="cuda"))
+    want = torch.arange(1, kv_heads + 1, device="cuda").to(BF)[None, :, None].expand_as(out)
+    assert torch.equal(out, want)
+    assert (codes[0][0, :, 5] == 0x88).all() and (ranges[0][0, :, 5] == 0).all()
+
+
+def test_repeats_streams_and_graph():
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    tokens = [(rand(g, 3, 8, 64, dtype=BF), rand(g, 3, 2, 64, dtype=BF), rand(g, 3, 2, 64, dtype=BF))
+              for _ in range(12)]
+    caches = [window_cache_4bit(3, 6, 1, 2, 64) for _ in range(3)]
+    positions = torch.zeros(3, dtype=torch.int64, device="cuda")
+    plain = [window_attention_step_4bit(*t, caches[0], positions + i, first=1)
+             for i, t in enumerate(tokens)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [window_attention_step_4bit(*t, caches[1], positions + i, first=1)
+                 for i, t in enumerate(tokens)]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    held, at = [t.clone() for t in tokens[0]], positions.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = window_attention_step_4bit(*held, caches[2], at, first=1)
+        at += 1
+    for i, t in enumerate(tokens):
+        for h, x in zip(held, t):
+            h.copy_(x)
+        graph.replay()
+        assert torch.equal(out, plain[i]) and torch.equal(other[i], plain[i])
+    for a, b, c in zip(*caches):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_strided_tokens_and_refusals():
+    from gaussian_splats_b200.attention import (FourBitCache, window_attention_step_4bit,
+                                                window_cache_4bit)
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    both = rand(g, 3, 12 * 64 + 3, dtype=HF)
+    parts = [both[:, 3 + a:3 + b].unflatten(1, (-1, 64)) for a, b in ((0, 512), (512, 640), (640, 768))]
+    positions = torch.tensor([0, 5, 900], device="cuda")
+    caches = [window_cache_4bit(3, 6, 1, 2, 64, HF) for _ in range(2)]
+    a = window_attention_step_4bit(*parts, caches[0], positions, first=1, scale=0.3)
+    b = window_attention_step_4bit(*(t.contiguous() for t in parts), caches[1], positions, first=1,
+                                   scale=0.3)
+    assert torch.equal(a, b)
+    none = window_attention_step_4bit(*(t[:0] for t in parts), window_cache_4bit(0, 6, 1, 2, 64, HF),
+                                      positions[:0], first=1)
+    assert none.shape == (0, 8, 64)
+    c = caches[0]
+    for bad in (dict(cache=FourBitCache(c[0], c[1], c[2], c[3].bfloat16())),
+                dict(cache=FourBitCache(c[0][:, :, :3], c[1], c[2], c[3])),
+                dict(cache=FourBitCache(c[0].transpose(1, 2), c[1], c[2], c[3])),
+                dict(first=8), dict(positions=positions.int()), dict(scale=0.0),
+                dict(valid=torch.ones(3, device="cuda", dtype=torch.bool)),
+                dict(cache_valid=torch.ones(3, 7, device="cuda", dtype=torch.bool))):
+        args = {**dict(cache=c, positions=positions, first=1), **bad}
+        with pytest.raises(ValueError):
+            window_attention_step_4bit(*parts, **args)
+    with pytest.raises(RuntimeError):
+        window_attention_step_4bit(*parts, FourBitCache(c[0].cpu(), *c[1:]), positions)

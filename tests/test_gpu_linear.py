@@ -1,0 +1,276 @@
+"""The linear layer with its epilogue against its definition in 64 bits."""
+
+import pytest
+import torch
+
+import operator_reference as R
+
+pytestmark = pytest.mark.gpu
+
+U = R.U
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+SHAPES = [(1, 1, 1), (1, 8, 8), (2, 64, 128), (3, 59, 11), (5, 7, 9), (16, 2048, 24),
+          (33, 136, 520), (96, 256, 1024), (127, 256, 96), (128, 64, 256), (129, 65, 257),
+          (300, 520, 136), (700, 1030, 264), (1000, 72, 1000), (4097, 24, 40)]
+# type, bias, residual, activation
+FORMS = [(BF, None, None, None), (BF, BF, None, "gelu"), (BF, FL, FL, "silu"),
+         (HF, HF, HF, "relu"), (HF, FL, None, "gelu"), (HF, None, FL, None),
+         (BF, FL, BF, "silu"), (HF, HF, None, "silu")]
+
+
+def make(rows, inputs, outputs, dtype, bias, residual, seed=0, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    out = dtype if residual is None else residual
+    return dict(x=(size * rand(rows, inputs)).to(dtype),
+                weight=(inputs ** -0.5 * rand(outputs, inputs)).to(dtype),
+                bias=None if bias is None else (0.5 * rand(outputs)).to(bias),
+                residual=None if residual is None else (2 * rand(rows, outputs)).to(residual),
+                grad=rand(rows, outputs).to(out))
+
+
+def call(s, activation, train=True):
+    from gaussian_splats_b200.linear import linear
+
+    names = [n for n in ("x", "weight", "bias", "residual") if s[n] is not None]
+    leaves = {n: s[n].detach().requires_grad_(train) for n in names}
+    y = linear(leaves["x"], leaves["weight"], leaves.get("bias"), leaves.get("residual"),
+               activation=activation)
+    got = {"y": y.detach()}
+    if train:
+        grads = torch.autograd.grad(y, [leaves[n] for n in names], s["grad"])
+        got.update({"d" + n: t for n, t in zip(names, grads)})
+    return got
+
+
+def bounds(s, ref, activation):
+    """A float sum of n products, 16 at a time: (n / 16 + 5) units 2^-23 of the sum
+    of their sizes, and one more for a float32 bias or residual. The activations' slopes
+    are below 1.13 and their own errors below 1e-5 of what they return and 1e-7 of z.
+    dz is rounded to the inputs' type (U), its slope to steps of 1 / 49152 before that,
+    and inherits z's error through act'' (below 0.8; relu's slope may jump where z is 0
+    within its error)."""
+    x, w, dtype = s["x"].double().abs(), s["weight"].double().abs(), s["x"].dtype
+    rows, inputs = x.shape
+    outputs = len(w)
+    unit = 2.0 ** -23
+    z_error = (inputs / 16 + 6) * unit * ref["size"]
+    out = {"y": 1.13 * z_error + 1e-5 * ref["act"].abs() + 1e-7 * ref["z"].abs() +
+           unit * ref["y"].abs()}
+    if "dz" not in ref:
+        return out
+    g = s["grad"].double().abs()
+    slope_error = 0.0 if activation is None else \
+        1e-5 * ref["slope"].abs() + 1.02e-5 + 1e-6 + 0.8 * z_error
+    if activation == "relu":
+        slope_error = slope_error + (ref["z"].abs() <= z_error)
+    # subnormal float16 dz: half a step of 2^-24
+    dz_error = U[dtype] * (ref["dz"].abs() + g * slope_error) + g * slope_error + 2.0 ** -25
+    dz = ref["dz"].abs() + dz_error
+    out["dx"] = dz_error @ w + (outputs / 16 + 6) * unit * (dz @ w) + 2.0 ** -25
+    out["dweight"] = dz_error.t() @ x + (rows / 16 + 40) * unit * (dz.t() @ x) + 2.0 ** -25
+    out["dbias"] = dz_error.sum(0) + (rows / 16 + 40) * unit * dz.sum(0) + 2.0 ** -25
+    out["dresidual"] = 0.0
+    return out
+
+
+def check(got, s, activation, train=True):
+    ref = R.linear(s["x"], s["weight"], s["bias"], s["residual"], activation,
+                   s["grad"] if train else None)
+    if train:
+        ref["dresidual"] = s["grad"].double()
+    inner = bounds(s, ref, activation)
+    for name, t in got.items():
+        assert t.shape == ref[name].shape
+        bound = 1.01 * U[t.dtype] * ref[name].abs() + 1.01 * inner[name]
+        error = (t.double() - ref[name]).abs()
+        assert (error <= bound).all(), f"{name}: {(error - bound).max().item():.3g} beyond"
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_against_the_definition(shape, form):
+    dtype, bias, residual, activation = form
+    s = make(*shape, dtype, bias, residual)
+    check(call(s, activation), s, activation)
+    check(call(s, activation, train=False), s, activation, train=False)
+
+
+@pytest.mark.parametrize("rows,inputs,outputs", [(40003, 264, 40), (20000, 512, 512),
+                                                 (3, 4096, 2056), (70000, 8, 256)])
+def test_larger(rows, inputs, outputs):
+    s = make(rows, inputs, outputs, BF, FL, FL)
+    check(call(s, "gelu"), s, "gelu")
+
+
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+def test_far_sums(activation):
+    """Sums of up to +-200, where slopes are 0 or 1 and exponentials leave their range."""
+    s = make(64, 64, 64, HF, FL, None, size=60.0)
+    check(call(s, activation), s, activation)
+
+
+def test_special_values():
+    """A row's infinities and NaN stay in that row of y and dx."""
+    from gaussian_splats_b200.linear import linear
+
+    s = make(300, 64, 72, BF, BF, FL)
+    clean = call(s, "silu")
+    x = s["x"].clone()
+    x[17, 3], x[200, 0] = float("nan"), float("inf")
+    leaf = x.requires_grad_()
+    y = linear(leaf, s["weight"], s["bias"], s["residual"], activation="silu")
+    dx, = torch.autograd.grad(y, leaf, s["grad"])
+    rows = torch.ones(300, dtype=torch.bool, device="cuda")
+    rows[17] = rows[200] = False
+    assert torch.equal(y[rows], clean["y"][rows]) and torch.equal(dx[rows], clean["dx"][rows])
+    assert y[17].isnan().all() and not y[200].isfinite().all()
+    big = linear(torch.full((1, 8), 60000.0, device="cuda", dtype=HF),
+                 torch.tensor([[1.0] * 8, [-1.0] * 8], device="cuda", dtype=HF),
+                 residual=torch.zeros(1, 2, device="cuda"), activation="gelu")
+    assert big.tolist() == [[480000.0, 0.0]]
+
+
+def test_strides_and_offsets():
+    """Slices of a projection, odd offsets and pitches, a transposed weight, three axes."""
+    from gaussian_splats_b200.linear import linear
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda").to(BF)  # noqa: E731
+    wide, weight = rand(200, 300), rand(80, 64)
+    residual = rand(200, 160).float()
+    for x in (wide[:, 8:72], wide[:, 5:69], wide[::2, 8:72], wide[1:, 1:65],
+              rand(64, 200).t(), wide[:1, :64].expand(200, 64)):
+        for w in (weight, rand(64, 80).t(), rand(80, 72)[:, 3:67]):
+            for res in (None, residual[:len(x), 3:83], residual[:len(x), ::2],
+                        residual[:1, :80].expand(len(x), 80)):
+                y = linear(x, w, None, res, activation="gelu")
+                whole = linear(x.contiguous(), w.contiguous(), None,
+                               None if res is None else res.contiguous(), activation="gelu")
+                assert torch.equal(y, whole)
+    x = rand(4, 50, 64).requires_grad_()
+    w = weight.clone().requires_grad_()
+    y = linear(x, w, activation="silu")
+    flat = linear(x.reshape(200, 64), w, activation="silu")
+    assert y.shape == (4, 50, 80) and torch.equal(y.reshape(200, 80), flat)
+    up = rand(4, 80, 50).transpose(1, 2)
+    got = torch.autograd.grad(y, (x, w), up)
+    whole = torch.autograd.grad(flat, (x, w), up.reshape(200, 80))
+    assert got[0].shape == x.shape and all(torch.equal(a, b) for a, b in zip(got, whole))
+    one = linear(x[0, 0], w)
+    assert one.shape == (80,) and torch.equal(one, linear(x[0, :1], w)[0])
+
+
+@pytest.mark.parametrize("wanted", range(1, 16))
+def test_gradients_asked_for(wanted):
+    from gaussian_splats_b200.linear import linear
+
+    s = make(130, 72, 40, BF, FL, FL)
+    whole = call(s, "gelu")
+    names = ("x", "weight", "bias", "residual")
+    leaves = {n: s[n].detach().requires_grad_(bool(wanted >> i & 1)) for i, n in enumerate(names)}
+    y = linear(*leaves.values(), activation="gelu")
+    some = [n for n in names if leaves[n].requires_grad]
+    for n, t in zip(some, torch.autograd.grad(y, [leaves[n] for n in some], s["grad"])):
+        assert torch.equal(t, whole["d" + n]), n
+
+
+def test_no_rows():
+    s = make(0, 24, 16, BF, FL, FL)
+    got = call(s, "gelu")
+    assert got["y"].shape == (0, 16) and got["dx"].shape == (0, 24)
+    assert got["dweight"].abs().max() == 0 and got["dbias"].abs().max() == 0
+
+
+def test_repeats_and_leaves_the_rest_alone():
+    """Bit for bit the same; rows behind the last one stay as they were."""
+    import ctypes
+
+    from gaussian_splats_b200 import native
+    from gaussian_splats_b200.sequences import call as library
+
+    s = make(5000, 136, 264, BF, BF, FL)
+    a, b = call(s, "gelu"), call(s, "gelu")
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    y = torch.full((5100, 264), 7.0, device="cuda")
+    slope = torch.full((5100, 264), 7, device="cuda", dtype=torch.int16)
+    args = native.LinearArgs(
+        rows=5000, inputs=136, outputs=264, dtype=1, bias_dtype=1, residual_dtype=0, activation=2,
+        x=s["x"].data_ptr(), weight=s["weight"].data_ptr(), bias=s["bias"].data_ptr(),
+        residual=s["residual"].data_ptr(), x_stride=136, weight_stride=136, residual_stride=264,
+        y=y.data_ptr(), slope=slope.data_ptr())
+    library("gs_linear", y.device, ctypes.byref(args))
+    assert torch.equal(y[:5000], a["y"]) and (y[5000:] == 7.0).all()
+    assert (slope[5000:] == 7).all() and (slope[:5000] != 7).float().mean() > 0.99
+
+
+def test_other_stream_and_graph():
+    """On another stream, and captured: a replay with new inputs is a call with them."""
+    from gaussian_splats_b200.linear import linear
+
+    sets = [make(300, 72, 264, HF, FL, FL, seed=i) for i in range(3)]
+    want = [call(s, "silu") for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call(sets[1], "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(got[n], want[1][n]) for n in got)
+    names = ("x", "weight", "bias", "residual")
+    held = {n: sets[0][n].clone().requires_grad_() for n in names}
+    up = sets[0]["grad"].clone()
+
+    def run():
+        y = linear(*held.values(), activation="silu")
+        return (y, *torch.autograd.grad(y, list(held.values()), up))
+
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for s, w in zip(sets[1:], want[1:]):
+        with torch.no_grad():
+            for n in names:
+                held[n].copy_(s[n])
+            up.copy_(s["grad"])
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, t in zip(("y", "dx", "dweight", "dbias", "dresidual"), out):
+            assert torch.equal(t.detach(), w[n]), n
+
+
+def test_saved_tensors_may_move():
+    """Hooks that take the saved tensors to the host and bring them back otherwise laid out."""
+    from gaussian_splats_b200.linear import linear
+
+    s = make(100, 72, 40, BF, FL, None)
+    want = call(s, "gelu")
+
+    def unpack(t):
+        t = t.cuda()
+        return t.t().contiguous().t() if t.dim() == 2 else t
+
+    leaves = [s[n].detach().requires_grad_() for n in ("x", "weight", "bias")]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+        y = linear(*leaves, activation="gelu")
+    for n, t in zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, leaves, s["grad"])):
+        assert torch.equal(t, want[n]), n
+
+
+def test_refusals():
+    from gaussian_splats_b200.linear import linear
+
+    x, w = torch.zeros(4, 16, device="cuda", dtype=BF), torch.zeros(8, 16, device="cuda", dtype=BF)
+    for bad in (lambda: linear(x, w.half()), lambda: linear(x.float(), w.float()),
+                lambda: linear(x, w[:, :8]), lambda: linear(x, w[0]),
+                lambda: linear(x, w, x[0]), lambda: linear(x, w, w[:, 0].half()),
+                lambda: linear(x, w, residual=x), lambda: linear(x, w, activation="tanh"),
+                lambda: linear(x, w, residual=torch.zeros(4, 8, device="cuda", dtype=HF)),
+                lambda: linear(x, w[:0]), lambda: linear(x[:, :0], w[:, :0])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        linear(x, w.cpu())
