@@ -21,9 +21,10 @@ using namespace tc;
 // to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact. (A
 // float32 bias's gradient is a sum of unrounded dz: there slopes are kept as floats.)
 constexpr float kSlopeScale = 49152.0f, kSlopeZero = 8192.0f, kTwo23 = 8388608.0f;
-__device__ __forceinline__ uint32_t slope_code(float slope) {
-  // The sum's low bits are the nearest whole number.
-  return __float_as_uint(fmaf(slope, kSlopeScale, kTwo23 + kSlopeZero)) & 0xffffu;
+__device__ __forceinline__ uint32_t slope_codes(float low, float high) {
+  // The sums' low bits are the nearest whole numbers.
+  return __byte_perm(__float_as_uint(fmaf(low, kSlopeScale, kTwo23 + kSlopeZero)),
+                     __float_as_uint(fmaf(high, kSlopeScale, kTwo23 + kSlopeZero)), 0x5410);
 }
 __device__ __forceinline__ float slope_value(uint32_t code) {
   return (__uint_as_float(0x4b000000u | code) - (kTwo23 + kSlopeZero)) * (1.0f / kSlopeScale);
@@ -98,6 +99,7 @@ constexpr int kRows = 128;   // of a tile
 constexpr int kDepth = 64;   // of a stage: 128 bytes of channels, or 64 rows
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kChunkBytes = 4096;  // 32 rows of 32 floats, or of 32 16-bit elements in half of it
 
 // What becomes of the sums D(m, n).
 struct Epilogue {
@@ -113,6 +115,13 @@ struct Epilogue {
   void* slope;
   int64_t slope_stride;
   bool slope_float;
+  // Whether `out` and the residual lie as TMA takes them (rows of whole 16-byte words).
+  bool tiled;
+};
+
+// The maps of what the epilogue reads and writes, in boxes of 32 rows of 32 columns.
+struct EpilogueMaps {
+  CUtensorMap out, residual, slope;
 };
 
 // Items are (split, row tile, column tile), the last one fastest.
@@ -129,16 +138,222 @@ struct ProductShared {
   static constexpr int kABytes = kRows * kDepth * 2, kBBytes = kN * kDepth * 2;
   alignas(1024) unsigned char a[kStages][kABytes];
   alignas(1024) unsigned char b[kStages][kBBytes];
-  alignas(1024) float out[kEpilogueWarps][32 * 32];
-  uint64_t full[kStages], empty[kStages], ready[2], drained[2];
+  alignas(1024) unsigned char out[kEpilogueWarps][2][kChunkBytes];
+  uint64_t full[kStages], empty[kStages], ready[2], drained[2], residual[kEpilogueWarps][2];
   uint32_t tensor;
 };
+
+// 32 columns of a row's chunk to shared memory and back, as TMA's swizzle has them:
+// rows of 128 bytes (floats) or 64 (16 bits), whose 16-byte words are exchanged so that
+// eight rows' same words lie in different banks.
+__device__ __forceinline__ uint32_t word_of(uint32_t chunk, int row, int word, bool wide) {
+  return wide ? chunk + row * 128 + ((word ^ (row & 7)) << 4)
+              : chunk + row * 64 + ((word ^ (row >> 1 & 3)) << 4);
+}
+__device__ __forceinline__ void put_word(uint32_t at, uint32_t a, uint32_t b, uint32_t c,
+                                         uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ uint4 get_word(uint32_t at) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+               : "r"(at)
+               : "memory");
+  return w;
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int row, uint32_t src) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(row), "r"(src)
+      : "memory");
+}
+__device__ __forceinline__ void commit_stores() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until all stores but the last kPending have read their shared memory.
+template <int kPending>
+__device__ __forceinline__ void wait_stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
+}
+__device__ __forceinline__ void wait_stores_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// The epilogue's warps: a row a thread, 32 columns at a time. Chunks pass through shared
+// memory, from which TMA writes them; the residual's come by TMA to the place of the
+// results, a chunk ahead. Where rows are no whole 16-byte words, a warp writes 32
+// columns of one row at a time instead.
+template <class T, int kN>
+__device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps& maps,
+                         ProductShared<kN>& s, uint32_t tensor, int warp, int lane) {
+  const int64_t tiles = int64_t{plan.row_tiles} * plan.column_tiles, items = tiles * plan.splits;
+  const bool wide = e.out_dtype == GS_FLOAT32;
+  const int slope_bytes = !e.slope ? 0 : e.slope_float ? kChunkBytes : kChunkBytes / 2;
+  const int chunk_bytes = (wide ? kChunkBytes : kChunkBytes / 2) + slope_bytes;
+  const bool two = 2 * chunk_bytes <= 2 * kChunkBytes;  // chunks in two places in turn
+  const uint32_t staged = shared_address(s.out[warp]);
+  struct Place {
+    int64_t item;
+    int c;  // chunk of the tile
+  };
+  const auto column_of = [&](const Place& p) {
+    return static_cast<int>(p.item % tiles % plan.column_tiles) * kN + 32 * p.c;
+  };
+  const auto row_of = [&](const Place& p) {
+    return static_cast<int>(p.item % tiles / plan.column_tiles) * kRows + 32 * (warp & 3);
+  };
+  // This place, or the warp's next one that has columns.
+  const auto from = [&](Place p) {
+    while (p.item < items && (p.c >= kN / 32 || column_of(p) >= e.columns))
+      p = {p.item + gridDim.x, warp >> 2};
+    return p;
+  };
+  const auto load_residual = [&](const Place& p, uint32_t use) {
+    if (p.item >= items) return;
+    const uint32_t at = two ? use & 1 : 0;
+    const uint32_t bar = shared_address(&s.residual[warp][at]);
+    barrier_expect(bar, wide ? kChunkBytes : kChunkBytes / 2);
+    load_box(staged + at * chunk_bytes, &maps.residual, column_of(p), row_of(p), bar);
+  };
+  const bool by_tma = e.tiled, add = e.residual != nullptr;
+  bool good = true;
+  uint32_t use = 0;  // chunks done
+  Place p = {blockIdx.x, warp >> 2};
+  if (by_tma && add && lane == 0) load_residual(from(p), 0);
+  uint32_t count = 0;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
+    const uint32_t buffer = count & 1;
+    p = {item, warp >> 2};
+    const int row = row_of(p);
+    const int64_t out_row = item / tiles * plan.split_rows + row;
+    good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
+    fence_after_sync();
+    for (; p.c < kN / 32; p.c += 2) {
+      const int n = column_of(p);
+      if (n >= e.columns) break;
+      float z[32], slope[32];
+      float bias = 0.0f;
+      if (e.bias && n + lane < e.columns) bias = read_as(e.bias, e.bias_dtype, n + lane);
+      load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * p.c,
+                     z);
+      wait_loads();
+      if (!good)
+        for (float& x : z) x = NAN;
+      if (e.bias)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] += __shfl_sync(0xffffffffu, bias, i);
+      activate(e.activation, z, slope);
+      if (by_tma) {
+        const uint32_t at = two ? use & 1 : 0, chunk = staged + at * chunk_bytes;
+        if (lane == 0) {
+          if (two && !add) wait_stores_read<1>();
+          else wait_stores_read<0>();
+          if (add && two) load_residual(from({p.item, p.c + 2}), use + 1);
+        }
+        if (add) {
+          good = good && barrier_wait_warp(shared_address(&s.residual[warp][at]),
+                                           (two ? use >> 1 : use) & 1);
+        }
+        __syncwarp();
+        if (wide) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const uint32_t word = word_of(chunk, lane, w, true);
+            if (add) {
+              const uint4 r = get_word(word);
+              z[4 * w] += __uint_as_float(r.x);
+              z[4 * w + 1] += __uint_as_float(r.y);
+              z[4 * w + 2] += __uint_as_float(r.z);
+              z[4 * w + 3] += __uint_as_float(r.w);
+            }
+            put_word(word, __float_as_uint(z[4 * w]), __float_as_uint(z[4 * w + 1]),
+                     __float_as_uint(z[4 * w + 2]), __float_as_uint(z[4 * w + 3]));
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t word = word_of(chunk, lane, w, false);
+            if (add) {
+              const uint4 r = get_word(word);
+              const T* v = reinterpret_cast<const T*>(&r);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) z[8 * w + k] += to_float(v[k]);
+            }
+            put_word(word, pack2<T>(z[8 * w], z[8 * w + 1]), pack2<T>(z[8 * w + 2], z[8 * w + 3]),
+                     pack2<T>(z[8 * w + 4], z[8 * w + 5]), pack2<T>(z[8 * w + 6], z[8 * w + 7]));
+          }
+        }
+        const uint32_t slope_chunk = chunk + (wide ? kChunkBytes : kChunkBytes / 2);
+        if (e.slope && e.slope_float) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+            put_word(word_of(slope_chunk, lane, w, true), __float_as_uint(slope[4 * w]),
+                     __float_as_uint(slope[4 * w + 1]), __float_as_uint(slope[4 * w + 2]),
+                     __float_as_uint(slope[4 * w + 3]));
+        } else if (e.slope) {
+          uint32_t code[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) code[i] = slope_codes(slope[2 * i], slope[2 * i + 1]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            put_word(word_of(slope_chunk, lane, w, false), code[4 * w], code[4 * w + 1],
+                     code[4 * w + 2], code[4 * w + 3]);
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          if (row < e.rows) {
+            store_box(&maps.out, n, static_cast<int>(out_row), chunk);
+            if (e.slope) store_box(&maps.slope, n, row, slope_chunk);
+          }
+          commit_stores();
+          if (add && !two) {
+            wait_stores_read<0>();
+            load_residual(from({p.item, p.c + 2}), use + 1);
+          }
+        }
+        ++use;
+      } else {
+        float* const square = reinterpret_cast<float*>(s.out[warp]);
+        const auto store = [&](const float(&x)[32], auto&& put) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) square[32 * lane + (i ^ lane)] = x[i];
+          __syncwarp();
+          if (n + lane < e.columns)
+            for (int r = 0; r < 32 && row + r < e.rows; ++r) put(r, square[32 * r + (lane ^ r)]);
+        };
+        store(z, [&](int r, float y) {
+          if (add) y += read_as(e.residual, e.out_dtype, (row + r) * e.residual_stride + n + lane);
+          write_as(e.out, e.out_dtype, (out_row + r) * e.out_stride + n + lane, y);
+        });
+        if (e.slope)
+          store(slope, [&](int r, float x) {
+            const int64_t to = (row + r) * e.slope_stride + n + lane;
+            if (e.slope_float) static_cast<float*>(e.slope)[to] = x;
+            else static_cast<uint16_t*>(e.slope)[to] = static_cast<uint16_t>(slope_codes(x, x));
+          });
+      }
+    }
+    fence_before_sync();
+    __syncwarp();
+    if (lane == 0) barrier_arrive(shared_address(&s.drained[buffer]));
+  }
+  if (lane == 0) wait_stores_done();
+  if (!good)
+    for (uint64_t& bar : s.residual[warp]) barrier_settle(shared_address(&bar));
+  return good;
+}
 
 // kRowsA, kRowsB: the operand's contraction runs along its rows.
 template <class T, int kN, bool kRowsA, bool kRowsB>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(Plan plan, Epilogue e, const __grid_constant__ CUtensorMap a_map,
-                   const __grid_constant__ CUtensorMap b_map) {
+                   const __grid_constant__ CUtensorMap b_map,
+                   const __grid_constant__ EpilogueMaps maps) {
   using Shared = ProductShared<kN>;
   constexpr int kStages = Shared::kStages;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
@@ -153,6 +368,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     for (int i = 0; i < 2; ++i) {
       barrier_init(shared_address(&s.ready[i]), 1);
       barrier_init(shared_address(&s.drained[i]), kEpilogueWarps);
+      for (int w = 0; w < kEpilogueWarps; ++w) barrier_init(shared_address(&s.residual[w][i]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
@@ -229,57 +445,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       if (good) commit(elected, shared_address(&s.ready[buffer]));
     }
-  } else {  // epilogue: a row a thread, 32 columns at a time
-    float* const staged = s.out[warp];
-    uint32_t count = 0;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
-      const int tile = static_cast<int>(item % tiles);
-      const int64_t split = item / tiles;
-      const int64_t m0 = int64_t{tile / plan.column_tiles} * kRows + 32 * (warp & 3);
-      const int n0 = tile % plan.column_tiles * kN;
-      const uint32_t buffer = count & 1;
-      good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
-      fence_after_sync();
-      for (int c = warp >> 2; c < kN / 32; c += 2) {
-        float z[32], slope[32];
-        load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * c,
-                       z);
-        wait_loads();
-        if (!good)
-          for (float& x : z) x = NAN;
-        const int n = n0 + 32 * c;
-        if (n >= e.columns) continue;
-        if (e.bias)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            z[i] += n + i < e.columns ? read_as(e.bias, e.bias_dtype, n + i) : 0.0f;
-        activate(e.activation, z, slope);
-        // Through shared memory, so that a warp writes 32 columns of one row at a time.
-        const auto store = [&](const float(&x)[32], auto&& put) {
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) staged[32 * lane + (i ^ lane)] = x[i];
-          __syncwarp();
-          if (n + lane < e.columns)
-            for (int r = 0; r < 32 && m0 + r < e.rows; ++r)
-              put(m0 + r, n + lane, staged[32 * r + (lane ^ r)]);
-        };
-        store(z, [&](int64_t m, int64_t column, float y) {
-          if (e.residual) y += read_as(e.residual, e.out_dtype, m * e.residual_stride + column);
-          write_as(e.out, e.out_dtype, (split * plan.split_rows + m) * e.out_stride + column, y);
-        });
-        if (e.slope)
-          store(slope, [&](int64_t m, int64_t column, float x) {
-            if (e.slope_float) static_cast<float*>(e.slope)[m * e.slope_stride + column] = x;
-            else
-              static_cast<uint16_t*>(e.slope)[m * e.slope_stride + column] =
-                  static_cast<uint16_t>(slope_code(x));
-          });
-      }
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) barrier_arrive(shared_address(&s.drained[buffer]));
-    }
+  } else {
+    good = epilogue<T, kN>(plan, e, maps, s, tensor, warp, lane);
   }
   if (!good) {  // let what is in flight land
     for (uint64_t& bar : s.full) barrier_settle(shared_address(&bar));
@@ -307,18 +474,43 @@ int32_t encode_operand(CUtensorMap* map, int32_t dtype, const Operand& o, int bo
   return encode(map, dtype, o.data, 2, size, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// A [rows, columns] array in the epilogue's chunks.
+int32_t encode_chunks(CUtensorMap* map, int32_t dtype, const void* data, int64_t rows,
+                      int64_t columns, int64_t row_stride) {
+  const cuuint64_t size[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t stride[1] = {static_cast<cuuint64_t>(row_stride) * element_size(dtype)};
+  const cuuint32_t box[2] = {32, 32};
+  return encode(map, dtype, data, 2, size, stride, box,
+                dtype == GS_FLOAT32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+bool tma_rows(const void* data, int64_t stride, int32_t dtype, int64_t columns) {
+  return is_aligned(data, 16) && stride * element_size(dtype) % 16 == 0 && stride >= columns;
+}
+
 template <class T, int kN, bool kRowsA, bool kRowsB>
 int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan,
                        const Epilogue& e, cudaStream_t stream) {
   CUtensorMap a_map, b_map;
   GS_TRY(encode_operand(&a_map, dtype, a, kRowsA ? kDepth : kRows));
   GS_TRY(encode_operand(&b_map, dtype, b, kRowsB ? kDepth : kN));
+  EpilogueMaps maps;
+  if (e.tiled) {
+    const int64_t out_rows = plan.splits > 1 ? plan.splits * plan.split_rows : e.rows;
+    GS_TRY(encode_chunks(&maps.out, e.out_dtype, e.out, out_rows, e.columns, e.out_stride));
+    if (e.residual)
+      GS_TRY(encode_chunks(&maps.residual, e.out_dtype, e.residual, e.rows, e.columns,
+                           e.residual_stride));
+    if (e.slope)  // bfloat16 stands for any 16 bits
+      GS_TRY(encode_chunks(&maps.slope, e.slope_float ? GS_FLOAT32 : GS_BFLOAT16, e.slope, e.rows,
+                           e.columns, e.slope_stride));
+  }
   constexpr size_t kShared = sizeof(ProductShared<kN>);
   GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB>>(kShared)));
   const int64_t items = int64_t{plan.row_tiles} * plan.column_tiles * plan.splits;
   launch_chained_shared(product_kernel<T, kN, kRowsA, kRowsB>,
                         dim3(static_cast<unsigned>(items < kSmCount ? items : kSmCount)),
-                        dim3(kProductThreads), kShared, stream, plan, e, a_map, b_map);
+                        dim3(kProductThreads), kShared, stream, plan, e, a_map, b_map, maps);
   return check_launch();
 }
 
@@ -363,40 +555,131 @@ int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Pla
 // ------------------------------------------------- the gradient of the sums
 
 constexpr int kSlopeThreads = 256;
-constexpr int kSlopeRows = 512;  // of a strip
+constexpr int kSlopeBlocks = 6 * kSmCount;
 
-// dz = grad_y act'(z) rounded to the operands' type, and each strip's sums of its columns
-// (of what was not rounded).
-template <class T, class G>
-__global__ void __launch_bounds__(kSlopeThreads)
-    slope_kernel(gs_linear_args a, int64_t stride, bool slope_float, T* dz, float* sums) {
-  chain_wait();
-  const int64_t column = blockIdx.y * int64_t{kSlopeThreads} + threadIdx.x;
-  const int64_t row0 = blockIdx.x * int64_t{kSlopeRows};
-  if (column >= a.outputs) return;
-  float sum = 0.0f;
-  for (int64_t m = row0; m < row0 + kSlopeRows && m < a.rows; ++m) {
-    float g = to_float(static_cast<const G*>(a.grad_y)[m * a.outputs + column]);
-    if (a.slope)
-      g *= slope_float ? static_cast<const float*>(a.slope)[m * stride + column]
-                       : slope_value(static_cast<const uint16_t*>(a.slope)[m * stride + column]);
-    sum += g;
-    if (dz) dz[m * stride + column] = from_float<T>(g);
+// How the work is cut: blocks of `lanes` words of eight columns, by strips of rows.
+struct Strips {
+  int32_t lanes, column_blocks;
+  int64_t rows, count;  // of a strip; strips
+};
+
+// N floats of a row at `p`, of which `valid` exist.
+template <class G>
+__device__ __forceinline__ void load_row(const G* p, int valid, bool aligned, float (&x)[8]) {
+  if (aligned && valid >= 8) {
+    if constexpr (sizeof(G) == 4) {
+      float lo[4], hi[4];
+      load_pack<4>(p, lo);
+      load_pack<4>(p + 4, hi);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = lo[k], x[4 + k] = hi[k];
+    } else {
+      load_pack<8>(p, x);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = k < valid ? to_float(p[k]) : 0.0f;
   }
-  if (sums) sums[blockIdx.x * int64_t{a.outputs} + column] = sum;
 }
 
-// The sums of the splits, or of the strips, in order, rounded to the result's type.
-__global__ void __launch_bounds__(256)
-    join_kernel(const float* parts, int count, int64_t part_size, int64_t rows, int columns,
-                int64_t stride, void* out, int dtype) {
+// dz = grad_y act'(z) rounded to the operands' type, and each strip's sums of its columns
+// (of what was not rounded). A thread has eight columns of every so many rows.
+template <class T, class G>
+__global__ void __launch_bounds__(kSlopeThreads)
+    slope_kernel(gs_linear_args a, Strips cut, int64_t stride, bool slope_float, bool aligned,
+                 T* dz, float* sums) {
   chain_wait();
-  const int64_t at = blockIdx.x * int64_t{256} + threadIdx.x;
-  if (at >= rows * columns) return;
-  const int64_t from = at / columns * stride + at % columns;
+  __shared__ float joined[kSlopeThreads][8 + 1];
+  const int lane = threadIdx.x % cut.lanes, first = threadIdx.x / cut.lanes;
+  const int step = kSlopeThreads / cut.lanes;
+  const int64_t column = (blockIdx.y * int64_t{cut.lanes} + lane) * 8;
+  const int valid = static_cast<int>(min(int64_t{8}, a.outputs - column));
+  const int64_t row0 = blockIdx.x * cut.rows, end = min(row0 + cut.rows, a.rows);
+  float sum[8] = {};
+  if (valid > 0) {
+    const G* const grad = static_cast<const G*>(a.grad_y);
+#pragma unroll 4
+    for (int64_t m = row0 + first; m < end; m += step) {
+      float g[8];
+      load_row(grad + m * a.outputs + column, valid, aligned, g);
+      if (a.slope && slope_float) {
+        const float* p = static_cast<const float*>(a.slope) + m * stride + column;
+        float x[8];
+        load_row(p, 8, true, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[k] = k < valid ? g[k] * x[k] : 0.0f;
+      } else if (a.slope) {
+        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.slope) +
+                                                        m * stride + column);
+        const uint32_t codes[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float x = slope_value(k & 1 ? codes[k >> 1] >> 16 : codes[k >> 1] & 0xffffu);
+          g[k] = k < valid ? g[k] * x : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += g[k];
+      if (dz) store_pack<8>(dz + m * stride + column, g);
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) joined[threadIdx.x][k] = sum[k];
+  __syncthreads();
+  for (int i = threadIdx.x; i < cut.lanes * 8; i += kSlopeThreads) {
+    const int64_t c = blockIdx.y * int64_t{cut.lanes} * 8 + i;
+    if (c >= a.outputs) break;
+    float total = 0.0f;
+    for (int r = 0; r < step; ++r) total += joined[r * cut.lanes + i / 8][i % 8];
+    sums[blockIdx.x * int64_t{a.outputs} + c] = total;
+  }
+}
+
+// The strips' sums of a column, in one order: 8 groups of strips, then the groups.
+__global__ void __launch_bounds__(256)
+    bias_kernel(const float* sums, int64_t strips, int columns, void* out, int dtype) {
+  chain_wait();
+  __shared__ float groups[8][33];
+  const int column = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
   float sum = 0.0f;
-  for (int i = 0; i < count; ++i) sum += parts[i * part_size + from];
-  write_as(out, dtype, at, sum);
+  if (column < columns)
+#pragma unroll 8
+    for (int64_t i = group; i < strips; i += 8) sum += sums[i * columns + column];
+  groups[group][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (group == 0 && column < columns) {
+    for (int g = 1; g < 8; ++g) sum += groups[g][threadIdx.x & 31];
+    write_as(out, dtype, column, sum);
+  }
+}
+
+// The splits' sums, in order, rounded to the result's type: four columns a thread.
+constexpr int kJoinThreads = 128;
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads)
+    join_kernel(const float* parts, int count, int64_t part_size, int rows, int columns, T* out) {
+  chain_wait();
+  const int64_t at = blockIdx.x * int64_t{kJoinThreads} + threadIdx.x;
+  const int words = (columns + 3) / 4;
+  if (at >= int64_t{rows} * words) return;
+  float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) {
+    const float4 x = reinterpret_cast<const float4*>(parts + i * part_size)[at];
+    sum.x += x.x;
+    sum.y += x.y;
+    sum.z += x.z;
+    sum.w += x.w;
+  }
+  const int column = static_cast<int>(at % words) * 4;
+  T* const to = out + at / words * columns + column;
+  const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+  if (columns % 4 == 0) {
+    store_pack<4>(to, x);
+  } else {
+    for (int k = 0; k < 4 && column + k < columns; ++k) to[k] = from_float<T>(x[k]);
+  }
 }
 
 // --------------------------------------------------------------------- host
@@ -427,17 +710,29 @@ int64_t slope_stride(const gs_linear_args& a) { return round_up(a.outputs, 8); }
 // sums of dz, the splits' sums of dz^T x.
 struct BackwardPlan {
   bool own_dz;
-  int64_t strips;
+  Strips strips;
   int columns, x_columns;
   Plan weight, x;
   uint64_t dz, sums, parts, size;  // byte offsets, and the whole
 };
 
+Strips strips_of(int64_t rows, int64_t columns) {
+  Strips s = {};
+  s.lanes = 1;
+  while (s.lanes < 32 && s.lanes * 8 < columns) s.lanes *= 2;
+  s.column_blocks = static_cast<int32_t>(ceil_div(columns, s.lanes * 8));
+  const int64_t step = kSlopeThreads / s.lanes;
+  const int64_t strips = ceil_div(kSlopeBlocks, s.column_blocks);
+  s.rows = round_up(ceil_div(rows, strips), 4 * step);  // four rows a thread at least
+  s.count = ceil_div(rows, s.rows);
+  return s;
+}
+
 BackwardPlan backward_plan(const gs_linear_args& a) {
   BackwardPlan p = {};
   if (a.rows == 0) return p;
   p.own_dz = a.activation != GS_IDENTITY || a.residual_dtype != a.dtype || a.outputs % 8 != 0;
-  p.strips = ceil_div(a.rows, kSlopeRows);
+  p.strips = strips_of(a.rows, a.outputs);
   // The weight's gradient has few tiles and a long contraction: split so that the items
   // are about one a multiprocessor.
   p.columns = columns_of(a.outputs, a.inputs, 1 << 20, 64);
@@ -454,7 +749,7 @@ BackwardPlan backward_plan(const gs_linear_args& a) {
     return from;
   };
   p.dz = take(p.own_dz ? static_cast<uint64_t>(a.rows) * slope_stride(a) * 2 : 0);
-  p.sums = take(static_cast<uint64_t>(p.strips) * a.outputs * 4);
+  p.sums = take(static_cast<uint64_t>(p.strips.count) * a.outputs * 4);
   p.parts = take(static_cast<uint64_t>(p.weight.splits) * p.weight.split_rows *
                  round_up(a.inputs, 4) * 4);
   p.size = at;
@@ -487,6 +782,9 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   e.slope = a.activation == GS_IDENTITY ? nullptr : a.slope;
   e.slope_stride = slope_stride(a);
   e.slope_float = a.bias && a.bias_dtype == GS_FLOAT32;
+  e.tiled = tma_rows(a.y, a.outputs, a.residual_dtype, a.outputs) &&
+            (!a.residual ||
+             tma_rows(a.residual, a.residual_stride, a.residual_dtype, a.outputs));
   const int n = columns_of(a.rows, a.outputs, 1, 32);
   return with_sixteen_bit(a.dtype, [&](auto t) {
     return run_product<decltype(t), false, false>(
@@ -521,23 +819,23 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
   return with_sixteen_bit(a.dtype, [&](auto t) {
     using T = decltype(t);
     if ((p.own_dz && products) || sums) {
-      const dim3 grid(static_cast<unsigned>(p.strips), ceil_div(a.outputs, kSlopeThreads));
-      const bool slope_float = a.bias && a.bias_dtype == GS_FLOAT32;
+      const dim3 grid(static_cast<unsigned>(p.strips.count), p.strips.column_blocks);
+      const bool slope_float = a.bias_dtype == GS_FLOAT32 && a.bias;
+      const bool aligned = a.outputs % 8 == 0;
       gs_linear_args b = a;
       if (a.activation == GS_IDENTITY) b.slope = nullptr;
       T* const to = p.own_dz && products ? static_cast<T*>(dz) : nullptr;
       if (a.residual_dtype == GS_FLOAT32)
-        launch_chained(slope_kernel<T, float>, grid, kSlopeThreads, stream, b, slope_stride(a),
-                       slope_float, to, sums);
+        launch_chained(slope_kernel<T, float>, grid, kSlopeThreads, stream, b, p.strips,
+                       slope_stride(a), slope_float, aligned, to, sums);
       else
-        launch_chained(slope_kernel<T, T>, grid, kSlopeThreads, stream, b, slope_stride(a),
-                       slope_float, to, sums);
+        launch_chained(slope_kernel<T, T>, grid, kSlopeThreads, stream, b, p.strips,
+                       slope_stride(a), slope_float, aligned, to, sums);
       GS_TRY(check_launch());
     }
     if (a.grad_bias) {
-      launch_chained(join_kernel, ceil_div(a.outputs, 256), 256, stream,
-                     static_cast<const float*>(sums), static_cast<int>(p.strips),
-                     int64_t{a.outputs}, int64_t{1}, a.outputs, int64_t{a.outputs}, a.grad_bias,
+      launch_chained(bias_kernel, ceil_div(a.outputs, 32), 256, stream,
+                     static_cast<const float*>(sums), p.strips.count, a.outputs, a.grad_bias,
                      a.bias_dtype);
       GS_TRY(check_launch());
     }
@@ -548,25 +846,31 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
       e.out = a.grad_x;
       e.out_stride = a.inputs;
       e.out_dtype = a.dtype;
+      e.tiled = tma_rows(a.grad_x, a.inputs, a.dtype, a.inputs);
       GS_TRY((run_product<T, false, true>(a.dtype, dz_operand,
                                           {a.weight, a.outputs, a.inputs, a.weight_stride}, p.x,
                                           p.x_columns, e, stream)));
     }
     if (a.grad_weight) {
       Epilogue e = {};
+      const bool whole = p.weight.splits == 1;  // no sums to join
       e.rows = a.outputs;
       e.columns = a.inputs;
-      e.out = parts;
-      e.out_stride = round_up(a.inputs, 4);
-      e.out_dtype = GS_FLOAT32;
+      e.out = whole ? a.grad_weight : parts;
+      e.out_stride = whole ? a.inputs : round_up(a.inputs, 4);
+      e.out_dtype = whole ? a.dtype : GS_FLOAT32;
+      e.tiled = tma_rows(e.out, e.out_stride, e.out_dtype, a.inputs);
       GS_TRY((run_product<T, true, true>(a.dtype, dz_operand,
                                          {a.x, a.rows, a.inputs, a.x_stride}, p.weight, p.columns,
                                          e, stream)));
-      launch_chained(join_kernel, ceil_div(int64_t{a.outputs} * a.inputs, 256), 256, stream,
-                     static_cast<const float*>(parts), p.weight.splits,
-                     p.weight.split_rows * round_up(a.inputs, 4), int64_t{a.outputs}, a.inputs,
-                     round_up(a.inputs, 4), a.grad_weight, a.dtype);
-      GS_TRY(check_launch());
+      if (!whole) {
+        const int64_t vectors = int64_t{a.outputs} * ceil_div(a.inputs, 4);
+        launch_chained(join_kernel<T>, ceil_div(vectors, kJoinThreads), kJoinThreads, stream,
+                       static_cast<const float*>(parts), p.weight.splits,
+                       p.weight.split_rows * round_up(a.inputs, 4), a.outputs, a.inputs,
+                       static_cast<T*>(a.grad_weight));
+        GS_TRY(check_launch());
+      }
     }
     return static_cast<int32_t>(GS_OK);
   });

@@ -97,7 +97,8 @@ def test_against_the_definition(shape, form):
 
 
 @pytest.mark.parametrize("rows,inputs,outputs", [(40003, 264, 40), (20000, 512, 512),
-                                                 (3, 4096, 2056), (70000, 8, 256)])
+                                                 (3, 4096, 2056), (70000, 8, 256),
+                                                 (40003, 64, 280), (20001, 72, 281)])
 def test_larger(rows, inputs, outputs):
     s = make(rows, inputs, outputs, BF, FL, FL)
     check(call(s, "gelu"), s, "gelu")
