@@ -1,15 +1,60 @@
 // One new token a stream against a window's cache held in 4 bits: the step of
-// attention.cu with rows of codes, x ~ (c - 7.5) step + middle, c in 0..15.
+// attention.cu over rows of codes, x ~ (c - 7.5) step + middle with c in 0..15.
 //
-//   score_t = scale q . k_t,  p = softmax(score) over the slots that count,
-//   out = sum p_t v_t
-#include "tensorcore.cuh"
+//   score_t = scale q . k_t = scale (step_t (q . c_t) + (middle_t - 7.5 step_t) sum q)
+//   out = sum p_t v_t = sum (p_t step_t) (c_t - 7.5) + sum p_t middle_t
+//
+// so that codes go to the products as they are, small whole numbers of the 16-bit
+// type, and the ranges stay outside: a key's in two numbers a score, a value's in
+// its weight p_t step_t (rounded to the type, as a weight has to be for a product)
+// and in one float sum a head, which no rounding meets.
+//
+// The cache is read once; the codes of a row are half a byte a channel, so that
+// taking them apart (8 to 12 instructions a word of 8) weighs about as much as the
+// reading. A cluster of blocks shares the slots of a stream and key-value head, up
+// to 16 query heads (more: more clusters). A warp takes 32 slots at a time from a
+// ring in shared memory of its own, filled some turns ahead by cp.async, so that warps
+// never wait for one another; sums are joined at the end in order, in the block and
+// across the cluster: one launch, no workspace, no atomics.
+#include "step.cuh"
 
 namespace gs {
 namespace {
 
-constexpr int kThreads = 128;
 constexpr int kMaxDim = 128;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kSlots = 32;  // of a warp's turn
+constexpr float kLog2e = 1.44269504f;
+// As in attention.cu: growth (log2) of the scores' maximum that passes without
+// rescaling, and float16 weights' place above it.
+constexpr float kSlack = 8.0f;
+template <class T>
+constexpr bool kHalf = std::is_same_v<T, __half>;
+template <class T>
+constexpr float kLift = kHalf<T> ? 7.0f : 0.0f;
+
+template <int kDim>
+struct Stage {
+  static constexpr int kCount = kDim == 128 ? 3 : 5;  // of a warp's ring
+  static constexpr int kRow = kDim / 2;  // bytes; shorter rows leave the rest as it is
+  alignas(16) unsigned char codes[2][kSlots * kRow];  // keys', values'
+  uint32_t range[2][kSlots];  // step in the low half, middle in the high one
+};
+
+// What a slot's ranges come to: score = dot * key_step + (sum of q) * key_base.
+struct Slot {
+  float key_step, key_base, value_step, value_middle;
+};
+
+template <int kDim, int kHalves>
+struct Shared {
+  union {
+    Stage<kDim> stage[kWarps][Stage<kDim>::kCount];
+    float out[kWarps][8 * kHalves][kDim];  // once the stages are done
+  };
+  alignas(16) Slot slot[kWarps][kSlots];
+  float top[kWarps][8 * kHalves], sum[kWarps][8 * kHalves];
+};
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -22,124 +67,487 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return y;
 }
 
-template <class T>
+// The code of x. In double: (x - middle) and the quotient are then far more exact than
+// any two codes' border is close (step has 8 or 11 bits), so that ties are ties.
 __device__ __forceinline__ uint32_t code_of(float x, float step, float middle) {
   if (!(step > 0.0f && step < INFINITY)) return 8;
   const double place = rint((static_cast<double>(x) - middle) / static_cast<double>(step) + 7.5);
   return static_cast<uint32_t>(fmin(fmax(place, 0.0), 15.0));
 }
 
+// The new token's rows as they are held: lanes 0 to 15 have a word of eight channels of
+// the key's row each, lanes 16 to 31 of the value's.
+struct Fresh {
+  uint32_t codes, range;
+};
 template <class T>
-__global__ void __launch_bounds__(kThreads) step_kernel(gs_window_attention_step_4bit_args a) {
-  __shared__ float q[kMaxDim], weight[kThreads], parts[kThreads / 32];
-  __shared__ uint8_t fresh[2][kMaxDim / 2];
-  __shared__ T fresh_range[2][2];
+__device__ __forceinline__ Fresh round_row(const T* row, int dim) {
+  const int word = threadIdx.x & 15;
+  float x[8], high = -INFINITY, low = INFINITY;
+  if (8 * word < dim) {
+    load_pack<8>(row + 8 * word, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      high = max_nan(high, x[k]);
+      low = min_nan(low, x[k]);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  const T step = from_float<T>((high - low) / 15.0f);
+  const T middle = from_float<T>(0.5f * high + 0.5f * low);
+  Fresh f = {0, 0};
+  if (8 * word < dim)
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      f.codes |= code_of(x[k], to_float(step), to_float(middle)) << 4 * k;
+  f.range = static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(step)) |
+            static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(middle)) << 16;
+  return f;
+}
+
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t word) {
+  const T* v = reinterpret_cast<const T*>(&word);
+  return make_float2(to_float(v[0]), to_float(v[1]));
+}
+
+// Codes at bits 0 to 3 of both halves of `word`, or at bits 4 to 7 (float16 only:
+// bfloat16 has 7 bits behind the leading one), as numbers: next to a large power of
+// two, whose low bits they are, and that taken off again. Exact.
+template <class T>
+__device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
+  uint32_t y;
+  if constexpr (kHalf<T>) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  else asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+template <class T>
+__device__ __forceinline__ uint32_t above(uint32_t word) {  // 1024 + c, or 128 + c
+  return (word & 0x000f000fu) | (kHalf<T> ? 0x64006400u : 0x43004300u);
+}
+template <class T>
+__device__ __forceinline__ uint32_t centred(uint32_t word) {  // c - 8
+  return add_pair<T>(above<T>(word), kHalf<T> ? 0xe408e408u : 0xc308c308u);
+}
+__device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16 c) / 16 - 72
+  uint32_t y;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;"
+      : "=r"(y)
+      : "r"((word & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));
+  return y;
+}
+// Codes 0 to 3 of both halves of a word as four pairs.
+template <class T>
+__device__ __forceinline__ void spread(uint32_t word, uint32_t (&pair)[4]) {
+  if constexpr (kHalf<T>) {
+    const uint32_t next = word >> 8;
+    pair[0] = centred<T>(word);
+    pair[1] = centred_high(word);
+    pair[2] = centred<T>(next);
+    pair[3] = centred_high(next);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pair[e] = centred<T>(word >> 4 * e);
+  }
+}
+// The same for a key's: bfloat16 leaves the 128 in, which is taken off the score (its
+// error there, 2^-23 of 136 sum |q| step, is far below what q's bits allow; float16's
+// 1024 would not be).
+template <class T>
+constexpr float kKeyOffset = kHalf<T> ? 8.0f : 0.0f;  // what a key's numbers lack
+template <class T>
+__device__ __forceinline__ void spread_key(uint32_t word, uint32_t (&pair)[4]) {
+  if constexpr (kHalf<T>) {
+    spread<T>(word, pair);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pair[e] = above<T>(word >> 4 * e);
+  }
+}
+
+template <int kWords>
+__device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)[kWords]) {
+  static_assert(kWords == 1 || kWords == 2 || kWords == 4);
+  if constexpr (kWords == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (kWords == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
+  }
+}
+
+// kMasked: with validity of the slots. kAligned: rows of codes are whole 16-byte words.
+template <class T, int kDim, int kHalves, bool kMasked, bool kAligned>
+__global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : kHalves == 1 ? 3 : 2)
+    step_kernel(gs_window_attention_step_4bit_args a) {
+  using S = Shared<kDim, kHalves>;
+  constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
+  constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
+  constexpr int kValueWords = kDim / 64;  // of a value's, of eight
+  constexpr int kHeads = 8 * kHalves;
+  extern __shared__ __align__(16) unsigned char shared_bytes[];
+  S& s = *reinterpret_cast<S*>(shared_bytes);
   chain_wait();
-  const int group = a.heads / a.kv_heads;
-  const int64_t b = blockIdx.x / a.heads;
-  const int head = blockIdx.x % a.heads, kv_head = head / group;
-  const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  const uint32_t rank = cluster_rank(), blocks = cluster_size();
+  const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
+  const int64_t item = blockIdx.x / blocks;
+  const int piece = static_cast<int>(item % pieces);
+  const int kv_head = static_cast<int>(item / pieces % a.kv_heads);
+  const int64_t b = item / pieces / a.kv_heads;
+  const int head0 = kv_head * group + piece * kHeads;
+  const int heads = min(kHeads, group - piece * kHeads);
   const int64_t position = a.positions[b];
-  T* const out = static_cast<T*>(a.out) + (b * a.heads + head) * a.dim;
-  if (position < 0) {
-    if (thread < a.dim) out[thread] = from_float<T>(0.0f);
-    return;
-  }
-  const int64_t slot = position < a.first
-                           ? position
-                           : a.first + (position - a.first) % (a.slots - a.first);
-  const int count = static_cast<int>(min(position + 1, int64_t{a.slots}));
+  const bool idle = position < 0;
+  const int slot = idle ? -1
+                        : static_cast<int>(position < a.first
+                                               ? position
+                                               : a.first + (position - a.first) %
+                                                               (a.slots - a.first));
+  const int count = idle ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
+  const int row_bytes = a.dim / 2;
   const int64_t row0 = (b * a.kv_heads + kv_head) * a.slots;
-  const bool token_valid = !a.cache_valid || !a.valid || a.valid[b];
-  const bool writes = head % group == 0;
-  if (a.cache_valid && head == 0 && thread == 0) a.cache_valid[b * a.slots + slot] = token_valid;
-  // The new token's rows as they are held.
-  for (int side = 0; side < 2; ++side) {
-    const T* x = side == 0
-                     ? static_cast<const T*>(a.k) + b * a.k_stride + kv_head * a.k_head_stride
-                     : static_cast<const T*>(a.v) + b * a.v_stride + kv_head * a.v_head_stride;
-    if (warp == 0) {
-      float high = -INFINITY, low = INFINITY;
-      for (int c = lane; c < a.dim; c += 32) {
-        high = max_nan(high, to_float(x[c]));
-        low = min_nan(low, to_float(x[c]));
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
-      }
-      const T step = from_float<T>((high - low) / 15.0f);
-      const T middle = from_float<T>(0.5f * high + 0.5f * low);
-      for (int c = lane; c < a.dim / 2; c += 32)
-        fresh[side][c] = static_cast<uint8_t>(
-            code_of<T>(to_float(x[2 * c]), to_float(step), to_float(middle)) |
-            code_of<T>(to_float(x[2 * c + 1]), to_float(step), to_float(middle)) << 4);
-      if (lane == 0) {
-        fresh_range[side][0] = step;
-        fresh_range[side][1] = middle;
+  uint8_t* const codes[2] = {a.k_codes + row0 * row_bytes, a.v_codes + row0 * row_bytes};
+  uint32_t* const range[2] = {static_cast<uint32_t*>(a.k_range) + row0,
+                              static_cast<uint32_t*>(a.v_range) + row0};
+  uint8_t* const slots_valid = kMasked ? a.cache_valid + b * a.slots : nullptr;
+  const bool token_valid = !kMasked || !a.valid || a.valid[b];
+
+  // This warp's turns of 32 slots: me, me + all, ...
+  const int me = static_cast<int>(rank) * kWarps + warp, all = static_cast<int>(blocks) * kWarps;
+  const int turns = max(0, ((count + kSlots - 1) / kSlots - me + all - 1) / all);
+  const auto base_of = [&](int t) { return (me + t * all) * kSlots; };
+  const auto load = [&](int t) {
+    if (t < turns) {
+      Stage<kDim>& st = s.stage[warp][t % kStages];
+      const int base = base_of(t);
+      const int last = count - 1 - base;  // slots behind it are that one again
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        if constexpr (kAligned) {
+          const int pieces16 = row_bytes >> 4;  // of a row: 1 to 4
+#pragma unroll
+          for (int r = 0; r < kDim / 32; ++r) {
+            const int i = lane + 32 * r;
+            const int row = i / (kDim / 32), piece16 = i % (kDim / 32);
+            if (piece16 >= pieces16) continue;
+            cp_async16(st.codes[side] + row * kRow + 16 * piece16,
+                       codes[side] + int64_t{base + min(row, last)} * row_bytes + 16 * piece16);
+          }
+        } else {
+          const uint8_t* from = codes[side] + int64_t{base + min(lane, last)} * row_bytes;
+          for (int w = 0; w < row_bytes; w += 4)
+            cp_async4(st.codes[side] + lane * kRow + w, from + w);
+        }
+        cp_async4(&st.range[side][lane], range[side] + base + min(lane, last));
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto seen_in = [&](int t) {  // whether the lane's slot of a turn may be seen
+    if (t >= turns) return false;
+    const int at = base_of(t) + lane;
+    if (at >= count) return false;
+    return !kMasked || (at == slot ? token_valid : slots_valid[at] != 0);
+  };
+#pragma unroll
+  for (int t = 0; t < kStages - 1; ++t) load(t);
+  bool seen_next = seen_in(0);
+
+  // The warp whose turn has the new token's slot rounds its rows.
+  const int slot_turn = idle ? -1 : slot / kSlots;
+  const bool owner = slot_turn >= 0 && slot_turn % all == me;
+  Fresh fresh = {0, 0};
+  if (owner) {
+    const bool value = lane >= 16;
+    fresh = round_row(value ? static_cast<const T*>(a.v) + b * a.v_stride + kv_head * a.v_head_stride
+                            : static_cast<const T*>(a.k) + b * a.k_stride + kv_head * a.k_head_stride,
+                      a.dim);
+    if (piece == 0) {
+      if (8 * (lane & 15) < a.dim)
+        *reinterpret_cast<uint32_t*>(codes[value] + int64_t{slot} * row_bytes + 4 * (lane & 15)) =
+            fresh.codes;
+      if ((lane & 15) == 0) range[value][slot] = fresh.range;
+      if (kMasked && kv_head == 0 && lane == 0) slots_valid[slot] = token_valid;
+    }
   }
-  if (thread < a.dim)
-    q[thread] = to_float(static_cast<const T*>(a.q)[b * a.q_stride + head * a.q_head_stride + thread]) *
-                a.scale;
+
+  // q's rows g (and g + 8), channels in the order of the keys' products: a word's are
+  // pairs (0, 4), (1, 5) of one product and (2, 6), (3, 7) of the next. And q's sums.
+  uint32_t q[kKeyWords][2][kHalves][2];
+  float q_sum[kHalves];
+#pragma unroll
+  for (int r = 0; r < kHalves; ++r) {
+    q_sum[r] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kKeyWords; ++w) {
+      const int channel = 8 * (kKeyWords * j + w);
+      uint4 word = make_uint4(0, 0, 0, 0);
+      if (g + 8 * r < heads && channel < a.dim)
+        word = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride +
+                                               (head0 + g + 8 * r) * a.q_head_stride + channel);
+      q[w][0][r][0] = __byte_perm(word.x, word.z, 0x5410);
+      q[w][0][r][1] = __byte_perm(word.x, word.z, 0x7632);
+      q[w][1][r][0] = __byte_perm(word.y, word.w, 0x5410);
+      q[w][1][r][1] = __byte_perm(word.y, word.w, 0x7632);
+      const float2 x01 = unpack2<T>(word.x), x23 = unpack2<T>(word.y);
+      const float2 x45 = unpack2<T>(word.z), x67 = unpack2<T>(word.w);
+      q_sum[r] += ((x01.x + x01.y) + (x23.x + x23.y)) + ((x45.x + x45.y) + (x67.x + x67.y));
+    }
+    q_sum[r] += __shfl_xor_sync(0xffffffffu, q_sum[r], 1);
+    q_sum[r] += __shfl_xor_sync(0xffffffffu, q_sum[r], 2);
+  }
+  const float scale = a.scale * kLog2e;
+  float out[kValueWords][8][kHalves][2] = {};
+  float top[kHalves], sum[kHalves] = {}, middle_sum[kHalves] = {};
+#pragma unroll
+  for (int r = 0; r < kHalves; ++r) top[r] = -INFINITY;
+  // float16: value steps are taken relative to a power of two above the largest so far,
+  // so that weights times steps stay in float16's range whatever the values' size.
+  uint32_t unit = 0;  // its bits
+  float per_unit = 1.0f;
+
+  // Slots in the order of the products' columns: column n of the first is slot n / 2 + 4
+  // (n % 2), so that a lane's four slots as rows of P V, and its neighbours', lie next to
+  // one another: j, 4 + j, 8 + j, 12 + j.
+  const int key_row = (g >> 1) + 4 * (g & 1);
+  for (int t = 0; t < turns; ++t) {
+    load(t + kStages - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    Stage<kDim>& st = s.stage[warp][t % kStages];
+    const int base = base_of(t);
+    const bool seen = seen_next;
+    seen_next = seen_in(t + 1);
+    if (owner && base == slot_turn * kSlots) {
+      const int side = lane >> 4, word = lane & 15;
+      if (8 * word < a.dim)
+        *reinterpret_cast<uint32_t*>(st.codes[side] + (slot - base) * kRow + 4 * word) = fresh.codes;
+      if (word == 0) st.range[side][slot - base] = fresh.range;
+      __syncwarp();
+    }
+    // A slot a lane: its ranges, zeros where it is not seen.
+    const uint32_t visible = __ballot_sync(0xffffffffu, seen);
+    {
+      const float2 key = unpack2<T>(seen ? st.range[0][lane] : 0);
+      const float2 value = unpack2<T>(seen ? st.range[1][lane] : 0);
+      float step = value.x;
+      if constexpr (kHalf<T>) {
+        const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(step) & 0x7fffffffu);
+        if (largest >= unit) {  // the same for the whole warp
+          const uint32_t next = min(largest & 0x7f800000u, 0x7e000000u) + 0x00800000u;
+          const float shrink = unit ? __uint_as_float(unit) / __uint_as_float(next) : 0.0f;
+#pragma unroll
+          for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int r = 0; r < kHalves; ++r) {
+                out[h][i][r][0] *= shrink;
+                out[h][i][r][1] *= shrink;
+              }
+          unit = next;
+          per_unit = __uint_as_float(0x7f000000u - next);
+        }
+        step *= per_unit;
+      }
+      s.slot[warp][lane] = {key.x * scale,
+                            fmaf(key.x, kKeyOffset<T> - (kHalf<T> ? 7.5f : 135.5f), key.y) * scale,
+                            step, fmaf(0.5f, value.x, value.y)};
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {  // 16 slots
+      Slot of[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) of[i] = s.slot[warp][16 * half + 4 * i + j];
+      float x[2][kHalves][2] = {};  // scores of the slots of[2n], of[2n + 1]
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        uint32_t word[kKeyWords];
+        read_words<kKeyWords>(
+            st.codes[0] + (16 * half + 8 * n + key_row) * kRow + 4 * kKeyWords * j, word);
+#pragma unroll
+        for (int w = 0; w < kKeyWords; ++w) {
+          uint32_t pair[4];
+          spread_key<T>(word[w], pair);
+          warp_product<T, kHalves>(x[n], q[w][0], pair[0], pair[1]);
+          warp_product<T, kHalves>(x[n], q[w][1], pair[2], pair[3]);
+        }
+      }
+      uint32_t p[kHalves][2];
+      const uint32_t mine = visible >> (16 * half + j);  // bits 0, 4, 8, 12
+#pragma unroll
+      for (int r = 0; r < kHalves; ++r) {
+        float next = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = 2 * n + e;
+            x[n][r][e] = fmaf(x[n][r][e], of[i].key_step, q_sum[r] * of[i].key_base);
+            if (!(mine >> 4 * i & 1)) x[n][r][e] = -INFINITY;
+            next = fmaxf(next, x[n][r][e]);
+          }
+        next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 1));
+        next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 2));
+        const bool grow = next > top[r] + kSlack || (top[r] == -INFINITY && next > top[r]);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float shrink = grow ? tc::exp2_approx(top[r] - next) : 1.0f;
+          if (grow) top[r] = next;
+          sum[r] *= shrink;
+          middle_sum[r] *= shrink;
+#pragma unroll
+          for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              out[h][i][r][0] *= shrink;
+              out[h][i][r][1] *= shrink;
+            }
+        }
+        const float shift = top[r] == -INFINITY ? 0.0f : kLift<T> - top[r];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = tc::exp2_approx(x[n][r][0] + shift);
+          const float p1 = tc::exp2_approx(x[n][r][1] + shift);
+          sum[r] += p0 + p1;
+          middle_sum[r] = fmaf(p0, of[2 * n].value_middle,
+                               fmaf(p1, of[2 * n + 1].value_middle, middle_sum[r]));
+          p[r][n] = tc::pack2<T>(p0 * of[2 * n].value_step, p1 * of[2 * n + 1].value_step);
+        }
+      }
+      uint32_t word[4][kValueWords];  // of the slots j, 4 + j, 8 + j, 12 + j
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        read_words<kValueWords>(
+            st.codes[1] + (16 * half + 4 * i + j) * kRow + 4 * kValueWords * g, word[i]);
+#pragma unroll
+      for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // a word's low and high half
+          uint32_t first[4], second[4];
+          const uint32_t order = c ? 0x7632 : 0x5410;
+          spread<T>(__byte_perm(word[0][h], word[1][h], order), first);
+          spread<T>(__byte_perm(word[2][h], word[3][h], order), second);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            warp_product<T, kHalves>(out[h][4 * c + e], p, first[e], second[e]);
+        }
+    }
+    __syncwarp();  // all lanes are done with the stage that the next turn fills
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the stages' place is free for the outputs
+
+  // The warp's rows to shared memory: product (h, i)'s column n is channel 8 (kValueWords n
+  // + h) + i.
+  const float unit_size = kHalf<T> ? __uint_as_float(unit) : 1.0f;
+#pragma unroll
+  for (int r = 0; r < kHalves; ++r) {
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+      middle_sum[r] += __shfl_xor_sync(0xffffffffu, middle_sum[r], o);
+    }
+    if (j == 0) {
+      s.top[warp][g + 8 * r] = top[r];
+      s.sum[warp][g + 8 * r] = sum[r];
+    }
+#pragma unroll
+    for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          s.out[warp][g + 8 * r][8 * (kValueWords * (2 * j + e) + h) + i] =
+              fmaf(out[h][i][r][e], unit_size, middle_sum[r]);
+  }
   __syncthreads();
-  if (writes)
-    for (int side = 0; side < 2; ++side) {
-      uint8_t* codes = (side == 0 ? a.k_codes : a.v_codes) + (row0 + slot) * (a.dim / 2);
-      T* range = static_cast<T*>(side == 0 ? a.k_range : a.v_range) + (row0 + slot) * 2;
-      if (thread < a.dim / 2) codes[thread] = fresh[side][thread];
-      if (thread < 2) range[thread] = fresh_range[side][thread];
-    }
-  const auto row_of = [&](int side, int at) {
-    return at == slot ? fresh[side]
-                      : (side == 0 ? a.k_codes : a.v_codes) + (row0 + at) * (a.dim / 2);
-  };
-  const auto range_of = [&](int side, int at) {
-    return at == slot ? fresh_range[side]
-                      : static_cast<const T*>(side == 0 ? a.k_range : a.v_range) + (row0 + at) * 2;
-  };
-  float top = -INFINITY, sum = 0.0f, o = 0.0f;
-  for (int base = 0; base < count; base += kThreads) {
-    const int at = base + thread;
-    float score = -INFINITY;
-    if (at < count &&
-        (!a.cache_valid || (at == slot ? token_valid : a.cache_valid[b * a.slots + at] != 0))) {
-      const uint8_t* codes = row_of(0, at);
-      const T* range = range_of(0, at);
-      const float step = to_float(range[0]), middle = to_float(range[1]);
-      score = 0.0f;
-      for (int c = 0; c < a.dim / 2; ++c) {
-        const uint32_t two = codes[c];
-        score = fmaf(q[2 * c], fmaf(static_cast<float>(two & 15) - 7.5f, step, middle), score);
-        score = fmaf(q[2 * c + 1], fmaf(static_cast<float>(two >> 4) - 7.5f, step, middle), score);
-      }
-    }
-    __syncthreads();  // parts and weights of the tile before are read
-    float high = warp_max(score);
-    if (lane == 0) parts[warp] = high;
-    weight[thread] = score;
-    __syncthreads();
-    for (float x : parts) high = fmaxf(high, x);
-    const float next = fmaxf(top, high), shift = next == -INFINITY ? 0.0f : next;
-    const float shrink = expf(top - shift);
-    top = next;
-    sum *= shrink;
-    o *= shrink;
-    const int tile = min(kThreads, count - base);
-    for (int t = 0; t < tile; ++t) {
-      if (weight[t] == -INFINITY) continue;  // what is left out must not meet its weight
-      const float p = expf(weight[t] - shift);
-      sum += p;
-      if (thread < a.dim) {
-        const uint32_t two = row_of(1, base + t)[thread / 2];
-        const T* range = range_of(1, base + t);
-        const float c = static_cast<float>(thread & 1 ? two >> 4 : two & 15);
-        o = fmaf(p, fmaf(c - 7.5f, to_float(range[0]), to_float(range[1])), o);
-      }
-    }
+  // The warps joined into the first one's place.
+  for (int c = threadIdx.x; c < heads * kDim; c += kThreads) {
+    const int h = c / kDim, d = c % kDim;
+    float whole = -INFINITY, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      o = fmaf(s.out[w][h][d], tc::exp2_approx(s.top[w][h] - shift), o);
+    s.out[0][h][d] = o;
   }
-  if (thread < a.dim) out[thread] = from_float<T>(sum == 0.0f ? 0.0f : o / sum);
+  __syncthreads();
+  if (threadIdx.x < heads) {
+    const int h = threadIdx.x;
+    float whole = -INFINITY, total = 0.0f;
+    for (int w = 0; w < kWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+    for (int w = 0; w < kWarps; ++w)
+      total = fmaf(s.sum[w][h], tc::exp2_approx(s.top[w][h] - shift), total);
+    s.top[0][h] = whole;
+    s.sum[0][h] = total;
+  }
+  cluster_sync();
+  // The blocks joined, each block a part of the outputs.
+  for (int c = static_cast<int>(rank) * kThreads + threadIdx.x; c < heads * kDim;
+       c += static_cast<int>(blocks) * kThreads) {
+    const int h = c / kDim, d = c % kDim;
+    float whole = -INFINITY, total = 0.0f, o = 0.0f;
+    for (uint32_t r = 0; r < blocks; ++r) whole = fmaxf(whole, read_block(&s.top[0][h], r));
+    const float shift = whole == -INFINITY ? 0.0f : whole;
+    for (uint32_t r = 0; r < blocks; ++r) {
+      const float w = tc::exp2_approx(read_block(&s.top[0][h], r) - shift);
+      total = fmaf(read_block(&s.sum[0][h], r), w, total);
+      o = fmaf(read_block(&s.out[0][h][d], r), w, o);
+    }
+    if (d < a.dim)
+      static_cast<T*>(a.out)[(b * a.heads + head0 + h) * a.dim + d] =
+          from_float<T>(total == 0.0f ? 0.0f : o / total);
+  }
+  cluster_sync();  // the others have read this block's shared memory
+}
+
+// Blocks of a cluster: enough that every multiprocessor has several, as far as every
+// warp still gets a turn.
+int step_blocks(const gs_window_attention_step_4bit_args& a, int64_t items) {
+  int blocks = 1;
+  while (blocks < 16 && items * blocks < 4 * kSmCount && blocks * kWarps * kSlots < a.slots)
+    blocks *= 2;
+  return blocks;
+}
+
+template <class T, int kDim, int kHalves, bool kMasked, bool kAligned>
+int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
+  const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kHalves);
+  const int blocks = step_blocks(a, items);
+  if (items * blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  constexpr size_t kShared = sizeof(Shared<kDim, kHalves>);
+  GS_TRY((allow_shared<step_kernel<T, kDim, kHalves, kMasked, kAligned>>(kShared, true)));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = static_cast<unsigned>(items * blocks);
+  config.blockDim = kThreads;
+  config.dynamicSmemBytes = kShared;
+  config.stream = stream;
+  config.attrs = attr;
+  config.numAttrs = 2;
+  cudaLaunchKernelEx(&config, step_kernel<T, kDim, kHalves, kMasked, kAligned>, a);
+  return check_launch();
 }
 
 bool strided16(const void* p, int64_t stride, int64_t head_stride) {
@@ -168,11 +576,24 @@ int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_ar
       !is_aligned(a.v_codes, 16) || !is_aligned(a.k_range, 16) || !is_aligned(a.v_range, 16) ||
       !is_aligned(a.out, 16) || !is_aligned(a.positions, 8))
     return GS_ERR_MISALIGNED;
-  if (a.batch * a.heads > INT32_MAX) return GS_ERR_CAPACITY;
-  const unsigned blocks = static_cast<unsigned>(a.batch * a.heads);
-  if (a.dtype == GS_BFLOAT16) launch_chained(step_kernel<__nv_bfloat16>, blocks, kThreads, stream, a);
-  else launch_chained(step_kernel<__half>, blocks, kThreads, stream, a);
-  return check_launch();
+  const auto typed = [&](auto t) {
+    using T = decltype(t);
+    const auto shaped = [&](auto masked, auto aligned) {
+      constexpr bool kMasked = decltype(masked)::value, kAligned = decltype(aligned)::value;
+      if (a.heads / a.kv_heads <= 8)
+        return a.dim <= 64 ? step<T, 64, 1, kMasked, kAligned>(a, stream)
+                           : step<T, 128, 1, kMasked, kAligned>(a, stream);
+      return a.dim <= 64 ? step<T, 64, 2, kMasked, kAligned>(a, stream)
+                         : step<T, 128, 2, kMasked, kAligned>(a, stream);
+    };
+    const bool aligned = a.dim % 32 == 0;
+    if (a.cache_valid)
+      return aligned ? shaped(std::true_type{}, std::true_type{})
+                     : shaped(std::true_type{}, std::false_type{});
+    return aligned ? shaped(std::false_type{}, std::true_type{})
+                   : shaped(std::false_type{}, std::false_type{});
+  };
+  return a.dtype == GS_BFLOAT16 ? typed(__nv_bfloat16{}) : typed(__half{});
 }
 
 }  // namespace gs

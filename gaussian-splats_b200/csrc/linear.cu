@@ -21,10 +21,11 @@ using namespace tc;
 // to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact. (A
 // float32 bias's gradient is a sum of unrounded dz: there slopes are kept as floats.)
 constexpr float kSlopeScale = 49152.0f, kSlopeZero = 8192.0f, kTwo23 = 8388608.0f;
-__device__ __forceinline__ uint32_t slope_codes(float low, float high) {
+__device__ __forceinline__ uint32_t slope_codes(float2 slopes) {
   // The sums' low bits are the nearest whole numbers.
-  return __byte_perm(__float_as_uint(fmaf(low, kSlopeScale, kTwo23 + kSlopeZero)),
-                     __float_as_uint(fmaf(high, kSlopeScale, kTwo23 + kSlopeZero)), 0x5410);
+  const float2 x = fma2(slopes, make_float2(kSlopeScale, kSlopeScale),
+                        make_float2(kTwo23 + kSlopeZero, kTwo23 + kSlopeZero));
+  return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x5410);
 }
 __device__ __forceinline__ float slope_value(uint32_t code) {
   return (__uint_as_float(0x4b000000u | code) - (kTwo23 + kSlopeZero)) * (1.0f / kSlopeScale);
@@ -36,45 +37,53 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
   return y;
 }
 
-// act(z) in z, act'(z) in slope.
+// act(z) in z, act'(z) in slope; two floats an instruction where there is one.
 //
 // gelu: with t = |z|, the normal distribution's upper tail is e^(-t^2/2) R(t), R smooth
 // (Mills' ratio over sqrt(2 pi)); R = u P(u) with u = 1 / (1 + 0.3 t) and P the polynomial
 // of degree 7 with the least relative error for t up to 14, 1.5e-7. The density that
 // the slope needs is the same exponential.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 template <int kCount>
-__device__ __forceinline__ void activate(int kind, float (&z)[kCount], float (&slope)[kCount]) {
+__device__ __forceinline__ void activate(int kind, float2 (&z)[kCount], float2 (&slope)[kCount]) {
   if (kind == GS_RELU) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      slope[i] = z[i] > 0.0f ? 1.0f : 0.0f;
-      z[i] = z[i] < 0.0f ? 0.0f : z[i];  // NaN stays
+      slope[i] = make_float2(z[i].x > 0.0f ? 1.0f : 0.0f, z[i].y > 0.0f ? 1.0f : 0.0f);
+      z[i] = make_float2(z[i].x < 0.0f ? 0.0f : z[i].x, z[i].y < 0.0f ? 0.0f : z[i].y);  // NaN stays
     }
   } else if (kind == GS_GELU) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const float t = fabsf(z[i]);
-      const float u = reciprocal_approx(fmaf(t, 0.3f, 1.0f));
-      const float e = exp2_approx(z[i] * z[i] * -0.72134752f);
-      float p = fmaf(0.0356748066842556f, u, -0.15720321238040924f);
-      p = fmaf(p, u, 0.20635370910167694f);
-      p = fmaf(p, u, -0.053683821111917496f);
-      p = fmaf(p, u, 0.12856172025203705f);
-      p = fmaf(p, u, 0.09991347044706345f);
-      p = fmaf(p, u, 0.12075395882129669f);
-      p = fmaf(p, u, 0.11962930113077164f);
-      const float tail = p * u * e;
-      const float below = z[i] < 0.0f ? tail : 1.0f - tail;
-      slope[i] = fmaf(z[i] * 0.39894228f, e, below);
-      z[i] = z[i] * below;
+      const float2 t = make_float2(fabsf(z[i].x), fabsf(z[i].y));
+      const float2 d = fma2(t, both(0.3f), both(1.0f));
+      const float2 u = make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
+      const float2 x = mul2(mul2(z[i], z[i]), both(-0.72134752f));
+      const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+      float2 p = fma2(both(0.0356748066842556f), u, both(-0.15720321238040924f));
+      p = fma2(p, u, both(0.20635370910167694f));
+      p = fma2(p, u, both(-0.053683821111917496f));
+      p = fma2(p, u, both(0.12856172025203705f));
+      p = fma2(p, u, both(0.09991347044706345f));
+      p = fma2(p, u, both(0.12075395882129669f));
+      p = fma2(p, u, both(0.11962930113077164f));
+      const float2 tail = mul2(mul2(p, u), e);
+      // What lies below z: the tail, or 1 less it. Not by 0.5 +- (0.5 - tail): small tails
+      // keep their digits.
+      const float2 rest = fma2(tail, both(-1.0f), both(1.0f));
+      const float2 below = make_float2(z[i].x < 0.0f ? tail.x : rest.x,
+                                       z[i].y < 0.0f ? tail.y : rest.y);
+      slope[i] = fma2(mul2(z[i], both(0.39894228f)), e, below);
+      z[i] = mul2(z[i], below);
     }
   } else if (kind == GS_SILU) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const float gate = reciprocal_approx(1.0f + exp2_approx(z[i] * -1.44269504f));
-      const float y = z[i] * gate;
-      slope[i] = fmaf(y, 1.0f - gate, gate);
-      z[i] = y;
+      const float2 x = mul2(z[i], both(-1.44269504f));
+      const float2 d = add2(make_float2(exp2_approx(x.x), exp2_approx(x.y)), both(1.0f));
+      const float2 gate = make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
+      z[i] = mul2(z[i], gate);
+      slope[i] = fma2(z[i], fma2(gate, both(-1.0f), both(1.0f)), gate);
     }
   }
 }
@@ -99,7 +108,7 @@ constexpr int kRows = 128;   // of a tile
 constexpr int kDepth = 64;   // of a stage: 128 bytes of channels, or 64 rows
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductThreads = 32 * (kEpilogueWarps + 2);
-constexpr int kChunkBytes = 4096;  // 32 rows of 32 floats, or of 32 16-bit elements in half of it
+constexpr int kChunkBytes = 4096;  // of the epilogue: 32 rows of 128 bytes
 
 // What becomes of the sums D(m, n).
 struct Epilogue {
@@ -119,7 +128,7 @@ struct Epilogue {
   bool tiled;
 };
 
-// The maps of what the epilogue reads and writes, in boxes of 32 rows of 32 columns.
+// The maps of what the epilogue reads and writes, in its chunks.
 struct EpilogueMaps {
   CUtensorMap out, residual, slope;
 };
@@ -139,16 +148,20 @@ struct ProductShared {
   alignas(1024) unsigned char a[kStages][kABytes];
   alignas(1024) unsigned char b[kStages][kBBytes];
   alignas(1024) unsigned char out[kEpilogueWarps][2][kChunkBytes];
+  // Columns of a 16-bit chunk: rows of 128 bytes (TMA takes about as long for rows of 64),
+  // unless the tile is too narrow to give all warps chunks of them.
+  static constexpr int kWide = kN >= 128 ? 64 : 32;
+  float bias[kEpilogueWarps][kN];
   uint64_t full[kStages], empty[kStages], ready[2], drained[2], residual[kEpilogueWarps][2];
   uint32_t tensor;
 };
 
-// 32 columns of a row's chunk to shared memory and back, as TMA's swizzle has them:
-// rows of 128 bytes (floats) or 64 (16 bits), whose 16-byte words are exchanged so that
-// eight rows' same words lie in different banks.
-__device__ __forceinline__ uint32_t word_of(uint32_t chunk, int row, int word, bool wide) {
-  return wide ? chunk + row * 128 + ((word ^ (row & 7)) << 4)
-              : chunk + row * 64 + ((word ^ (row >> 1 & 3)) << 4);
+// A 16-byte word of a chunk's row, where TMA's swizzle has it: rows of 128 bytes or
+// of 64, whose words are exchanged so that eight rows' same words lie in different banks.
+template <int kBytes>
+__device__ __forceinline__ uint32_t word_of(uint32_t chunk, int row, int word) {
+  return kBytes == 128 ? chunk + row * 128 + ((word ^ (row & 7)) << 4)
+                       : chunk + row * 64 + ((word ^ (row >> 1 & 3)) << 4);
 }
 __device__ __forceinline__ void put_word(uint32_t at, uint32_t a, uint32_t b, uint32_t c,
                                          uint32_t d) {
@@ -182,146 +195,176 @@ __device__ __forceinline__ void wait_stores_done() {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// The epilogue's warps: a row a thread, 32 columns at a time. Chunks pass through shared
-// memory, from which TMA writes them; the residual's come by TMA to the place of the
-// results, a chunk ahead. Where rows are no whole 16-byte words, a warp writes 32
-// columns of one row at a time instead.
+// The epilogue's warps: a row a thread, 32 columns at a time. Chunks of 32 floats' or
+// kWide 16-bit columns pass through shared memory, from which TMA writes them; the
+// residual's come by TMA to the place of the results, a chunk ahead if two fit. Where
+// rows are no whole 16-byte words, a warp writes 32 columns of one row at a time instead.
 template <class T, int kN>
 __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps& maps,
                          ProductShared<kN>& s, uint32_t tensor, int warp, int lane) {
+  constexpr int kWide = ProductShared<kN>::kWide, kNarrowBytes = kWide * 2;
+  constexpr int kParts = kWide / 32;  // steps of 32 columns of a 16-bit chunk
   const int64_t tiles = int64_t{plan.row_tiles} * plan.column_tiles, items = tiles * plan.splits;
   const bool wide = e.out_dtype == GS_FLOAT32;
-  const int slope_bytes = !e.slope ? 0 : e.slope_float ? kChunkBytes : kChunkBytes / 2;
-  const int chunk_bytes = (wide ? kChunkBytes : kChunkBytes / 2) + slope_bytes;
-  const bool two = 2 * chunk_bytes <= 2 * kChunkBytes;  // chunks in two places in turn
+  const bool two = !e.slope;  // two chunks in turn; with slopes, one and its slopes
   const uint32_t staged = shared_address(s.out[warp]);
+  float* const biases = s.bias[warp];
   struct Place {
     int64_t item;
-    int c;  // chunk of the tile
+    int c;  // step of 32 columns: kParts of them in a row, then the other warps' kParts
   };
+  const int c0 = (warp >> 2) * kParts;
   const auto column_of = [&](const Place& p) {
     return static_cast<int>(p.item % tiles % plan.column_tiles) * kN + 32 * p.c;
   };
   const auto row_of = [&](const Place& p) {
     return static_cast<int>(p.item % tiles / plan.column_tiles) * kRows + 32 * (warp & 3);
   };
-  // This place, or the warp's next one that has columns.
-  const auto from = [&](Place p) {
+  const auto next_step = [&](int c) { return (c + 1) % kParts ? c + 1 : c + 1 + kParts; };
+  // The place, or the warp's next one, that has columns and starts a chunk.
+  const auto chunk_from = [&](Place p) {
     while (p.item < items && (p.c >= kN / 32 || column_of(p) >= e.columns))
-      p = {p.item + gridDim.x, warp >> 2};
+      p = {p.item + gridDim.x, c0};
     return p;
+  };
+  const auto chunk_after = [&](Place p) {
+    p.c = wide ? next_step(p.c) : p.c + 2 * kParts;
+    return chunk_from(p);
   };
   const auto load_residual = [&](const Place& p, uint32_t use) {
     if (p.item >= items) return;
     const uint32_t at = two ? use & 1 : 0;
     const uint32_t bar = shared_address(&s.residual[warp][at]);
-    barrier_expect(bar, wide ? kChunkBytes : kChunkBytes / 2);
-    load_box(staged + at * chunk_bytes, &maps.residual, column_of(p), row_of(p), bar);
+    barrier_expect(bar, wide ? kChunkBytes : 32 * kNarrowBytes);
+    load_box(staged + at * kChunkBytes, &maps.residual, column_of(p), row_of(p), bar);
   };
   const bool by_tma = e.tiled, add = e.residual != nullptr;
   bool good = true;
   uint32_t use = 0;  // chunks done
-  Place p = {blockIdx.x, warp >> 2};
-  if (by_tma && add && lane == 0) load_residual(from(p), 0);
+  if (by_tma && add && lane == 0) load_residual(chunk_from({blockIdx.x, c0}), 0);
   uint32_t count = 0;
+  int bias_column = -1;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
     const uint32_t buffer = count & 1;
-    p = {item, warp >> 2};
-    const int row = row_of(p);
+    const int n0 = column_of({item, 0});
+    if (e.bias && n0 != bias_column) {
+      __syncwarp();
+      for (int i = lane; i < kN; i += 32)
+        biases[i] = n0 + i < e.columns ? read_as(e.bias, e.bias_dtype, n0 + i) : 0.0f;
+      __syncwarp();
+      bias_column = n0;
+    }
+    const int row = row_of({item, 0});
     const int64_t out_row = item / tiles * plan.split_rows + row;
     good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
     fence_after_sync();
-    for (; p.c < kN / 32; p.c += 2) {
-      const int n = column_of(p);
+    for (int c = c0; c < kN / 32; c = next_step(c)) {
+      const Place p = {item, c};
+      const int n = n0 + 32 * c;
       if (n >= e.columns) break;
-      float z[32], slope[32];
-      float bias = 0.0f;
-      if (e.bias && n + lane < e.columns) bias = read_as(e.bias, e.bias_dtype, n + lane);
-      load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * p.c,
-                     z);
+      float2 z[16], slope[16];
+      load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * c,
+                     reinterpret_cast<float(&)[32]>(z));
       wait_loads();
       if (!good)
-        for (float& x : z) x = NAN;
+        for (float2& x : z) x = both(NAN);
       if (e.bias)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) z[i] += __shfl_sync(0xffffffffu, bias, i);
+        for (int i = 0; i < 8; ++i) {
+          const float4 b = *reinterpret_cast<const float4*>(biases + 32 * c + 4 * i);
+          z[2 * i] = add2(z[2 * i], make_float2(b.x, b.y));
+          z[2 * i + 1] = add2(z[2 * i + 1], make_float2(b.z, b.w));
+        }
       activate(e.activation, z, slope);
+      const int part = c % kParts;  // of a 16-bit chunk
       if (by_tma) {
-        const uint32_t at = two ? use & 1 : 0, chunk = staged + at * chunk_bytes;
-        if (lane == 0) {
-          if (two && !add) wait_stores_read<1>();
-          else wait_stores_read<0>();
-          if (add && two) load_residual(from({p.item, p.c + 2}), use + 1);
+        const uint32_t at = two ? use & 1 : 0, chunk = staged + at * kChunkBytes;
+        const uint32_t slope_chunk = staged + kChunkBytes;
+        if (wide || part == 0) {
+          if (lane == 0) {
+            if (two && !add) wait_stores_read<1>();
+            else wait_stores_read<0>();
+            if (add && two) load_residual(chunk_after(p), use + 1);
+          }
+          if (add)
+            good = good && barrier_wait_warp(shared_address(&s.residual[warp][at]),
+                                             (two ? use >> 1 : use) & 1);
+          __syncwarp();
         }
-        if (add) {
-          good = good && barrier_wait_warp(shared_address(&s.residual[warp][at]),
-                                           (two ? use >> 1 : use) & 1);
-        }
-        __syncwarp();
         if (wide) {
 #pragma unroll
           for (int w = 0; w < 8; ++w) {
-            const uint32_t word = word_of(chunk, lane, w, true);
+            const uint32_t word = word_of<128>(chunk, lane, w);
             if (add) {
               const uint4 r = get_word(word);
-              z[4 * w] += __uint_as_float(r.x);
-              z[4 * w + 1] += __uint_as_float(r.y);
-              z[4 * w + 2] += __uint_as_float(r.z);
-              z[4 * w + 3] += __uint_as_float(r.w);
+              z[2 * w] = add2(z[2 * w], make_float2(__uint_as_float(r.x), __uint_as_float(r.y)));
+              z[2 * w + 1] = add2(z[2 * w + 1],
+                                  make_float2(__uint_as_float(r.z), __uint_as_float(r.w)));
             }
-            put_word(word, __float_as_uint(z[4 * w]), __float_as_uint(z[4 * w + 1]),
-                     __float_as_uint(z[4 * w + 2]), __float_as_uint(z[4 * w + 3]));
+            put_word(word, __float_as_uint(z[2 * w].x), __float_as_uint(z[2 * w].y),
+                     __float_as_uint(z[2 * w + 1].x), __float_as_uint(z[2 * w + 1].y));
           }
         } else {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t word = word_of(chunk, lane, w, false);
+            const uint32_t word = word_of<kNarrowBytes>(chunk, lane, 4 * part + w);
             if (add) {
               const uint4 r = get_word(word);
               const T* v = reinterpret_cast<const T*>(&r);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) z[8 * w + k] += to_float(v[k]);
+              for (int k = 0; k < 4; ++k)
+                z[4 * w + k] = add2(z[4 * w + k],
+                                    make_float2(to_float(v[2 * k]), to_float(v[2 * k + 1])));
             }
-            put_word(word, pack2<T>(z[8 * w], z[8 * w + 1]), pack2<T>(z[8 * w + 2], z[8 * w + 3]),
-                     pack2<T>(z[8 * w + 4], z[8 * w + 5]), pack2<T>(z[8 * w + 6], z[8 * w + 7]));
+            put_word(word, pack2<T>(z[4 * w].x, z[4 * w].y),
+                     pack2<T>(z[4 * w + 1].x, z[4 * w + 1].y),
+                     pack2<T>(z[4 * w + 2].x, z[4 * w + 2].y),
+                     pack2<T>(z[4 * w + 3].x, z[4 * w + 3].y));
           }
         }
-        const uint32_t slope_chunk = chunk + (wide ? kChunkBytes : kChunkBytes / 2);
         if (e.slope && e.slope_float) {
+          if (!wide && part > 0) {  // the slopes of the chunk's part before
+            if (lane == 0) wait_stores_read<0>();
+            __syncwarp();
+          }
 #pragma unroll
           for (int w = 0; w < 8; ++w)
-            put_word(word_of(slope_chunk, lane, w, true), __float_as_uint(slope[4 * w]),
-                     __float_as_uint(slope[4 * w + 1]), __float_as_uint(slope[4 * w + 2]),
-                     __float_as_uint(slope[4 * w + 3]));
+            put_word(word_of<128>(slope_chunk, lane, w), __float_as_uint(slope[2 * w].x),
+                     __float_as_uint(slope[2 * w].y), __float_as_uint(slope[2 * w + 1].x),
+                     __float_as_uint(slope[2 * w + 1].y));
         } else if (e.slope) {
-          uint32_t code[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) code[i] = slope_codes(slope[2 * i], slope[2 * i + 1]);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            put_word(word_of(slope_chunk, lane, w, false), code[4 * w], code[4 * w + 1],
-                     code[4 * w + 2], code[4 * w + 3]);
+            put_word(word_of<kNarrowBytes>(slope_chunk, lane, 4 * part + w),
+                     slope_codes(slope[4 * w]), slope_codes(slope[4 * w + 1]),
+                     slope_codes(slope[4 * w + 2]), slope_codes(slope[4 * w + 3]));
         }
+        const bool ends = part == kParts - 1 || n + 32 >= e.columns;  // a 16-bit chunk
         fence_async_shared();
         __syncwarp();
         if (lane == 0) {
           if (row < e.rows) {
-            store_box(&maps.out, n, static_cast<int>(out_row), chunk);
-            if (e.slope) store_box(&maps.slope, n, row, slope_chunk);
+            if (wide) store_box(&maps.out, n, static_cast<int>(out_row), chunk);
+            else if (ends) store_box(&maps.out, n - 32 * part, static_cast<int>(out_row), chunk);
+            if (e.slope && e.slope_float) store_box(&maps.slope, n, row, slope_chunk);
+            else if (e.slope && ends) store_box(&maps.slope, n - 32 * part, row, slope_chunk);
           }
           commit_stores();
-          if (add && !two) {
+          if (add && !two && (wide || ends)) {
             wait_stores_read<0>();
-            load_residual(from({p.item, p.c + 2}), use + 1);
+            load_residual(chunk_after({item, c - (wide ? 0 : part)}), use + 1);
           }
         }
-        ++use;
+        if (wide || ends) ++use;
       } else {
         float* const square = reinterpret_cast<float*>(s.out[warp]);
-        const auto store = [&](const float(&x)[32], auto&& put) {
+        const auto store = [&](const float2(&x)[16], auto&& put) {
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) square[32 * lane + (i ^ lane)] = x[i];
+          for (int i = 0; i < 16; ++i) {
+            square[32 * lane + (2 * i ^ lane)] = x[i].x;
+            square[32 * lane + ((2 * i + 1) ^ lane)] = x[i].y;
+          }
           __syncwarp();
           if (n + lane < e.columns)
             for (int r = 0; r < 32 && row + r < e.rows; ++r) put(r, square[32 * r + (lane ^ r)]);
@@ -334,7 +377,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
           store(slope, [&](int r, float x) {
             const int64_t to = (row + r) * e.slope_stride + n + lane;
             if (e.slope_float) static_cast<float*>(e.slope)[to] = x;
-            else static_cast<uint16_t*>(e.slope)[to] = static_cast<uint16_t>(slope_codes(x, x));
+            else static_cast<uint16_t*>(e.slope)[to] = static_cast<uint16_t>(slope_codes(both(x)));
           });
       }
     }
@@ -476,12 +519,13 @@ int32_t encode_operand(CUtensorMap* map, int32_t dtype, const Operand& o, int bo
 
 // A [rows, columns] array in the epilogue's chunks.
 int32_t encode_chunks(CUtensorMap* map, int32_t dtype, const void* data, int64_t rows,
-                      int64_t columns, int64_t row_stride) {
+                      int64_t columns, int64_t row_stride, int narrow_columns) {
   const cuuint64_t size[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
   const cuuint64_t stride[1] = {static_cast<cuuint64_t>(row_stride) * element_size(dtype)};
-  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t box_columns = dtype == GS_FLOAT32 ? 32 : narrow_columns, box[2] = {box_columns, 32};
   return encode(map, dtype, data, 2, size, stride, box,
-                dtype == GS_FLOAT32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                box_columns * element_size(dtype) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                                         : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 bool tma_rows(const void* data, int64_t stride, int32_t dtype, int64_t columns) {
@@ -497,13 +541,14 @@ int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const 
   EpilogueMaps maps;
   if (e.tiled) {
     const int64_t out_rows = plan.splits > 1 ? plan.splits * plan.split_rows : e.rows;
-    GS_TRY(encode_chunks(&maps.out, e.out_dtype, e.out, out_rows, e.columns, e.out_stride));
+    constexpr int kWide = ProductShared<kN>::kWide;
+    GS_TRY(encode_chunks(&maps.out, e.out_dtype, e.out, out_rows, e.columns, e.out_stride, kWide));
     if (e.residual)
       GS_TRY(encode_chunks(&maps.residual, e.out_dtype, e.residual, e.rows, e.columns,
-                           e.residual_stride));
+                           e.residual_stride, kWide));
     if (e.slope)  // bfloat16 stands for any 16 bits
       GS_TRY(encode_chunks(&maps.slope, e.slope_float ? GS_FLOAT32 : GS_BFLOAT16, e.slope, e.rows,
-                           e.columns, e.slope_stride));
+                           e.columns, e.slope_stride, kWide));
   }
   constexpr size_t kShared = sizeof(ProductShared<kN>);
   GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB>>(kShared)));
@@ -527,14 +572,17 @@ Plan plan_of(int64_t rows, int64_t columns, int64_t depth, int n, int splits) {
   return p;
 }
 
-// The tile's columns: the widest of which there are enough tiles for every
-// multiprocessor, or the narrowest.
-int columns_of(int64_t rows, int64_t columns, int splits, int least) {
-  int n = 256;
-  while (n > least && (n / 2 >= columns || int64_t{ceil_div(rows, kRows)} * ceil_div(columns, n) *
-                                                   splits < kSmCount))
-    n /= 2;
-  return n;
+// The tile's columns: those with which the multiprocessors' last turn ends first. A turn
+// takes a tile's columns and about 32 more for its start and end.
+int columns_of(int64_t rows, int64_t columns, int least) {
+  int best = 0;
+  int64_t best_time = 0;
+  for (int n = 256; n >= least; n /= 2) {
+    const int64_t tiles = int64_t{ceil_div(rows, kRows)} * ceil_div(columns, n);
+    const int64_t time = (tiles + kSmCount - 1) / kSmCount * (n + 32);
+    if (!best || time < best_time) best = n, best_time = time;
+  }
+  return best;
 }
 
 // D = A B^T by `e`, with tiles of n columns.
@@ -598,29 +646,40 @@ __global__ void __launch_bounds__(kSlopeThreads)
   float sum[8] = {};
   if (valid > 0) {
     const G* const grad = static_cast<const G*>(a.grad_y);
-#pragma unroll 4
-    for (int64_t m = row0 + first; m < end; m += step) {
-      float g[8];
-      load_row(grad + m * a.outputs + column, valid, aligned, g);
-      if (a.slope && slope_float) {
-        const float* p = static_cast<const float*>(a.slope) + m * stride + column;
-        float x[8];
-        load_row(p, 8, true, x);
+    // Several rows' loads before the first one's arithmetic.
+    constexpr int kBatch = 4;
+    for (int64_t m0 = row0 + first; m0 < end; m0 += kBatch * step) {
+      float g[kBatch][8];
+      uint4 codes[kBatch];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] = k < valid ? g[k] * x[k] : 0.0f;
-      } else if (a.slope) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.slope) +
-                                                        m * stride + column);
-        const uint32_t codes[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float x = slope_value(k & 1 ? codes[k >> 1] >> 16 : codes[k >> 1] & 0xffffu);
-          g[k] = k < valid ? g[k] * x : 0.0f;
-        }
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t m = min(m0 + i * step, a.rows - 1);
+        load_row(grad + m * a.outputs + column, valid, aligned, g[i]);
+        if (a.slope && !slope_float)
+          codes[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.slope) +
+                                                          m * stride + column));
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += g[k];
-      if (dz) store_pack<8>(dz + m * stride + column, g);
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t m = m0 + i * step;
+        if (m >= end) break;
+        if (a.slope && slope_float) {
+          float x[8];
+          load_row(static_cast<const float*>(a.slope) + m * stride + column, 8, true, x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) g[i][k] = k < valid ? g[i][k] * x[k] : 0.0f;
+        } else if (a.slope) {
+          const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float x = slope_value(k & 1 ? words[k >> 1] >> 16 : words[k >> 1] & 0xffffu);
+            g[i][k] = k < valid ? g[i][k] * x : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += g[i][k];
+        if (dz) store_pack<8>(dz + m * stride + column, g[i]);
+      }
     }
   }
   if (!sums) return;
@@ -735,12 +794,13 @@ BackwardPlan backward_plan(const gs_linear_args& a) {
   p.strips = strips_of(a.rows, a.outputs);
   // The weight's gradient has few tiles and a long contraction: split so that the items
   // are about one a multiprocessor.
-  p.columns = columns_of(a.outputs, a.inputs, 1 << 20, 64);
+  p.columns = 256;
+  while (p.columns > 64 && p.columns / 2 >= a.inputs) p.columns /= 2;
   const int64_t tiles = int64_t{ceil_div(a.outputs, kRows)} * ceil_div(a.inputs, p.columns);
   const int64_t splits = kSmCount / tiles;
   p.weight = plan_of(a.outputs, a.inputs, a.rows, p.columns,
                      static_cast<int>(splits < 1 ? 1 : splits));
-  p.x_columns = columns_of(a.rows, a.inputs, 1, 64);
+  p.x_columns = columns_of(a.rows, a.inputs, 64);
   p.x = plan_of(a.rows, a.inputs, a.outputs, p.x_columns, 1);
   uint64_t at = 0;
   const auto take = [&](uint64_t bytes) {
@@ -785,7 +845,7 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   e.tiled = tma_rows(a.y, a.outputs, a.residual_dtype, a.outputs) &&
             (!a.residual ||
              tma_rows(a.residual, a.residual_stride, a.residual_dtype, a.outputs));
-  const int n = columns_of(a.rows, a.outputs, 1, 32);
+  const int n = columns_of(a.rows, a.outputs, 32);
   return with_sixteen_bit(a.dtype, [&](auto t) {
     return run_product<decltype(t), false, false>(
         a.dtype, {a.x, a.rows, a.inputs, a.x_stride},
