@@ -4,18 +4,27 @@
 //   score_t = scale q . k_t = scale (step_t (q . c_t) + (middle_t - 7.5 step_t) sum q)
 //   out = sum p_t v_t = sum (p_t step_t) (c_t - 7.5) + sum p_t middle_t
 //
-// so that codes go to the products as they are, small whole numbers of the 16-bit
-// type, and the ranges stay outside: a key's in two numbers a score, a value's in
-// its weight p_t step_t (rounded to the type, as a weight has to be for a product)
-// and in one float sum a head, which no rounding meets.
+// so that codes go to the products as they are, small whole numbers in float16, which
+// are exact, and the ranges stay outside: a key's in two numbers a score, a value's in
+// its weight p_t step_t and in one float sum a head, which no rounding meets. q and the
+// weights are scaled by powers of two into float16's range, whatever the tokens' type:
+// of a head's q nothing is lost within 2^-25 of its largest channel, and the weights
+// are rounded once, to 11 bits.
 //
-// The cache is read once; the codes of a row are half a byte a channel, so that
-// taking them apart (8 to 12 instructions a word of 8) weighs about as much as the
-// reading. A cluster of blocks shares the slots of a stream and key-value head, up
-// to 16 query heads (more: more clusters). A warp takes 32 slots at a time from a
-// ring in shared memory of its own, filled some turns ahead by cp.async, so that warps
-// never wait for one another; sums are joined at the end in order, in the block and
-// across the cluster: one launch, no workspace, no atomics.
+// The cache is read once; taking a word of eight codes apart costs 9 to 10 instructions
+// though, which together weigh about as much as the reading. A cluster of blocks shares
+// the slots of a stream and key-value head, up to 16 query heads (more: more clusters). A
+// warp takes 32 slots at a time from a ring in shared memory of its own, filled some
+// turns ahead by cp.async, so that warps never wait for one another:
+//
+//   scores [slots x heads] = K q^T: a lane's words of two key rows are its parts of
+//     the products, with q's channels permuted alike;
+//   out [dim x heads] += V^T P^T: a lane's words of two value rows, interleaved, are
+//     its parts of four products; P turns around in registers (movmatrix).
+//
+// So slots and channels fill the products' 16 rows, and 8 heads their columns. Sums are
+// joined at the end in order, in the block and across the cluster: one launch, no
+// workspace, no atomics.
 #include "step.cuh"
 
 namespace gs {
@@ -26,12 +35,8 @@ constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kSlots = 32;  // of a warp's turn
 constexpr float kLog2e = 1.44269504f;
 // As in attention.cu: growth (log2) of the scores' maximum that passes without
-// rescaling, and float16 weights' place above it.
-constexpr float kSlack = 8.0f;
-template <class T>
-constexpr bool kHalf = std::is_same_v<T, __half>;
-template <class T>
-constexpr float kLift = kHalf<T> ? 7.0f : 0.0f;
+// rescaling, and the weights' place above it in float16.
+constexpr float kSlack = 8.0f, kLift = 7.0f;
 
 template <int kDim>
 struct Stage {
@@ -41,19 +46,20 @@ struct Stage {
   uint32_t range[2][kSlots];  // step in the low half, middle in the high one
 };
 
-// What a slot's ranges come to: score = dot * key_step + (sum of q) * key_base.
+// What a slot's ranges come to: score = dot * key_step + (sum of q) * key_base, where
+// dot has c - 8.
 struct Slot {
   float key_step, key_base, value_step, value_middle;
 };
 
-template <int kDim, int kHalves>
+template <int kDim, int kSets>
 struct Shared {
   union {
     Stage<kDim> stage[kWarps][Stage<kDim>::kCount];
-    float out[kWarps][8 * kHalves][kDim];  // once the stages are done
+    float out[kWarps][8 * kSets][kDim];  // once the stages are done
   };
   alignas(16) Slot slot[kWarps][kSlots];
-  float top[kWarps][8 * kHalves], sum[kWarps][8 * kHalves];
+  float top[kWarps][8 * kSets], sum[kWarps][8 * kSets];
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -115,23 +121,12 @@ __device__ __forceinline__ float2 unpack2(uint32_t word) {
   return make_float2(to_float(v[0]), to_float(v[1]));
 }
 
-// Codes at bits 0 to 3 of both halves of `word`, or at bits 4 to 7 (float16 only:
-// bfloat16 has 7 bits behind the leading one), as numbers: next to a large power of
-// two, whose low bits they are, and that taken off again. Exact.
-template <class T>
-__device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b) {
+// c - 8 in float16 of the codes at bits 0 to 3 (low), or 4 to 7, of both halves of a
+// word: next to 1024, whose low bits they are, and that taken off again. Exact.
+__device__ __forceinline__ uint32_t centred_low(uint32_t word) {  // (1024 + c) - 1032
   uint32_t y;
-  if constexpr (kHalf<T>) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  else asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"((word & 0x000f000fu) | 0x64006400u), "r"(0xe408e408u));
   return y;
-}
-template <class T>
-__device__ __forceinline__ uint32_t above(uint32_t word) {  // 1024 + c, or 128 + c
-  return (word & 0x000f000fu) | (kHalf<T> ? 0x64006400u : 0x43004300u);
-}
-template <class T>
-__device__ __forceinline__ uint32_t centred(uint32_t word) {  // c - 8
-  return add_pair<T>(above<T>(word), kHalf<T> ? 0xe408e408u : 0xc308c308u);
 }
 __device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16 c) / 16 - 72
   uint32_t y;
@@ -141,32 +136,27 @@ __device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16
   return y;
 }
 // Codes 0 to 3 of both halves of a word as four pairs.
-template <class T>
 __device__ __forceinline__ void spread(uint32_t word, uint32_t (&pair)[4]) {
-  if constexpr (kHalf<T>) {
-    const uint32_t next = word >> 8;
-    pair[0] = centred<T>(word);
-    pair[1] = centred_high(word);
-    pair[2] = centred<T>(next);
-    pair[3] = centred_high(next);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) pair[e] = centred<T>(word >> 4 * e);
-  }
+  const uint32_t next = word >> 8;
+  pair[0] = centred_low(word);
+  pair[1] = centred_high(word);
+  pair[2] = centred_low(next);
+  pair[3] = centred_high(next);
 }
-// The same for a key's: bfloat16 leaves the 128 in, which is taken off the score (its
-// error there, 2^-23 of 136 sum |q| step, is far below what q's bits allow; float16's
-// 1024 would not be).
-template <class T>
-constexpr float kKeyOffset = kHalf<T> ? 8.0f : 0.0f;  // what a key's numbers lack
-template <class T>
-__device__ __forceinline__ void spread_key(uint32_t word, uint32_t (&pair)[4]) {
-  if constexpr (kHalf<T>) {
-    spread<T>(word, pair);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) pair[e] = above<T>(word >> 4 * e);
-  }
+
+// c += a b, 16 x 16 by 16 x 8.
+__device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of pairs, a row in four lanes, turned around.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 template <int kWords>
@@ -187,15 +177,16 @@ __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)
   }
 }
 
-// kMasked: with validity of the slots. kAligned: rows of codes are whole 16-byte words.
-template <class T, int kDim, int kHalves, bool kMasked, bool kAligned>
-__global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : kHalves == 1 ? 3 : 2)
+// kSets: of 8 heads. kMasked: with validity of the slots. kAligned: rows of codes are
+// whole 16-byte words.
+template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
+__global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
     step_kernel(gs_window_attention_step_4bit_args a) {
-  using S = Shared<kDim, kHalves>;
+  using S = Shared<kDim, kSets>;
   constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
   constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
   constexpr int kValueWords = kDim / 64;  // of a value's, of eight
-  constexpr int kHeads = 8 * kHalves;
+  constexpr int kHeads = 8 * kSets;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   S& s = *reinterpret_cast<S*>(shared_bytes);
   chain_wait();
@@ -235,20 +226,20 @@ __global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : kHalves == 1 ? 3 : 
       const int last = count - 1 - base;  // slots behind it are that one again
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
+        const uint8_t* const from = codes[side] + int64_t{base} * row_bytes;
         if constexpr (kAligned) {
-          const int pieces16 = row_bytes >> 4;  // of a row: 1 to 4
+          // Four lanes (64 channels: two) have a row's 16-byte words.
+          constexpr int kLanes = kDim / 32;
+          const int word = 16 * (lane % kLanes);
+          if (word < row_bytes)
 #pragma unroll
-          for (int r = 0; r < kDim / 32; ++r) {
-            const int i = lane + 32 * r;
-            const int row = i / (kDim / 32), piece16 = i % (kDim / 32);
-            if (piece16 >= pieces16) continue;
-            cp_async16(st.codes[side] + row * kRow + 16 * piece16,
-                       codes[side] + int64_t{base + min(row, last)} * row_bytes + 16 * piece16);
-          }
+            for (int r = 0; r < kLanes; ++r) {
+              const int row = lane / kLanes + 32 / kLanes * r;
+              cp_async16(st.codes[side] + row * kRow + word, from + min(row, last) * row_bytes + word);
+            }
         } else {
-          const uint8_t* from = codes[side] + int64_t{base + min(lane, last)} * row_bytes;
           for (int w = 0; w < row_bytes; w += 4)
-            cp_async4(st.codes[side] + lane * kRow + w, from + w);
+            cp_async4(st.codes[side] + lane * kRow + w, from + min(lane, last) * row_bytes + w);
         }
         cp_async4(&st.range[side][lane], range[side] + base + min(lane, last));
       }
@@ -283,44 +274,62 @@ __global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : kHalves == 1 ? 3 : 
     }
   }
 
-  // q's rows g (and g + 8), channels in the order of the keys' products: a word's are
-  // pairs (0, 4), (1, 5) of one product and (2, 6), (3, 7) of the next. And q's sums.
-  uint32_t q[kKeyWords][2][kHalves][2];
-  float q_sum[kHalves];
+  // Head g's q (and head g + 8's), channels in the order of the keys' products: a word's
+  // are pairs (0, 4), (1, 5) of one product and (2, 6), (3, 7) of the next. A head's largest
+  // channel goes to 2^10.
+  uint32_t q[kSets][kKeyWords][4];
+  // Of the lane's columns, heads 2j and 2j + 1: what takes their dots and sums of q to
+  // scores in base 2.
+  float dot_scale[kSets][2], base_scale[kSets][2];
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
-    q_sum[r] = 0.0f;
+  for (int r = 0; r < kSets; ++r) {
+    float x[kKeyWords][8], total = 0.0f, largest = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKeyWords; ++w) {
       const int channel = 8 * (kKeyWords * j + w);
-      uint4 word = make_uint4(0, 0, 0, 0);
-      if (g + 8 * r < heads && channel < a.dim)
-        word = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride +
-                                               (head0 + g + 8 * r) * a.q_head_stride + channel);
-      q[w][0][r][0] = __byte_perm(word.x, word.z, 0x5410);
-      q[w][0][r][1] = __byte_perm(word.x, word.z, 0x7632);
-      q[w][1][r][0] = __byte_perm(word.y, word.w, 0x5410);
-      q[w][1][r][1] = __byte_perm(word.y, word.w, 0x7632);
-      const float2 x01 = unpack2<T>(word.x), x23 = unpack2<T>(word.y);
-      const float2 x45 = unpack2<T>(word.z), x67 = unpack2<T>(word.w);
-      q_sum[r] += ((x01.x + x01.y) + (x23.x + x23.y)) + ((x45.x + x45.y) + (x67.x + x67.y));
-    }
-    q_sum[r] += __shfl_xor_sync(0xffffffffu, q_sum[r], 1);
-    q_sum[r] += __shfl_xor_sync(0xffffffffu, q_sum[r], 2);
-  }
-  const float scale = a.scale * kLog2e;
-  float out[kValueWords][8][kHalves][2] = {};
-  float top[kHalves], sum[kHalves] = {}, middle_sum[kHalves] = {};
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) top[r] = -INFINITY;
-  // float16: value steps are taken relative to a power of two above the largest so far,
-  // so that weights times steps stay in float16's range whatever the values' size.
+      for (int k = 0; k < 8; ++k) x[w][k] = 0.0f;
+      if (g + 8 * r < heads && channel < a.dim)
+        load_pack<8>(static_cast<const T*>(a.q) + b * a.q_stride +
+                         (head0 + g + 8 * r) * a.q_head_stride + channel,
+                     x[w]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        total += x[w][k];
+        largest = max_nan(largest, fabsf(x[w][k]));
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    }
+    const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, 11u << 23);
+    const float up = __uint_as_float((264u << 23) - exponent);
+    const float down = __uint_as_float((254u << 23) - __float_as_uint(up));
+#pragma unroll
+    for (int w = 0; w < kKeyWords; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        q[r][w][e] = tc::pack2<__half>(x[w][e] * up, x[w][e + 4] * up);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int from = 4 * (2 * j + e);
+      dot_scale[r][e] = __shfl_sync(0xffffffffu, down, from) * (a.scale * kLog2e);
+      base_scale[r][e] = __shfl_sync(0xffffffffu, total, from) * (a.scale * kLog2e);
+    }
+  }
+  float out[kSets][kValueWords][4][4] = {};
+  float top[kSets][2], sum[kSets][2] = {}, middle_sum[kSets][2] = {};
+#pragma unroll
+  for (int r = 0; r < kSets; ++r) top[r][0] = top[r][1] = -INFINITY;
+  // Value steps are taken relative to a power of two above the largest so far.
   uint32_t unit = 0;  // its bits
   float per_unit = 1.0f;
 
-  // Slots in the order of the products' columns: column n of the first is slot n / 2 + 4
-  // (n % 2), so that a lane's four slots as rows of P V, and its neighbours', lie next to
-  // one another: j, 4 + j, 8 + j, 12 + j.
+  // Slots in the order of the products' rows: row n of 8 is slot n / 2 + 4 (n % 2), so that
+  // a lane's four slots of V, j, 4 + j, 8 + j and 12 + j, and its neighbours', lie next to one
+  // another.
   const int key_row = (g >> 1) + 4 * (g & 1);
   for (int t = 0; t < turns; ++t) {
     load(t + kStages - 1);
@@ -342,137 +351,153 @@ __global__ void __launch_bounds__(kThreads, kDim == 64 ? 4 : kHalves == 1 ? 3 : 
     {
       const float2 key = unpack2<T>(seen ? st.range[0][lane] : 0);
       const float2 value = unpack2<T>(seen ? st.range[1][lane] : 0);
-      float step = value.x;
-      if constexpr (kHalf<T>) {
-        const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(step) & 0x7fffffffu);
-        if (largest >= unit) {  // the same for the whole warp
-          const uint32_t next = min(largest & 0x7f800000u, 0x7e000000u) + 0x00800000u;
-          const float shrink = unit ? __uint_as_float(unit) / __uint_as_float(next) : 0.0f;
+      const uint32_t largest =
+          __reduce_max_sync(0xffffffffu, __float_as_uint(value.x) & 0x7fffffffu);
+      if (largest >= unit) {  // the same for the whole warp
+        const uint32_t next = min(largest & 0x7f800000u, 0x7e000000u) + 0x00800000u;
+        const float shrink = unit ? __uint_as_float(unit) / __uint_as_float(next) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < kSets; ++r)
 #pragma unroll
           for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int r = 0; r < kHalves; ++r) {
-                out[h][i][r][0] *= shrink;
-                out[h][i][r][1] *= shrink;
-              }
-          unit = next;
-          per_unit = __uint_as_float(0x7f000000u - next);
-        }
-        step *= per_unit;
+              for (int c = 0; c < 4; ++c) out[r][h][i][c] *= shrink;
+        unit = next;
+        per_unit = __uint_as_float(0x7f000000u - next);
       }
-      s.slot[warp][lane] = {key.x * scale,
-                            fmaf(key.x, kKeyOffset<T> - (kHalf<T> ? 7.5f : 135.5f), key.y) * scale,
-                            step, fmaf(0.5f, value.x, value.y)};
+      s.slot[warp][lane] = {key.x, fmaf(0.5f, key.x, key.y), value.x * per_unit,
+                            fmaf(0.5f, value.x, value.y)};
     }
     __syncwarp();
-#pragma unroll 1
+    Slot of[4];  // the lane's slots as rows of the scores: key_row, + 8, + 16, + 24
+#pragma unroll
+    for (int i = 0; i < 4; ++i) of[i] = s.slot[warp][key_row + 8 * i];
+    float x[kSets][2][4] = {};
+#pragma unroll
     for (int half = 0; half < 2; ++half) {  // 16 slots
-      Slot of[4];
+      uint32_t low[kKeyWords], high[kKeyWords];
+      read_words<kKeyWords>(st.codes[0] + (16 * half + key_row) * kRow + 4 * kKeyWords * j, low);
+      read_words<kKeyWords>(st.codes[0] + (16 * half + 8 + key_row) * kRow + 4 * kKeyWords * j, high);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) of[i] = s.slot[warp][16 * half + 4 * i + j];
-      float x[2][kHalves][2] = {};  // scores of the slots of[2n], of[2n + 1]
+      for (int w = 0; w < kKeyWords; ++w) {
+        uint32_t p0[4], p8[4];
+        spread(low[w], p0);
+        spread(high[w], p8);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        uint32_t word[kKeyWords];
-        read_words<kKeyWords>(
-            st.codes[0] + (16 * half + 8 * n + key_row) * kRow + 4 * kKeyWords * j, word);
-#pragma unroll
-        for (int w = 0; w < kKeyWords; ++w) {
-          uint32_t pair[4];
-          spread_key<T>(word[w], pair);
-          warp_product<T, kHalves>(x[n], q[w][0], pair[0], pair[1]);
-          warp_product<T, kHalves>(x[n], q[w][1], pair[2], pair[3]);
+        for (int r = 0; r < kSets; ++r) {
+          multiply(x[r][half], p0[0], p8[0], p0[1], p8[1], q[r][w][0], q[r][w][1]);
+          multiply(x[r][half], p0[2], p8[2], p0[3], p8[3], q[r][w][2], q[r][w][3]);
         }
       }
-      uint32_t p[kHalves][2];
-      const uint32_t mine = visible >> (16 * half + j);  // bits 0, 4, 8, 12
+    }
+    uint32_t weight[kSets][4];  // of the slots of[i], both heads, then turned around
 #pragma unroll
-      for (int r = 0; r < kHalves; ++r) {
-        float next = -INFINITY;
+    for (int r = 0; r < kSets; ++r) {
+      float score[4][2], next[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = 2 * n + e;
-            x[n][r][e] = fmaf(x[n][r][e], of[i].key_step, q_sum[r] * of[i].key_base);
-            if (!(mine >> 4 * i & 1)) x[n][r][e] = -INFINITY;
-            next = fmaxf(next, x[n][r][e]);
+        for (int e = 0; e < 2; ++e)
+          score[i][e] = fmaf(x[r][i >> 1][2 * (i & 1) + e] * dot_scale[r][e], of[i].key_step,
+                             base_scale[r][e] * of[i].key_base);
+      if (visible != 0xffffffffu)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(visible >> (key_row + 8 * i) & 1)) score[i][0] = score[i][1] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) next[e] = fmaxf(next[e], score[i][e]);
+      if (__any_sync(0xffffffffu, next[0] > top[r][0] + kSlack || next[1] > top[r][1] + kSlack)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1)
+            next[e] = fmaxf(next[e], __shfl_xor_sync(0xffffffffu, next[e], o));
+          if (next[e] > top[r][e] + kSlack) {
+            const float shrink = tc::exp2_approx(top[r][e] - next[e]);
+            top[r][e] = next[e];
+            sum[r][e] *= shrink;
+            middle_sum[r][e] *= shrink;
+#pragma unroll
+            for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                out[r][h][i][e] *= shrink;
+                out[r][h][i][2 + e] *= shrink;
+              }
           }
-        next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 1));
-        next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 2));
-        const bool grow = next > top[r] + kSlack || (top[r] == -INFINITY && next > top[r]);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float shrink = grow ? tc::exp2_approx(top[r] - next) : 1.0f;
-          if (grow) top[r] = next;
-          sum[r] *= shrink;
-          middle_sum[r] *= shrink;
-#pragma unroll
-          for (int h = 0; h < kValueWords; ++h)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              out[h][i][r][0] *= shrink;
-              out[h][i][r][1] *= shrink;
-            }
-        }
-        const float shift = top[r] == -INFINITY ? 0.0f : kLift<T> - top[r];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = tc::exp2_approx(x[n][r][0] + shift);
-          const float p1 = tc::exp2_approx(x[n][r][1] + shift);
-          sum[r] += p0 + p1;
-          middle_sum[r] = fmaf(p0, of[2 * n].value_middle,
-                               fmaf(p1, of[2 * n + 1].value_middle, middle_sum[r]));
-          p[r][n] = tc::pack2<T>(p0 * of[2 * n].value_step, p1 * of[2 * n + 1].value_step);
         }
       }
+      float shift[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) shift[e] = top[r][e] == -INFINITY ? 0.0f : kLift - top[r][e];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[e] = tc::exp2_approx(score[i][e] + shift[e]);
+          sum[r][e] += p[e];
+          middle_sum[r][e] = fmaf(p[e], of[i].value_middle, middle_sum[r][e]);
+        }
+        weight[r][i] = transposed(
+            tc::pack2<__half>(p[0] * of[i].value_step, p[1] * of[i].value_step));
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
       uint32_t word[4][kValueWords];  // of the slots j, 4 + j, 8 + j, 12 + j
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         read_words<kValueWords>(
             st.codes[1] + (16 * half + 4 * i + j) * kRow + 4 * kValueWords * g, word[i]);
 #pragma unroll
-      for (int h = 0; h < kValueWords; ++h)
+      for (int h = 0; h < kValueWords; ++h) {
+        uint32_t a0[4], a1[4], a2[4], a3[4];  // channels 0 to 3 and 4 to 7, two slots each
+        spread(__byte_perm(word[0][h], word[1][h], 0x5410), a0);
+        spread(__byte_perm(word[0][h], word[1][h], 0x7632), a1);
+        spread(__byte_perm(word[2][h], word[3][h], 0x5410), a2);
+        spread(__byte_perm(word[2][h], word[3][h], 0x7632), a3);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // a word's low and high half
-          uint32_t first[4], second[4];
-          const uint32_t order = c ? 0x7632 : 0x5410;
-          spread<T>(__byte_perm(word[0][h], word[1][h], order), first);
-          spread<T>(__byte_perm(word[2][h], word[3][h], order), second);
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            warp_product<T, kHalves>(out[h][4 * c + e], p, first[e], second[e]);
-        }
+          for (int r = 0; r < kSets; ++r)
+            multiply(out[r][h][e], a0[e], a1[e], a2[e], a3[e], weight[r][2 * half],
+                     weight[r][2 * half + 1]);
+      }
     }
     __syncwarp();  // all lanes are done with the stage that the next turn fills
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // the stages' place is free for the outputs
 
-  // The warp's rows to shared memory: product (h, i)'s column n is channel 8 (kValueWords n
-  // + h) + i.
-  const float unit_size = kHalf<T> ? __uint_as_float(unit) : 1.0f;
+  // The warp's columns to shared memory: row g of product (h, e) is channel 8 (kValueWords g
+  // + h) + e, row g + 8 channel e + 4.
+  const float unit_size = __uint_as_float(unit);
 #pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
+  for (int r = 0; r < kSets; ++r)
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
-      middle_sum[r] += __shfl_xor_sync(0xffffffffu, middle_sum[r], o);
-    }
-    if (j == 0) {
-      s.top[warp][g + 8 * r] = top[r];
-      s.sum[warp][g + 8 * r] = sum[r];
-    }
+    for (int e = 0; e < 2; ++e) {
+      const int head = 8 * r + 2 * j + e;
 #pragma unroll
-    for (int h = 0; h < kValueWords; ++h)
+      for (int o = 4; o < 32; o <<= 1) {
+        sum[r][e] += __shfl_xor_sync(0xffffffffu, sum[r][e], o);
+        middle_sum[r][e] += __shfl_xor_sync(0xffffffffu, middle_sum[r][e], o);
+      }
+      if (g == 0) {
+        s.top[warp][head] = top[r][e];
+        s.sum[warp][head] = sum[r][e];
+      }
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          s.out[warp][g + 8 * r][8 * (kValueWords * (2 * j + e) + h) + i] =
-              fmaf(out[h][i][r][e], unit_size, middle_sum[r]);
-  }
+          s.out[warp][head][8 * (kValueWords * g + h) + i] =
+              fmaf(out[r][h][i & 3][2 * (i >> 2) + e], unit_size, middle_sum[r][e]);
+    }
   __syncthreads();
   // The warps joined into the first one's place.
   for (int c = threadIdx.x; c < heads * kDim; c += kThreads) {
@@ -526,13 +551,13 @@ int step_blocks(const gs_window_attention_step_4bit_args& a, int64_t items) {
   return blocks;
 }
 
-template <class T, int kDim, int kHalves, bool kMasked, bool kAligned>
+template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
-  const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kHalves);
+  const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kSets);
   const int blocks = step_blocks(a, items);
   if (items * blocks > INT32_MAX) return GS_ERR_CAPACITY;
-  constexpr size_t kShared = sizeof(Shared<kDim, kHalves>);
-  GS_TRY((allow_shared<step_kernel<T, kDim, kHalves, kMasked, kAligned>>(kShared, true)));
+  constexpr size_t kShared = sizeof(Shared<kDim, kSets>);
+  GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared, true)));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -546,7 +571,7 @@ int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, step_kernel<T, kDim, kHalves, kMasked, kAligned>, a);
+  cudaLaunchKernelEx(&config, step_kernel<T, kDim, kSets, kMasked, kAligned>, a);
   return check_launch();
 }
 
