@@ -344,6 +344,9 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
                       scale=_scale(what, scale, dim), positions=positions.data_ptr(),
                       out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid),
                       **{name: t.data_ptr() for name, t in cache._asdict().items()})
+    size = native.lib().gs_window_attention_step_4bit_workspace_size(ctypes.byref(args))
+    workspace = q.new_empty((size,), dtype=torch.uint8)
+    args.workspace, args.workspace_size = workspace.data_ptr(), size
     call("gs_window_attention_step_4bit", device, ctypes.byref(args))
     changed_in_place(*cache, cache_valid)
     return out

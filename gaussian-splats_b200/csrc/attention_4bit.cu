@@ -12,26 +12,33 @@
 // are rounded once, to 11 bits.
 //
 // The cache is read once; taking a word of eight codes apart costs 9 to 10 instructions
-// though, which together weigh about as much as the reading. A cluster of blocks shares
-// the slots of a stream and key-value head, up to 16 query heads (more: more clusters). A
-// warp takes 32 slots at a time from a ring in shared memory of its own, filled some
-// turns ahead by cp.async, so that warps never wait for one another:
+// though, which together weigh about as much as the reading. So the work is cut evenly:
+// the turns of 32 slots of all streams and key-value heads (up to 16 query heads; more:
+// several times) in one line, of which every warp has the same share, wherever that
+// begins and ends. A warp keeps a ring in shared memory filled some turns ahead, waits for
+// no other, and leaves the sums of its part of each stream's head in a workspace, which
+// a second kernel joins in order.
 //
 //   scores [slots x heads] = K q^T: a lane's words of two key rows are its parts of
 //     the products, with q's channels permuted alike;
 //   out [dim x heads] += V^T P^T: a lane's words of two value rows, interleaved, are
 //     its parts of four products; P turns around in registers (movmatrix).
 //
-// So slots and channels fill the products' 16 rows, and 8 heads their columns. Sums are
-// joined at the end in order, in the block and across the cluster: one launch, no
-// workspace, no atomics.
-#include "step.cuh"
+// So slots and channels fill the products' 16 rows, and 8 heads their columns.
+#include <algorithm>
+
+#include "tensorcore.cuh"
 
 namespace gs {
 namespace {
 
+// Set when a bounded wait ran out (window_attention_4bit_status).
+__device__ uint32_t g_timeout;
+
 constexpr int kMaxDim = 128;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
+// What registers and shared memory allow.
+constexpr int blocks_per_sm(int dim, int sets) { return sets == 1 ? 4 : dim == 64 ? 3 : 2; }
 constexpr int kSlots = 32;  // of a warp's turn
 constexpr float kLog2e = 1.44269504f;
 // As in attention.cu: growth (log2) of the scores' maximum that passes without
@@ -43,24 +50,79 @@ struct Stage {
   static constexpr int kCount = kDim == 128 ? 3 : 5;  // of a warp's ring
   static constexpr int kRow = kDim / 2;  // bytes; shorter rows leave the rest as it is
   alignas(16) unsigned char codes[2][kSlots * kRow];  // keys', values'
-  uint32_t range[2][kSlots];  // step in the low half, middle in the high one
 };
 
 // What a slot's ranges come to: score = dot * key_step + (sum of q) * key_base, where
 // dot has c - 8.
+// Each twice, for instructions on two floats (a lane's two heads).
 struct Slot {
-  float key_step, key_base, value_step, value_middle;
+  float2 key_step, key_base, value_step, value_middle;
 };
 
-template <int kDim, int kSets>
+template <int kDim>
 struct Shared {
-  union {
-    Stage<kDim> stage[kWarps][Stage<kDim>::kCount];
-    float out[kWarps][8 * kSets][kDim];  // once the stages are done
-  };
+  Stage<kDim> stage[kWarps][Stage<kDim>::kCount];
   alignas(16) Slot slot[kWarps][kSlots];
-  float top[kWarps][8 * kSets], sum[kWarps][8 * kSets];
+  uint64_t full[kWarps][Stage<kDim>::kCount];
 };
+
+// What a warp leaves of its part of an item: outputs times the sum, maxima, sums.
+template <int kDim, int kSets>
+struct Part {
+  float out[8 * kSets][kDim];
+  float top[8 * kSets], sum[8 * kSets];
+};
+
+// A stream's slots that count (0: idle), and its turns.
+struct Stream {
+  int64_t position;
+  int count, turns;
+};
+__device__ __forceinline__ Stream stream_at(const gs_window_attention_step_4bit_args& a, int64_t b) {
+  const int64_t position = a.positions[b];
+  const int count = position < 0 ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
+  return {position, count, (count + kSlots - 1) / kSlots};
+}
+
+// The line of turns: stream after stream, each `heads` (key-value heads times pieces of
+// query heads) times its turns. Warp w of `warps` has turns [w total / warps, (w + 1) total
+// / warps) of it, one at least.
+struct Line {
+  int64_t total, warps;
+  int64_t stream, before;  // the stream that has the warp's first turn, the turns before it
+};
+// By a whole warp.
+__device__ Line find_turn(const gs_window_attention_step_4bit_args& a, int heads, int64_t w,
+                          int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  int64_t total = 0;
+  for (int64_t b = lane; b < a.batch; b += 32) total += int64_t{stream_at(a, b).turns} * heads;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  warps = min(warps, total);
+  Line line = {total, warps, 0, 0};
+  if (w >= warps) return line;
+  const int64_t at = w * total / warps;
+  for (int64_t b0 = 0; b0 < a.batch; b0 += 32) {
+    const int64_t mine = b0 + lane < a.batch ? int64_t{stream_at(a, b0 + lane).turns} * heads : 0;
+    int64_t through = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o) through += x;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, line.before + through > at);
+    if (past) {
+      const int first = __ffs(past) - 1;
+      line.stream = b0 + first;
+      line.before += __shfl_sync(0xffffffffu, through - mine, first);
+      return line;
+    }
+    line.before += __shfl_sync(0xffffffffu, through, 31);
+  }
+  line.stream = a.batch;
+  return line;
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -123,16 +185,23 @@ __device__ __forceinline__ float2 unpack2(uint32_t word) {
 
 // c - 8 in float16 of the codes at bits 0 to 3 (low), or 4 to 7, of both halves of a
 // word: next to 1024, whose low bits they are, and that taken off again. Exact.
+__device__ __forceinline__ uint32_t among(uint32_t word, uint32_t bits, uint32_t base) {
+  uint32_t y;  // (word & bits) | base
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(word), "r"(bits), "r"(base));
+  return y;
+}
 __device__ __forceinline__ uint32_t centred_low(uint32_t word) {  // (1024 + c) - 1032
   uint32_t y;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"((word & 0x000f000fu) | 0x64006400u), "r"(0xe408e408u));
+  asm("add.rn.f16x2 %0, %1, %2;"
+      : "=r"(y)
+      : "r"(among(word, 0x000f000fu, 0x64006400u)), "r"(0xe408e408u));
   return y;
 }
 __device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16 c) / 16 - 72
   uint32_t y;
   asm("fma.rn.f16x2 %0, %1, %2, %3;"
       : "=r"(y)
-      : "r"((word & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));
+      : "r"(among(word, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
   return y;
 }
 // Codes 0 to 3 of both halves of a word as four pairs.
@@ -180,9 +249,9 @@ __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)
 // kSets: of 8 heads. kMasked: with validity of the slots. kAligned: rows of codes are
 // whole 16-byte words.
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
-__global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
-    step_kernel(gs_window_attention_step_4bit_args a) {
-  using S = Shared<kDim, kSets>;
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
+    step_kernel(gs_window_attention_step_4bit_args a, Part<kDim, kSets>* parts) {
+  using S = Shared<kDim>;
   constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
   constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
   constexpr int kValueWords = kDim / 64;  // of a value's, of eight
@@ -190,24 +259,46 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   S& s = *reinterpret_cast<S*>(shared_bytes);
   chain_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const uint32_t rank = cluster_rank(), blocks = cluster_size();
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // one for the whole warp
+  const int lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
-  const int64_t item = blockIdx.x / blocks;
-  const int piece = static_cast<int>(item % pieces);
-  const int kv_head = static_cast<int>(item / pieces % a.kv_heads);
-  const int64_t b = item / pieces / a.kv_heads;
+  const int row_bytes = a.dim / 2;
+  const int pitch = kAligned ? row_bytes : kRow;  // of a staged row
+  if constexpr (kAligned) {
+    if (lane == 0) {
+      for (uint64_t& bar : s.full[warp]) tc::barrier_init(tc::shared_address(&bar), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      tc::fence_async_shared();
+    }
+    __syncwarp();
+  }
+  const int64_t me = int64_t{blockIdx.x} * kWarps + warp;
+  const Line line = find_turn(a, a.kv_heads * pieces, me, int64_t{gridDim.x} * kWarps);
+  if (me >= line.warps) return;
+  int64_t at = me * line.total / line.warps, b = line.stream;
+  int64_t before = line.before;  // turns before the stream's
+  const int64_t end = (me + 1) * line.total / line.warps;
+  bool good = true;
+  uint32_t filled = 0;  // turns loaded by the parts before: the ring goes on behind them
+  while (at < end) {
+  const Stream stream = stream_at(a, b);
+  if (stream.turns == 0 || at - before >= int64_t{stream.turns} * a.kv_heads * pieces) {
+    before += int64_t{stream.turns} * a.kv_heads * pieces;
+    ++b;
+    continue;
+  }
+  const int64_t head_piece = (at - before) / stream.turns;
+  const int first_turn = static_cast<int>((at - before) % stream.turns);
+  const int turns = static_cast<int>(min(int64_t{stream.turns - first_turn}, end - at));
+  at += turns;
+  const int piece = static_cast<int>(head_piece % pieces);
+  const int kv_head = static_cast<int>(head_piece / pieces);
   const int head0 = kv_head * group + piece * kHeads;
   const int heads = min(kHeads, group - piece * kHeads);
-  const int64_t position = a.positions[b];
-  const bool idle = position < 0;
-  const int slot = idle ? -1
-                        : static_cast<int>(position < a.first
-                                               ? position
-                                               : a.first + (position - a.first) %
-                                                               (a.slots - a.first));
-  const int count = idle ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
-  const int row_bytes = a.dim / 2;
+  const int64_t position = stream.position;
+  const int count = stream.count;
+  const int slot = static_cast<int>(
+      position < a.first ? position : a.first + (position - a.first) % (a.slots - a.first));
   const int64_t row0 = (b * a.kv_heads + kv_head) * a.slots;
   uint8_t* const codes[2] = {a.k_codes + row0 * row_bytes, a.v_codes + row0 * row_bytes};
   uint32_t* const range[2] = {static_cast<uint32_t*>(a.k_range) + row0,
@@ -215,36 +306,40 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
   uint8_t* const slots_valid = kMasked ? a.cache_valid + b * a.slots : nullptr;
   const bool token_valid = !kMasked || !a.valid || a.valid[b];
 
-  // This warp's turns of 32 slots: me, me + all, ...
-  const int me = static_cast<int>(rank) * kWarps + warp, all = static_cast<int>(blocks) * kWarps;
-  const int turns = max(0, ((count + kSlots - 1) / kSlots - me + all - 1) / all);
-  const auto base_of = [&](int t) { return (me + t * all) * kSlots; };
+  const auto base_of = [&](int t) { return (first_turn + t) * kSlots; };
   const auto load = [&](int t) {
-    if (t < turns) {
-      Stage<kDim>& st = s.stage[warp][t % kStages];
-      const int base = base_of(t);
-      const int last = count - 1 - base;  // slots behind it are that one again
+    const uint32_t stage = (filled + t) % kStages;
+    if constexpr (kAligned) {  // the turn's rows are one run of memory
+      if (t < turns && good && lane == 0) {
+        const int base = base_of(t);
+        const uint32_t bytes = min(kSlots, count - base) * row_bytes;
+        const uint32_t bar = tc::shared_address(&s.full[warp][stage]);
+        tc::barrier_expect(bar, 2 * bytes);
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const uint8_t* const from = codes[side] + int64_t{base} * row_bytes;
-        if constexpr (kAligned) {
-          // Four lanes (64 channels: two) have a row's 16-byte words.
-          constexpr int kLanes = kDim / 32;
-          const int word = 16 * (lane % kLanes);
-          if (word < row_bytes)
-#pragma unroll
-            for (int r = 0; r < kLanes; ++r) {
-              const int row = lane / kLanes + 32 / kLanes * r;
-              cp_async16(st.codes[side] + row * kRow + word, from + min(row, last) * row_bytes + word);
-            }
-        } else {
-          for (int w = 0; w < row_bytes; w += 4)
-            cp_async4(st.codes[side] + lane * kRow + w, from + min(lane, last) * row_bytes + w);
-        }
-        cp_async4(&st.range[side][lane], range[side] + base + min(lane, last));
+        for (int side = 0; side < 2; ++side)
+          asm volatile(
+              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, "
+              "[%3];" ::"r"(tc::shared_address(s.stage[warp][stage].codes[side])),
+              "l"(codes[side] + int64_t{base} * row_bytes), "r"(bytes), "r"(bar)
+              : "memory");
       }
+    } else {
+      if (t < turns) {
+        Stage<kDim>& st = s.stage[warp][stage];
+        const int row = base_of(t) + min(lane, count - 1 - base_of(t));
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+          for (int w = 0; w < row_bytes; w += 4)
+            cp_async4(st.codes[side] + lane * kRow + w,
+                      codes[side] + int64_t{row} * row_bytes + w);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // The ranges of the lane's slot of a turn, keys' and values', zeros behind the last one.
+  const auto ranges_of = [&](int t) {
+    if (t >= turns || base_of(t) + lane >= count) return make_uint2(0, 0);
+    return make_uint2(__ldcg(range[0] + base_of(t) + lane), __ldcg(range[1] + base_of(t) + lane));
   };
   const auto seen_in = [&](int t) {  // whether the lane's slot of a turn may be seen
     if (t >= turns) return false;
@@ -255,10 +350,11 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
 #pragma unroll
   for (int t = 0; t < kStages - 1; ++t) load(t);
   bool seen_next = seen_in(0);
+  uint2 range_next = ranges_of(0);
 
   // The warp whose turn has the new token's slot rounds its rows.
-  const int slot_turn = idle ? -1 : slot / kSlots;
-  const bool owner = slot_turn >= 0 && slot_turn % all == me;
+  const int slot_turn = slot / kSlots - first_turn;
+  const bool owner = slot_turn >= 0 && slot_turn < turns;
   Fresh fresh = {0, 0};
   if (owner) {
     const bool value = lane >= 16;
@@ -280,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
   uint32_t q[kSets][kKeyWords][4];
   // Of the lane's columns, heads 2j and 2j + 1: what takes their dots and sums of q to
   // scores in base 2.
-  float dot_scale[kSets][2], base_scale[kSets][2];
+  float2 dot_scale[kSets], base_scale[kSets];
 #pragma unroll
   for (int r = 0; r < kSets; ++r) {
     float x[kKeyWords][8], total = 0.0f, largest = 0.0f;
@@ -312,15 +408,15 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         q[r][w][e] = tc::pack2<__half>(x[w][e] * up, x[w][e + 4] * up);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int from = 4 * (2 * j + e);
-      dot_scale[r][e] = __shfl_sync(0xffffffffu, down, from) * (a.scale * kLog2e);
-      base_scale[r][e] = __shfl_sync(0xffffffffu, total, from) * (a.scale * kLog2e);
-    }
+    const float scale = a.scale * kLog2e;
+    dot_scale[r] = make_float2(__shfl_sync(0xffffffffu, down, 8 * j) * scale,
+                               __shfl_sync(0xffffffffu, down, 8 * j + 4) * scale);
+    base_scale[r] = make_float2(__shfl_sync(0xffffffffu, total, 8 * j) * scale,
+                                __shfl_sync(0xffffffffu, total, 8 * j + 4) * scale);
   }
   float out[kSets][kValueWords][4][4] = {};
-  float top[kSets][2], sum[kSets][2] = {}, middle_sum[kSets][2] = {};
+  float top[kSets][2];
+  float2 sum[kSets] = {}, middle_sum[kSets] = {};
 #pragma unroll
   for (int r = 0; r < kSets; ++r) top[r][0] = top[r][1] = -INFINITY;
   // Value steps are taken relative to a power of two above the largest so far.
@@ -331,26 +427,37 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
   // a lane's four slots of V, j, 4 + j, 8 + j and 12 + j, and its neighbours', lie next to one
   // another.
   const int key_row = (g >> 1) + 4 * (g & 1);
-  for (int t = 0; t < turns; ++t) {
+  for (int t = 0; t < turns && good; ++t) {
     load(t + kStages - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    __syncwarp();
-    Stage<kDim>& st = s.stage[warp][t % kStages];
+    Stage<kDim>& st = s.stage[warp][(filled + t) % kStages];
     const int base = base_of(t);
     const bool seen = seen_next;
+    uint2 ranges = range_next;
     seen_next = seen_in(t + 1);
-    if (owner && base == slot_turn * kSlots) {
+    range_next = ranges_of(t + 1);
+    if constexpr (kAligned) {
+      good = tc::barrier_wait_warp(tc::shared_address(&s.full[warp][(filled + t) % kStages]),
+                                   (filled + t) / kStages & 1);
+      if (!good) break;
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+    }
+    if (owner && t == slot_turn) {
       const int side = lane >> 4, word = lane & 15;
       if (8 * word < a.dim)
-        *reinterpret_cast<uint32_t*>(st.codes[side] + (slot - base) * kRow + 4 * word) = fresh.codes;
-      if (word == 0) st.range[side][slot - base] = fresh.range;
+        *reinterpret_cast<uint32_t*>(st.codes[side] + (slot - base) * pitch + 4 * word) = fresh.codes;
+      const uint32_t key = __shfl_sync(0xffffffffu, fresh.range, 0);
+      const uint32_t value = __shfl_sync(0xffffffffu, fresh.range, 16);
+      if (lane == slot - base) ranges = make_uint2(key, value);
+      tc::fence_async_shared();  // before the stage's next load
       __syncwarp();
     }
     // A slot a lane: its ranges, zeros where it is not seen.
     const uint32_t visible = __ballot_sync(0xffffffffu, seen);
     {
-      const float2 key = unpack2<T>(seen ? st.range[0][lane] : 0);
-      const float2 value = unpack2<T>(seen ? st.range[1][lane] : 0);
+      const float2 key = unpack2<T>(seen ? ranges.x : 0);
+      const float2 value = unpack2<T>(seen ? ranges.y : 0);
       const uint32_t largest =
           __reduce_max_sync(0xffffffffu, __float_as_uint(value.x) & 0x7fffffffu);
       if (largest >= unit) {  // the same for the whole warp
@@ -367,8 +474,12 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
         unit = next;
         per_unit = __uint_as_float(0x7f000000u - next);
       }
-      s.slot[warp][lane] = {key.x, fmaf(0.5f, key.x, key.y), value.x * per_unit,
-                            fmaf(0.5f, value.x, value.y)};
+      const float key_base = fmaf(0.5f, key.x, key.y), value_step = value.x * per_unit;
+      const float value_middle = fmaf(0.5f, value.x, value.y);
+      s.slot[warp][lane] = {{key.x, key.x},
+                            {key_base, key_base},
+                            {value_step, value_step},
+                            {value_middle, value_middle}};
     }
     __syncwarp();
     Slot of[4];  // the lane's slots as rows of the scores: key_row, + 8, + 16, + 24
@@ -378,8 +489,8 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {  // 16 slots
       uint32_t low[kKeyWords], high[kKeyWords];
-      read_words<kKeyWords>(st.codes[0] + (16 * half + key_row) * kRow + 4 * kKeyWords * j, low);
-      read_words<kKeyWords>(st.codes[0] + (16 * half + 8 + key_row) * kRow + 4 * kKeyWords * j, high);
+      read_words<kKeyWords>(st.codes[0] + (16 * half + key_row) * pitch + 4 * kKeyWords * j, low);
+      read_words<kKeyWords>(st.codes[0] + (16 * half + 8 + key_row) * pitch + 4 * kKeyWords * j, high);
 #pragma unroll
       for (int w = 0; w < kKeyWords; ++w) {
         uint32_t p0[4], p8[4];
@@ -395,56 +506,52 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
     uint32_t weight[kSets][4];  // of the slots of[i], both heads, then turned around
 #pragma unroll
     for (int r = 0; r < kSets; ++r) {
-      float score[4][2], next[2] = {-INFINITY, -INFINITY};
+      float2 score[4];  // of the lane's two heads
+      float next[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          score[i][e] = fmaf(x[r][i >> 1][2 * (i & 1) + e] * dot_scale[r][e], of[i].key_step,
-                             base_scale[r][e] * of[i].key_base);
+      for (int i = 0; i < 4; ++i) {
+        const float* const c = x[r][i >> 1] + 2 * (i & 1);
+        score[i] = tc::fma2(tc::mul2(make_float2(c[0], c[1]), dot_scale[r]), of[i].key_step,
+                            tc::mul2(base_scale[r], of[i].key_base));
+      }
       if (visible != 0xffffffffu)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!(visible >> (key_row + 8 * i) & 1)) score[i][0] = score[i][1] = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) next[e] = fmaxf(next[e], score[i][e]);
+          if (!(visible >> (key_row + 8 * i) & 1)) score[i].x = score[i].y = -INFINITY;
+      next[0] = fmaxf(tc::max3(score[0].x, score[1].x, score[2].x), score[3].x);
+      next[1] = fmaxf(tc::max3(score[0].y, score[1].y, score[2].y), score[3].y);
       if (__any_sync(0xffffffffu, next[0] > top[r][0] + kSlack || next[1] > top[r][1] + kSlack)) {
+        float shrink[2] = {1.0f, 1.0f};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1)
             next[e] = fmaxf(next[e], __shfl_xor_sync(0xffffffffu, next[e], o));
           if (next[e] > top[r][e] + kSlack) {
-            const float shrink = tc::exp2_approx(top[r][e] - next[e]);
+            shrink[e] = tc::exp2_approx(top[r][e] - next[e]);
             top[r][e] = next[e];
-            sum[r][e] *= shrink;
-            middle_sum[r][e] *= shrink;
-#pragma unroll
-            for (int h = 0; h < kValueWords; ++h)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                out[r][h][i][e] *= shrink;
-                out[r][h][i][2 + e] *= shrink;
-              }
           }
-        }
-      }
-      float shift[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) shift[e] = top[r][e] == -INFINITY ? 0.0f : kLift - top[r][e];
+          for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              out[r][h][i][e] *= shrink[e];
+              out[r][h][i][2 + e] *= shrink[e];
+            }
+        }
+        sum[r] = tc::mul2(sum[r], make_float2(shrink[0], shrink[1]));
+        middle_sum[r] = tc::mul2(middle_sum[r], make_float2(shrink[0], shrink[1]));
+      }
+      const float2 shift = make_float2(top[r][0] == -INFINITY ? 0.0f : kLift - top[r][0],
+                                       top[r][1] == -INFINITY ? 0.0f : kLift - top[r][1]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float p[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          p[e] = tc::exp2_approx(score[i][e] + shift[e]);
-          sum[r][e] += p[e];
-          middle_sum[r][e] = fmaf(p[e], of[i].value_middle, middle_sum[r][e]);
-        }
-        weight[r][i] = transposed(
-            tc::pack2<__half>(p[0] * of[i].value_step, p[1] * of[i].value_step));
+        const float2 y = tc::add2(score[i], shift);
+        const float2 p = make_float2(tc::exp2_approx(y.x), tc::exp2_approx(y.y));
+        sum[r] = tc::add2(sum[r], p);
+        middle_sum[r] = tc::fma2(p, of[i].value_middle, middle_sum[r]);
+        const float2 w = tc::mul2(p, of[i].value_step);
+        weight[r][i] = transposed(tc::pack2<__half>(w.x, w.y));
       }
     }
 #pragma unroll
@@ -453,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         read_words<kValueWords>(
-            st.codes[1] + (16 * half + 4 * i + j) * kRow + 4 * kValueWords * g, word[i]);
+            st.codes[1] + (16 * half + 4 * i + j) * pitch + 4 * kValueWords * g, word[i]);
 #pragma unroll
       for (int h = 0; h < kValueWords; ++h) {
         uint32_t a0[4], a1[4], a2[4], a3[4];  // channels 0 to 3 and 4 to 7, two slots each
@@ -471,118 +578,151 @@ __global__ void __launch_bounds__(kThreads, kSets == 1 ? 4 : kDim == 64 ? 4 : 3)
     }
     __syncwarp();  // all lanes are done with the stage that the next turn fills
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();  // the stages' place is free for the outputs
+  filled += turns;
+  if (!good) {  // let what is in flight land, and show that the result is not valid
+    for (uint64_t& bar : s.full[warp]) tc::barrier_settle(tc::shared_address(&bar));
+    for (float2& x : sum) x = make_float2(NAN, NAN);
+    if (lane == 0) atomicExch(&g_timeout, 1u);
+  }
 
-  // The warp's columns to shared memory: row g of product (h, e) is channel 8 (kValueWords g
-  // + h) + e, row g + 8 channel e + 4.
+  // What the warp leaves: row g of product (h, e) is channel 8 (kValueWords g + h) + e, row g
+  // + 8 channel e + 4. Parts are numbered by warp and item together: both only grow.
+  Part<kDim, kSets>& part = parts[me + (b * a.kv_heads + kv_head) * pieces + piece];
   const float unit_size = __uint_as_float(unit);
 #pragma unroll
   for (int r = 0; r < kSets; ++r)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int head = 8 * r + 2 * j + e;
+      float total = e ? sum[r].y : sum[r].x, middle = e ? middle_sum[r].y : middle_sum[r].x;
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
-        sum[r][e] += __shfl_xor_sync(0xffffffffu, sum[r][e], o);
-        middle_sum[r][e] += __shfl_xor_sync(0xffffffffu, middle_sum[r][e], o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        middle += __shfl_xor_sync(0xffffffffu, middle, o);
       }
+      if (head >= heads) continue;
       if (g == 0) {
-        s.top[warp][head] = top[r][e];
-        s.sum[warp][head] = sum[r][e];
+        part.top[head] = top[r][e];
+        part.sum[head] = total;
       }
 #pragma unroll
       for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          s.out[warp][head][8 * (kValueWords * g + h) + i] =
-              fmaf(out[r][h][i & 3][2 * (i >> 2) + e], unit_size, middle_sum[r][e]);
+        for (int i = 0; i < 2; ++i) {
+          const float(&x)[4][4] = out[r][h];
+          *reinterpret_cast<float4*>(&part.out[head][8 * (kValueWords * g + h) + 4 * i]) =
+              make_float4(fmaf(x[0][2 * i + e], unit_size, middle),
+                          fmaf(x[1][2 * i + e], unit_size, middle),
+                          fmaf(x[2][2 * i + e], unit_size, middle),
+                          fmaf(x[3][2 * i + e], unit_size, middle));
+        }
     }
-  __syncthreads();
-  // The warps joined into the first one's place.
-  for (int c = threadIdx.x; c < heads * kDim; c += kThreads) {
-    const int h = c / kDim, d = c % kDim;
-    float whole = -INFINITY, o = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
-    const float shift = whole == -INFINITY ? 0.0f : whole;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      o = fmaf(s.out[w][h][d], tc::exp2_approx(s.top[w][h] - shift), o);
-    s.out[0][h][d] = o;
+  __syncwarp();  // the next part's slots
   }
-  __syncthreads();
-  if (threadIdx.x < heads) {
-    const int h = threadIdx.x;
-    float whole = -INFINITY, total = 0.0f;
-    for (int w = 0; w < kWarps; ++w) whole = fmaxf(whole, s.top[w][h]);
-    const float shift = whole == -INFINITY ? 0.0f : whole;
-    for (int w = 0; w < kWarps; ++w)
-      total = fmaf(s.sum[w][h], tc::exp2_approx(s.top[w][h] - shift), total);
-    s.top[0][h] = whole;
-    s.sum[0][h] = total;
-  }
-  cluster_sync();
-  // The blocks joined, each block a part of the outputs.
-  for (int c = static_cast<int>(rank) * kThreads + threadIdx.x; c < heads * kDim;
-       c += static_cast<int>(blocks) * kThreads) {
-    const int h = c / kDim, d = c % kDim;
-    float whole = -INFINITY, total = 0.0f, o = 0.0f;
-    for (uint32_t r = 0; r < blocks; ++r) whole = fmaxf(whole, read_block(&s.top[0][h], r));
-    const float shift = whole == -INFINITY ? 0.0f : whole;
-    for (uint32_t r = 0; r < blocks; ++r) {
-      const float w = tc::exp2_approx(read_block(&s.top[0][h], r) - shift);
-      total = fmaf(read_block(&s.sum[0][h], r), w, total);
-      o = fmaf(read_block(&s.out[0][h][d], r), w, o);
-    }
-    if (d < a.dim)
-      static_cast<T*>(a.out)[(b * a.heads + head0 + h) * a.dim + d] =
-          from_float<T>(total == 0.0f ? 0.0f : o / total);
-  }
-  cluster_sync();  // the others have read this block's shared memory
+  if constexpr (!kAligned) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Blocks of a cluster: enough that every multiprocessor has several, as far as every
-// warp still gets a turn.
-int step_blocks(const gs_window_attention_step_4bit_args& a, int64_t items) {
-  int blocks = 1;
-  while (blocks < 16 && items * blocks < 4 * kSmCount && blocks * kWarps * kSlots < a.slots)
-    blocks *= 2;
-  return blocks;
+// An item's parts joined in order, a block an item and head.
+constexpr int kJoinThreads = 256;
+template <class T, int kDim, int kSets>
+__global__ void __launch_bounds__(kJoinThreads)
+    join_kernel(gs_window_attention_step_4bit_args a, const Part<kDim, kSets>* parts,
+                int64_t warps) {
+  constexpr int kHeads = 8 * kSets, kGroups = kJoinThreads / kDim;
+  __shared__ float joined[kGroups][kDim], totals[kGroups];
+  __shared__ int64_t found[2];
+  chain_wait();
+  const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
+  const int64_t item = blockIdx.x, b = item / pieces / a.kv_heads;
+  const int kv_head = static_cast<int>(item / pieces % a.kv_heads);
+  const int piece = static_cast<int>(item % pieces);
+  const int head0 = kv_head * group + piece * kHeads;
+  const int heads = min(kHeads, group - piece * kHeads);
+  const Stream stream = stream_at(a, b);
+  if (threadIdx.x < 32) {  // the warps of the item's first and last turn
+    int64_t total = 0, before = 0;
+    for (int64_t i = threadIdx.x; i < a.batch; i += 32) {
+      const int64_t turns = int64_t{stream_at(a, i).turns} * a.kv_heads * pieces;
+      total += turns;
+      if (i < b) before += turns;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (threadIdx.x == 0 && stream.turns > 0) {
+      warps = min(warps, total);
+      const int64_t first = before + (int64_t{kv_head} * pieces + piece) * stream.turns;
+      // Warp w's turns end at floor((w + 1) total / warps): the first w with that above x.
+      found[0] = ((first + 1) * warps + total - 1) / total - 1;
+      found[1] = ((first + stream.turns) * warps + total - 1) / total - 1;
+    }
+  }
+  __syncthreads();
+  const int d = threadIdx.x % kDim, mine = threadIdx.x / kDim, h = blockIdx.y;
+  if (h >= heads) return;
+  T* const out = static_cast<T*>(a.out) + (b * a.heads + head0 + h) * a.dim;
+  if (stream.turns == 0) {
+    if (threadIdx.x < a.dim) out[threadIdx.x] = from_float<T>(0.0f);
+    return;
+  }
+  const Part<kDim, kSets>* const from = parts + item;
+  float whole = -INFINITY;
+#pragma unroll 4
+  for (int64_t w = found[0]; w <= found[1]; ++w) whole = fmaxf(whole, from[w].top[h]);
+  const float shift = whole == -INFINITY ? 0.0f : whole;
+  float o = 0.0f, total = 0.0f;
+#pragma unroll 4
+  for (int64_t w = found[0] + mine; w <= found[1]; w += kGroups) {
+    const float scale = tc::exp2_approx(from[w].top[h] - shift);
+    total = fmaf(from[w].sum[h], scale, total);
+    o = fmaf(from[w].out[h][d], scale, o);
+  }
+  joined[mine][d] = o;
+  if (d == 0) totals[mine] = total;
+  __syncthreads();
+  if (mine == 0 && d < a.dim) {
+    for (int i = 1; i < kGroups; ++i) {
+      o += joined[i][d];
+      total += totals[i];
+    }
+    out[d] = from_float<T>(total == 0.0f ? 0.0f : o / total);
+  }
+}
+
+// Blocks of the first kernel: all that are resident at once, as far as every warp has a turn.
+int64_t blocks_of(const gs_window_attention_step_4bit_args& a, int64_t items, int sets) {
+  const int64_t turns = items * ceil_div(a.slots, kSlots);
+  return std::min<int64_t>(blocks_per_sm(a.dim <= 64 ? 64 : 128, sets) * kSmCount,
+                           (turns + kWarps - 1) / kWarps);
+}
+
+int64_t items_of(const gs_window_attention_step_4bit_args& a, int sets) {
+  return a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * sets);
 }
 
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
-  const int64_t items = a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * kSets);
-  const int blocks = step_blocks(a, items);
-  if (items * blocks > INT32_MAX) return GS_ERR_CAPACITY;
-  constexpr size_t kShared = sizeof(Shared<kDim, kSets>);
-  GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared, true)));
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = blocks;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = static_cast<unsigned>(items * blocks);
-  config.blockDim = kThreads;
-  config.dynamicSmemBytes = kShared;
-  config.stream = stream;
-  config.attrs = attr;
-  config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, step_kernel<T, kDim, kSets, kMasked, kAligned>, a);
+  const int64_t items = items_of(a, kSets), blocks = blocks_of(a, items, kSets);
+  if (items > INT32_MAX) return GS_ERR_CAPACITY;
+  using P = Part<kDim, kSets>;
+  P* const parts = static_cast<P*>(a.workspace);
+  constexpr size_t kShared = sizeof(Shared<kDim>);
+  GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared)));
+  launch_chained_shared(step_kernel<T, kDim, kSets, kMasked, kAligned>,
+                        dim3(static_cast<unsigned>(blocks)), dim3(kThreads), kShared, stream, a,
+                        parts);
+  GS_TRY(check_launch());
+  launch_chained(join_kernel<T, kDim, kSets>,
+                 dim3(static_cast<unsigned>(items), std::min(a.heads / a.kv_heads, 8 * kSets)), kJoinThreads,
+                 stream, a, static_cast<const P*>(parts), blocks * kWarps);
   return check_launch();
 }
 
-bool strided16(const void* p, int64_t stride, int64_t head_stride) {
-  return is_aligned(p, 16) && stride % 8 == 0 && head_stride % 8 == 0;
-}
+int sets_of(const gs_window_attention_step_4bit_args& a) { return a.heads / a.kv_heads <= 8 ? 1 : 2; }
 
-}  // namespace
-
-int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_args& a,
-                                          cudaStream_t stream) {
+int32_t check_args(const gs_window_attention_step_4bit_args& a) {
   if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.heads > 65535 || a.dim < 8 ||
       a.dim % 8)
     return GS_ERR_INVALID_ARGUMENT;
@@ -591,21 +731,45 @@ int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_ar
   if (a.batch < 0 || a.first < 0 || a.slots <= a.first ||
       a.batch > GS_MAX_SEQUENCE_TOKENS / a.slots || !(a.scale > 0.0f && a.scale < INFINITY))
     return GS_ERR_INVALID_ARGUMENT;
+  return GS_OK;
+}
+
+bool strided16(const void* p, int64_t stride, int64_t head_stride) {
+  return is_aligned(p, 16) && stride % 8 == 0 && head_stride % 8 == 0;
+}
+
+}  // namespace
+
+uint64_t window_attention_step_4bit_workspace_size(const gs_window_attention_step_4bit_args& a) {
+  if (check_args(a) != GS_OK || a.batch == 0) return 0;
+  const int sets = sets_of(a);
+  const int64_t items = items_of(a, sets);
+  const uint64_t part = a.dim <= 64 ? (sets == 1 ? sizeof(Part<64, 1>) : sizeof(Part<64, 2>))
+                                    : (sets == 1 ? sizeof(Part<128, 1>) : sizeof(Part<128, 2>));
+  return part * static_cast<uint64_t>(blocks_of(a, items, sets) * kWarps + items);
+}
+
+int32_t window_attention_4bit_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
+
+int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_args& a,
+                                          cudaStream_t stream) {
+  GS_TRY(check_args(a));
   if (a.batch == 0) return GS_OK;
   if (!a.q || !a.k || !a.v || !a.k_codes || !a.v_codes || !a.k_range || !a.v_range ||
-      !a.positions || !a.out || (a.valid && !a.cache_valid))
+      !a.positions || !a.out || !a.workspace || (a.valid && !a.cache_valid))
     return GS_ERR_INVALID_ARGUMENT;
   if (!strided16(a.q, a.q_stride, a.q_head_stride) ||
       !strided16(a.k, a.k_stride, a.k_head_stride) ||
       !strided16(a.v, a.v_stride, a.v_head_stride) || !is_aligned(a.k_codes, 16) ||
       !is_aligned(a.v_codes, 16) || !is_aligned(a.k_range, 16) || !is_aligned(a.v_range, 16) ||
-      !is_aligned(a.out, 16) || !is_aligned(a.positions, 8))
+      !is_aligned(a.out, 16) || !is_aligned(a.positions, 8) || !is_aligned(a.workspace, 16))
     return GS_ERR_MISALIGNED;
+  if (a.workspace_size < window_attention_step_4bit_workspace_size(a)) return GS_ERR_CAPACITY;
   const auto typed = [&](auto t) {
     using T = decltype(t);
     const auto shaped = [&](auto masked, auto aligned) {
       constexpr bool kMasked = decltype(masked)::value, kAligned = decltype(aligned)::value;
-      if (a.heads / a.kv_heads <= 8)
+      if (sets_of(a) == 1)
         return a.dim <= 64 ? step<T, 64, 1, kMasked, kAligned>(a, stream)
                            : step<T, 128, 1, kMasked, kAligned>(a, stream);
       return a.dim <= 64 ? step<T, 64, 2, kMasked, kAligned>(a, stream)

@@ -34,6 +34,8 @@ int32_t launch_window_attention_step(const gs_window_attention_step_args&, cudaS
 int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_args&, cudaStream_t);
 uint64_t window_attention_workspace_size(const gs_window_attention_args&);
 int32_t window_attention_status(cudaStream_t);
+int32_t window_attention_4bit_status(cudaStream_t);
+uint64_t window_attention_step_4bit_workspace_size(const gs_window_attention_step_4bit_args&);
 int32_t launch_gated_scan(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_backward(const gs_gated_scan_args&, cudaStream_t);
 int32_t launch_gated_scan_step(int64_t, int32_t, int32_t, const void*, int64_t, const void*,
@@ -576,7 +578,14 @@ int32_t gs_window_attention_step(const gs_window_attention_step_args* args, gs_s
 }
 
 int32_t gs_window_attention_status(gs_stream_t stream) {
-  return gs::window_attention_status(as_cuda(stream));
+  const int32_t status = gs::window_attention_status(as_cuda(stream));
+  const int32_t four_bit = gs::window_attention_4bit_status(as_cuda(stream));  // read and cleared both
+  return status ? status : four_bit;
+}
+
+uint64_t gs_window_attention_step_4bit_workspace_size(
+    const gs_window_attention_step_4bit_args* a) {
+  return a ? gs::window_attention_step_4bit_workspace_size(*a) : 0;
 }
 
 int32_t gs_window_attention_step_4bit(const gs_window_attention_step_4bit_args* args,

@@ -74,6 +74,7 @@ EXPORTED_SYMBOLS = (
     "gs_window_attention_status",
     "gs_window_attention_step",
     "gs_window_attention_step_4bit",
+    "gs_window_attention_step_4bit_workspace_size",
     "gs_window_attention_workspace_size",
     "gs_gated_scan",
     "gs_gated_scan_backward",
@@ -242,7 +243,8 @@ class WindowAttentionStep4BitArgs(ctypes.Structure):
                 _fields(ctypes.c_int64, "q_stride q_head_stride k_stride k_head_stride v_stride "
                                         "v_head_stride") +
                 _fields(ctypes.c_void_p, "k_codes v_codes k_range v_range positions out valid "
-                                         "cache_valid"))
+                                         "cache_valid workspace") +
+                _fields(ctypes.c_uint64, "workspace_size"))
 
 
 class GatedScanArgs(ctypes.Structure):
@@ -379,6 +381,8 @@ def lib() -> ctypes.CDLL:
         "gs_window_attention_status": ([vp], i32),
         "gs_window_attention_step": ([ctypes.POINTER(WindowAttentionStepArgs), vp], i32),
         "gs_window_attention_step_4bit": ([ctypes.POINTER(WindowAttentionStep4BitArgs), vp], i32),
+        "gs_window_attention_step_4bit_workspace_size": (
+            [ctypes.POINTER(WindowAttentionStep4BitArgs)], u64),
         "gs_window_attention_workspace_size": ([ctypes.POINTER(WindowAttentionArgs)], u64),
         "gs_gated_scan": ([ctypes.POINTER(GatedScanArgs), vp], i32),
         "gs_gated_scan_backward": ([ctypes.POINTER(GatedScanArgs), vp], i32),

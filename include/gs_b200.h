@@ -612,7 +612,12 @@ typedef struct gs_window_attention_step_4bit_args {
   void *out;
   const uint8_t *valid;
   uint8_t *cache_valid;
+  void *workspace; /* gs_window_attention_step_4bit_workspace_size bytes, 16-byte aligned */
+  uint64_t workspace_size;
 } gs_window_attention_step_4bit_args;
+
+uint64_t gs_window_attention_step_4bit_workspace_size(
+    const gs_window_attention_step_4bit_args *args);
 
 int32_t gs_window_attention_step_4bit(const gs_window_attention_step_4bit_args *args,
                                       gs_stream_t stream);

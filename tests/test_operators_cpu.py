@@ -93,13 +93,14 @@ def test_4bit_step_checks_arguments():
     good = dict(batch=2, heads=4, kv_heads=2, dim=64, dtype=1, slots=10, first=2, scale=0.1, q=a,
                 k=a, v=a, q_stride=64, q_head_stride=64, k_stride=64, k_head_stride=64,
                 v_stride=64, v_head_stride=64, k_codes=a, v_codes=a, k_range=a, v_range=a,
-                positions=a, out=a)
+                positions=a, out=a, workspace=a, workspace_size=1 << 40)
     for status, bad in [(-1, dict(heads=3)), (-1, dict(dim=12)), (-4, dict(dim=136)),
                         (-4, dict(dtype=0)), (-1, dict(batch=-1)), (-1, dict(first=10)),
                         (-1, dict(slots=0)), (-1, dict(batch=2 ** 30)),
                         (-1, dict(scale=float("nan"))), (-1, dict(k_codes=None)),
                         (-1, dict(v_range=None)), (-1, dict(valid=a)), (-5, dict(k=a + 2)),
-                        (-5, dict(v_stride=4)), (-5, dict(v_codes=a + 4))]:
+                        (-5, dict(v_stride=4)), (-5, dict(v_codes=a + 4)),
+                        (-1, dict(workspace=None)), (-3, dict(workspace_size=16))]:
         args = native.WindowAttentionStep4BitArgs(**{**good, **bad})
         assert lib.gs_window_attention_step_4bit(ctypes.byref(args), None) == status, bad
     assert lib.gs_window_attention_step_4bit(None, None) == -1
