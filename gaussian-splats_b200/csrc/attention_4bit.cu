@@ -52,11 +52,11 @@ struct Stage {
   alignas(16) unsigned char codes[2][kSlots * kRow];  // keys', values'
 };
 
-// What a slot's ranges come to: score = dot * key_step + (sum of q) * key_base, where
-// dot has c - 8.
+// What a slot's ranges come to: score = (dot with c - 7.5) * key_step + (sum of q) *
+// key_middle.
 // Each twice, for instructions on two floats (a lane's two heads).
 struct Slot {
-  float2 key_step, key_base, value_step, value_middle;
+  float2 key_step, key_middle, value_step, value_middle;
 };
 
 template <int kDim>
@@ -71,6 +71,11 @@ template <int kDim, int kSets>
 struct Part {
   float out[8 * kSets][kDim];
   float top[8 * kSets], sum[8 * kSets];
+};
+
+// The warps that have an item's first and last turn.
+struct Reach {
+  int32_t first, last;
 };
 
 // A stream's slots that count (0: idle), and its turns.
@@ -177,6 +182,7 @@ __device__ __forceinline__ Fresh round_row(const T* row, int dim) {
   return f;
 }
 
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 template <class T>
 __device__ __forceinline__ float2 unpack2(uint32_t word) {
   const T* v = reinterpret_cast<const T*>(&word);
@@ -204,13 +210,26 @@ __device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16
       : "r"(among(word, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
   return y;
 }
-// Codes 0 to 3 of both halves of a word as four pairs.
+// Codes 0 to 3 of both halves of a value's word as four pairs.
 __device__ __forceinline__ void spread(uint32_t word, uint32_t (&pair)[4]) {
   const uint32_t next = word >> 8;
   pair[0] = centred_low(word);
   pair[1] = centred_high(word);
   pair[2] = centred_low(next);
   pair[3] = centred_high(next);
+}
+
+// A key's codes keep what they lie next to, which is taken off the dots: pairs 0 and 2
+// are 1024 + 4 c, pairs 1 and 3 1024 + 64 c, so that in units of the code, with q scaled
+// to match, they are off by 256 and 16. (In the dots' float sums that costs 2^-23 of
+// 256 sum |q| a product: 1e-5 of a score. The values' sums are too long for it.)
+constexpr float kLowOffset = 256.0f, kHighOffset = 16.0f;
+__device__ __forceinline__ void spread_key(uint32_t word, uint32_t (&pair)[4]) {
+  const uint32_t up = word << 2, down = word >> 6;
+  pair[0] = among(up, 0x003c003cu, 0x64006400u);
+  pair[1] = among(up, 0x03c003c0u, 0x64006400u);
+  pair[2] = among(down, 0x003c003cu, 0x64006400u);
+  pair[3] = among(down, 0x03c003c0u, 0x64006400u);
 }
 
 // c += a b, 16 x 16 by 16 x 8.
@@ -250,7 +269,7 @@ __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)
 // whole 16-byte words.
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
-    step_kernel(gs_window_attention_step_4bit_args a, Part<kDim, kSets>* parts) {
+    step_kernel(gs_window_attention_step_4bit_args a, Part<kDim, kSets>* parts, Reach* reach) {
   using S = Shared<kDim>;
   constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
   constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
@@ -350,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 #pragma unroll
   for (int t = 0; t < kStages - 1; ++t) load(t);
   bool seen_next = seen_in(0);
-  uint2 range_next = ranges_of(0);
+  uint2 range_next = ranges_of(0), range_after = ranges_of(1);  // two turns ahead
 
   // The warp whose turn has the new token's slot rounds its rows.
   const int slot_turn = slot / kSlots - first_turn;
@@ -372,14 +391,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 
   // Head g's q (and head g + 8's), channels in the order of the keys' products: a word's
   // are pairs (0, 4), (1, 5) of one product and (2, 6), (3, 7) of the next. A head's largest
-  // channel goes to 2^10.
+  // channel goes to 2^10, or 2^6 where codes are 16 times as large.
   uint32_t q[kSets][kKeyWords][4];
-  // Of the lane's columns, heads 2j and 2j + 1: what takes their dots and sums of q to
-  // scores in base 2.
-  float2 dot_scale[kSets], base_scale[kSets];
+  // Of the lane's columns, heads 2j and 2j + 1: what takes their dots to those with c - 7.5,
+  // and the sums of q; both in base 2.
+  float2 dot_scale[kSets], dot_offset[kSets], q_sum[kSets];
 #pragma unroll
   for (int r = 0; r < kSets; ++r) {
-    float x[kKeyWords][8], total = 0.0f, largest = 0.0f;
+    float x[kKeyWords][8], low_total = 0.0f, high_total = 0.0f, largest = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKeyWords; ++w) {
       const int channel = 8 * (kKeyWords * j + w);
@@ -391,13 +410,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
                      x[w]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        total += x[w][k];
+        if (k & 1) high_total += x[w][k];
+        else low_total += x[w][k];
         largest = max_nan(largest, fabsf(x[w][k]));
       }
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
+      low_total += __shfl_xor_sync(0xffffffffu, low_total, o);
+      high_total += __shfl_xor_sync(0xffffffffu, high_total, o);
       largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
     }
     const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, 11u << 23);
@@ -407,12 +428,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     for (int w = 0; w < kKeyWords; ++w)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        q[r][w][e] = tc::pack2<__half>(x[w][e] * up, x[w][e + 4] * up);
-    const float scale = a.scale * kLog2e;
-    dot_scale[r] = make_float2(__shfl_sync(0xffffffffu, down, 8 * j) * scale,
-                               __shfl_sync(0xffffffffu, down, 8 * j + 4) * scale);
-    base_scale[r] = make_float2(__shfl_sync(0xffffffffu, total, 8 * j) * scale,
-                                __shfl_sync(0xffffffffu, total, 8 * j + 4) * scale);
+        q[r][w][e] = tc::pack2<__half>(x[w][e] * (e & 1 ? 0.0625f * up : up),
+                                       x[w][e + 4] * (e & 1 ? 0.0625f * up : up));
+    const float scale = a.scale * kLog2e, total = low_total + high_total;
+    const float offset = kLowOffset * low_total + kHighOffset * high_total + 7.5f * total;
+    const auto heads_of = [&](float x) {
+      return make_float2(__shfl_sync(0xffffffffu, x, 8 * j), __shfl_sync(0xffffffffu, x, 8 * j + 4));
+    };
+    dot_scale[r] = heads_of(0.25f * down * scale);
+    dot_offset[r] = heads_of(-offset * scale);
+    q_sum[r] = heads_of(total * scale);
   }
   float out[kSets][kValueWords][4][4] = {};
   float top[kSets][2];
@@ -434,7 +459,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     const bool seen = seen_next;
     uint2 ranges = range_next;
     seen_next = seen_in(t + 1);
-    range_next = ranges_of(t + 1);
+    range_next = range_after;
+    range_after = ranges_of(t + 2);
     if constexpr (kAligned) {
       good = tc::barrier_wait_warp(tc::shared_address(&s.full[warp][(filled + t) % kStages]),
                                    (filled + t) / kStages & 1);
@@ -474,12 +500,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         unit = next;
         per_unit = __uint_as_float(0x7f000000u - next);
       }
-      const float key_base = fmaf(0.5f, key.x, key.y), value_step = value.x * per_unit;
-      const float value_middle = fmaf(0.5f, value.x, value.y);
-      s.slot[warp][lane] = {{key.x, key.x},
-                            {key_base, key_base},
-                            {value_step, value_step},
-                            {value_middle, value_middle}};
+      const float weight_step = value.x * per_unit, middle = fmaf(0.5f, value.x, value.y);
+      s.slot[warp][lane] = {both(key.x), both(key.y), both(weight_step), both(middle)};
     }
     __syncwarp();
     Slot of[4];  // the lane's slots as rows of the scores: key_row, + 8, + 16, + 24
@@ -494,8 +516,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 #pragma unroll
       for (int w = 0; w < kKeyWords; ++w) {
         uint32_t p0[4], p8[4];
-        spread(low[w], p0);
-        spread(high[w], p8);
+        spread_key(low[w], p0);
+        spread_key(high[w], p8);
 #pragma unroll
         for (int r = 0; r < kSets; ++r) {
           multiply(x[r][half], p0[0], p8[0], p0[1], p8[1], q[r][w][0], q[r][w][1]);
@@ -511,8 +533,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float* const c = x[r][i >> 1] + 2 * (i & 1);
-        score[i] = tc::fma2(tc::mul2(make_float2(c[0], c[1]), dot_scale[r]), of[i].key_step,
-                            tc::mul2(base_scale[r], of[i].key_base));
+        score[i] = tc::fma2(tc::fma2(make_float2(c[0], c[1]), dot_scale[r], dot_offset[r]),
+                            of[i].key_step, tc::mul2(q_sum[r], of[i].key_middle));
       }
       if (visible != 0xffffffffu)
 #pragma unroll
@@ -587,7 +609,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 
   // What the warp leaves: row g of product (h, e) is channel 8 (kValueWords g + h) + e, row g
   // + 8 channel e + 4. Parts are numbered by warp and item together: both only grow.
-  Part<kDim, kSets>& part = parts[me + (b * a.kv_heads + kv_head) * pieces + piece];
+  const int64_t item = (b * a.kv_heads + kv_head) * pieces + piece;
+  Part<kDim, kSets>& part = parts[me + item];
+  if (lane == 0 && first_turn == 0) reach[item].first = static_cast<int32_t>(me);
+  if (lane == 0 && first_turn + turns == stream.turns) reach[item].last = static_cast<int32_t>(me);
   const float unit_size = __uint_as_float(unit);
 #pragma unroll
   for (int r = 0; r < kSets; ++r)
@@ -622,71 +647,70 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   if constexpr (!kAligned) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// An item's parts joined in order, a block an item and head.
-constexpr int kJoinThreads = 256;
+// An item's parts joined in order, a block an item and head: the threads of a channel take
+// every so many parts. What is left of the time is latency, so what a thread needs first
+// is requested before it is known what it is multiplied by.
+constexpr int kMostParts = 256, kAhead = 8;
 template <class T, int kDim, int kSets>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(1024)
     join_kernel(gs_window_attention_step_4bit_args a, const Part<kDim, kSets>* parts,
-                int64_t warps) {
-  constexpr int kHeads = 8 * kSets, kGroups = kJoinThreads / kDim;
-  __shared__ float joined[kGroups][kDim], totals[kGroups];
-  __shared__ int64_t found[2];
+                const Reach* reach) {
+  constexpr int kHeads = 8 * kSets;
+  __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32];
   chain_wait();
   const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
   const int64_t item = blockIdx.x, b = item / pieces / a.kv_heads;
   const int kv_head = static_cast<int>(item / pieces % a.kv_heads);
-  const int piece = static_cast<int>(item % pieces);
-  const int head0 = kv_head * group + piece * kHeads;
-  const int heads = min(kHeads, group - piece * kHeads);
-  const Stream stream = stream_at(a, b);
-  if (threadIdx.x < 32) {  // the warps of the item's first and last turn
-    int64_t total = 0, before = 0;
-    for (int64_t i = threadIdx.x; i < a.batch; i += 32) {
-      const int64_t turns = int64_t{stream_at(a, i).turns} * a.kv_heads * pieces;
-      total += turns;
-      if (i < b) before += turns;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (threadIdx.x == 0 && stream.turns > 0) {
-      warps = min(warps, total);
-      const int64_t first = before + (int64_t{kv_head} * pieces + piece) * stream.turns;
-      // Warp w's turns end at floor((w + 1) total / warps): the first w with that above x.
-      found[0] = ((first + 1) * warps + total - 1) / total - 1;
-      found[1] = ((first + stream.turns) * warps + total - 1) / total - 1;
-    }
-  }
-  __syncthreads();
-  const int d = threadIdx.x % kDim, mine = threadIdx.x / kDim, h = blockIdx.y;
-  if (h >= heads) return;
-  T* const out = static_cast<T*>(a.out) + (b * a.heads + head0 + h) * a.dim;
-  if (stream.turns == 0) {
+  const int piece = static_cast<int>(item % pieces), h = blockIdx.y;
+  if (h >= min(kHeads, group - piece * kHeads)) return;
+  const Reach r = reach[item];  // of an idle stream's items: whatever was there
+  T* const out = static_cast<T*>(a.out) +
+                 (b * a.heads + kv_head * group + piece * kHeads + h) * a.dim;
+  if (a.positions[b] < 0) {
     if (threadIdx.x < a.dim) out[threadIdx.x] = from_float<T>(0.0f);
     return;
   }
-  const Part<kDim, kSets>* const from = parts + item;
-  float whole = -INFINITY;
-#pragma unroll 4
-  for (int64_t w = found[0]; w <= found[1]; ++w) whole = fmaxf(whole, from[w].top[h]);
+  const int count = r.last - r.first + 1, threads = blockDim.x, thread = threadIdx.x;
+  const int d = thread % kDim, groups = threads / kDim, mine = thread / kDim;
+  const Part<kDim, kSets>* const from = parts + item + r.first;
+  float ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    ahead[k] = mine + k * groups < count ? from[mine + k * groups].out[h][d] : 0.0f;
+  float top = -INFINITY, sum = 0.0f;
+  if (thread < count) top = from[thread].top[h], sum = from[thread].sum[h];
+  float whole = top;
+  for (int i = thread + threads; i < count; i += threads) whole = fmaxf(whole, from[i].top[h]);
+  whole = warp_max(whole);
+  if ((thread & 31) == 0) tops[thread >> 5] = whole;
+  __syncthreads();
+  for (int w = 0; w < threads / 32; ++w) whole = fmaxf(whole, tops[w]);
   const float shift = whole == -INFINITY ? 0.0f : whole;
   float o = 0.0f, total = 0.0f;
-#pragma unroll 4
-  for (int64_t w = found[0] + mine; w <= found[1]; w += kGroups) {
-    const float scale = tc::exp2_approx(from[w].top[h] - shift);
-    total = fmaf(from[w].sum[h], scale, total);
-    o = fmaf(from[w].out[h][d], scale, o);
-  }
-  joined[mine][d] = o;
-  if (d == 0) totals[mine] = total;
-  __syncthreads();
-  if (mine == 0 && d < a.dim) {
-    for (int i = 1; i < kGroups; ++i) {
-      o += joined[i][d];
-      total += totals[i];
+  for (int i0 = 0; i0 < count; i0 += kMostParts) {
+    __syncthreads();
+    const int some = min(kMostParts, count - i0);
+    if (thread < some) {  // kMostParts threads at least
+      if (i0 > 0) top = from[i0 + thread].top[h], sum = from[i0 + thread].sum[h];
+      scales[thread] = tc::exp2_approx(top - shift);
+      sums[thread] = sum * scales[thread];
     }
+    __syncthreads();
+    int i = mine;
+    if (i0 == 0) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k, i += groups)
+        if (i < some) o = fmaf(ahead[k], scales[i], o);
+    }
+#pragma unroll 8
+    for (; i < some; i += groups) o = fmaf(from[i0 + i].out[h][d], scales[i], o);
+    if (thread < a.dim)
+      for (int k = 0; k < some; ++k) total += sums[k];
+  }
+  joined[thread] = o;
+  __syncthreads();
+  if (thread < a.dim) {
+    for (int i = 1; i < groups; ++i) o += joined[i * kDim + d];
     out[d] = from_float<T>(total == 0.0f ? 0.0f : o / total);
   }
 }
@@ -702,21 +726,27 @@ int64_t items_of(const gs_window_attention_step_4bit_args& a, int sets) {
   return a.batch * a.kv_heads * ceil_div(a.heads / a.kv_heads, 8 * sets);
 }
 
+uint64_t reach_bytes(int64_t items) { return (sizeof(Reach) * static_cast<uint64_t>(items) + 15) / 16 * 16; }
+
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
   const int64_t items = items_of(a, kSets), blocks = blocks_of(a, items, kSets);
   if (items > INT32_MAX) return GS_ERR_CAPACITY;
   using P = Part<kDim, kSets>;
-  P* const parts = static_cast<P*>(a.workspace);
+  Reach* const reach = static_cast<Reach*>(a.workspace);
+  P* const parts = reinterpret_cast<P*>(static_cast<unsigned char*>(a.workspace) + reach_bytes(items));
   constexpr size_t kShared = sizeof(Shared<kDim>);
   GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared)));
   launch_chained_shared(step_kernel<T, kDim, kSets, kMasked, kAligned>,
                         dim3(static_cast<unsigned>(blocks)), dim3(kThreads), kShared, stream, a,
-                        parts);
+                        parts, reach);
   GS_TRY(check_launch());
+  // Threads by the parts of an item: few parts, many items; many parts, few items.
+  const int threads = blocks * kWarps >= 16 * items ? 1024 : 256;
   launch_chained(join_kernel<T, kDim, kSets>,
-                 dim3(static_cast<unsigned>(items), std::min(a.heads / a.kv_heads, 8 * kSets)), kJoinThreads,
-                 stream, a, static_cast<const P*>(parts), blocks * kWarps);
+                 dim3(static_cast<unsigned>(items), std::min(a.heads / a.kv_heads, 8 * kSets)),
+                 threads, stream, a, static_cast<const P*>(parts),
+                 static_cast<const Reach*>(reach));
   return check_launch();
 }
 
@@ -746,7 +776,8 @@ uint64_t window_attention_step_4bit_workspace_size(const gs_window_attention_ste
   const int64_t items = items_of(a, sets);
   const uint64_t part = a.dim <= 64 ? (sets == 1 ? sizeof(Part<64, 1>) : sizeof(Part<64, 2>))
                                     : (sets == 1 ? sizeof(Part<128, 1>) : sizeof(Part<128, 2>));
-  return part * static_cast<uint64_t>(blocks_of(a, items, sets) * kWarps + items);
+  return reach_bytes(items) +
+         part * static_cast<uint64_t>(blocks_of(a, items, sets) * kWarps + items);
 }
 
 int32_t window_attention_4bit_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
