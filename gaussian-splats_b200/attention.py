@@ -314,21 +314,19 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     128; ``positions``, ``first``, ``scale``, ``valid`` and ``cache_valid`` as
     :func:`window_attention_step` takes them. No gradient."""
     what = "window_attention_step_4bit"
-    cache = FourBitCache(*cache)
-    device = check_cuda(what, q=q, k=k, v=v, **cache._asdict(), positions=positions, valid=valid,
+    k_codes, k_range, v_codes, v_range = cache
+    device = check_cuda(what, q=q, k=k, v=v, k_codes=k_codes, k_range=k_range, v_codes=v_codes,
+                        v_range=v_range, positions=positions, valid=valid,
                         cache_valid=cache_valid)
     dtype = _heads(what, q, k, v, "batch")
     batch, heads, dim = q.shape
     kv_heads = k.shape[1]
-    slots = cache.k_codes.shape[2] if cache.k_codes.dim() == 4 else 0
-    for name, t in cache._asdict().items():
-        codes = name.endswith("codes")
-        shape, kind = (batch, kv_heads, slots, dim // 2 if codes else 2), \
-            torch.uint8 if codes else q.dtype
-        if slots < 1 or tuple(t.shape) != shape or t.dtype != kind:
-            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} is not [batch, kv_heads, "
-                             f"slots, {'dim / 2' if codes else '2'}] of {kind} for k "
-                             f"{tuple(k.shape)}")
+    slots = k_codes.shape[2] if k_codes.dim() == 4 else 0
+    for t, last, kind in ((k_codes, dim // 2, torch.uint8), (k_range, 2, q.dtype),
+                          (v_codes, dim // 2, torch.uint8), (v_range, 2, q.dtype)):
+        if slots < 1 or t.shape != (batch, kv_heads, slots, last) or t.dtype != kind:
+            raise ValueError(f"{what}: a cache's {tuple(t.shape)} {t.dtype} is not [batch, "
+                             f"kv_heads, slots, {last}] of {kind} for k {tuple(k.shape)}")
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f"{what}: the cache must be contiguous and 16-byte aligned (it is "
                              "updated in place)")
@@ -343,10 +341,11 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
                       kv_heads=kv_heads, dim=dim, dtype=dtype, slots=slots, first=first,
                       scale=_scale(what, scale, dim), positions=positions.data_ptr(),
                       out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid),
-                      **{name: t.data_ptr() for name, t in cache._asdict().items()})
+                      k_codes=k_codes.data_ptr(), k_range=k_range.data_ptr(),
+                      v_codes=v_codes.data_ptr(), v_range=v_range.data_ptr())
     size = native.lib().gs_window_attention_step_4bit_workspace_size(ctypes.byref(args))
     workspace = q.new_empty((size,), dtype=torch.uint8)
     args.workspace, args.workspace_size = workspace.data_ptr(), size
     call("gs_window_attention_step_4bit", device, ctypes.byref(args))
-    changed_in_place(*cache, cache_valid)
+    changed_in_place(k_codes, k_range, v_codes, v_range, cache_valid)
     return out

@@ -20,6 +20,7 @@ from .sequences import address, call, check_cuda, check_tokens, element_type
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}  # GS_IDENTITY, ...
 _TYPES = (torch.bfloat16, torch.float16)
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_FLOAT32, ...
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
@@ -35,35 +36,42 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 def _arguments(x, weight, bias, **values):
     """``gs_linear_args`` of operands ``x`` and ``weight``."""
-    dtype = element_type(x.dtype, "")
+    dtype = _CODES[x.dtype]
     return native.LinearArgs(
         rows=x.shape[0], inputs=x.shape[1], outputs=weight.shape[0], dtype=dtype,
-        bias_dtype=dtype if bias is None else element_type(bias.dtype, ""),
-        x=address(x), weight=address(weight), bias=address(bias), x_stride=x.stride(0),
+        bias_dtype=dtype if bias is None else _CODES[bias.dtype], x=x.data_ptr(),
+        weight=weight.data_ptr(), bias=address(bias), x_stride=x.stride(0),
         weight_stride=weight.stride(0), **values)
+
+
+def _forward(x, weight, bias, residual, activation, train):
+    """The result, and what the backward keeps."""
+    inputs, outputs = x.shape[-1], weight.shape[0]
+    rows, w = _operand(x if x.dim() == 2 else x.reshape(-1, inputs)), _operand(weight)
+    b = None if bias is None else bias.contiguous()
+    if residual is None:
+        y, res, stride = x.new_empty(x.shape[:-1] + (outputs,)), None, 0
+    else:
+        y, res = residual.new_empty(residual.shape), _rows(residual)
+        stride = res.stride(0)
+    slope = None
+    if train and activation:
+        exact = b is not None and b.dtype == torch.float32
+        slope = x.new_empty((rows.shape[0], -(-outputs // 8) * 8),
+                            dtype=torch.float32 if exact else torch.int16)
+    args = _arguments(rows, w, b, activation=activation, residual_dtype=_CODES[y.dtype],
+                      residual=address(res), residual_stride=stride, y=y.data_ptr(),
+                      slope=address(slope))
+    call("gs_linear", x.device, ctypes.byref(args))
+    return y, (rows, w, b, slope)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, train):
-        shape = x.shape[:-1] + weight.shape[:1]
-        rows, w = _operand(x.reshape(-1, x.shape[-1])), _operand(weight)
-        b = None if bias is None else bias.contiguous()
-        res = None if residual is None else _rows(residual)
-        y = (x if res is None else res).new_empty(shape)
-        slope = None
-        if train and activation:
-            exact = b is not None and b.dtype == torch.float32
-            slope = x.new_empty((rows.shape[0], -(-w.shape[0] // 8) * 8),
-                                dtype=torch.float32 if exact else torch.int16)
-        args = _arguments(rows, w, b, activation=activation,
-                          residual_dtype=element_type(y.dtype, ""), residual=address(res),
-                          residual_stride=0 if res is None else res.stride(0), y=address(y),
-                          slope=address(slope))
-        call("gs_linear", x.device, ctypes.byref(args))
-        if train:
-            ctx.save_for_backward(rows, w, b, slope)
-            ctx.activation, ctx.shape = activation, x.shape
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, kept = _forward(x, weight, bias, residual, activation, True)
+        ctx.save_for_backward(*kept)
+        ctx.activation, ctx.shape = activation, x.shape
         return y
 
     @staticmethod
@@ -80,14 +88,14 @@ class _Linear(torch.autograd.Function):
         if want_x or want_weight or want_bias:
             rows = _whole(grad_y.reshape(x.shape[0], weight.shape[0]))
             args = _arguments(x, weight, bias, activation=ctx.activation,
-                              residual_dtype=element_type(rows.dtype, ""), slope=address(slope),
+                              residual_dtype=_CODES[rows.dtype], slope=address(slope),
                               grad_y=address(rows), grad_x=address(grads[0]),
                               grad_weight=address(grads[1]), grad_bias=address(grads[2]))
             size = native.lib().gs_linear_workspace_size(ctypes.byref(args))
             workspace = x.new_empty((size,), dtype=torch.uint8)
             args.workspace, args.workspace_size = address(workspace), size
             call("gs_linear_backward", x.device, ctypes.byref(args))
-        return (*grads, grad_y if want_residual else None, None, None)
+        return (*grads, grad_y if want_residual else None, None)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -134,4 +142,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise ValueError(f"{what}: the {name} must be {x.dtype} or float32, got {t.dtype}")
     train = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, weight, bias, residual))
-    return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation], train)
+    if train:
+        return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
+    return _forward(x, weight, bias, residual, ACTIVATIONS[activation], False)[0]

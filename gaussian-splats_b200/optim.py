@@ -56,24 +56,30 @@ def _max_norm(what: str, max_norm: float) -> float:
 def _norm(what: str, tensors: list[torch.Tensor], max_norm: float, scale: bool) -> torch.Tensor:
     """The norm of dense tensors on one device and the factor that clips it to
     ``max_norm``, two floats; with ``scale`` the tensors are multiplied by it."""
-    device, entries = tensors[0].device, (native.Gradient * len(tensors))()
-    for entry, t in zip(entries, tensors):
+    device, words = tensors[0].device, []
+    index = tensors[0].get_device()
+    for t in tensors:
         dtype = _TYPES.get(t.dtype)
-        if dtype is None or t.device != device or not t.is_cuda or t.layout != torch.strided:
-            if t.is_cuda and t.device != device:
-                raise RuntimeError(f"{what}: a gradient is on {t.device}, another on {device}")
-            if not t.is_cuda:
-                raise RuntimeError(f"{what} runs on CUDA devices only (there is no CPU path); a "
-                                   f"gradient is on {t.device}")
-            raise ValueError(f"{what}: gradients must be dense and float32, bfloat16 or float16, "
-                             f"got {t.dtype} ({t.layout})")
-        entry.data, entry.count, entry.dtype = t.data_ptr(), t.numel(), dtype
+        if dtype is None or t.get_device() != index or index < 0 or t.layout != torch.strided:
+            _refuse(what, t, device)
+        words += (t.data_ptr(), t.numel(), dtype)
+    entries = (ctypes.c_int64 * len(words))(*words)  # gs_gradient: three words each
     size = native.lib().gs_clip_grad_norm_workspace_size(len(tensors))
     result = torch.empty(2, dtype=torch.float32, device=device)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    call("gs_clip_grad_norm", device, len(tensors), ctypes.byref(entries), max_norm, int(scale),
-         ctypes.c_void_p(result.data_ptr()), ctypes.c_void_p(workspace.data_ptr()), size)
+    call("gs_clip_grad_norm", device, len(tensors), entries, max_norm, int(scale),
+         result.data_ptr(), workspace.data_ptr(), size)
     return result
+
+
+def _refuse(what: str, t: torch.Tensor, device: torch.device) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs on CUDA devices only (there is no CPU path); a gradient "
+                           f"is on {t.device}")
+    if t.layout != torch.strided or t.dtype not in _TYPES:
+        raise ValueError(f"{what}: gradients must be dense and float32, bfloat16 or float16, got "
+                         f"{t.dtype} ({t.layout})")
+    raise RuntimeError(f"{what}: a gradient is on {t.device}, another on {device}")
 
 
 def _check_finite(what: str, norm: torch.Tensor) -> None:
@@ -115,16 +121,16 @@ def clip_grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: 
     grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=parameters[0].device)
-    tensors = [g.detach() for g in grads]
-    copies = []
-    woven = _woven(tensors)
-    for i, t in enumerate(tensors):
-        if t.layout == torch.strided and (woven or not _dense(t)):
-            if 0 in (s for s, n in zip(t.stride(), t.shape) if n > 1):
-                raise ValueError(f"{what}: a gradient of strides {t.stride()} shares memory "
-                                 "between its elements")
-            tensors[i] = t.clone(memory_format=torch.contiguous_format)
-            copies.append((t, tensors[i]))
+    tensors, copies, spans = list(grads), [], []
+    whole = True
+    for g in grads:
+        if g.layout != torch.strided or not g.is_contiguous():
+            whole = False
+            break
+        at = g.data_ptr()
+        spans.append((at, at + g.nbytes))
+    if not whole or _overlap(spans):
+        copies = _apart(what, tensors)
     if error_if_nonfinite:
         _check_finite(what, _norm(what, tensors, max_norm, False)[0])
     result = _norm(what, tensors, max_norm, True)
@@ -134,17 +140,28 @@ def clip_grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: 
     return result[0]
 
 
-def _woven(tensors: list[torch.Tensor]) -> bool:
-    """Whether the memory that tensors span overlaps (slices of one tensor, say)."""
-    spans = []
-    for t in tensors:
-        if t.layout == torch.strided and t.numel():
-            size = t.numel() if t.is_contiguous() else \
-                1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))
-            at = t.data_ptr()
-            spans.append((at, at + size * t.element_size()))
-    spans.sort()
+def _overlap(spans: list[tuple[int, int]]) -> bool:
+    spans = sorted(s for s in spans if s[0] < s[1])
     return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
+def _apart(what: str, tensors: list[torch.Tensor]) -> list[tuple[torch.Tensor, torch.Tensor]]:
+    """Replaces gradients that do not fill one run of memory by contiguous copies, and
+    all of them where what they span overlaps (slices of one tensor, say); returns
+    those replaced and their copies."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(
+        s * (n - 1) for s, n in zip(t.stride(), t.shape)))) for t in tensors
+        if t.layout == torch.strided and t.numel()]
+    woven, copies = _overlap(spans), []
+    for i, t in enumerate(tensors):
+        if t.layout == torch.strided and (woven or not _dense(t)):
+            if 0 in (s for s, n in zip(t.stride(), t.shape) if n > 1):
+                raise ValueError(f"{what}: a gradient of strides {t.stride()} shares memory "
+                                 "between its elements")
+            t = t.detach()
+            tensors[i] = t.clone(memory_format=torch.contiguous_format)
+            copies.append((t, tensors[i]))
+    return copies
 
 
 class FusedAdam(torch.optim.Adam):
