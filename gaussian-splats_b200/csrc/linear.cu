@@ -133,12 +133,51 @@ struct EpilogueMaps {
   CUtensorMap out, residual, slope;
 };
 
+// What an epilogue has to do, where the kernel is built for it: code that decides as it
+// goes takes twice the instructions. kAny decides, and writes what TMA does not take.
+enum class Form {
+  kAny,
+  kNarrow,    // 16-bit result
+  kActive,    // 16-bit result of an activation
+  kTraining,  // the same, and its slopes in 16 bits
+  kWide,      // float result (sums to be joined)
+  kStream,    // float result added to a residual
+};
+
 // Items are (split, row tile, column tile), the last one fastest.
 struct Plan {
   int32_t row_tiles, column_tiles, splits;
   int32_t steps;            // of kDepth, in the whole contraction
   int32_t steps_per_split;
   int64_t split_rows;       // rows of `out` from one split's sums to the next one's
+};
+
+// A block's items: its own, and every one that many blocks further.
+struct Walk {
+  int32_t split, row, column;  // tiles
+  int32_t split_step, row_step, column_step;
+  __device__ explicit Walk(const Plan& p) {
+    const auto cut = [&](uint32_t item, int32_t& s, int32_t& r, int32_t& c) {
+      c = item % p.column_tiles;
+      item /= p.column_tiles;
+      r = item % p.row_tiles;
+      s = item / p.row_tiles;
+    };
+    cut(blockIdx.x, split, row, column);
+    cut(gridDim.x, split_step, row_step, column_step);
+  }
+  __device__ bool more(const Plan& p) const { return split < p.splits; }
+  __device__ void advance(const Plan& p) {
+    column += column_step;
+    row += row_step;
+    split += split_step;
+    if (column >= p.column_tiles) column -= p.column_tiles, ++row;
+    if (row >= p.row_tiles) row -= p.row_tiles, ++split;
+  }
+  __device__ int first_step(const Plan& p) const { return split * p.steps_per_split; }
+  __device__ int steps(const Plan& p) const {
+    return min(p.steps_per_split, p.steps - first_step(p));
+  }
 };
 
 template <int kN>
@@ -156,12 +195,12 @@ struct ProductShared {
   uint32_t tensor;
 };
 
-// A 16-byte word of a chunk's row, where TMA's swizzle has it: rows of 128 bytes or
-// of 64, whose words are exchanged so that eight rows' same words lie in different banks.
+// Where word 0 of a thread's row of a chunk is, in rows of 128 bytes or of 64; word w is
+// there with its number flipped into bits 4 and up. So TMA's swizzle has it: words are
+// exchanged so that eight rows' same words lie in different banks.
 template <int kBytes>
-__device__ __forceinline__ uint32_t word_of(uint32_t chunk, int row, int word) {
-  return kBytes == 128 ? chunk + row * 128 + ((word ^ (row & 7)) << 4)
-                       : chunk + row * 64 + ((word ^ (row >> 1 & 3)) << 4);
+__device__ __forceinline__ uint32_t row_of_chunk(uint32_t chunk, int row) {
+  return kBytes == 128 ? chunk + row * 128 + ((row & 7) << 4) : chunk + row * 64 + ((row >> 1 & 3) << 4);
 }
 __device__ __forceinline__ void put_word(uint32_t at, uint32_t a, uint32_t b, uint32_t c,
                                          uint32_t d) {
@@ -199,54 +238,52 @@ __device__ __forceinline__ void wait_stores_done() {
 // kWide 16-bit columns pass through shared memory, from which TMA writes them; the
 // residual's come by TMA to the place of the results, a chunk ahead if two fit. Where
 // rows are no whole 16-byte words, a warp writes 32 columns of one row at a time instead.
-template <class T, int kN>
+template <class T, int kN, Form kForm>
 __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps& maps,
                          ProductShared<kN>& s, uint32_t tensor, int warp, int lane) {
   constexpr int kWide = ProductShared<kN>::kWide, kNarrowBytes = kWide * 2;
   constexpr int kParts = kWide / 32;  // steps of 32 columns of a 16-bit chunk
-  const int64_t tiles = int64_t{plan.row_tiles} * plan.column_tiles, items = tiles * plan.splits;
-  const bool wide = e.out_dtype == GS_FLOAT32;
-  const bool two = !e.slope;  // two chunks in turn; with slopes, one and its slopes
+  constexpr bool kAny = kForm == Form::kAny;
+  const bool wide = kAny ? e.out_dtype == GS_FLOAT32 : kForm == Form::kWide || kForm == Form::kStream;
+  const bool add = kAny ? e.residual != nullptr : kForm == Form::kStream;
+  const bool active = kAny || kForm == Form::kActive || kForm == Form::kTraining;
+  const bool slopes = kAny ? e.slope != nullptr : kForm == Form::kTraining;
+  const bool slope_float = kAny && e.slope_float;
+  const bool by_tma = !kAny || e.tiled;
+  const bool two = !slopes;  // two chunks in turn; with slopes, one and its slopes
   const uint32_t staged = shared_address(s.out[warp]);
   float* const biases = s.bias[warp];
-  struct Place {
-    int64_t item;
-    int c;  // step of 32 columns: kParts of them in a row, then the other warps' kParts
-  };
-  const int c0 = (warp >> 2) * kParts;
-  const auto column_of = [&](const Place& p) {
-    return static_cast<int>(p.item % tiles % plan.column_tiles) * kN + 32 * p.c;
-  };
-  const auto row_of = [&](const Place& p) {
-    return static_cast<int>(p.item % tiles / plan.column_tiles) * kRows + 32 * (warp & 3);
-  };
+  const int c0 = (warp >> 2) * kParts;  // the warp's first step; then every other chunk's
   const auto next_step = [&](int c) { return (c + 1) % kParts ? c + 1 : c + 1 + kParts; };
+  struct Place {
+    Walk walk;
+    int c;
+  };
+  const auto column_of = [&](const Place& p) { return p.walk.column * kN + 32 * p.c; };
+  const auto row_of = [&](const Place& p) { return p.walk.row * kRows + 32 * (warp & 3); };
   // The place, or the warp's next one, that has columns and starts a chunk.
   const auto chunk_from = [&](Place p) {
-    while (p.item < items && (p.c >= kN / 32 || column_of(p) >= e.columns))
-      p = {p.item + gridDim.x, c0};
+    while (p.walk.more(plan) && (p.c >= kN / 32 || column_of(p) >= e.columns)) {
+      p.walk.advance(plan);
+      p.c = c0;
+    }
     return p;
   };
-  const auto chunk_after = [&](Place p) {
-    p.c = wide ? next_step(p.c) : p.c + 2 * kParts;
-    return chunk_from(p);
-  };
   const auto load_residual = [&](const Place& p, uint32_t use) {
-    if (p.item >= items) return;
+    if (!p.walk.more(plan)) return;
     const uint32_t at = two ? use & 1 : 0;
     const uint32_t bar = shared_address(&s.residual[warp][at]);
     barrier_expect(bar, wide ? kChunkBytes : 32 * kNarrowBytes);
     load_box(staged + at * kChunkBytes, &maps.residual, column_of(p), row_of(p), bar);
   };
-  const bool by_tma = e.tiled, add = e.residual != nullptr;
   bool good = true;
   uint32_t use = 0;  // chunks done
-  if (by_tma && add && lane == 0) load_residual(chunk_from({blockIdx.x, c0}), 0);
-  uint32_t count = 0;
+  Walk walk(plan);
+  if (by_tma && add && lane == 0) load_residual(chunk_from({walk, c0}), 0);
   int bias_column = -1;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++count) {
+  for (uint32_t count = 0; walk.more(plan); walk.advance(plan), ++count) {
     const uint32_t buffer = count & 1;
-    const int n0 = column_of({item, 0});
+    const int n0 = walk.column * kN;
     if (e.bias && n0 != bias_column) {
       __syncwarp();
       for (int i = lane; i < kN; i += 32)
@@ -254,19 +291,20 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
       __syncwarp();
       bias_column = n0;
     }
-    const int row = row_of({item, 0});
-    const int64_t out_row = item / tiles * plan.split_rows + row;
+    const int row = walk.row * kRows + 32 * (warp & 3);
+    const int64_t out_row = walk.split * plan.split_rows + row;
     good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
     fence_after_sync();
+    const uint32_t sums = tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN;
+#pragma unroll 1
     for (int c = c0; c < kN / 32; c = next_step(c)) {
-      const Place p = {item, c};
       const int n = n0 + 32 * c;
       if (n >= e.columns) break;
       float2 z[16], slope[16];
-      load_columns32(tensor + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + buffer * kN + 32 * c,
-                     reinterpret_cast<float(&)[32]>(z));
+      load_columns32(sums + 32 * c, reinterpret_cast<float(&)[32]>(z));
       wait_loads();
       if (!good)
+#pragma unroll
         for (float2& x : z) x = both(NAN);
       if (e.bias)
 #pragma unroll
@@ -275,7 +313,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
           z[2 * i] = add2(z[2 * i], make_float2(b.x, b.y));
           z[2 * i + 1] = add2(z[2 * i + 1], make_float2(b.z, b.w));
         }
-      activate(e.activation, z, slope);
+      if (active) activate(e.activation, z, slope);
       const int part = c % kParts;  // of a 16-bit chunk
       if (by_tma) {
         const uint32_t at = two ? use & 1 : 0, chunk = staged + at * kChunkBytes;
@@ -284,7 +322,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
           if (lane == 0) {
             if (two && !add) wait_stores_read<1>();
             else wait_stores_read<0>();
-            if (add && two) load_residual(chunk_after(p), use + 1);
+            if (add && two) load_residual(chunk_from({walk, wide ? next_step(c) : c + 2 * kParts}), use + 1);
           }
           if (add)
             good = good && barrier_wait_warp(shared_address(&s.residual[warp][at]),
@@ -292,70 +330,76 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
           __syncwarp();
         }
         if (wide) {
+          const uint32_t to = row_of_chunk<128>(chunk, lane);
+          if (add)
 #pragma unroll
-          for (int w = 0; w < 8; ++w) {
-            const uint32_t word = word_of<128>(chunk, lane, w);
-            if (add) {
-              const uint4 r = get_word(word);
+            for (int w = 0; w < 8; ++w) {
+              const uint4 r = get_word(to ^ w << 4);
               z[2 * w] = add2(z[2 * w], make_float2(__uint_as_float(r.x), __uint_as_float(r.y)));
               z[2 * w + 1] = add2(z[2 * w + 1],
                                   make_float2(__uint_as_float(r.z), __uint_as_float(r.w)));
             }
-            put_word(word, __float_as_uint(z[2 * w].x), __float_as_uint(z[2 * w].y),
-                     __float_as_uint(z[2 * w + 1].x), __float_as_uint(z[2 * w + 1].y));
-          }
-        } else {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t word = word_of<kNarrowBytes>(chunk, lane, 4 * part + w);
-            if (add) {
-              const uint4 r = get_word(word);
+          for (int w = 0; w < 8; ++w)
+            put_word(to ^ w << 4, __float_as_uint(z[2 * w].x), __float_as_uint(z[2 * w].y),
+                     __float_as_uint(z[2 * w + 1].x), __float_as_uint(z[2 * w + 1].y));
+        } else {
+          const uint32_t to = row_of_chunk<kNarrowBytes>(chunk, lane) ^ part << 6;
+          if (add)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint4 r = get_word(to ^ w << 4);
               const T* v = reinterpret_cast<const T*>(&r);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 z[4 * w + k] = add2(z[4 * w + k],
                                     make_float2(to_float(v[2 * k]), to_float(v[2 * k + 1])));
             }
-            put_word(word, pack2<T>(z[4 * w].x, z[4 * w].y),
-                     pack2<T>(z[4 * w + 1].x, z[4 * w + 1].y),
-                     pack2<T>(z[4 * w + 2].x, z[4 * w + 2].y),
-                     pack2<T>(z[4 * w + 3].x, z[4 * w + 3].y));
-          }
+          uint32_t word[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) word[i] = pack2<T>(z[i].x, z[i].y);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            put_word(to ^ w << 4, word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]);
         }
-        if (e.slope && e.slope_float) {
+        if (slopes && slope_float) {
           if (!wide && part > 0) {  // the slopes of the chunk's part before
             if (lane == 0) wait_stores_read<0>();
             __syncwarp();
           }
+          const uint32_t to = row_of_chunk<128>(slope_chunk, lane);
 #pragma unroll
           for (int w = 0; w < 8; ++w)
-            put_word(word_of<128>(slope_chunk, lane, w), __float_as_uint(slope[2 * w].x),
-                     __float_as_uint(slope[2 * w].y), __float_as_uint(slope[2 * w + 1].x),
-                     __float_as_uint(slope[2 * w + 1].y));
-        } else if (e.slope) {
+            put_word(to ^ w << 4, __float_as_uint(slope[2 * w].x), __float_as_uint(slope[2 * w].y),
+                     __float_as_uint(slope[2 * w + 1].x), __float_as_uint(slope[2 * w + 1].y));
+        } else if (slopes) {
+          const uint32_t to = row_of_chunk<kNarrowBytes>(slope_chunk, lane) ^ part << 6;
+          uint32_t word[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) word[i] = slope_codes(slope[i]);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            put_word(word_of<kNarrowBytes>(slope_chunk, lane, 4 * part + w),
-                     slope_codes(slope[4 * w]), slope_codes(slope[4 * w + 1]),
-                     slope_codes(slope[4 * w + 2]), slope_codes(slope[4 * w + 3]));
+            put_word(to ^ w << 4, word[4 * w], word[4 * w + 1], word[4 * w + 2], word[4 * w + 3]);
         }
         const bool ends = part == kParts - 1 || n + 32 >= e.columns;  // a 16-bit chunk
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          if (row < e.rows) {
-            if (wide) store_box(&maps.out, n, static_cast<int>(out_row), chunk);
-            else if (ends) store_box(&maps.out, n - 32 * part, static_cast<int>(out_row), chunk);
-            if (e.slope && e.slope_float) store_box(&maps.slope, n, row, slope_chunk);
-            else if (e.slope && ends) store_box(&maps.slope, n - 32 * part, row, slope_chunk);
+        if (wide || ends || slope_float) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if (row < e.rows) {
+              if (wide) store_box(&maps.out, n, static_cast<int>(out_row), chunk);
+              else if (ends) store_box(&maps.out, n - 32 * part, static_cast<int>(out_row), chunk);
+              if (slopes && slope_float) store_box(&maps.slope, n, row, slope_chunk);
+              else if (slopes && ends) store_box(&maps.slope, n - 32 * part, row, slope_chunk);
+            }
+            commit_stores();
+            if (add && !two && (wide || ends)) {
+              wait_stores_read<0>();
+              load_residual(chunk_from({walk, wide ? next_step(c) : c - part + 2 * kParts}), use + 1);
+            }
           }
-          commit_stores();
-          if (add && !two && (wide || ends)) {
-            wait_stores_read<0>();
-            load_residual(chunk_after({item, c - (wide ? 0 : part)}), use + 1);
-          }
+          if (wide || ends) ++use;
         }
-        if (wide || ends) ++use;
       } else {
         float* const square = reinterpret_cast<float*>(s.out[warp]);
         const auto store = [&](const float2(&x)[16], auto&& put) {
@@ -373,10 +417,10 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
           if (add) y += read_as(e.residual, e.out_dtype, (row + r) * e.residual_stride + n + lane);
           write_as(e.out, e.out_dtype, (out_row + r) * e.out_stride + n + lane, y);
         });
-        if (e.slope)
+        if (slopes)
           store(slope, [&](int r, float x) {
             const int64_t to = (row + r) * e.slope_stride + n + lane;
-            if (e.slope_float) static_cast<float*>(e.slope)[to] = x;
+            if (slope_float) static_cast<float*>(e.slope)[to] = x;
             else static_cast<uint16_t*>(e.slope)[to] = static_cast<uint16_t>(slope_codes(both(x)));
           });
       }
@@ -392,7 +436,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
 }
 
 // kRowsA, kRowsB: the operand's contraction runs along its rows.
-template <class T, int kN, bool kRowsA, bool kRowsB>
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(Plan plan, Epilogue e, const __grid_constant__ CUtensorMap a_map,
                    const __grid_constant__ CUtensorMap b_map,
@@ -421,21 +465,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   __syncthreads();
   fence_after_sync();
   const uint32_t tensor = s.tensor;
-  const int64_t tiles = int64_t{plan.row_tiles} * plan.column_tiles, items = tiles * plan.splits;
   bool good = true;
-  const auto steps_of = [&](int64_t item) {
-    const int first = static_cast<int>(item / tiles) * plan.steps_per_split;
-    return min(plan.steps_per_split, plan.steps - first);
-  };
+  Walk walk(plan);
 
   if (warp == kEpilogueWarps) {  // loads
     if (lane == 0) {
       uint32_t turn = 0;  // stages used so far
-      for (int64_t item = blockIdx.x; item < items && good; item += gridDim.x) {
-        const int tile = static_cast<int>(item % tiles);
-        const int m0 = tile / plan.column_tiles * kRows, n0 = tile % plan.column_tiles * kN;
-        const int first = static_cast<int>(item / tiles) * plan.steps_per_split;
-        const int steps = steps_of(item);
+      for (; walk.more(plan) && good; walk.advance(plan)) {
+        const int m0 = walk.row * kRows, n0 = walk.column * kN;
+        const int first = walk.first_step(plan), steps = walk.steps(plan);
         for (int k = 0; k < steps; ++k, ++turn) {
           const uint32_t stage = turn % kStages, round = turn / kStages;
           if (round > 0) good = barrier_wait(shared_address(&s.empty[stage]), (round - 1) & 1);
@@ -465,10 +503,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
                                    : channels_word<kRows>(shared_address(s.a[0]));
     const uint32_t b_word = kRowsB ? rows_word<kDepth>(shared_address(s.b[0]))
                                    : channels_word<kN>(shared_address(s.b[0]));
-    uint32_t turn = 0, count = 0;
-    for (int64_t item = blockIdx.x; item < items && good; item += gridDim.x, ++count) {
+    uint32_t turn = 0;
+    for (uint32_t count = 0; walk.more(plan) && good; walk.advance(plan), ++count) {
       const uint32_t buffer = count & 1, round = count >> 1;
-      const int steps = steps_of(item);
+      const int steps = walk.steps(plan);
       if (round > 0)
         good = barrier_wait_warp(shared_address(&s.drained[buffer]), (round - 1) & 1);
       fence_after_sync();
@@ -489,7 +527,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       if (good) commit(elected, shared_address(&s.ready[buffer]));
     }
   } else {
-    good = epilogue<T, kN>(plan, e, maps, s, tensor, warp, lane);
+    good = epilogue<T, kN, kForm>(plan, e, maps, s, tensor, warp, lane);
   }
   if (!good) {  // let what is in flight land
     for (uint64_t& bar : s.full) barrier_settle(shared_address(&bar));
@@ -532,7 +570,7 @@ bool tma_rows(const void* data, int64_t stride, int32_t dtype, int64_t columns) 
   return is_aligned(data, 16) && stride * element_size(dtype) % 16 == 0 && stride >= columns;
 }
 
-template <class T, int kN, bool kRowsA, bool kRowsB>
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm>
 int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan,
                        const Epilogue& e, cudaStream_t stream) {
   CUtensorMap a_map, b_map;
@@ -551,12 +589,22 @@ int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const 
                            e.columns, e.slope_stride, kWide));
   }
   constexpr size_t kShared = sizeof(ProductShared<kN>);
-  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB>>(kShared)));
+  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB, kForm>>(kShared)));
   const int64_t items = int64_t{plan.row_tiles} * plan.column_tiles * plan.splits;
-  launch_chained_shared(product_kernel<T, kN, kRowsA, kRowsB>,
+  launch_chained_shared(product_kernel<T, kN, kRowsA, kRowsB, kForm>,
                         dim3(static_cast<unsigned>(items < kSmCount ? items : kSmCount)),
                         dim3(kProductThreads), kShared, stream, plan, e, a_map, b_map, maps);
   return check_launch();
+}
+
+// The form that an epilogue has.
+Form form_of(const Epilogue& e) {
+  if (!e.tiled) return Form::kAny;
+  const bool active = e.activation != GS_IDENTITY;
+  if (e.out_dtype == GS_FLOAT32)
+    return active || e.slope ? Form::kAny : e.residual ? Form::kStream : Form::kWide;
+  if (e.residual || (e.slope && e.slope_float)) return Form::kAny;
+  return !active ? Form::kNarrow : e.slope ? Form::kTraining : Form::kActive;
 }
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -585,17 +633,38 @@ int columns_of(int64_t rows, int64_t columns, int least) {
   return best;
 }
 
-// D = A B^T by `e`, with tiles of n columns.
+// D = A B^T by `e`, with tiles of n columns. The gradients' products have 16-bit results
+// or sums to be joined only.
 template <class T, bool kRowsA, bool kRowsB>
 int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan, int n,
                     const Epilogue& e, cudaStream_t stream) {
+  const auto formed = [&](auto columns) {
+    constexpr int kN = decltype(columns)::value;
+    switch (form_of(e)) {
+      case Form::kNarrow:
+        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow>(dtype, a, b, plan, e, stream);
+      case Form::kWide:
+        if constexpr (kRowsA || !kRowsB)
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide>(dtype, a, b, plan, e, stream);
+      case Form::kActive:
+        if constexpr (!kRowsB)
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive>(dtype, a, b, plan, e, stream);
+      case Form::kTraining:
+        if constexpr (!kRowsB)
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining>(dtype, a, b, plan, e, stream);
+      case Form::kStream:
+        if constexpr (!kRowsB)
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream>(dtype, a, b, plan, e, stream);
+      default: break;
+    }
+    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny>(dtype, a, b, plan, e, stream);
+  };
   switch (n) {
-    case 256: return launch_product<T, 256, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
-    case 128: return launch_product<T, 128, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
-    case 64: return launch_product<T, 64, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+    case 256: return formed(std::integral_constant<int, 256>{});
+    case 128: return formed(std::integral_constant<int, 128>{});
+    case 64: return formed(std::integral_constant<int, 64>{});
     case 32:
-      if constexpr (!kRowsB)
-        return launch_product<T, 32, kRowsA, kRowsB>(dtype, a, b, plan, e, stream);
+      if constexpr (!kRowsB) return formed(std::integral_constant<int, 32>{});
   }
   return GS_ERR_UNSUPPORTED;
 }
