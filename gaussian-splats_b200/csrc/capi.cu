@@ -49,6 +49,7 @@ int32_t launch_linear(const gs_linear_args&, cudaStream_t);
 int32_t launch_linear_backward(const gs_linear_args&, cudaStream_t);
 uint64_t linear_workspace_size(const gs_linear_args&);
 int32_t linear_status(cudaStream_t);
+int32_t launch_align_rows(int64_t, int64_t, const void*, int64_t, void*, cudaStream_t);
 uint64_t bin_count_workspace_size(int64_t);
 uint64_t bin_sort_workspace_size(int64_t, int64_t, const gs_params&);
 uint64_t bin_error_word_offset();
@@ -641,6 +642,11 @@ int32_t gs_linear(const gs_linear_args* args, gs_stream_t stream) {
 
 int32_t gs_linear_backward(const gs_linear_args* args, gs_stream_t stream) {
   return args ? gs::launch_linear_backward(*args, as_cuda(stream)) : GS_ERR_INVALID_ARGUMENT;
+}
+
+int32_t gs_align_rows(int64_t rows, int64_t channels, const void* from, int64_t from_stride,
+                      void* to, gs_stream_t stream) {
+  return gs::launch_align_rows(rows, channels, from, from_stride, to, as_cuda(stream));
 }
 
 int32_t gs_linear_status(gs_stream_t stream) { return gs::linear_status(as_cuda(stream)); }

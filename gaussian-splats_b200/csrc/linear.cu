@@ -680,31 +680,33 @@ struct Strips {
   int64_t rows, count;  // of a strip; strips
 };
 
-// N floats of a row at `p`, of which `valid` exist.
-template <class G>
-__device__ __forceinline__ void load_row(const G* p, int valid, bool aligned, float (&x)[8]) {
-  if (aligned && valid >= 8) {
-    if constexpr (sizeof(G) == 4) {
-      float lo[4], hi[4];
-      load_pack<4>(p, lo);
-      load_pack<4>(p + 4, hi);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = lo[k], x[4 + k] = hi[k];
-    } else {
-      load_pack<8>(p, x);
-    }
-  } else {
+// Eight floats of a row at `p`, of which `valid` exist.
+template <bool kWhole, class G>
+__device__ __forceinline__ void load_row(const G* p, int valid, float (&x)[8]) {
+  if constexpr (!kWhole) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = k < valid ? to_float(p[k]) : 0.0f;
+  } else if constexpr (sizeof(G) == 4) {
+    float lo[4], hi[4];
+    load_pack<4>(p, lo);
+    load_pack<4>(p + 4, hi);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = lo[k], x[4 + k] = hi[k];
+  } else {
+    load_pack<8>(p, x);
   }
 }
 
+enum class Slopes { kNone, kCodes, kFloats };
+
 // dz = grad_y act'(z) rounded to the operands' type, and each strip's sums of its columns
-// (of what was not rounded). A thread has eight columns of every so many rows.
-template <class T, class G>
-__global__ void __launch_bounds__(kSlopeThreads)
-    slope_kernel(gs_linear_args a, Strips cut, int64_t stride, bool slope_float, bool aligned,
-                 T* dz, float* sums) {
+// (of what was not rounded). A thread has eight columns of every so many rows, and loads
+// several rows before it works on the first: memory is the bound (65,536 x 4096 in
+// float16: 1.6 GB). kWhole: rows are whole 16-byte words.
+template <class T, class G, Slopes kSlopes, bool kWhole>
+__global__ void __launch_bounds__(kSlopeThreads, 3)
+    slope_kernel(gs_linear_args a, Strips cut, int64_t stride, T* __restrict__ dz,
+                 float* __restrict__ sums) {
   chain_wait();
   __shared__ float joined[kSlopeThreads][8 + 1];
   const int lane = threadIdx.x % cut.lanes, first = threadIdx.x / cut.lanes;
@@ -712,42 +714,56 @@ __global__ void __launch_bounds__(kSlopeThreads)
   const int64_t column = (blockIdx.y * int64_t{cut.lanes} + lane) * 8;
   const int valid = static_cast<int>(min(int64_t{8}, a.outputs - column));
   const int64_t row0 = blockIdx.x * cut.rows, end = min(row0 + cut.rows, a.rows);
+  const G* __restrict__ const grad = static_cast<const G*>(a.grad_y) + column;
   float sum[8] = {};
   if (valid > 0) {
-    const G* const grad = static_cast<const G*>(a.grad_y);
-    // Several rows' loads before the first one's arithmetic.
-    constexpr int kBatch = 4;
+    constexpr int kBatch = sizeof(G) == 4 || kSlopes == Slopes::kFloats ? 4 : 6;
     for (int64_t m0 = row0 + first; m0 < end; m0 += kBatch * step) {
-      float g[kBatch][8];
+      Pack<G, 8> g[kBatch];
       uint4 codes[kBatch];
+      float exact[kBatch][8];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int64_t m = min(m0 + i * step, a.rows - 1);
-        load_row(grad + m * a.outputs + column, valid, aligned, g[i]);
-        if (a.slope && !slope_float)
-          codes[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.slope) +
-                                                          m * stride + column));
+        const int64_t m = min(m0 + i * step, end - 1);
+        if constexpr (kWhole) {
+          if constexpr (sizeof(G) == 4) {
+            reinterpret_cast<uint4*>(&g[i])[0] = __ldcs(reinterpret_cast<const uint4*>(grad + m * a.outputs));
+            reinterpret_cast<uint4*>(&g[i])[1] = __ldcs(reinterpret_cast<const uint4*>(grad + m * a.outputs) + 1);
+          } else {
+            reinterpret_cast<uint4&>(g[i]) = __ldcs(reinterpret_cast<const uint4*>(grad + m * a.outputs));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            g[i].v[k] = k < valid ? grad[m * a.outputs + k] : from_float<G>(0.0f);
+        }
+        if constexpr (kSlopes == Slopes::kCodes)
+          codes[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.slope) +
+                                                           m * stride + column));
+        if constexpr (kSlopes == Slopes::kFloats)
+          load_row<true>(static_cast<const float*>(a.slope) + m * stride + column, 8, exact[i]);
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int64_t m = m0 + i * step;
         if (m >= end) break;
-        if (a.slope && slope_float) {
-          float x[8];
-          load_row(static_cast<const float*>(a.slope) + m * stride + column, 8, true, x);
+        float x[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) g[i][k] = k < valid ? g[i][k] * x[k] : 0.0f;
-        } else if (a.slope) {
+        for (int k = 0; k < 8; ++k) x[k] = to_float(g[i].v[k]);
+        if constexpr (kSlopes == Slopes::kCodes) {
           const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float x = slope_value(k & 1 ? words[k >> 1] >> 16 : words[k >> 1] & 0xffffu);
-            g[i][k] = k < valid ? g[i][k] * x : 0.0f;
+            const float slope = slope_value(__byte_perm(words[k >> 1], 0, k & 1 ? 0x4432 : 0x4410));
+            x[k] = kWhole || k < valid ? x[k] * slope : 0.0f;
           }
         }
+        if constexpr (kSlopes == Slopes::kFloats)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] += g[i][k];
-        if (dz) store_pack<8>(dz + m * stride + column, g[i]);
+          for (int k = 0; k < 8; ++k) x[k] = kWhole || k < valid ? x[k] * exact[i][k] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] += x[k];
+        if (dz) store_pack<8>(dz + m * stride + column, x);
       }
     }
   }
@@ -807,6 +823,24 @@ __global__ void __launch_bounds__(kJoinThreads)
     store_pack<4>(to, x);
   } else {
     for (int k = 0; k < 4 && column + k < columns; ++k) to[k] = from_float<T>(x[k]);
+  }
+}
+
+// Rows of 16-bit elements at any 2-byte address, to rows of whole 16-byte words: a
+// word a thread.
+__global__ void __launch_bounds__(256)
+    align_kernel(int64_t rows, int channels, const uint16_t* __restrict__ from, int64_t from_stride,
+                 uint4* __restrict__ to, int words) {
+  chain_wait();
+  const int64_t total = rows * words;
+  for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += int64_t{gridDim.x} * 256) {
+    const int64_t row = i / words;
+    const int channel = static_cast<int>(i - row * words) * 8;
+    const uint16_t* const p = from + row * from_stride + channel;
+    uint32_t x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = channel + k < channels ? p[k] : 0;
+    to[i] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
   }
 }
 
@@ -891,6 +925,22 @@ uint64_t linear_workspace_size(const gs_linear_args& a) {
   return check_args(a) == GS_OK ? backward_plan(a).size : 0;
 }
 
+int32_t launch_align_rows(int64_t rows, int64_t channels, const void* from, int64_t from_stride,
+                          void* to, cudaStream_t stream) {
+  if (rows < 0 || rows > GS_MAX_SEQUENCE_TOKENS || channels < 1 ||
+      channels > GS_MAX_LINEAR_FEATURES || from_stride < 0)
+    return GS_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return GS_OK;
+  if (!from || !to) return GS_ERR_INVALID_ARGUMENT;
+  if (!is_aligned(from, 2) || !is_aligned(to, 16)) return GS_ERR_MISALIGNED;
+  const int words = static_cast<int>((channels + 7) / 8);
+  const int64_t blocks = (rows * words + 255) / 256;
+  launch_chained(align_kernel, static_cast<unsigned>(blocks < 16 * kSmCount ? blocks : 16 * kSmCount),
+                 256, stream, rows, static_cast<int>(channels), static_cast<const uint16_t*>(from),
+                 from_stride, static_cast<uint4*>(to), words);
+  return check_launch();
+}
+
 int32_t linear_status(cudaStream_t stream) { return take_timeout(g_timeout, stream); }
 
 int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
@@ -949,17 +999,26 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
     using T = decltype(t);
     if ((p.own_dz && products) || sums) {
       const dim3 grid(static_cast<unsigned>(p.strips.count), p.strips.column_blocks);
-      const bool slope_float = a.bias_dtype == GS_FLOAT32 && a.bias;
-      const bool aligned = a.outputs % 8 == 0;
-      gs_linear_args b = a;
-      if (a.activation == GS_IDENTITY) b.slope = nullptr;
       T* const to = p.own_dz && products ? static_cast<T*>(dz) : nullptr;
-      if (a.residual_dtype == GS_FLOAT32)
-        launch_chained(slope_kernel<T, float>, grid, kSlopeThreads, stream, b, p.strips,
-                       slope_stride(a), slope_float, aligned, to, sums);
-      else
-        launch_chained(slope_kernel<T, T>, grid, kSlopeThreads, stream, b, p.strips,
-                       slope_stride(a), slope_float, aligned, to, sums);
+      const auto launch = [&](auto g, auto slopes, auto whole) {
+        using G = decltype(g);
+        launch_chained(slope_kernel<T, G, decltype(slopes)::value, decltype(whole)::value>, grid,
+                       kSlopeThreads, stream, a, p.strips, slope_stride(a), to, sums);
+      };
+      const auto with_whole = [&](auto g, auto slopes) {
+        if (a.outputs % 8 == 0) launch(g, slopes, std::true_type{});
+        else launch(g, slopes, std::false_type{});
+      };
+      const auto with_slopes = [&](auto g) {
+        if (a.activation == GS_IDENTITY)
+          with_whole(g, std::integral_constant<Slopes, Slopes::kNone>{});
+        else if (a.bias && a.bias_dtype == GS_FLOAT32)
+          with_whole(g, std::integral_constant<Slopes, Slopes::kFloats>{});
+        else
+          with_whole(g, std::integral_constant<Slopes, Slopes::kCodes>{});
+      };
+      if (a.residual_dtype == GS_FLOAT32) with_slopes(float{});
+      else with_slopes(T{});
       GS_TRY(check_launch());
     }
     if (a.grad_bias) {

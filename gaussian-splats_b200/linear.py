@@ -30,8 +30,11 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
             t.data_ptr() % 16 == 0:
         return t
     rows, channels = t.shape
-    copy = t.new_empty((rows, -(-channels // 8) * 8))[:, :channels]
-    return copy.copy_(t)
+    if t.stride(1) != 1:
+        t = t.contiguous()
+    copy = t.new_empty((rows, -(-channels // 8) * 8))
+    call("gs_align_rows", t.device, rows, channels, t.data_ptr(), t.stride(0), copy.data_ptr())
+    return copy[:, :channels]
 
 
 def _arguments(x, weight, bias, **values):

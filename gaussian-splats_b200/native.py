@@ -85,6 +85,7 @@ EXPORTED_SYMBOLS = (
     "gs_rms_norm_backward",
     "gs_rms_norm_workspace_size",
     "gs_linear",
+    "gs_align_rows",
     "gs_linear_backward",
     "gs_linear_status",
     "gs_linear_workspace_size",
@@ -394,6 +395,7 @@ def lib() -> ctypes.CDLL:
         "gs_rms_norm_workspace_size": ([ctypes.POINTER(RmsNormArgs)], u64),
         "gs_linear": ([ctypes.POINTER(LinearArgs), vp], i32),
         "gs_linear_backward": ([ctypes.POINTER(LinearArgs), vp], i32),
+        "gs_align_rows": ([i64, i64, vp, i64, vp, vp], i32),
         "gs_linear_status": ([vp], i32),
         "gs_linear_workspace_size": ([ctypes.POINTER(LinearArgs)], u64),
         "gs_det_exp": ([i64, vp, vp, vp], i32),

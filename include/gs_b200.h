@@ -724,6 +724,11 @@ typedef struct gs_linear_args {
 uint64_t gs_linear_workspace_size(const gs_linear_args *args);
 int32_t gs_linear(const gs_linear_args *args, gs_stream_t stream);
 int32_t gs_linear_backward(const gs_linear_args *args, gs_stream_t stream);
+/* Rows of `channels` 16-bit elements (1 to GS_MAX_LINEAR_FEATURES), contiguous, from_stride
+ * elements apart, at any address their type allows, copied to rows of channels rounded up
+ * to 8, filled up with zeros, 16-byte aligned: an operand for gs_linear. */
+int32_t gs_align_rows(int64_t rows, int64_t channels, const void *from, int64_t from_stride,
+                      void *to, gs_stream_t stream);
 /* As gs_window_attention_status, for these products (the block's tiles hold NaN). */
 int32_t gs_linear_status(gs_stream_t stream);
 

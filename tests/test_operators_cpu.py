@@ -65,6 +65,16 @@ def test_linear_checks_arguments():
     assert lib.gs_linear_workspace_size(ctypes.byref(args)) > 2 ** 47
 
 
+def test_align_rows_checks_arguments():
+    from gaussian_splats_b200 import native
+
+    lib, a = native.lib(), 256
+    for status, bad in [(-1, (-1, 8, a, 8, a)), (-1, (4, 0, a, 8, a)), (-1, (4, 8, a, -8, a)),
+                        (-1, (4, 8, None, 8, a)), (-1, (4, 65537, a, 8, a)), (-5, (4, 8, a + 1, 8, a)),
+                        (-5, (4, 8, a, 8, a + 8)), (0, (0, 8, a, 8, a))]:
+        assert lib.gs_align_rows(*bad, None) == status, bad
+
+
 def test_clip_checks_arguments():
     from gaussian_splats_b200 import native
 
