@@ -4,9 +4,11 @@
 //   dz = grad_y act'(z),  dx = dz W,  dW = dz^T x,  db = sum of dz over the rows
 //
 // One product kernel makes all three products D = A B^T on the tensor cores: tiles of
-// 128 x kN, operands by TMA, sums in tensor memory. x W^T contracts along the channels
-// of both operands, dz W along W's rows, dz^T x along the rows of both (an operand's
-// descriptor says which, nothing is transposed).
+// 128 x kN a block, operands by TMA, sums in tensor memory. x W^T contracts along the
+// channels of both operands, dz W along W's rows, dz^T x along the rows of both (an
+// operand's descriptor says which, nothing is transposed).
+#include <algorithm>
+
 #include "tensorcore.cuh"
 
 namespace gs {
@@ -152,19 +154,19 @@ struct Plan {
   int64_t split_rows;       // rows of `out` from one split's sums to the next one's
 };
 
-// A block's items: its own, and every one that many blocks further.
+// A block's (or a pair's) items: its own, and every one that many blocks further.
 struct Walk {
   int32_t split, row, column;  // tiles
   int32_t split_step, row_step, column_step;
-  __device__ explicit Walk(const Plan& p) {
+  __device__ Walk(const Plan& p, int blocks) {
     const auto cut = [&](uint32_t item, int32_t& s, int32_t& r, int32_t& c) {
       c = item % p.column_tiles;
       item /= p.column_tiles;
       r = item % p.row_tiles;
       s = item / p.row_tiles;
     };
-    cut(blockIdx.x, split, row, column);
-    cut(gridDim.x, split_step, row_step, column_step);
+    cut(blockIdx.x / blocks, split, row, column);
+    cut(gridDim.x / blocks, split_step, row_step, column_step);
   }
   __device__ bool more(const Plan& p) const { return split < p.splits; }
   __device__ void advance(const Plan& p) {
@@ -180,10 +182,13 @@ struct Walk {
   }
 };
 
-template <int kN>
+// kPair: two blocks share a tile of 2 kRows x kN.
+template <int kN, bool kPair>
 struct ProductShared {
-  static constexpr int kStages = kN == 256 ? 3 : 4;
-  static constexpr int kABytes = kRows * kDepth * 2, kBBytes = kN * kDepth * 2;
+  static constexpr int kBRows = kPair ? kN / 2 : kN;  // of B here
+  static constexpr int kABytes = kRows * kDepth * 2, kBBytes = kBRows * kDepth * 2;
+  // As many as fit: narrow tiles are for few rows, whose time is the loads' latency.
+  static constexpr int kStages = kN == 256 ? (kPair ? 4 : 3) : kN == 128 ? 4 : kN == 64 ? 6 : 7;
   alignas(1024) unsigned char a[kStages][kABytes];
   alignas(1024) unsigned char b[kStages][kBBytes];
   alignas(1024) unsigned char out[kEpilogueWarps][2][kChunkBytes];
@@ -238,10 +243,13 @@ __device__ __forceinline__ void wait_stores_done() {
 // kWide 16-bit columns pass through shared memory, from which TMA writes them; the
 // residual's come by TMA to the place of the results, a chunk ahead if two fit. Where
 // rows are no whole 16-byte words, a warp writes 32 columns of one row at a time instead.
-template <class T, int kN, Form kForm>
+template <class T, int kN, Form kForm, bool kPair>
 __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps& maps,
-                         ProductShared<kN>& s, uint32_t tensor, int warp, int lane) {
-  constexpr int kWide = ProductShared<kN>::kWide, kNarrowBytes = kWide * 2;
+                         ProductShared<kN, kPair>& s, uint32_t tensor, int warp, int lane) {
+  constexpr int kWide = ProductShared<kN, kPair>::kWide, kNarrowBytes = kWide * 2;
+  // The block's rows of a tile.
+  constexpr int kTileRows = kPair ? 2 * kRows : kRows;
+  const int row_in_tile = 32 * (warp & 3) + (kPair ? kRows * static_cast<int>(pair_rank()) : 0);
   constexpr int kParts = kWide / 32;  // steps of 32 columns of a 16-bit chunk
   constexpr bool kAny = kForm == Form::kAny;
   const bool wide = kAny ? e.out_dtype == GS_FLOAT32 : kForm == Form::kWide || kForm == Form::kStream;
@@ -260,7 +268,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
     int c;
   };
   const auto column_of = [&](const Place& p) { return p.walk.column * kN + 32 * p.c; };
-  const auto row_of = [&](const Place& p) { return p.walk.row * kRows + 32 * (warp & 3); };
+  const auto row_of = [&](const Place& p) { return p.walk.row * kTileRows + row_in_tile; };
   // The place, or the warp's next one, that has columns and starts a chunk.
   const auto chunk_from = [&](Place p) {
     while (p.walk.more(plan) && (p.c >= kN / 32 || column_of(p) >= e.columns)) {
@@ -278,7 +286,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
   };
   bool good = true;
   uint32_t use = 0;  // chunks done
-  Walk walk(plan);
+  Walk walk(plan, kPair ? 2 : 1);
   if (by_tma && add && lane == 0) load_residual(chunk_from({walk, c0}), 0);
   int bias_column = -1;
   for (uint32_t count = 0; walk.more(plan); walk.advance(plan), ++count) {
@@ -291,7 +299,7 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
       __syncwarp();
       bias_column = n0;
     }
-    const int row = walk.row * kRows + 32 * (warp & 3);
+    const int row = walk.row * kTileRows + row_in_tile;
     const int64_t out_row = walk.split * plan.split_rows + row;
     good = good && barrier_wait_warp(shared_address(&s.ready[buffer]), count >> 1 & 1);
     fence_after_sync();
@@ -427,7 +435,11 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
     }
     fence_before_sync();
     __syncwarp();
-    if (lane == 0) barrier_arrive(shared_address(&s.drained[buffer]));
+    if (lane == 0) {
+      const uint32_t bar = shared_address(&s.drained[buffer]);
+      if constexpr (kPair) barrier_arrive_cluster(of_first_block(bar));
+      else barrier_arrive(bar);
+    }
   }
   if (lane == 0) wait_stores_done();
   if (!good)
@@ -436,12 +448,12 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
 }
 
 // kRowsA, kRowsB: the operand's contraction runs along its rows.
-template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm>
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair>
 __global__ void __launch_bounds__(kProductThreads, 1)
     product_kernel(Plan plan, Epilogue e, const __grid_constant__ CUtensorMap a_map,
                    const __grid_constant__ CUtensorMap b_map,
                    const __grid_constant__ EpilogueMaps maps) {
-  using Shared = ProductShared<kN>;
+  using Shared = ProductShared<kN, kPair>;
   constexpr int kStages = Shared::kStages;
   extern __shared__ __align__(1024) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
@@ -454,57 +466,73 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       barrier_init(shared_address(&s.ready[i]), 1);
-      barrier_init(shared_address(&s.drained[i]), kEpilogueWarps);
+      barrier_init(shared_address(&s.drained[i]), kPair ? 2 * kEpilogueWarps : kEpilogueWarps);
       for (int w = 0; w < kEpilogueWarps; ++w) barrier_init(shared_address(&s.residual[w][i]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_shared();
   }
-  if (warp == kEpilogueWarps + 1) tensor_alloc<2 * kN>(shared_address(&s.tensor));
+  if (warp == kEpilogueWarps + 1) {
+    if constexpr (kPair) tensor_alloc_pair<2 * kN>(shared_address(&s.tensor));
+    else tensor_alloc<2 * kN>(shared_address(&s.tensor));
+  }
   fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) pair_sync();  // both blocks' barriers are ready
   fence_after_sync();
   const uint32_t tensor = s.tensor;
+  const int rank = kPair ? static_cast<int>(pair_rank()) : 0;
   bool good = true;
-  Walk walk(plan);
+  Walk walk(plan, kPair ? 2 : 1);
 
   if (warp == kEpilogueWarps) {  // loads
     if (lane == 0) {
       uint32_t turn = 0;  // stages used so far
       for (; walk.more(plan) && good; walk.advance(plan)) {
-        const int m0 = walk.row * kRows, n0 = walk.column * kN;
+        const int m0 = (kPair ? 2 * walk.row + rank : walk.row) * kRows;
+        const int n0 = walk.column * kN + rank * Shared::kBRows;
         const int first = walk.first_step(plan), steps = walk.steps(plan);
         for (int k = 0; k < steps; ++k, ++turn) {
           const uint32_t stage = turn % kStages, round = turn / kStages;
           if (round > 0) good = barrier_wait(shared_address(&s.empty[stage]), (round - 1) & 1);
           if (!good) break;
-          const uint32_t bar = shared_address(&s.full[stage]);
+          uint32_t bar = shared_address(&s.full[stage]);
           const uint32_t a = shared_address(s.a[stage]), b = shared_address(s.b[stage]);
           const int k0 = (first + k) * kDepth;
-          barrier_expect(bar, Shared::kABytes + Shared::kBBytes);
+          if (rank == 0)
+            barrier_expect(bar, (kPair ? 2 : 1) * (Shared::kABytes + Shared::kBBytes));
+          if constexpr (kPair) bar = of_first_block(bar);
+          const auto load = [&](uint32_t to, const CUtensorMap* map, int x, int r) {
+            if constexpr (kPair) load_box_pair(to, map, x, r, bar);
+            else load_box(to, map, x, r, bar);
+          };
           if constexpr (kRowsA)
             for (int i = 0; i < kRows / 64; ++i)
-              load_box(a + i * kDepth * 128, &a_map, m0 + 64 * i, k0, bar);
+              load(a + i * kDepth * 128, &a_map, m0 + 64 * i, k0);
           else
-            load_box(a, &a_map, k0, m0, bar);
+            load(a, &a_map, k0, m0);
           if constexpr (kRowsB)
-            for (int i = 0; i < kN / 64; ++i)
-              load_box(b + i * kDepth * 128, &b_map, n0 + 64 * i, k0, bar);
+            for (int i = 0; i < Shared::kBRows / 64; ++i)
+              load(b + i * kDepth * 128, &b_map, n0 + 64 * i, k0);
           else
-            load_box(b, &b_map, k0, n0, bar);
+            load(b, &b_map, k0, n0);
         }
       }
+      if constexpr (kPair)  // the first block's products no longer signal to this one
+        for (uint32_t last = turn > kStages ? turn - kStages : 0; last < turn && good; ++last)
+          good = barrier_wait(shared_address(&s.empty[last % kStages]), last / kStages & 1);
     }
     __syncwarp();
   } else if (warp == kEpilogueWarps + 1) {  // products
     const uint32_t elected = elect_lane();
-    const uint32_t kind = product_kind<T>(kN, kRowsB) | (kRowsA ? 1u << 15 : 0u);
+    const uint32_t kind = (kPair ? product_kind_pair<T>(kN, kRowsB) : product_kind<T>(kN, kRowsB)) |
+                          (kRowsA ? 1u << 15 : 0u);
     const uint32_t a_word = kRowsA ? rows_word<kDepth>(shared_address(s.a[0]))
                                    : channels_word<kRows>(shared_address(s.a[0]));
     const uint32_t b_word = kRowsB ? rows_word<kDepth>(shared_address(s.b[0]))
-                                   : channels_word<kN>(shared_address(s.b[0]));
+                                   : channels_word<Shared::kBRows>(shared_address(s.b[0]));
     uint32_t turn = 0;
-    for (uint32_t count = 0; walk.more(plan) && good; walk.advance(plan), ++count) {
+    for (uint32_t count = 0; rank == 0 && walk.more(plan) && good; walk.advance(plan), ++count) {
       const uint32_t buffer = count & 1, round = count >> 1;
       const int steps = walk.steps(plan);
       if (round > 0)
@@ -518,16 +546,24 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         const uint32_t a = a_word + stage * (Shared::kABytes >> 4);
         const uint32_t b = b_word + stage * (Shared::kBBytes >> 4);
 #pragma unroll
-        for (int i = 0; i < kDepth / 16; ++i)
-          multiply(elected, tensor + buffer * kN,
-                   a + (kRowsA ? rows_step(i) : channels_step<kRows>(i)),
-                   b + (kRowsB ? rows_step(i) : channels_step<kN>(i)), kind, k > 0 || i > 0);
-        commit(elected, shared_address(&s.empty[stage]));
+        for (int i = 0; i < kDepth / 16; ++i) {
+          const uint32_t a_step = a + (kRowsA ? rows_step(i) : channels_step<kRows>(i));
+          const uint32_t b_step = b + (kRowsB ? rows_step(i) : channels_step<Shared::kBRows>(i));
+          if constexpr (kPair)
+            multiply_pair(elected, tensor + buffer * kN, a_step, b_step, kind, k > 0 || i > 0);
+          else
+            multiply(elected, tensor + buffer * kN, a_step, b_step, kind, k > 0 || i > 0);
+        }
+        if constexpr (kPair) commit_pair(elected, shared_address(&s.empty[stage]));
+        else commit(elected, shared_address(&s.empty[stage]));
       }
-      if (good) commit(elected, shared_address(&s.ready[buffer]));
+      if (good) {
+        if constexpr (kPair) commit_pair(elected, shared_address(&s.ready[buffer]));
+        else commit(elected, shared_address(&s.ready[buffer]));
+      }
     }
   } else {
-    good = epilogue<T, kN, kForm>(plan, e, maps, s, tensor, warp, lane);
+    good = epilogue<T, kN, kForm, kPair>(plan, e, maps, s, tensor, warp, lane);
   }
   if (!good) {  // let what is in flight land
     for (uint64_t& bar : s.full) barrier_settle(shared_address(&bar));
@@ -537,8 +573,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) pair_sync();  // neither block needs the other's memory any more
   fence_after_sync();
-  if (warp == kEpilogueWarps + 1) tensor_free<2 * kN>(tensor);
+  if (warp == kEpilogueWarps + 1) {
+    if constexpr (kPair) tensor_free_pair<2 * kN>(tensor);
+    else tensor_free<2 * kN>(tensor);
+  }
 }
 
 // An operand: a [rows, channels] array of 16-bit elements, and whether the
@@ -570,16 +610,17 @@ bool tma_rows(const void* data, int64_t stride, int32_t dtype, int64_t columns) 
   return is_aligned(data, 16) && stride * element_size(dtype) % 16 == 0 && stride >= columns;
 }
 
-template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm>
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair>
 int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan,
                        const Epilogue& e, cudaStream_t stream) {
   CUtensorMap a_map, b_map;
   GS_TRY(encode_operand(&a_map, dtype, a, kRowsA ? kDepth : kRows));
-  GS_TRY(encode_operand(&b_map, dtype, b, kRowsB ? kDepth : kN));
+  using Shared = ProductShared<kN, kPair>;
+  GS_TRY(encode_operand(&b_map, dtype, b, kRowsB ? kDepth : Shared::kBRows));
   EpilogueMaps maps;
   if (e.tiled) {
     const int64_t out_rows = plan.splits > 1 ? plan.splits * plan.split_rows : e.rows;
-    constexpr int kWide = ProductShared<kN>::kWide;
+    constexpr int kWide = Shared::kWide;
     GS_TRY(encode_chunks(&maps.out, e.out_dtype, e.out, out_rows, e.columns, e.out_stride, kWide));
     if (e.residual)
       GS_TRY(encode_chunks(&maps.residual, e.out_dtype, e.residual, e.rows, e.columns,
@@ -588,12 +629,25 @@ int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const 
       GS_TRY(encode_chunks(&maps.slope, e.slope_float ? GS_FLOAT32 : GS_BFLOAT16, e.slope, e.rows,
                            e.columns, e.slope_stride, kWide));
   }
-  constexpr size_t kShared = sizeof(ProductShared<kN>);
-  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB, kForm>>(kShared)));
+  constexpr size_t kShared = sizeof(Shared);
+  constexpr int kBlocks = kPair ? 2 : 1;
+  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair>>(kShared)));
   const int64_t items = int64_t{plan.row_tiles} * plan.column_tiles * plan.splits;
-  launch_chained_shared(product_kernel<T, kN, kRowsA, kRowsB, kForm>,
-                        dim3(static_cast<unsigned>(items < kSmCount ? items : kSmCount)),
-                        dim3(kProductThreads), kShared, stream, plan, e, a_map, b_map, maps);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kBlocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = static_cast<unsigned>(kBlocks * std::min<int64_t>(items, kSmCount / kBlocks));
+  config.blockDim = kProductThreads;
+  config.dynamicSmemBytes = kShared;
+  config.stream = stream;
+  config.attrs = attr;
+  config.numAttrs = kPair ? 2 : 1;
+  cudaLaunchKernelEx(&config, product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair>, plan, e, a_map,
+                     b_map, maps);
   return check_launch();
 }
 
@@ -609,62 +663,79 @@ Form form_of(const Epilogue& e) {
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-Plan plan_of(int64_t rows, int64_t columns, int64_t depth, int n, int splits) {
+constexpr int kPairDepth = 512;
+
+// A tile: its columns, and whether a pair of blocks shares one of 2 kRows.
+struct ProductTile {
+  int columns;
+  bool pair;
+  int rows() const { return pair ? 2 * kRows : kRows; }
+  int workers() const { return pair ? kSmCount / 2 : kSmCount; }
+};
+
+Plan plan_of(int64_t rows, int64_t columns, int64_t depth, ProductTile tile, int splits) {
   Plan p = {};
-  p.row_tiles = static_cast<int32_t>(ceil_div(rows, kRows));
-  p.column_tiles = static_cast<int32_t>(ceil_div(columns, n));
+  p.row_tiles = static_cast<int32_t>(ceil_div(rows, tile.rows()));
+  p.column_tiles = static_cast<int32_t>(ceil_div(columns, tile.columns));
   p.steps = static_cast<int32_t>(ceil_div(depth, kDepth));
   p.steps_per_split = static_cast<int32_t>(ceil_div(p.steps, splits));
   p.splits = static_cast<int32_t>(ceil_div(p.steps, p.steps_per_split));
-  p.split_rows = int64_t{p.row_tiles} * kRows;
+  p.split_rows = int64_t{p.row_tiles} * tile.rows();
   return p;
 }
 
-// The tile's columns: those with which the multiprocessors' last turn ends first. A turn
-// takes a tile's columns and about 32 more for its start and end.
-int columns_of(int64_t rows, int64_t columns, int least) {
-  int best = 0;
+// The tile with which the multiprocessors' last turn ends first. A turn takes a tile's
+// columns and about 32 more for its start and end; a pair's takes three quarters as long
+// for its columns, whose half it stages, where the contraction is long enough that the
+// products and not the results bound it (131,101 x 256: contracting 1024, 93 us against 98;
+// 131,101 x 1024: contracting 256, 90 against 78).
+ProductTile tile_of(int64_t rows, int64_t columns, int64_t depth, int least) {
+  ProductTile best = {};
   int64_t best_time = 0;
-  for (int n = 256; n >= least; n /= 2) {
-    const int64_t tiles = int64_t{ceil_div(rows, kRows)} * ceil_div(columns, n);
-    const int64_t time = (tiles + kSmCount - 1) / kSmCount * (n + 32);
-    if (!best || time < best_time) best = n, best_time = time;
-  }
+  const auto consider = [&](ProductTile t, int64_t turn) {
+    const int64_t tiles = int64_t{ceil_div(rows, t.rows())} * ceil_div(columns, t.columns);
+    const int64_t time = (tiles + t.workers() - 1) / t.workers() * turn;
+    if (!best.columns || time < best_time) best = t, best_time = time;
+  };
+  if (depth >= kPairDepth) consider({256, true}, 192 + 32);
+  for (int n = 256; n >= least; n /= 2) consider({n, false}, n + 32);
   return best;
 }
 
-// D = A B^T by `e`, with tiles of n columns. The gradients' products have 16-bit results
+// D = A B^T by `e`, in such tiles. The gradients' products have 16-bit results
 // or sums to be joined only.
 template <class T, bool kRowsA, bool kRowsB>
-int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan, int n,
+int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan, ProductTile tile,
                     const Epilogue& e, cudaStream_t stream) {
-  const auto formed = [&](auto columns) {
+  const auto formed = [&](auto columns, auto pair) {
     constexpr int kN = decltype(columns)::value;
+    constexpr bool kPair = decltype(pair)::value;
     switch (form_of(e)) {
       case Form::kNarrow:
-        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow>(dtype, a, b, plan, e, stream);
+        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow, kPair>(dtype, a, b, plan, e, stream);
       case Form::kWide:
         if constexpr (kRowsA || !kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide, kPair>(dtype, a, b, plan, e, stream);
       case Form::kActive:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive, kPair>(dtype, a, b, plan, e, stream);
       case Form::kTraining:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining, kPair>(dtype, a, b, plan, e, stream);
       case Form::kStream:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream, kPair>(dtype, a, b, plan, e, stream);
       default: break;
     }
-    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny>(dtype, a, b, plan, e, stream);
+    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny, kPair>(dtype, a, b, plan, e, stream);
   };
-  switch (n) {
-    case 256: return formed(std::integral_constant<int, 256>{});
-    case 128: return formed(std::integral_constant<int, 128>{});
-    case 64: return formed(std::integral_constant<int, 64>{});
+  if (tile.pair) return formed(std::integral_constant<int, 256>{}, std::true_type{});
+  switch (tile.columns) {
+    case 256: return formed(std::integral_constant<int, 256>{}, std::false_type{});
+    case 128: return formed(std::integral_constant<int, 128>{}, std::false_type{});
+    case 64: return formed(std::integral_constant<int, 64>{}, std::false_type{});
     case 32:
-      if constexpr (!kRowsB) return formed(std::integral_constant<int, 32>{});
+      if constexpr (!kRowsB) return formed(std::integral_constant<int, 32>{}, std::false_type{});
   }
   return GS_ERR_UNSUPPORTED;
 }
@@ -780,54 +851,64 @@ __global__ void __launch_bounds__(kSlopeThreads, 3)
   }
 }
 
-// The strips' sums of a column, in one order: 8 groups of strips, then the groups.
-__global__ void __launch_bounds__(256)
-    bias_kernel(const float* sums, int64_t strips, int columns, void* out, int dtype) {
-  chain_wait();
-  __shared__ float groups[8][33];
-  const int column = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
-  float sum = 0.0f;
-  if (column < columns)
-#pragma unroll 8
-    for (int64_t i = group; i < strips; i += 8) sum += sums[i * columns + column];
-  groups[group][threadIdx.x & 31] = sum;
-  __syncthreads();
-  if (group == 0 && column < columns) {
-    for (int g = 1; g < 8; ++g) sum += groups[g][threadIdx.x & 31];
-    write_as(out, dtype, column, sum);
-  }
-}
-
-// The splits' sums, in order, rounded to the result's type: four columns a thread.
-constexpr int kJoinThreads = 128;
+// What is left of the weight's and the bias's gradients, one launch: the splits' sums in
+// order, rounded to the result's type, four columns a thread; and, in the first blocks,
+// the strips' sums of 32 columns, in one order: 8 groups of strips, then the groups.
+constexpr int kJoinThreads = 256;
+struct Joins {
+  // the bias's: blocks, and strips of `outputs` sums
+  int32_t bias_blocks, outputs, bias_dtype;
+  int64_t strips;
+  const float* sums;
+  void* bias;
+  // the weight's
+  int32_t splits, rows, columns;
+  int64_t part_size;
+  const float* parts;
+  void* weight;
+};
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads)
-    join_kernel(const float* parts, int count, int64_t part_size, int rows, int columns, T* out) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Joins j) {
   chain_wait();
-  const int64_t at = blockIdx.x * int64_t{kJoinThreads} + threadIdx.x;
-  const int words = (columns + 3) / 4;
-  if (at >= int64_t{rows} * words) return;
+  if (blockIdx.x < j.bias_blocks) {
+    __shared__ float groups[8][33];
+    const int column = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+    float sum = 0.0f;
+    if (column < j.outputs)
+#pragma unroll 8
+      for (int64_t i = group; i < j.strips; i += 8) sum += j.sums[i * j.outputs + column];
+    groups[group][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (group == 0 && column < j.outputs) {
+      for (int g = 1; g < 8; ++g) sum += groups[g][threadIdx.x & 31];
+      write_as(j.bias, j.bias_dtype, column, sum);
+    }
+    return;
+  }
+  const int64_t at = (blockIdx.x - j.bias_blocks) * int64_t{kJoinThreads} + threadIdx.x;
+  const int words = (j.columns + 3) / 4;
+  if (at >= int64_t{j.rows} * words) return;
   float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-  for (int i = 0; i < count; ++i) {
-    const float4 x = reinterpret_cast<const float4*>(parts + i * part_size)[at];
+  for (int i = 0; i < j.splits; ++i) {
+    const float4 x = reinterpret_cast<const float4*>(j.parts + i * j.part_size)[at];
     sum.x += x.x;
     sum.y += x.y;
     sum.z += x.z;
     sum.w += x.w;
   }
   const int column = static_cast<int>(at % words) * 4;
-  T* const to = out + at / words * columns + column;
+  T* const to = static_cast<T*>(j.weight) + at / words * j.columns + column;
   const float x[4] = {sum.x, sum.y, sum.z, sum.w};
-  if (columns % 4 == 0) {
+  if (j.columns % 4 == 0) {
     store_pack<4>(to, x);
   } else {
-    for (int k = 0; k < 4 && column + k < columns; ++k) to[k] = from_float<T>(x[k]);
+    for (int k = 0; k < 4 && column + k < j.columns; ++k) to[k] = from_float<T>(x[k]);
   }
 }
 
 // Rows of 16-bit elements at any 2-byte address, to rows of whole 16-byte words: a
-// word a thread.
+// word a thread, from the four or five 4-byte words that its elements lie in.
 __global__ void __launch_bounds__(256)
     align_kernel(int64_t rows, int channels, const uint16_t* __restrict__ from, int64_t from_stride,
                  uint4* __restrict__ to, int words) {
@@ -836,11 +917,21 @@ __global__ void __launch_bounds__(256)
   for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += int64_t{gridDim.x} * 256) {
     const int64_t row = i / words;
     const int channel = static_cast<int>(i - row * words) * 8;
+    const int valid = min(8, channels - channel);
     const uint16_t* const p = from + row * from_stride + channel;
-    uint32_t x[8];
+    const bool odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
+    const uint32_t* const w = reinterpret_cast<const uint32_t*>(p - odd);
+    const int last = valid + odd;  // elements from w on
+    uint32_t x[5];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = channel + k < channels ? p[k] : 0;
-    to[i] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+    for (int k = 0; k < 5; ++k) x[k] = 2 * k < last ? w[k] : 0;
+    uint32_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      y[k] = odd ? __byte_perm(x[k], x[k + 1], 0x5432) : x[k];
+      if (2 * k + 1 >= valid) y[k] = 2 * k < valid ? y[k] & 0xffffu : 0;
+    }
+    to[i] = make_uint4(y[0], y[1], y[2], y[3]);
   }
 }
 
@@ -873,7 +964,7 @@ int64_t slope_stride(const gs_linear_args& a) { return round_up(a.outputs, 8); }
 struct BackwardPlan {
   bool own_dz;
   Strips strips;
-  int columns, x_columns;
+  ProductTile weight_tile, x_tile;
   Plan weight, x;
   uint64_t dz, sums, parts, size;  // byte offsets, and the whole
 };
@@ -897,14 +988,16 @@ BackwardPlan backward_plan(const gs_linear_args& a) {
   p.strips = strips_of(a.rows, a.outputs);
   // The weight's gradient has few tiles and a long contraction: split so that the items
   // are about one a multiprocessor.
-  p.columns = 256;
-  while (p.columns > 64 && p.columns / 2 >= a.inputs) p.columns /= 2;
-  const int64_t tiles = int64_t{ceil_div(a.outputs, kRows)} * ceil_div(a.inputs, p.columns);
-  const int64_t splits = kSmCount / tiles;
-  p.weight = plan_of(a.outputs, a.inputs, a.rows, p.columns,
+  p.weight_tile = {256, a.rows >= kPairDepth && a.outputs > kRows && a.inputs > 128};
+  while (p.weight_tile.columns > 64 && p.weight_tile.columns / 2 >= a.inputs)
+    p.weight_tile.columns /= 2;
+  const int64_t tiles = int64_t{ceil_div(a.outputs, p.weight_tile.rows())} *
+                        ceil_div(a.inputs, p.weight_tile.columns);
+  const int64_t splits = p.weight_tile.workers() / tiles;
+  p.weight = plan_of(a.outputs, a.inputs, a.rows, p.weight_tile,
                      static_cast<int>(splits < 1 ? 1 : splits));
-  p.x_columns = columns_of(a.rows, a.inputs, 64);
-  p.x = plan_of(a.rows, a.inputs, a.outputs, p.x_columns, 1);
+  p.x_tile = tile_of(a.rows, a.inputs, a.outputs, 64);
+  p.x = plan_of(a.rows, a.inputs, a.outputs, p.x_tile, 1);
   uint64_t at = 0;
   const auto take = [&](uint64_t bytes) {
     const uint64_t from = at;
@@ -964,12 +1057,12 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   e.tiled = tma_rows(a.y, a.outputs, a.residual_dtype, a.outputs) &&
             (!a.residual ||
              tma_rows(a.residual, a.residual_stride, a.residual_dtype, a.outputs));
-  const int n = columns_of(a.rows, a.outputs, 32);
+  const ProductTile tile = tile_of(a.rows, a.outputs, a.inputs, 32);
   return with_sixteen_bit(a.dtype, [&](auto t) {
     return run_product<decltype(t), false, false>(
         a.dtype, {a.x, a.rows, a.inputs, a.x_stride},
         {a.weight, a.outputs, a.inputs, a.weight_stride},
-        plan_of(a.rows, a.outputs, a.inputs, n, 1), n, e, stream);
+        plan_of(a.rows, a.outputs, a.inputs, tile, 1), tile, e, stream);
   });
 }
 
@@ -1021,11 +1114,14 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
       else with_slopes(T{});
       GS_TRY(check_launch());
     }
+    Joins j = {};
     if (a.grad_bias) {
-      launch_chained(bias_kernel, ceil_div(a.outputs, 32), 256, stream,
-                     static_cast<const float*>(sums), p.strips.count, a.outputs, a.grad_bias,
-                     a.bias_dtype);
-      GS_TRY(check_launch());
+      j.bias_blocks = ceil_div(a.outputs, 32);
+      j.outputs = a.outputs;
+      j.bias_dtype = a.bias_dtype;
+      j.strips = p.strips.count;
+      j.sums = sums;
+      j.bias = a.grad_bias;
     }
     if (a.grad_x) {
       Epilogue e = {};
@@ -1037,7 +1133,7 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
       e.tiled = tma_rows(a.grad_x, a.inputs, a.dtype, a.inputs);
       GS_TRY((run_product<T, false, true>(a.dtype, dz_operand,
                                           {a.weight, a.outputs, a.inputs, a.weight_stride}, p.x,
-                                          p.x_columns, e, stream)));
+                                          p.x_tile, e, stream)));
     }
     if (a.grad_weight) {
       Epilogue e = {};
@@ -1049,16 +1145,21 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
       e.out_dtype = whole ? a.dtype : GS_FLOAT32;
       e.tiled = tma_rows(e.out, e.out_stride, e.out_dtype, a.inputs);
       GS_TRY((run_product<T, true, true>(a.dtype, dz_operand,
-                                         {a.x, a.rows, a.inputs, a.x_stride}, p.weight, p.columns,
+                                         {a.x, a.rows, a.inputs, a.x_stride}, p.weight, p.weight_tile,
                                          e, stream)));
       if (!whole) {
-        const int64_t vectors = int64_t{a.outputs} * ceil_div(a.inputs, 4);
-        launch_chained(join_kernel<T>, ceil_div(vectors, kJoinThreads), kJoinThreads, stream,
-                       static_cast<const float*>(parts), p.weight.splits,
-                       p.weight.split_rows * round_up(a.inputs, 4), a.outputs, a.inputs,
-                       static_cast<T*>(a.grad_weight));
-        GS_TRY(check_launch());
+        j.splits = p.weight.splits;
+        j.rows = a.outputs;
+        j.columns = a.inputs;
+        j.part_size = p.weight.split_rows * round_up(a.inputs, 4);
+        j.parts = parts;
+        j.weight = a.grad_weight;
       }
+    }
+    const int64_t words = int64_t{j.rows} * ceil_div(j.columns, 4);
+    if (const unsigned blocks = j.bias_blocks + ceil_div(words, kJoinThreads)) {
+      launch_chained(join_kernel<T>, blocks, kJoinThreads, stream, j);
+      GS_TRY(check_launch());
     }
     return static_cast<int32_t>(GS_OK);
   });

@@ -1,4 +1,4 @@
-// The 5th-generation tensor cores as attention.cu uses them: tiles loaded by
+// The 5th-generation tensor cores as attention.cu and linear.cu use them: tiles loaded by
 // TMA into 128-byte-swizzled shared memory, products issued by one thread
 // (tcgen05.mma, 16-bit operands, float accumulators in tensor memory), results
 // read back a row a thread.
@@ -233,6 +233,76 @@ __device__ __forceinline__ void commit(uint32_t elected, uint32_t bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
           bar),
       "r"(elected)
+      : "memory");
+}
+
+// --------------------------------------------------------- pairs of blocks
+//
+// The two blocks of a cluster work on one tile of 256 rows (cta_group::2): each has
+// its 128 rows of A and of the sums, and half of B, which the products read from both
+// blocks' shared memory, so that a block stages half of B for a whole tile. The first
+// block issues the products and gets the loads' arrivals of both.
+
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The first block's barrier (or other shared memory) at this block's address.
+__device__ __forceinline__ uint32_t of_first_block(uint32_t address) {
+  uint32_t there;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(address));
+  return there;
+}
+__device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Loads a box to this block; `bar` may be the first block's.
+__device__ __forceinline__ void load_box_pair(uint32_t dst, const CUtensorMap* map, int x, int row,
+                                              uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+      : "memory");
+}
+template <int kColumns>
+__device__ __forceinline__ void tensor_alloc_pair(uint32_t shared_slot) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   shared_slot),
+               "n"(kColumns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+template <int kColumns>
+__device__ __forceinline__ void tensor_free_pair(uint32_t address) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address),
+               "n"(kColumns));
+}
+// product_kind for 256 rows.
+template <class T>
+__device__ __forceinline__ uint32_t product_kind_pair(int n, bool rows_b) {
+  return product_kind<T>(n, rows_b) + ((256u >> 4) - (128u >> 4) << 24);
+}
+__device__ __forceinline__ void multiply_pair(uint32_t elected, uint32_t d, uint32_t a, uint32_t b,
+                                              uint32_t kind, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(descriptor(a)), "l"(descriptor(b)), "r"(kind), "r"(static_cast<uint32_t>(add)),
+      "r"(elected)
+      : "memory");
+}
+// The phases of both blocks' barriers at this address complete.
+__device__ __forceinline__ void commit_pair(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %2;\n\t}" ::"r"(bar),
+      "r"(elected), "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 
