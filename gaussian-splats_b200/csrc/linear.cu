@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kSlopeThreads, 3)
 // What is left of the weight's and the bias's gradients, one launch: the splits' sums in
 // order, rounded to the result's type, four columns a thread; and, in the first blocks,
 // the strips' sums of 32 columns, in one order: 8 groups of strips, then the groups.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kBiasColumns = 8;
 struct Joins {
   // the bias's: blocks, and strips of `outputs` sums
   int32_t bias_blocks, outputs, bias_dtype;
@@ -871,16 +871,16 @@ template <class T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Joins j) {
   chain_wait();
   if (blockIdx.x < j.bias_blocks) {
-    __shared__ float groups[8][33];
-    const int column = blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+    __shared__ float groups[32][9];
+    const int column = blockIdx.x * kBiasColumns + (threadIdx.x & 7), group = threadIdx.x >> 3;
     float sum = 0.0f;
     if (column < j.outputs)
 #pragma unroll 8
-      for (int64_t i = group; i < j.strips; i += 8) sum += j.sums[i * j.outputs + column];
-    groups[group][threadIdx.x & 31] = sum;
+      for (int64_t i = group; i < j.strips; i += 32) sum += j.sums[i * j.outputs + column];
+    groups[group][threadIdx.x & 7] = sum;
     __syncthreads();
     if (group == 0 && column < j.outputs) {
-      for (int g = 1; g < 8; ++g) sum += groups[g][threadIdx.x & 31];
+      for (int g = 1; g < 32; ++g) sum += groups[g][threadIdx.x & 7];
       write_as(j.bias, j.bias_dtype, column, sum);
     }
     return;
@@ -1116,7 +1116,7 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
     }
     Joins j = {};
     if (a.grad_bias) {
-      j.bias_blocks = ceil_div(a.outputs, 32);
+      j.bias_blocks = ceil_div(a.outputs, kBiasColumns);
       j.outputs = a.outputs;
       j.bias_dtype = a.bias_dtype;
       j.strips = p.strips.count;

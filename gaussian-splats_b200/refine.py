@@ -11,7 +11,8 @@ as they are meant to be used:
 * training and whole-scene inference: :meth:`SplatRefiner.forward`
 * one new Gaussian at a time (a scene that arrives as a stream):
   :meth:`SplatRefiner.stream` and :meth:`SplatRefiner.step`, for a causal refiner
-  (``right=0``)
+  (``right=0``); ``stream(batch, four_bit=True)`` holds the streams' keys and values
+  in 4 bits
 * 8-bit products for serving: :meth:`SplatRefiner.quantize`
 
 Activations are bfloat16, the residual stream float32.
@@ -25,7 +26,9 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
-from .attention import window_attention, window_attention_step, window_cache
+from .attention import (FourBitCache, window_attention, window_attention_step,
+                        window_attention_step_4bit, window_cache, window_cache_4bit)
+from .linear import linear
 from .norm import rms_norm, rms_norm_e4m3
 from .recurrence import gated_scan, gated_scan_step
 from .sequences import PackedSequences
@@ -90,7 +93,8 @@ class _Product(nn.Linear):
 @dataclass(frozen=True)
 class RefinerShape:
     """Sizes of a refiner. ``left`` and ``right``: the attention's window along
-    the order; ``first``: scene tokens, which stay visible."""
+    the order; ``first``: scene tokens, which stay visible; ``hidden``: channels of
+    a feed-forward layer beside each block's recurrence (0: none)."""
 
     width: int = 256
     blocks: int = 2
@@ -99,6 +103,27 @@ class RefinerShape:
     left: int = 256
     right: int = 256
     first: int = 4
+    hidden: int = 0
+
+
+class _FeedForward(nn.Module):
+    """``x + down(gelu(up(y)))``: both products with their epilogues."""
+
+    def __init__(self, width: int, hidden: int, device=None):
+        super().__init__()
+        self.up = _Product(width, hidden, device)
+        self.up_bias = nn.Parameter(torch.zeros(hidden, device=device, dtype=torch.bfloat16))
+        self.down = nn.Linear(hidden, width, device=device, dtype=torch.bfloat16)
+
+    def forward(self, y, x):
+        return self._down(linear(y, self.up.weight, self.up_bias, activation="gelu"), x)
+
+    def eight_bit(self, codes, scale, x):
+        z = self.up.eight_bit(codes, scale).float() + self.up_bias.float()
+        return self._down(nn.functional.gelu(z).bfloat16(), x)
+
+    def _down(self, hidden, x):
+        return linear(hidden, self.down.weight, self.down.bias, x)
 
 
 class _Block(nn.Module):
@@ -117,36 +142,47 @@ class _Block(nn.Module):
         self.attend_out = _Product(self.split[0], shape.width, device)
         self.mix = _Product(shape.width, 2 * shape.width, device)
         self.mix_out = _Product(shape.width, shape.width, device)
+        self.feed = _FeedForward(shape.width, shape.hidden, device) if shape.hidden else None
 
     def _normed(self, x, residual, weight, product):
-        """The product of the norm of ``x + residual``, and the sum."""
+        """The product of the norm of ``x + residual``, the sum, and the norm itself
+        (codes and scale where the products are in 8 bits)."""
         if product.codes is not None and not torch.is_grad_enabled():
             codes, scale, residual = rms_norm_e4m3(x, weight, residual)
-            return product.eight_bit(codes, scale), residual
+            return product.eight_bit(codes, scale), residual, (codes, scale)
         y, residual = rms_norm(x, weight, residual)
-        return product(y), residual
+        return product(y), residual, (y,)
+
+    def _fed(self, x, normed):
+        """``x`` and the feed-forward layer's output of the norm that the recurrence had."""
+        if self.feed is None:
+            return x
+        return self.feed(*normed, x) if len(normed) == 1 else self.feed.eight_bit(*normed, x)
 
     def _heads(self, qkv):
         return (t.unflatten(-1, (-1, self.dim)) for t in qkv.split(self.split, -1))
 
     def forward(self, x, residual, packed, valid):
         s = self.shape
-        qkv, residual = self._normed(x, residual, self.norm_attend, self.qkv)
+        qkv, residual, _ = self._normed(x, residual, self.norm_attend, self.qkv)
         x = window_attention(*self._heads(qkv), packed, left=s.left, right=s.right, first=s.first,
                              valid=valid)
         x = self.attend_out(x.flatten(1))
-        mix, residual = self._normed(x, residual, self.norm_mix, self.mix)
+        mix, residual, normed = self._normed(x, residual, self.norm_mix, self.mix)
         x, _ = gated_scan(*mix.chunk(2, -1), packed)
-        return self.mix_out(x), residual
+        return self._fed(self.mix_out(x), normed), residual
 
     def step(self, x, residual, positions, cache, state, valid, cache_valid):
-        qkv, residual = self._normed(x, residual, self.norm_attend, self.qkv)
-        x = window_attention_step(*self._heads(qkv), *cache, positions, first=self.shape.first,
-                                  valid=valid, cache_valid=cache_valid)
+        qkv, residual, _ = self._normed(x, residual, self.norm_attend, self.qkv)
+        slots = dict(first=self.shape.first, valid=valid, cache_valid=cache_valid)
+        if isinstance(cache, FourBitCache):
+            x = window_attention_step_4bit(*self._heads(qkv), cache, positions, **slots)
+        else:
+            x = window_attention_step(*self._heads(qkv), *cache, positions, **slots)
         x = self.attend_out(x.flatten(1))
-        mix, residual = self._normed(x, residual, self.norm_mix, self.mix)
+        mix, residual, normed = self._normed(x, residual, self.norm_mix, self.mix)
         x = gated_scan_step(*mix.chunk(2, -1), state)
-        return self.mix_out(x), residual
+        return self._fed(self.mix_out(x), normed), residual
 
 
 class SplatRefiner(nn.Module):
@@ -175,6 +211,8 @@ class SplatRefiner(nn.Module):
         for block in self.blocks:
             block.qkv.quantize()
             block.mix.quantize()
+            if block.feed is not None:
+                block.feed.up.quantize()
 
     def _features(self, splats: GaussianSplat) -> torch.Tensor:
         features = torch.cat([getattr(splats, name).flatten(1) for name in _NAMES], 1)
@@ -223,14 +261,17 @@ class SplatRefiner(nn.Module):
     # ------------------------------------------------------------- streams
 
     @torch.no_grad()
-    def stream(self, batch: int) -> dict:
-        """The state of ``batch`` streams that have seen the scene tokens."""
+    def stream(self, batch: int, four_bit: bool = False) -> dict:
+        """The state of ``batch`` streams that have seen the scene tokens. With
+        ``four_bit`` their keys and values are held in 4 bits: about a quarter of the
+        memory, at the price of their rounding."""
         if self.shape.right:
             raise ValueError("only a causal refiner (right=0) takes splats one by one")
         s, device = self.shape, self.scene.device
         alive = torch.zeros(batch, s.first + s.left + 1, dtype=torch.bool, device=device)
+        cache = window_cache_4bit if four_bit else window_cache
         state = {"length": 0, "alive": alive, "blocks": [
-            (window_cache(batch, s.left, s.first, s.kv_heads, block.dim, device=device),
+            (cache(batch, s.left, s.first, s.kv_heads, block.dim, device=device),
              torch.zeros(batch, s.width, device=device)) for block in self.blocks]}
         for token in self.scene:
             self._advance(token.expand(batch, -1).contiguous(), None, state)
