@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 // An item's parts joined in order, a block an item and head: the threads of a channel take
 // every so many parts. What is left of the time is latency, so what a thread needs first
 // is requested before it is known what it is multiplied by.
-constexpr int kMostParts = 256, kAhead = 8;
+constexpr int kMostParts = 128, kAhead = 8;  // at a time: threads of the smallest block
 template <class T, int kDim, int kSets>
 __global__ void __launch_bounds__(1024)
     join_kernel(gs_window_attention_step_4bit_args a, const Part<kDim, kSets>* parts,
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(1024)
   for (int i0 = 0; i0 < count; i0 += kMostParts) {
     __syncthreads();
     const int some = min(kMostParts, count - i0);
-    if (thread < some) {  // kMostParts threads at least
+    if (thread < some) {
       if (i0 > 0) top = from[i0 + thread].top[h], sum = from[i0 + thread].sum[h];
       scales[thread] = tc::exp2_approx(top - shift);
       sums[thread] = sum * scales[thread];
@@ -742,7 +742,8 @@ int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
                         parts, reach);
   GS_TRY(check_launch());
   // Threads by the parts of an item: few parts, many items; many parts, few items.
-  const int threads = blocks * kWarps >= 16 * items ? 1024 : 256;
+  const int64_t each = blocks * kWarps / items;
+  const int threads = each >= 16 ? 1024 : each >= 8 ? 256 : 128;
   launch_chained(join_kernel<T, kDim, kSets>,
                  dim3(static_cast<unsigned>(items), std::min(a.heads / a.kv_heads, 8 * kSets)),
                  threads, stream, a, static_cast<const P*>(parts),
