@@ -109,7 +109,10 @@ __device__ uint32_t g_timeout;
 constexpr int kRows = 128;   // of a tile
 constexpr int kDepth = 64;   // of a stage: 128 bytes of channels, or 64 rows
 constexpr int kEpilogueWarps = 8;
-constexpr int kProductThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kGatherWarps = 8;  // of 16 rows: a tile's are all on their way at once
+constexpr int product_threads(bool gather) {
+  return 32 * (kEpilogueWarps + 2 + (gather ? kGatherWarps : 0));
+}
 constexpr int kChunkBytes = 4096;  // of the epilogue: 32 rows of 128 bytes
 
 // What becomes of the sums D(m, n).
@@ -447,10 +450,56 @@ __device__ bool epilogue(const Plan& plan, const Epilogue& e, const EpilogueMaps
   return good;
 }
 
-// kRowsA, kRowsB: the operand's contraction runs along its rows.
-template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair>
-__global__ void __launch_bounds__(kProductThreads, 1)
-    product_kernel(Plan plan, Epilogue e, const __grid_constant__ CUtensorMap a_map,
+// An operand: a [rows, channels] array of 16-bit elements.
+struct Operand {
+  const void* data;
+  int64_t rows, channels, stride;
+};
+
+// Rows of A that TMA does not take (no whole 16-byte words): a warp loads a row's 64
+// channels at a time, two a lane, and puts them where TMA would have. All its rows
+// are requested before the first is put down. No copy of A is made for it: that
+// took a third of the time of a forward whose bound is its result (500,000 x 59 -> 256,
+// 90 us a pass).
+__device__ __forceinline__ void gather_rows(const Operand& a, int64_t row0, int k0, uint32_t tile,
+                                            int lane) {
+  constexpr int kBatch = kRows / kGatherWarps;
+  const int valid = static_cast<int>(min(int64_t{kDepth}, a.channels - k0));
+  const uint16_t* const data = static_cast<const uint16_t*>(a.data) + row0 * a.stride + k0;
+  const int rows = static_cast<int>(min(int64_t{kBatch}, a.rows - row0));
+  const auto odd = [&](int i) {  // 1 if row i starts in the middle of a 4-byte word
+    return static_cast<int>((reinterpret_cast<uintptr_t>(data) >> 1 ^ (i & a.stride)) & 1);
+  };
+  const auto words = [&](int i) {
+    return reinterpret_cast<const uint32_t*>(data + i * a.stride - odd(i));
+  };
+  uint32_t word[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i)
+    word[i] = i < rows && 2 * lane < valid + odd(i) ? __ldg(words(i) + lane) : 0;
+  // An odd row's 64th channel lies in a 33rd word: row i's is lane i's.
+  uint32_t more = 0;
+  if (lane < rows && odd(lane) && valid == kDepth) more = __ldg(words(lane) + 32);
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {  // eight rows' swizzle starts over with the warp's rows
+    uint32_t next = __shfl_down_sync(0xffffffffu, word[i], 1);
+    const uint32_t last = __shfl_sync(0xffffffffu, more, i);
+    if (lane == 31) next = last;
+    uint32_t two = odd(i) ? __byte_perm(word[i], next, 0x5432) : word[i];
+    if (2 * lane + 1 >= valid) two = 2 * lane < valid ? two & 0xffffu : 0;
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + i * 128 + ((lane >> 2 ^ (i & 7)) << 4) +
+                                                 (lane & 3) * 4),
+                 "r"(two)
+                 : "memory");
+  }
+}
+
+// kRowsA, kRowsB: the operand's contraction runs along its rows. kGather: A's rows by
+// gather_rows.
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair, bool kGather>
+__global__ void __launch_bounds__(product_threads(kGather), 1)
+    product_kernel(Plan plan, Epilogue e, Operand a_rows,
+                   const __grid_constant__ CUtensorMap a_map,
                    const __grid_constant__ CUtensorMap b_map,
                    const __grid_constant__ EpilogueMaps maps) {
   using Shared = ProductShared<kN, kPair>;
@@ -461,7 +510,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 32 * kEpilogueWarps) {
     for (int i = 0; i < kStages; ++i) {
-      barrier_init(shared_address(&s.full[i]), 1);
+      barrier_init(shared_address(&s.full[i]), kGather ? 1 + kGatherWarps : 1);
       barrier_init(shared_address(&s.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -500,7 +549,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const uint32_t a = shared_address(s.a[stage]), b = shared_address(s.b[stage]);
           const int k0 = (first + k) * kDepth;
           if (rank == 0)
-            barrier_expect(bar, (kPair ? 2 : 1) * (Shared::kABytes + Shared::kBBytes));
+            barrier_expect(bar, (kPair ? 2 : 1) * ((kGather ? 0 : Shared::kABytes) + Shared::kBBytes));
           if constexpr (kPair) bar = of_first_block(bar);
           const auto load = [&](uint32_t to, const CUtensorMap* map, int x, int r) {
             if constexpr (kPair) load_box_pair(to, map, x, r, bar);
@@ -509,7 +558,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           if constexpr (kRowsA)
             for (int i = 0; i < kRows / 64; ++i)
               load(a + i * kDepth * 128, &a_map, m0 + 64 * i, k0);
-          else
+          else if constexpr (!kGather)
             load(a, &a_map, k0, m0);
           if constexpr (kRowsB)
             for (int i = 0; i < Shared::kBRows / 64; ++i)
@@ -562,6 +611,23 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         else commit(elected, shared_address(&s.ready[buffer]));
       }
     }
+  } else if (kGather && warp >= kEpilogueWarps + 2) {
+    const int rows_in_tile = kRows / kGatherWarps * (warp - kEpilogueWarps - 2);
+    uint32_t turn = 0;
+    for (; walk.more(plan) && good; walk.advance(plan)) {
+      const int64_t row0 = int64_t{walk.row} * kRows + rows_in_tile;
+      const int first = walk.first_step(plan), steps = walk.steps(plan);
+      for (int k = 0; k < steps; ++k, ++turn) {
+        const uint32_t stage = turn % kStages, round = turn / kStages;
+        if (round > 0) good = barrier_wait_warp(shared_address(&s.empty[stage]), (round - 1) & 1);
+        if (!good) break;
+        gather_rows(a_rows, row0, (first + k) * kDepth, shared_address(s.a[stage]) + rows_in_tile * 128,
+                    lane);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(shared_address(&s.full[stage]));
+      }
+    }
   } else {
     good = epilogue<T, kN, kForm, kPair>(plan, e, maps, s, tensor, warp, lane);
   }
@@ -580,13 +646,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     else tensor_free<2 * kN>(tensor);
   }
 }
-
-// An operand: a [rows, channels] array of 16-bit elements, and whether the
-// contraction runs along its rows.
-struct Operand {
-  const void* data;
-  int64_t rows, channels, stride;
-};
 
 int32_t encode_operand(CUtensorMap* map, int32_t dtype, const Operand& o, int box_rows) {
   const cuuint64_t size[2] = {static_cast<cuuint64_t>(o.channels), static_cast<cuuint64_t>(o.rows)};
@@ -610,11 +669,11 @@ bool tma_rows(const void* data, int64_t stride, int32_t dtype, int64_t columns) 
   return is_aligned(data, 16) && stride * element_size(dtype) % 16 == 0 && stride >= columns;
 }
 
-template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair>
+template <class T, int kN, bool kRowsA, bool kRowsB, Form kForm, bool kPair, bool kGather>
 int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan,
                        const Epilogue& e, cudaStream_t stream) {
   CUtensorMap a_map, b_map;
-  GS_TRY(encode_operand(&a_map, dtype, a, kRowsA ? kDepth : kRows));
+  if (!kGather) GS_TRY(encode_operand(&a_map, dtype, a, kRowsA ? kDepth : kRows));
   using Shared = ProductShared<kN, kPair>;
   GS_TRY(encode_operand(&b_map, dtype, b, kRowsB ? kDepth : Shared::kBRows));
   EpilogueMaps maps;
@@ -631,7 +690,7 @@ int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const 
   }
   constexpr size_t kShared = sizeof(Shared);
   constexpr int kBlocks = kPair ? 2 : 1;
-  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair>>(kShared)));
+  GS_TRY((allow_shared<product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair, kGather>>(kShared)));
   const int64_t items = int64_t{plan.row_tiles} * plan.column_tiles * plan.splits;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -641,13 +700,13 @@ int32_t launch_product(int32_t dtype, const Operand& a, const Operand& b, const 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = static_cast<unsigned>(kBlocks * std::min<int64_t>(items, kSmCount / kBlocks));
-  config.blockDim = kProductThreads;
+  config.blockDim = product_threads(kGather);
   config.dynamicSmemBytes = kShared;
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = kPair ? 2 : 1;
-  cudaLaunchKernelEx(&config, product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair>, plan, e, a_map,
-                     b_map, maps);
+  cudaLaunchKernelEx(&config, product_kernel<T, kN, kRowsA, kRowsB, kForm, kPair, kGather>, plan, e,
+                     a, a_map, b_map, maps);
   return check_launch();
 }
 
@@ -689,7 +748,7 @@ Plan plan_of(int64_t rows, int64_t columns, int64_t depth, ProductTile tile, int
 // for its columns, whose half it stages, where the contraction is long enough that the
 // products and not the results bound it (131,101 x 256: contracting 1024, 93 us against 98;
 // 131,101 x 1024: contracting 256, 90 against 78).
-ProductTile tile_of(int64_t rows, int64_t columns, int64_t depth, int least) {
+ProductTile tile_of(int64_t rows, int64_t columns, int64_t depth, int least, bool pairs = true) {
   ProductTile best = {};
   int64_t best_time = 0;
   const auto consider = [&](ProductTile t, int64_t turn) {
@@ -697,14 +756,14 @@ ProductTile tile_of(int64_t rows, int64_t columns, int64_t depth, int least) {
     const int64_t time = (tiles + t.workers() - 1) / t.workers() * turn;
     if (!best.columns || time < best_time) best = t, best_time = time;
   };
-  if (depth >= kPairDepth) consider({256, true}, 192 + 32);
+  if (pairs && depth >= kPairDepth) consider({256, true}, 192 + 32);
   for (int n = 256; n >= least; n /= 2) consider({n, false}, n + 32);
   return best;
 }
 
 // D = A B^T by `e`, in such tiles. The gradients' products have 16-bit results
 // or sums to be joined only.
-template <class T, bool kRowsA, bool kRowsB>
+template <class T, bool kRowsA, bool kRowsB, bool kGather = false>
 int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Plan& plan, ProductTile tile,
                     const Epilogue& e, cudaStream_t stream) {
   const auto formed = [&](auto columns, auto pair) {
@@ -712,24 +771,25 @@ int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Pla
     constexpr bool kPair = decltype(pair)::value;
     switch (form_of(e)) {
       case Form::kNarrow:
-        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow, kPair>(dtype, a, b, plan, e, stream);
+        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow, kPair, kGather>(dtype, a, b, plan, e, stream);
       case Form::kWide:
-        if constexpr (kRowsA || !kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide, kPair>(dtype, a, b, plan, e, stream);
+        if constexpr (kRowsA && kRowsB)
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide, kPair, kGather>(dtype, a, b, plan, e, stream);
       case Form::kActive:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive, kPair>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive, kPair, kGather>(dtype, a, b, plan, e, stream);
       case Form::kTraining:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining, kPair>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining, kPair, kGather>(dtype, a, b, plan, e, stream);
       case Form::kStream:
         if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream, kPair>(dtype, a, b, plan, e, stream);
+          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream, kPair, kGather>(dtype, a, b, plan, e, stream);
       default: break;
     }
-    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny, kPair>(dtype, a, b, plan, e, stream);
+    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny, kPair, kGather>(dtype, a, b, plan, e, stream);
   };
-  if (tile.pair) return formed(std::integral_constant<int, 256>{}, std::true_type{});
+  if constexpr (!kGather)
+    if (tile.pair) return formed(std::integral_constant<int, 256>{}, std::true_type{});
   switch (tile.columns) {
     case 256: return formed(std::integral_constant<int, 256>{}, std::false_type{});
     case 128: return formed(std::integral_constant<int, 128>{}, std::false_type{});
@@ -788,7 +848,8 @@ __global__ void __launch_bounds__(kSlopeThreads, 3)
   const G* __restrict__ const grad = static_cast<const G*>(a.grad_y) + column;
   float sum[8] = {};
   if (valid > 0) {
-    constexpr int kBatch = sizeof(G) == 4 || kSlopes == Slopes::kFloats ? 4 : 6;
+    constexpr bool kLong = sizeof(G) == 4, kExact = kSlopes == Slopes::kFloats;
+    constexpr int kBatch = !kWhole ? 2 : kLong && kExact ? 3 : kLong || kExact ? 4 : 6;
     for (int64_t m0 = row0 + first; m0 < end; m0 += kBatch * step) {
       Pack<G, 8> g[kBatch];
       uint4 codes[kBatch];
@@ -946,10 +1007,15 @@ int32_t check_args(const gs_linear_args& a) {
   for (int32_t t : {a.bias_dtype, a.residual_dtype})
     if (t != a.dtype && t != GS_FLOAT32) return GS_ERR_INVALID_ARGUMENT;
   if (!a.weight || (a.rows > 0 && !a.x)) return GS_ERR_INVALID_ARGUMENT;
-  if (a.x_stride < a.inputs || a.weight_stride < a.inputs) return GS_ERR_INVALID_ARGUMENT;
-  if (!is_aligned(a.x, 16) || !is_aligned(a.weight, 16) || a.x_stride % 8 || a.weight_stride % 8)
+  if (a.x_stride < 0 || a.weight_stride < a.inputs) return GS_ERR_INVALID_ARGUMENT;
+  if (!is_aligned(a.x, 2) || !is_aligned(a.weight, 16) || a.weight_stride % 8)
     return GS_ERR_MISALIGNED;
   return GS_OK;
+}
+
+// Whether TMA takes x.
+bool aligned_x(const gs_linear_args& a) {
+  return is_aligned(a.x, 16) && a.x_stride % 8 == 0 && a.x_stride >= a.inputs;
 }
 
 template <class F>
@@ -1057,12 +1123,15 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   e.tiled = tma_rows(a.y, a.outputs, a.residual_dtype, a.outputs) &&
             (!a.residual ||
              tma_rows(a.residual, a.residual_stride, a.residual_dtype, a.outputs));
-  const ProductTile tile = tile_of(a.rows, a.outputs, a.inputs, 32);
+  const bool gather = !aligned_x(a);
+  const ProductTile tile = tile_of(a.rows, a.outputs, a.inputs, 32, !gather);
+  const Plan plan = plan_of(a.rows, a.outputs, a.inputs, tile, 1);
+  const Operand x = {a.x, a.rows, a.inputs, a.x_stride};
+  const Operand weight = {a.weight, a.outputs, a.inputs, a.weight_stride};
   return with_sixteen_bit(a.dtype, [&](auto t) {
-    return run_product<decltype(t), false, false>(
-        a.dtype, {a.x, a.rows, a.inputs, a.x_stride},
-        {a.weight, a.outputs, a.inputs, a.weight_stride},
-        plan_of(a.rows, a.outputs, a.inputs, tile, 1), tile, e, stream);
+    using T = decltype(t);
+    return gather ? run_product<T, false, false, true>(a.dtype, x, weight, plan, tile, e, stream)
+                  : run_product<T, false, false>(a.dtype, x, weight, plan, tile, e, stream);
   });
 }
 
@@ -1070,7 +1139,8 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
   GS_TRY(check_args(a));
   if (a.rows > 0 && (!a.grad_y || !a.workspace || (a.activation != GS_IDENTITY && !a.slope)))
     return GS_ERR_INVALID_ARGUMENT;
-  if (!is_aligned(a.grad_y, 16) || !is_aligned(a.slope, 16) || !is_aligned(a.workspace, 256))
+  if (!aligned_x(a) || !is_aligned(a.grad_y, 16) || !is_aligned(a.slope, 16) ||
+      !is_aligned(a.workspace, 256))
     return GS_ERR_MISALIGNED;
   const BackwardPlan p = backward_plan(a);
   if (a.workspace_size < p.size) return GS_ERR_CAPACITY;

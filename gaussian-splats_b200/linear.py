@@ -50,7 +50,9 @@ def _arguments(x, weight, bias, **values):
 def _forward(x, weight, bias, residual, activation, train):
     """The result, and what the backward keeps."""
     inputs, outputs = x.shape[-1], weight.shape[0]
-    rows, w = _operand(x if x.dim() == 2 else x.reshape(-1, inputs)), _operand(weight)
+    rows, w = x if x.dim() == 2 else x.reshape(-1, inputs), _operand(weight)
+    if train or rows.stride(1) != 1 or rows.stride(0) < 0:  # the backward reads it by columns
+        rows = _operand(rows)
     b = None if bias is None else bias.contiguous()
     if residual is None:
         y, res, stride = x.new_empty(x.shape[:-1] + (outputs,)), None, 0

@@ -694,7 +694,8 @@ int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
 
 /* A linear layer with its epilogue: z = x W^T + bias, y = act(z) + residual. x [rows,
  * inputs] and weight [outputs, inputs] of `dtype` (GS_BFLOAT16 or GS_FLOAT16), 16-byte
- * aligned, row strides multiples of 8; bias [outputs] of bias_dtype (may be NULL);
+ * aligned, row strides multiples of 8 (x may have any address and row stride in the
+ * forward; the products are then fed by plain loads); bias [outputs] of bias_dtype (may be NULL);
  * residual [rows, outputs] of residual_dtype with a row stride (may be NULL); both
  * types are dtype or GS_FLOAT32. y [rows, outputs] of residual_dtype, contiguous.
  * `slope` [rows, outputs rounded up to 8], 16-byte aligned, receives act'(z) for the

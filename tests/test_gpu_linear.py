@@ -111,6 +111,25 @@ def test_far_sums(activation):
     check(call(s, activation), s, activation)
 
 
+@pytest.mark.parametrize("inputs", [1, 2, 7, 10, 59, 62, 63, 64, 65, 70, 131])
+@pytest.mark.parametrize("rows,outputs", [(1, 8), (130, 300), (40000, 24)])
+def test_rows_that_lie_anyhow(rows, inputs, outputs):
+    """Without gradients x is read in place, wherever its rows begin; what lies around
+    them does not matter."""
+    from gaussian_splats_b200.linear import linear
+
+    s = make(rows, inputs, outputs, BF, FL, None)
+    want = call(s, "silu", train=False)["y"]
+    check({"y": want}, s, "silu", train=False)
+    for offset, pitch in ((1, inputs + 3), (2, inputs + 4), (3, inputs + 2), (1, inputs)):
+        whole = torch.full((rows * pitch + offset + 1,), float("nan"), device="cuda", dtype=BF)
+        x = whole.as_strided((rows, inputs), (pitch, 1), offset)
+        x.copy_(s["x"])
+        with torch.no_grad():
+            y = linear(x, s["weight"], s["bias"], activation="silu")
+        assert torch.equal(y, want), (offset, pitch)
+
+
 def test_special_values():
     """A row's infinities and NaN stay in that row of y and dx."""
     from gaussian_splats_b200.linear import linear

@@ -43,8 +43,8 @@ def test_linear_checks_arguments():
     for status, bad in [(-1, dict(rows=-1)), (-1, dict(rows=2 ** 31)), (-1, dict(inputs=0)),
                         (-1, dict(outputs=65537)), (-1, dict(activation=4)), (-4, dict(dtype=0)),
                         (-1, dict(bias_dtype=2)), (-1, dict(residual_dtype=2)), (-1, dict(x=None)),
-                        (-1, dict(weight=None)), (-1, dict(x_stride=56)), (-5, dict(x=a + 8)),
-                        (-5, dict(weight_stride=68))]:
+                        (-1, dict(weight=None)), (-1, dict(x_stride=-1)), (-5, dict(x=a + 1)),
+                        (-1, dict(weight_stride=56)), (-5, dict(weight_stride=68))]:
         args = native.LinearArgs(**{**good, **bad})
         assert lib.gs_linear(ctypes.byref(args), None) == status, bad
         assert lib.gs_linear_backward(ctypes.byref(args), None) == status, bad
@@ -52,7 +52,7 @@ def test_linear_checks_arguments():
         args = native.LinearArgs(**{**good, **bad})
         assert lib.gs_linear(ctypes.byref(args), None) == -1, bad
     for status, bad in ((-1, dict(grad_y=None)), (-1, dict(slope=None)), (-1, dict(workspace=None)),
-                        (-3, dict(workspace_size=0))):
+                        (-3, dict(workspace_size=0)), (-5, dict(x=a + 8)), (-5, dict(x_stride=60))):
         args = native.LinearArgs(**{**good, **bad})
         assert lib.gs_linear_backward(ctypes.byref(args), None) == status, bad
     assert lib.gs_linear(None, None) == -1 and lib.gs_linear_backward(None, None) == -1
