@@ -4,15 +4,15 @@
 //   score_t = scale q . k_t = scale (step_t (q . c_t) + (middle_t - 7.5 step_t) sum q)
 //   out = sum p_t v_t = sum (p_t step_t) (c_t - 7.5) + sum p_t middle_t
 //
-// so that codes go to the products as they are, small whole numbers in float16, which
-// are exact, and the ranges stay outside: a key's in two numbers a score, a value's in
+// so that codes go to the products as they are, as float16 numbers, which
+// is exact, and the ranges stay outside: a key's in two numbers a score, a value's in
 // its weight p_t step_t and in one float sum a head, which no rounding meets. q and the
 // weights are scaled by powers of two into float16's range, whatever the tokens' type:
 // of a head's q nothing is lost within 2^-25 of its largest channel, and the weights
 // are rounded once, to 11 bits.
 //
-// The cache is read once; taking a word of eight codes apart costs 9 to 10 instructions
-// though, which together weigh about as much as the reading. So the work is cut evenly:
+// The cache is read once; taking a word of eight codes apart costs 5 or 6 instructions
+// though, which with the rest weigh about as much as the reading. So the work is cut evenly:
 // the turns of 32 slots of all streams and key-value heads (up to 16 query heads; more:
 // several times) in one line, of which every warp has the same share, wherever that
 // begins and ends. A warp keeps a ring in shared memory filled some turns ahead, waits for
@@ -189,47 +189,16 @@ __device__ __forceinline__ float2 unpack2(uint32_t word) {
   return make_float2(to_float(v[0]), to_float(v[1]));
 }
 
-// c - 8 in float16 of the codes at bits 0 to 3 (low), or 4 to 7, of both halves of a
-// word: next to 1024, whose low bits they are, and that taken off again. Exact.
-__device__ __forceinline__ uint32_t among(uint32_t word, uint32_t bits, uint32_t base) {
-  uint32_t y;  // (word & bits) | base
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(word), "r"(bits), "r"(base));
-  return y;
-}
-__device__ __forceinline__ uint32_t centred_low(uint32_t word) {  // (1024 + c) - 1032
-  uint32_t y;
-  asm("add.rn.f16x2 %0, %1, %2;"
-      : "=r"(y)
-      : "r"(among(word, 0x000f000fu, 0x64006400u)), "r"(0xe408e408u));
-  return y;
-}
-__device__ __forceinline__ uint32_t centred_high(uint32_t word) {  // (1024 + 16 c) / 16 - 72
-  uint32_t y;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;"
-      : "=r"(y)
-      : "r"(among(word, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
-  return y;
-}
-// Codes 0 to 3 of both halves of a value's word as four pairs.
+// Codes 0 to 3 of both halves of a word as four pairs of float16 numbers, with nothing to
+// convert: the bits 0 to 3 of a half are the subnormal number c 2^-24, bits 4 to 7 are 16 c
+// 2^-24, which the products take exactly. So pairs 1 and 3 are 16 times as large.
+constexpr float kCodeUnit = 16777216.0f;  // 2^24
 __device__ __forceinline__ void spread(uint32_t word, uint32_t (&pair)[4]) {
   const uint32_t next = word >> 8;
-  pair[0] = centred_low(word);
-  pair[1] = centred_high(word);
-  pair[2] = centred_low(next);
-  pair[3] = centred_high(next);
-}
-
-// A key's codes keep what they lie next to, which is taken off the dots: pairs 0 and 2
-// are 1024 + 4 c, pairs 1 and 3 1024 + 64 c, so that in units of the code, with q scaled
-// to match, they are off by 256 and 16. (In the dots' float sums that costs 2^-23 of
-// 256 sum |q| a product: 1e-5 of a score. The values' sums are too long for it.)
-constexpr float kLowOffset = 256.0f, kHighOffset = 16.0f;
-__device__ __forceinline__ void spread_key(uint32_t word, uint32_t (&pair)[4]) {
-  const uint32_t up = word << 2, down = word >> 6;
-  pair[0] = among(up, 0x003c003cu, 0x64006400u);
-  pair[1] = among(up, 0x03c003c0u, 0x64006400u);
-  pair[2] = among(down, 0x003c003cu, 0x64006400u);
-  pair[3] = among(down, 0x03c003c0u, 0x64006400u);
+  pair[0] = word & 0x000f000fu;
+  pair[1] = word & 0x00f000f0u;
+  pair[2] = next & 0x000f000fu;
+  pair[3] = next & 0x00f000f0u;
 }
 
 // c += a b, 16 x 16 by 16 x 8.
@@ -239,6 +208,14 @@ __device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1
       "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// c = a b.
+__device__ __forceinline__ void multiply_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // An 8 x 8 matrix of pairs, a row in four lanes, turned around.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
@@ -398,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   float2 dot_scale[kSets], dot_offset[kSets], q_sum[kSets];
 #pragma unroll
   for (int r = 0; r < kSets; ++r) {
-    float x[kKeyWords][8], low_total = 0.0f, high_total = 0.0f, largest = 0.0f;
+    float x[kKeyWords][8], total = 0.0f, largest = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKeyWords; ++w) {
       const int channel = 8 * (kKeyWords * j + w);
@@ -410,15 +387,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
                      x[w]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (k & 1) high_total += x[w][k];
-        else low_total += x[w][k];
+        total += x[w][k];
         largest = max_nan(largest, fabsf(x[w][k]));
       }
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-      low_total += __shfl_xor_sync(0xffffffffu, low_total, o);
-      high_total += __shfl_xor_sync(0xffffffffu, high_total, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
       largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
     }
     const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, 11u << 23);
@@ -430,18 +405,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       for (int e = 0; e < 4; ++e)
         q[r][w][e] = tc::pack2<__half>(x[w][e] * (e & 1 ? 0.0625f * up : up),
                                        x[w][e + 4] * (e & 1 ? 0.0625f * up : up));
-    const float scale = a.scale * kLog2e, total = low_total + high_total;
-    const float offset = kLowOffset * low_total + kHighOffset * high_total + 7.5f * total;
+    const float scale = a.scale * kLog2e;
     const auto heads_of = [&](float x) {
       return make_float2(__shfl_sync(0xffffffffu, x, 8 * j), __shfl_sync(0xffffffffu, x, 8 * j + 4));
     };
-    dot_scale[r] = heads_of(0.25f * down * scale);
-    dot_offset[r] = heads_of(-offset * scale);
+    dot_scale[r] = heads_of(kCodeUnit * down * scale);
+    dot_offset[r] = heads_of(-7.5f * total * scale);
     q_sum[r] = heads_of(total * scale);
   }
-  float out[kSets][kValueWords][4][4] = {};
+  float2 out[kSets][kValueWords][4][2] = {};  // of both heads: channels e, and e + 4
   float top[kSets][2];
-  float2 sum[kSets] = {}, middle_sum[kSets] = {};
+  float2 sum[kSets] = {}, middle_sum[kSets] = {}, weight_sum[kSets] = {};
 #pragma unroll
   for (int r = 0; r < kSets; ++r) top[r][0] = top[r][1] = -INFINITY;
   // Value steps are taken relative to a power of two above the largest so far.
@@ -490,24 +464,25 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         const uint32_t next = min(largest & 0x7f800000u, 0x7e000000u) + 0x00800000u;
         const float shrink = unit ? __uint_as_float(unit) / __uint_as_float(next) : 0.0f;
 #pragma unroll
+        for (int r = 0; r < kSets; ++r) weight_sum[r] = tc::mul2(weight_sum[r], both(shrink));
+#pragma unroll
         for (int r = 0; r < kSets; ++r)
 #pragma unroll
           for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) out[r][h][i][c] *= shrink;
+              for (int c = 0; c < 2; ++c) out[r][h][i][c] = tc::mul2(out[r][h][i][c], both(shrink));
         unit = next;
         per_unit = __uint_as_float(0x7f000000u - next);
       }
-      const float weight_step = value.x * per_unit, middle = fmaf(0.5f, value.x, value.y);
-      s.slot[warp][lane] = {both(key.x), both(key.y), both(weight_step), both(middle)};
+      s.slot[warp][lane] = {both(key.x), both(key.y), both(value.x * per_unit), both(value.y)};
     }
     __syncwarp();
     Slot of[4];  // the lane's slots as rows of the scores: key_row, + 8, + 16, + 24
 #pragma unroll
     for (int i = 0; i < 4; ++i) of[i] = s.slot[warp][key_row + 8 * i];
-    float x[kSets][2][4] = {};
+    float x[kSets][2][4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {  // 16 slots
       uint32_t low[kKeyWords], high[kKeyWords];
@@ -516,11 +491,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 #pragma unroll
       for (int w = 0; w < kKeyWords; ++w) {
         uint32_t p0[4], p8[4];
-        spread_key(low[w], p0);
-        spread_key(high[w], p8);
+        spread(low[w], p0);
+        spread(high[w], p8);
 #pragma unroll
         for (int r = 0; r < kSets; ++r) {
-          multiply(x[r][half], p0[0], p8[0], p0[1], p8[1], q[r][w][0], q[r][w][1]);
+          if (w == 0) multiply_new(x[r][half], p0[0], p8[0], p0[1], p8[1], q[r][w][0], q[r][w][1]);
+          else multiply(x[r][half], p0[0], p8[0], p0[1], p8[1], q[r][w][0], q[r][w][1]);
           multiply(x[r][half], p0[2], p8[2], p0[3], p8[3], q[r][w][2], q[r][w][3]);
         }
       }
@@ -553,16 +529,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
             shrink[e] = tc::exp2_approx(top[r][e] - next[e]);
             top[r][e] = next[e];
           }
-#pragma unroll
-          for (int h = 0; h < kValueWords; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              out[r][h][i][e] *= shrink[e];
-              out[r][h][i][2 + e] *= shrink[e];
-            }
         }
-        sum[r] = tc::mul2(sum[r], make_float2(shrink[0], shrink[1]));
-        middle_sum[r] = tc::mul2(middle_sum[r], make_float2(shrink[0], shrink[1]));
+        const float2 shrinks = make_float2(shrink[0], shrink[1]);
+        sum[r] = tc::mul2(sum[r], shrinks);
+        middle_sum[r] = tc::mul2(middle_sum[r], shrinks);
+        weight_sum[r] = tc::mul2(weight_sum[r], shrinks);
+#pragma unroll
+        for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) out[r][h][i][c] = tc::mul2(out[r][h][i][c], shrinks);
       }
       const float2 shift = make_float2(top[r][0] == -INFINITY ? 0.0f : kLift - top[r][0],
                                        top[r][1] == -INFINITY ? 0.0f : kLift - top[r][1]);
@@ -575,6 +552,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         const float2 w = tc::mul2(p, of[i].value_step);
         weight[r][i] = transposed(tc::pack2<__half>(w.x, w.y));
       }
+    }
+    // The turn's sums of weights times codes, all of them positive, are added to the others'
+    // in float arithmetic: the products' own sums, which are cut and not rounded, would
+    // all err to one side, by more than the few digits that are left once 7.5 times the
+    // weights is taken off (`weight_sum`, the weights as they were rounded).
+    float turn[kSets][kValueWords][4][4], turn_weight[kSets][4];
+#pragma unroll
+    for (int r = 0; r < kSets; ++r) {
+      constexpr uint32_t kOnes = 0x3c003c00u;
+      multiply_new(turn_weight[r], kOnes, kOnes, kOnes, kOnes, weight[r][0], weight[r][1]);
+      multiply(turn_weight[r], kOnes, kOnes, kOnes, kOnes, weight[r][2], weight[r][3]);
+      weight_sum[r] = tc::add2(weight_sum[r], make_float2(turn_weight[r][0], turn_weight[r][1]));
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -594,10 +583,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int r = 0; r < kSets; ++r)
-            multiply(out[r][h][e], a0[e], a1[e], a2[e], a3[e], weight[r][2 * half],
-                     weight[r][2 * half + 1]);
+            if (half == 0)
+              multiply_new(turn[r][h][e], a0[e], a1[e], a2[e], a3[e], weight[r][0], weight[r][1]);
+            else
+              multiply(turn[r][h][e], a0[e], a1[e], a2[e], a3[e], weight[r][2], weight[r][3]);
       }
     }
+#pragma unroll
+    for (int r = 0; r < kSets; ++r)
+#pragma unroll
+      for (int h = 0; h < kValueWords; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            out[r][h][e][c] = tc::add2(out[r][h][e][c], make_float2(turn[r][h][e][2 * c],
+                                                                   turn[r][h][e][2 * c + 1]));
     __syncwarp();  // all lanes are done with the stage that the next turn fills
   }
   filled += turns;
@@ -630,17 +631,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         part.top[head] = top[r][e];
         part.sum[head] = total;
       }
+      // Weights times codes are in units of 2^-24, or 2^-20, and the weights in `unit`.
+      const float size = unit_size * kCodeUnit;
+      const float off = fmaf(-7.5f * unit_size, e ? weight_sum[r].y : weight_sum[r].x, middle);
+      const auto value = [&](float2 x, float by) { return fmaf(e ? x.y : x.x, by, off); };
 #pragma unroll
       for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float(&x)[4][4] = out[r][h];
+        for (int i = 0; i < 2; ++i)
           *reinterpret_cast<float4*>(&part.out[head][8 * (kValueWords * g + h) + 4 * i]) =
-              make_float4(fmaf(x[0][2 * i + e], unit_size, middle),
-                          fmaf(x[1][2 * i + e], unit_size, middle),
-                          fmaf(x[2][2 * i + e], unit_size, middle),
-                          fmaf(x[3][2 * i + e], unit_size, middle));
-        }
+              make_float4(value(out[r][h][0][i], size), value(out[r][h][1][i], 0.0625f * size),
+                          value(out[r][h][2][i], size), value(out[r][h][3][i], 0.0625f * size));
     }
   __syncwarp();  // the next part's slots
   }
