@@ -322,14 +322,19 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     batch, heads, dim = q.shape
     kv_heads = k.shape[1]
     slots = k_codes.shape[2] if k_codes.dim() == 4 else 0
-    for t, last, kind in ((k_codes, dim // 2, torch.uint8), (k_range, 2, q.dtype),
-                          (v_codes, dim // 2, torch.uint8), (v_range, 2, q.dtype)):
-        if slots < 1 or t.shape != (batch, kv_heads, slots, last) or t.dtype != kind:
-            raise ValueError(f"{what}: a cache's {tuple(t.shape)} {t.dtype} is not [batch, "
-                             f"kv_heads, slots, {last}] of {kind} for k {tuple(k.shape)}")
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"{what}: the cache must be contiguous and 16-byte aligned (it is "
-                             "updated in place)")
+    codes, ranges = (batch, kv_heads, slots, dim // 2), (batch, kv_heads, slots, 2)
+    pointers = [t.data_ptr() for t in (k_codes, k_range, v_codes, v_range)]
+    if slots < 1 or k_codes.shape != codes or v_codes.shape != codes or \
+            k_range.shape != ranges or v_range.shape != ranges or \
+            k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or \
+            k_range.dtype != q.dtype or v_range.dtype != q.dtype:
+        given = ", ".join(f"{tuple(t.shape)} {t.dtype}" for t in cache)
+        raise ValueError(f"{what}: a cache of {given} is not [batch, kv_heads, slots, dim / 2] "
+                         f"uint8 codes and [..., 2] {q.dtype} ranges for k {tuple(k.shape)}")
+    if any(p % 16 for p in pointers) or not (k_codes.is_contiguous() and k_range.is_contiguous() and
+                                             v_codes.is_contiguous() and v_range.is_contiguous()):
+        raise ValueError(f"{what}: the cache must be contiguous and 16-byte aligned (it is "
+                         "updated in place)")
     if batch * slots > native.MAX_SEQUENCE_TOKENS:
         raise ValueError(f"{what}: caches of {batch} x {slots} slots, at most "
                          f"{native.MAX_SEQUENCE_TOKENS} in all are supported")
@@ -341,8 +346,8 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
                       kv_heads=kv_heads, dim=dim, dtype=dtype, slots=slots, first=first,
                       scale=_scale(what, scale, dim), positions=positions.data_ptr(),
                       out=out.data_ptr(), valid=address(valid), cache_valid=address(cache_valid),
-                      k_codes=k_codes.data_ptr(), k_range=k_range.data_ptr(),
-                      v_codes=v_codes.data_ptr(), v_range=v_range.data_ptr())
+                      k_codes=pointers[0], k_range=pointers[1], v_codes=pointers[2],
+                      v_range=pointers[3])
     size = native.lib().gs_window_attention_step_4bit_workspace_size(ctypes.byref(args))
     workspace = q.new_empty((size,), dtype=torch.uint8)
     args.workspace, args.workspace_size = workspace.data_ptr(), size

@@ -129,6 +129,10 @@ def address(t: torch.Tensor | None) -> int | None:
 
 def check_cuda(what: str, **tensors: torch.Tensor | None) -> torch.device:
     """The CUDA device of the tensors; raises unless all are on the same one."""
+    present = [t for t in tensors.values() if t is not None]
+    index = present[0].get_device()
+    if index >= 0 and all(t.get_device() == index for t in present):
+        return present[0].device
     device = None
     for name, t in tensors.items():
         if t is None:
