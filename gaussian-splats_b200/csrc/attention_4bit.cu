@@ -66,11 +66,18 @@ struct Shared {
   uint64_t full[kWarps][Stage<kDim>::kCount];
 };
 
-// What a warp leaves of its part of an item: outputs times the sum, maxima, sums.
-template <int kDim, int kSets>
-struct Part {
-  float out[8 * kSets][kDim];
-  float top[8 * kSets], sum[8 * kSets];
+// What a warp leaves of its part of an item, for each of `heads` query heads: outputs
+// times the sum, then the heads' maxima and sums.
+template <int kDim>
+struct Parts {
+  float* data;
+  int32_t heads;
+  __host__ __device__ int64_t floats() const { return int64_t{heads} * (kDim + 2) + (heads & 1) * 2; }
+  __device__ float* out(int64_t part, int h) const { return data + part * floats() + h * kDim; }
+  __device__ float* top(int64_t part, int h) const {
+    return data + part * floats() + heads * kDim + h;
+  }
+  __device__ float* sum(int64_t part, int h) const { return top(part, h) + heads; }
 };
 
 // The warps that have an item's first and last turn.
@@ -90,16 +97,28 @@ __device__ __forceinline__ Stream stream_at(const gs_window_attention_step_4bit_
 }
 
 // The line of turns: stream after stream, each `heads` (key-value heads times pieces of
-// query heads) times its turns. Warp w of `warps` has turns [w total / warps, (w + 1) total
+// query heads) times its turns. (More than kCounted streams are not counted first, which
+// would take a microsecond a thousand: each is in the line with the turns of a full cache,
+// and a warp passes over those that it lacks.) Warp w of `warps` has turns [w total / warps, (w + 1) total
 // / warps) of it, one at least.
 struct Line {
   int64_t total, warps;
   int64_t stream, before;  // the stream that has the warp's first turn, the turns before it
 };
+constexpr int kCounted = 1024;
+__device__ __forceinline__ int turns_in_line(const gs_window_attention_step_4bit_args& a,
+                                             const Stream& s) {
+  return a.batch > kCounted ? (a.slots + kSlots - 1) / kSlots : s.turns;
+}
 // By a whole warp.
 __device__ Line find_turn(const gs_window_attention_step_4bit_args& a, int heads, int64_t w,
                           int64_t warps) {
   const int lane = threadIdx.x & 31;
+  if (a.batch > kCounted) {
+    const int64_t each = int64_t{turns_in_line(a, {})} * heads;
+    const int64_t total = a.batch * each, at = w * total / min(warps, total);
+    return {total, min(warps, total), at / each, at / each * each};
+  }
   int64_t total = 0;
   for (int64_t b = lane; b < a.batch; b += 32) total += int64_t{stream_at(a, b).turns} * heads;
 #pragma unroll
@@ -246,7 +265,7 @@ __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)
 // whole 16-byte words.
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
-    step_kernel(gs_window_attention_step_4bit_args a, Part<kDim, kSets>* parts, Reach* reach) {
+    step_kernel(gs_window_attention_step_4bit_args a, Parts<kDim> parts, Reach* reach) {
   using S = Shared<kDim>;
   constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
   constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
@@ -278,15 +297,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   uint32_t filled = 0;  // turns loaded by the parts before: the ring goes on behind them
   while (at < end) {
   const Stream stream = stream_at(a, b);
-  if (stream.turns == 0 || at - before >= int64_t{stream.turns} * a.kv_heads * pieces) {
-    before += int64_t{stream.turns} * a.kv_heads * pieces;
+  const int places = turns_in_line(a, stream);
+  if (at - before >= int64_t{places} * a.kv_heads * pieces) {
+    before += int64_t{places} * a.kv_heads * pieces;
     ++b;
     continue;
   }
-  const int64_t head_piece = (at - before) / stream.turns;
-  const int first_turn = static_cast<int>((at - before) % stream.turns);
-  const int turns = static_cast<int>(min(int64_t{stream.turns - first_turn}, end - at));
-  at += turns;
+  const int64_t head_piece = (at - before) / places;
+  const int first_turn = static_cast<int>((at - before) % places);
+  const int here = static_cast<int>(min(int64_t{places - first_turn}, end - at));
+  const int turns = min(here, stream.turns - first_turn);
+  at += here;
+  if (turns <= 0) continue;
   const int piece = static_cast<int>(head_piece % pieces);
   const int kv_head = static_cast<int>(head_piece / pieces);
   const int head0 = kv_head * group + piece * kHeads;
@@ -611,7 +633,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   // What the warp leaves: row g of product (h, e) is channel 8 (kValueWords g + h) + e, row g
   // + 8 channel e + 4. Parts are numbered by warp and item together: both only grow.
   const int64_t item = (b * a.kv_heads + kv_head) * pieces + piece;
-  Part<kDim, kSets>& part = parts[me + item];
   if (lane == 0 && first_turn == 0) reach[item].first = static_cast<int32_t>(me);
   if (lane == 0 && first_turn + turns == stream.turns) reach[item].last = static_cast<int32_t>(me);
   const float unit_size = __uint_as_float(unit);
@@ -628,8 +649,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       }
       if (head >= heads) continue;
       if (g == 0) {
-        part.top[head] = top[r][e];
-        part.sum[head] = total;
+        *parts.top(me + item, head) = top[r][e];
+        *parts.sum(me + item, head) = total;
       }
       // Weights times codes are in units of 2^-24, or 2^-20, and the weights in `unit`.
       const float size = unit_size * kCodeUnit;
@@ -639,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       for (int h = 0; h < kValueWords; ++h)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float4*>(&part.out[head][8 * (kValueWords * g + h) + 4 * i]) =
+          *reinterpret_cast<float4*>(parts.out(me + item, head) + 8 * (kValueWords * g + h) + 4 * i) =
               make_float4(value(out[r][h][0][i], size), value(out[r][h][1][i], 0.0625f * size),
                           value(out[r][h][2][i], size), value(out[r][h][3][i], 0.0625f * size));
     }
@@ -654,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 constexpr int kMostParts = 128, kAhead = 8;  // at a time: threads of the smallest block
 template <class T, int kDim, int kSets>
 __global__ void __launch_bounds__(1024)
-    join_kernel(gs_window_attention_step_4bit_args a, const Part<kDim, kSets>* parts,
-                const Reach* reach) {
+    join_kernel(gs_window_attention_step_4bit_args a, Parts<kDim> parts, const Reach* reach) {
   constexpr int kHeads = 8 * kSets;
   __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32];
   chain_wait();
@@ -673,15 +693,15 @@ __global__ void __launch_bounds__(1024)
   }
   const int count = r.last - r.first + 1, threads = blockDim.x, thread = threadIdx.x;
   const int d = thread % kDim, groups = threads / kDim, mine = thread / kDim;
-  const Part<kDim, kSets>* const from = parts + item + r.first;
+  const int64_t from = item + r.first;
   float ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
-    ahead[k] = mine + k * groups < count ? from[mine + k * groups].out[h][d] : 0.0f;
+    ahead[k] = mine + k * groups < count ? parts.out(from + mine + k * groups, h)[d] : 0.0f;
   float top = -INFINITY, sum = 0.0f;
-  if (thread < count) top = from[thread].top[h], sum = from[thread].sum[h];
+  if (thread < count) top = *parts.top(from + thread, h), sum = *parts.sum(from + thread, h);
   float whole = top;
-  for (int i = thread + threads; i < count; i += threads) whole = fmaxf(whole, from[i].top[h]);
+  for (int i = thread + threads; i < count; i += threads) whole = fmaxf(whole, *parts.top(from + i, h));
   whole = warp_max(whole);
   if ((thread & 31) == 0) tops[thread >> 5] = whole;
   __syncthreads();
@@ -692,7 +712,7 @@ __global__ void __launch_bounds__(1024)
     __syncthreads();
     const int some = min(kMostParts, count - i0);
     if (thread < some) {
-      if (i0 > 0) top = from[i0 + thread].top[h], sum = from[i0 + thread].sum[h];
+      if (i0 > 0) top = *parts.top(from + i0 + thread, h), sum = *parts.sum(from + i0 + thread, h);
       scales[thread] = tc::exp2_approx(top - shift);
       sums[thread] = sum * scales[thread];
     }
@@ -704,7 +724,7 @@ __global__ void __launch_bounds__(1024)
         if (i < some) o = fmaf(ahead[k], scales[i], o);
     }
 #pragma unroll 8
-    for (; i < some; i += groups) o = fmaf(from[i0 + i].out[h][d], scales[i], o);
+    for (; i < some; i += groups) o = fmaf(parts.out(from + i0 + i, h)[d], scales[i], o);
     if (thread < a.dim)
       for (int k = 0; k < some; ++k) total += sums[k];
   }
@@ -729,13 +749,18 @@ int64_t items_of(const gs_window_attention_step_4bit_args& a, int sets) {
 
 uint64_t reach_bytes(int64_t items) { return (sizeof(Reach) * static_cast<uint64_t>(items) + 15) / 16 * 16; }
 
+int part_heads(const gs_window_attention_step_4bit_args& a, int sets) {
+  return std::min(a.heads / a.kv_heads, 8 * sets);
+}
+
 template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
 int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
   const int64_t items = items_of(a, kSets), blocks = blocks_of(a, items, kSets);
   if (items > INT32_MAX) return GS_ERR_CAPACITY;
-  using P = Part<kDim, kSets>;
   Reach* const reach = static_cast<Reach*>(a.workspace);
-  P* const parts = reinterpret_cast<P*>(static_cast<unsigned char*>(a.workspace) + reach_bytes(items));
+  const Parts<kDim> parts = {
+      reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + reach_bytes(items)),
+      part_heads(a, kSets)};
   constexpr size_t kShared = sizeof(Shared<kDim>);
   GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared)));
   launch_chained_shared(step_kernel<T, kDim, kSets, kMasked, kAligned>,
@@ -746,9 +771,8 @@ int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
   const int64_t each = blocks * kWarps / items;
   const int threads = each >= 16 ? 1024 : each >= 8 ? 256 : 128;
   launch_chained(join_kernel<T, kDim, kSets>,
-                 dim3(static_cast<unsigned>(items), std::min(a.heads / a.kv_heads, 8 * kSets)),
-                 threads, stream, a, static_cast<const P*>(parts),
-                 static_cast<const Reach*>(reach));
+                 dim3(static_cast<unsigned>(items), parts.heads),
+                 threads, stream, a, parts, static_cast<const Reach*>(reach));
   return check_launch();
 }
 
@@ -776,8 +800,9 @@ uint64_t window_attention_step_4bit_workspace_size(const gs_window_attention_ste
   if (check_args(a) != GS_OK || a.batch == 0) return 0;
   const int sets = sets_of(a);
   const int64_t items = items_of(a, sets);
-  const uint64_t part = a.dim <= 64 ? (sets == 1 ? sizeof(Part<64, 1>) : sizeof(Part<64, 2>))
-                                    : (sets == 1 ? sizeof(Part<128, 1>) : sizeof(Part<128, 2>));
+  const int heads = part_heads(a, sets);
+  const uint64_t part = 4 * (a.dim <= 64 ? Parts<64>{nullptr, heads}.floats()
+                                         : Parts<128>{nullptr, heads}.floats());
   return reach_bytes(items) +
          part * static_cast<uint64_t>(blocks_of(a, items, sets) * kWarps + items);
 }

@@ -127,6 +127,51 @@ def test_long_caches(batch, heads, kv_heads, dim, left, first, dtype):
         compare(out, ref.step(q, k, v, few, dim ** -0.5, valid), dtype, dim)
 
 
+def test_many_streams():
+    """More streams than are counted first, some idle, at different places; and one head
+    that many query heads share."""
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    for batch, heads, kv_heads, dim, slots in ((1025, 2, 1, 16, 70), (1500, 3, 3, 8, 40),
+                                               (1024, 1, 1, 64, 65)):
+        g = torch.Generator(device="cuda").manual_seed(batch)
+        ref = R.Streams(batch, slots, 2, kv_heads, dim, BF, "cuda")
+        fill(ref, g, BF, batch, kv_heads, slots, dim)
+        positions = torch.randint(-1, 2 * slots, (batch,), generator=g, device="cuda")
+        ref.seen[:] = torch.arange(slots, device="cuda") < positions[:, None]
+        cache = FourBitCache(ref.codes[0].clone(), ref.ranges[0].clone(), ref.codes[1].clone(),
+                             ref.ranges[1].clone())
+        q = rand(g, batch, heads, dim, dtype=BF)
+        k, v = (rand(g, batch, kv_heads, dim, dtype=BF) for _ in range(2))
+        out = window_attention_step_4bit(q, k, v, cache, positions, first=2)
+        compare(out, ref.step(q, k, v, positions, dim ** -0.5), BF, dim)
+        assert (out[positions < 0] == 0).all() and (positions < 0).any()
+        for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
+            assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
+
+
+def test_all_idle():
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for batch in (3, 2000):
+        cache = window_cache_4bit(batch, 5, 0, 1, 32)
+        q = rand(g, batch, 2, 32, dtype=BF)
+        out = window_attention_step_4bit(q, q[:, :1], q[:, 1:], cache,
+                                         torch.full((batch,), -1, device="cuda"))
+        assert (out == 0).all() and all((t == 0).all() for t in cache)
+
+
+def test_status():
+    import ctypes
+
+    from gaussian_splats_b200 import native
+
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert native.lib().gs_window_attention_status(stream) == 0
+    assert native.lib().gs_linear_status(stream) == 0
+
+
 def test_rows_that_are_special():
     """Rows of one value, of zeros, of subnormals, of the type's limits, and not finite."""
     from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit

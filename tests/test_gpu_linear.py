@@ -15,7 +15,7 @@ SHAPES = [(1, 1, 1), (1, 8, 8), (2, 64, 128), (3, 59, 11), (5, 7, 9), (16, 2048,
 # type, bias, residual, activation
 FORMS = [(BF, None, None, None), (BF, BF, None, "gelu"), (BF, FL, FL, "silu"),
          (HF, HF, HF, "relu"), (HF, FL, None, "gelu"), (HF, None, FL, None),
-         (BF, FL, BF, "silu"), (HF, HF, None, "silu")]
+         (BF, FL, BF, "silu"), (HF, HF, None, "silu"), (BF, BF, FL, "gelu"), (BF, BF, BF, None)]
 
 
 def make(rows, inputs, outputs, dtype, bias, residual, seed=0, size=1.0):
@@ -90,6 +90,16 @@ def check(got, s, activation, train=True):
 @pytest.mark.parametrize("form", FORMS, ids=str)
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 def test_against_the_definition(shape, form):
+    dtype, bias, residual, activation = form
+    s = make(*shape, dtype, bias, residual)
+    check(call(s, activation), s, activation)
+    check(call(s, activation, train=False), s, activation, train=False)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("shape", [(20003, 72, 520), (9001, 520, 300)], ids=str)
+def test_many_tiles(shape, form):
+    """Several tiles a block, in every form of the epilogue; with 520 inputs in pairs."""
     dtype, bias, residual, activation = form
     s = make(*shape, dtype, bias, residual)
     check(call(s, activation), s, activation)
@@ -193,6 +203,24 @@ def test_gradients_asked_for(wanted):
     some = [n for n in names if leaves[n].requires_grad]
     for n, t in zip(some, torch.autograd.grad(y, [leaves[n] for n in some], s["grad"])):
         assert torch.equal(t, whole["d" + n]), n
+
+
+@pytest.mark.parametrize("wanted", range(1, 8))
+def test_gradients_asked_for_without_activation(wanted):
+    """The gradient itself is an operand then, and needs no copy."""
+    from gaussian_splats_b200.linear import linear
+
+    s = make(1030, 136, 200, HF, HF, None)
+    whole = call(s, None)
+    names = ("x", "weight", "bias")
+    leaves = {n: s[n].detach().requires_grad_(bool(wanted >> i & 1)) for i, n in enumerate(names)}
+    y = linear(*leaves.values())
+    some = [n for n in names if leaves[n].requires_grad]
+    wide = torch.empty(1030 * 200 + 1, device="cuda", dtype=HF)
+    for up in (s["grad"], wide[1:].view(1030, 200).copy_(s["grad"])):  # off its 16-byte borders
+        grads = torch.autograd.grad(y, [leaves[n] for n in some], up, retain_graph=True)
+        for n, t in zip(some, grads):
+            assert torch.equal(t, whole["d" + n]), n
 
 
 def test_no_rows():
