@@ -20,8 +20,9 @@ using namespace tc;
 
 // act'(z) is kept in 16 bits, as (slope + 1/6) 49152: slopes lie in [-0.13, 1.13], so
 // the error is 1.02e-5 at most, where float16's would be 2.4e-4 next to 1 and add
-// to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact. (A
-// float32 bias's gradient is a sum of unrounded dz: there slopes are kept as floats.)
+// to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact, and NaN,
+// whose low bits are all ones, is the code that no slope has. (A float32 bias's gradient
+// is a sum of unrounded dz: there slopes are kept as floats.)
 constexpr float kSlopeScale = 49152.0f, kSlopeZero = 8192.0f, kTwo23 = 8388608.0f;
 __device__ __forceinline__ uint32_t slope_codes(float2 slopes) {
   // The sums' low bits are the nearest whole numbers.
@@ -30,7 +31,7 @@ __device__ __forceinline__ uint32_t slope_codes(float2 slopes) {
   return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x5410);
 }
 __device__ __forceinline__ float slope_value(uint32_t code) {
-  return (__uint_as_float(0x4b000000u | code) - (kTwo23 + kSlopeZero)) * (1.0f / kSlopeScale);
+  return code == 0xffffu ? NAN : (__uint_as_float(0x4b000000u | code) - (kTwo23 + kSlopeZero)) * (1.0f / kSlopeScale);
 }
 
 __device__ __forceinline__ float reciprocal_approx(float x) {
@@ -1106,6 +1107,10 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   GS_TRY(check_args(a));
   if (a.rows == 0) return GS_OK;
   if (!a.y) return GS_ERR_INVALID_ARGUMENT;
+  const size_t element = element_size(a.residual_dtype);
+  if (!is_aligned(a.y, element) || !is_aligned(a.residual, element) ||
+      !is_aligned(a.bias, element_size(a.bias_dtype)) || !is_aligned(a.slope, 16))
+    return GS_ERR_MISALIGNED;
   Epilogue e = {};
   e.rows = a.rows;
   e.columns = a.outputs;
@@ -1140,7 +1145,8 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
   if (a.rows > 0 && (!a.grad_y || !a.workspace || (a.activation != GS_IDENTITY && !a.slope)))
     return GS_ERR_INVALID_ARGUMENT;
   if (!aligned_x(a) || !is_aligned(a.grad_y, 16) || !is_aligned(a.slope, 16) ||
-      !is_aligned(a.workspace, 256))
+      !is_aligned(a.workspace, 256) || !is_aligned(a.grad_x, 2) || !is_aligned(a.grad_weight, 8) ||
+      !is_aligned(a.grad_bias, element_size(a.bias_dtype)))
     return GS_ERR_MISALIGNED;
   const BackwardPlan p = backward_plan(a);
   if (a.workspace_size < p.size) return GS_ERR_CAPACITY;

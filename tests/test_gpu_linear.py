@@ -161,6 +161,21 @@ def test_special_values():
     assert big.tolist() == [[480000.0, 0.0]]
 
 
+@pytest.mark.parametrize("bias", [BF, FL], ids=str)
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_nan_reaches_the_gradients(activation, bias):
+    """A channel whose sums are NaN has NaN gradients, and the others theirs."""
+    s = make(300, 64, 72, BF, bias, None)
+    clean = call(s, activation)
+    s["bias"][5] = float("nan")
+    got = call(s, activation)
+    others = torch.arange(72, device="cuda") != 5
+    assert got["y"][:, 5].isnan().all() and got["dx"].isnan().all()
+    assert got["dweight"][5].isnan().all() and got["dbias"][5].isnan()
+    for name in ("dweight", "dbias"):
+        assert torch.equal(got[name][others], clean[name][others])
+
+
 def test_strides_and_offsets():
     """Slices of a projection, odd offsets and pitches, a transposed weight, three axes."""
     from gaussian_splats_b200.linear import linear

@@ -48,11 +48,15 @@ def test_linear_checks_arguments():
         args = native.LinearArgs(**{**good, **bad})
         assert lib.gs_linear(ctypes.byref(args), None) == status, bad
         assert lib.gs_linear_backward(ctypes.byref(args), None) == status, bad
-    for bad in (dict(y=None),):
+    for status, bad in ((-1, dict(y=None)), (-5, dict(y=a + 2)), (-5, dict(residual=a + 2)),
+                        (-5, dict(bias=a + 2)), (-5, dict(slope=a + 8)),
+                        (-5, dict(y=a + 1, residual_dtype=1)), (-5, dict(bias=a + 1, bias_dtype=1))):
         args = native.LinearArgs(**{**good, **bad})
-        assert lib.gs_linear(ctypes.byref(args), None) == -1, bad
+        assert lib.gs_linear(ctypes.byref(args), None) == status, bad
     for status, bad in ((-1, dict(grad_y=None)), (-1, dict(slope=None)), (-1, dict(workspace=None)),
-                        (-3, dict(workspace_size=0)), (-5, dict(x=a + 8)), (-5, dict(x_stride=60))):
+                        (-3, dict(workspace_size=0)), (-5, dict(x=a + 8)), (-5, dict(x_stride=60)),
+                        (-5, dict(grad_x=a + 1)), (-5, dict(grad_weight=a + 4)),
+                        (-5, dict(grad_bias=a + 2)), (-5, dict(workspace=a + 128))):
         args = native.LinearArgs(**{**good, **bad})
         assert lib.gs_linear_backward(ctypes.byref(args), None) == status, bad
     assert lib.gs_linear(None, None) == -1 and lib.gs_linear_backward(None, None) == -1
