@@ -2,7 +2,7 @@
 
 For Gaussians along a space-filling order, a token's neighbours in the sequence
 are its neighbours in space, so a refiner attends in a window of them, and to a
-few first tokens that stand for the scene or the camera. Two entry points:
+few first tokens that stand for the scene or the camera. Three entry points:
 
 :func:`window_attention`
     whole sequences, packed, differentiable: training, and inference over a

@@ -707,7 +707,9 @@ int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
  * grad_weight [outputs, inputs] (both of dtype, contiguous) and grad_bias [outputs]
  * (bias_dtype) that are not NULL; what reaches the products is dz = grad_y act'(z)
  * rounded to dtype. It needs a workspace of gs_linear_workspace_size bytes, 256-byte
- * aligned. Outputs are 16-byte aligned. No atomics: results repeat bit for bit. */
+ * aligned. x and grad_y are 16-byte aligned here and x has a stride as the weight,
+ * grad_weight is 8-byte aligned; everything else lies as its type allows (16-byte
+ * aligned and of whole 16-byte rows is faster). No atomics: results repeat bit for bit. */
 enum { GS_IDENTITY = 0, GS_RELU = 1, GS_GELU = 2, GS_SILU = 3 }; /* activations */
 enum { GS_MAX_LINEAR_FEATURES = 65536 };                         /* inputs, outputs */
 typedef struct gs_linear_args {
