@@ -41,13 +41,13 @@ def _heads(what, q, k, v, rows_name):
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"{what}: expected [{rows_name}, heads, dim] tensors, got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    (rows, heads, dim), (k_rows, kv_heads, k_dim) = q.shape, k.shape
+    if k.shape != v.shape or k_rows != rows or k_dim != dim:
         raise ValueError(f"{what}: q {tuple(q.shape)} does not go with k {tuple(k.shape)} and v "
                          f"{tuple(v.shape)}")
-    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{what}: {q.shape[1]} query heads are not a multiple of {k.shape[1]} "
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{what}: {heads} query heads are not a multiple of {kv_heads} "
                          "key-value heads")
-    dim = q.shape[2]
     if dim < 8 or dim % 8 or dim > MAX_HEAD_DIM:
         raise ValueError(f"{what}: head dim {dim} is not a multiple of 8 in [8, {MAX_HEAD_DIM}]")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -66,8 +66,9 @@ def _scale(what, scale, dim):
 def _strided(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where the kernels can read it in place (rows of whole,
     aligned 16-byte words), else a contiguous copy."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and \
-            t.stride(0) > 0 and t.stride(1) > 0 and t.data_ptr() % 16 == 0:
+    row, head, channel = t.stride()
+    if channel == 1 and row % 8 == 0 and head % 8 == 0 and row > 0 and head > 0 and \
+            t.data_ptr() % 16 == 0:
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone(
         memory_format=torch.contiguous_format)
@@ -81,9 +82,11 @@ def _whole(t: torch.Tensor) -> torch.Tensor:
 
 def _place(q, k, v):
     """The fields of an operator's arguments that say where q, k and v lie."""
-    return dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q.stride(0),
-                q_head_stride=q.stride(1), k_stride=k.stride(0), k_head_stride=k.stride(1),
-                v_stride=v.stride(0), v_head_stride=v.stride(1))
+    (q_stride, q_head, _), (k_stride, k_head, _), (v_stride, v_head, _) = \
+        q.stride(), k.stride(), v.stride()
+    return dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q_stride,
+                q_head_stride=q_head, k_stride=k_stride, k_head_stride=k_head,
+                v_stride=v_stride, v_head_stride=v_head)
 
 
 def _arguments(kind, q, k, v, **values):

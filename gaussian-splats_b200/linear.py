@@ -31,11 +31,10 @@ _GATHERED = 128
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, channels] as the kernels read a product's operand: rows of contiguous
     channels that start on 16-byte borders. ``t`` itself if it lies so, else a copy."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and \
-            t.data_ptr() % 16 == 0:
+    (row, channel), (rows, channels) = t.stride(), t.shape
+    if channel == 1 and row % 8 == 0 and row >= channels and t.data_ptr() % 16 == 0:
         return t
-    rows, channels = t.shape
-    if t.stride(1) != 1:
+    if channel != 1:
         t = t.contiguous()
     copy = t.new_empty((rows, -(-channels // 8) * 8))
     call("gs_align_rows", t.device, rows, channels, t.data_ptr(), t.stride(0), copy.data_ptr())
@@ -44,9 +43,9 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 def _arguments(x, weight, bias, **values):
     """``gs_linear_args`` of operands ``x`` and ``weight``."""
-    dtype = _CODES[x.dtype]
+    dtype, (rows, inputs) = _CODES[x.dtype], x.shape
     return native.LinearArgs(
-        rows=x.shape[0], inputs=x.shape[1], outputs=weight.shape[0], dtype=dtype,
+        rows=rows, inputs=inputs, outputs=weight.shape[0], dtype=dtype,
         bias_dtype=dtype if bias is None else _CODES[bias.dtype], x=x.data_ptr(),
         weight=weight.data_ptr(), bias=address(bias), x_stride=x.stride(0),
         weight_stride=weight.stride(0), **values)
@@ -54,7 +53,7 @@ def _arguments(x, weight, bias, **values):
 
 def _forward(x, weight, bias, residual, activation, train):
     """The result, and what the backward keeps."""
-    inputs, outputs = x.shape[-1], weight.shape[0]
+    outputs, inputs = weight.shape
     rows, w = x if x.dim() == 2 else x.reshape(-1, inputs), _operand(weight)
     if train or inputs > _GATHERED or rows.stride(1) != 1:
         rows = _operand(rows)
@@ -108,6 +107,13 @@ class _Linear(torch.autograd.Function):
         return (*grads, grad_y if want_residual else None, None)
 
 
+def _check_added(what, name, t, shape, dtype):
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} {tuple(t.shape)} is not {shape}")
+    if t.dtype != dtype and t.dtype != torch.float32:
+        raise ValueError(f"{what}: the {name} must be {dtype} or float32, got {t.dtype}")
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
            residual: torch.Tensor | None = None, *, activation: str | None = None) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual`` for ``x`` [..., inputs] and ``weight``
@@ -142,16 +148,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if activation not in ACTIVATIONS:
         raise ValueError(f"{what}: activation must be one of {tuple(ACTIVATIONS)}, got "
                          f"{activation!r}")
-    for name, t, shape in (("bias", bias, (outputs,)),
-                           ("residual", residual, (*x.shape[:-1], outputs))):
-        if t is None:
-            continue
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{what}: {name} {tuple(t.shape)} is not {shape}")
-        if t.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{what}: the {name} must be {x.dtype} or float32, got {t.dtype}")
-    train = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias, residual))
-    if train:
+    if bias is not None:
+        _check_added(what, "bias", bias, (outputs,), x.dtype)
+    if residual is not None:
+        _check_added(what, "residual", residual, (*x.shape[:-1], outputs), x.dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
     return _forward(x, weight, bias, residual, ACTIVATIONS[activation], False)[0]
