@@ -13,9 +13,10 @@
 //     of the rate of a long bare product in a burst; with gelu 400, with its slopes 456. In
 //     a training pass the power limit lowers the clock: 510 to 600 us, and 380 to 460 each
 //     for dx and dW, with the tensor cores active for 84 to 88 % of the time.
-//   short ones: what is written. 131,072 x 256 -> 1024: 80 us for 268 MB of results (a
-//     plain fill of as many bytes takes 72, and 74 with all stores to one place that stays
-//     in L2); dx of 131,101 x 1024 from 256 channels 78.
+//   short ones: the results, 268 MB of 131,072 x 64 or 128 -> 1024 in 57 us (the epilogue
+//     without its stores: 49). From 256 channels 80 us, as dx of 131,101 x 1024 from 256: the
+//     loads take longer under the stores' traffic (53 without stores; 74 to 78 without half of
+//     the products, or B's loads, or x in L2, or a stage more).
 //   activations: gelu makes 137 us of these 80, with its slopes 156: two instructions an
 //     element of the kind that a multiprocessor makes 16 a clock of, and a long chain. relu
 //     80 and 109.
@@ -473,35 +474,47 @@ struct Operand {
 };
 
 // Rows of A that TMA does not take (no whole 16-byte words): a warp loads a row's 64
-// channels at a time, two a lane, and puts them where TMA would have. All its rows
-// are requested before the first is put down. No copy of A is made for it: that
-// took a third of the time of a forward whose bound is its result (500,000 x 59 -> 256,
-// 90 us a pass).
-__device__ __forceinline__ void gather_rows(const Operand& a, int64_t row0, int k0, uint32_t tile,
-                                            int lane) {
-  constexpr int kBatch = kRows / kGatherWarps;
+// channels at a time, two a lane, and puts them where TMA would have. All its rows of a
+// stage are requested before the stage before is put down, so that their latency passes
+// while that one waits for its place. No copy of A is made for it: that took a third of
+// the time of a forward whose bound is its result (500,000 x 59 -> 256: 90 us a pass with
+// one, 69 so; 72 without requests ahead).
+constexpr int kGatherRows = kRows / kGatherWarps;
+struct Gathered {
+  uint32_t word[kGatherRows];
+  uint32_t more;  // an odd row's 64th channel lies in a 33rd word: row i's is lane i's
+};
+// 1 if row i of the rows at `data` starts in the middle of a 4-byte word.
+__device__ __forceinline__ int odd_row(const uint16_t* data, int64_t stride, int i) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(data) >> 1 ^ (i & stride)) & 1);
+}
+__device__ __forceinline__ const uint16_t* gathered_from(const Operand& a, int64_t row0, int k0) {
+  return static_cast<const uint16_t*>(a.data) + row0 * a.stride + k0;
+}
+__device__ __forceinline__ Gathered gather_rows(const Operand& a, int64_t row0, int k0, int lane) {
   const int valid = static_cast<int>(min(int64_t{kDepth}, a.channels - k0));
-  const uint16_t* const data = static_cast<const uint16_t*>(a.data) + row0 * a.stride + k0;
-  const int rows = static_cast<int>(min(int64_t{kBatch}, a.rows - row0));
-  const auto odd = [&](int i) {  // 1 if row i starts in the middle of a 4-byte word
-    return static_cast<int>((reinterpret_cast<uintptr_t>(data) >> 1 ^ (i & a.stride)) & 1);
-  };
+  const uint16_t* const data = gathered_from(a, row0, k0);
+  const int rows = static_cast<int>(min(int64_t{kGatherRows}, a.rows - row0));
   const auto words = [&](int i) {
-    return reinterpret_cast<const uint32_t*>(data + i * a.stride - odd(i));
+    return reinterpret_cast<const uint32_t*>(data + i * a.stride - odd_row(data, a.stride, i));
   };
-  uint32_t word[kBatch];
+  Gathered g;
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i)
-    word[i] = i < rows && 2 * lane < valid + odd(i) ? __ldg(words(i) + lane) : 0;
-  // An odd row's 64th channel lies in a 33rd word: row i's is lane i's.
-  uint32_t more = 0;
-  if (lane < rows && odd(lane) && valid == kDepth) more = __ldg(words(lane) + 32);
+  for (int i = 0; i < kGatherRows; ++i)
+    g.word[i] = i < rows && 2 * lane < valid + odd_row(data, a.stride, i) ? __ldg(words(i) + lane) : 0;
+  g.more = lane < rows && odd_row(data, a.stride, lane) && valid == kDepth ? __ldg(words(lane) + 32) : 0;
+  return g;
+}
+__device__ __forceinline__ void put_rows(const Gathered& g, const Operand& a, int64_t row0, int k0,
+                                         uint32_t tile, int lane) {
+  const int valid = static_cast<int>(min(int64_t{kDepth}, a.channels - k0));
+  const uint16_t* const data = gathered_from(a, row0, k0);
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i) {  // eight rows' swizzle starts over with the warp's rows
-    uint32_t next = __shfl_down_sync(0xffffffffu, word[i], 1);
-    const uint32_t last = __shfl_sync(0xffffffffu, more, i);
+  for (int i = 0; i < kGatherRows; ++i) {  // eight rows' swizzle starts over with the warp's rows
+    uint32_t next = __shfl_down_sync(0xffffffffu, g.word[i], 1);
+    const uint32_t last = __shfl_sync(0xffffffffu, g.more, i);
     if (lane == 31) next = last;
-    uint32_t two = odd(i) ? __byte_perm(word[i], next, 0x5432) : word[i];
+    uint32_t two = odd_row(data, a.stride, i) ? __byte_perm(g.word[i], next, 0x5432) : g.word[i];
     if (2 * lane + 1 >= valid) two = 2 * lane < valid ? two & 0xffffu : 0;
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + i * 128 + ((lane >> 2 ^ (i & 7)) << 4) +
                                                  (lane & 3) * 4),
@@ -631,21 +644,33 @@ __global__ void __launch_bounds__(product_threads(kGather), 1)
       }
     }
   } else if (kGather && warp >= kEpilogueWarps + 2) {
-    const int rows_in_tile = kRows / kGatherWarps * (warp - kEpilogueWarps - 2);
-    uint32_t turn = 0;
-    for (; walk.more(plan) && good; walk.advance(plan)) {
-      const int64_t row0 = int64_t{walk.row} * kRows + rows_in_tile;
-      const int first = walk.first_step(plan), steps = walk.steps(plan);
-      for (int k = 0; k < steps; ++k, ++turn) {
-        const uint32_t stage = turn % kStages, round = turn / kStages;
-        if (round > 0) good = barrier_wait_warp(shared_address(&s.empty[stage]), (round - 1) & 1);
-        if (!good) break;
-        gather_rows(a_rows, row0, (first + k) * kDepth, shared_address(s.a[stage]) + rows_in_tile * 128,
-                    lane);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(shared_address(&s.full[stage]));
+    const int rows_in_tile = kGatherRows * (warp - kEpilogueWarps - 2);
+    struct Place {
+      Walk walk;
+      int k;  // of the item's steps
+    };
+    const auto row_of = [&](const Place& p) { return int64_t{p.walk.row} * kRows + rows_in_tile; };
+    const auto depth_of = [&](const Place& p) { return (p.walk.first_step(plan) + p.k) * kDepth; };
+    Place here = {walk, 0};
+    Gathered now = gather_rows(a_rows, row_of(here), depth_of(here), lane);
+    for (uint32_t turn = 0; here.walk.more(plan) && good; ++turn) {
+      Place next = here;
+      if (++next.k == here.walk.steps(plan)) {
+        next.walk.advance(plan);
+        next.k = 0;
       }
+      Gathered ahead = now;
+      if (next.walk.more(plan)) ahead = gather_rows(a_rows, row_of(next), depth_of(next), lane);
+      const uint32_t stage = turn % kStages, round = turn / kStages;
+      if (round > 0) good = barrier_wait_warp(shared_address(&s.empty[stage]), (round - 1) & 1);
+      if (!good) break;
+      put_rows(now, a_rows, row_of(here), depth_of(here), shared_address(s.a[stage]) + rows_in_tile * 128,
+               lane);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(shared_address(&s.full[stage]));
+      here = next;
+      now = ahead;
     }
   } else {
     good = epilogue<T, kN, kForm, kPair>(plan, e, maps, s, tensor, warp, lane);
