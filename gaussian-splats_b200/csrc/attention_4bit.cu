@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   int64_t before = line.before;  // turns before the stream's
   const int64_t end = (me + 1) * line.total / line.warps;
   bool good = true;
-  uint32_t filled = 0;  // turns loaded by the parts before: the ring goes on behind them
+  // The ring goes on from part to part: the next turn's stage, and its barrier's phase.
+  uint32_t stage = 0, phase = 0;
   while (at < end) {
   const Stream stream = stream_at(a, b);
   const int places = turns_in_line(a, stream);
@@ -330,55 +331,59 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   uint8_t* const slots_valid = kMasked ? a.cache_valid + b * a.slots : nullptr;
   const bool token_valid = !kMasked || !a.valid || a.valid[b];
 
-  const auto base_of = [&](int t) { return (first_turn + t) * kSlots; };
-  const auto load = [&](int t) {
-    const uint32_t stage = (filled + t) % kStages;
+  const int base0 = first_turn * kSlots;
+  const int end_slot = min(count, base0 + turns * kSlots);  // the part's
+  int next_base = base0;  // of the next turn to load
+  const uint8_t* next_codes[2] = {codes[0] + int64_t{base0} * row_bytes,
+                                  codes[1] + int64_t{base0} * row_bytes};
+  const auto load = [&](uint32_t to) {  // it, to stage `to`
     if constexpr (kAligned) {  // the turn's rows are one run of memory
-      if (t < turns && good && lane == 0) {
-        const int base = base_of(t);
-        const uint32_t bytes = min(kSlots, count - base) * row_bytes;
-        const uint32_t bar = tc::shared_address(&s.full[warp][stage]);
+      if (next_base < end_slot && good && lane == 0) {
+        const uint32_t bytes = min(kSlots, end_slot - next_base) * row_bytes;
+        const uint32_t bar = tc::shared_address(&s.full[warp][to]);
         tc::barrier_expect(bar, 2 * bytes);
 #pragma unroll
         for (int side = 0; side < 2; ++side)
           asm volatile(
               "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, "
-              "[%3];" ::"r"(tc::shared_address(s.stage[warp][stage].codes[side])),
-              "l"(codes[side] + int64_t{base} * row_bytes), "r"(bytes), "r"(bar)
+              "[%3];" ::"r"(tc::shared_address(s.stage[warp][to].codes[side])),
+              "l"(next_codes[side]), "r"(bytes), "r"(bar)
               : "memory");
       }
     } else {
-      if (t < turns) {
-        Stage<kDim>& st = s.stage[warp][stage];
-        const int row = base_of(t) + min(lane, count - 1 - base_of(t));
+      if (next_base < end_slot) {
+        Stage<kDim>& st = s.stage[warp][to];
+        const int row = min(lane, end_slot - 1 - next_base);
 #pragma unroll
         for (int side = 0; side < 2; ++side)
           for (int w = 0; w < row_bytes; w += 4)
-            cp_async4(st.codes[side] + lane * kRow + w,
-                      codes[side] + int64_t{row} * row_bytes + w);
+            cp_async4(st.codes[side] + lane * kRow + w, next_codes[side] + row * row_bytes + w);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    next_base += kSlots;
+    next_codes[0] += kSlots * row_bytes;
+    next_codes[1] += kSlots * row_bytes;
   };
   // The ranges of the lane's slot of a turn, keys' and values', zeros behind the last one.
-  const auto ranges_of = [&](int t) {
-    if (t >= turns || base_of(t) + lane >= count) return make_uint2(0, 0);
-    return make_uint2(__ldcg(range[0] + base_of(t) + lane), __ldcg(range[1] + base_of(t) + lane));
+  const uint32_t* const lane_range[2] = {range[0] + lane, range[1] + lane};
+  const auto ranges_of = [&](int base) {
+    if (base + lane >= end_slot) return make_uint2(0, 0);
+    return make_uint2(__ldcg(lane_range[0] + base), __ldcg(lane_range[1] + base));
   };
-  const auto seen_in = [&](int t) {  // whether the lane's slot of a turn may be seen
-    if (t >= turns) return false;
-    const int at = base_of(t) + lane;
-    if (at >= count) return false;
+  const auto seen_in = [&](int base) {  // whether the lane's slot of a turn may be seen
+    const int at = base + lane;
+    if (at >= end_slot) return false;
     return !kMasked || (at == slot ? token_valid : slots_valid[at] != 0);
   };
 #pragma unroll
-  for (int t = 0; t < kStages - 1; ++t) load(t);
-  bool seen_next = seen_in(0);
-  uint2 range_next = ranges_of(0), range_after = ranges_of(1);  // two turns ahead
+  for (uint32_t t = 0; t < kStages - 1; ++t)
+    load(stage + t < kStages ? stage + t : stage + t - kStages);
+  bool seen_next = seen_in(base0);
+  uint2 range_next = ranges_of(base0), range_after = ranges_of(base0 + kSlots);  // two turns ahead
 
   // The warp whose turn has the new token's slot rounds its rows.
-  const int slot_turn = slot / kSlots - first_turn;
-  const bool owner = slot_turn >= 0 && slot_turn < turns;
+  const bool owner = slot >= base0 && slot < end_slot;
   Fresh fresh = {0, 0};
   if (owner) {
     const bool value = lane >= 16;
@@ -454,24 +459,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   // a lane's four slots of V, j, 4 + j, 8 + j and 12 + j, and its neighbours', lie next to one
   // another.
   const int key_row = (g >> 1) + 4 * (g & 1);
-  for (int t = 0; t < turns && good; ++t) {
-    load(t + kStages - 1);
-    Stage<kDim>& st = s.stage[warp][(filled + t) % kStages];
-    const int base = base_of(t);
+  for (int base = base0; base < end_slot && good; base += kSlots) {
+    load(stage == 0 ? kStages - 1 : stage - 1);  // the turn before's
+    Stage<kDim>& st = s.stage[warp][stage];
     const bool seen = seen_next;
     uint2 ranges = range_next;
-    seen_next = seen_in(t + 1);
+    seen_next = seen_in(base + kSlots);
     range_next = range_after;
-    range_after = ranges_of(t + 2);
+    range_after = ranges_of(base + 2 * kSlots);
     if constexpr (kAligned) {
-      good = tc::barrier_wait_warp(tc::shared_address(&s.full[warp][(filled + t) % kStages]),
-                                   (filled + t) / kStages & 1);
+      good = tc::barrier_wait_warp(tc::shared_address(&s.full[warp][stage]), phase);
       if (!good) break;
     } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
     }
-    if (owner && t == slot_turn) {
+    if (owner && static_cast<uint32_t>(slot - base) < kSlots) {
       const int side = lane >> 4, word = lane & 15;
       if (8 * word < a.dim)
         *reinterpret_cast<uint32_t*>(st.codes[side] + (slot - base) * pitch + 4 * word) = fresh.codes;
@@ -628,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
             out[r][h][e][c] = tc::add2(out[r][h][e][c], make_float2(turn[r][h][e][2 * c],
                                                                    turn[r][h][e][2 * c + 1]));
     __syncwarp();  // all lanes are done with the stage that the next turn fills
+    if (++stage == kStages) stage = 0, phase ^= 1;
   }
-  filled += turns;
   if (!good) {  // let what is in flight land, and show that the result is not valid
     for (uint64_t& bar : s.full[warp]) tc::barrier_settle(tc::shared_address(&bar));
     for (float2& x : sum) x = make_float2(NAN, NAN);
