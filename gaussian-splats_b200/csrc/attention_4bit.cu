@@ -19,11 +19,11 @@
 // no other, and leaves the sums of its part of each stream's head in a workspace, which
 // a second kernel joins in order.
 //
-// 96 streams of 4100 slots, 16 heads (4) of 128 channels, 214 MB: 60 us (3.6 TB/s); 3 streams
-// of 65,536 slots, 24 heads (8) of 96 channels, 164 MB: 50 us. The first's reading alone
-// takes 40 to 48 us, all but the reading 44: the two do not overlap entirely. Joining takes 6 to 8
-// us. Other numbers of blocks on a multiprocessor, deeper rings, turns loaded by whole blocks or
-// clusters: none was faster. One stream of 1028 slots: 8 and 5 us, launches and latency.
+// 96 streams of 4100 slots, 16 heads (4) of 128 channels, 214 MB: 58 us (3.7 TB/s); 3 streams
+// of 65,536 slots, 24 heads (8) of 96 channels, 164 MB: 47 us. The first's reading alone
+// takes 40 to 48 us, all but the reading 44, starting and ending about 7 of either: the
+// two do not overlap entirely. Joining takes 6 to 8 us. Between 12 and 20 warps a
+// multiprocessor, deeper rings, turns loaded by whole blocks or clusters: none was faster. One stream of 1028 slots: 8 and 5 us, launches and latency.
 //
 //   scores [slots x heads] = K q^T: a lane's words of two key rows are its parts of
 //     the products, with q's channels permuted alike;
