@@ -253,6 +253,31 @@ def test_repeats_streams_and_graph():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_steps_at_once():
+    """Steps of three batches on three streams at the same time, each its own caches."""
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    shapes = [(1, 8, 2, 64, 200), (40, 16, 4, 128, 300), (7, 3, 3, 96, 1000)]
+
+    def run(streams):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        caches = [window_cache_4bit(b, left, 1, kv, d) for b, _, kv, d, left in shapes]
+        tokens = [[(rand(g, b, h, d, dtype=BF), rand(g, b, kv, d, dtype=BF),
+                    rand(g, b, kv, d, dtype=BF)) for b, h, kv, d, _ in shapes] for _ in range(6)]
+        places = [[torch.full((shape[0],), p, device="cuda") for p in range(6)] for shape in shapes]
+        torch.cuda.synchronize()
+        out = []
+        for p, step in enumerate(tokens):
+            for i, (q, k, v) in enumerate(step):
+                with torch.cuda.stream(streams[i]):
+                    out.append(window_attention_step_4bit(q, k, v, caches[i], places[i][p], first=1))
+        torch.cuda.synchronize()
+        return out + [t for cache in caches for t in cache]
+
+    apart = run([torch.cuda.Stream() for _ in shapes])
+    assert all(torch.equal(a, b) for a, b in zip(run([torch.cuda.current_stream()] * 3), apart))
+
+
 def test_strided_tokens_and_refusals():
     from gaussian_splats_b200.attention import (FourBitCache, window_attention_step_4bit,
                                                 window_cache_4bit)

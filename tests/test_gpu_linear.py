@@ -305,6 +305,50 @@ def test_other_stream_and_graph():
             assert torch.equal(t.detach(), w[n]), n
 
 
+def test_arrays_past_32_bits():
+    """Results, slopes and gradients of more than 2^31 elements: their last rows are those
+    of a call with these rows alone, and all that reaches the weight's gradient."""
+    from gaussian_splats_b200.linear import linear
+
+    rows, tail = 2_200_003, 5001
+    s = make(tail, 8, 1000, BF, BF, None)
+    want = call(s, "gelu")
+    x = torch.zeros(rows, 8, device="cuda", dtype=BF)
+    x[-tail:] = s["x"]
+    leaves = [x.requires_grad_(), s["weight"].requires_grad_()]
+    y = linear(*leaves, s["bias"], activation="gelu")
+    assert y.numel() > 2 ** 31
+    up = torch.ones_like(y)
+    up[-tail:] = s["grad"]
+    dx, dw = torch.autograd.grad(y, leaves, up)
+    assert torch.equal(y[-tail:], want["y"]) and torch.equal(dx[-tail:], want["dx"])
+    assert torch.equal(y[0], y[-tail - 1]) and torch.equal(dx[0], dx[-tail - 1])
+    # Both are sums of the same products in another order, each rounded: dz is at most 1.13 grad.
+    sizes = 1.13 * s["grad"].double().abs().t() @ s["x"].double().abs()
+    bound = 2 * (tail / 16 + 40) * 2.0 ** -23 * sizes + 1.01 * U[BF] * 2 * want["dweight"].double().abs()
+    assert ((dw.double() - want["dweight"].double()).abs() <= 1.01 * bound + 2.0 ** -25).all()
+
+
+def test_calls_at_once():
+    """Products of all kinds on four streams at the same time, with nothing between them."""
+    sets = [(make(3001, 264, 520, BF, FL, FL, seed=1), "gelu"),
+            (make(40, 1030, 300, HF, HF, None, seed=2), "silu"),
+            (make(5000, 59, 72, BF, BF, None, seed=3), "relu"),
+            (make(2000, 1024, 640, HF, None, None, seed=4), None)]
+    want = [call(s, a) for s, a in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(5):
+        for i, stream in enumerate(streams):
+            s, activation = sets[(i + turn) % len(sets)]
+            with torch.cuda.stream(stream):
+                got.append(((i + turn) % len(sets), call(s, activation)))
+    torch.cuda.synchronize()
+    for i, results in got:
+        assert all(torch.equal(results[n], want[i][n]) for n in results), i
+
+
 def test_saved_tensors_may_move():
     """Hooks that take the saved tensors to the host and bring them back otherwise laid out."""
     from gaussian_splats_b200.linear import linear
