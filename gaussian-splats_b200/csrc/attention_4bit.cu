@@ -20,7 +20,7 @@
 // a second kernel joins in order.
 //
 // 96 streams of 4100 slots, 16 heads (4) of 128 channels, 214 MB: 58 us (3.7 TB/s); 3 streams
-// of 65,536 slots, 24 heads (8) of 96 channels, 164 MB: 47 us. The first's reading alone
+// of 65,536 slots, 24 heads (8) of 96 channels, 164 MB: 44 us. The first's reading alone
 // takes 40 to 48 us, all but the reading 44, starting and ending about 7 of either: the
 // two do not overlap entirely. Joining takes 6 to 8 us. Between 12 and 20 warps a
 // multiprocessor, deeper rings, turns loaded by whole blocks or clusters: none was faster. One stream of 1028 slots: 8 and 5 us, launches and latency.
@@ -260,9 +260,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 
 template <int kWords>
 __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)[kWords]) {
-  static_assert(kWords == 1 || kWords == 2 || kWords == 4);
-  if constexpr (kWords == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  static_assert(kWords <= 4);
+  if constexpr (kWords == 1 || kWords == 3) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
   } else if constexpr (kWords == 2) {
     const uint2 x = *reinterpret_cast<const uint2*>(p);
     w[0] = x.x;
@@ -276,15 +277,14 @@ __device__ __forceinline__ void read_words(const unsigned char* p, uint32_t (&w)
   }
 }
 
-// kSets: of 8 heads. kMasked: with validity of the slots. kAligned: rows of codes are
+// kKeyWords: a lane's words of a key's row, which four share. kSets: of 8 heads. kMasked: with validity of the slots. kAligned: rows of codes are
 // whole 16-byte words.
-template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
+template <class T, int kDim, int kKeyWords, int kSets, bool kMasked, bool kAligned>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     step_kernel(gs_window_attention_step_4bit_args a, Parts<kDim> parts, Reach* reach) {
   using S = Shared<kDim>;
   constexpr int kRow = Stage<kDim>::kRow, kStages = Stage<kDim>::kCount;
-  constexpr int kKeyWords = kDim / 32;    // a lane's words of a key's row, of four lanes
-  constexpr int kValueWords = kDim / 64;  // of a value's, of eight
+  constexpr int kValueWords = kDim / 64;  // a lane's words of a value's row, which eight share
   constexpr int kHeads = 8 * kSets;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   S& s = *reinterpret_cast<S*>(shared_bytes);
@@ -775,7 +775,7 @@ int part_heads(const gs_window_attention_step_4bit_args& a, int sets) {
   return std::min(a.heads / a.kv_heads, 8 * sets);
 }
 
-template <class T, int kDim, int kSets, bool kMasked, bool kAligned>
+template <class T, int kDim, int kKeyWords, int kSets, bool kMasked, bool kAligned>
 int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
   const int64_t items = items_of(a, kSets), blocks = blocks_of(a, items, kSets);
   if (items > INT32_MAX) return GS_ERR_CAPACITY;
@@ -784,8 +784,8 @@ int32_t step(const gs_window_attention_step_4bit_args& a, cudaStream_t stream) {
       reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + reach_bytes(items)),
       part_heads(a, kSets)};
   constexpr size_t kShared = sizeof(Shared<kDim>);
-  GS_TRY((allow_shared<step_kernel<T, kDim, kSets, kMasked, kAligned>>(kShared)));
-  launch_chained_shared(step_kernel<T, kDim, kSets, kMasked, kAligned>,
+  GS_TRY((allow_shared<step_kernel<T, kDim, kKeyWords, kSets, kMasked, kAligned>>(kShared)));
+  launch_chained_shared(step_kernel<T, kDim, kKeyWords, kSets, kMasked, kAligned>,
                         dim3(static_cast<unsigned>(blocks)), dim3(kThreads), kShared, stream, a,
                         parts, reach);
   GS_TRY(check_launch());
@@ -849,11 +849,16 @@ int32_t launch_window_attention_step_4bit(const gs_window_attention_step_4bit_ar
     using T = decltype(t);
     const auto shaped = [&](auto masked, auto aligned) {
       constexpr bool kMasked = decltype(masked)::value, kAligned = decltype(aligned)::value;
-      if (sets_of(a) == 1)
-        return a.dim <= 64 ? step<T, 64, 1, kMasked, kAligned>(a, stream)
-                           : step<T, 128, 1, kMasked, kAligned>(a, stream);
-      return a.dim <= 64 ? step<T, 64, 2, kMasked, kAligned>(a, stream)
-                         : step<T, 128, 2, kMasked, kAligned>(a, stream);
+      // Keys of up to 96 channels in three words a lane: 44 us against 47 with four (3
+      // streams of 65,536 slots, 24 heads of 96).
+      const auto with_sets = [&](auto sets) {
+        constexpr int kSets = decltype(sets)::value;
+        return a.dim <= 64   ? step<T, 64, 2, kSets, kMasked, kAligned>(a, stream)
+               : a.dim <= 96 ? step<T, 128, 3, kSets, kMasked, kAligned>(a, stream)
+                             : step<T, 128, 4, kSets, kMasked, kAligned>(a, stream);
+      };
+      return sets_of(a) == 1 ? with_sets(std::integral_constant<int, 1>{})
+                             : with_sets(std::integral_constant<int, 2>{});
     };
     const bool aligned = a.dim % 32 == 0;
     if (a.cache_valid)
