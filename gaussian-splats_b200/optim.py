@@ -176,10 +176,12 @@ class FusedAdam(torch.optim.Adam):
     ``ValueError``. There is no CPU path.
     """
 
+    # Of the last step with a max_norm. Here, since copies are not made by __init__.
+    grad_norm: torch.Tensor | None = None
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                          foreach=False)
-        self.grad_norm: torch.Tensor | None = None  # of the last step with a max_norm
         names = [group.get("name") for group in self.param_groups]
         if sorted(map(str, names)) != sorted(GROUP_NAMES):
             raise ValueError(f"FusedAdam needs one group per name in {GROUP_NAMES}, got {names}")

@@ -100,6 +100,19 @@ def test_clip_checks_arguments():
     assert lib.gs_clip_grad_norm_workspace_size(5000) > lib.gs_clip_grad_norm_workspace_size(5) > 0
 
 
+def test_copied_optimizer_has_a_norm():
+    import copy
+    import pickle
+
+    from gaussian_splats_b200.optim import GROUP_NAMES, FusedAdam
+
+    shapes = [(4, 3), (4, 4), (4, 3), (4, 1), (4, 1, 3)]
+    opt = FusedAdam([{"params": [torch.nn.Parameter(torch.zeros(*shape))], "name": name}
+                     for shape, name in zip(shapes, GROUP_NAMES)])
+    assert opt.grad_norm is None
+    assert copy.deepcopy(opt).grad_norm is None and pickle.loads(pickle.dumps(opt)).grad_norm is None
+
+
 def test_4bit_step_checks_arguments():
     from gaussian_splats_b200 import native
 
