@@ -813,24 +813,29 @@ int32_t run_product(int32_t dtype, const Operand& a, const Operand& b, const Pla
   const auto formed = [&](auto columns, auto pair) {
     constexpr int kN = decltype(columns)::value;
     constexpr bool kPair = decltype(pair)::value;
+    const auto launch = [&](auto form) {
+      return launch_product<T, kN, kRowsA, kRowsB, decltype(form)::value, kPair, kGather>(
+          dtype, a, b, plan, e, stream);
+    };
+    // What is not built for these operands (a float result without a residual, forward) is
+    // the general form's.
     switch (form_of(e)) {
-      case Form::kNarrow:
-        return launch_product<T, kN, kRowsA, kRowsB, Form::kNarrow, kPair, kGather>(dtype, a, b, plan, e, stream);
+      case Form::kNarrow: return launch(std::integral_constant<Form, Form::kNarrow>{});
       case Form::kWide:
-        if constexpr (kRowsA && kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kWide, kPair, kGather>(dtype, a, b, plan, e, stream);
+        if constexpr (kRowsA && kRowsB) return launch(std::integral_constant<Form, Form::kWide>{});
+        break;
       case Form::kActive:
-        if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kActive, kPair, kGather>(dtype, a, b, plan, e, stream);
+        if constexpr (!kRowsB) return launch(std::integral_constant<Form, Form::kActive>{});
+        break;
       case Form::kTraining:
-        if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kTraining, kPair, kGather>(dtype, a, b, plan, e, stream);
+        if constexpr (!kRowsB) return launch(std::integral_constant<Form, Form::kTraining>{});
+        break;
       case Form::kStream:
-        if constexpr (!kRowsB)
-          return launch_product<T, kN, kRowsA, kRowsB, Form::kStream, kPair, kGather>(dtype, a, b, plan, e, stream);
-      default: break;
+        if constexpr (!kRowsB) return launch(std::integral_constant<Form, Form::kStream>{});
+        break;
+      case Form::kAny: break;
     }
-    return launch_product<T, kN, kRowsA, kRowsB, Form::kAny, kPair, kGather>(dtype, a, b, plan, e, stream);
+    return launch(std::integral_constant<Form, Form::kAny>{});
   };
   if constexpr (!kGather)
     if (tile.pair) return formed(std::integral_constant<int, 256>{}, std::true_type{});

@@ -381,3 +381,32 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError):
         linear(x, w.cpu())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("rows,inputs,outputs", [
+    (1, 136, 32), (96, 136, 1024), (300, 59, 128), (640, 64, 4096), (5000, 136, 264),
+    (20003, 72, 520), (9001, 520, 300), (4000, 59, 260), (70, 136, 37)])
+def test_float_results_without_a_residual(rows, inputs, outputs, dtype):
+    """Which only a C caller asks for: rows by TMA and gathered, by pairs of blocks, tiles
+    of every width, results that TMA takes and others."""
+    import ctypes
+
+    from gaussian_splats_b200 import native
+    from gaussian_splats_b200.linear import _operand
+    from gaussian_splats_b200.sequences import call as library
+
+    for bias, activation in ((None, None), (dtype, None), (FL, None), (FL, "gelu")):
+        s = make(rows, inputs, outputs, dtype, bias, None)
+        w = _operand(s["weight"])
+        whole = torch.full((rows * outputs + 4,), 7.0, device="cuda")
+        for offset in (0, 1):  # 1: off its 16-byte borders
+            y = whole[offset:offset + rows * outputs].view(rows, outputs)
+            args = native.LinearArgs(
+                rows=rows, inputs=inputs, outputs=outputs, dtype=1 if dtype == BF else 2,
+                bias_dtype=0 if bias == FL else 1 if dtype == BF else 2, residual_dtype=0,
+                activation=0 if activation is None else 2, x=s["x"].data_ptr(),
+                weight=w.data_ptr(), bias=None if bias is None else s["bias"].data_ptr(),
+                x_stride=inputs, weight_stride=w.stride(0), y=y.data_ptr())
+            library("gs_linear", y.device, ctypes.byref(args))
+            check({"y": y}, s, activation, train=False)
