@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 from .attention import _whole
@@ -125,12 +126,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x's where there is none: a float32 residual stream stays one. Sums, bias, activation
     and the residual's addition are in float32, rounded once.
 
-    Differentiable in x, weight, bias and residual, and deterministic in both
-    directions. The backward rounds the gradient of the sums, ``grad * act'``, to the
-    inputs' type, as its products need; float16 gradients below 6e-8 vanish there, as in
-    any float16 tensor (scale the loss). Operands are read in place if their rows are
-    contiguous and start on 16-byte borders (any slice of a projection does whose
-    channels are multiples of 8) and copied otherwise."""
+    Differentiable in x, weight, bias and residual (in reverse mode; a forward-mode
+    tangent is refused), and deterministic in both directions. The backward rounds the
+    gradient of the sums, ``grad * act'``, to the inputs' type, as its products need;
+    float16 gradients below 6e-8 vanish there, as in any float16 tensor (scale the loss).
+    Operands are read in place if their rows are contiguous and start on 16-byte borders
+    (any slice of a projection does whose channels are multiples of 8) and copied
+    otherwise."""
     what = "linear"
     device = check_cuda(what, x=x, weight=weight, bias=bias, residual=residual)
     element_type(x.dtype, what, _TYPES)
@@ -152,8 +154,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         _check_added(what, "bias", bias, (outputs,), x.dtype)
     if residual is not None:
         _check_added(what, "residual", residual, (*x.shape[:-1], outputs), x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    # Within a level of forward-mode differentiation any of them may carry a tangent, which
+    # the function's call refuses.
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or
+            (bias is not None and bias.requires_grad) or
+            (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation])
     return _forward(x, weight, bias, residual, ACTIVATIONS[activation], False)[0]

@@ -410,3 +410,22 @@ def test_float_results_without_a_residual(rows, inputs, outputs, dtype):
                 x_stride=inputs, weight_stride=w.stride(0), y=y.data_ptr())
             library("gs_linear", y.device, ctypes.byref(args))
             check({"y": y}, s, activation, train=False)
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "bias", "residual"])
+def test_forward_mode_is_refused(name):
+    """A tangent is refused, with reverse-mode gradients or without, and not dropped."""
+    from torch.autograd import forward_ad
+
+    from gaussian_splats_b200.linear import linear
+
+    s = make(5, 16, 8, BF, BF, FL)
+    given = {n: s[n] for n in ("x", "weight", "bias", "residual")}
+    want = linear(*given.values(), activation="silu")
+    with forward_ad.dual_level():
+        assert torch.equal(linear(*given.values(), activation="silu"), want)  # no tangent in it
+        given[name] = forward_ad.make_dual(given[name], torch.ones_like(given[name]))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(NotImplementedError):
+                linear(*given.values(), activation="silu")
+    assert torch.equal(linear(*(s[n] for n in given), activation="silu"), want)
