@@ -1802,7 +1802,7 @@ __global__ void __launch_bounds__(kStepThreads, kDim == 64 ? 4 : 2)
   const int64_t slot = idle                 ? -1
                        : position < a.first ? position
                                             : a.first + (position - a.first) % (a.slots - a.first);
-  const int count = idle ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
+  const int count = idle ? 0 : static_cast<int>(min(position, int64_t{a.slots} - 1)) + 1;
   const int64_t row = int64_t{a.kv_heads} * a.dim;
   T* cache_k = static_cast<T*>(a.cache_k) + b * a.slots * row + kv_head * a.dim;
   T* cache_v = static_cast<T*>(a.cache_v) + b * a.slots * row + kv_head * a.dim;

@@ -98,7 +98,7 @@ struct Stream {
 };
 __device__ __forceinline__ Stream stream_at(const gs_window_attention_step_4bit_args& a, int64_t b) {
   const int64_t position = a.positions[b];
-  const int count = position < 0 ? 0 : static_cast<int>(min(position + 1, int64_t{a.slots}));
+  const int count = position < 0 ? 0 : static_cast<int>(min(position, int64_t{a.slots} - 1)) + 1;
   return {position, count, (count + kSlots - 1) / kSlots};
 }
 

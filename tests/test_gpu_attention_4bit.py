@@ -306,3 +306,26 @@ def test_strided_tokens_and_refusals():
             window_attention_step_4bit(*parts, **args)
     with pytest.raises(RuntimeError):
         window_attention_step_4bit(*parts, FourBitCache(c[0].cpu(), *c[1:]), positions)
+
+
+def test_positions_to_the_last():
+    """The greatest position that there is counts a full cache, in both steps."""
+    from gaussian_splats_b200.attention import (window_attention_step, window_attention_step_4bit,
+                                                window_cache, window_cache_4bit)
+
+    g = torch.Generator(device="cuda").manual_seed(11)
+    last, first, left = 2 ** 63 - 1, 2, 40
+    near = first + left + 1 + (last - first) % (left + 1)  # the same slot, the cache full too
+    q = rand(g, 2, 4, 64, dtype=BF)
+    k, v = (rand(g, 2, 2, 64, dtype=BF) for _ in range(2))
+    results = []
+    for place in (near, last):
+        positions = torch.tensor([place, 5], device="cuda")
+        four, whole = window_cache_4bit(2, left, first, 2, 64), window_cache(2, left, first, 2, 64)
+        gen = torch.Generator(device="cuda").manual_seed(12)
+        for t in (*four, *whole):
+            t.copy_(torch.randint(0, 256, t.shape, generator=gen, device="cuda") if
+                    t.dtype == torch.uint8 else torch.randn(t.shape, generator=gen, device="cuda"))
+        results.append([window_attention_step_4bit(q, k, v, four, positions, first=first),
+                        window_attention_step(q, k, v, *whole, positions, first=first), *four, *whole])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and (results[0][0] != 0).any()
