@@ -73,17 +73,18 @@ struct Shared {
 };
 
 // What a warp leaves of its part of an item, for each of `heads` query heads: outputs
-// times the sum, then the heads' maxima and sums.
+// times the sum, in units of their own, then the heads' maxima, sums and units.
 template <int kDim>
 struct Parts {
   float* data;
   int32_t heads;
-  __host__ __device__ int64_t floats() const { return int64_t{heads} * (kDim + 2) + (heads & 1) * 2; }
+  __host__ __device__ int64_t floats() const { return (int64_t{heads} * (kDim + 3) + 3) / 4 * 4; }
   __device__ float* out(int64_t part, int h) const { return data + part * floats() + h * kDim; }
   __device__ float* top(int64_t part, int h) const {
     return data + part * floats() + heads * kDim + h;
   }
   __device__ float* sum(int64_t part, int h) const { return top(part, h) + heads; }
+  __device__ float* unit(int64_t part, int h) const { return sum(part, h) + heads; }
 };
 
 // The warps that have an item's first and last turn.
@@ -460,7 +461,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   float2 sum[kSets] = {}, middle_sum[kSets] = {}, weight_sum[kSets] = {};
 #pragma unroll
   for (int r = 0; r < kSets; ++r) top[r][0] = top[r][1] = -INFINITY;
-  // Value steps are taken relative to a power of two above the largest so far.
+  // Value steps and middles are taken relative to a power of two above the largest step so
+  // far, so that sums of weights times values stay finite wherever the values are; and above
+  // 2^-60 of the largest middle, for rows without a spread. (A step 2^-21 of another's
+  // that is seen as little as it weighs loses digits of its weight in float16: all of
+  // them together are less than 2^-29 of that other's spread a slot.)
   uint32_t unit = 0;  // its bits
   float per_unit = 1.0f;
 
@@ -498,13 +503,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     {
       const float2 key = unpack2<T>(seen ? ranges.x : 0);
       const float2 value = unpack2<T>(seen ? ranges.y : 0);
-      const uint32_t largest =
-          __reduce_max_sync(0xffffffffu, __float_as_uint(value.x) & 0x7fffffffu);
+      const uint32_t largest = __reduce_max_sync(
+          0xffffffffu, __float_as_uint(fmaxf(fabsf(value.x), 0x1p-60f * fabsf(value.y))));
       if (largest >= unit) {  // the same for the whole warp
         const uint32_t next = min(largest & 0x7f800000u, 0x7e000000u) + 0x00800000u;
         const float shrink = unit ? __uint_as_float(unit) / __uint_as_float(next) : 0.0f;
 #pragma unroll
-        for (int r = 0; r < kSets; ++r) weight_sum[r] = tc::mul2(weight_sum[r], both(shrink));
+        for (int r = 0; r < kSets; ++r) {
+          weight_sum[r] = tc::mul2(weight_sum[r], both(shrink));
+          middle_sum[r] = tc::mul2(middle_sum[r], both(shrink));
+        }
 #pragma unroll
         for (int r = 0; r < kSets; ++r)
 #pragma unroll
@@ -516,7 +524,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
         unit = next;
         per_unit = __uint_as_float(0x7f000000u - next);
       }
-      s.slot[warp][lane] = {both(key.x), both(key.y), both(value.x * per_unit), both(value.y)};
+      s.slot[warp][lane] = {both(key.x), both(key.y), both(value.x * per_unit),
+                            both(value.y * per_unit)};
     }
     __syncwarp();
     Slot of[4];  // the lane's slots as rows of the scores: key_row, + 8, + 16, + 24
@@ -653,7 +662,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   const int64_t item = (b * a.kv_heads + kv_head) * pieces + piece;
   if (lane == 0 && first_turn == 0) reach[item].first = static_cast<int32_t>(me);
   if (lane == 0 && first_turn + turns == stream.turns) reach[item].last = static_cast<int32_t>(me);
-  const float unit_size = __uint_as_float(unit);
 #pragma unroll
   for (int r = 0; r < kSets; ++r)
 #pragma unroll
@@ -669,14 +677,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       if (g == 0) {
         *parts.top(me + item, head) = top[r][e];
         *parts.sum(me + item, head) = total;
+        *parts.unit(me + item, head) = __uint_as_float(unit);
       }
-      // Weights times codes are in units of 2^-24, and the weights in `unit`. Odd channels' come
-      // 16 times as large and on top of their neighbours'.
-      const float size = unit_size * kCodeUnit;
-      const float off = fmaf(-7.5f * unit_size, e ? weight_sum[r].y : weight_sum[r].x, middle);
-      const auto low = [&](float2 x) { return fmaf(e ? x.y : x.x, size, off); };
+      // Weights times codes come 2^-24 as large; odd channels' 16 times as large as that and on
+      // top of their neighbours'.
+      const float off = fmaf(-7.5f, e ? weight_sum[r].y : weight_sum[r].x, middle);
+      const auto low = [&](float2 x) { return fmaf(e ? x.y : x.x, kCodeUnit, off); };
       const auto high = [&](float2 x, float2 both) {
-        return fmaf(e ? both.y - x.y : both.x - x.x, 0.0625f * size, off);
+        return fmaf(e ? both.y - x.y : both.x - x.x, 0.0625f * kCodeUnit, off);
       };
 #pragma unroll
       for (int h = 0; h < kValueWords; ++h)
@@ -699,7 +707,7 @@ template <class T, int kDim, int kSets>
 __global__ void __launch_bounds__(1024)
     join_kernel(gs_window_attention_step_4bit_args a, Parts<kDim> parts, const Reach* reach) {
   constexpr int kHeads = 8 * kSets;
-  __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32];
+  __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32], units[32];
   chain_wait();
   const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
   const int64_t item = blockIdx.x, b = item / pieces / a.kv_heads;
@@ -720,23 +728,36 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     ahead[k] = mine + k * groups < count ? parts.out(from + mine + k * groups, h)[d] : 0.0f;
-  float top = -INFINITY, sum = 0.0f;
-  if (thread < count) top = *parts.top(from + thread, h), sum = *parts.sum(from + thread, h);
-  float whole = top;
-  for (int i = thread + threads; i < count; i += threads) whole = fmaxf(whole, *parts.top(from + i, h));
+  float top = -INFINITY, sum = 0.0f, unit = 0.0f;
+  const auto part_at = [&](int i) {
+    top = *parts.top(from + i, h);
+    sum = *parts.sum(from + i, h);
+    unit = *parts.unit(from + i, h);
+  };
+  if (thread < count) part_at(thread);
+  float whole = top, whole_unit = unit;
+  for (int i = thread + threads; i < count; i += threads) {
+    whole = fmaxf(whole, *parts.top(from + i, h));
+    whole_unit = fmaxf(whole_unit, *parts.unit(from + i, h));
+  }
   whole = warp_max(whole);
-  if ((thread & 31) == 0) tops[thread >> 5] = whole;
+  whole_unit = warp_max(whole_unit);
+  if ((thread & 31) == 0) tops[thread >> 5] = whole, units[thread >> 5] = whole_unit;
   __syncthreads();
-  for (int w = 0; w < threads / 32; ++w) whole = fmaxf(whole, tops[w]);
+  for (int w = 0; w < threads / 32; ++w) {
+    whole = fmaxf(whole, tops[w]);
+    whole_unit = fmaxf(whole_unit, units[w]);
+  }
   const float shift = whole == -INFINITY ? 0.0f : whole;
   float o = 0.0f, total = 0.0f;
   for (int i0 = 0; i0 < count; i0 += kMostParts) {
     __syncthreads();
     const int some = min(kMostParts, count - i0);
     if (thread < some) {
-      if (i0 > 0) top = *parts.top(from + i0 + thread, h), sum = *parts.sum(from + i0 + thread, h);
-      scales[thread] = tc::exp2_approx(top - shift);
-      sums[thread] = sum * scales[thread];
+      if (i0 > 0) part_at(i0 + thread);
+      const float scale = tc::exp2_approx(top - shift);
+      scales[thread] = scale * (unit / whole_unit);
+      sums[thread] = sum * scale;
     }
     __syncthreads();
     int i = mine;
@@ -754,7 +775,7 @@ __global__ void __launch_bounds__(1024)
   __syncthreads();
   if (thread < a.dim) {
     for (int i = 1; i < groups; ++i) o += joined[i * kDim + d];
-    out[d] = from_float<T>(total == 0.0f ? 0.0f : o / total);
+    out[d] = from_float<T>(total == 0.0f ? 0.0f : o / total * whole_unit);
   }
 }
 

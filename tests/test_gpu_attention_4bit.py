@@ -329,3 +329,37 @@ def test_positions_to_the_last():
         results.append([window_attention_step_4bit(q, k, v, four, positions, first=first),
                         window_attention_step(q, k, v, *whole, positions, first=first), *four, *whole])
     assert all(torch.equal(a, b) for a, b in zip(*results)) and (results[0][0] != 0).any()
+
+
+def test_values_of_the_whole_range():
+    """Values next to bfloat16's limits, alone and among small ones, and rows without a
+    spread: finite wherever the definition is."""
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(9)
+    top = torch.finfo(BF).max
+    sizes = [2.0 ** -126, 1e-30, 1.0, 1e30, 1e33, 1e36, 0.4 * top]
+    for heads, kv_heads, dim, slots in ((4, 2, 64, 70), (16, 1, 128, 300), (3, 3, 40, 33)):
+        batch = len(sizes) + 2
+        v = 2.0 * torch.rand(batch, kv_heads, slots, dim, generator=g, device="cuda").double() - 1.0
+        for b, size in enumerate(sizes):
+            v[b] *= size
+        v[-2] = 1e37  # no spread
+        v[-1, :, ::2] *= 1e37  # large and small ones
+        ref = R.Streams(batch, slots, 0, kv_heads, dim, BF, "cuda")
+        for i, (x, kept) in enumerate(((rand(g, *v.shape, dtype=BF), ref.k), (v.to(BF), ref.v))):
+            code, step, middle = R.held(x)
+            ref.codes[i][:], ref.ranges[i][:] = R.packed(code), torch.stack((step, middle), -1)
+            kept[:] = (code.double() - 7.5) * step.double()[..., None] + middle.double()[..., None]
+        ref.seen[:] = True
+        cache = FourBitCache(ref.codes[0].clone(), ref.ranges[0].clone(), ref.codes[1].clone(),
+                             ref.ranges[1].clone())
+        q = rand(g, batch, heads, dim, dtype=BF)
+        k = rand(g, batch, kv_heads, dim, dtype=BF)
+        positions = torch.full((batch,), 5 * slots + 2, device="cuda")
+        out = window_attention_step_4bit(q, k, v[:, :, 1].to(BF), cache, positions)
+        want = ref.step(q, k, v[:, :, 1].to(BF), positions, dim ** -0.5)
+        for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
+            assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
+        assert out.isfinite().all()
+        compare(out, want, BF, dim)
