@@ -73,19 +73,21 @@ struct Shared {
 };
 
 // What a warp leaves of its part of an item, for each of `heads` query heads: outputs
-// times the sum, in units of their own, then the heads' maxima, sums and units.
+// times the sum, then the heads' maxima and sums. A part with a unit of values from 2^20 on is
+// large: its outputs are 2^-64 as large, and its sums negative to show it.
 template <int kDim>
 struct Parts {
   float* data;
   int32_t heads;
-  __host__ __device__ int64_t floats() const { return (int64_t{heads} * (kDim + 3) + 3) / 4 * 4; }
+  __host__ __device__ int64_t floats() const { return int64_t{heads} * (kDim + 2) + (heads & 1) * 2; }
   __device__ float* out(int64_t part, int h) const { return data + part * floats() + h * kDim; }
   __device__ float* top(int64_t part, int h) const {
     return data + part * floats() + heads * kDim + h;
   }
   __device__ float* sum(int64_t part, int h) const { return top(part, h) + heads; }
-  __device__ float* unit(int64_t part, int h) const { return sum(part, h) + heads; }
 };
+constexpr uint32_t kLargeUnit = (127 + 20) << 23;  // 2^20's bits
+constexpr float kLargeScale = 0x1p64f;
 
 // The warps that have an item's first and last turn.
 struct Reach {
@@ -662,6 +664,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   const int64_t item = (b * a.kv_heads + kv_head) * pieces + piece;
   if (lane == 0 && first_turn == 0) reach[item].first = static_cast<int32_t>(me);
   if (lane == 0 && first_turn + turns == stream.turns) reach[item].last = static_cast<int32_t>(me);
+  const bool large = unit >= kLargeUnit;
+  const float unit_size = __uint_as_float(unit) * (large ? 1.0f / kLargeScale : 1.0f);
 #pragma unroll
   for (int r = 0; r < kSets; ++r)
 #pragma unroll
@@ -676,15 +680,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       if (head >= heads) continue;
       if (g == 0) {
         *parts.top(me + item, head) = top[r][e];
-        *parts.sum(me + item, head) = total;
-        *parts.unit(me + item, head) = __uint_as_float(unit);
+        *parts.sum(me + item, head) = large ? -total : total;
       }
-      // Weights times codes come 2^-24 as large; odd channels' 16 times as large as that and on
-      // top of their neighbours'.
-      const float off = fmaf(-7.5f, e ? weight_sum[r].y : weight_sum[r].x, middle);
-      const auto low = [&](float2 x) { return fmaf(e ? x.y : x.x, kCodeUnit, off); };
+      // Weights times codes are in units of 2^-24, and the weights in `unit`. Odd channels' come
+      // 16 times as large and on top of their neighbours'.
+      const float size = unit_size * kCodeUnit;
+      const float off = unit_size * fmaf(-7.5f, e ? weight_sum[r].y : weight_sum[r].x, middle);
+      const auto low = [&](float2 x) { return fmaf(e ? x.y : x.x, size, off); };
       const auto high = [&](float2 x, float2 both) {
-        return fmaf(e ? both.y - x.y : both.x - x.x, 0.0625f * kCodeUnit, off);
+        return fmaf(e ? both.y - x.y : both.x - x.x, 0.0625f * size, off);
       };
 #pragma unroll
       for (int h = 0; h < kValueWords; ++h)
@@ -707,7 +711,7 @@ template <class T, int kDim, int kSets>
 __global__ void __launch_bounds__(1024)
     join_kernel(gs_window_attention_step_4bit_args a, Parts<kDim> parts, const Reach* reach) {
   constexpr int kHeads = 8 * kSets;
-  __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32], units[32];
+  __shared__ float joined[1024], scales[kMostParts], sums[kMostParts], tops[32];
   chain_wait();
   const int group = a.heads / a.kv_heads, pieces = (group + kHeads - 1) / kHeads;
   const int64_t item = blockIdx.x, b = item / pieces / a.kv_heads;
@@ -728,36 +732,28 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     ahead[k] = mine + k * groups < count ? parts.out(from + mine + k * groups, h)[d] : 0.0f;
-  float top = -INFINITY, sum = 0.0f, unit = 0.0f;
-  const auto part_at = [&](int i) {
-    top = *parts.top(from + i, h);
-    sum = *parts.sum(from + i, h);
-    unit = *parts.unit(from + i, h);
-  };
-  if (thread < count) part_at(thread);
-  float whole = top, whole_unit = unit;
+  float top = -INFINITY, sum = 0.0f;
+  if (thread < count) top = *parts.top(from + thread, h), sum = *parts.sum(from + thread, h);
+  float whole = top;
+  bool large = signbit(sum);
   for (int i = thread + threads; i < count; i += threads) {
     whole = fmaxf(whole, *parts.top(from + i, h));
-    whole_unit = fmaxf(whole_unit, *parts.unit(from + i, h));
+    large = large || signbit(*parts.sum(from + i, h));
   }
   whole = warp_max(whole);
-  whole_unit = warp_max(whole_unit);
-  if ((thread & 31) == 0) tops[thread >> 5] = whole, units[thread >> 5] = whole_unit;
-  __syncthreads();
-  for (int w = 0; w < threads / 32; ++w) {
-    whole = fmaxf(whole, tops[w]);
-    whole_unit = fmaxf(whole_unit, units[w]);
-  }
+  if ((thread & 31) == 0) tops[thread >> 5] = whole;
+  const bool any_large = __syncthreads_or(large);
+  for (int w = 0; w < threads / 32; ++w) whole = fmaxf(whole, tops[w]);
   const float shift = whole == -INFINITY ? 0.0f : whole;
   float o = 0.0f, total = 0.0f;
   for (int i0 = 0; i0 < count; i0 += kMostParts) {
     __syncthreads();
     const int some = min(kMostParts, count - i0);
     if (thread < some) {
-      if (i0 > 0) part_at(i0 + thread);
+      if (i0 > 0) top = *parts.top(from + i0 + thread, h), sum = *parts.sum(from + i0 + thread, h);
       const float scale = tc::exp2_approx(top - shift);
-      scales[thread] = scale * (unit / whole_unit);
-      sums[thread] = sum * scale;
+      scales[thread] = any_large && !signbit(sum) ? scale / kLargeScale : scale;
+      sums[thread] = fabsf(sum) * scale;
     }
     __syncthreads();
     int i = mine;
@@ -775,7 +771,7 @@ __global__ void __launch_bounds__(1024)
   __syncthreads();
   if (thread < a.dim) {
     for (int i = 1; i < groups; ++i) o += joined[i * kDim + d];
-    out[d] = from_float<T>(total == 0.0f ? 0.0f : o / total * whole_unit);
+    out[d] = from_float<T>(total == 0.0f ? 0.0f : any_large ? o / total * kLargeScale : o / total);
   }
 }
 
