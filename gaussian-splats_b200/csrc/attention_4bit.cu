@@ -198,7 +198,10 @@ __device__ __forceinline__ Fresh round_row(const T* row, int dim) {
     high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
     low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
-  const T step = from_float<T>((high - low) / 15.0f);
+  // Where the spread leaves float's range, by halves.
+  const float spread = high - low;
+  const T step = from_float<T>(isinf(spread) ? (0.5f * high - 0.5f * low) / 15.0f * 2.0f
+                                             : spread / 15.0f);
   const T middle = from_float<T>(0.5f * high + 0.5f * low);
   Fresh f = {0, 0};
   if (8 * word < dim)

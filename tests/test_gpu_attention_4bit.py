@@ -363,3 +363,26 @@ def test_values_of_the_whole_range():
             assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
         assert out.isfinite().all()
         compare(out, want, BF, dim)
+
+
+@pytest.mark.parametrize("side", ["keys", "values"])
+def test_rows_of_the_whole_range(side):
+    """A row whose greatest and least channel lie further apart than float32 reaches is
+    held as the definition has it."""
+    from gaussian_splats_b200.attention import window_attention_step_4bit, window_cache_4bit
+
+    top = torch.finfo(BF).max
+    wide = torch.stack([torch.linspace(-0.9, 0.9, 32).double() * top,
+                        torch.tensor([-0.6 * top] * 31 + [0.6 * top]).double(),
+                        torch.linspace(-1.0, 1.0, 32).double()]).to(BF).cuda()[:, None]
+    one = torch.linspace(-1.0, 1.0, 32).to(BF).cuda().expand(3, 1, 32)
+    k, v = (wide, one) if side == "keys" else (one, wide)
+    cache = window_cache_4bit(3, 4, 0, 1, 32)
+    ref = R.Streams(3, 5, 0, 1, 32, BF, "cuda")
+    q = torch.zeros(3, 1, 32, device="cuda", dtype=BF)
+    positions = torch.zeros(3, dtype=torch.int64, device="cuda")
+    out = window_attention_step_4bit(q, k, v, cache, positions)
+    want = ref.step(q, k, v, positions, 32 ** -0.5)
+    for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
+        assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
+    compare(out, want, BF, 32)
