@@ -88,6 +88,7 @@ struct Parts {
 };
 constexpr uint32_t kLargeUnit = (127 + 20) << 23;  // 2^20's bits
 constexpr float kLargeScale = 0x1p64f;
+constexpr float kFar = 0x1p64f;  // of queries' channels
 
 // The warps that have an item's first and last turn.
 struct Reach {
@@ -421,6 +422,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   // Of the lane's columns, heads 2j and 2j + 1: what takes their dots to those with c - 7.5,
   // and the sums of q; both in base 2.
   float2 dot_scale[kSets], dot_offset[kSets], q_sum[kSets];
+  // Where a head's q has channels from 2^64 on, these are 2^-64 as large and the keys' ranges
+  // 2^64: then no part of a score leaves float's range that the score does not.
+  constexpr bool kWideRange = std::is_same_v<T, __nv_bfloat16>;  // float16 ends at 2^16
+  bool far[kSets], any_far = false;
 #pragma unroll
   for (int r = 0; r < kSets; ++r) {
     float x[kKeyWords][8], total = 0.0f, largest = 0.0f;
@@ -434,16 +439,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
                          (head0 + g + 8 * r) * a.q_head_stride + channel,
                      x[w]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        total += x[w][k];
-        largest = max_nan(largest, fabsf(x[w][k]));
-      }
+      for (int k = 0; k < 8; ++k) largest = max_nan(largest, fabsf(x[w][k]));
     }
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int o = 1; o < 4; o <<= 1)
       largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    }
+    far[r] = kWideRange && __any_sync(0xffffffffu, largest >= kFar);
+    any_far = any_far || far[r];
+    const float shrink = far[r] ? 1.0f / kFar : 1.0f;
+#pragma unroll
+    for (int w = 0; w < kKeyWords; ++w)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) total += x[w][k] * shrink;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const uint32_t exponent = max(__float_as_uint(largest) & 0x7f800000u, 11u << 23);
     const float up = __uint_as_float((264u << 23) - exponent);
     const float down = __uint_as_float((254u << 23) - __float_as_uint(up));
@@ -457,10 +466,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     const auto heads_of = [&](float x) {
       return make_float2(__shfl_sync(0xffffffffu, x, 8 * j), __shfl_sync(0xffffffffu, x, 8 * j + 4));
     };
-    dot_scale[r] = heads_of(kCodeUnit * down * scale);
+    dot_scale[r] = heads_of(kCodeUnit * (down * shrink) * scale);
     dot_offset[r] = heads_of(-7.5f * total * scale);
     q_sum[r] = heads_of(total * scale);
   }
+#pragma unroll
+  for (int r = 0; r < kSets; ++r)
+    if (any_far && !far[r]) {
+      dot_scale[r] = tc::mul2(dot_scale[r], both(1.0f / kFar));
+      dot_offset[r] = tc::mul2(dot_offset[r], both(1.0f / kFar));
+      q_sum[r] = tc::mul2(q_sum[r], both(1.0f / kFar));
+    }
   float2 out[kSets][kValueWords][4][2] = {};  // of both heads: channels e, and e + 4
   float top[kSets][2];
   float2 sum[kSets] = {}, middle_sum[kSets] = {}, weight_sum[kSets] = {};
@@ -506,7 +522,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     // A slot a lane: its ranges, zeros where it is not seen.
     const uint32_t visible = __ballot_sync(0xffffffffu, seen);
     {
-      const float2 key = unpack2<T>(seen ? ranges.x : 0);
+      float2 key = unpack2<T>(seen ? ranges.x : 0);
+      if (any_far) key = tc::mul2(key, both(kFar));
       const float2 value = unpack2<T>(seen ? ranges.y : 0);
       const uint32_t largest = __reduce_max_sync(
           0xffffffffu, __float_as_uint(fmaxf(fabsf(value.x), 0x1p-60f * fabsf(value.y))));

@@ -386,3 +386,27 @@ def test_rows_of_the_whole_range(side):
     for i, (codes, ranges) in enumerate((cache[:2], cache[2:])):
         assert torch.equal(codes, ref.codes[i]) and torch.equal(ranges, ref.ranges[i])
     compare(out, want, BF, 32)
+
+
+@pytest.mark.parametrize("power", [-120, -64, 60, 64, 100, 112, 120, 126])
+def test_queries_of_the_whole_range(power):
+    """Queries of any size against keys of its inverse: the scores are those of 1 and 1."""
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(10)
+    for heads, kv_heads, dim, slots in ((4, 2, 64, 70), (16, 1, 128, 300), (3, 3, 40, 33)):
+        batch = 3
+        q = (rand(g, batch, heads, dim, dtype=BF).clamp(-1.9, 1.9).double() * 2.0 ** power).to(BF)
+        ref = R.Streams(batch, slots, 0, kv_heads, dim, BF, "cuda")
+        fill(ref, g, BF, batch, kv_heads, slots, dim)
+        keys = (rand(g, batch, kv_heads, slots, dim, dtype=BF).double() * 2.0 ** -power).to(BF)
+        code, step, middle = R.held(keys)
+        ref.codes[0][:], ref.ranges[0][:] = R.packed(code), torch.stack((step, middle), -1)
+        ref.k[:] = (code.double() - 7.5) * step.double()[..., None] + middle.double()[..., None]
+        cache = FourBitCache(ref.codes[0].clone(), ref.ranges[0].clone(), ref.codes[1].clone(),
+                             ref.ranges[1].clone())
+        k, v = keys[:, :, 0].contiguous(), rand(g, batch, kv_heads, dim, dtype=BF)
+        positions = torch.full((batch,), 3 * slots + 2, device="cuda")
+        out = window_attention_step_4bit(q, k, v, cache, positions)
+        assert out.isfinite().all()
+        compare(out, ref.step(q, k, v, positions, dim ** -0.5), BF, dim)
