@@ -37,7 +37,7 @@ using namespace tc;
 // the error is 1.02e-5 at most, where float16's would be 2.4e-4 next to 1 and add
 // to the rounding of dz, which has 11 bits in float16 itself. 0 and 1 are exact, and NaN,
 // whose low bits are all ones, is the code that no slope has. (A float32 bias's gradient
-// is a sum of unrounded dz: there slopes are kept as floats.)
+// is a sum of unrounded dz: for it slopes can be kept as floats.)
 constexpr float kSlopeScale = 49152.0f, kSlopeZero = 8192.0f, kTwo23 = 8388608.0f;
 __device__ __forceinline__ uint32_t slope_codes(float2 slopes) {
   // The sums' low bits are the nearest whole numbers.
@@ -1175,7 +1175,7 @@ int32_t launch_linear(const gs_linear_args& a, cudaStream_t stream) {
   e.residual_stride = a.residual_stride;
   e.slope = a.activation == GS_IDENTITY ? nullptr : a.slope;
   e.slope_stride = slope_stride(a);
-  e.slope_float = a.bias && a.bias_dtype == GS_FLOAT32;
+  e.slope_float = a.slope_float != 0;
   e.tiled = tma_rows(a.y, a.outputs, a.residual_dtype, a.outputs) &&
             (!a.residual ||
              tma_rows(a.residual, a.residual_stride, a.residual_dtype, a.outputs));
@@ -1232,7 +1232,7 @@ int32_t launch_linear_backward(const gs_linear_args& a, cudaStream_t stream) {
       const auto with_slopes = [&](auto g) {
         if (a.activation == GS_IDENTITY)
           with_whole(g, std::integral_constant<Slopes, Slopes::kNone>{});
-        else if (a.bias && a.bias_dtype == GS_FLOAT32)
+        else if (a.slope_float)
           with_whole(g, std::integral_constant<Slopes, Slopes::kFloats>{});
         else
           with_whole(g, std::integral_constant<Slopes, Slopes::kCodes>{});

@@ -52,6 +52,10 @@ def _arguments(x, weight, bias, **values):
         weight_stride=weight.stride(0), **values)
 
 
+def _in_float(slope: torch.Tensor | None) -> int:
+    return int(slope is not None and slope.dtype == torch.float32)
+
+
 def _forward(x, weight, bias, residual, activation, train):
     """The result, and what the backward keeps."""
     outputs, inputs = weight.shape
@@ -71,7 +75,7 @@ def _forward(x, weight, bias, residual, activation, train):
                             dtype=torch.float32 if exact else torch.int16)
     args = _arguments(rows, w, b, activation=activation, residual_dtype=_CODES[y.dtype],
                       residual=address(res), residual_stride=stride, y=y.data_ptr(),
-                      slope=address(slope))
+                      slope=address(slope), slope_float=_in_float(slope))
     call("gs_linear", x.device, ctypes.byref(args))
     return y, (rows, w, b, slope)
 
@@ -99,7 +103,7 @@ class _Linear(torch.autograd.Function):
             rows = _whole(grad_y.reshape(x.shape[0], weight.shape[0]))
             args = _arguments(x, weight, bias, activation=ctx.activation,
                               residual_dtype=_CODES[rows.dtype], slope=address(slope),
-                              grad_y=address(rows), grad_x=address(grads[0]),
+                              slope_float=_in_float(slope), grad_y=address(rows), grad_x=address(grads[0]),
                               grad_weight=address(grads[1]), grad_bias=address(grads[2]))
             size = native.lib().gs_linear_workspace_size(ctypes.byref(args))
             workspace = x.new_empty((size,), dtype=torch.uint8)

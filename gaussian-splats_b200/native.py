@@ -282,7 +282,8 @@ class LinearArgs(ctypes.Structure):
                 _fields(ctypes.c_int64, "x_stride weight_stride residual_stride") +
                 _fields(ctypes.c_void_p, "y slope grad_y grad_x grad_weight grad_bias "
                                          "workspace") +
-                _fields(ctypes.c_uint64, "workspace_size"))
+                _fields(ctypes.c_uint64, "workspace_size") +
+                _fields(ctypes.c_int32, "slope_float"))
 
 
 VIEW_RECORD_WORDS = 29  # gs_params (17 words) + camera rotation (9) + translation (3)

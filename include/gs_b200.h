@@ -699,11 +699,13 @@ int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
  * residual [rows, outputs] of residual_dtype with a row stride (may be NULL); both
  * types are dtype or GS_FLOAT32. y [rows, outputs] of residual_dtype, contiguous.
  * `slope` [rows, outputs rounded up to 8], 16-byte aligned, receives act'(z) for the
- * backward (NULL: not kept): floats where there is a bias of GS_FLOAT32, else 16 bits,
- * (act' + 1/6) * 49152 rounded. Sums and epilogue in float.
+ * backward (NULL: not kept): floats if slope_float != 0 (for a float bias's gradient, which
+ * is a sum of unrounded dz), else 16 bits, (act' + 1/6) * 49152 rounded, an error of 1.02e-5
+ * at most. Sums and epilogue in float.
  *
  * The backward reads x, weight, grad_y (contiguous, residual_dtype) and, unless the
- * activation is GS_IDENTITY, slope, and writes those of grad_x [rows, inputs],
+ * activation is GS_IDENTITY, slope, which slope_float has to describe as in the forward;
+ * it does not look at bias and residual. It writes those of grad_x [rows, inputs],
  * grad_weight [outputs, inputs] (both of dtype, contiguous) and grad_bias [outputs]
  * (bias_dtype) that are not NULL; what reaches the products is dz = grad_y act'(z)
  * rounded to dtype. It needs a workspace of gs_linear_workspace_size bytes, 256-byte
@@ -722,6 +724,7 @@ typedef struct gs_linear_args {
   void *grad_x, *grad_weight, *grad_bias;
   void *workspace;
   uint64_t workspace_size;
+  int32_t slope_float;
 } gs_linear_args;
 
 uint64_t gs_linear_workspace_size(const gs_linear_args *args);

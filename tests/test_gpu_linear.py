@@ -429,3 +429,42 @@ def test_forward_mode_is_refused(name):
             with mode(), pytest.raises(NotImplementedError):
                 linear(*given.values(), activation="silu")
     assert torch.equal(linear(*(s[n] for n in given), activation="silu"), want)
+
+
+@pytest.mark.parametrize("bias", [None, BF, FL], ids=str)
+def test_backward_without_the_bias(bias):
+    """A C caller's backward need not have the bias, whose values it does not read; the
+    arguments say how the slopes are held."""
+    import ctypes
+
+    from gaussian_splats_b200 import native
+    from gaussian_splats_b200.sequences import call as library
+
+    rows, inputs, outputs = 700, 136, 264
+    s = make(rows, inputs, outputs, BF, bias, None)
+    want = call(s, "gelu")
+    for slope_float in (0, 1):
+        slope = torch.empty(rows, outputs, device="cuda", dtype=FL if slope_float else torch.int16)
+        y = torch.empty(rows, outputs, device="cuda", dtype=BF)
+        args = native.LinearArgs(
+            rows=rows, inputs=inputs, outputs=outputs, dtype=1, bias_dtype=1 if bias == BF else 0,
+            residual_dtype=1, activation=2, x=s["x"].data_ptr(), weight=s["weight"].data_ptr(),
+            bias=None if bias is None else s["bias"].data_ptr(), x_stride=inputs,
+            weight_stride=inputs, y=y.data_ptr(), slope=slope.data_ptr(), slope_float=slope_float)
+        library("gs_linear", y.device, ctypes.byref(args))
+        assert torch.equal(y, want["y"])
+        grads = {"dx": torch.empty_like(s["x"]), "dweight": torch.empty_like(s["weight"]),
+                 "dbias": torch.empty(outputs, device="cuda", dtype=BF if bias == BF else FL)}
+        args.bias = None
+        args.grad_y, args.grad_x = s["grad"].data_ptr(), grads["dx"].data_ptr()
+        args.grad_weight, args.grad_bias = grads["dweight"].data_ptr(), grads["dbias"].data_ptr()
+        size = native.lib().gs_linear_workspace_size(ctypes.byref(args))
+        workspace = torch.empty(size, device="cuda", dtype=torch.uint8)
+        args.workspace, args.workspace_size = workspace.data_ptr(), size
+        library("gs_linear_backward", y.device, ctypes.byref(args))
+        if bias is None:  # its gradient is written all the same
+            check({n: grads[n] for n in ("dx", "dweight")}, s, "gelu")
+        else:
+            check(grads, s, "gelu")
+            if slope_float == (bias == FL):  # as the function holds them
+                assert all(torch.equal(grads[n], want[n]) for n in grads)
