@@ -468,3 +468,31 @@ def test_backward_without_the_bias(bias):
             check(grads, s, "gelu")
             if slope_float == (bias == FL):  # as the function holds them
                 assert all(torch.equal(grads[n], want[n]) for n in grads)
+
+
+@pytest.mark.parametrize("dtype,bias", [(BF, FL), (HF, FL), (BF, BF), (HF, HF)], ids=str)
+@pytest.mark.parametrize("activation", [None, "gelu", "silu"])
+@pytest.mark.parametrize("rows,inputs,outputs", [(1, 8, 1000), (1, 8, 1001), (300, 24, 264)])
+def test_gradient_of_the_bias(rows, inputs, outputs, activation, dtype, bias):
+    """It is a sum of dz before its rounding to the inputs' type, with slopes that are exact
+    to their own errors where the bias is float32: exponentials and reciprocals of 2^-22,
+    a polynomial of 1.6e-7 and a dozen roundings of 2^-24, times 1.13 at most, less than
+    2e-6 together; 1.02e-5 more where slopes are held in 16 bits. The sum is `rows` floats'.
+    A float16 result below 2^-14 is rounded to steps of 2^-24."""
+    s = make(rows, inputs, outputs, dtype, bias, None)
+    got = call(s, activation)["dbias"]
+    ref = R.linear(s["x"], s["weight"], s["bias"], None, activation, s["grad"])
+    g, unit = s["grad"].double().abs(), 2.0 ** -23
+    slope = 0.0 if activation is None else \
+        2e-6 + 0.8 * (inputs / 16 + 6) * unit * ref["size"] + (0.0 if bias == FL else 1.02e-5)
+    inner = (g * slope).sum(0) + (0.0 if rows == 1 else rows * unit / 2) * \
+        (ref["dz"].abs() + g * slope).sum(0) + unit * ref["dz"].abs().sum(0)
+    limit = 1.01 * (inner + U[bias] * ref["dbias"].abs() + (2.0 ** -25 if bias == HF else 0.0))
+    error = (got.double() - ref["dbias"]).abs()
+    assert (error <= limit).all(), f"{(error - limit).max().item():.3g} beyond"
+    if bias == FL and activation:  # neither rounded dz nor slopes in 16 bits would do
+        rounded = (ref["dz"].to(dtype).double().sum(0) - ref["dbias"]).abs()
+        assert (rounded > limit).any()
+        if rows == 1:
+            codes = ((ref["slope"] + 1 / 6) * 49152).round() / 49152 - 1 / 6
+            assert (((s["grad"].double() * codes).sum(0) - ref["dbias"]).abs() > limit).any()
