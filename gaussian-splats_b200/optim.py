@@ -93,7 +93,7 @@ def grad_norm(tensors: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor:
     (float32, bfloat16 and float16, on one device, any strides and sizes) as a
     float32 scalar on their device, without a wait. One pass over the data; sums
     in float32 over 128 bytes of elements and in float64 beyond that, so that no
-    finite norm overflows on the way; the same result every time."""
+    finite norm overflows on the way; the same result every time. No gradient."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError("grad_norm needs at least one tensor")
@@ -107,18 +107,20 @@ def clip_grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: 
     """Multiplies the ``.grad`` of all ``parameters`` by ``min(1, max_norm / (norm
     + 1e-6))``, ``norm`` their :func:`grad_norm`, and returns the norm from before
     (``torch.nn.utils.clip_grad_norm_`` with the 2-norm). Parameters without a
-    gradient are passed over, one listed twice counts once; nothing is written
-    where the norm is small enough. An infinity makes the factor 0 and a NaN makes
-    it NaN, for every gradient; ``error_if_nonfinite`` raises instead, before
-    anything is written, which costs a wait for the norm. Gradients may be float32,
-    bfloat16 or float16 in any mixture and of any strides, on one device; an element
-    that two of them share counts twice and is multiplied once."""
+    gradient are passed over, one listed twice counts once; where the norm is small
+    enough, every gradient keeps its values (those that lie in one run of memory,
+    apart from the others, are not written at all). An infinity makes the factor 0 and
+    a NaN makes it NaN, for every gradient, as an infinity does where ``max_norm`` is
+    one itself; ``error_if_nonfinite`` raises instead, before anything is written, which
+    costs a wait for the norm. Gradients may be float32, bfloat16 or float16 in any
+    mixture and of any strides, on one device; an element that two of them share counts
+    twice and is multiplied once. No gradient."""
     what = "clip_grad_norm"
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = _max_norm(what, max_norm)
     if not parameters:
         raise ValueError(f"{what} needs at least one parameter")
-    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
+    grads = [g for p in {id(p): p for p in parameters}.values() if (g := p.grad) is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=parameters[0].device)
     tensors, copies, spans = list(grads), [], []

@@ -237,3 +237,19 @@ def test_clipped_step(n, max_norm):
     assert fused.grad_norm is None
     with pytest.raises(ValueError):
         fused.step(max_norm=-1.0)
+
+
+def test_parameters_with_one_gradient():
+    """Two parameters whose gradient is one tensor: it counts twice and is multiplied once."""
+    from gaussian_splats_b200.optim import clip_grad_norm
+
+    g, other = rand(1, 1000), rand(2, 50, dtype=BF)
+    kept, kept_other = g.double(), other.double()
+    a, b, c = parameters([g, g, other])
+    want = R.norm([g, g, other])
+    norm = clip_grad_norm([a, b, c, b], 1.0)
+    assert abs(norm.item() - want) <= NORM * want
+    f = R.factor(want, 1.0)
+    for t, k in ((g, kept), (other, kept_other)):
+        assert ((t.double() - f * k).abs() <= 1.01 * (NORM + 2.0 ** -23 + U[t.dtype]) *
+                (f * k).abs()).all()
