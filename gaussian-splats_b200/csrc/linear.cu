@@ -1077,8 +1077,9 @@ int32_t with_sixteen_bit(int32_t dtype, F&& f) {
 
 int64_t slope_stride(const gs_linear_args& a) { return round_up(a.outputs, 8); }
 
-// The backward's workspace: dz (where grad_y cannot be read in its place), the strips'
-// sums of dz, the splits' sums of dz^T x.
+// The backward's workspace: dz (where grad_y cannot be read in its place, and more than the
+// bias's gradient is wanted), the strips' sums of dz, the splits' sums of dz^T x (where there
+// are several splits: one writes the gradient itself).
 struct BackwardPlan {
   bool own_dz;
   Strips strips;
@@ -1122,10 +1123,12 @@ BackwardPlan backward_plan(const gs_linear_args& a) {
     at += (bytes + 255) / 256 * 256;
     return from;
   };
-  p.dz = take(p.own_dz ? static_cast<uint64_t>(a.rows) * slope_stride(a) * 2 : 0);
+  const bool bias_only = a.grad_bias && !a.grad_x && !a.grad_weight;
+  p.dz = take(p.own_dz && !bias_only ? static_cast<uint64_t>(a.rows) * slope_stride(a) * 2 : 0);
   p.sums = take(static_cast<uint64_t>(p.strips.count) * a.outputs * 4);
-  p.parts = take(static_cast<uint64_t>(p.weight.splits) * p.weight.split_rows *
-                 round_up(a.inputs, 4) * 4);
+  p.parts = take(p.weight.splits == 1 ? 0
+                                      : static_cast<uint64_t>(p.weight.splits) *
+                                            p.weight.split_rows * round_up(a.inputs, 4) * 4);
   p.size = at;
   return p;
 }

@@ -708,8 +708,8 @@ int32_t gs_rms_norm_backward(const gs_rms_norm_args *args, gs_stream_t stream);
  * it does not look at bias and residual. It writes those of grad_x [rows, inputs],
  * grad_weight [outputs, inputs] (both of dtype, contiguous) and grad_bias [outputs]
  * (bias_dtype) that are not NULL; what reaches the products is dz = grad_y act'(z)
- * rounded to dtype. It needs a workspace of gs_linear_workspace_size bytes, 256-byte
- * aligned. x and grad_y are 16-byte aligned here and x has a stride as the weight,
+ * rounded to dtype. It needs a workspace of gs_linear_workspace_size bytes, of the same
+ * arguments, 256-byte aligned. x and grad_y are 16-byte aligned here and x has a stride as the weight,
  * grad_weight is 8-byte aligned; everything else lies as its type allows (16-byte
  * aligned and of whole 16-byte rows is faster). No atomics: results repeat bit for bit. */
 enum { GS_IDENTITY = 0, GS_RELU = 1, GS_GELU = 2, GS_SILU = 3 }; /* activations */

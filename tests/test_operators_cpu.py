@@ -170,3 +170,26 @@ def test_oracle_codes():
     assert step.item() == 1.0 and middle.item() == 7.5
     assert code.tolist() == [[0, 1, 15, 0, 2, 8]]
     assert R.held(torch.full((1, 4), 3.0).half())[0].tolist() == [[8] * 4]
+
+
+def test_linear_workspace_holds_what_is_used():
+    """The gradient of the sums where a product reads it from there, and the splits' sums
+    where there are several."""
+    from gaussian_splats_b200 import native
+
+    def size(rows, inputs, outputs, wanted="xwb", **more):
+        a = 256
+        args = native.LinearArgs(**{**dict(
+            rows=rows, inputs=inputs, outputs=outputs, dtype=1, bias_dtype=1, residual_dtype=1,
+            activation=2, x=a, weight=a, x_stride=inputs, weight_stride=inputs,
+            grad_x=a if "x" in wanted else None, grad_weight=a if "w" in wanted else None,
+            grad_bias=a if "b" in wanted else None), **more})
+        return native.lib().gs_linear_workspace_size(ctypes.byref(args))
+
+    dz, strips = 1000 * 8192 * 2, 1000 * 8192 * 4 // 4  # four rows a strip at least
+    assert dz < size(1000, 8192, 8192) <= dz + strips + 1024
+    assert size(1000, 65536, 65536) < 2 ** 30
+    assert size(1000, 8192, 8192, "b") <= strips + 1024
+    assert size(1000, 8192, 8192, "") == size(1000, 8192, 8192) == size(1000, 8192, 8192, "x")
+    assert size(1000, 8192, 8192, activation=0) <= strips + 1024  # grad_y is read in its place
+    assert size(100000, 256, 256, "w", activation=0) >= 18 * 256 * 256 * 4
