@@ -29,14 +29,21 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_FLOAT32, 
 _GATHERED = 128
 
 
+def _lies_as_operand(t: torch.Tensor) -> bool:
+    row, channel = t.stride()
+    return channel == 1 and row % 8 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0
+
+
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, channels] as the kernels read a product's operand: rows of contiguous
     channels that start on 16-byte borders. ``t`` itself if it lies so, else a copy."""
-    (row, channel), (rows, channels) = t.stride(), t.shape
-    if channel == 1 and row % 8 == 0 and row >= channels and t.data_ptr() % 16 == 0:
+    rows, channels = t.shape
+    if _lies_as_operand(t):
         return t
-    if channel != 1:
+    if t.stride(1) != 1:
         t = t.contiguous()
+        if _lies_as_operand(t):
+            return t
     copy = t.new_empty((rows, -(-channels // 8) * 8))
     call("gs_align_rows", t.device, rows, channels, t.data_ptr(), t.stride(0), copy.data_ptr())
     return copy[:, :channels]

@@ -193,3 +193,19 @@ def test_linear_workspace_holds_what_is_used():
     assert size(1000, 8192, 8192, "") == size(1000, 8192, 8192) == size(1000, 8192, 8192, "x")
     assert size(1000, 8192, 8192, activation=0) <= strips + 1024  # grad_y is read in its place
     assert size(100000, 256, 256, "w", activation=0) >= 18 * 256 * 256 * 4
+
+
+def test_operands_are_copied_once(monkeypatch):
+    """A transposed operand by torch, where that makes it whole 16-byte words, and by the
+    kernel that aligns rows only where it does not."""
+    from gaussian_splats_b200 import linear as L
+
+    calls = []
+    monkeypatch.setattr(L, "call", lambda name, *args: calls.append(name))
+    t = torch.zeros(64, 48, dtype=torch.bfloat16)
+    assert L._operand(t) is t and L._operand(t[:, 8:24]).data_ptr() == t[:, 8:].data_ptr()
+    turned = L._operand(t.t())
+    assert calls == [] and turned.shape == (48, 64) and turned.is_contiguous()
+    for other in (t[:, 1:9], t.view(-1)[:45].view(9, 5), t[:5].t(), t[:1].expand(9, 48)):
+        assert L._operand(other).shape == other.shape
+        assert calls.pop() == "gs_align_rows" and calls == []
