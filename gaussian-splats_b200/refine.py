@@ -207,7 +207,11 @@ class SplatRefiner(nn.Module):
         """Switches the products behind a norm to 8 bits for calls without
         gradients. Their weights are rounded here, and again by the first such call
         after they have changed in place; training goes on in bfloat16, and what
-        ``state_dict`` saves is the bfloat16 weights."""
+        ``state_dict`` saves is the bfloat16 weights. 8-bit products have outputs in
+        multiples of 16, so ``hidden`` has to be one."""
+        if self.shape.hidden % 16:
+            raise ValueError(f"8-bit products take a hidden layer of a multiple of 16 channels, "
+                             f"not of {self.shape.hidden}")
         for block in self.blocks:
             block.qkv.quantize()
             block.mix.quantize()

@@ -209,3 +209,15 @@ def test_operands_are_copied_once(monkeypatch):
     for other in (t[:, 1:9], t.view(-1)[:45].view(9, 5), t[:5].t(), t[:1].expand(9, 48)):
         assert L._operand(other).shape == other.shape
         assert calls.pop() == "gs_align_rows" and calls == []
+
+
+def test_refiner_with_a_hidden_layer_that_8_bit_products_do_not_take():
+    from gaussian_splats_b200.refine import RefinerShape, SplatRefiner
+
+    refiner = SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1, hidden=40), device="cpu")
+    with pytest.raises(ValueError, match="multiple of 16"):
+        refiner.quantize()
+    assert all(block.qkv.codes is None for block in refiner.blocks)  # nothing is switched
+    for hidden in (0, 48):
+        SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1, hidden=hidden),
+                     device="cpu").quantize()
