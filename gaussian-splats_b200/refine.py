@@ -144,6 +144,11 @@ class _Block(nn.Module):
         self.mix_out = _Product(shape.width, shape.width, device)
         self.feed = _FeedForward(shape.width, shape.hidden, device) if shape.hidden else None
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "feed" not in self._modules:
+            self.__dict__.setdefault("feed", None)  # of a block saved before there were any
+
     def _normed(self, x, residual, weight, product):
         """The product of the norm of ``x + residual``, the sum, and the norm itself
         (codes and scale where the products are in 8 bits)."""

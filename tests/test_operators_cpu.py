@@ -221,3 +221,20 @@ def test_refiner_with_a_hidden_layer_that_8_bit_products_do_not_take():
     for hidden in (0, 48):
         SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1, hidden=hidden),
                      device="cpu").quantize()
+
+
+def test_refiner_saved_before_it_had_feed_forward_layers():
+    """A whole module, saved by a version whose blocks and shapes knew of none."""
+    import pickle
+
+    from gaussian_splats_b200.refine import RefinerShape, SplatRefiner
+
+    refiner = SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1), device="cpu")
+    for block in refiner.blocks:
+        del block.feed
+    del refiner.shape.__dict__["hidden"]
+    loaded = pickle.loads(pickle.dumps(refiner))
+    assert loaded.shape.hidden == 0 and all(block.feed is None for block in loaded.blocks)
+    x = torch.zeros(3, 64)
+    assert loaded.blocks[0]._fed(x, (x,)) is x
+    loaded.quantize()
