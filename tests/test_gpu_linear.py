@@ -496,3 +496,11 @@ def test_gradient_of_the_bias(rows, inputs, outputs, activation, dtype, bias):
         if rows == 1:
             codes = ((ref["slope"] + 1 / 6) * 49152).round() / 49152 - 1 / 6
             assert (((s["grad"].double() * codes).sum(0) - ref["dbias"]).abs() > limit).any()
+
+
+@pytest.mark.parametrize("rows", [300, 1000])
+def test_weight_gradients_of_several_turns(rows):
+    """More tiles of the weight's gradient than multiprocessors, or pairs of them, and a last
+    turn and last tiles that are not full."""
+    s = make(rows, 2500, 5130, BF, BF, None)
+    check(call(s, "gelu"), s, "gelu")
