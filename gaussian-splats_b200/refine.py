@@ -83,11 +83,12 @@ class _Product(nn.Linear):
         self.scales = (w.abs().amax(1) / 448.0).clamp(min=1e-12)
         self.codes = (w / self.scales[:, None]).to(torch.float8_e4m3fn)
 
-    def eight_bit(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    def eight_bit(self, codes: torch.Tensor, scale: torch.Tensor,
+                  bias: torch.Tensor | None = None) -> torch.Tensor:
         if self.rounded != self._changes():  # an optimizer's step, a loaded checkpoint
             self.quantize()
         return torch._scaled_mm(codes, self.codes.t(), scale[:, None], self.scales[None],
-                                out_dtype=torch.bfloat16)
+                                bias=bias, out_dtype=torch.bfloat16)
 
 
 @dataclass(frozen=True)
@@ -119,8 +120,9 @@ class _FeedForward(nn.Module):
         return self._down(linear(y, self.up.weight, self.up_bias, activation="gelu"), x)
 
     def eight_bit(self, codes, scale, x):
-        z = self.up.eight_bit(codes, scale).float() + self.up_bias.float()
-        return self._down(nn.functional.gelu(z).bfloat16(), x)
+        """The way up as an 8-bit product, whose result with its bias is rounded to bfloat16
+        before the activation."""
+        return self._down(nn.functional.gelu(self.up.eight_bit(codes, scale, self.up_bias)), x)
 
     def _down(self, hidden, x):
         return linear(hidden, self.down.weight, self.down.bias, x)
