@@ -83,12 +83,11 @@ class _Product(nn.Linear):
         self.scales = (w.abs().amax(1) / 448.0).clamp(min=1e-12)
         self.codes = (w / self.scales[:, None]).to(torch.float8_e4m3fn)
 
-    def eight_bit(self, codes: torch.Tensor, scale: torch.Tensor,
-                  bias: torch.Tensor | None = None) -> torch.Tensor:
+    def eight_bit(self, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
         if self.rounded != self._changes():  # an optimizer's step, a loaded checkpoint
             self.quantize()
         return torch._scaled_mm(codes, self.codes.t(), scale[:, None], self.scales[None],
-                                bias=bias, out_dtype=torch.bfloat16)
+                                out_dtype=torch.bfloat16)
 
 
 @dataclass(frozen=True)
@@ -108,23 +107,18 @@ class RefinerShape:
 
 
 class _FeedForward(nn.Module):
-    """``x + down(gelu(up(y)))``: both products with their epilogues."""
+    """``x + down(gelu(up(y)))``: both products with their epilogues. ``x`` is the output of
+    the recurrence's product, in bfloat16; the next norm adds the sum to the float32
+    residual stream."""
 
     def __init__(self, width: int, hidden: int, device=None):
         super().__init__()
-        self.up = _Product(width, hidden, device)
+        self.up = nn.Linear(width, hidden, bias=False, device=device, dtype=torch.bfloat16)
         self.up_bias = nn.Parameter(torch.zeros(hidden, device=device, dtype=torch.bfloat16))
         self.down = nn.Linear(hidden, width, device=device, dtype=torch.bfloat16)
 
     def forward(self, y, x):
-        return self._down(linear(y, self.up.weight, self.up_bias, activation="gelu"), x)
-
-    def eight_bit(self, codes, scale, x):
-        """The way up as an 8-bit product, whose result with its bias is rounded to bfloat16
-        before the activation."""
-        return self._down(nn.functional.gelu(self.up.eight_bit(codes, scale, self.up_bias)), x)
-
-    def _down(self, hidden, x):
+        hidden = linear(y, self.up.weight, self.up_bias, activation="gelu")
         return linear(hidden, self.down.weight, self.down.bias, x)
 
 
@@ -152,19 +146,20 @@ class _Block(nn.Module):
             self.__dict__.setdefault("feed", None)  # of a block saved before there were any
 
     def _normed(self, x, residual, weight, product):
-        """The product of the norm of ``x + residual``, the sum, and the norm itself
-        (codes and scale where the products are in 8 bits)."""
-        if product.codes is not None and not torch.is_grad_enabled():
+        """The product of the norm of ``x + residual``, the sum, and the norm itself in
+        bfloat16 (None where the product is in 8 bits: not where a feed-forward layer
+        reads the norm too)."""
+        fed = self.feed is not None and product is self.mix
+        if product.codes is not None and not fed and not torch.is_grad_enabled():
             codes, scale, residual = rms_norm_e4m3(x, weight, residual)
-            return product.eight_bit(codes, scale), residual, (codes, scale)
+            return product.eight_bit(codes, scale), residual, None
         y, residual = rms_norm(x, weight, residual)
-        return product(y), residual, (y,)
+        return product(y), residual, y
 
-    def _fed(self, x, normed):
-        """``x`` and the feed-forward layer's output of the norm that the recurrence had."""
-        if self.feed is None:
-            return x
-        return self.feed(*normed, x) if len(normed) == 1 else self.feed.eight_bit(*normed, x)
+    def _fed(self, x, y):
+        """``x`` and the feed-forward layer's output of ``y``, the norm that the recurrence
+        had."""
+        return x if self.feed is None else self.feed(y, x)
 
     def _heads(self, qkv):
         return (t.unflatten(-1, (-1, self.dim)) for t in qkv.split(self.split, -1))
@@ -175,9 +170,9 @@ class _Block(nn.Module):
         x = window_attention(*self._heads(qkv), packed, left=s.left, right=s.right, first=s.first,
                              valid=valid)
         x = self.attend_out(x.flatten(1))
-        mix, residual, normed = self._normed(x, residual, self.norm_mix, self.mix)
+        mix, residual, y = self._normed(x, residual, self.norm_mix, self.mix)
         x, _ = gated_scan(*mix.chunk(2, -1), packed)
-        return self._fed(self.mix_out(x), normed), residual
+        return self._fed(self.mix_out(x), y), residual
 
     def step(self, x, residual, positions, cache, state, valid, cache_valid):
         qkv, residual, _ = self._normed(x, residual, self.norm_attend, self.qkv)
@@ -187,9 +182,9 @@ class _Block(nn.Module):
         else:
             x = window_attention_step(*self._heads(qkv), *cache, positions, **slots)
         x = self.attend_out(x.flatten(1))
-        mix, residual, normed = self._normed(x, residual, self.norm_mix, self.mix)
+        mix, residual, y = self._normed(x, residual, self.norm_mix, self.mix)
         x = gated_scan_step(*mix.chunk(2, -1), state)
-        return self._fed(self.mix_out(x), normed), residual
+        return self._fed(self.mix_out(x), y), residual
 
 
 class SplatRefiner(nn.Module):
@@ -214,16 +209,13 @@ class SplatRefiner(nn.Module):
         """Switches the products behind a norm to 8 bits for calls without
         gradients. Their weights are rounded here, and again by the first such call
         after they have changed in place; training goes on in bfloat16, and what
-        ``state_dict`` saves is the bfloat16 weights. 8-bit products have outputs in
-        multiples of 16, so ``hidden`` has to be one."""
-        if self.shape.hidden % 16:
-            raise ValueError(f"8-bit products take a hidden layer of a multiple of 16 channels, "
-                             f"not of {self.shape.hidden}")
+        ``state_dict`` saves is the bfloat16 weights. A feed-forward layer stays in
+        bfloat16, and the recurrence's product beside it, which reads the same norm: an
+        8-bit way up, with its activation in a pass of its own, is slower."""
         for block in self.blocks:
             block.qkv.quantize()
-            block.mix.quantize()
-            if block.feed is not None:
-                block.feed.up.quantize()
+            if block.feed is None:
+                block.mix.quantize()
 
     def _features(self, splats: GaussianSplat) -> torch.Tensor:
         features = torch.cat([getattr(splats, name).flatten(1) for name in _NAMES], 1)

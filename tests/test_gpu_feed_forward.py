@@ -200,33 +200,22 @@ def test_streams_with_four_bit_caches(monkeypatch):
     assert held < 0.29 * whole
 
 
-def test_eight_bit_way_up():
-    """The 8-bit product with its bias is rounded once before the activation: a bias that
-    takes most of the product away leaves the rest its digits."""
-    from gaussian_splats_b200.norm import rms_norm_e4m3
-    from gaussian_splats_b200.refine import _FeedForward
+def test_quantized_refiner_keeps_its_feed_forward(monkeypatch):
+    """8-bit products are those of the attention then: both ways of the feed-forward layer
+    run through the linear layer, whatever its size, as before."""
+    from gaussian_splats_b200 import refine
 
-    torch.manual_seed(3)
-    rows, width = 300, 64
-    feed = _FeedForward(width, width, "cuda")
-    with torch.no_grad():
-        feed.up.weight.abs_().mul_(8.0)
-        feed.down.weight.copy_(torch.eye(width))
-        feed.down.bias.zero_()
-    feed.up.quantize()
-    x = (1.0 + 0.05 * torch.randn(rows, width, device="cuda")).bfloat16()
-    codes, scale, _ = rms_norm_e4m3(x, torch.ones(width, device="cuda", dtype=torch.bfloat16),
-                                    torch.zeros(rows, width, device="cuda"))
-    a = codes.float().double() * scale.double()[:, None]
-    w = feed.up.codes.float().double() * feed.up.scales.double()[:, None]
-    with torch.no_grad():
-        feed.up_bias.copy_(-(a @ w.t()).mean(0))
-        got = feed.eight_bit(codes, scale, torch.zeros(rows, width, device="cuda",
-                                                       dtype=torch.bfloat16)).double()
-    z = a @ w.t() + feed.up_bias.detach().double()
-    want, _ = R.activate("gelu", z)
-    # z's rounding and float sums of 64 products and the scales, gelu's slope, the result's
-    size = a @ w.t() + feed.up_bias.detach().double().abs()
-    limit = 1.13 * (R.U[torch.bfloat16] * z.abs() + 70 * 2.0 ** -23 * size) + \
-        1.01 * R.U[torch.bfloat16] * want.abs() + 2.0 ** -30
-    assert (z.abs().mean() < 0.1 * size.mean()) and ((got - want).abs() <= 1.01 * limit).all()
+    for hidden in (512, 40):
+        refiner, splats, calls = made(hidden=hidden), scene(100, 6), []
+        refiner.quantize()
+
+        def recorded(x, *args, **more):
+            calls.append(more.get("activation"))
+            return plain_linear(x, *args, **more)
+
+        with torch.no_grad(), monkeypatch.context() as m:
+            m.setattr(refine, "linear", recorded)
+            out = refiner([splats])[0]
+        assert calls == ["gelu", None] * len(refiner.blocks)
+        assert all(t.isfinite().all() for t in out.values())
+        assert all(block.qkv.codes is not None for block in refiner.blocks)

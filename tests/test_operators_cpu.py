@@ -211,18 +211,6 @@ def test_operands_are_copied_once(monkeypatch):
         assert calls.pop() == "gs_align_rows" and calls == []
 
 
-def test_refiner_with_a_hidden_layer_that_8_bit_products_do_not_take():
-    from gaussian_splats_b200.refine import RefinerShape, SplatRefiner
-
-    refiner = SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1, hidden=40), device="cpu")
-    with pytest.raises(ValueError, match="multiple of 16"):
-        refiner.quantize()
-    assert all(block.qkv.codes is None for block in refiner.blocks)  # nothing is switched
-    for hidden in (0, 48):
-        SplatRefiner(shape=RefinerShape(width=64, heads=2, kv_heads=1, hidden=hidden),
-                     device="cpu").quantize()
-
-
 def test_refiner_saved_before_it_had_feed_forward_layers():
     """A whole module, saved by a version whose blocks and shapes knew of none."""
     import pickle
