@@ -310,8 +310,9 @@ def window_attention_step_4bit(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     x) / 15, (max x + min x) / 2)`` rounded to the tokens' type and codes ``(x -
     range[1]) / range[0] + 7.5`` rounded to the nearest, ties to even. The output is
     the attention over what the cache then holds, the new token as it is held
-    included; scores and sums in float32. A row with a channel that is not finite is
-    held as one that is not finite.
+    included; scores and sums in float32, the weights times the values' steps rounded to
+    11 bits (relative to the steps' largest where they are 2^21 apart). A row with a
+    channel that is not finite is held as one that is not finite.
 
     q, k and v [batch, heads, dim], bfloat16 or float16, dim a multiple of 8 up to
     128; ``positions``, ``first``, ``scale``, ``valid`` and ``cache_valid`` as

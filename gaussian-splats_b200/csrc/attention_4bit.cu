@@ -9,7 +9,9 @@
 // its weight p_t step_t and in one float sum a head, which no rounding meets. q and the
 // weights are scaled by powers of two into float16's range, whatever the tokens' type:
 // of a head's q nothing is lost within 2^-25 of its largest channel, and the weights
-// are rounded once, to 11 bits.
+// are rounded once, to 11 bits: the products take no wider operands, codes in 16 bits are
+// exact, and a second product of what the rounding takes would be the dearest part made twice
+// (3 long memories in float16: error against 64 bits 3.1e-4, with float weights 2.1e-4).
 //
 // The cache is read once; taking a word of eight codes apart costs 5 or 6 instructions
 // though, which with the rest weigh about as much as the reading. So the work is cut evenly:
@@ -23,7 +25,11 @@
 // of 65,536 slots, 24 heads (8) of 96 channels, 164 MB: 44 us. The first's reading alone
 // takes 40 to 48 us, all but the reading 44, starting and ending about 7 of either: the
 // two do not overlap entirely. Joining takes 6 to 8 us. Between 12 and 20 warps a
-// multiprocessor, deeper rings, turns loaded by whole blocks or clusters: none was faster. One stream of 1028 slots: 8 and 5 us, launches and latency.
+// multiprocessor, deeper rings, turns loaded by whole blocks or clusters: none was faster;
+// the kernels for more than 64 channels spill 50 to 170 bytes a thread at 16 warps, and were no
+// faster with fewer warps that spill nothing. Rows that are not whole 16-byte words come by
+// 4-byte copies: of 120 channels 146 us, of 72 103, where 128 and 96 take 59 and 54. One stream
+// of 1028 slots: 7 and 5 us, launches and latency.
 //
 //   scores [slots x heads] = K q^T: a lane's words of two key rows are its parts of
 //     the products, with q's channels permuted alike;

@@ -23,8 +23,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVectors = 8;                             // 16-byte words a thread and chunk
 constexpr int64_t kChunkWords = kThreads * kVectors;    // 32 KB
-constexpr int kSmallTable = 80, kLargeTable = 1024;     // tensors of one launch: 2 KB, 25 KB
-constexpr int kBlocks = 6 * kSmCount;                   // all resident at once
+constexpr int kSmallTable = 80, kLargeTable = 1024;     // tensors of one launch: 1.7 KB, 21.5 KB
+constexpr int kBlocks = 6 * kSmCount;                   // 3 of 6 resident at once (scaling: 2)
 constexpr double kEps = 1e-6;
 
 template <int kEntries>

@@ -11,7 +11,7 @@
 // What bounds a product, and what it takes, forward unless said otherwise:
 //   long contractions: the tensor cores. 65,536 x 1024 -> 4096: 360 us, 1.53 PFLOP/s, 0.91
 //     of the rate of a long bare product in a burst; with gelu 400, with its slopes 456. In
-//     a training pass the power limit lowers the clock: 510 to 600 us, and 380 to 460 each
+//     a training pass the power limit lowers the clock: 490 to 640 us, and 365 to 480 each
 //     for dx and dW, with the tensor cores active for 84 to 88 % of the time.
 //   short ones: the results, 268 MB of 131,072 x 64 or 128 -> 1024 in 57 us (the epilogue
 //     without its stores: 49). From 256 channels 80 us, as dx of 131,101 x 1024 from 256: the
@@ -20,6 +20,8 @@
 //   activations: gelu makes 137 us of these 80, with its slopes 156: two instructions an
 //     element of the kind that a multiprocessor makes 16 a clock of, and a long chain. relu
 //     80 and 109.
+//   the general epilogue (Form::kAny): its decisions. gelu onto a float residual 239 us,
+//     slopes in float 208; results of 1021 columns, which no TMA store takes, 341.
 //   few rows: the loads' latency, and a launch. 96 x 2048 -> 8192: 14 us for 34 MB of
 //     weights that are not in L2; 1 x 256 -> 1024: 5 us.
 #include <algorithm>
@@ -59,7 +61,7 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 //
 // gelu: with t = |z|, the normal distribution's upper tail is e^(-t^2/2) R(t), R smooth
 // (Mills' ratio over sqrt(2 pi)); R = u P(u) with u = 1 / (1 + 0.3 t) and P the polynomial
-// of degree 7 with the least relative error for t up to 14, 1.5e-7. The density that
+// of degree 7 with the least relative error for t up to 14, 1.6e-7. The density that
 // the slope needs is the same exponential.
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 template <int kCount>
@@ -155,7 +157,9 @@ struct EpilogueMaps {
 };
 
 // What an epilogue has to do, where the kernel is built for it: code that decides as it
-// goes takes twice the instructions. kAny decides, and writes what TMA does not take.
+// goes takes twice the instructions. kAny decides: it writes what TMA does not take, and does
+// what none of the others is built for (a 16-bit residual, an activation before a float
+// result, slopes in float, a float result without a residual in the forward).
 enum class Form {
   kAny,
   kNarrow,    // 16-bit result
@@ -880,7 +884,10 @@ __device__ __forceinline__ void load_row(const G* p, int valid, float (&x)[8]) {
 enum class Slopes { kNone, kCodes, kFloats };
 
 // dz = grad_y act'(z) rounded to the operands' type, and each strip's sums of its columns
-// (of what was not rounded). A thread has eight columns of every so many rows, and loads
+// (of what was not rounded). Rounded because it is an operand of two products: to keep what
+// the rounding takes, each would be made twice, of dz's upper and lower bits, for gradients
+// that are rounded to the same type themselves (a training pass's errors against 64 bits 2.4e-3 and 3.0e-4 in
+// bfloat16 and float16, with dz in float 1.7e-3 and 2.1e-4). A thread has eight columns of every so many rows, and loads
 // several rows before it works on the first: memory is the bound (65,536 x 4096 in
 // float16: 280 us for 1.6 GB, 5.8 TB/s; 131,101 x 256 of a float gradient: 30 us for 200
 // MB, 6.7 TB/s). kWhole: rows are whole 16-byte words.

@@ -446,7 +446,7 @@ typedef struct gs_gradient {
  * bytes of elements, so that no norm over- or underflows on the way). `scale` != 0
  * multiplies every element by the factor (the gradients must not overlap; a factor of
  * 1 writes nothing); a NaN in a gradient makes norm and factor NaN, an infinity the
- * factor 0. max_norm >= 0, infinity for the norm alone. The workspace is 8-byte
+ * factor 0 (NaN where max_norm is infinite too). max_norm >= 0, infinity for the norm alone. The workspace is 8-byte
  * aligned. Results repeat bit for bit. */
 uint64_t gs_clip_grad_norm_workspace_size(int64_t tensors);
 int32_t gs_clip_grad_norm(int64_t tensors, const gs_gradient *list, double max_norm,
