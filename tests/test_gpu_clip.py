@@ -253,3 +253,29 @@ def test_parameters_with_one_gradient():
     for t, k in ((g, kept), (other, kept_other)):
         assert ((t.double() - f * k).abs() <= 1.01 * (NORM + 2.0 ** -23 + U[t.dtype]) *
                 (f * k).abs()).all()
+
+
+def test_clipped_step_with_noise_and_skipped_groups():
+    """Beside the position noise and with gradients that are not there, the step is that of
+    the clipped ones too."""
+    from gaussian_splats_b200.optim import GROUP_NAMES, FusedAdam, clip_grad_norm
+
+    shapes = [(333, 3), (333, 4), (333, 3), (333, 1), (333, 4, 3)]
+
+    def optimizer():
+        ps = parameters([rand(10 + i, *s) for i, s in enumerate(shapes)])
+        return ps, FusedAdam([{"params": [p], "name": name, "lr": 1e-2}
+                              for p, name in zip(ps, GROUP_NAMES)], eps=1e-15)
+
+    (ps, fused), (qs, plain) = optimizer(), optimizer()
+    for turn, missing in enumerate(((), (1, 4), (0,))):
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            p.grad = None if i in missing else rand(20 + 5 * turn + i, *p.shape)
+            q.grad = None if i in missing else p.grad.clone()
+        want = clip_grad_norm(qs, 0.5)
+        torch.manual_seed(turn)
+        plain.step(noise=(5e5, 5e-4))
+        torch.manual_seed(turn)
+        fused.step(noise=(5e5, 5e-4), max_norm=0.5)
+        assert torch.equal(fused.grad_norm, want)
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))

@@ -386,7 +386,8 @@ def test_refusals():
 @pytest.mark.parametrize("dtype", [BF, HF], ids=str)
 @pytest.mark.parametrize("rows,inputs,outputs", [
     (1, 136, 32), (96, 136, 1024), (300, 59, 128), (640, 64, 4096), (5000, 136, 264),
-    (20003, 72, 520), (9001, 520, 300), (4000, 59, 260), (70, 136, 37)])
+    (20003, 72, 520), (9001, 520, 300), (4000, 59, 260), (70, 136, 37), (1280, 136, 640),
+    (1280, 59, 640), (9000, 59, 256), (18944, 59, 256)])
 def test_float_results_without_a_residual(rows, inputs, outputs, dtype):
     """Which only a C caller asks for: rows by TMA and gathered, by pairs of blocks, tiles
     of every width, results that TMA takes and others."""
