@@ -29,20 +29,15 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_FLOAT32, 
 _GATHERED = 128
 
 
-def _lies_as_operand(t: torch.Tensor) -> bool:
-    row, channel = t.stride()
-    return channel == 1 and row % 8 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0
-
-
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, channels] as the kernels read a product's operand: rows of contiguous
     channels that start on 16-byte borders. ``t`` itself if it lies so, else a copy."""
-    rows, channels = t.shape
-    if _lies_as_operand(t):
+    (row, channel), (rows, channels) = t.stride(), t.shape
+    if channel == 1 and row % 8 == 0 and row >= channels and t.data_ptr() % 16 == 0:
         return t
-    if t.stride(1) != 1:
+    if channel != 1:
         t = t.contiguous()
-        if _lies_as_operand(t):
+        if rows and channels % 8 == 0:  # a new one, then, and whole words
             return t
     copy = t.new_empty((rows, -(-channels // 8) * 8))
     call("gs_align_rows", t.device, rows, channels, t.data_ptr(), t.stride(0), copy.data_ptr())
@@ -57,10 +52,6 @@ def _arguments(x, weight, bias, **values):
         bias_dtype=dtype if bias is None else _CODES[bias.dtype], x=x.data_ptr(),
         weight=weight.data_ptr(), bias=address(bias), x_stride=x.stride(0),
         weight_stride=weight.stride(0), **values)
-
-
-def _in_float(slope: torch.Tensor | None) -> int:
-    return int(slope is not None and slope.dtype == torch.float32)
 
 
 def _forward(x, weight, bias, residual, activation, train):
@@ -82,7 +73,9 @@ def _forward(x, weight, bias, residual, activation, train):
                             dtype=torch.float32 if exact else torch.int16)
     args = _arguments(rows, w, b, activation=activation, residual_dtype=_CODES[y.dtype],
                       residual=address(res), residual_stride=stride, y=y.data_ptr(),
-                      slope=address(slope), slope_float=_in_float(slope))
+                      slope=address(slope))
+    if slope is not None:
+        args.slope_float = slope.dtype == torch.float32
     call("gs_linear", x.device, ctypes.byref(args))
     return y, (rows, w, b, slope)
 
@@ -110,8 +103,10 @@ class _Linear(torch.autograd.Function):
             rows = _whole(grad_y.reshape(x.shape[0], weight.shape[0]))
             args = _arguments(x, weight, bias, activation=ctx.activation,
                               residual_dtype=_CODES[rows.dtype], slope=address(slope),
-                              slope_float=_in_float(slope), grad_y=address(rows), grad_x=address(grads[0]),
+                              grad_y=address(rows), grad_x=address(grads[0]),
                               grad_weight=address(grads[1]), grad_bias=address(grads[2]))
+            if slope is not None:
+                args.slope_float = slope.dtype == torch.float32
             size = native.lib().gs_linear_workspace_size(ctypes.byref(args))
             workspace = x.new_empty((size,), dtype=torch.uint8)
             args.workspace, args.workspace_size = address(workspace), size

@@ -505,3 +505,17 @@ def test_weight_gradients_of_several_turns(rows):
     turn and last tiles that are not full."""
     s = make(rows, 2500, 5130, BF, BF, None)
     check(call(s, "gelu"), s, "gelu")
+
+
+def test_no_rows_of_any_strides():
+    from gaussian_splats_b200.linear import linear
+
+    whole = torch.zeros(4, 17, 3, device="cuda", dtype=BF)
+    weight = torch.ones(8, 16, device="cuda", dtype=BF, requires_grad=True)
+    for x in (whole[:0, :16, 0], whole[:0, 1:, 1], whole[0, :16, :0].t(), whole[:0, 0, :1].expand(0, 16)):
+        x = x.detach().requires_grad_()
+        y = linear(x, weight, activation="gelu")
+        dx, dw = torch.autograd.grad(y.sum(), (x, weight))
+        assert y.shape == (0, 8) and dx.shape == x.shape and (dw == 0).all()
+        with torch.no_grad():
+            assert linear(x, weight).shape == (0, 8)
