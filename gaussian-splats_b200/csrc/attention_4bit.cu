@@ -94,7 +94,7 @@ struct Parts {
 };
 constexpr uint32_t kLargeUnit = (127 + 20) << 23;  // 2^20's bits
 constexpr float kLargeScale = 0x1p64f;
-constexpr float kFar = 0x1p64f;  // of queries' channels
+constexpr float kFar = 0x1p100f, kFarScale = 0x1p64f;  // of queries' channels
 
 // The warps that have an item's first and last turn.
 struct Reach {
@@ -428,8 +428,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
   // Of the lane's columns, heads 2j and 2j + 1: what takes their dots to those with c - 7.5,
   // and the sums of q; both in base 2.
   float2 dot_scale[kSets], dot_offset[kSets], q_sum[kSets];
-  // Where a head's q has channels from 2^64 on, these are 2^-64 as large and the keys' ranges
-  // 2^64: then no part of a score leaves float's range that the score does not.
+  // Where a head's q has channels from 2^100 on, these are 2^-64 as large and the keys' ranges
+  // 2^64: then no part of a score leaves float's range that the score does not. (The group's
+  // other heads share the ranges: they lose keys of 2^64 and more, which leave that head
+  // no finite scores.)
   constexpr bool kWideRange = std::is_same_v<T, __nv_bfloat16>;  // float16 ends at 2^16
   bool far[kSets], any_far = false;
 #pragma unroll
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
       largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
     far[r] = kWideRange && __any_sync(0xffffffffu, largest >= kFar);
     any_far = any_far || far[r];
-    const float shrink = far[r] ? 1.0f / kFar : 1.0f;
+    const float shrink = far[r] ? 1.0f / kFarScale : 1.0f;
 #pragma unroll
     for (int w = 0; w < kKeyWords; ++w)
 #pragma unroll
@@ -479,9 +481,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
 #pragma unroll
   for (int r = 0; r < kSets; ++r)
     if (any_far && !far[r]) {
-      dot_scale[r] = tc::mul2(dot_scale[r], both(1.0f / kFar));
-      dot_offset[r] = tc::mul2(dot_offset[r], both(1.0f / kFar));
-      q_sum[r] = tc::mul2(q_sum[r], both(1.0f / kFar));
+      dot_scale[r] = tc::mul2(dot_scale[r], both(1.0f / kFarScale));
+      dot_offset[r] = tc::mul2(dot_offset[r], both(1.0f / kFarScale));
+      q_sum[r] = tc::mul2(q_sum[r], both(1.0f / kFarScale));
     }
   float2 out[kSets][kValueWords][4][2] = {};  // of both heads: channels e, and e + 4
   float top[kSets][2];
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(kDim, kSets))
     const uint32_t visible = __ballot_sync(0xffffffffu, seen);
     {
       float2 key = unpack2<T>(seen ? ranges.x : 0);
-      if (any_far) key = tc::mul2(key, both(kFar));
+      if (any_far) key = tc::mul2(key, both(kFarScale));
       const float2 value = unpack2<T>(seen ? ranges.y : 0);
       const uint32_t largest = __reduce_max_sync(
           0xffffffffu, __float_as_uint(fmaxf(fabsf(value.x), 0x1p-60f * fabsf(value.y))));

@@ -410,3 +410,32 @@ def test_queries_of_the_whole_range(power):
         out = window_attention_step_4bit(q, k, v, cache, positions)
         assert out.isfinite().all()
         compare(out, ref.step(q, k, v, positions, dim ** -0.5), BF, dim)
+
+
+def test_large_queries_leave_their_groups_other_heads_alone():
+    """A head whose scores leave float32's range, or whose query is not finite, has no
+    finite output; the heads beside it have theirs, of large keys too."""
+    from gaussian_splats_b200.attention import FourBitCache, window_attention_step_4bit
+
+    g = torch.Generator(device="cuda").manual_seed(13)
+    slots, heads, dim = 70, 12, 64
+    for size in (2.0 ** 70, 2.0 ** 99, float("inf"), float("nan")):
+        ref = R.Streams(1, slots, 0, 1, dim, BF, "cuda")
+        fill(ref, g, BF, 1, 1, slots, dim)
+        q = rand(g, 1, heads, dim, dtype=BF)
+        many = 2.0 ** 66 if size < 2.0 ** 100 else 1.0
+        keys = (rand(g, 1, 1, slots, dim, dtype=BF).double() * many).to(BF)
+        code, step, middle = R.held(keys)
+        ref.codes[0][:], ref.ranges[0][:] = R.packed(code), torch.stack((step, middle), -1)
+        ref.k[:] = (code.double() - 7.5) * step.double()[..., None] + middle.double()[..., None]
+        cache = FourBitCache(ref.codes[0].clone(), ref.ranges[0].clone(), ref.codes[1].clone(),
+                             ref.ranges[1].clone())
+        q = (q.double() / many).to(BF)
+        q[:, 3] = size
+        k, v = keys[:, :, 0].contiguous(), rand(g, 1, 1, dim, dtype=BF)
+        positions = torch.full((1,), 3 * slots + 2, device="cuda")
+        out = window_attention_step_4bit(q, k, v, cache, positions)
+        others = torch.arange(heads, device="cuda") != 3
+        want = ref.step(q[:, others], k, v, positions, dim ** -0.5)
+        compare(out[:, others], want, BF, dim)
+        assert not out[:, 3].isfinite().all() or size < 2.0 ** 100
